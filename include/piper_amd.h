@@ -424,6 +424,55 @@ PK_API int pk_grouped_swiglu_wgrad_scaled_t(const void* d_out, const void* hsT, 
 #define PK_SCHED_SETS 1024
 PK_API int pk_sched_slot_index(int device, uint64_t stream_handle, uint64_t capture_sequence, uint64_t thread_key);
 
+/* ------------------------------------------- experts in 8-bit floating point
+ * No counterpart in the reference, whose experts are bf16 products (qwen3_bmm_experts_patch.py:39-41).
+ * Values are OCP e4m3 codes with a power of two for each block of PK_FP8_BLOCK (rows: 128 neighbouring
+ * values of a row; weights: 128 x 128), held as its biased exponent: value = code * 2^(byte - 127).  The
+ * byte is the smallest, from 1 on, with which the block's largest magnitude is at most 448 in codes; codes
+ * round to nearest even; a block with an infinity or a NaN is NaN throughout.  With w' = ceil(w / 128) * 128:
+ *   rows     q [R][K'] (zeros behind K), scales [R][K'/128]
+ *   weights  q [E][N][K'], scales [E][N'/128][K'/128]; transposed codes q_t [E][K][N'] share the scales
+ * Code buffers must be 16-byte aligned.  The products take bf16 tensors of any width up to
+ * H = PK_FP8_MAX_HIDDEN, I = PK_FP8_MAX_INTER; an operand's codes must span less than 4 GiB
+ * (PK_ERR_SHAPE).  Expert e owns rows [starts[e], starts[e+1]); other rows are neither read nor written. */
+#define PK_FP8_BLOCK 128
+#define PK_FP8_MAX_HIDDEN 8192
+#define PK_FP8_MAX_INTER 4096
+
+/* Rows of x [., K] (dtype) in blocks: row r of the result is x[r], or with row_map (i32 [rows])
+ * x[row_map[r] / row_map_div]. */
+PK_API int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map, int64_t row_map_div, uint8_t* q,
+                         uint8_t* scales, int64_t rows, int64_t K, pk_stream_t stream);
+/* w [E, N, K] (dtype) in blocks; q_t may be NULL. */
+PK_API int pk_fp8_quantize_weights(const void* w, int dtype, uint8_t* q, uint8_t* q_t, uint8_t* scales, int64_t E,
+                            int64_t N, int64_t K, pk_stream_t stream);
+
+/* g = x . w1[e]^T, u = x . w3[e]^T (both bf16 [A, I], or both NULL where no backward follows), and
+ * h = silu(g) * u of what g and u hold, in blocks.  Operand row r is x[r], or x[row_map[r] / row_map_div];
+ * the rows that the map can name are the first ceil(A / row_map_div). */
+PK_API int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const int32_t* row_map, int64_t row_map_div,
+                   const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3, const int32_t* starts,
+                   void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E,
+                   pk_stream_t stream);
+/* y[A, H] (bf16) = h . w2[e]^T */
+PK_API int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2,
+                const int32_t* starts, void* y, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
+/* d_h = d_y . w2[e] (w2_t: the transposed codes) in fp32, and from it d_g = d_h * u * silu'(g) and
+ * d_u = d_h * silu(g), both bf16 [A, I] (for pk_grouped_swiglu_wgrad) and in blocks (for pk_fp8_dgrad_dx), and
+ * h = silu(g) * u (bf16).  With scores (f32, of every routed slot) and row_map, as
+ * pk_grouped_swiglu_dgrad_dh_scaled: d_y is d_out, operand row r is d_out[row_map[r] / row_map_div], d_h is
+ * multiplied by scores[row_map[r]], so is h, and ds_part [ceil(I / 128)][A] receives the parts of
+ * <d_out . w2, silu(g) * u> that pk_region_router_bwd adds up. */
+PK_API int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div,
+                    const float* scores, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
+                    const int32_t* starts, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales,
+                    uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H, int64_t I, int64_t E,
+                    pk_stream_t stream);
+/* d_x[A, H] (bf16) = d_g . w1[e] + d_u . w3[e] (w1_t, w3_t: the transposed codes) */
+PK_API int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales,
+                    const uint8_t* w1_t, const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3,
+                    const int32_t* starts, void* d_x, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
+
 /* ------------------------------------------------------------- ZeRO bucket path */
 
 /* HOST function.  offsets[i] (in elements) of n tensors laid out back to back, each start
@@ -486,6 +535,35 @@ PK_API int pk_adamw_fused_packed(float* master, float* exp_avg, float* exp_avg_s
                           int grad_dtype, void* shadow, int shadow_dtype, float lr, float beta1, float beta2,
                           float eps, float weight_decay, int64_t step, float grad_scale, int zero_grad,
                           pk_stream_t stream);
+
+/* pk_adamw_fused with both moments in 8-bit floating point, 18 bytes an element instead of 30:
+ *   exp_avg     [n] OCP e4m3 codes, exp_avg_sq [n] OCP e5m2 codes (no sign in use), and for each block of
+ *   PK_ADAMW8_BLOCK elements, counted from the bucket's first, a power of two as its biased exponent in
+ *   *_scale [ceil(n / 64)]: moment = code * 2^(byte - 127).  Zeros throughout are moments of zero.
+ * The update is pk_adamw_fused's, in fp32 from the decoded moments; master and shadow never see the rounding of
+ * the new ones.  These are stored with the smallest byte, from 1 on, with which the block's largest finite
+ * magnitude is a code (448, 57344), and rounded up or down at random with 16 bits an element and moment,
+ * so that the mean of what is stored is the moment: rounded to nearest the averages would stand still, since a
+ * step moves exp_avg_sq by (1 - beta2) of itself and half a step of the format is a sixteenth to an eighth.  A
+ * positive exp_avg_sq does not become zero (the update would divide by eps alone).  A moment that is not finite
+ * is stored as a NaN and touches no other element's.
+ * The bits: h = index * 0x6A09E667 + seed, h ^= h >> 16, h *= 0xBB67AE85, h ^= h >> 15, h *= 0x9E3779B1,
+ * h ^= h >> 16, all mod 2^32; the upper half for exp_avg, the lower one for exp_avg_sq.  A caller gives every
+ * step a seed of its own.  1 - beta1 and the like are formed in double precision. */
+#define PK_ADAMW8_BLOCK 64
+PK_API int pk_adamw8_fused(float* master, uint8_t* exp_avg, uint8_t* exp_avg_scale, uint8_t* exp_avg_sq,
+                    uint8_t* exp_avg_sq_scale, float* grad, void* shadow, int shadow_dtype, int64_t n, double lr,
+                    double beta1, double beta2, double eps, double weight_decay, int64_t step, uint32_t seed,
+                    float grad_scale, int zero_grad, pk_stream_t stream);
+/* The same for the tensors of a bucket, their own gradients read in place as in pk_adamw_fused_packed (16 bytes
+ * an element with bf16 gradients and no flat_grad): what pk_bucket_pack (accumulate) followed by pk_adamw8_fused
+ * leaves in a bucket whose padding is zero.  Every offset must be a multiple of PK_ADAMW8_BLOCK (PK_ERR_ALIGN; those of
+ * pk_bucket_plan with 256-byte alignment are), so that no block belongs to two tensors, and tensors must not overlap. */
+PK_API int pk_adamw8_fused_packed(float* master, uint8_t* exp_avg, uint8_t* exp_avg_scale, uint8_t* exp_avg_sq,
+                           uint8_t* exp_avg_sq_scale, float* flat_grad, const void* const* grads,
+                           const int64_t* offsets, const int64_t* numels, int64_t n, int grad_dtype, void* shadow,
+                           int shadow_dtype, double lr, double beta1, double beta2, double eps, double weight_decay,
+                           int64_t step, uint32_t seed, float grad_scale, int zero_grad, pk_stream_t stream);
 
 /* ------------------------------------------------------------- kernel timing
  * Measurement aid with no counterpart in the reference: when enabled, every kernel launch of

@@ -104,6 +104,18 @@ SIGNATURES = {
                                 _c_f32, _c_i64, _c_f32, _c_int, _p]),
     "pk_adamw_fused_packed": (_c_int, [_p, _p, _p, _p, _p, _p, _p, _c_i64, _c_int, _p, _c_int, _c_f32, _c_f32, _c_f32,
                                        _c_f32, _c_f32, _c_i64, _c_f32, _c_int, _p]),
+    # rows: x dtype row_map div q scales rows K stream; weights: w dtype q q_t scales E N K stream
+    "pk_fp8_quantize_rows": (_c_int, [_p, _c_int, _p, _c_i64, _p, _p, _c_i64, _c_i64, _p]),
+    "pk_fp8_quantize_weights": (_c_int, [_p, _c_int, _p, _p, _p, _c_i64, _c_i64, _c_i64, _p]),
+    # ... A H I E stream
+    "pk_fp8_gate_up": (_c_int, [_p, _p, _p, _c_i64, *[_p] * 9, *[_c_i64] * 4, _p]),
+    "pk_fp8_down": (_c_int, [*[_p] * 6, *[_c_i64] * 4, _p]),
+    "pk_fp8_dgrad_dh": (_c_int, [_p, _p, _p, _c_i64, *[_p] * 14, *[_c_i64] * 4, _p]),
+    "pk_fp8_dgrad_dx": (_c_int, [*[_p] * 10, *[_c_i64] * 4, _p]),
+    # master m m_scale v v_scale grad shadow shadow_dtype n lr b1 b2 eps wd step seed grad_scale zero_grad stream
+    "pk_adamw8_fused": (_c_int, [*[_p] * 7, _c_int, _c_i64, *[C.c_double] * 5, _c_i64, C.c_uint32, _c_f32, _c_int, _p]),
+    # master m m_scale v v_scale flat_grad grads offsets numels n grad_dtype shadow shadow_dtype lr ... stream
+    "pk_adamw8_fused_packed": (_c_int, [*[_p] * 9, _c_i64, _c_int, _p, _c_int, *[C.c_double] * 5, _c_i64, C.c_uint32, _c_f32, _c_int, _p]),
     "pk_timing_enable": (_c_int, [_c_int]),
     "pk_timing_collect": (_c_i64, [_p, _p, _c_i64]),
     "pk_timing_select": (_c_int, [_c_int]),

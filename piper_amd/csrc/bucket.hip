@@ -1,7 +1,7 @@
 // ZeRO bucket path: multi-tensor pack/unpack, zero fill, fused AdamW over an fp32 bucket.
 // All kernels are pure HBM streams: 16 bytes per lane per access, no LDS (the layout does
 // not change, so staging through LDS would only add latency).
-#include "pk_common.h"
+#include "fp8_blocks.h"
 
 namespace {
 
@@ -363,6 +363,232 @@ __global__ __launch_bounds__(kStreamThreads) void adamw_packed_kernel(
   }
 }
 
+// AdamW with both moments in 8-bit floating point (format and rounding: piper_amd.h).  Four elements to a lane as above, so a block
+// of 64 is 16 lanes, whose largest magnitude takes four vector instructions and no LDS.  Scales are powers of two, so decoding and
+// scaling are exact, and everything in between is the fp32 update with every operation rounded by itself
+// (no contraction): the same codes come out wherever it is computed.
+struct Adam8Args {
+  float decay, one_m_b1, beta2, one_m_b2, step_size, inv_bc2_sqrt, eps, grad_scale;
+  uint32_t seed;
+};
+struct Adam8State {
+  float* master;
+  uint8_t *m, *m_scale, *v, *v_scale;
+};
+
+__device__ __forceinline__ uint32_t adam8_random(int64_t index, uint32_t seed) {
+  uint32_t h = (uint32_t)index * 0x6A09E667u + seed;
+  h ^= h >> 16;
+  h *= 0xBB67AE85u;
+  h ^= h >> 15;
+  h *= 0x9E3779B1u;
+  return h ^ (h >> 16);
+}
+// The code of t = magnitude / scale, at most the format's largest value: MANT mantissa bits, exponents biased by BIAS.  Adding
+// the random bits below the last one kept and cutting off rounds up with the probability of the part cut off.
+template <int MANT, int BIAS>
+__device__ __forceinline__ uint32_t adam8_round(float t, uint32_t random16) {
+#pragma clang fp contract(off)
+  constexpr int DROP = 23 - MANT;
+  const uint32_t normal = ((__float_as_uint(t) + (random16 << (DROP - 16))) >> DROP) - ((127 - BIAS) << MANT);
+  const float scaled = t * (float)(1 << (BIAS - 1 + MANT)), threshold = (float)random16 * 0x1p-16f;
+  const uint32_t small = (uint32_t)(scaled + threshold);     // zero, subnormals, and the first normal value
+  return t < 1.f / (float)(1 << (BIAS - 1)) ? small : normal;
+}
+
+// Elements o .. o + 3 of the bucket, the first `cnt` of them there (any number, also none: such lanes only take part in the
+// blocks' maxima).  o is a multiple of 4; vec: the whole four are there and 16-byte accesses are fine.
+template <typename TSH, bool SHADOW>
+__device__ __forceinline__ void adam8_four(const Adam8State& st, TSH* shadow, int64_t o, int cnt, bool vec, const float (&g)[4],
+                                           const Adam8Args& a) {
+#pragma clang fp contract(off)
+  const int64_t block = o / PK_ADAMW8_BLOCK;
+  float p[4] = {}, m[4] = {}, v[4] = {};
+  uint32_t cm = 0u, cv = 0u;
+  if (vec) {
+    const floatx4_t q = __builtin_nontemporal_load(reinterpret_cast<const floatx4_t*>(st.master + o));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = q[j];
+    cm = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(st.m + o));
+    cv = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(st.v + o));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < cnt) {
+        p[j] = st.master[o + j];
+        cm |= (uint32_t)st.m[o + j] << (8 * j);
+        cv |= (uint32_t)st.v[o + j] << (8 * j);
+      }
+  }
+  float sm = 0.f, sv = 0.f;
+  if (cnt > 0) {
+    sm = pk_fp8::scale_of(st.m_scale[block]);
+    sv = pk_fp8::scale_of(st.v_scale[block]);
+  }
+  {
+    const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)cm, false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)cm, true);
+    const auto v01 = __builtin_amdgcn_cvt_pk_f32_bf8((int)cv, false), v23 = __builtin_amdgcn_cvt_pk_f32_bf8((int)cv, true);
+    m[0] = m01[0] * sm; m[1] = m01[1] * sm; m[2] = m23[0] * sm; m[3] = m23[1] * sm;
+    v[0] = v01[0] * sv; v[1] = v01[1] * sv; v[2] = v23[0] * sv; v[3] = v23[1] * sv;
+  }
+  uint32_t am = 0u, av = 0u;                 // the lane's largest finite magnitudes
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float gj = g[j] * a.grad_scale;
+    p[j] = p[j] * a.decay;
+    m[j] = m[j] + (gj - m[j]) * a.one_m_b1;
+    v[j] = v[j] * a.beta2 + (a.one_m_b2 * gj) * gj;
+    const float denom = sqrtf(v[j]) * a.inv_bc2_sqrt + a.eps;
+    p[j] = p[j] - a.step_size * (m[j] / denom);
+    const uint32_t bm = __float_as_uint(m[j]) & 0x7fffffffu, bv = __float_as_uint(v[j]) & 0x7fffffffu;
+    if (j < cnt) {
+      am = bm < pk_fp8::INF_BITS && bm > am ? bm : am;
+      av = bv < pk_fp8::INF_BITS && bv > av ? bv : av;
+    }
+  }
+  const uint32_t byte_m = pk_fp8::scale_byte(pk_fp8::row_max(am), pk_fp8::TOP_E4M3);
+  const uint32_t byte_v = pk_fp8::scale_byte(pk_fp8::row_max(av), pk_fp8::TOP_E5M2);
+  const float im = pk_fp8::inverse_scale_of(byte_m), iv = pk_fp8::inverse_scale_of(byte_v);
+  cm = cv = 0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t r = adam8_random(o + j, a.seed);
+    const float tm = fabsf(m[j]) * im, tv = v[j] * iv;
+    uint32_t km = adam8_round<3, 7>(tm, r >> 16), kv = adam8_round<2, 15>(tv, r & 0xffffu);
+    km = (__float_as_uint(m[j]) & 0x7fffffffu) < pk_fp8::INF_BITS ? km : pk_fp8::NAN_CODE;
+    kv = kv == 0u && tv > 0.f ? 1u : kv;
+    kv = (__float_as_uint(v[j]) & 0x7fffffffu) < pk_fp8::INF_BITS ? kv : pk_fp8::NAN_CODE;
+    cm |= (km | (__float_as_uint(m[j]) >> 31 << 7)) << (8 * j);
+    cv |= kv << (8 * j);
+  }
+  if (vec) {
+    __builtin_nontemporal_store(floatx4_t{p[0], p[1], p[2], p[3]}, reinterpret_cast<floatx4_t*>(st.master + o));
+    __builtin_nontemporal_store(cm, reinterpret_cast<uint32_t*>(st.m + o));
+    __builtin_nontemporal_store(cv, reinterpret_cast<uint32_t*>(st.v + o));
+    if constexpr (SHADOW && sizeof(TSH) == 2) {
+      bf16x4_t sh;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sh[j] = (bf16_t)p[j];
+      __builtin_nontemporal_store(sh, reinterpret_cast<bf16x4_t*>(shadow + o));
+    } else if constexpr (SHADOW) {
+      __builtin_nontemporal_store(floatx4_t{p[0], p[1], p[2], p[3]}, reinterpret_cast<floatx4_t*>(shadow + o));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < cnt) {
+        st.master[o + j] = p[j];
+        st.m[o + j] = (uint8_t)(cm >> (8 * j));
+        st.v[o + j] = (uint8_t)(cv >> (8 * j));
+        if constexpr (SHADOW) shadow[o + j] = pk_from_float<TSH>(p[j]);
+      }
+  }
+  if ((threadIdx.x & 15) == 0 && cnt > 0) {
+    st.m_scale[block] = (uint8_t)byte_m;
+    st.v_scale[block] = (uint8_t)byte_v;
+  }
+}
+
+template <typename TSH, bool SHADOW, bool ZERO>
+__global__ __launch_bounds__(kStreamThreads) void adamw8_kernel(const Adam8State st, float* __restrict__ grad, TSH* __restrict__ shadow,
+                                                                int64_t n, const Adam8Args a) {
+  const int64_t o = ((int64_t)blockIdx.x * kStreamThreads + threadIdx.x) * 4;
+  const int cnt = (int)(n - o < 4 ? n - o : 4);
+  const bool vec = cnt == 4;
+  float g[4] = {};
+  if (vec) {
+    const floatx4_t q = __builtin_nontemporal_load(reinterpret_cast<const floatx4_t*>(grad + o));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = q[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < cnt) g[j] = grad[o + j];
+  }
+  adam8_four<TSH, SHADOW>(st, shadow, o, cnt, vec, g, a);
+  if constexpr (ZERO) {
+    if (vec) {
+      __builtin_nontemporal_store(floatx4_t{0.f, 0.f, 0.f, 0.f}, reinterpret_cast<floatx4_t*>(grad + o));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < cnt) grad[o + j] = 0.f;
+    }
+  }
+}
+
+template <typename TG, bool SHADOW, bool FLAT, bool ZERO>
+__global__ __launch_bounds__(kStreamThreads) void adamw8_packed_kernel(const PackArgs args, const Adam8State st, float* __restrict__ flat_grad,
+                                                                       bf16_t* __restrict__ shadow, const Adam8Args a) {
+  int lo = 0, hi = args.n;  // blk_start[lo] <= blockIdx.x < blk_start[hi]
+  const int b = blockIdx.x;
+  while (hi - lo > 1) {
+    int mid = (lo + hi) >> 1;
+    if (args.blk_start[mid] <= b) lo = mid; else hi = mid;
+  }
+  const int64_t e = (int64_t)(b - args.blk_start[lo]) * kAdamPackChunk + (int64_t)threadIdx.x * 4;
+  const int64_t left = args.numel[lo] - e, o = args.off[lo] + e;
+  const int cnt = (int)(left < 0 ? 0 : left < 4 ? left : 4);
+  const bool vec = cnt == 4;
+  const TG* const src = args.src[lo] ? reinterpret_cast<const TG*>(args.src[lo]) + e : nullptr;
+  float g[4] = {};
+  if (FLAT) {
+    if (vec) {
+      const floatx4_t q = __builtin_nontemporal_load(reinterpret_cast<const floatx4_t*>(flat_grad + o));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = q[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < cnt) g[j] = flat_grad[o + j];
+    }
+  }
+  if (src) {
+    float t[4] = {};
+    if (vec && ((uintptr_t)src & (sizeof(TG) * 4 - 1)) == 0) {
+      if constexpr (sizeof(TG) == 2) {
+        const bf16x4_t r = __builtin_nontemporal_load(reinterpret_cast<const bf16x4_t*>(src));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = (float)r[j];
+      } else {
+        const floatx4_t r = __builtin_nontemporal_load(reinterpret_cast<const floatx4_t*>(src));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = r[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < cnt) t[j] = pk_to_float<TG>(src[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = g[j] + t[j];      // the sum that the pack kernel stores
+  }
+  adam8_four<bf16_t, SHADOW>(st, shadow, o, cnt, vec, g, a);
+  if constexpr (FLAT && ZERO) {
+    if (vec) {
+      __builtin_nontemporal_store(floatx4_t{0.f, 0.f, 0.f, 0.f}, reinterpret_cast<floatx4_t*>(flat_grad + o));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < cnt) flat_grad[o + j] = 0.f;
+    }
+  }
+}
+
+Adam8Args make_adam8_args(double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step, uint32_t seed, float grad_scale) {
+  Adam8Args a;
+  a.decay = (float)(1.0 - lr * weight_decay);
+  a.one_m_b1 = (float)(1.0 - beta1);
+  a.beta2 = (float)beta2;
+  a.one_m_b2 = (float)(1.0 - beta2);
+  a.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+  a.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+  a.eps = (float)eps;
+  a.grad_scale = grad_scale;
+  a.seed = seed;
+  return a;
+}
+
 AdamArgs make_adam_args(float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step, float grad_scale) {
   // scalar prologue in double, as torch does on the host (python floats)
   const double bc1 = 1.0 - pow((double)beta1, (double)step);
@@ -526,6 +752,101 @@ int pk_adamw_fused_packed(float* master, float* exp_avg, float* exp_avg_sq, floa
     else PK_ADAMP_G(float);
 #undef PK_ADAMP_G
 #undef PK_ADAMP
+    PK_RETURN_IF_LAUNCH_FAILED();
+  }
+  return PK_OK;
+}
+
+int pk_adamw8_fused(float* master, uint8_t* exp_avg, uint8_t* exp_avg_scale, uint8_t* exp_avg_sq, uint8_t* exp_avg_sq_scale, float* grad,
+                    void* shadow, int shadow_dtype, int64_t n, double lr, double beta1, double beta2, double eps, double weight_decay,
+                    int64_t step, uint32_t seed, float grad_scale, int zero_grad, pk_stream_t stream) {
+  if (n < 0 || step < 1) return PK_ERR_ARG;
+  if (n == 0) return PK_OK;
+  if (!master || !exp_avg || !exp_avg_scale || !exp_avg_sq || !exp_avg_sq_scale || !grad) return PK_ERR_ARG;
+  if (shadow && !pk_dtype_ok(shadow_dtype)) return PK_ERR_ARG;
+  if (!pk_aligned16(master) || !pk_aligned16(exp_avg) || !pk_aligned16(exp_avg_sq) || !pk_aligned16(grad) || (shadow && !pk_aligned16(shadow)))
+    return PK_ERR_ALIGN;
+  const Adam8Args a = make_adam8_args(lr, beta1, beta2, eps, weight_decay, step, seed, grad_scale);
+  const Adam8State st = {master, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale};
+  hipStream_t s = (hipStream_t)stream;
+  const int64_t nblocks = pk_ceil_div(n, kStreamThreads * 4);
+  if (nblocks > 0x7fffffffll) return PK_ERR_SHAPE;
+  const dim3 grid((unsigned)nblocks), block(kStreamThreads);
+#define PK_ADAM8_LAUNCH(TSH, SH, ZE) \
+  PK_LAUNCH_NOCHECK(pk_timing::K_ADAMW8, s, (adamw8_kernel<TSH, SH, ZE>), grid, block, 0, s, st, grad, reinterpret_cast<TSH*>(shadow), n, a)
+  if (!shadow) {
+    if (zero_grad) PK_ADAM8_LAUNCH(float, false, true); else PK_ADAM8_LAUNCH(float, false, false);
+  } else if (shadow_dtype == PK_BF16) {
+    if (zero_grad) PK_ADAM8_LAUNCH(bf16_t, true, true); else PK_ADAM8_LAUNCH(bf16_t, true, false);
+  } else {
+    if (zero_grad) PK_ADAM8_LAUNCH(float, true, true); else PK_ADAM8_LAUNCH(float, true, false);
+  }
+#undef PK_ADAM8_LAUNCH
+  PK_RETURN_IF_LAUNCH_FAILED();
+  return PK_OK;
+}
+
+int pk_adamw8_fused_packed(float* master, uint8_t* exp_avg, uint8_t* exp_avg_scale, uint8_t* exp_avg_sq, uint8_t* exp_avg_sq_scale,
+                           float* flat_grad, const void* const* grads, const int64_t* offsets, const int64_t* numels, int64_t n, int grad_dtype,
+                           void* shadow, int shadow_dtype, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                           uint32_t seed, float grad_scale, int zero_grad, pk_stream_t stream) {
+  if (n < 0 || step < 1 || !pk_dtype_ok(grad_dtype)) return PK_ERR_ARG;
+  if (n == 0) return PK_OK;
+  if (!master || !exp_avg || !exp_avg_scale || !exp_avg_sq || !exp_avg_sq_scale || !grads || !offsets || !numels) return PK_ERR_ARG;
+  if (shadow && shadow_dtype != PK_BF16) return PK_ERR_UNSUPPORTED;
+  if (!pk_aligned16(master) || !pk_aligned16(exp_avg) || !pk_aligned16(exp_avg_sq) || (flat_grad && !pk_aligned16(flat_grad)) ||
+      (shadow && !pk_aligned16(shadow)))
+    return PK_ERR_ALIGN;
+  for (int64_t i = 0; i < n; ++i)
+    if (numels[i] < 0 || offsets[i] < 0) return PK_ERR_ARG;
+  for (int64_t i = 0; i < n; ++i)
+    if (offsets[i] % PK_ADAMW8_BLOCK != 0) return PK_ERR_ALIGN;
+  const Adam8Args a = make_adam8_args(lr, beta1, beta2, eps, weight_decay, step, seed, grad_scale);
+  const Adam8State st = {master, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale};
+  hipStream_t s = (hipStream_t)stream;
+  int64_t i = 0;
+  while (i < n) {
+    PackArgs pa;
+    pa.n = 0;
+    int64_t blocks = 0;
+    while (i < n && pa.n < kPackTensorsPerLaunch) {
+      if (numels[i] > 0) {      // a tensor without a gradient of its own is still stepped
+        const int64_t nb = pk_ceil_div(numels[i], kAdamPackChunk);
+        if (blocks + nb > 0x7fffffff) break;
+        pa.src[pa.n] = grads[i];
+        pa.off[pa.n] = offsets[i];
+        pa.numel[pa.n] = numels[i];
+        pa.blk_start[pa.n] = (int32_t)blocks;
+        blocks += nb;
+        ++pa.n;
+      }
+      ++i;
+    }
+    if (pa.n == 0) {
+      if (i < n) return PK_ERR_SHAPE;
+      break;
+    }
+    pa.blk_start[pa.n] = (int32_t)blocks;
+    const dim3 grid((unsigned)blocks), block(kStreamThreads);
+#define PK_ADAMP8(TG, SH, FL, ZE)                                                                                                      \
+  PK_LAUNCH_NOCHECK(pk_timing::K_ADAMW8, s, (adamw8_packed_kernel<TG, SH, FL, ZE>), grid, block, 0, s, pa, st, flat_grad, \
+                    reinterpret_cast<bf16_t*>(shadow), a)
+#define PK_ADAMP8_G(TG)                                                                      \
+  do {                                                                                       \
+    if (shadow) {                                                                            \
+      if (!flat_grad) PK_ADAMP8(TG, true, false, false);                                     \
+      else if (zero_grad) PK_ADAMP8(TG, true, true, true);                                   \
+      else PK_ADAMP8(TG, true, true, false);                                                 \
+    } else {                                                                                 \
+      if (!flat_grad) PK_ADAMP8(TG, false, false, false);                                    \
+      else if (zero_grad) PK_ADAMP8(TG, false, true, true);                                  \
+      else PK_ADAMP8(TG, false, true, false);                                                \
+    }                                                                                        \
+  } while (0)
+    if (grad_dtype == PK_BF16) PK_ADAMP8_G(bf16_t);
+    else PK_ADAMP8_G(float);
+#undef PK_ADAMP8_G
+#undef PK_ADAMP8
     PK_RETURN_IF_LAUNCH_FAILED();
   }
   return PK_OK;

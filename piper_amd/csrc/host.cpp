@@ -908,6 +908,192 @@ std::optional<Tensor> bmm_experts(const Tensor& w1, const Tensor& w2, const Tens
   return ExpertsFn::run(w1, w2, w3, x, ExpertsFn::counts_to_starts(counts), nullptr, nullptr);
 }
 
+// ------------------------------------------------------------------------------ bmm_experts in 8-bit blocks
+int64_t whole_blocks(int64_t n) { return (n + PK_FP8_BLOCK - 1) / PK_FP8_BLOCK; }
+uint8_t* u8(const Tensor& t) { return static_cast<uint8_t*>(ptr(t)); }
+
+// Of one weight [E, N, K]: codes, scales and, where wanted, the transposed codes
+std::array<Tensor, 3> quantize_weight(const Tensor& w_, bool transposed) {
+  const Tensor w = contig(w_);
+  const int64_t E = w.size(0), N = w.size(1), K = w.size(2), nb = whole_blocks(N), kb = whole_blocks(K);
+  const auto f8 = w.options().dtype(at::kFloat8_e4m3fn);
+  Tensor q = at::empty({E, N, kb * PK_FP8_BLOCK}, f8), s = at::empty({E, nb, kb}, w.options().dtype(at::kFloat8_e8m0fnu)), t;
+  if (transposed) t = at::empty({E, K, nb * PK_FP8_BLOCK}, f8);
+  PK_CALL(pk_fp8_quantize_weights, ptr(w), dtype_code(w), u8(q), u8(t), u8(s), E, N, K, stream_of(w));
+  return {q, s, t};
+}
+// [q1, q2, q3, s1, s2, s3, t1, t2, t3]; the transposed codes undefined where not wanted
+std::vector<Tensor> quantize_experts(const Tensor& w1, const Tensor& w2, const Tensor& w3, bool transposed) {
+  require_gpu(w1);
+  refuse_transforms({&w1, &w2, &w3}, "quantize_experts");
+  TORCH_CHECK_VALUE(w1.dim() == 3 && w2.dim() == 3 && w3.dim() == 3, "expert weights must be [E,I,H], [E,H,I], [E,I,H]");
+  TORCH_CHECK_VALUE(w3.sizes() == w1.sizes() && w2.size(0) == w1.size(0) && w2.size(1) == w1.size(2) && w2.size(2) == w1.size(1),
+                    "expert weight shapes disagree");
+  TORCH_CHECK_VALUE(w2.scalar_type() == w1.scalar_type() && w3.scalar_type() == w1.scalar_type(), "expert weights must share a dtype");
+  dtype_code(w1);
+  same_device(w1, {&w2, &w3});
+  at::NoGradGuard no_grad;
+  c10::hip::HIPGuard device(w1.device().index());
+  const auto a = quantize_weight(w1, transposed), b = quantize_weight(w2, transposed), c = quantize_weight(w3, transposed);
+  return {a[0], b[0], c[0], a[1], b[1], c[1], a[2], b[2], c[2]};
+}
+// Rows of x [., K] in blocks: (codes [R, K'], scales [R, K' / 128])
+std::pair<Tensor, Tensor> quantize_rows(const Tensor& x_, const OptTensor& row_map_, int64_t map_div) {
+  const Tensor row_map = opt(row_map_);
+  require_gpu(x_);
+  refuse_transforms({&x_, &row_map}, "quantize_rows");
+  TORCH_CHECK_VALUE(x_.dim() == 2 && x_.size(1) > 0, "quantize_rows: x [R,K]");
+  TORCH_CHECK_VALUE(map_div >= 1 && (!row_map.defined() || (row_map.scalar_type() == at::kInt && row_map.dim() == 1 && row_map.is_contiguous())),
+                    "quantize_rows: int32 row map and a divisor of at least 1");
+  TORCH_CHECK_VALUE(row_map.defined() || map_div == 1, "quantize_rows: a divisor needs a row map");
+  same_device(x_, {&row_map});
+  at::NoGradGuard no_grad;
+  c10::hip::HIPGuard device(x_.device().index());
+  const Tensor x = contig(x_);
+  const int64_t R = row_map.defined() ? row_map.numel() : x.size(0), K = x.size(1), kb = whole_blocks(K);
+  Tensor q = at::empty({R, kb * PK_FP8_BLOCK}, x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({R, kb}, x.options().dtype(at::kFloat8_e8m0fnu));
+  PK_CALL(pk_fp8_quantize_rows, ptr(x), dtype_code(x), row_map.defined() ? row_map.data_ptr<int32_t>() : nullptr, map_div, u8(q), u8(s), R, K,
+          stream_of(x));
+  return {q, s};
+}
+
+// The experts' quantized weights, checked against each other.
+struct Fp8Weights {
+  Tensor q[3], s[3], t[3];
+  int64_t E, H, I;
+  Fp8Weights(const Tensor& q1, const Tensor& q2, const Tensor& q3, const Tensor& s1, const Tensor& s2, const Tensor& s3, const Tensor& t1,
+             const Tensor& t2, const Tensor& t3)
+      : q{q1, q2, q3}, s{s1, s2, s3}, t{t1, t2, t3} {
+    TORCH_CHECK_VALUE(q1.dim() == 3 && q2.dim() == 3, "bmm_experts_fp8: codes [E,I,H'], [E,H,I'], [E,I,H']");
+    E = q1.size(0); I = q1.size(1); H = q2.size(1);
+    const int64_t hb = whole_blocks(H), ib = whole_blocks(I), hp = hb * PK_FP8_BLOCK, ip = ib * PK_FP8_BLOCK;
+    const auto is = [&](const Tensor& x, at::ScalarType type, at::IntArrayRef shape) {
+      TORCH_CHECK_VALUE(x.scalar_type() == type && x.sizes() == shape && x.is_contiguous(), "bmm_experts_fp8: expected a contiguous ", type,
+                        " tensor ", shape, ", got ", x.scalar_type(), " ", x.sizes());
+      require_gpu(x);
+      same_device(q1, {&x});
+    };
+    constexpr auto code = at::kFloat8_e4m3fn, scale = at::kFloat8_e8m0fnu;
+    is(q1, code, {E, I, hp}); is(q2, code, {E, H, ip}); is(q3, code, {E, I, hp});
+    is(s1, scale, {E, ib, hb}); is(s2, scale, {E, hb, ib}); is(s3, scale, {E, ib, hb});
+    TORCH_CHECK_VALUE(t1.defined() == t2.defined() && t1.defined() == t3.defined(), "bmm_experts_fp8: transposed codes of all three weights or of none");
+    if (t1.defined()) { is(t1, code, {E, H, ip}); is(t2, code, {E, I, hp}); is(t3, code, {E, H, ip}); }
+  }
+};
+
+struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
+  // buffers of a pass over A rows: x, d_y in blocks ([A, H']), h, d_g, d_u in blocks ([A, I'])
+  static int64_t codes(int64_t A, int64_t width) { return A * whole_blocks(width) * PK_FP8_BLOCK; }
+  static int64_t scales(int64_t A, int64_t width) { return A * whole_blocks(width); }
+  // y [A,H]; gu [2,A,I]: where the pre-activations are left
+  static Tensor run(const Fp8Weights& w, const Tensor& x, const Tensor& starts, Tensor* gu) {
+    const int64_t A = x.size(0), H = w.H, I = w.I;
+    Block b;
+    const size_t x8 = b.add(codes(A, H)), xs = b.add(scales(A, H)), h8 = b.add(codes(A, I)), hs = b.add(scales(A, I));
+    b.allocate(x);
+    Tensor y = at::empty({A, H}, x.options());
+    char* g = nullptr;
+    if (gu) {
+      *gu = at::empty({2, A, I}, x.options());
+      g = static_cast<char*>(gu->data_ptr());
+    }
+    const pk_stream_t st = stream_of(x);
+    const int32_t* const at = starts.data_ptr<int32_t>();
+    const auto p = [&](size_t pos) { return static_cast<uint8_t*>(b.at_(pos)); };
+    PK_CALL(pk_fp8_quantize_rows, ptr(x), PK_BF16, nullptr, 1, p(x8), p(xs), A, H, st);
+    PK_CALL(pk_fp8_gate_up, p(x8), p(xs), nullptr, 1, u8(w.q[0]), u8(w.s[0]), u8(w.q[2]), u8(w.s[2]), at, g, g ? g + A * I * 2 : nullptr, p(h8),
+            p(hs), A, H, I, w.E, st);
+    PK_CALL(pk_fp8_down, p(h8), p(hs), u8(w.q[1]), u8(w.s[1]), at, ptr(y), A, H, I, w.E, st);
+    ExpertsFn::zero_tail(y, starts);
+    return y;
+  }
+  static Tensor forward(AutogradContext* ctx, const OptTensor& w1, const OptTensor& w2, const OptTensor& w3, const Tensor& x, const Fp8Weights* w,
+                        const Tensor& starts) {
+    Tensor gu;
+    const Tensor xc = contig(x);
+    Tensor y = run(*w, xc, starts, &gu);
+    ctx->save_for_backward({xc, starts, gu, w->t[0], w->t[1], w->t[2], w->s[0], w->s[1], w->s[2]});
+    const Tensor p1 = opt(w1), p2 = opt(w2), p3 = opt(w3);
+    keep_parameters(ctx, {&p1, &p2, &p3});
+    ctx->saved_data["weights"] = p1.defined();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list sv = ctx->get_saved_variables();
+    const variable_list params = parameters_of(ctx);
+    const Tensor &p1 = params[0], &p2 = params[1], &p3 = params[2], starts = sv[1], gu = sv[2];
+    const Tensor x = sv[0], d_y = contig(grads[0]), &t1 = sv[3], &t2 = sv[4], &t3 = sv[5], &s1 = sv[6], &s2 = sv[7], &s3 = sv[8];
+    const int64_t E = t1.size(0), H = t1.size(1), I = t2.size(1), A = x.size(0);
+    const bool weights = ctx->saved_data["weights"].toBool();
+    const bool n1 = weights && ctx->needs_input_grad(0), n2 = weights && ctx->needs_input_grad(1), n3 = weights && ctx->needs_input_grad(2);
+    const bool nx = ctx->needs_input_grad(weights ? 3 : 0);
+    const pk_stream_t st = stream_of(x);
+    const int32_t* const at = starts.data_ptr<int32_t>();
+    const int64_t step = A * I * 2;
+    char* const g = static_cast<char*>(gu.data_ptr());
+    Block b;
+    const size_t y8 = b.add(codes(A, H)), ys = b.add(scales(A, H)), g8 = b.add(codes(A, I)), gs = b.add(scales(A, I)), u8_ = b.add(codes(A, I)),
+                 us = b.add(scales(A, I));
+    b.allocate(x);
+    const auto p = [&](size_t pos) { return static_cast<uint8_t*>(b.at_(pos)); };
+    Tensor dguh = at::empty({3, A, I}, x.options()), d_x;      // d_g, d_u, h
+    char* const dg = static_cast<char*>(dguh.data_ptr());
+    PK_CALL(pk_fp8_quantize_rows, ptr(d_y), PK_BF16, nullptr, 1, p(y8), p(ys), A, H, st);
+    PK_CALL(pk_fp8_dgrad_dh, p(y8), p(ys), nullptr, 1, nullptr, u8(t2), u8(s2), g, g + step, at, dg, dg + step, dg + 2 * step, p(g8), p(gs), p(u8_),
+            p(us), nullptr, A, H, I, E, st);
+    if (nx) {
+      d_x = at::empty({A, H}, x.options());
+      PK_CALL(pk_fp8_dgrad_dx, p(g8), p(gs), p(u8_), p(us), u8(t1), u8(s1), u8(t3), u8(s3), at, ptr(d_x), A, H, I, E, st);
+      ExpertsFn::zero_tail(d_x, starts);
+    }
+    const auto wgrad = [d_y, dguh, x, starts, A, H, I, E, step](const Tensor& d1, const Tensor& d2, const Tensor& d3, bool accumulate) {
+      char* const ds = static_cast<char*>(dguh.data_ptr());
+      PK_CALL(pk_grouped_swiglu_wgrad, ptr(d_y), ds + 2 * step, ds, ds + step, ptr(x), nullptr, 1, starts.data_ptr<int32_t>(), nullptr, ptr(d1),
+              ptr(d2), ptr(d3), accumulate, A, H, I, E, PK_BF16, stream_of(x));
+    };
+    Tensor d1, d2, d3;
+    if (n1 && n2 && n3 && g_deferring.load() && leaf(p1) && leaf(p2) && leaf(p3)) {
+      push_deferred([wgrad, p1, p2, p3] { weight_grads_into_params(p1, p2, p3, wgrad); });
+    } else if (n1 && n2 && n3 && g_accumulate.load() && accumulates_in_place(p1) && accumulates_in_place(p2) && accumulates_in_place(p3)) {
+      wgrad(p1.grad(), p2.grad(), p3.grad(), true);
+    } else if (n1 || n2 || n3) {
+      d1 = at::empty({E, I, H}, x.options());
+      d2 = at::empty({E, H, I}, x.options());
+      d3 = at::empty({E, I, H}, x.options());
+      wgrad(d1, d2, d3, false);
+    }
+    if (!weights) return {Tensor(), Tensor(), Tensor(), d_x, Tensor(), Tensor()};
+    return {d1, d2, d3, d_x, Tensor(), Tensor()};
+  }
+};
+std::optional<Tensor> bmm_experts_fp8(const OptTensor& w1_, const OptTensor& w2_, const OptTensor& w3_, const Tensor& q1, const Tensor& q2,
+                                      const Tensor& q3, const Tensor& s1, const Tensor& s2, const Tensor& s3, const OptTensor& t1_,
+                                      const OptTensor& t2_, const OptTensor& t3_, const Tensor& x, const Tensor& counts, bool direct) {
+  const Tensor w1 = opt(w1_), w2 = opt(w2_), w3 = opt(w3_), t1 = opt(t1_), t2 = opt(t2_), t3 = opt(t3_);
+  if (direct && !plain({&w1, &w2, &w3, &q1, &q2, &q3, &s1, &s2, &s3, &t1, &t2, &t3, &x, &counts})) return std::nullopt;
+  refuse_transforms({&w1, &w2, &w3, &q1, &q2, &q3, &s1, &s2, &s3, &t1, &t2, &t3, &x, &counts}, "bmm_experts_fp8");
+  const RecordDirect record(direct, "piper_amd::bmm_experts_fp8");
+  require_gpu(x);
+  require_gpu(counts);
+  const Fp8Weights w(q1, q2, q3, s1, s2, s3, t1, t2, t3);
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16, "bmm_experts_fp8: rows are bfloat16, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == w.H && counts.dim() == 1 && counts.numel() == w.E, "bmm_experts_fp8: x [A,H] and a row count for every expert");
+  TORCH_CHECK_VALUE(w1.defined() == w2.defined() && w1.defined() == w3.defined(), "bmm_experts_fp8: all three weights or none");
+  if (w1.defined())
+    TORCH_CHECK_VALUE(w1.sizes() == at::IntArrayRef({w.E, w.I, w.H}) && w3.sizes() == w1.sizes() && w2.sizes() == at::IntArrayRef({w.E, w.H, w.I}),
+                      "expert weight shapes disagree");
+  same_device(x, {&w1, &w2, &w3, &q1, &counts});
+  c10::hip::HIPGuard device(x.device().index());
+  const Tensor starts = ExpertsFn::counts_to_starts(counts);
+  if (wants_grad({&w1, &w2, &w3, &x})) {
+    TORCH_CHECK_VALUE(t1.defined(), "bmm_experts_fp8: a backward needs the transposed codes (quantize_experts(..., for_backward=True))");
+    TORCH_CHECK_TYPE(!wants_grad({&w1, &w2, &w3}) || (w1.scalar_type() == at::kBFloat16 && w2.scalar_type() == at::kBFloat16 && w3.scalar_type() == at::kBFloat16),
+                     "bmm_experts_fp8: weights that want gradients are bfloat16");
+    return Fp8ExpertsFn::apply(w1_, w2_, w3_, x, &w, starts);
+  }
+  return Fp8ExpertsFn::run(w, contig(x), starts, nullptr);
+}
+
 // ------------------------------------------------------------------------------ bucket path
 // A bucket's tensors with their places, as BucketState.param_view_specs lists them:
 // (parameter, element offset, element count, shape).
@@ -1032,6 +1218,49 @@ void adamw_packed(const Tensor& master, const Tensor& exp_avg, const Tensor& exp
           (float)weight_decay, step, (float)grad_scale, zero_grad, stream_of(master));
 }
 
+// The same checks for the step with 8-bit moments.
+void adamw8_packed(const Tensor& master, const std::array<Tensor, 4>& moments, const Tensor& flat_grad, const std::vector<OptTensor>& grads,
+                   const std::vector<int64_t>& offsets, const std::vector<int64_t>& numels, int64_t step, double lr, double beta1, double beta2,
+                   double eps, double weight_decay, uint32_t seed, const Tensor& shadow, double grad_scale, bool zero_grad) {
+  require_gpu(master);
+  c10::hip::HIPGuard device(master.device().index());
+  const size_t n = grads.size();
+  TORCH_CHECK_VALUE(offsets.size() == n && numels.size() == n, "adamw8_fused_packed: one offset and element count per tensor");
+  const int64_t total = master.numel(), blocks = (total + PK_ADAMW8_BLOCK - 1) / PK_ADAMW8_BLOCK;
+  TORCH_CHECK_VALUE(master.scalar_type() == at::kFloat && master.is_contiguous(), "adamw8_fused_packed: fp32 contiguous master");
+  const at::ScalarType types[4] = {at::kFloat8_e4m3fn, at::kFloat8_e8m0fnu, at::kFloat8_e5m2, at::kFloat8_e8m0fnu};
+  for (int i = 0; i < 4; ++i)
+    TORCH_CHECK_VALUE(moments[i].scalar_type() == types[i] && moments[i].numel() == (i % 2 ? blocks : total) && moments[i].is_contiguous(),
+                      "adamw8_fused_packed: exp_avg e4m3 and exp_avg_sq e5m2 of the bucket's size, with an e8m0 scale for each ", PK_ADAMW8_BLOCK,
+                      " elements");
+  TORCH_CHECK_VALUE(!flat_grad.defined() || (flat_grad.scalar_type() == at::kFloat && flat_grad.numel() == total && flat_grad.is_contiguous()),
+                    "adamw8_fused_packed: flat_grad must match the bucket");
+  TORCH_CHECK_VALUE(!shadow.defined() || (shadow.scalar_type() == at::kBFloat16 && shadow.numel() == total && shadow.is_contiguous()),
+                    "adamw8_fused_packed: bf16 shadow of the bucket's size");
+  same_device(master, {&moments[0], &moments[1], &moments[2], &moments[3], &flat_grad, &shadow});
+  std::vector<const void*> ptrs(std::max<size_t>(n, 1), nullptr);
+  std::vector<Tensor> keep;
+  std::optional<at::ScalarType> dtype;
+  for (size_t i = 0; i < n; ++i) {
+    TORCH_CHECK_VALUE(offsets[i] >= 0 && numels[i] >= 0 && numels[i] <= total && offsets[i] <= total - numels[i], "adamw8_fused_packed: tensor outside the bucket");
+    TORCH_CHECK_VALUE(offsets[i] % PK_ADAMW8_BLOCK == 0, "adamw8_fused_packed: tensors start at multiples of ", PK_ADAMW8_BLOCK, " elements");
+    TORCH_CHECK_VALUE(i == 0 || offsets[i] >= offsets[i - 1] + numels[i - 1], "adamw8_fused_packed: tensors in the order of their places, none over another");
+    if (!grads[i].has_value() || !grads[i]->defined()) continue;
+    const Tensor& g = *grads[i];
+    TORCH_CHECK_VALUE(g.numel() == numels[i], "adamw8_fused_packed: gradient size differs from the tensor's");
+    same_device(master, {&g});
+    TORCH_CHECK_VALUE(!dtype || *dtype == g.scalar_type(), "adamw8_fused_packed: gradients of one call must share a dtype");
+    dtype = g.scalar_type();
+    dtype_code(g);
+    keep.push_back(contig(g));
+    ptrs[i] = keep.back().data_ptr();
+  }
+  const int code = !dtype || *dtype == at::kBFloat16 ? PK_BF16 : PK_F32;
+  PK_CALL(pk_adamw8_fused_packed, master.data_ptr<float>(), u8(moments[0]), u8(moments[1]), u8(moments[2]), u8(moments[3]),
+          static_cast<float*>(ptr(flat_grad)), ptrs.data(), offsets.data(), numels.data(), (int64_t)n, code, ptr(shadow), PK_BF16, lr, beta1, beta2,
+          eps, weight_decay, step, seed, (float)grad_scale, zero_grad, stream_of(master));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1052,6 +1281,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                            bool zero_grad) {
     adamw_packed(master, exp_avg, exp_avg_sq, opt(flat_grad), grads, offsets, numels, step, lr, beta1, beta2, eps, weight_decay, opt(shadow),
                  grad_scale, zero_grad);
+  });
+  m.def("quantize_experts", &quantize_experts, nogil);
+  m.def("quantize_rows", &quantize_rows, nogil);
+  m.def("bmm_experts_fp8", &bmm_experts_fp8, nogil);
+  m.def("adamw8_packed", [](const Tensor& master, const Tensor& exp_avg, const Tensor& exp_avg_scale, const Tensor& exp_avg_sq,
+                            const Tensor& exp_avg_sq_scale, const OptTensor& flat_grad, const std::vector<OptTensor>& grads,
+                            const std::vector<int64_t>& offsets, const std::vector<int64_t>& numels, int64_t step, double lr, double beta1, double beta2,
+                            double eps, double weight_decay, uint32_t seed, const OptTensor& shadow, double grad_scale, bool zero_grad) {
+    adamw8_packed(master, {exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale}, opt(flat_grad), grads, offsets, numels, step, lr, beta1, beta2, eps,
+                  weight_decay, seed, opt(shadow), grad_scale, zero_grad);
   });
   py::class_<StreamScope>(m, "StreamScope")
       .def(py::init<int64_t, int64_t, int64_t>())

@@ -13,6 +13,8 @@ Two ways in:
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 from torch.overrides import has_torch_function_variadic
 
@@ -169,6 +171,63 @@ def bmm_experts(w1, w2, w3, x, num_tokens_per_expert):
     return torch.ops.piper_artifact.bmm_experts(w1, w2, w3, x, num_tokens_per_expert)
 
 
+# --------------------------------------------------------------------------- experts in 8-bit blocks
+class Fp8Experts(NamedTuple):
+    """The three expert weights in 8-bit floating point (``quantize_experts``): e4m3 codes (``q``; ``t`` transposed, for the
+    backward) with a power of two for each block of 128 x 128 (``s``, float8_e8m0fnu), rows padded with zeros to whole blocks.
+    ``w1``, ``w2``, ``w3`` are the weights that the gradients belong to (None: none are wanted)."""
+
+    w1: torch.Tensor | None      # [E,I,H]
+    w2: torch.Tensor | None      # [E,H,I]
+    w3: torch.Tensor | None      # [E,I,H]
+    q1: torch.Tensor             # [E,I,H']   H' = ceil(H / 128) * 128
+    q2: torch.Tensor             # [E,H,I']
+    q3: torch.Tensor             # [E,I,H']
+    s1: torch.Tensor             # [E,I'/128,H'/128]
+    s2: torch.Tensor             # [E,H'/128,I'/128]
+    s3: torch.Tensor             # [E,I'/128,H'/128]
+    t1: torch.Tensor | None = None      # [E,H,I']
+    t2: torch.Tensor | None = None      # [E,I,H']
+    t3: torch.Tensor | None = None      # [E,H,I']
+
+
+def quantize_experts(w1, w2, w3, *, for_backward: bool = True) -> Fp8Experts:
+    """The experts' weights (bfloat16 or float32) for ``bmm_experts_fp8``.  The result is a copy of what they are now: make
+    a new one after every optimizer step.  ``for_backward=False`` leaves out the transposed codes, which only a backward reads."""
+    return Fp8Experts(w1, w2, w3, *host().quantize_experts(w1, w2, w3, bool(for_backward)))
+
+
+def _bmm_experts_fp8(*args):
+    x = args[12]
+    if _traced_without_data(x):
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (*args[:3], x) if t is not None):
+            out.requires_grad_(True)
+        return out
+    return host().bmm_experts_fp8(*args, False)
+
+
+def _bmm_experts_fp8_forward_only(*args):
+    with torch.no_grad():
+        return _bmm_experts_fp8(*args)
+
+
+def bmm_experts_fp8(experts: Fp8Experts, x, num_tokens_per_expert):
+    """``bmm_experts`` with its products in 8-bit floating point.  x [A,H] (bfloat16, sorted by expert) is held in blocks of 128
+    values of a row with a power of two each, the weights in blocks of 128 x 128; sums are fp32.  gate and up are
+    rounded to bfloat16 as there, silu(gate) * up goes into such blocks again.
+
+    Backward: d_y and the gradients of gate and up are held in the same blocks for the products that lead to x, rounding counts
+    as the identity; the weights' gradients (of ``experts.w1``, ``w2``, ``w3``) are bfloat16 products of the rows as they came.
+    ``defer_weight_grads`` and ``accumulate_weight_grads`` apply as they do to ``bmm_experts``."""
+    args = (*experts, x, num_tokens_per_expert)
+    if _direct(*args):
+        out = host().bmm_experts_fp8(*args, True)
+        if out is not None:
+            return out
+    return torch.ops.piper_amd.bmm_experts_fp8(*args)
+
+
 def _combine(y, perm, top_scores):
     return host().combine(y, perm, _inverse_of(perm), top_scores)
 
@@ -294,8 +353,11 @@ def register_region_ops() -> bool:
     lib.define("expert_region(Tensor x, Tensor w_gate, Tensor? gate_bias, Tensor w1, Tensor w2, Tensor w3, "
                "int top_k, bool route_norm, float route_scale, Tensor? residual) -> Tensor")
     lib.define("rmsnorm(Tensor x, Tensor weight, float eps) -> Tensor")
+    lib.define("bmm_experts_fp8(Tensor? w1, Tensor? w2, Tensor? w3, Tensor q1, Tensor q2, Tensor q3, Tensor s1, Tensor s2, Tensor s3, "
+               "Tensor? t1, Tensor? t2, Tensor? t3, Tensor x, Tensor num_tokens_per_expert) -> Tensor")
     for name, fwd, auto in (("expert_region", _expert_region_forward_only, _expert_region_autograd),
-                            ("rmsnorm", _rmsnorm_forward_only, _rmsnorm_autograd)):
+                            ("rmsnorm", _rmsnorm_forward_only, _rmsnorm_autograd),
+                            ("bmm_experts_fp8", _bmm_experts_fp8_forward_only, _bmm_experts_fp8)):
         lib.impl(name, fwd, "CUDA")
         lib.impl(name, auto, "AutogradCUDA")
         lib.impl(name, fwd, "Meta")

@@ -72,7 +72,14 @@ class BmmExperts(nn.Module):
         self.w2 = nn.Parameter(torch.empty(num_experts, dim, hidden_dim, dtype=dtype))
         self.w3 = nn.Parameter(torch.empty(num_experts, hidden_dim, dim, dtype=dtype))
 
-    def forward(self, x: torch.Tensor, num_tokens_per_expert: torch.Tensor) -> torch.Tensor:
+    def quantize(self, *, for_backward: bool = True) -> F_.Fp8Experts:
+        """The weights as they are now in 8-bit blocks, for forward passes until the next optimizer step."""
+        return F_.quantize_experts(self.w1, self.w2, self.w3, for_backward=for_backward)
+
+    def forward(self, x: torch.Tensor, num_tokens_per_expert: torch.Tensor, experts_fp8: F_.Fp8Experts | None = None) -> torch.Tensor:
+        """``experts_fp8`` (of ``quantize``): the products run in 8-bit floating point."""
+        if experts_fp8 is not None:
+            return F_.bmm_experts_fp8(experts_fp8, x, num_tokens_per_expert)
         return F_.bmm_experts(self.w1, self.w2, self.w3, x, num_tokens_per_expert)
 
 
@@ -104,12 +111,13 @@ class AnnotatedMoE(nn.Module):
         if self.router.gate.bias is not None:
             nn.init.zeros_(self.router.gate.bias)
 
-    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
-        """``residual`` (same shape as x; fused path only) is added in the combine kernel."""
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, experts_fp8: F_.Fp8Experts | None = None) -> torch.Tensor:
+        """``residual`` (same shape as x; fused path only) is added in the combine kernel.  ``experts_fp8`` (of
+        ``experts.quantize()``): the experts' products run in 8-bit floating point, through the piecewise operators."""
         bs, slen, dim = x.shape
         x2 = x.reshape(-1, dim)
         top_k = self.router.top_k
-        if self.fused:
+        if self.fused and experts_fp8 is None:
             with annotate(EP_TAG):
                 out = F_.expert_region(x2, self.router.gate.weight, self.router.gate.bias, self.experts.w1,
                                        self.experts.w2, self.experts.w3, top_k=top_k,
@@ -117,14 +125,15 @@ class AnnotatedMoE(nn.Module):
                                        residual=None if residual is None else residual.reshape(-1, dim))
             return out.reshape(bs, slen, dim)
         if residual is not None:
-            return residual + self.forward(x)
+            return residual + self.forward(x, experts_fp8=experts_fp8)
 
         top_scores, selected_experts_indices, num_tokens_per_expert = self.router(x2, self.expert_bias)
         _scores_sorted, token_indices_experts_sorted, num_tokens_per_expert = self.reorderer(
             top_scores, selected_experts_indices)
         routed_input = F_.permute(x2, token_indices_experts_sorted, top_k)
         with annotate(EP_TAG):
-            gathered_output = self.experts(routed_input, num_tokens_per_expert)
+            gathered_output = (self.experts(routed_input, num_tokens_per_expert) if experts_fp8 is None else
+                               self.experts(routed_input, num_tokens_per_expert, experts_fp8))
         out_experts = F_.combine(gathered_output.reshape(-1, dim), token_indices_experts_sorted, top_scores)
         return out_experts.reshape(bs, slen, dim)
 

@@ -392,6 +392,12 @@ def grouped_swiglu_wgrad(d_y, h, d_g, d_u, x_rows, starts, E, *, row_map=None, r
     return d_w1, d_w2, d_w3
 
 
+def quantize_rows_fp8(x: torch.Tensor, row_map: torch.Tensor | None = None, row_map_div: int = 1):
+    """Rows of x [R,K] (or x[row_map // row_map_div]) in 8-bit floating point: (e4m3 codes [R,K'], e8m0 scales [R,K'/128]) with
+    K' = ceil(K / 128) * 128; a value is code * scale of its block of 128, the rest of the last block is zero."""
+    return host().quantize_rows(x, row_map, int(row_map_div))
+
+
 # ------------------------------------------------------------------------- bucket path
 def bucket_plan(numels: Sequence[int], elem_size: int, align_bytes: int = 256):
     """Host-only: element offsets of tensors laid out back to back with aligned starts.
@@ -477,3 +483,49 @@ def adamw_fused_packed(master, exp_avg, exp_avg_sq, flat_grad, grads: Sequence[t
     result equals bucket_pack(accumulate=True) followed by adamw_fused bit for bit."""
     host().adamw_packed(master, exp_avg, exp_avg_sq, flat_grad, list(grads), list(offsets), list(numels), int(step), float(lr),
                         float(beta1), float(beta2), float(eps), float(weight_decay), shadow, float(grad_scale), bool(zero_grad))
+
+
+ADAMW8_BLOCK = 64      # elements that share a scale in the 8-bit moments
+
+
+def adamw8_state(n: int, device) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Moments of zero for adamw8_fused over n elements: (exp_avg e4m3 [n], its scales e8m0 [ceil(n / 64)], exp_avg_sq e5m2 [n], its
+    scales)."""
+    blocks = -(-n // ADAMW8_BLOCK)
+    return tuple(torch.zeros(k, dtype=torch.uint8, device=device).view(dt)
+                 for k, dt in ((n, torch.float8_e4m3fn), (blocks, torch.float8_e8m0fnu), (n, torch.float8_e5m2), (blocks, torch.float8_e8m0fnu)))
+
+
+def adamw8_fused(master, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, grad, *, step: int, lr: float, beta1: float, beta2: float,
+                 eps: float, weight_decay: float, seed: int, shadow: torch.Tensor | None = None, grad_scale: float = 1.0,
+                 zero_grad: bool = False) -> None:
+    """adamw_fused with both moments in 8-bit floating point, a power of two for each 64 elements (adamw8_state).  They are
+    rounded up or down at random so that their means are right; `seed` (its lowest 32 bits) chooses the bits: another one for every
+    step."""
+    require_gpu(master)
+    n, blocks = master.numel(), -(-master.numel() // ADAMW8_BLOCK)
+    for t in (master, grad):
+        _check(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous(), "adamw8_fused: fp32 contiguous buffers of equal size")
+    for t, k, dt in ((exp_avg, n, torch.float8_e4m3fn), (exp_avg_scale, blocks, torch.float8_e8m0fnu),
+                     (exp_avg_sq, n, torch.float8_e5m2), (exp_avg_sq_scale, blocks, torch.float8_e8m0fnu)):
+        _check(t.dtype == dt and t.numel() == k and t.is_contiguous(),
+               "adamw8_fused: exp_avg e4m3 and exp_avg_sq e5m2 of the bucket's size, with an e8m0 scale for each 64 elements")
+    if shadow is not None:
+        _check(shadow.numel() == n and shadow.is_contiguous(), "adamw8_fused: shadow must match the bucket")
+    _check(all(t.device == master.device for t in (exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, grad, shadow) if t is not None),
+           "adamw8_fused: all tensors of a call must be on one device")
+    with torch.cuda.device(master.device):
+        call("pk_adamw8_fused", ptr(master), ptr(exp_avg), ptr(exp_avg_scale), ptr(exp_avg_sq), ptr(exp_avg_sq_scale), ptr(grad), ptr(shadow),
+             dtype_code(shadow.dtype) if shadow is not None else 0, n, float(lr), float(beta1), float(beta2), float(eps), float(weight_decay),
+             int(step), int(seed) & 0xFFFFFFFF, float(grad_scale), int(bool(zero_grad)), current_stream(master.device))
+
+
+def adamw8_fused_packed(master, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, flat_grad, grads: Sequence[torch.Tensor | None],
+                        offsets: Sequence[int], numels: Sequence[int], *, step: int, lr: float, beta1: float, beta2: float, eps: float,
+                        weight_decay: float, seed: int, shadow: torch.Tensor | None = None, grad_scale: float = 1.0,
+                        zero_grad: bool = False) -> None:
+    """adamw_fused_packed with the moments of adamw8_fused.  Offsets are multiples of 64, tensors in the order of their places.  The
+    result equals bucket_pack(accumulate=True) followed by adamw8_fused bit for bit in a bucket whose padding is zero."""
+    host().adamw8_packed(master, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, flat_grad, list(grads), list(offsets), list(numels),
+                         int(step), float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF, shadow,
+                         float(grad_scale), bool(zero_grad))

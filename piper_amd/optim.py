@@ -6,6 +6,10 @@ Every parameter handed in is treated as one flat buffer and updated by ONE kerne
 reads grad/master/exp_avg/exp_avg_sq and writes master/exp_avg/exp_avg_sq (28 B/element) plus,
 for a bf16 parameter, the bf16 value the model reads (+2 B/element).  bf16 parameters get an fp32
 master copy; fp32 parameters are their own master.
+
+``state_bits=8``: both moments are held in 8-bit floating point with a power of two for each 64 elements, rounded up or down
+at random so that their means are right (ops.adamw8_fused): 2 instead of 8 bytes of state an element, 18 instead of 30 B of traffic.
+``seed`` chooses the random bits; runs with one seed repeat bit for bit.
 """
 from __future__ import annotations
 
@@ -16,12 +20,16 @@ from . import ops
 
 class FusedAdamW(torch.optim.Optimizer):
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 1e-2, fused: bool = True, zero_grad_in_step: bool = False):
+                 weight_decay: float = 1e-2, fused: bool = True, zero_grad_in_step: bool = False, state_bits: int = 32,
+                 seed: int = 0):
         if lr < 0 or eps < 0 or not (0 <= betas[0] < 1) or not (0 <= betas[1] < 1) or weight_decay < 0:
             raise ValueError("invalid AdamW hyper-parameters")
+        if state_bits not in (8, 32):
+            raise ValueError(f"FusedAdamW holds its moments in 32 or 8 bits, not {state_bits}")
         defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
         self.zero_grad_in_step = zero_grad_in_step
+        self.state_bits, self.seed = state_bits, int(seed)
 
     def _init_state(self, p: torch.Tensor) -> dict:
         st = self.state[p]
@@ -29,6 +37,12 @@ class FusedAdamW(torch.optim.Optimizer):
             flat = p.detach().reshape(-1)
             st["step"] = 0
             st["master"] = flat if p.dtype == torch.float32 else flat.float()
+            if self.state_bits == 8:
+                for name, t in zip(_MOMENTS8, ops.adamw8_state(flat.numel(), flat.device)):
+                    st[name] = t
+                # elements of different buckets with the same index get other bits
+                st["seed"] = self.seed + 0x632BE5AB * (len(self.state) - 1)
+                return st
             st["exp_avg"] = torch.zeros_like(st["master"])
             st["exp_avg_sq"] = torch.zeros_like(st["master"])
         return st
@@ -53,6 +67,9 @@ class FusedAdamW(torch.optim.Optimizer):
                 if not owns_grad:
                     grad = grad.float().contiguous()
                 shadow = None if p.dtype == torch.float32 else p.detach().reshape(-1)
+                if self.state_bits == 8:
+                    self._step8(st, grad, group, shadow, self.zero_grad_in_step and owns_grad)
+                    continue
                 ops.adamw_fused(st["master"], st["exp_avg"], st["exp_avg_sq"], grad, step=st["step"],
                                 lr=group["lr"], beta1=b1, beta2=b2, eps=group["eps"],
                                 weight_decay=group["weight_decay"], shadow=shadow,
@@ -73,7 +90,53 @@ class FusedAdamW(torch.optim.Optimizer):
         st["step"] += 1
         b1, b2 = group["betas"]
         shadow = None if p.dtype == torch.float32 else p.detach().reshape(-1)
+        if self.state_bits == 8:
+            clear = self.zero_grad_in_step and flat_grad is not None
+            if all(o % ops.ADAMW8_BLOCK == 0 for o in offsets):
+                ops.adamw8_fused_packed(st["master"], *(st[k] for k in _MOMENTS8), flat_grad, list(grads), list(offsets), list(numels),
+                                        shadow=shadow, zero_grad=clear, **self._how8(st, group))
+                return
+            # a block of the moments may belong to two tensors (a bucket without aligned starts): packed first, into a copy
+            flat = torch.zeros_like(st["master"]) if flat_grad is None else flat_grad.clone()
+            ops.bucket_pack(list(grads), list(offsets), flat, accumulate=True, numels=list(numels))
+            self._step8(st, flat, group, shadow, False)
+            if clear:
+                for o, n in zip(offsets, numels):
+                    flat_grad[o:o + n].zero_()
+            return
         ops.adamw_fused_packed(st["master"], st["exp_avg"], st["exp_avg_sq"], flat_grad, list(grads), list(offsets),
                                list(numels), step=st["step"], lr=group["lr"], beta1=b1, beta2=b2, eps=group["eps"],
                                weight_decay=group["weight_decay"], shadow=shadow,
                                zero_grad=self.zero_grad_in_step and flat_grad is not None)
+
+    def _how8(self, st: dict, group: dict) -> dict:
+        b1, b2 = group["betas"]
+        return dict(step=st["step"], lr=group["lr"], beta1=b1, beta2=b2, eps=group["eps"], weight_decay=group["weight_decay"],
+                    seed=st["seed"] + 0x9E3779B1 * st["step"])
+
+    def _step8(self, st: dict, grad: torch.Tensor, group: dict, shadow, zero_grad: bool) -> None:
+        ops.adamw8_fused(st["master"], *(st[k] for k in _MOMENTS8), grad, shadow=shadow, zero_grad=zero_grad, **self._how8(st, group))
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict) -> None:
+        """torch's, which gives every floating-point state the parameter's type: the 8-bit moments and their master keep theirs."""
+        super().load_state_dict(state_dict)
+        if self.state_bits != 8:
+            return
+        params = [p for group in self.param_groups for p in group["params"]]
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for p, i in zip(params, saved):
+            st = state_dict["state"].get(i)
+            if st is None:
+                continue
+            if any(k not in st for k in _MOMENTS8):
+                raise ValueError("FusedAdamW(state_bits=8): the saved state has no 8-bit moments")
+            for name in _MOMENTS8:
+                self.state[p][name] = st[name].to(p.device).clone()
+            if p.dtype == torch.float32:      # its own master
+                self.state[p]["master"] = p.detach().reshape(-1)
+            else:
+                self.state[p]["master"] = st["master"].to(p.device).clone()
+
+
+_MOMENTS8 = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")

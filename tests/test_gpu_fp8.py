@@ -1,0 +1,321 @@
+"""The experts in 8-bit blocks: quantisation bit for bit, products and gradients within the bounds that oracle/blocks.py derives for
+sums and functions in fp32, and the operator where callers meet it (strides, streams, graphs, split backward, tracing)."""
+import math
+
+import pytest
+import torch
+
+from oracle import blocks as B
+from piper_amd import functional as F_
+from piper_amd import ops
+from piper_amd.moe import AnnotatedMoE, BmmExperts, MoEArgs
+
+pytestmark = pytest.mark.gpu
+
+E4M3 = torch.float8_e4m3fn
+
+
+def _same(got, want):
+    """Equal values, NaN in the same places."""
+    got, want = got.double().cpu(), want.double().cpu()
+    return torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+def _exponents(s):
+    return s.view(torch.uint8).cpu().to(torch.int64) - 127
+
+
+def _awkward(shape, dtype, seed):
+    """Normal values with rows of every magnitude, zeros, subnormals, values on the border of two scales."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g)
+    flat = x.view(-1, shape[-1])
+    for i, f in enumerate((1.0, 0.0, 1e-38, 1e-30, 1e30, 448.0, 1e-45, 3.0)):
+        if i < flat.shape[0]:
+            flat[i] *= f
+    flat[-1, : shape[-1] // 2] = 1.75
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,width", [(1, 1), (9, 128), (3, 129), (17, 1000), (5, 2048), (40, 127), (300, 384)])
+def test_rows_are_quantized_bit_for_bit(dev, rows, width, dtype):
+    print(f"[case] quantize rows {rows} x {width} {dtype}", flush=True)
+    x = _awkward((rows, width), dtype, rows)
+    q, s = ops.quantize_rows_fp8(x.to(dev))
+    want, k = B.rows(x)
+    assert q.dtype == E4M3 and q.shape == want.shape and _same(q, want) and torch.equal(_exponents(s), k)
+
+
+def test_rows_gathered_strided_unaligned_and_not_finite(dev):
+    print("[case] quantize rows: map, strides, offsets, NaN", flush=True)
+    x = _awkward((12, 264), torch.bfloat16, 3)
+    x[4, 130], x[7, 0], x[8, 263] = math.inf, math.nan, -math.inf
+    perm = torch.tensor([23, 0, 5, 5, 11, 22, 9], dtype=torch.int32)
+    want, k = B.rows(x[(perm // 2).long()])
+    q, s = ops.quantize_rows_fp8(x.to(dev), perm.to(dev), 2)
+    assert _same(q, want) and torch.equal(_exponents(s), k)
+    wide = torch.zeros(12, 300, dtype=torch.bfloat16)
+    wide[:, 3:267] = x
+    for view in (wide.to(dev)[:, 3:267], x.to(dev).t().contiguous().t(), torch.cat([torch.zeros(1, dtype=x.dtype), x.reshape(-1)]).to(dev)[1:].view(12, 264)):
+        q, s = ops.quantize_rows_fp8(view)
+        want, k = B.rows(x)
+        assert _same(q, want) and torch.equal(_exponents(s), k)
+    q, s = ops.quantize_rows_fp8(x[:0].to(dev))
+    assert q.shape == (0, 384) and s.shape == (0, 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("E,I,H", [(1, 128, 128), (2, 1, 1), (3, 130, 257), (2, 360, 1000), (1, 384, 256), (4, 127, 200)])
+def test_weights_are_quantized_bit_for_bit_both_ways(dev, E, I, H, dtype):
+    print(f"[case] quantize weights {E} x {I} x {H} {dtype}", flush=True)
+    w1, w3, w2 = _awkward((E, I, H), dtype, 0), _awkward((E, I, H), dtype, 1), _awkward((E, H, I), dtype, 2)
+    w1[-1, -1, -1] = math.nan
+    got = F_.quantize_experts(w1.to(dev), w2.to(dev), w3.to(dev))
+    for w, q, s, t in ((w1, got.q1, got.s1, got.t1), (w2, got.q2, got.s2, got.t2), (w3, got.q3, got.s3, got.t3)):
+        want, k = B.weights(w)
+        N, K = w.shape[1:]
+        assert torch.equal(_exponents(s), k)
+        assert q.shape == (E, N, want.shape[2]) and _same(q, want[:, :N])
+        assert t.shape == (E, K, want.shape[1]) and _same(t, want[:, :, :K].transpose(1, 2))
+    less = F_.quantize_experts(w1.to(dev), w2.to(dev), w3.to(dev), for_backward=False)
+    assert less.t1 is None and _same(less.q2, got.q2)
+
+
+# ------------------------------------------------------------------------------ products
+def _inputs(E, H, I, counts, spare, seed, integers):
+    g = torch.Generator().manual_seed(seed)
+    A = sum(counts) + spare
+    if integers:      # sums of these are exact in fp32 in any order, and every value is a code
+        mk = lambda *shape, unit: (torch.randint(-4, 5, shape, generator=g) * unit).bfloat16()  # noqa: E731
+        return (mk(E, I, H, unit=2.0 ** -7), mk(E, H, I, unit=2.0 ** -6), mk(E, I, H, unit=2.0 ** -7), mk(A, H, unit=0.5), mk(A, H, unit=1.0))
+    mk = lambda *shape, unit: (torch.randn(shape, generator=g) * unit).bfloat16()  # noqa: E731
+    return mk(E, I, H, unit=0.05), mk(E, H, I, unit=0.05), mk(E, I, H, unit=0.05), mk(A, H, unit=1.0), mk(A, H, unit=1.0)
+
+
+def _within(name, got, value, err, deviation):
+    got = got.detach().double().cpu()
+    far = (got - value).abs()
+    outside = int((far > err).sum())
+    assert outside == 0, f"{name}: {outside} of {far.numel()} values are outside, the worst by {(far - err).max().item():.3g}"
+    assert far.norm() <= deviation.norm(), f"{name}: off by {(far.norm() / value.norm()).item():.3g}, at most {(deviation.norm() / value.norm()).item():.3g}"
+
+
+SHAPES = [
+    (2, 256, 128, [5, 0], 0, "one row tile, an empty expert"),
+    (3, 128, 256, [1, 257, 0], 3, "a row, a row more than a tile, none; rows of nobody"),
+    (4, 130, 70, [17, 33, 1, 16], 0, "odd widths below a block"),
+    (2, 1000, 360, [40, 61], 37, "widths that are no multiple of a block"),
+    (1, 8, 8, [3], 0, "tiny"),
+    (3, 384, 512, [255, 256, 129], 1, "around a tile's rows"),
+    (2, 257, 300, [30, 12], 0, "odd widths of two and three blocks"),
+    (70, 128, 128, [i % 4 for i in range(70)], 0, "more experts than lanes"),
+]
+
+
+@pytest.mark.parametrize("integers", [True, False])
+@pytest.mark.parametrize("E,H,I,counts,spare,what", SHAPES)
+def test_forward_and_backward_are_within_their_bounds(dev, E, H, I, counts, spare, what, integers):
+    print(f"[case] fp8 experts {what} integers={integers}", flush=True)
+    w1, w2, w3, x, d_y = _inputs(E, H, I, counts, spare, E + H, integers)
+    want = B.experts_between(w1, w2, w3, x, counts, d_y)
+    leaves = [t.to(dev).requires_grad_(True) for t in (w1, w2, w3, x)]
+    n = torch.tensor(counts, dtype=torch.int32, device=dev)
+    y = F_.bmm_experts_fp8(F_.quantize_experts(*leaves[:3]), leaves[3], n)
+    with torch.no_grad():
+        plain = F_.bmm_experts_fp8(F_.quantize_experts(*leaves[:3], for_backward=False), leaves[3], n.long())
+    assert torch.equal(plain, y)
+    y.backward(d_y.to(dev))
+    _within("y", y, *want["y"])
+    for name, leaf in zip(("d_w1", "d_w2", "d_w3", "d_x"), leaves):
+        _within(name, leaf.grad, *want[name])
+
+
+@pytest.mark.parametrize("A,E,H,I", [(8, 8, 2048, 768), (1, 1, 2048, 768), (24, 16, 1024, 512), (3, 2, 200, 130)])
+def test_few_rows(dev, A, E, H, I):
+    print(f"[case] fp8 experts, few rows {A} {E} {H} {I}", flush=True)
+    g = torch.Generator().manual_seed(A)
+    counts = torch.bincount(torch.randint(0, E, (A,), generator=g), minlength=E).tolist()
+    w1, w2, w3, x, _ = _inputs(E, H, I, counts, 0, A, False)
+    want = B.experts_between(w1, w2, w3, x, counts)
+    with torch.no_grad():
+        y = F_.bmm_experts_fp8(F_.quantize_experts(*(w.to(dev) for w in (w1, w2, w3)), for_backward=False), x.to(dev),
+                               torch.tensor(counts, device=dev))
+    _within("y", y, *want["y"])
+
+
+def test_a_row_that_is_not_finite_stays_a_row(dev):
+    print("[case] fp8 experts, NaN and infinity", flush=True)
+    counts = [4, 5]
+    w1, w2, w3, x, _ = _inputs(2, 256, 128, counts, 0, 5, False)
+    bad = x.clone()
+    bad[1, 7], bad[6, 200] = math.inf, math.nan
+    experts = F_.quantize_experts(*(w.to(dev) for w in (w1, w2, w3)))
+    n = torch.tensor(counts, device=dev)
+    y, z = F_.bmm_experts_fp8(experts, x.to(dev), n), F_.bmm_experts_fp8(experts, bad.to(dev), n)
+    whole = torch.ones(9, dtype=torch.bool)
+    whole[[1, 6]] = False
+    assert torch.equal(y[whole], z[whole]) and torch.isnan(z[~whole]).all()
+
+
+# ------------------------------------------------------------------------------ the operator
+def _setup(dev, seed=0, counts=(20, 0, 44), H=256, I=128):
+    w1, w2, w3, x, d_y = _inputs(len(counts), H, I, counts, 0, seed, False)
+    w = [t.to(dev).requires_grad_(True) for t in (w1, w2, w3)]
+    return w, x.to(dev).requires_grad_(True), d_y.to(dev), torch.tensor(counts, dtype=torch.int32, device=dev)
+
+
+def _pass(w, x, d_y, n):
+    y = F_.bmm_experts_fp8(F_.quantize_experts(*w), x, n)
+    return (y.detach(), *torch.autograd.grad(y, (*w, x), d_y))
+
+
+def _equal(a, b):
+    return all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_strides_streams_and_which_gradients(dev):
+    print("[case] fp8 experts: strides, a stream, partial gradients", flush=True)
+    w, x, d_y, n = _setup(dev)
+    want = _pass(w, x, d_y, n)
+    xt = x.detach().t().contiguous().t().requires_grad_(True)
+    assert _equal(want, _pass(w, xt, d_y.t().contiguous().t(), n))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _pass(w, x, d_y, n)
+    torch.cuda.current_stream().wait_stream(side)
+    assert _equal(want, got)
+    experts = F_.quantize_experts(*w)
+    only_x = torch.autograd.grad(F_.bmm_experts_fp8(experts._replace(w1=None, w2=None, w3=None), x, n), x, d_y)[0]
+    assert torch.equal(only_x, want[4])
+    only_w = torch.autograd.grad(F_.bmm_experts_fp8(experts, x.detach(), n), w[1], d_y)[0]
+    assert torch.equal(only_w, want[2])
+    expanded = torch.autograd.grad(F_.bmm_experts_fp8(experts, x, n).sum(), x)[0]      # a gradient of stride zero
+    assert torch.equal(expanded, torch.autograd.grad(F_.bmm_experts_fp8(experts, x, n), x, torch.ones_like(d_y))[0])
+
+
+def test_empty_input(dev):
+    print("[case] fp8 experts: no rows", flush=True)
+    w, x, d_y, _ = _setup(dev)
+    n = torch.zeros(3, dtype=torch.int32, device=dev)
+    got = _pass(w, x.detach()[:0].requires_grad_(True), d_y[:0], n)
+    assert got[0].shape == (0, 256) and all((t == 0).all() for t in got[1:4]) and got[4].shape == (0, 256)
+    got = _pass(w, x, d_y, n)                              # rows, but nobody's
+    assert all((t == 0).all() for t in got)
+
+
+def test_accumulated_and_postponed_weight_gradients(dev):
+    print("[case] fp8 experts: accumulate, defer", flush=True)
+    w, x, d_y, n = _setup(dev)
+    want = _pass(w, x, d_y, n)
+    experts = F_.quantize_experts(*w)
+    with F_.defer_weight_grads() as q:
+        F_.bmm_experts_fp8(experts, x, n).backward(d_y)
+    assert torch.equal(x.grad, want[4]) and all(p.grad is None for p in w) and len(q) == 1
+    q.run()
+    assert _equal([p.grad for p in w], want[1:4])
+    kept = [p.grad for p in w]
+    with F_.accumulate_weight_grads():
+        F_.bmm_experts_fp8(experts, x, n).backward(d_y)
+    for p, k, g in zip(w, kept, want[1:4]):
+        assert p.grad is k
+        # the old gradient is bf16 and twice it is exact; the new one is added before it is rounded: half a step of bf16 of the sum
+        assert ((p.grad.double() - 2 * g.double()).abs() <= 2.0 ** -8 * 2 * g.double().abs() + 2.0 ** -8 * g.double().abs()).all()
+
+
+def test_captured_and_replayed(dev):
+    print("[case] fp8 experts in a graph", flush=True)
+    w, x, d_y, n = _setup(dev, counts=(30, 3, 31))
+    w = [p.detach() for p in w]
+    x = x.detach()
+    n = n.clone()
+
+    def forward():
+        with torch.no_grad():
+            return F_.bmm_experts_fp8(F_.quantize_experts(*w, for_backward=False), x, n)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        forward()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = forward()
+    for rep in range(4):
+        g = torch.Generator().manual_seed(rep)
+        x.copy_(torch.randn(x.shape, generator=g))
+        n.copy_(torch.tensor([(64, 0, 0), (1, 62, 1), (0, 0, 17), (20, 22, 22)][rep], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, forward()), f"replay {rep}"
+
+
+def test_modules_call_it(dev):
+    print("[case] fp8 experts in the modules", flush=True)
+    torch.manual_seed(0)
+    args = MoEArgs(num_experts=4, top_k=2, route_norm=True)
+    moe = AnnotatedMoE(args, 256, 128, dtype=torch.bfloat16, fused=False).to(dev)
+    moe.init_weights()
+    x = torch.randn(2, 33, 256, device=dev).bfloat16()
+    e8 = moe.experts.quantize()
+    out = moe(x, experts_fp8=e8)
+    out.float().square().sum().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in moe.parameters())
+    ref = moe(x)
+    # the two differ by the rounding of three operands to e4m3 (half a step 2^-4 each), averaged over sums of 128 terms and more
+    assert (out - ref).float().norm() <= 3 * 2.0 ** -4 * ref.float().norm()
+    experts = BmmExperts(256, 128, 2, dtype=torch.bfloat16).to(dev)
+    for p in experts.parameters():
+        torch.nn.init.normal_(p, std=0.05)
+    rows, n = torch.randn(9, 256, device=dev).bfloat16(), torch.tensor([4, 5], device=dev)
+    assert torch.equal(experts(rows, n, experts.quantize()), F_.bmm_experts_fp8(F_.quantize_experts(experts.w1, experts.w2, experts.w3), rows, n))
+
+
+def test_captured_by_dynamo_as_one_node(dev):
+    print("[case] fp8 experts under dynamo", flush=True)
+    w, x, d_y, n = _setup(dev)
+    experts = F_.quantize_experts(*w)
+    seen = []
+
+    def backend(gm, inputs):
+        seen.extend(str(node.target) for node in gm.graph.nodes if node.op == "call_function")
+        return gm.forward
+
+    def fn(x):
+        return F_.bmm_experts_fp8(experts, x * 1, n)
+
+    got = torch.compile(fn, backend=backend, fullgraph=True)(x)
+    assert any("bmm_experts_fp8" in s for s in seen)
+    assert torch.equal(got, fn(x))
+
+
+def test_refusals(dev):
+    w, x, d_y, n = _setup(dev)
+    e = F_.quantize_experts(*w)
+    with pytest.raises(TypeError, match="rows are bfloat16"):
+        F_.bmm_experts_fp8(e, x.float(), n)
+    with pytest.raises(ValueError, match="row count for every expert"):
+        F_.bmm_experts_fp8(e, x[:, :-1], n)
+    with pytest.raises(ValueError, match="row count for every expert"):
+        F_.bmm_experts_fp8(e, x, n[:2])
+    with pytest.raises(ValueError, match="transposed codes"):
+        F_.bmm_experts_fp8(F_.quantize_experts(*w, for_backward=False), x, n)
+    with pytest.raises(ValueError, match="expected a contiguous"):
+        F_.bmm_experts_fp8(e._replace(q2=e.q1), x, n)
+    with pytest.raises(ValueError, match="expected a contiguous"):
+        F_.bmm_experts_fp8(e._replace(s1=e.s1.view(torch.uint8)), x, n)
+    with pytest.raises(ValueError, match="counts must be int32 or int64"):
+        F_.bmm_experts_fp8(e, x, n.float())
+    with pytest.raises(TypeError, match="float32 and bfloat16"):
+        F_.quantize_experts(*(p.detach().half() for p in w))
+    with pytest.raises(ValueError, match="shapes disagree"):
+        F_.quantize_experts(w[0], w[0], w[2])
+    with pytest.raises(ValueError):
+        ops.quantize_rows_fp8(x, row_map_div=2)
+    wide = torch.zeros(1, 8, 8200, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match="shape not supported"):
+        with torch.no_grad():
+            F_.bmm_experts_fp8(F_.quantize_experts(wide, wide.view(1, 8200, 8), wide), torch.zeros(2, 8200, dtype=torch.bfloat16, device=dev),
+                               torch.tensor([2], device=dev))
