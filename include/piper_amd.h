@@ -434,7 +434,8 @@ PK_API int pk_sched_slot_index(int device, uint64_t stream_handle, uint64_t capt
  *   weights  q [E][N][K'], scales [E][N'/128][K'/128]; transposed codes q_t [E][K][N'] share the scales
  * Code buffers must be 16-byte aligned.  The products take bf16 tensors of any width up to
  * H = PK_FP8_MAX_HIDDEN, I = PK_FP8_MAX_INTER; an operand's codes must span less than 4 GiB
- * (PK_ERR_SHAPE).  Expert e owns rows [starts[e], starts[e+1]); other rows are neither read nor written. */
+ * (PK_ERR_SHAPE).  Which rows are whose comes from a plan (pk_fp8_plan); rows of no expert are neither
+ * read nor written. */
 #define PK_FP8_BLOCK 128
 #define PK_FP8_MAX_HIDDEN 8192
 #define PK_FP8_MAX_INTER 4096
@@ -447,16 +448,23 @@ PK_API int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map
 PK_API int pk_fp8_quantize_weights(const void* w, int dtype, uint8_t* q, uint8_t* q_t, uint8_t* scales, int64_t E,
                             int64_t N, int64_t K, pk_stream_t stream);
 
+/* The row ranges of a pass over A rows, for the four products below: expert e owns counts[e] rows (int32, or
+ * int64 with counts_is_i64) behind those of the experts before it.  plan: pk_fp8_plan_bytes(A, E) bytes, 16-byte
+ * aligned; its first E + 1 words are starts[] as the other entry points take them.  Counts that are negative
+ * count as zero, and rows past A are cut off.  A plan serves passes over the A and E that it was made for. */
+PK_API int64_t pk_fp8_plan_bytes(int64_t A, int64_t E);
+PK_API int pk_fp8_plan(const void* counts, int counts_is_i64, int64_t E, int64_t A, int32_t* plan, pk_stream_t stream);
+
 /* g = x . w1[e]^T, u = x . w3[e]^T (both bf16 [A, I], or both NULL where no backward follows), and
  * h = silu(g) * u of what g and u hold, in blocks.  Operand row r is x[r], or x[row_map[r] / row_map_div];
  * the rows that the map can name are the first ceil(A / row_map_div). */
 PK_API int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const int32_t* row_map, int64_t row_map_div,
-                   const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3, const int32_t* starts,
+                   const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3, const int32_t* plan,
                    void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E,
                    pk_stream_t stream);
 /* y[A, H] (bf16) = h . w2[e]^T */
 PK_API int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2,
-                const int32_t* starts, void* y, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
+                const int32_t* plan, void* y, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
 /* d_h = d_y . w2[e] (w2_t: the transposed codes) in fp32, and from it d_g = d_h * u * silu'(g) and
  * d_u = d_h * silu(g), both bf16 [A, I] (for pk_grouped_swiglu_wgrad) and in blocks (for pk_fp8_dgrad_dx), and
  * h = silu(g) * u (bf16).  With scores (f32, of every routed slot) and row_map, as
@@ -465,13 +473,13 @@ PK_API int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t*
  * <d_out . w2, silu(g) * u> that pk_region_router_bwd adds up. */
 PK_API int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div,
                     const float* scores, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
-                    const int32_t* starts, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales,
+                    const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales,
                     uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H, int64_t I, int64_t E,
                     pk_stream_t stream);
 /* d_x[A, H] (bf16) = d_g . w1[e] + d_u . w3[e] (w1_t, w3_t: the transposed codes) */
 PK_API int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales,
                     const uint8_t* w1_t, const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3,
-                    const int32_t* starts, void* d_x, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
+                    const int32_t* plan, void* d_x, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
 
 /* ------------------------------------------------------------- ZeRO bucket path */
 

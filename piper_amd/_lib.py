@@ -107,6 +107,8 @@ SIGNATURES = {
     # rows: x dtype row_map div q scales rows K stream; weights: w dtype q q_t scales E N K stream
     "pk_fp8_quantize_rows": (_c_int, [_p, _c_int, _p, _c_i64, _p, _p, _c_i64, _c_i64, _p]),
     "pk_fp8_quantize_weights": (_c_int, [_p, _c_int, _p, _p, _p, _c_i64, _c_i64, _c_i64, _p]),
+    "pk_fp8_plan_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "pk_fp8_plan": (_c_int, [_p, _c_int, _c_i64, _c_i64, _p, _p]),
     # ... A H I E stream
     "pk_fp8_gate_up": (_c_int, [_p, _p, _p, _c_i64, *[_p] * 9, *[_c_i64] * 4, _p]),
     "pk_fp8_down": (_c_int, [*[_p] * 6, *[_c_i64] * 4, _p]),

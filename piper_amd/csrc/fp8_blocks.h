@@ -34,14 +34,6 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
 #undef PK_STEP
   return v;
 }
-// and their sum, added in the same order everywhere
-__device__ __forceinline__ float row_sum(float v) {
-#define PK_STEP(CTRL) v += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
-  PK_STEP(0x128) PK_STEP(0x124) PK_STEP(0x4e) PK_STEP(0xb1)
-#undef PK_STEP
-  return v;
-}
-
 // Four e4m3 codes of values of at most 448, rounded to nearest even (half a step, 2^-4 of the value: the products of a block
 // average such errors, and nothing here is summed up over steps).
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
@@ -49,8 +41,31 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
 }
 
-// Eight neighbouring values of a lane and those of the 15 lanes beside it are one block of 128: its codes and its byte.  A block
-// with an infinity or a NaN is NaN throughout, so that its rows' products are.
+// What a block of largest magnitude `bits` is divided by.  A block with an infinity or a NaN is NaN throughout, so that its rows'
+// products are.
+struct BlockScale {
+  uint32_t byte;
+  float inverse;
+  bool finite;
+};
+__device__ __forceinline__ BlockScale block_scale(uint32_t bits) {
+  BlockScale s;
+  s.finite = bits < INF_BITS;
+  s.byte = s.finite ? scale_byte(bits, TOP_E4M3) : 127u;
+  s.inverse = inverse_scale_of(s.byte);
+  return s;
+}
+// 16 values of a block
+__device__ __forceinline__ u32x4_t codes16(const float (&f)[16], const BlockScale& s) {
+  u32x4_t v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] = s.finite ? e4m3x4(f[4 * i] * s.inverse, f[4 * i + 1] * s.inverse, f[4 * i + 2] * s.inverse, f[4 * i + 3] * s.inverse)
+                    : NAN_CODE * 0x01010101u;
+  return v;
+}
+
+// Eight neighbouring values of a lane and those of the 15 lanes beside it are one block of 128: its codes and its byte.
 __device__ __forceinline__ void quantize8(const float (&f)[8], uint32_t (&codes)[2], uint32_t& byte) {
   uint32_t m = 0u;
 #pragma unroll
@@ -58,16 +73,12 @@ __device__ __forceinline__ void quantize8(const float (&f)[8], uint32_t (&codes)
     const uint32_t b = __float_as_uint(f[i]) & 0x7fffffffu;
     m = b > m ? b : m;
   }
-  m = row_max(m);
-  if (m >= INF_BITS) {
-    byte = 127u;
-    codes[0] = codes[1] = NAN_CODE * 0x01010101u;
-    return;
-  }
-  byte = scale_byte(m, TOP_E4M3);
-  const float inv = inverse_scale_of(byte);
-  codes[0] = e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-  codes[1] = e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+  const BlockScale s = block_scale(row_max(m));
+  byte = s.byte;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    codes[i] = s.finite ? e4m3x4(f[4 * i] * s.inverse, f[4 * i + 1] * s.inverse, f[4 * i + 2] * s.inverse, f[4 * i + 3] * s.inverse)
+                        : NAN_CODE * 0x01010101u;
 }
 
 }  // namespace pk_fp8

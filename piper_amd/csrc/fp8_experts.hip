@@ -123,6 +123,70 @@ __global__ __launch_bounds__(THREADS) void quantize_weights_kernel(const T* __re
   }
 }
 
+// ------------------------------------------------------------------------------------------------ plan
+// Where every expert's rows are and which expert a tile of TILE_ROWS rows belongs to, once for all products of a pass: a workgroup of a product
+// then finds its tile with one read of the table, where a search through starts[] costs it three dependent ones, 2 us each while the
+// chip is busy (per workgroup, 512 rows an expert, 2048 x 768: 6.5 -> 3 us in front of a loop of 30).
+//   [E + 1] starts (cut off at A), tiles, padding to 8; then for every tile 8 words: expert, its first tile, its tiles, its first
+//   row and the row behind its last, padding.  Counts that do not fit into A rows, or are negative, cannot lead a kernel out of bounds.
+constexpr int TILE_ROWS = 128, PLAN_THREADS = 1024, ENTRY = 8;
+__host__ __device__ inline int64_t plan_head(int64_t E) { return (E + 2 + ENTRY - 1) / ENTRY * ENTRY; }
+__host__ __device__ inline int64_t plan_tiles(int64_t A, int64_t E) { return A / TILE_ROWS + (A < E ? A : E); }
+
+// sum over the threads before this one (exclusive), all of PLAN_THREADS; *total: over all of them
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* waves /* 16 */, int64_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t incl = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t o = __shfl_up(incl, off, PK_WAVE);
+    if (lane >= off) incl += o;
+  }
+  __syncthreads();
+  if (lane == 63) waves[wave] = incl;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+  for (int i = 0; i < PLAN_THREADS / 64; ++i) {
+    before += i < wave ? waves[i] : 0;
+    all += waves[i];
+  }
+  *total = all;
+  return before + incl - v;
+}
+__global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const void* counts, int is_i64, int E, int64_t A, int32_t* __restrict__ plan) {
+  __shared__ int64_t waves[16];
+  __shared__ int32_t first[PK_MAX_EXPERTS + 1], begin[PK_MAX_EXPERTS + 1];
+  const int e = threadIdx.x;
+  int64_t n = 0, total;
+  if (e < E) n = is_i64 ? reinterpret_cast<const int64_t*>(counts)[e] : reinterpret_cast<const int32_t*>(counts)[e];
+  n = n < 0 ? 0 : n > A ? A : n;
+  int64_t start = block_scan(n, waves, &total);
+  start = start > A ? A : start;
+  const int64_t end = start + n > A ? A : start + n;
+  const int64_t tiles = (end - start + TILE_ROWS - 1) / TILE_ROWS;
+  const int64_t f = block_scan(tiles, waves, &total);
+  if (e < E) {
+    plan[e] = begin[e] = (int32_t)start;
+    first[e] = (int32_t)f;
+    if (e == E - 1) {
+      plan[E] = begin[E] = (int32_t)end;
+      plan[E + 1] = first[E] = (int32_t)total;
+    }
+  }
+  __syncthreads();
+  int32_t* const table = plan + plan_head(E);
+  for (int t = threadIdx.x; t < (int)total; t += PLAN_THREADS) {
+    int lo = 0, hi = E;                      // first[lo] <= t < first[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= t) lo = mid; else hi = mid;
+    }
+    // (of experts without tiles, which share their first one with the next, the last one is found)
+    *reinterpret_cast<u32x4_t*>(table + t * ENTRY) = u32x4_t{(uint32_t)lo, (uint32_t)first[lo], (uint32_t)(first[lo + 1] - first[lo]), (uint32_t)begin[lo]};
+    table[t * ENTRY + 4] = begin[lo + 1];
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ products
 // C[rows_e, N] = sum_seg A_seg[rows_e, K] . B_seg[e][N, K]^T, one workgroup to a tile of BM rows and 256 columns (gate and up: 128
 // of each).
@@ -140,7 +204,8 @@ struct Product {
   const uint8_t* Bs[2];     // scale of block (n, k) of expert e: Bs[e * bs_e + n * bs_n + k * bs_k]
   int64_t ld, strideB, bs_e;
   int32_t bs_n, bs_k;
-  const int32_t* starts;
+  const int32_t* plan;
+  FastDiv by_n_tiles;
   int32_t E, kt, nseg, N, n_tiles;
   bool vec;                 // rows of the bf16 tensors are whole 16-byte pieces
   bf16_t* O0;               // C;  GATE_UP: g (optional);  BWD: d_g
@@ -153,6 +218,7 @@ struct Product {
   const float* scores;      // BWD_SCALED: of every routed slot
   float* ds_part;           //             [N / 128][total_rows]: the score gradient in parts
   int64_t total_rows;
+  int32_t units, head;      // most units that a plan for as many rows can have; words in front of its table
 };
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(lds_ptr_t)p; }
@@ -173,43 +239,78 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
   return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
 }
 
-constexpr int KT_BYTES = 128;                // a k-tile is one block: 128 bytes of every row
-__device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
+// A k-tile is KB bytes of every row: a block of 128, or half of one.  16-byte pieces of a row are XOR-ed with bits of the row, so that 16
+// neighbouring rows' pieces of one number cover the banks.
+template <int KB>
+__device__ __forceinline__ int swz(int r) { return KB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
 
 // 32 of the 64 reduction bytes of step `half` of a k-tile, for row row0 + lane % 32.  Both operands are dealt alike, and a
-// k-tile has one scale, so it does not matter which lane holds which of them.
+// step has one scale, so it does not matter which lane holds which of them.
+template <int KB>
 __device__ __forceinline__ intx8_t fragment(const char* tile, int row0, int half, int lane) {
   const int r = row0 + (lane & 31), c = 4 * half + 2 * (lane >> 5);
-  const char* const p = tile + r * KT_BYTES;
-  const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(p + ((c ^ swz(r)) << 4));
-  const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(p + (((c + 1) ^ swz(r)) << 4));
+  const char* const p = tile + r * KB;
+  const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(p + ((c ^ swz<KB>(r)) << 4));
+  const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(p + (((c + 1) ^ swz<KB>(r)) << 4));
   return intx8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
-// fp32 staging of a tile's rows in LDS, 16-byte units of a row XOR-ed with the row against bank conflicts
-template <int X>
-__device__ __forceinline__ void stage4(float* lds, int row, int col, const float* four) {
-  *reinterpret_cast<floatx4_t*>(lds + row * X + (((col >> 2) ^ (row & (X / 4 - 1))) << 2)) = floatx4_t{four[0], four[1], four[2], four[3]};
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// the value of the lane 32 further or back
+__device__ __forceinline__ uint32_t other_half(uint32_t v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return (threadIdx.x & 32) ? r[0] : r[1];
 }
-template <int X>
-__device__ __forceinline__ void staged8(const float* lds, int row, int col, float (&f)[8]) {
+// From fours of 32 columns, dealt to the lower and upper lanes in turn, 16 neighbouring ones to each.
+__device__ __forceinline__ void exchange_halves(const floatx16_t& x, float (&f)[16]) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const floatx4_t v = *reinterpret_cast<const floatx4_t*>(lds + row * X + ((((col >> 2) + h) ^ (row & (X / 4 - 1))) << 2));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[4 * h + i] = v[i];
+  for (int v = 0; v < 8; ++v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[v]), __float_as_uint(x[v + 8]), false, false);
+    const int to = (v & 3) + (v & 4) * 2;
+    f[to] = __uint_as_float(r[0]);
+    f[to + 4] = __uint_as_float(r[1]);
   }
 }
-__device__ __forceinline__ void store8(bf16_t* p, int have, bool vec, const float (&f)[8]) {
-  if (vec && have >= 8) {
-    bf16x8_t v;
+__device__ __forceinline__ bf16x8_t pack8(const float (&f)[8]) {
+  bf16x8_t v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (bf16_t)f[i];
-    *reinterpret_cast<bf16x8_t*>(p) = v;
+  for (int i = 0; i < 8; ++i) v[i] = (bf16_t)f[i];
+  return v;
+}
+// In this form: the compiler would keep the eight floats of a value that is unpacked again, twice the registers.
+__device__ __forceinline__ bf16x8_t kept(bf16x8_t v) {
+  u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+  asm volatile("" : "+v"(w));
+  return __builtin_bit_cast(bf16x8_t, w);
+}
+// Eight neighbouring bf16 of a row, of which the first `have` are there (any number); vec: rows are whole 16-byte pieces
+__device__ __forceinline__ void store8(bf16_t* p, int have, bool vec, bf16x8_t v) {
+  if (vec) {
+    if (have > 0) *reinterpret_cast<bf16x8_t*>(p) = v;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < have) p[i] = (bf16_t)f[i];
+      if (i < have) p[i] = v[i];
+  }
+}
+__device__ __forceinline__ void store16(bf16_t* p, int have, bool vec, const float (&f)[16]) {
+  float a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { a[i] = f[i]; b[i] = f[8 + i]; }
+  store8(p, have, vec, pack8(a));
+  store8(p + 8, have - 8, vec, pack8(b));
+}
+__device__ __forceinline__ void load16(const bf16_t* p, int have, bool vec, bf16x8_t (&v)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    v[h] = bf16x8_t{};
+    if (vec) {
+      if (have > 8 * h) v[h] = *reinterpret_cast<const bf16x8_t*>(p + 8 * h);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (8 * h + i < have) v[h][i] = p[8 * h + i];
+    }
   }
 }
 __device__ __forceinline__ float held(float v) { return (float)(bf16_t)v; }
@@ -221,71 +322,93 @@ __device__ __forceinline__ int unit_of_block(int b) {      // neighbouring units
   return ((q / unit_chunk) * pk_rules::NXCD + x) * unit_chunk + (q % unit_chunk);
 }
 
-// WM x 2 waves of 64 x 128 outputs.
-template <int WM, int NS, int EPI>
-__global__ __launch_bounds__(128 * WM) void product_kernel(const Product p) {
+// WM x 2 waves of 64 x 128 outputs; NS k-tiles of KB bytes a row in the ring.
+template <int WM, int KB, int NS, int EPI, bool VEC>
+__global__ __launch_bounds__(128 * WM, 2) void product_kernel(const Product p) {
   constexpr int NT = 128 * WM, BM = 64 * WM, BN = 256, TM = 2, TN = 4;
-  constexpr int LA = BM * 8 / NT, LB = BN * 8 / NT, L = LA + LB;
-  constexpr int A_BYTES = BM * KT_BYTES, STAGE = A_BYTES + BN * KT_BYTES;
+  constexpr int PIECES = KB / 16, LA = BM * PIECES / NT, LB = BN * PIECES / NT, L = LA + LB;
+  constexpr int A_BYTES = BM * KB, STAGE = A_BYTES + BN * KB;
+  constexpr int PER_BLOCK = BLOCK / KB;      // k-tiles of a block
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
-  const pk_units::UnitIndex ui = pk_units::build_unit_index<BM>(p.starts, p.E, p.n_tiles);
+  static_assert(BM == TILE_ROWS, "the plan's tiles");
+  // units of an expert are laid out [column tile][row tile]: neighbours share the weights
   const int unit = unit_of_block(blockIdx.x);
-  if (unit >= ui.total) return;
-  int e, mt, nt;
-  pk_units::locate_unit<BM>(ui, pk_units::as_const(p.starts), p.E, p.n_tiles, unit, e, mt, nt);
-  const int row0 = p.starts[e] + mt * BM, rows = min(BM, p.starts[e + 1] - row0);
-  const int nkt = p.kt * p.nseg;
+  if (unit >= p.units) return;
+  const pk_units::const_i32_ptr plan = pk_units::as_const(p.plan);
+  const pk_units::const_i32_ptr entry = plan + p.head + pk_units::fastdiv(unit, p.by_n_tiles) * ENTRY;
+  const int total = plan[p.E + 1], e = entry[0], first = entry[1], tiles = entry[2], begin = entry[3], end = entry[4];
+  if (unit >= total * p.n_tiles) return;
+  const int local = unit - first * p.n_tiles, nt = local / tiles, mt = local - nt * tiles;
+  const int row0 = begin + mt * BM, rows = min(BM, end - row0);
+  const int nblk = p.kt * p.nseg, nkt = nblk * PER_BLOCK;
   const int n0 = nt * (EPI == GATE_UP ? BLOCK : BN);
-
-  // scales of the tile's rows and columns, behind the ring: a row of them is nkt bytes
-  char* const sa = smem + NS * STAGE;
-  const int sld = (nkt + 7) / 8 * 8 + 4;
-  char* const sb = sa + BM * sld;
-  for (int i = tid; i < BM * nkt; i += NT) {
-    const int r = i / nkt, k = i - r * nkt, seg = k >= p.kt;
-    int64_t src = row0 + (r < rows ? r : 0);
-    if (p.row_map) src = pk_units::fastdiv(p.row_map[src], p.map_div);
-    sa[r * sld + k] = (char)p.As[seg][src * p.kt + (seg ? k - p.kt : k)];
-  }
-  const int n_blocks = (p.N + BLOCK - 1) / BLOCK;
-  for (int i = tid; i < 2 * nkt; i += NT) {
-    const int b = i >= nkt, k = b ? i - nkt : i, seg = k >= p.kt;
-    const int nb = EPI == GATE_UP ? nt : min(2 * nt + b, n_blocks - 1);
-    sb[i] = (char)p.Bs[EPI == GATE_UP ? b : seg][e * p.bs_e + (int64_t)nb * p.bs_n + (int64_t)(seg ? k - p.kt : k) * p.bs_k];
-  }
 
   // Byte offsets of the 16-byte pieces that the thread brings; rows past the expert's end and columns past N read the tile's first
   // ones instead, and what comes of them is stored nowhere.
   uint32_t a_off[LA], b_off[LB];
 #pragma unroll
   for (int i = 0; i < LA; ++i) {
-    const int s = tid + i * NT, r = s >> 3, c = (s & 7) ^ swz(r);
+    const int s = tid + i * NT, r = s / PIECES, c = (s % PIECES) ^ swz<KB>(r);
     int64_t src = row0 + (r < rows ? r : 0);
     if (p.row_map) src = pk_units::fastdiv(p.row_map[src], p.map_div);
     a_off[i] = (uint32_t)(src * p.ld + c * 16);
   }
 #pragma unroll
   for (int i = 0; i < LB; ++i) {
-    const int s = tid + i * NT, r = s >> 3, c = (s & 7) ^ swz(r);
-    const int n = n0 + (EPI == GATE_UP ? r & (BLOCK - 1) : r);
+    const int s = tid + i * NT, r = s / PIECES, c = (s % PIECES) ^ swz<KB>(r);
+    // GATE_UP: a wave has 64 columns of both: rows [64 gate | 64 up] for each of the two
+    const int n = n0 + (EPI == GATE_UP ? (r >> 7) * 64 + (r & 63) : r);
     b_off[i] = (uint32_t)((int64_t)(n < p.N ? n : n0) * p.ld + c * 16);
   }
   const uint32_t ring = lds_addr(smem) + wave * 1024;
   const auto fetch = [&](int kt, int stage) {
-    const int seg = kt >= p.kt, k = (seg ? kt - p.kt : kt) * KT_BYTES;
+    const int seg = kt >= p.kt * PER_BLOCK, k = (seg ? kt - p.kt * PER_BLOCK : kt) * KB;
     const uint8_t* const a = uniform(p.A[seg] + k);
     const uint32_t at = ring + stage * STAGE;
 #pragma unroll
     for (int i = 0; i < LA; ++i) dma16(a_off[i], a, at + i * NT * 16);
 #pragma unroll
     for (int i = 0; i < LB; ++i) {
-      // GATE_UP: the first half of the tile's rows are gate weights, the second half up weights
-      const int which = EPI == GATE_UP ? (i >= LB / 2) : seg;
+      static_assert(64 * PIECES % NT == 0 || EPI != GATE_UP, "the 64 rows of one matrix are whole passes of the workgroup");
+      const int which = EPI == GATE_UP ? i * NT / (64 * PIECES) & 1 : seg;
       dma16(b_off[i], uniform(p.B[which] + e * p.strideB + k), at + A_BYTES + i * NT * 16);
     }
   };
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s)
+    if (s < nkt) fetch(s, s);
+
+  // scales of the tile's rows and columns, behind the ring: a row of them is nblk bytes
+  char* const sa = smem + NS * STAGE;
+  const int sld = (nblk + 7) / 8 * 8 + 4;
+  char* const sb = sa + BM * sld;
+  const int n_blocks = (p.N + BLOCK - 1) / BLOCK;
+  {
+    const int r = tid >> 1, part = tid & 1;  // two threads to a row
+    int64_t src = row0 + (r < rows ? r : 0);
+    if (p.row_map) src = pk_units::fastdiv(p.row_map[src], p.map_div);
+    char* const to = sa + r * sld;
+    for (int seg = 0; seg < p.nseg; ++seg) {
+      const uint8_t* const from = p.As[seg] + src * p.kt;
+      if (p.kt % 16 == 0 && ((uintptr_t)p.As[seg] & 7) == 0) {      // rows are whole 16-byte pieces, 8 bytes for each of the two
+        for (int k = part * 8; k < p.kt; k += 16) {
+          const u32x2_t v = *reinterpret_cast<const u32x2_t*>(from + k);
+          *reinterpret_cast<uint32_t*>(to + seg * p.kt + k) = v[0];
+          *reinterpret_cast<uint32_t*>(to + seg * p.kt + k + 4) = v[1];
+        }
+      } else {
+#pragma unroll 4
+        for (int k = part; k < p.kt; k += 2) to[seg * p.kt + k] = (char)from[k];
+      }
+    }
+    for (int i = tid; i < 2 * nblk; i += NT) {
+      const int b = i >= nblk, k = b ? i - nblk : i, seg = k >= p.kt;
+      const int nb = EPI == GATE_UP ? nt : min(2 * nt + b, n_blocks - 1);
+      sb[i] = (char)p.Bs[EPI == GATE_UP ? b : seg][e * p.bs_e + (int64_t)nb * p.bs_n + (int64_t)(seg ? k - p.kt : k) * p.bs_k];
+    }
+  }
 
   floatx16_t acc[TM][TN];
 #pragma unroll
@@ -294,149 +417,206 @@ __global__ __launch_bounds__(128 * WM) void product_kernel(const Product p) {
     for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
-  __syncthreads();                           // the scales are there; every ordinary load has been waited for
-#pragma unroll
-  for (int s = 0; s < NS - 1; ++s)
-    if (s < nkt) fetch(s, s);
+  __syncthreads();                           // the scales are there
+  const bool wave_has_rows = wm * 64 < rows;
   int stage = 0;
   for (int kt = 0; kt < nkt; ++kt) {
     // all but the youngest NS - 2 k-tiles have landed, everywhere; the stage that the next one goes to has been read
-    if (NS > 2 && kt + 1 < nkt) dma_wait<(NS - 2) * L>();
+    if (NS > 2 && kt + NS - 2 < nkt) dma_wait<(NS - 2) * L>();
     else dma_wait<0>();
     block_barrier();
     const int next = stage == 0 ? NS - 1 : stage - 1;
     if (kt + NS - 1 < nkt) fetch(kt + NS - 1, next);
-    const char* const at = smem + stage * STAGE;
-    const int scale_b = (unsigned char)sb[wn * nkt + kt];
-    int scale_a[TM];
+    if (wave_has_rows) {
+      const char* const at = smem + stage * STAGE;
+      const int scale_b = (unsigned char)sb[(EPI == GATE_UP ? 0 : wn * nblk) + kt / PER_BLOCK];
+      const int scale_u = EPI == GATE_UP ? (unsigned char)sb[nblk + kt / PER_BLOCK] : scale_b;
+      int scale_a[TM];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) scale_a[i] = (unsigned char)sa[(wm * 64 + i * 32 + (lane & 31)) * sld + kt];
+      for (int i = 0; i < TM; ++i) scale_a[i] = (unsigned char)sa[(wm * 64 + i * 32 + (lane & 31)) * sld + kt / PER_BLOCK];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      intx8_t a[TM], b[TN];
+      for (int half = 0; half < KB / 64; ++half) {
+        intx8_t a[TM], b[TN];
 #pragma unroll
-      for (int i = 0; i < TM; ++i) a[i] = fragment(at, wm * 64 + i * 32, half, lane);
+        for (int i = 0; i < TM; ++i) a[i] = fragment<KB>(at, wm * 64 + i * 32, half, lane);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) b[j] = fragment(at + A_BYTES, wn * 128 + j * 32, half, lane);
-      // operands swapped: a lane then holds 4 neighbouring columns of one row,
-      //   acc[v] = C[row = lane % 32][col = 8 * (v / 4) + 4 * (lane / 32) + v % 4]
+        for (int j = 0; j < TN; ++j) b[j] = fragment<KB>(at + A_BYTES, wn * 128 + j * 32, half, lane);
+        // operands swapped: a lane then holds 4 neighbouring columns of one row,
+        //   acc[v] = C[row = lane % 32][col = 8 * (v / 4) + 4 * (lane / 32) + v % 4]
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][j], 0, 0, 0, scale_b, 0, scale_a[i]);
+          for (int j = 0; j < TN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][j], 0, 0, 0, j < TN / 2 ? scale_b : scale_u, 0,
+                                                                        scale_a[i]);
+      }
     }
     stage = stage == NS - 1 ? 0 : stage + 1;
   }
 
-  // 32 rows of every wave at a time through the LDS; then 16 lanes have 128 columns, a block, of a row
-  constexpr int CHUNK = 32 * WM;
-  static_assert(CHUNK * BN * 4 <= NS * STAGE, "the staged rows reuse the ring");
-  float* const lds = reinterpret_cast<float*>(smem);
+  // A lane and the one 32 further have the 32 columns of a row of acc[i][j], in fours; after exchanging halves of them each has 16
+  // neighbouring ones, so that loads and stores are 16 bytes wide without a way through the LDS, and the wave's 128
+  // columns of a row, a block, are in these two lanes.
+  if (!wave_has_rows && EPI != GATE_UP) return;
+  const int half16 = (lane >> 5) * 16;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    __syncthreads();                         // the LDS has been read for the last time
+    asm volatile("" ::: "memory");           // the second half's loads and addresses not before the first half has left its registers
+    __builtin_amdgcn_sched_barrier(0);
+    const int r = wm * 64 + 32 * i + (lane & 31);
+    const bool live = r < rows;              // the same in both lanes of a row
+    float f[TN][16];                         // (scalars: a vector keeps its 16 registers until its last element has been used)
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < TN; ++j) exchange_halves(acc[i][j], f[j]);
+    const int64_t row = row0 + (live ? r : 0);
+    if constexpr (EPI == PLAIN) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        stage4<BN>(lds, 32 * wm + (lane & 31), wn * 128 + 32 * j + 8 * q + 4 * (lane >> 5), reinterpret_cast<const float*>(&acc[i][j]) + 4 * q);
-    __syncthreads();
-    constexpr int PIECES = (EPI == GATE_UP ? BLOCK : BN) / 8;
-    for (int s = tid; s < CHUNK * PIECES; s += NT) {
-      const int lr = s / PIECES, c = (s % PIECES) * 8, n = n0 + c;
-      const int r = (lr >> 5) * 64 + 32 * i + (lr & 31);
-      const bool live = r < rows;            // the same for the 16 lanes of a block
-      const int have = live ? p.N - n : 0;
-      const int64_t o = (int64_t)(row0 + r) * p.N + n;
-      const int64_t unit_out = (int64_t)(row0 + r) * n_blocks + n / BLOCK;
-      float a[8];
-      staged8<BN>(lds, lr, c, a);
-      if constexpr (EPI == PLAIN) {
-        store8(p.O0 + o, have, p.vec, a);
-      } else if constexpr (EPI == GATE_UP) {
-        float u[8], h[8];
-        staged8<BN>(lds, lr, c + BLOCK, u);
+      for (int j = 0; j < TN; ++j) {
+        const int n = n0 + wn * 128 + 32 * j + half16;
+        if (live) store16(p.O0 + row * p.N + n, p.N - n, VEC, f[j]);
+      }
+    } else if constexpr (EPI == GATE_UP) {
+      // 64 columns of h here, 64 in the other wave of these rows
+      float h[2][16];
+      uint32_t m = 0u;
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          a[t] = held(a[t]);                 // g and u are bf16 tensors, written or not
-          u[t] = held(u[t]);
-          h[t] = t < have ? a[t] * sigmoid(a[t]) * u[t] : 0.f;
+      for (int j = 0; j < 2; ++j) {
+        const int n = n0 + wn * 64 + 32 * j + half16;
+        int have = p.N - n;
+        asm volatile("" : "+v"(have));       // compared here and not kept: such masks are more than there are scalar registers
+        float g[16], u[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          g[v] = held(f[j][v]);     // g and u are bf16 tensors, written or not
+          u[v] = held(f[j + 2][v]);
+          h[j][v] = (VEC ? have > v / 8 * 8 : have > v) ? g[v] * sigmoid(g[v]) * u[v] : 0.f;
+          m = umax(m, __float_as_uint(h[j][v]) & 0x7fffffffu);
         }
-        uint32_t codes[2], byte;
-        pk_fp8::quantize8(h, codes, byte);
-        if (live) {
-          if (p.O0) store8(p.O0 + o, have, p.vec, a);
-          if (p.O1) store8(p.O1 + o, have, p.vec, u);
-          *reinterpret_cast<u32x2_t*>(p.Q[0] + unit_out * BLOCK + (n & (BLOCK - 1))) = u32x2_t{codes[0], codes[1]};
-          if ((tid & 15) == 0) p.Qs[0][unit_out] = (uint8_t)byte;
+        if (live && p.O0) {
+          store16(p.O0 + row * p.N + n, p.N - n, VEC, g);
+          store16(p.O1 + row * p.N + n, p.N - n, VEC, u);
         }
-      } else {
-        float g[8], u[8], h[8], ds = 0.f;
-        load8<bf16_t>(p.G + o, have, p.vec, g);
-        load8<bf16_t>(p.U + o, have, p.vec, u);
-        const float sc = EPI == BWD_SCALED && live ? p.scores[p.row_map[row0 + r]] : 1.f;
+      }
+      m = umax(m, other_half(m));
+      uint32_t* const amax = reinterpret_cast<uint32_t*>(smem);      // [TM][2][BM / TM]
+      if (i == 0) __syncthreads();           // the ring has been read
+      amax[(i * 2 + wn) * 32 * WM + wm * 32 + (lane & 31)] = m;
+      __syncthreads();
+      m = umax(m, amax[(i * 2 + (wn ^ 1)) * 32 * WM + wm * 32 + (lane & 31)]);
+      const pk_fp8::BlockScale sc = pk_fp8::block_scale(m);
+      if (live) {
+        const int64_t block = row * n_blocks + nt;
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          const float sg = sigmoid(g[t]), silu = g[t] * sg, hv = silu * u[t];
-          if (EPI == BWD_SCALED) ds += t < have ? a[t] * hv : 0.f;
-          const float d = sc * a[t];
-          h[t] = sc * hv;
-          const float dg = d * u[t] * (sg * (1.f + g[t] * (1.f - sg))), du = d * silu;
-          g[t] = t < have ? held(dg) : 0.f;  // bf16 tensors, whose blocks are of what they hold
-          u[t] = t < have ? held(du) : 0.f;
-        }
-        uint32_t cg[2], cu[2], bg, bu;
-        pk_fp8::quantize8(g, cg, bg);
-        pk_fp8::quantize8(u, cu, bu);
-        if (EPI == BWD_SCALED) ds = pk_fp8::row_sum(ds);
-        if (live) {
-          store8(p.O0 + o, have, p.vec, g);
-          store8(p.O1 + o, have, p.vec, u);
-          store8(p.O2 + o, have, p.vec, h);
-          if (n / BLOCK < n_blocks) {
-            const int64_t at = unit_out * BLOCK + (n & (BLOCK - 1));
-            *reinterpret_cast<u32x2_t*>(p.Q[0] + at) = u32x2_t{cg[0], cg[1]};
-            *reinterpret_cast<u32x2_t*>(p.Q[1] + at) = u32x2_t{cu[0], cu[1]};
-            if ((tid & 15) == 0) {
-              p.Qs[0][unit_out] = (uint8_t)bg;
-              p.Qs[1][unit_out] = (uint8_t)bu;
-              if (EPI == BWD_SCALED) p.ds_part[(int64_t)(n / BLOCK) * p.total_rows + row0 + r] = ds;
-            }
+        for (int j = 0; j < 2; ++j) *reinterpret_cast<u32x4_t*>(p.Q[0] + block * BLOCK + wn * 64 + 32 * j + half16) = pk_fp8::codes16(h[j], sc);
+        if (wn == 0 && lane < 32) p.Qs[0][block] = (uint8_t)sc.byte;
+      }
+    } else {
+      const int nb = 2 * nt + wn;            // the wave's block of columns
+      if (nb >= n_blocks) return;            // (the same for the whole wave)
+      // g and u of 32 columns are requested while the 32 before them are worked on; what becomes of them takes the place of
+      // the accumulators
+      bf16x8_t gs[2][2], us[2][2], dgs[TN][2], dus[TN][2];
+      const bf16_t* const gp = p.G + row * p.N;
+      const bf16_t* const up = p.U + row * p.N;
+      const auto request = [&](int j) {
+        const int n = nb * BLOCK + 32 * j + half16;
+        load16(gp + n, p.N - n, VEC, gs[j & 1]);
+        load16(up + n, p.N - n, VEC, us[j & 1]);
+      };
+      request(0);
+      const float score = EPI == BWD_SCALED ? p.scores[p.row_map[row]] : 1.f;
+      float ds = 0.f;
+      uint32_t mg = 0u, mu = 0u;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        if (j + 1 < TN) request(j + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {        // eight columns at a time
+          const int n = nb * BLOCK + 32 * j + half16 + 8 * k;
+          int have = p.N - n;
+          asm volatile("" : "+v"(have));     // compared here and not kept: 64 such masks are more than there are scalar registers
+          float g[8], u[8], h[8];
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            const float gv = (float)gs[j & 1][k][v], uv = (float)us[j & 1][k][v], a = f[j][8 * k + v];
+            const float sg = sigmoid(gv), silu = gv * sg, hv = silu * uv, d = score * a;
+            const bool in = VEC ? have > 0 : have > v;
+            if (EPI == BWD_SCALED) ds += in ? a * hv : 0.f;
+            h[v] = score * hv;
+            const float dg = d * uv * (sg * (1.f + gv * (1.f - sg))), du = d * silu;
+            g[v] = in ? held(dg) : 0.f;      // bf16 tensors, whose blocks are of what they hold
+            u[v] = in ? held(du) : 0.f;
+            mg = umax(mg, __float_as_uint(g[v]) & 0x7fffffffu);
+            mu = umax(mu, __float_as_uint(u[v]) & 0x7fffffffu);
           }
+          asm volatile("" : "+v"(mg), "+v"(mu), "+v"(ds));      // step by step: as one reduction it would keep all values
+          dgs[j][k] = kept(pack8(g));
+          dus[j][k] = kept(pack8(u));
+          if (live) {
+            store8(p.O0 + row * p.N + n, have, VEC, dgs[j][k]);
+            store8(p.O1 + row * p.N + n, have, VEC, dus[j][k]);
+            store8(p.O2 + row * p.N + n, have, VEC, pack8(h));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      mg = umax(mg, other_half(mg));
+      mu = umax(mu, other_half(mu));
+      const pk_fp8::BlockScale scg = pk_fp8::block_scale(mg), scu = pk_fp8::block_scale(mu);
+      if (EPI == BWD_SCALED) ds += __uint_as_float(other_half(__float_as_uint(ds)));
+      if (live) {
+        const int64_t block = row * n_blocks + nb;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          float g[16], u[16];
+#pragma unroll
+          for (int v = 0; v < 16; ++v) { g[v] = (float)dgs[j][v >> 3][v & 7]; u[v] = (float)dus[j][v >> 3][v & 7]; }
+          *reinterpret_cast<u32x4_t*>(p.Q[0] + block * BLOCK + 32 * j + half16) = pk_fp8::codes16(g, scg);
+          *reinterpret_cast<u32x4_t*>(p.Q[1] + block * BLOCK + 32 * j + half16) = pk_fp8::codes16(u, scu);
+        }
+        if (lane < 32) {
+          p.Qs[0][block] = (uint8_t)scg.byte;
+          p.Qs[1][block] = (uint8_t)scu.byte;
+          if (EPI == BWD_SCALED) p.ds_part[(int64_t)nb * p.total_rows + row0 + r] = ds;
         }
       }
     }
   }
 }
 
-template <int WM, int NS, int EPI>
+template <int WM, int KB, int NS, int EPI>
 int launch_tiles(Product p, int64_t A, int kernel_id, hipStream_t s) {
-  constexpr int BM = 64 * WM, STAGE = (BM + 256) * KT_BYTES;
+  constexpr int BM = 64 * WM, STAGE = (BM + 256) * KB;
   p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP ? BLOCK : 256);
-  const int64_t units = (A / BM + (A < p.E ? A : p.E)) * p.n_tiles;
+  p.by_n_tiles = pk_units::make_fastdiv(p.n_tiles);
+  p.head = (int32_t)plan_head(p.E);
+  const int64_t units = plan_tiles(A, p.E) * p.n_tiles;
   if (units > 0x7fffff00ll) return PK_ERR_SHAPE;
-  if (units == 0) return PK_OK;
-  const int nkt = p.kt * p.nseg, sld = (nkt + 7) / 8 * 8 + 4;
-  const int lds = NS * STAGE + BM * sld + 2 * nkt;
-  static bool ready[PK_MAX_DEVICES] = {};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= PK_MAX_DEVICES) return PK_ERR_UNSUPPORTED;
-  if (!ready[dev]) {
-    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<WM, NS, EPI>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                               160 * 1024);
-    if (err != hipSuccess) return (int)err;
-    ready[dev] = true;
-  }
+  p.units = (int32_t)units;
+  const int nblk = p.kt * p.nseg, sld = (nblk + 7) / 8 * 8 + 4;
+  const int lds = NS * STAGE + BM * sld + 2 * nblk;
   const int64_t per = unit_chunk * pk_rules::NXCD;
-  PK_LAUNCH_NOCHECK(kernel_id, s, (product_kernel<WM, NS, EPI>), dim3((unsigned)(pk_ceil_div(units, per) * per)), dim3(128 * WM), lds, s, p);
-  PK_RETURN_IF_LAUNCH_FAILED();
-  return PK_OK;
+  const dim3 grid((unsigned)(pk_ceil_div(units, per) * per)), block(128 * WM);
+  const auto launch = [&](auto kernel, bool (&ready)[PK_MAX_DEVICES]) -> int {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= PK_MAX_DEVICES) return PK_ERR_UNSUPPORTED;
+    if (!ready[dev]) {                       // (more than one thread may do it)
+      const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+      if (err != hipSuccess) return (int)err;
+      ready[dev] = true;
+    }
+    PK_LAUNCH_NOCHECK(kernel_id, s, kernel, grid, block, lds, s, p);
+    PK_RETURN_IF_LAUNCH_FAILED();
+    return PK_OK;
+  };
+  static bool ready[2][PK_MAX_DEVICES] = {};
+  return p.vec ? launch(product_kernel<WM, KB, NS, EPI, true>, ready[1]) : launch(product_kernel<WM, KB, NS, EPI, false>, ready[0]);
 }
 
 template <int EPI>
 int launch_product(const Product& p, int64_t A, int kernel_id, hipStream_t s) {
-  return launch_tiles<4, 2, EPI>(p, A, kernel_id, s);
+  return launch_tiles<2, 64, 3, EPI>(p, A, kernel_id, s);
 }
 
 // Common checks of the products.  Offsets from an operand's first row are 32 bits wide.
@@ -505,19 +685,35 @@ int pk_fp8_quantize_weights(const void* w, int dtype, uint8_t* q, uint8_t* q_t, 
   return PK_OK;
 }
 
+int64_t pk_fp8_plan_bytes(int64_t A, int64_t E) {
+  if (A < 0 || E <= 0 || E > PK_MAX_EXPERTS || A > 0x7fffffffll) return PK_ERR_ARG;
+  return (plan_head(E) + plan_tiles(A, E) * ENTRY) * 4;
+}
+
+int pk_fp8_plan(const void* counts, int counts_is_i64, int64_t E, int64_t A, int32_t* plan, pk_stream_t stream) {
+  if (A < 0 || E <= 0) return PK_ERR_ARG;
+  if (E > PK_MAX_EXPERTS || A > 0x7fffffffll) return PK_ERR_SHAPE;
+  if (!counts || !plan) return PK_ERR_ARG;
+  if (!pk_aligned16(plan)) return PK_ERR_ALIGN;
+  PK_LAUNCH_NOCHECK(pk_timing::K_COUNTS_TO_STARTS, (hipStream_t)stream, plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, (hipStream_t)stream, counts,
+                    counts_is_i64, (int)E, A, plan);
+  PK_RETURN_IF_LAUNCH_FAILED();
+  return PK_OK;
+}
+
 int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const int32_t* row_map, int64_t row_map_div, const uint8_t* w1, const uint8_t* s1,
-                   const uint8_t* w3, const uint8_t* s3, const int32_t* starts, void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A,
+                   const uint8_t* w3, const uint8_t* s3, const int32_t* plan, void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A,
                    int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
   if (const int rc = check(A, H, I, E)) return rc;
   if (row_map_div < 1 || row_map_div > 0x7fffffffll) return PK_ERR_ARG;
   if (A == 0) return PK_OK;
-  if (!all_set({x, x_scales, w1, s1, w3, s3, starts, h, h_scales}) || !g != !u) return PK_ERR_ARG;
-  if (!all_aligned({x, w1, w3, h})) return PK_ERR_ALIGN;
+  if (!all_set({x, x_scales, w1, s1, w3, s3, plan, h, h_scales}) || !g != !u) return PK_ERR_ARG;
+  if (!all_aligned({x, w1, w3, h, plan})) return PK_ERR_ALIGN;
   Product p = {};
   p.A[0] = x; p.As[0] = x_scales; p.row_map = row_map; p.map_div = pk_units::make_fastdiv(row_map_div);
   p.A[1] = x; p.As[1] = x_scales;
   p.B[0] = w1; p.B[1] = w3; p.Bs[0] = s1; p.Bs[1] = s3;
-  p.kt = (int32_t)blocks_of(H); p.nseg = 1; p.N = (int32_t)I; p.E = (int32_t)E; p.starts = starts;
+  p.kt = (int32_t)blocks_of(H); p.nseg = 1; p.N = (int32_t)I; p.E = (int32_t)E; p.plan = plan;
   p.ld = blocks_of(H) * BLOCK; p.strideB = I * p.ld;
   p.bs_n = p.kt; p.bs_k = 1; p.bs_e = blocks_of(I) * p.kt;
   p.vec = bf16_pieces(I, {g, u});
@@ -525,16 +721,16 @@ int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const int32_t* row
   return launch_product<GATE_UP>(p, A, pk_timing::K_FP8_GATE_UP, (hipStream_t)stream);
 }
 
-int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2, const int32_t* starts, void* y, int64_t A,
+int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2, const int32_t* plan, void* y, int64_t A,
                 int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
   if (const int rc = check(A, H, I, E)) return rc;
   if (A == 0) return PK_OK;
-  if (!all_set({h, h_scales, w2, s2, starts, y})) return PK_ERR_ARG;
-  if (!all_aligned({h, w2})) return PK_ERR_ALIGN;
+  if (!all_set({h, h_scales, w2, s2, plan, y})) return PK_ERR_ARG;
+  if (!all_aligned({h, w2, plan})) return PK_ERR_ALIGN;
   Product p = {};
   p.A[0] = p.A[1] = h; p.As[0] = p.As[1] = h_scales;
   p.B[0] = p.B[1] = w2; p.Bs[0] = p.Bs[1] = s2;
-  p.kt = (int32_t)blocks_of(I); p.nseg = 1; p.N = (int32_t)H; p.E = (int32_t)E; p.starts = starts;
+  p.kt = (int32_t)blocks_of(I); p.nseg = 1; p.N = (int32_t)H; p.E = (int32_t)E; p.plan = plan;
   p.ld = blocks_of(I) * BLOCK; p.strideB = H * p.ld;
   p.bs_n = p.kt; p.bs_k = 1; p.bs_e = blocks_of(H) * p.kt;
   p.vec = bf16_pieces(H, {y});
@@ -543,19 +739,19 @@ int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, co
 }
 
 int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div, const float* scores,
-                    const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u, const int32_t* starts, void* d_g, void* d_u, void* h,
+                    const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u, const int32_t* plan, void* d_g, void* d_u, void* h,
                     uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H, int64_t I,
                     int64_t E, pk_stream_t stream) {
   if (const int rc = check(A, H, I, E)) return rc;
   if (row_map_div < 1 || row_map_div > 0x7fffffffll) return PK_ERR_ARG;
   if (A == 0) return PK_OK;
-  if (!all_set({d_y, d_y_scales, w2_t, s2, g, u, starts, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales})) return PK_ERR_ARG;
+  if (!all_set({d_y, d_y_scales, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales})) return PK_ERR_ARG;
   if (!scores != !ds_part || (scores && !row_map)) return PK_ERR_ARG;
-  if (!all_aligned({d_y, w2_t, d_g8, d_u8})) return PK_ERR_ALIGN;
+  if (!all_aligned({d_y, w2_t, d_g8, d_u8, plan})) return PK_ERR_ALIGN;
   Product p = {};
   p.A[0] = p.A[1] = d_y; p.As[0] = p.As[1] = d_y_scales; p.row_map = row_map; p.map_div = pk_units::make_fastdiv(row_map_div);
   p.B[0] = p.B[1] = w2_t; p.Bs[0] = p.Bs[1] = s2;
-  p.kt = (int32_t)blocks_of(H); p.nseg = 1; p.N = (int32_t)I; p.E = (int32_t)E; p.starts = starts;
+  p.kt = (int32_t)blocks_of(H); p.nseg = 1; p.N = (int32_t)I; p.E = (int32_t)E; p.plan = plan;
   p.ld = blocks_of(H) * BLOCK; p.strideB = I * p.ld;
   p.bs_n = 1; p.bs_k = (int32_t)blocks_of(I); p.bs_e = blocks_of(H) * blocks_of(I);
   p.vec = bf16_pieces(I, {g, u, d_g, d_u, h});
@@ -568,16 +764,16 @@ int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t
 }
 
 int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales, const uint8_t* w1_t,
-                    const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3, const int32_t* starts, void* d_x, int64_t A, int64_t H, int64_t I,
+                    const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3, const int32_t* plan, void* d_x, int64_t A, int64_t H, int64_t I,
                     int64_t E, pk_stream_t stream) {
   if (const int rc = check(A, H, I, E)) return rc;
   if (A == 0) return PK_OK;
-  if (!all_set({d_g8, d_g_scales, d_u8, d_u_scales, w1_t, s1, w3_t, s3, starts, d_x})) return PK_ERR_ARG;
-  if (!all_aligned({d_g8, d_u8, w1_t, w3_t})) return PK_ERR_ALIGN;
+  if (!all_set({d_g8, d_g_scales, d_u8, d_u_scales, w1_t, s1, w3_t, s3, plan, d_x})) return PK_ERR_ARG;
+  if (!all_aligned({d_g8, d_u8, w1_t, w3_t, plan})) return PK_ERR_ALIGN;
   Product p = {};
   p.A[0] = d_g8; p.As[0] = d_g_scales; p.A[1] = d_u8; p.As[1] = d_u_scales;
   p.B[0] = w1_t; p.Bs[0] = s1; p.B[1] = w3_t; p.Bs[1] = s3;
-  p.kt = (int32_t)blocks_of(I); p.nseg = 2; p.N = (int32_t)H; p.E = (int32_t)E; p.starts = starts;
+  p.kt = (int32_t)blocks_of(I); p.nseg = 2; p.N = (int32_t)H; p.E = (int32_t)E; p.plan = plan;
   p.ld = blocks_of(I) * BLOCK; p.strideB = H * p.ld;
   p.bs_n = 1; p.bs_k = (int32_t)blocks_of(H); p.bs_e = blocks_of(H) * blocks_of(I);
   p.vec = bf16_pieces(H, {d_x});

@@ -985,6 +985,9 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
   // buffers of a pass over A rows: x, d_y in blocks ([A, H']), h, d_g, d_u in blocks ([A, I'])
   static int64_t codes(int64_t A, int64_t width) { return A * whole_blocks(width) * PK_FP8_BLOCK; }
   static int64_t scales(int64_t A, int64_t width) { return A * whole_blocks(width); }
+  static void zero_tail(const Tensor& buf, const Tensor& plan, int64_t E) {
+    PK_CALL(pk_zero_rows_from, ptr(buf), PK_BF16, plan.data_ptr<int32_t>() + E, buf.size(0), buf.size(1), stream_of(buf));
+  }
   // y [A,H]; gu [2,A,I]: where the pre-activations are left
   static Tensor run(const Fp8Weights& w, const Tensor& x, const Tensor& starts, Tensor* gu) {
     const int64_t A = x.size(0), H = w.H, I = w.I;
@@ -1004,7 +1007,7 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     PK_CALL(pk_fp8_gate_up, p(x8), p(xs), nullptr, 1, u8(w.q[0]), u8(w.s[0]), u8(w.q[2]), u8(w.s[2]), at, g, g ? g + A * I * 2 : nullptr, p(h8),
             p(hs), A, H, I, w.E, st);
     PK_CALL(pk_fp8_down, p(h8), p(hs), u8(w.q[1]), u8(w.s[1]), at, ptr(y), A, H, I, w.E, st);
-    ExpertsFn::zero_tail(y, starts);
+    zero_tail(y, starts, w.E);
     return y;
   }
   static Tensor forward(AutogradContext* ctx, const OptTensor& w1, const OptTensor& w2, const OptTensor& w3, const Tensor& x, const Fp8Weights* w,
@@ -1044,7 +1047,7 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     if (nx) {
       d_x = at::empty({A, H}, x.options());
       PK_CALL(pk_fp8_dgrad_dx, p(g8), p(gs), p(u8_), p(us), u8(t1), u8(s1), u8(t3), u8(s3), at, ptr(d_x), A, H, I, E, st);
-      ExpertsFn::zero_tail(d_x, starts);
+      zero_tail(d_x, starts, E);
     }
     const auto wgrad = [d_y, dguh, x, starts, A, H, I, E, step](const Tensor& d1, const Tensor& d2, const Tensor& d3, bool accumulate) {
       char* const ds = static_cast<char*>(dguh.data_ptr());
@@ -1084,7 +1087,11 @@ std::optional<Tensor> bmm_experts_fp8(const OptTensor& w1_, const OptTensor& w2_
                       "expert weight shapes disagree");
   same_device(x, {&w1, &w2, &w3, &q1, &counts});
   c10::hip::HIPGuard device(x.device().index());
-  const Tensor starts = ExpertsFn::counts_to_starts(counts);
+  TORCH_CHECK_VALUE(counts.scalar_type() == at::kInt || counts.scalar_type() == at::kLong, "counts must be int32 or int64");
+  const int64_t A = x.size(0), bytes = pk_fp8_plan_bytes(A, w.E);
+  TORCH_CHECK(bytes > 0, "pk_fp8_plan_bytes failed: ", pk_status_string((int)bytes));
+  Tensor starts = at::empty({bytes / 4}, counts.options().dtype(at::kInt));      // the plan, which begins with them
+  PK_CALL(pk_fp8_plan, ptr(contig(counts)), counts.scalar_type() == at::kLong, w.E, A, starts.data_ptr<int32_t>(), stream_of(x));
   if (wants_grad({&w1, &w2, &w3, &x})) {
     TORCH_CHECK_VALUE(t1.defined(), "bmm_experts_fp8: a backward needs the transposed codes (quantize_experts(..., for_backward=True))");
     TORCH_CHECK_TYPE(!wants_grad({&w1, &w2, &w3}) || (w1.scalar_type() == at::kBFloat16 && w2.scalar_type() == at::kBFloat16 && w3.scalar_type() == at::kBFloat16),

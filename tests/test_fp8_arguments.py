@@ -39,6 +39,10 @@ def test_quantize(p):
 
 def test_products(p):
     lib = _lib.load()
+    assert lib.pk_fp8_plan(p, 0, 0, 8, p, None) == ARG and lib.pk_fp8_plan(None, 0, 4, 8, p, None) == ARG and lib.pk_fp8_plan(p, 0, 4, -1, p, None) == ARG
+    assert lib.pk_fp8_plan(p, 0, 1025, 8, p, None) == SHAPE and lib.pk_fp8_plan(p, 0, 4, 8, p + 4, None) == ALIGN
+    assert lib.pk_fp8_plan_bytes(-1, 4) < 0 and lib.pk_fp8_plan_bytes(8, 0) < 0 and lib.pk_fp8_plan_bytes(8, 1025) < 0
+    assert lib.pk_fp8_plan_bytes(1000, 6) == 4 * (8 + 8 * (1000 // 128 + 6)) and lib.pk_fp8_plan_bytes(0, 7) == 4 * 16
 
     def calls(A, H, I, E, q=p):
         yield lib.pk_fp8_gate_up(q, p, None, 1, p, p, p, p, p, p, p, p, p, A, H, I, E, None)
