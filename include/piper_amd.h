@@ -465,6 +465,14 @@ PK_API int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const int32
 /* y[A, H] (bf16) = h . w2[e]^T */
 PK_API int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2,
                 const int32_t* plan, void* y, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
+/* The forward of a pass with few rows in two launches, without a plan: what pk_fp8_quantize_rows, pk_fp8_plan, pk_fp8_gate_up
+ * and pk_fp8_down compute from x (bf16 [A, H]) and the row counts, up to the order of the sums, and zeros in the rows of
+ * y that no expert owns.  h: workspace, fp32 [A, I]; g and u as in pk_fp8_gate_up.  Right for any A; pk_fp8_few_rows_pays (HOST,
+ * tuning hint): 1 where it is the faster way. */
+PK_API int pk_fp8_few_rows_pays(int64_t A, int64_t H, int64_t I, int64_t E);
+PK_API int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64, const uint8_t* w1, const uint8_t* s1,
+                            const uint8_t* w2, const uint8_t* s2, const uint8_t* w3, const uint8_t* s3, void* g, void* u,
+                            float* h, void* y, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
 /* d_h = d_y . w2[e] (w2_t: the transposed codes) in fp32, and from it d_g = d_h * u * silu'(g) and
  * d_u = d_h * silu(g), both bf16 [A, I] (for pk_grouped_swiglu_wgrad) and in blocks (for pk_fp8_dgrad_dx), and
  * h = silu(g) * u (bf16).  With scores (f32, of every routed slot) and row_map, as

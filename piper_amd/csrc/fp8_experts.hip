@@ -619,6 +619,233 @@ int launch_product(const Product& p, int64_t A, int kernel_id, hipStream_t s) {
   return launch_tiles<2, 64, 3, EPI>(p, A, kernel_id, s);
 }
 
+// ------------------------------------------------------------------------------------------------ few rows
+// A handful of rows an expert: the weights are the traffic (one token, 8 of 128 experts, 2048 x 768: 38 MB), so every wave requests
+// all it needs of them at once, straight into registers, and nothing runs before that needs a launch of its own.  The rows are
+// quantized on their way in, and a workgroup finds its expert in the row counts by itself.  v_mfma_scale_f32_16x16x128_f8f6f4: 16
+// rows of x, 16 of a weight, one block of both.
+//   gate_up_few: 16 columns of gate and up to a workgroup, its eight waves take every eighth block of the reduction; h stays fp32,
+//                since a block of it belongs to eight workgroups
+//   down_few:    h in blocks into the LDS, then 16 columns to each of four waves
+constexpr int FEW_ROWS = 16;
+
+struct Few {
+  const void* counts;
+  int32_t is_i64, E, H, I;
+  int64_t A;
+  const bf16_t* x;
+  const uint8_t *q1, *s1, *q3, *s3, *q2, *s2;
+  bf16_t *g, *u;            // optional
+  float* h;                 // [A, I]
+  bf16_t* y;
+  int32_t n_cols;           // column tiles
+  FastDiv by_cols;
+  bool vec;                 // x: rows are whole 16-byte pieces
+};
+
+// The row tile of that number: its expert and rows.  Every wave looks for itself.  total_rows: rows that belong to an expert.
+__device__ __forceinline__ bool find_rows(const Few& p, int tile, int& e_out, int& row0, int& rows, int& total_rows) {
+  const int lane = threadIdx.x & 63, epl = (p.E + 63) >> 6, lo = lane * epl, hi = min(p.E, lo + epl);
+  const auto count = [&](int e) {
+    const int64_t n = p.is_i64 ? reinterpret_cast<const int64_t*>(p.counts)[e] : reinterpret_cast<const int32_t*>(p.counts)[e];
+    return n < 0 ? (int64_t)0 : n > p.A ? p.A : n;
+  };
+  int64_t mine = 0;
+  for (int e = lo; e < hi; ++e) mine += count(e);
+  int64_t incl = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t o = __shfl_up(incl, off, PK_WAVE);
+    if (lane >= off) incl += o;
+  }
+  const int64_t begin = min(incl - mine, p.A);
+  total_rows = (int)min(__shfl(incl, 63, PK_WAVE), p.A);
+  int tiles = 0;
+  for (int64_t e = lo, at = begin; e < hi; ++e) {
+    const int64_t end = min(at + count((int)e), p.A);
+    tiles += (int)((end - at + FEW_ROWS - 1) / FEW_ROWS);
+    at = end;
+  }
+  int sum = tiles;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(sum, off, PK_WAVE);
+    if (lane >= off) sum += o;
+  }
+  const unsigned long long owner = __ballot(tile >= sum - tiles && tile < sum);
+  if (owner == 0ull) return false;
+  const int src = __ffsll((long long)owner) - 1;
+  int left = tile - __shfl(sum - tiles, src, PK_WAVE);
+  int64_t at = __shfl(begin, src, PK_WAVE);
+  int e = src * epl;
+  for (;; ++e) {                             // ends: the tile is one of this lane's experts'
+    const int64_t end = min(at + count(e), p.A);
+    const int n = (int)((end - at + FEW_ROWS - 1) / FEW_ROWS);
+    if (left < n) {
+      e_out = __builtin_amdgcn_readfirstlane(e);
+      row0 = __builtin_amdgcn_readfirstlane((int)at + left * FEW_ROWS);
+      rows = __builtin_amdgcn_readfirstlane((int)min((int64_t)FEW_ROWS, end - at - left * FEW_ROWS));
+      return true;
+    }
+    left -= n;
+    at = end;
+  }
+}
+
+__device__ __forceinline__ uint32_t max_of_row(uint32_t m) {      // over the four lanes that share a row of 16
+  m = umax(m, __shfl_xor(m, 16));
+  return umax(m, __shfl_xor(m, 32));
+}
+__device__ __forceinline__ floatx4_t mfma16(intx8_t w, int sw, intx8_t x, int sx, floatx4_t acc) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc, 0, 0, 0, sw, 0, sx);
+}
+__device__ __forceinline__ intx8_t as_fragment(u32x4_t a, u32x4_t b) {
+  return intx8_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+
+__global__ __launch_bounds__(512, 2) void gate_up_few_kernel(const Few p) {
+  constexpr int WAVES = 8, AHEAD = 2;        // blocks of a wave that are requested at once
+  __shared__ float part[WAVES][2][4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int tile = pk_units::fastdiv((int)blockIdx.x, p.by_cols), ct = (int)blockIdx.x - tile * p.n_cols;
+  int e, row0, rows, total_rows;
+  if (!find_rows(p, tile, e, row0, rows, total_rows)) return;
+  const int hb = (p.H + BLOCK - 1) / BLOCK, ib = (p.I + BLOCK - 1) / BLOCK, Hp = hb * BLOCK;
+  const int r = lane & 15, quarter = lane >> 4, n0 = ct * 16;
+  const int64_t wrow = (int64_t)e * p.I + (n0 + r < p.I ? n0 + r : n0);
+  const uint8_t* const w1 = p.q1 + wrow * Hp + quarter * 32;
+  const uint8_t* const w3 = p.q3 + wrow * Hp + quarter * 32;
+  const int64_t srow = ((int64_t)e * ib + n0 / BLOCK) * hb;
+  const bf16_t* const x = p.x + (int64_t)(row0 + (r < rows ? r : 0)) * p.H + quarter * 32;
+  floatx4_t ag = {0.f, 0.f, 0.f, 0.f}, au = ag;
+  for (int b0 = wave; b0 < hb; b0 += WAVES * AHEAD) {
+    u32x4_t wg[AHEAD][2], wu[AHEAD][2];
+    int sg[AHEAD], su[AHEAD];
+    bf16x8_t xs[AHEAD][4];
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) {
+      const int b = b0 + t * WAVES < hb ? b0 + t * WAVES : b0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        wg[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(w1 + b * BLOCK + 16 * i));
+        wu[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(w3 + b * BLOCK + 16 * i));
+      }
+      sg[t] = p.s1[srow + b];
+      su[t] = p.s3[srow + b];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = b * BLOCK + quarter * 32 + 8 * i, have = r < rows ? p.H - k : 0;
+        if (p.vec) {
+          xs[t][i] = bf16x8_t{};
+          if (have > 0) xs[t][i] = *reinterpret_cast<const bf16x8_t*>(x + b * BLOCK + 8 * i);
+        } else {
+#pragma unroll
+          for (int v = 0; v < 8; ++v) xs[t][i][v] = v < have ? x[b * BLOCK + 8 * i + v] : (bf16_t)0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) {
+      if (b0 + t * WAVES >= hb) break;
+      float f[2][16];
+      uint32_t m = 0u;
+#pragma unroll
+      for (int v = 0; v < 32; ++v) {
+        f[v >> 4][v & 15] = (float)xs[t][v >> 3][v & 7];
+        m = umax(m, __float_as_uint(f[v >> 4][v & 15]) & 0x7fffffffu);
+      }
+      const pk_fp8::BlockScale sc = pk_fp8::block_scale(max_of_row(m));
+      const intx8_t xf = as_fragment(pk_fp8::codes16(f[0], sc), pk_fp8::codes16(f[1], sc));
+      ag = mfma16(as_fragment(wg[t][0], wg[t][1]), sg[t], xf, (int)sc.byte, ag);
+      au = mfma16(as_fragment(wu[t][0], wu[t][1]), su[t], xf, (int)sc.byte, au);
+    }
+  }
+  // acc[v] = C[row = lane % 16][col = 4 * (lane / 16) + v]
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    part[wave][0][v][lane] = ag[v];
+    part[wave][1][v][lane] = au[v];
+  }
+  __syncthreads();
+  if (threadIdx.x >= 256) return;
+  const int v = threadIdx.x >> 6, n = n0 + 4 * quarter + v;
+  float g = 0.f, u = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    g += part[w][0][v][lane];
+    u += part[w][1][v][lane];
+  }
+  if (r >= rows || n >= p.I) return;
+  const int64_t o = (int64_t)(row0 + r) * p.I + n;
+  g = held(g);
+  u = held(u);
+  if (p.g) {
+    p.g[o] = (bf16_t)g;
+    p.u[o] = (bf16_t)u;
+  }
+  p.h[o] = g * sigmoid(g) * u;
+}
+
+__global__ __launch_bounds__(256, 4) void down_few_kernel(const Few p, int units) {
+  constexpr int AHEAD = 4;
+  extern __shared__ __attribute__((aligned(16))) char smem[];      // [16 rows][I' + 16] codes, [16][I' / 128] scales
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int hb = (p.H + BLOCK - 1) / BLOCK, ib = (p.I + BLOCK - 1) / BLOCK, Ip = ib * BLOCK, ld = Ip + 16;
+  int e, row0, rows, total_rows;
+  if ((int)blockIdx.x >= units) {            // rows of no expert: zeros
+    find_rows(p, -1, e, row0, rows, total_rows);
+    const int64_t first = (int64_t)total_rows * p.H, step = (int64_t)(gridDim.x - units) * blockDim.x;
+    for (int64_t i = first + (int64_t)(blockIdx.x - units) * blockDim.x + threadIdx.x; i < p.A * p.H; i += step) p.y[i] = (bf16_t)0.f;
+    return;
+  }
+  const int tile = pk_units::fastdiv((int)blockIdx.x, p.by_cols), ct = (int)blockIdx.x - tile * p.n_cols;
+  if (!find_rows(p, tile, e, row0, rows, total_rows)) return;
+  const int r = lane & 15, quarter = lane >> 4, n0 = (ct * 4 + wave) * 16;
+  const bool columns = n0 < p.H;
+  const uint8_t* const w = p.q2 + ((int64_t)e * p.H + (n0 + r < p.H ? n0 + r : 0)) * Ip + quarter * 32;
+  const uint8_t* const sw = p.s2 + ((int64_t)e * hb + (columns ? n0 / BLOCK : 0)) * ib;
+  u32x4_t wv[AHEAD][2];
+  const auto request = [&](int b0) {
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (b0 + t < ib) wv[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(w + (b0 + t) * BLOCK + 16 * i));
+  };
+  if (columns) request(0);
+  uint8_t* const q = reinterpret_cast<uint8_t*>(smem);
+  uint8_t* const qs = q + FEW_ROWS * ld;
+  for (int i = threadIdx.x >> 4; i < FEW_ROWS * ib; i += 16) {      // 16 lanes to a block
+    const int hr = i / ib, b = i - hr * ib, k = b * BLOCK + (threadIdx.x & 15) * 8;
+    const float* const from = p.h + (int64_t)(row0 + (hr < rows ? hr : 0)) * p.I + k;
+    float f[8];
+#pragma unroll
+    for (int v = 0; v < 8; ++v) f[v] = hr < rows && k + v < p.I ? from[v] : 0.f;
+    uint32_t codes[2], byte;
+    pk_fp8::quantize8(f, codes, byte);
+    *reinterpret_cast<u32x2_t*>(q + hr * ld + k) = u32x2_t{codes[0], codes[1]};
+    if ((threadIdx.x & 15) == 0) qs[hr * ib + b] = (uint8_t)byte;
+  }
+  __syncthreads();
+  if (!columns) return;
+  floatx4_t acc = {0.f, 0.f, 0.f, 0.f};
+  for (int b0 = 0; b0 < ib; b0 += AHEAD) {
+    if (b0 > 0) request(b0);
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) {
+      const int b = b0 + t;
+      if (b >= ib) break;
+      const u32x4_t* const f = reinterpret_cast<const u32x4_t*>(q + r * ld + b * BLOCK + quarter * 32);
+      acc = mfma16(as_fragment(wv[t][0], wv[t][1]), sw[b], as_fragment(f[0], f[1]), qs[r * ib + b], acc);
+    }
+  }
+  if (r >= rows) return;
+  bf16_t* const to = p.y + (int64_t)(row0 + r) * p.H + n0 + 4 * quarter;
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+    if (n0 + 4 * quarter + v < p.H) to[v] = (bf16_t)acc[v];
+}
+
 // Common checks of the products.  Offsets from an operand's first row are 32 bits wide.
 int check(int64_t A, int64_t H, int64_t I, int64_t E) {
   if (A < 0 || H <= 0 || I <= 0 || E <= 0) return PK_ERR_ARG;
@@ -779,6 +1006,45 @@ int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_
   p.vec = bf16_pieces(H, {d_x});
   p.O0 = (bf16_t*)d_x;
   return launch_product<PLAIN>(p, A, pk_timing::K_FP8_DGRAD_DX, (hipStream_t)stream);
+}
+
+int pk_fp8_few_rows_pays(int64_t A, int64_t H, int64_t I, int64_t E) {
+  if (check(A, H, I, E) != PK_OK || A == 0) return 0;
+  return A <= 8 * E;
+}
+
+int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64, const uint8_t* w1, const uint8_t* s1, const uint8_t* w2,
+                            const uint8_t* s2, const uint8_t* w3, const uint8_t* s3, void* g, void* u, float* h, void* y, int64_t A, int64_t H,
+                            int64_t I, int64_t E, pk_stream_t stream) {
+  if (const int rc = check(A, H, I, E)) return rc;
+  if (A == 0) return PK_OK;
+  if (!all_set({x, counts, w1, s1, w2, s2, w3, s3, h, y}) || !g != !u) return PK_ERR_ARG;
+  if (!all_aligned({w1, w2, w3})) return PK_ERR_ALIGN;
+  Few p = {};
+  p.counts = counts; p.is_i64 = counts_is_i64; p.E = (int32_t)E; p.H = (int32_t)H; p.I = (int32_t)I; p.A = A;
+  p.x = (const bf16_t*)x; p.q1 = w1; p.s1 = s1; p.q2 = w2; p.s2 = s2; p.q3 = w3; p.s3 = s3;
+  p.g = (bf16_t*)g; p.u = (bf16_t*)u; p.h = h; p.y = (bf16_t*)y;
+  p.vec = bf16_pieces(H, {x});
+  const int64_t tiles = A / FEW_ROWS + (A < E ? A : E), up = pk_ceil_div(I, 16), down = pk_ceil_div(H, 64);
+  if (tiles * up > 0x7fffff00ll || tiles * down > 0x7fffff00ll) return PK_ERR_SHAPE;
+  hipStream_t s = (hipStream_t)stream;
+  p.n_cols = (int32_t)up; p.by_cols = pk_units::make_fastdiv(up);
+  PK_LAUNCH_NOCHECK(pk_timing::K_FP8_GATE_UP, s, gate_up_few_kernel, dim3((unsigned)(tiles * up)), dim3(512), 0, s, p);
+  PK_RETURN_IF_LAUNCH_FAILED();
+  p.n_cols = (int32_t)down; p.by_cols = pk_units::make_fastdiv(down);
+  const int units = (int)(tiles * down), zeros = (int)(A < 32 ? A : 32);
+  const int lds = (int)(FEW_ROWS * (blocks_of(I) * BLOCK + 16) + FEW_ROWS * blocks_of(I));      // at most 66,304 bytes
+  static bool ready[PK_MAX_DEVICES] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= PK_MAX_DEVICES) return PK_ERR_UNSUPPORTED;
+  if (!ready[dev]) {
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(down_few_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+    if (err != hipSuccess) return (int)err;
+    ready[dev] = true;
+  }
+  PK_LAUNCH_NOCHECK(pk_timing::K_FP8_DOWN, s, down_few_kernel, dim3((unsigned)(units + zeros)), dim3(256), lds, s, p, units);
+  PK_RETURN_IF_LAUNCH_FAILED();
+  return PK_OK;
 }
 
 }  // extern "C"

@@ -988,34 +988,52 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
   static void zero_tail(const Tensor& buf, const Tensor& plan, int64_t E) {
     PK_CALL(pk_zero_rows_from, ptr(buf), PK_BF16, plan.data_ptr<int32_t>() + E, buf.size(0), buf.size(1), stream_of(buf));
   }
-  // y [A,H]; gu [2,A,I]: where the pre-activations are left
-  static Tensor run(const Fp8Weights& w, const Tensor& x, const Tensor& starts, Tensor* gu) {
-    const int64_t A = x.size(0), H = w.H, I = w.I;
-    Block b;
-    const size_t x8 = b.add(codes(A, H)), xs = b.add(scales(A, H)), h8 = b.add(codes(A, I)), hs = b.add(scales(A, I));
-    b.allocate(x);
+  // The plan of a pass; it begins with starts[]
+  static Tensor plan_of(const Tensor& counts, int64_t E, int64_t A) {
+    const int64_t bytes = pk_fp8_plan_bytes(A, E);
+    TORCH_CHECK(bytes > 0, "pk_fp8_plan_bytes failed: ", pk_status_string((int)bytes));
+    Tensor plan = at::empty({bytes / 4}, counts.options().dtype(at::kInt));
+    PK_CALL(pk_fp8_plan, ptr(counts), counts.scalar_type() == at::kLong, E, A, plan.data_ptr<int32_t>(), stream_of(counts));
+    return plan;
+  }
+  // y [A,H]; gu [2,A,I]: where the pre-activations are left, plan_out: the pass's plan (both null without a backward)
+  static Tensor run(const Fp8Weights& w, const Tensor& x, const Tensor& counts, Tensor* gu, Tensor* plan_out) {
+    const int64_t A = x.size(0), H = w.H, I = w.I, E = w.E;
     Tensor y = at::empty({A, H}, x.options());
-    char* g = nullptr;
+    char *g = nullptr, *u = nullptr;
     if (gu) {
       *gu = at::empty({2, A, I}, x.options());
       g = static_cast<char*>(gu->data_ptr());
+      u = g + A * I * 2;
     }
     const pk_stream_t st = stream_of(x);
-    const int32_t* const at = starts.data_ptr<int32_t>();
+    Block b;
+    if (pk_fp8_few_rows_pays(A, H, I, E)) {
+      const size_t h = b.add(A * I * 4);
+      b.allocate(x);
+      PK_CALL(pk_fp8_experts_few_rows, ptr(x), ptr(counts), counts.scalar_type() == at::kLong, u8(w.q[0]), u8(w.s[0]), u8(w.q[1]), u8(w.s[1]),
+              u8(w.q[2]), u8(w.s[2]), g, u, b.f32(h), ptr(y), A, H, I, E, st);
+      if (plan_out) *plan_out = plan_of(counts, E, A);
+      return y;
+    }
+    const size_t x8 = b.add(codes(A, H)), xs = b.add(scales(A, H)), h8 = b.add(codes(A, I)), hs = b.add(scales(A, I));
+    b.allocate(x);
+    const Tensor plan = plan_of(counts, E, A);
+    const int32_t* const at = plan.data_ptr<int32_t>();
     const auto p = [&](size_t pos) { return static_cast<uint8_t*>(b.at_(pos)); };
     PK_CALL(pk_fp8_quantize_rows, ptr(x), PK_BF16, nullptr, 1, p(x8), p(xs), A, H, st);
-    PK_CALL(pk_fp8_gate_up, p(x8), p(xs), nullptr, 1, u8(w.q[0]), u8(w.s[0]), u8(w.q[2]), u8(w.s[2]), at, g, g ? g + A * I * 2 : nullptr, p(h8),
-            p(hs), A, H, I, w.E, st);
-    PK_CALL(pk_fp8_down, p(h8), p(hs), u8(w.q[1]), u8(w.s[1]), at, ptr(y), A, H, I, w.E, st);
-    zero_tail(y, starts, w.E);
+    PK_CALL(pk_fp8_gate_up, p(x8), p(xs), nullptr, 1, u8(w.q[0]), u8(w.s[0]), u8(w.q[2]), u8(w.s[2]), at, g, u, p(h8), p(hs), A, H, I, E, st);
+    PK_CALL(pk_fp8_down, p(h8), p(hs), u8(w.q[1]), u8(w.s[1]), at, ptr(y), A, H, I, E, st);
+    zero_tail(y, plan, E);
+    if (plan_out) *plan_out = plan;
     return y;
   }
   static Tensor forward(AutogradContext* ctx, const OptTensor& w1, const OptTensor& w2, const OptTensor& w3, const Tensor& x, const Fp8Weights* w,
-                        const Tensor& starts) {
-    Tensor gu;
+                        const Tensor& counts) {
+    Tensor gu, plan;
     const Tensor xc = contig(x);
-    Tensor y = run(*w, xc, starts, &gu);
-    ctx->save_for_backward({xc, starts, gu, w->t[0], w->t[1], w->t[2], w->s[0], w->s[1], w->s[2]});
+    Tensor y = run(*w, xc, counts, &gu, &plan);
+    ctx->save_for_backward({xc, plan, gu, w->t[0], w->t[1], w->t[2], w->s[0], w->s[1], w->s[2]});
     const Tensor p1 = opt(w1), p2 = opt(w2), p3 = opt(w3);
     keep_parameters(ctx, {&p1, &p2, &p3});
     ctx->saved_data["weights"] = p1.defined();
@@ -1088,17 +1106,14 @@ std::optional<Tensor> bmm_experts_fp8(const OptTensor& w1_, const OptTensor& w2_
   same_device(x, {&w1, &w2, &w3, &q1, &counts});
   c10::hip::HIPGuard device(x.device().index());
   TORCH_CHECK_VALUE(counts.scalar_type() == at::kInt || counts.scalar_type() == at::kLong, "counts must be int32 or int64");
-  const int64_t A = x.size(0), bytes = pk_fp8_plan_bytes(A, w.E);
-  TORCH_CHECK(bytes > 0, "pk_fp8_plan_bytes failed: ", pk_status_string((int)bytes));
-  Tensor starts = at::empty({bytes / 4}, counts.options().dtype(at::kInt));      // the plan, which begins with them
-  PK_CALL(pk_fp8_plan, ptr(contig(counts)), counts.scalar_type() == at::kLong, w.E, A, starts.data_ptr<int32_t>(), stream_of(x));
+  const Tensor n = contig(counts);
   if (wants_grad({&w1, &w2, &w3, &x})) {
     TORCH_CHECK_VALUE(t1.defined(), "bmm_experts_fp8: a backward needs the transposed codes (quantize_experts(..., for_backward=True))");
     TORCH_CHECK_TYPE(!wants_grad({&w1, &w2, &w3}) || (w1.scalar_type() == at::kBFloat16 && w2.scalar_type() == at::kBFloat16 && w3.scalar_type() == at::kBFloat16),
                      "bmm_experts_fp8: weights that want gradients are bfloat16");
-    return Fp8ExpertsFn::apply(w1_, w2_, w3_, x, &w, starts);
+    return Fp8ExpertsFn::apply(w1_, w2_, w3_, x, &w, n);
   }
-  return Fp8ExpertsFn::run(w, contig(x), starts, nullptr);
+  return Fp8ExpertsFn::run(w, contig(x), n, nullptr, nullptr);
 }
 
 // ------------------------------------------------------------------------------ bucket path

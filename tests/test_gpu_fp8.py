@@ -6,8 +6,8 @@ import pytest
 import torch
 
 from oracle import blocks as B
+from piper_amd import _lib, ops
 from piper_amd import functional as F_
-from piper_amd import ops
 from piper_amd.moe import AnnotatedMoE, BmmExperts, MoEArgs
 
 pytestmark = pytest.mark.gpu
@@ -142,6 +142,56 @@ def test_few_rows(dev, A, E, H, I):
         y = F_.bmm_experts_fp8(F_.quantize_experts(*(w.to(dev) for w in (w1, w2, w3)), for_backward=False), x.to(dev),
                                torch.tensor(counts, device=dev))
     _within("y", y, *want["y"])
+
+
+@pytest.mark.parametrize("E,H,I,counts,spare", [(3, 256, 384, [40, 0, 17], 5), (2, 130, 70, [1, 33], 0), (130, 72, 200, [i % 3 for i in range(130)], 2)])
+def test_both_ways_of_the_forward_take_any_rows(dev, E, H, I, counts, spare):
+    """pk_fp8_experts_few_rows where pk_fp8_few_rows_pays would not choose it, and the tiles where it would."""
+    print(f"[case] fp8 experts both ways E={E} H={H} I={I}", flush=True)
+    lib, A = _lib.load(), sum(counts) + spare
+    w1, w2, w3, x, _ = _inputs(E, H, I, counts, spare, 9, False)
+    want = B.experts_between(w1, w2, w3, x, counts)
+    e = F_.quantize_experts(*(w.to(dev) for w in (w1, w2, w3)))
+    xd, n, st = x.to(dev), torch.tensor(counts, dtype=torch.int64, device=dev), _lib.current_stream(dev)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    y, h = torch.full((A, H), 7.0, device=dev).bfloat16(), torch.empty(A, I, device=dev)
+    g, u = (torch.empty(A, I, device=dev).bfloat16() for _ in range(2))
+    assert lib.pk_fp8_experts_few_rows(p(xd), p(n), 1, p(e.q1), p(e.s1), p(e.q2), p(e.s2), p(e.q3), p(e.s3), p(g), p(u), p(h), p(y), A, H, I, E, st) == 0
+    _within("y, few rows", y, *want["y"])
+    bare = torch.full((A, H), 7.0, device=dev).bfloat16()
+    assert lib.pk_fp8_experts_few_rows(p(xd), p(n), 1, p(e.q1), p(e.s1), p(e.q2), p(e.s2), p(e.q3), p(e.s3), None, None, p(h), p(bare), A, H, I, E, st) == 0
+    assert torch.equal(y, bare)
+    q, s = ops.quantize_rows_fp8(xd)
+    plan = torch.empty(lib.pk_fp8_plan_bytes(A, E) // 4, dtype=torch.int32, device=dev)
+    h8, hs = torch.empty(A, -(-I // 128) * 128, dtype=torch.uint8, device=dev), torch.empty(A, -(-I // 128), dtype=torch.uint8, device=dev)
+    tiles = torch.full((A, H), 7.0, device=dev).bfloat16()
+    g2, u2 = (torch.empty(A, I, device=dev).bfloat16() for _ in range(2))
+    assert lib.pk_fp8_plan(p(n), 1, E, A, p(plan), st) == 0
+    assert plan[:E + 1].tolist() == [0] + torch.tensor(counts).cumsum(0).tolist()
+    assert lib.pk_fp8_gate_up(p(q), p(s), None, 1, p(e.q1), p(e.s1), p(e.q3), p(e.s3), p(plan), p(g2), p(u2), p(h8), p(hs), A, H, I, E, st) == 0
+    assert lib.pk_fp8_down(p(h8), p(hs), p(e.q2), p(e.s2), p(plan), p(tiles), A, H, I, E, st) == 0
+    owned = sum(counts)
+    assert (tiles[owned:] == 7.0).all() and (y[owned:] == 0).all()
+    _within("y, tiles", tiles[:owned], *(t[:owned] for t in want["y"]))
+    # both are the bf16 rounding of sums that differ in the last places
+    for a, b in ((g, g2), (u, u2)):
+        assert ((a[:owned].float() - b[:owned].float()).abs() <= 2.0 ** -7 * a[:owned].float().abs() + 1e-3).all()
+
+
+def test_counts_that_do_not_fit_lead_nowhere(dev):
+    """More rows than there are, and negative counts: cut off, so that nothing is read or written out of bounds."""
+    print("[case] fp8 experts, counts that do not fit", flush=True)
+    w, x, d_y, _ = _setup(dev, counts=(20, 0, 44))
+    with torch.no_grad():
+        e = F_.quantize_experts(*w)
+        for bad, good in (((20, -3, 1000), (20, 0, 44)), ((10 ** 6, 5, 5), (64, 0, 0)), ((-1, -1, 7), (0, 0, 7)), ((2 ** 40, 2 ** 40, 2 ** 40), (64, 0, 0))):
+            for A in (64, 20):
+                b, g = torch.tensor(bad, device=dev), [0, 0, 0]
+                left = A
+                for i, c in enumerate(good):
+                    g[i] = min(c, left)
+                    left -= g[i]
+                assert torch.equal(F_.bmm_experts_fp8(e, x[:A], b), F_.bmm_experts_fp8(e, x[:A], torch.tensor(g, device=dev)))
 
 
 def test_a_row_that_is_not_finite_stays_a_row(dev):
