@@ -786,9 +786,118 @@ __global__ __launch_bounds__(512, 2) void gate_up_few_kernel(const Few p) {
   p.h[o] = g * sigmoid(g) * u;
 }
 
-__global__ __launch_bounds__(256, 4) void down_few_kernel(const Few p, int units) {
-  constexpr int AHEAD = 4;
-  extern __shared__ __attribute__((aligned(16))) char smem[];      // [16 rows][I' + 16] codes, [16][I' / 128] scales
+// A row tile's rows of K values in blocks into the LDS, 16 lanes to a block; rows that are not there stay as they are, since no other
+// row sees them.
+template <typename T>
+__device__ __forceinline__ void rows_into_lds(const T* from, int64_t ld_from, int rows, int K, bool vec, uint8_t* q, int ld, uint8_t* qs) {
+  const int nb = (K + BLOCK - 1) / BLOCK;
+  for (int i = threadIdx.x >> 4; i < rows * nb; i += (int)blockDim.x >> 4) {
+    const int r = i / nb, b = i - r * nb, k = b * BLOCK + (threadIdx.x & 15) * 8;
+    float f[8];
+    load8<T>(from + r * ld_from + k, K - k, vec, f);
+    uint32_t codes[2], byte;
+    pk_fp8::quantize8(f, codes, byte);
+    *reinterpret_cast<u32x2_t*>(q + r * ld + k) = u32x2_t{codes[0], codes[1]};
+    if ((threadIdx.x & 15) == 0) qs[r * nb + b] = (uint8_t)byte;
+  }
+}
+__host__ __device__ inline int few_lds(int64_t K) {
+  const int nb = (int)((K + BLOCK - 1) / BLOCK);
+  return FEW_ROWS * (nb * BLOCK + 16) + FEW_ROWS * nb;
+}
+
+// The products of a row tile in the LDS with `tiles` times 16 columns of MATS weights, a block after the other with D blocks of them
+// in flight; done(c, acc) for every 16 columns.  w: the lane's part of column tile 0, `next` bytes further for the next one.
+template <int MATS, int D, typename Done>
+__device__ __forceinline__ void stream_columns(const uint8_t* const (&w)[MATS], int64_t next, const uint8_t* const (&sw)[MATS], int64_t next_scale,
+                                               int nb, int tiles, const uint8_t* q, int ld, const uint8_t* qs, bool ready, Done&& done) {
+  const int r = threadIdx.x & 15, quarter = (threadIdx.x >> 4) & 3, steps = tiles * nb;
+  u32x4_t ring[D][MATS][2];
+  int fc = 0, fb = 0;                        // what is requested next; the last one again where nothing is left
+  const auto request = [&](auto& slot) {
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) slot[m][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(w[m] + fc * next + fb * BLOCK + 16 * i));
+    if (fc * nb + fb + 1 < steps) {
+      ++fb;
+      if (fb == nb) { fb = 0; ++fc; }
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < D; ++t) {
+    request(ring[t]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (!ready) __syncthreads();               // the rows are in the LDS
+  floatx4_t acc[MATS];
+#pragma unroll
+  for (int m = 0; m < MATS; ++m) acc[m] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+  int c = 0, b = 0;
+  const auto step = [&](auto& slot) {
+    const u32x4_t* const f = reinterpret_cast<const u32x4_t*>(q + r * ld + b * BLOCK + quarter * 32);
+    const intx8_t x = as_fragment(f[0], f[1]);
+    const int sx = qs[r * nb + b];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) acc[m] = mfma16(as_fragment(slot[m][0], slot[m][1]), sw[m][c * next_scale + b], x, sx, acc[m]);
+    if (++b == nb) {
+      done(c, acc);
+#pragma unroll
+      for (int m = 0; m < MATS; ++m) acc[m] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+      b = 0;
+      ++c;
+    }
+  };
+  int s = 0;
+  for (; s + D < steps; s += D) {
+#pragma unroll
+    for (int t = 0; t < D; ++t) {
+      step(ring[t]);
+      request(ring[t]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < D; ++t)
+    if (s + t < steps) step(ring[t]);
+}
+
+// gate and up with more workgroups than it takes to fill the chip: 16 columns and the whole reduction to a wave, nothing to add up.
+__global__ __launch_bounds__(512, 4) void gate_up_stream_kernel(const Few p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int tile = pk_units::fastdiv((int)blockIdx.x, p.by_cols), ct = (int)blockIdx.x - tile * p.n_cols;
+  int e, row0, rows, total_rows;
+  if (!find_rows(p, tile, e, row0, rows, total_rows)) return;
+  const int hb = (p.H + BLOCK - 1) / BLOCK, ib = (p.I + BLOCK - 1) / BLOCK, Hp = hb * BLOCK, ld = Hp + 16;
+  const int r = lane & 15, quarter = lane >> 4, n0 = (ct * 8 + wave) * 16;
+  uint8_t* const q = reinterpret_cast<uint8_t*>(smem);
+  uint8_t* const qs = q + FEW_ROWS * ld;
+  // (a wave behind the last column reads the first ones' weights and stores nothing)
+  const int64_t at = ((int64_t)e * p.I + (n0 + r < p.I ? n0 + r : 0)) * Hp + quarter * 32, sat = ((int64_t)e * ib + ct) * hb;
+  const uint8_t* const w[2] = {p.q1 + at, p.q3 + at};
+  const uint8_t* const sw[2] = {p.s1 + sat, p.s3 + sat};
+  rows_into_lds<bf16_t>(p.x + (int64_t)row0 * p.H, p.H, rows, p.H, p.vec, q, ld, qs);
+  stream_columns<2, 4>(w, 0, sw, 0, hb, 1, q, ld, qs, false, [&](int, const floatx4_t (&acc)[2]) {
+    if (r >= rows) return;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int n = n0 + 4 * quarter + v;
+      if (n >= p.I) continue;
+      const int64_t o = (int64_t)(row0 + r) * p.I + n;
+      const float g = held(acc[0][v]), u = held(acc[1][v]);
+      if (p.g) {
+        p.g[o] = (bf16_t)g;
+        p.u[o] = (bf16_t)u;
+      }
+      p.h[o] = g * sigmoid(g) * u;
+    }
+  });
+}
+
+// `tiles` times 64 columns to a workgroup of four waves.
+__global__ __launch_bounds__(256, 4) void down_few_kernel(const Few p, int units, int tiles) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int hb = (p.H + BLOCK - 1) / BLOCK, ib = (p.I + BLOCK - 1) / BLOCK, Ip = ib * BLOCK, ld = Ip + 16;
   int e, row0, rows, total_rows;
@@ -800,50 +909,30 @@ __global__ __launch_bounds__(256, 4) void down_few_kernel(const Few p, int units
   }
   const int tile = pk_units::fastdiv((int)blockIdx.x, p.by_cols), ct = (int)blockIdx.x - tile * p.n_cols;
   if (!find_rows(p, tile, e, row0, rows, total_rows)) return;
-  const int r = lane & 15, quarter = lane >> 4, n0 = (ct * 4 + wave) * 16;
-  const bool columns = n0 < p.H;
-  const uint8_t* const w = p.q2 + ((int64_t)e * p.H + (n0 + r < p.H ? n0 + r : 0)) * Ip + quarter * 32;
-  const uint8_t* const sw = p.s2 + ((int64_t)e * hb + (columns ? n0 / BLOCK : 0)) * ib;
-  u32x4_t wv[AHEAD][2];
-  const auto request = [&](int b0) {
-#pragma unroll
-    for (int t = 0; t < AHEAD; ++t)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (b0 + t < ib) wv[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(w + (b0 + t) * BLOCK + 16 * i));
-  };
-  if (columns) request(0);
+  // the wave's columns: 16 * tiles of them from n0 on
+  const int r = lane & 15, quarter = lane >> 4, n0 = (ct * 4 + wave) * 16 * tiles;
   uint8_t* const q = reinterpret_cast<uint8_t*>(smem);
   uint8_t* const qs = q + FEW_ROWS * ld;
-  for (int i = threadIdx.x >> 4; i < FEW_ROWS * ib; i += 16) {      // 16 lanes to a block
-    const int hr = i / ib, b = i - hr * ib, k = b * BLOCK + (threadIdx.x & 15) * 8;
-    const float* const from = p.h + (int64_t)(row0 + (hr < rows ? hr : 0)) * p.I + k;
-    float f[8];
-#pragma unroll
-    for (int v = 0; v < 8; ++v) f[v] = hr < rows && k + v < p.I ? from[v] : 0.f;
-    uint32_t codes[2], byte;
-    pk_fp8::quantize8(f, codes, byte);
-    *reinterpret_cast<u32x2_t*>(q + hr * ld + k) = u32x2_t{codes[0], codes[1]};
-    if ((threadIdx.x & 15) == 0) qs[hr * ib + b] = (uint8_t)byte;
-  }
+  const int mine = min(tiles, (p.H - n0 + 15) / 16);
+  rows_into_lds<float>(p.h + (int64_t)row0 * p.I, p.I, rows, p.I, p.I % 4 == 0 && ((uintptr_t)p.h & 15) == 0, q, ld, qs);
   __syncthreads();
-  if (!columns) return;
-  floatx4_t acc = {0.f, 0.f, 0.f, 0.f};
-  for (int b0 = 0; b0 < ib; b0 += AHEAD) {
-    if (b0 > 0) request(b0);
+  if (mine <= 0) return;
+  for (int c0 = 0; c0 < mine;) {             // columns that share a row of scales, and whole tiles or a last one that is not
+    const int n = n0 + 16 * c0;
+    int take = min(mine - c0, (BLOCK - n % BLOCK) / 16);
+    if (n + 16 * take > p.H && take > 1) --take;
+    const uint8_t* const w[1] = {p.q2 + ((int64_t)e * p.H + (n + r < p.H ? n + r : n)) * Ip + quarter * 32};
+    const uint8_t* const sw[1] = {p.s2 + ((int64_t)e * hb + n / BLOCK) * ib};
+    stream_columns<1, 6>(w, (int64_t)16 * Ip, sw, 0, ib, take, q, ld, qs, true, [&](int c, const floatx4_t (&acc)[1]) {
+      if (r >= rows) return;
+      const int at = n + 16 * c + 4 * quarter;
+      bf16_t* const to = p.y + (int64_t)(row0 + r) * p.H + at;
 #pragma unroll
-    for (int t = 0; t < AHEAD; ++t) {
-      const int b = b0 + t;
-      if (b >= ib) break;
-      const u32x4_t* const f = reinterpret_cast<const u32x4_t*>(q + r * ld + b * BLOCK + quarter * 32);
-      acc = mfma16(as_fragment(wv[t][0], wv[t][1]), sw[b], as_fragment(f[0], f[1]), qs[r * ib + b], acc);
-    }
+      for (int v = 0; v < 4; ++v)
+        if (at + v < p.H) to[v] = (bf16_t)acc[0][v];
+    });
+    c0 += take;
   }
-  if (r >= rows) return;
-  bf16_t* const to = p.y + (int64_t)(row0 + r) * p.H + n0 + 4 * quarter;
-#pragma unroll
-  for (int v = 0; v < 4; ++v)
-    if (n0 + 4 * quarter + v < p.H) to[v] = (bf16_t)acc[v];
 }
 
 // Common checks of the products.  Offsets from an operand's first row are 32 bits wide.
@@ -1025,24 +1114,31 @@ int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64
   p.x = (const bf16_t*)x; p.q1 = w1; p.s1 = s1; p.q2 = w2; p.s2 = s2; p.q3 = w3; p.s3 = s3;
   p.g = (bf16_t*)g; p.u = (bf16_t*)u; p.h = h; p.y = (bf16_t*)y;
   p.vec = bf16_pieces(H, {x});
-  const int64_t tiles = A / FEW_ROWS + (A < E ? A : E), up = pk_ceil_div(I, 16), down = pk_ceil_div(H, 64);
+  const int64_t tiles = A / FEW_ROWS + (A < E ? A : E);
+  // whole reductions to a wave where that gives every CU a workgroup
+  const bool stream_up = tiles * blocks_of(I) >= 256;
+  const int64_t up = stream_up ? blocks_of(I) : pk_ceil_div(I, 16), per = tiles * pk_ceil_div(H, 64) >= 2048 ? 4 : 1, down = pk_ceil_div(H, 64 * per);
   if (tiles * up > 0x7fffff00ll || tiles * down > 0x7fffff00ll) return PK_ERR_SHAPE;
-  hipStream_t s = (hipStream_t)stream;
-  p.n_cols = (int32_t)up; p.by_cols = pk_units::make_fastdiv(up);
-  PK_LAUNCH_NOCHECK(pk_timing::K_FP8_GATE_UP, s, gate_up_few_kernel, dim3((unsigned)(tiles * up)), dim3(512), 0, s, p);
-  PK_RETURN_IF_LAUNCH_FAILED();
-  p.n_cols = (int32_t)down; p.by_cols = pk_units::make_fastdiv(down);
-  const int units = (int)(tiles * down), zeros = (int)(A < 32 ? A : 32);
-  const int lds = (int)(FEW_ROWS * (blocks_of(I) * BLOCK + 16) + FEW_ROWS * blocks_of(I));      // at most 66,304 bytes
   static bool ready[PK_MAX_DEVICES] = {};
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= PK_MAX_DEVICES) return PK_ERR_UNSUPPORTED;
   if (!ready[dev]) {
-    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(down_few_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
-    if (err != hipSuccess) return (int)err;
+    for (const void* k : {reinterpret_cast<const void*>(down_few_kernel), reinterpret_cast<const void*>(gate_up_stream_kernel)}) {
+      const hipError_t err = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, few_lds(PK_FP8_MAX_HIDDEN));
+      if (err != hipSuccess) return (int)err;
+    }
     ready[dev] = true;
   }
-  PK_LAUNCH_NOCHECK(pk_timing::K_FP8_DOWN, s, down_few_kernel, dim3((unsigned)(units + zeros)), dim3(256), lds, s, p, units);
+  hipStream_t s = (hipStream_t)stream;
+  p.n_cols = (int32_t)up; p.by_cols = pk_units::make_fastdiv(up);
+  if (stream_up)
+    PK_LAUNCH_NOCHECK(pk_timing::K_FP8_GATE_UP, s, gate_up_stream_kernel, dim3((unsigned)(tiles * up)), dim3(512), few_lds(H), s, p);
+  else
+    PK_LAUNCH_NOCHECK(pk_timing::K_FP8_GATE_UP, s, gate_up_few_kernel, dim3((unsigned)(tiles * up)), dim3(512), 0, s, p);
+  PK_RETURN_IF_LAUNCH_FAILED();
+  p.n_cols = (int32_t)down; p.by_cols = pk_units::make_fastdiv(down);
+  const int units = (int)(tiles * down), zeros = (int)(A < 32 ? A : 32);
+  PK_LAUNCH_NOCHECK(pk_timing::K_FP8_DOWN, s, down_few_kernel, dim3((unsigned)(units + zeros)), dim3(256), few_lds(I), s, p, units, (int)per);
   PK_RETURN_IF_LAUNCH_FAILED();
   return PK_OK;
 }
