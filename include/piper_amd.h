@@ -484,6 +484,17 @@ PK_API int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const 
                     const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales,
                     uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H, int64_t I, int64_t E,
                     pk_stream_t stream);
+/* The same with d_g, d_u and h as the transposed copies [ldt / 32][I][32] of pk_grouped_swiglu_dgrad_dh_scaled_t (which
+ * see), for pk_grouped_swiglu_wgrad_scaled_t: the faster pair with more than about 40 rows an expert.  ldt and the shapes that
+ * have such a path: pk_grouped_swiglu_transposed_ld. */
+PK_API int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div,
+                      const float* scores, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
+                      const int32_t* plan, void* d_gT, void* d_uT, void* hT, int64_t ldt, uint8_t* d_g8,
+                      uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H,
+                      int64_t I, int64_t E, pk_stream_t stream);
+/* row_map[r] = r for rows of an expert, the last such row for the others: the row map (divisor 1) of
+ * pk_grouped_swiglu_wgrad_scaled_t where the rows are sorted already. */
+PK_API int pk_fp8_row_map(const int32_t* plan, int64_t E, int64_t A, int32_t* row_map, pk_stream_t stream);
 /* d_x[A, H] (bf16) = d_g . w1[e] + d_u . w3[e] (w1_t, w3_t: the transposed codes) */
 PK_API int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales,
                     const uint8_t* w1_t, const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3,

@@ -187,6 +187,13 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const void* counts, 
   }
 }
 
+// Every row its own number, those of no expert the last one that has one: a row map for pk_grouped_swiglu_wgrad_scaled_t, which multiplies
+// rows behind an expert's last one by zeros.  What stands in rows of no expert (it may be anything) is thereby not read.
+__global__ __launch_bounds__(THREADS) void row_map_kernel(const int32_t* __restrict__ owned, int64_t A, int32_t* __restrict__ map) {
+  const int64_t r = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+  if (r < A) map[r] = (int32_t)(r < *owned ? r : *owned > 0 ? *owned - 1 : 0);
+}
+
 // ------------------------------------------------------------------------------------------------ products
 // C[rows_e, N] = sum_seg A_seg[rows_e, K] . B_seg[e][N, K]^T, one workgroup to a tile of BM rows and 256 columns (gate and up: 128
 // of each).
@@ -210,7 +217,7 @@ struct Product {
   bool vec;                 // rows of the bf16 tensors are whole 16-byte pieces
   bf16_t* O0;               // C;  GATE_UP: g (optional);  BWD: d_g
   bf16_t* O1;               //     GATE_UP: u (optional);  BWD: d_u
-  bf16_t* O2;               //                             BWD: h (BWD_SCALED: score * h)
+  bf16_t* O2;               //                             BWD: h (BWD_SCALED: score * h);  with TRANSPOSED the transposed copies
   uint8_t* Q[2];            //     GATE_UP: h;             BWD: d_g, d_u   in blocks
   uint8_t* Qs[2];
   const bf16_t* G;          // BWD: g and u of the forward
@@ -316,6 +323,31 @@ __device__ __forceinline__ void load16(const bf16_t* p, int have, bool vec, bf16
 __device__ __forceinline__ float held(float v) { return (float)(bf16_t)v; }
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
+// A wave's way of 32 rows x 128 columns of bf16 to 128 columns of 32 rows.  16-byte pieces of a row are XOR-ed with a mix of the row's bits
+// that keeps 16 neighbouring rows' writes and the four rows of each of two groups of a transposing read on banks of their own.
+constexpr int TR_BYTES = 32 * 128 * 2;
+typedef short shortx4_t __attribute__((ext_vector_type(4)));
+typedef short shortx8_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ int tr_swz(int r) { return (r & 3) << 1 | (r >> 2 & 1) | (r & 8); }
+__device__ __forceinline__ void put_row(char* t, int row, int piece, bf16x8_t v) {
+  *reinterpret_cast<bf16x8_t*>(t + row * 256 + ((piece ^ tr_swz(row)) << 4)) = v;
+}
+__device__ __forceinline__ void store_columns(const char* t, int lane, bf16_t* to) {
+  // within 16 lanes, lane i points at 4 neighbouring columns of row i / 4 and receives 4 neighbouring rows of column i
+  const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    shortx4_t half[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = 8 * g + 4 * h + (i >> 2), col = 16 * c + 4 * (i & 3);
+      half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) shortx4_t*)(t + row * 256 + (((col >> 3) ^ tr_swz(row)) << 4) + (col & 7) * 2));
+    }
+    *reinterpret_cast<shortx8_t*>(to + (16 * c + i) * 32 + 8 * g) = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
 constexpr int unit_chunk = 16;
 __device__ __forceinline__ int unit_of_block(int b) {      // neighbouring units on one XCD
   const int x = b % pk_rules::NXCD, q = b / pk_rules::NXCD;
@@ -323,7 +355,9 @@ __device__ __forceinline__ int unit_of_block(int b) {      // neighbouring units
 }
 
 // WM x 2 waves of 64 x 128 outputs; NS k-tiles of KB bytes a row in the ring.
-template <int WM, int KB, int NS, int EPI, bool VEC>
+// TRANSPOSED (BWD, whole blocks of columns): O0 to O2 are the transposed copies that pk_grouped_swiglu_wgrad_scaled_t reads,
+// [padded rows / 32][N][32], expert e's rows from (begin & ~63) + 64 e on, zeros behind its last row up to the end of its last block.
+template <int WM, int KB, int NS, int EPI, bool VEC, bool TRANSPOSED>
 __global__ __launch_bounds__(128 * WM, 2) void product_kernel(const Product p) {
   constexpr int NT = 128 * WM, BM = 64 * WM, BN = 256, TM = 2, TN = 4;
   constexpr int PIECES = KB / 16, LA = BM * PIECES / NT, LB = BN * PIECES / NT, L = LA + LB;
@@ -371,8 +405,7 @@ __global__ __launch_bounds__(128 * WM, 2) void product_kernel(const Product p) {
     for (int i = 0; i < LA; ++i) dma16(a_off[i], a, at + i * NT * 16);
 #pragma unroll
     for (int i = 0; i < LB; ++i) {
-      static_assert(64 * PIECES % NT == 0 || EPI != GATE_UP, "the 64 rows of one matrix are whole passes of the workgroup");
-      const int which = EPI == GATE_UP ? i * NT / (64 * PIECES) & 1 : seg;
+      const int which = EPI == GATE_UP ? (i * NT + wave * 64) / (64 * PIECES) & 1 : seg;
       dma16(b_off[i], uniform(p.B[which] + e * p.strideB + k), at + A_BYTES + i * NT * 16);
     }
   };
@@ -457,6 +490,7 @@ __global__ __launch_bounds__(128 * WM, 2) void product_kernel(const Product p) {
   // A lane and the one 32 further have the 32 columns of a row of acc[i][j], in fours; after exchanging halves of them each has 16
   // neighbouring ones, so that loads and stores are 16 bytes wide without a way through the LDS, and the wave's 128
   // columns of a row, a block, are in these two lanes.
+  if (TRANSPOSED) __syncthreads();           // the ring has been read
   if (!wave_has_rows && EPI != GATE_UP) return;
   const int half16 = (lane >> 5) * 16;
 #pragma unroll
@@ -524,6 +558,11 @@ __global__ __launch_bounds__(128 * WM, 2) void product_kernel(const Product p) {
         load16(up + n, p.N - n, VEC, us[j & 1]);
       };
       request(0);
+      static_assert(!TRANSPOSED || 4 * TR_BYTES * WM <= NS * STAGE, "two tiles of 32 x 128 for every wave in the ring");
+      char* const tr = smem + wave * 2 * TR_BYTES;
+      if (TRANSPOSED && wm * 64 + 32 * i >= rows) break;              // (the same for the whole wave)
+      const int64_t padded = (begin & ~63) + 64 * (int64_t)e + mt * BM + wm * 64 + 32 * i;
+      const int64_t tr_at = (padded / 32 * p.N + nb * BLOCK) * 32;
       const float score = EPI == BWD_SCALED ? p.scores[p.row_map[row]] : 1.f;
       float ds = 0.f;
       uint32_t mg = 0u, mu = 0u;
@@ -541,9 +580,9 @@ __global__ __launch_bounds__(128 * WM, 2) void product_kernel(const Product p) {
           for (int v = 0; v < 8; ++v) {
             const float gv = (float)gs[j & 1][k][v], uv = (float)us[j & 1][k][v], a = f[j][8 * k + v];
             const float sg = sigmoid(gv), silu = gv * sg, hv = silu * uv, d = score * a;
-            const bool in = VEC ? have > 0 : have > v;
+            const bool in = TRANSPOSED ? live : VEC ? have > 0 : have > v;
             if (EPI == BWD_SCALED) ds += in ? a * hv : 0.f;
-            h[v] = score * hv;
+            h[v] = !TRANSPOSED || in ? score * hv : 0.f;
             const float dg = d * uv * (sg * (1.f + gv * (1.f - sg))), du = d * silu;
             g[v] = in ? held(dg) : 0.f;      // bf16 tensors, whose blocks are of what they hold
             u[v] = in ? held(du) : 0.f;
@@ -553,13 +592,25 @@ __global__ __launch_bounds__(128 * WM, 2) void product_kernel(const Product p) {
           asm volatile("" : "+v"(mg), "+v"(mu), "+v"(ds));      // step by step: as one reduction it would keep all values
           dgs[j][k] = kept(pack8(g));
           dus[j][k] = kept(pack8(u));
-          if (live) {
+          if constexpr (TRANSPOSED) {
+            put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, pack8(h));
+            put_row(tr + TR_BYTES, lane & 31, 4 * j + 2 * (lane >> 5) + k, dgs[j][k]);
+          } else if (live) {
             store8(p.O0 + row * p.N + n, have, VEC, dgs[j][k]);
             store8(p.O1 + row * p.N + n, have, VEC, dus[j][k]);
             store8(p.O2 + row * p.N + n, have, VEC, pack8(h));
           }
           __builtin_amdgcn_sched_barrier(0);
         }
+      }
+      if constexpr (TRANSPOSED) {
+        store_columns(tr, lane, p.O2 + tr_at);
+        store_columns(tr + TR_BYTES, lane, p.O0 + tr_at);
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, dus[j][k]);
+        store_columns(tr, lane, p.O1 + tr_at);
       }
       mg = umax(mg, other_half(mg));
       mu = umax(mu, other_half(mu));
@@ -586,7 +637,7 @@ __global__ __launch_bounds__(128 * WM, 2) void product_kernel(const Product p) {
 }
 
 template <int WM, int KB, int NS, int EPI>
-int launch_tiles(Product p, int64_t A, int kernel_id, hipStream_t s) {
+int launch_tiles(Product p, int64_t A, bool transposed, int kernel_id, hipStream_t s) {
   constexpr int BM = 64 * WM, STAGE = (BM + 256) * KB;
   p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP ? BLOCK : 256);
   p.by_n_tiles = pk_units::make_fastdiv(p.n_tiles);
@@ -610,13 +661,15 @@ int launch_tiles(Product p, int64_t A, int kernel_id, hipStream_t s) {
     PK_RETURN_IF_LAUNCH_FAILED();
     return PK_OK;
   };
-  static bool ready[2][PK_MAX_DEVICES] = {};
-  return p.vec ? launch(product_kernel<WM, KB, NS, EPI, true>, ready[1]) : launch(product_kernel<WM, KB, NS, EPI, false>, ready[0]);
+  static bool ready[3][PK_MAX_DEVICES] = {};
+  if constexpr (EPI == BWD || EPI == BWD_SCALED)
+    if (transposed) return launch(product_kernel<WM, KB, NS, EPI, true, true>, ready[2]);
+  return p.vec ? launch(product_kernel<WM, KB, NS, EPI, true, false>, ready[1]) : launch(product_kernel<WM, KB, NS, EPI, false, false>, ready[0]);
 }
 
 template <int EPI>
-int launch_product(const Product& p, int64_t A, int kernel_id, hipStream_t s) {
-  return launch_tiles<2, 64, 3, EPI>(p, A, kernel_id, s);
+int launch_product(const Product& p, int64_t A, int kernel_id, hipStream_t s, bool transposed = false) {
+  return launch_tiles<2, 64, 3, EPI>(p, A, transposed, kernel_id, s);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -1054,11 +1107,10 @@ int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, co
   return launch_product<PLAIN>(p, A, pk_timing::K_FP8_DOWN, (hipStream_t)stream);
 }
 
-int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div, const float* scores,
+static int dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div, const float* scores,
                     const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u, const int32_t* plan, void* d_g, void* d_u, void* h,
                     uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H, int64_t I,
-                    int64_t E, pk_stream_t stream) {
-  if (const int rc = check(A, H, I, E)) return rc;
+                    int64_t E, bool transposed, pk_stream_t stream) {
   if (row_map_div < 1 || row_map_div > 0x7fffffffll) return PK_ERR_ARG;
   if (A == 0) return PK_OK;
   if (!all_set({d_y, d_y_scales, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales})) return PK_ERR_ARG;
@@ -1071,12 +1123,45 @@ int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t
   p.ld = blocks_of(H) * BLOCK; p.strideB = I * p.ld;
   p.bs_n = 1; p.bs_k = (int32_t)blocks_of(I); p.bs_e = blocks_of(H) * blocks_of(I);
   p.vec = bf16_pieces(I, {g, u, d_g, d_u, h});
+  if (transposed && !p.vec) return PK_ERR_ALIGN;
   p.O0 = (bf16_t*)d_g; p.O1 = (bf16_t*)d_u; p.O2 = (bf16_t*)h;
   p.Q[0] = d_g8; p.Qs[0] = d_g_scales; p.Q[1] = d_u8; p.Qs[1] = d_u_scales;
   p.G = (const bf16_t*)g; p.U = (const bf16_t*)u;
   p.scores = scores; p.ds_part = ds_part; p.total_rows = A;
-  return scores ? launch_product<BWD_SCALED>(p, A, pk_timing::K_FP8_DGRAD_DH, (hipStream_t)stream)
-                : launch_product<BWD>(p, A, pk_timing::K_FP8_DGRAD_DH, (hipStream_t)stream);
+  return scores ? launch_product<BWD_SCALED>(p, A, pk_timing::K_FP8_DGRAD_DH, (hipStream_t)stream, transposed)
+                : launch_product<BWD>(p, A, pk_timing::K_FP8_DGRAD_DH, (hipStream_t)stream, transposed);
+}
+
+int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div, const float* scores,
+                    const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u, const int32_t* plan, void* d_g, void* d_u, void* h,
+                    uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H, int64_t I,
+                    int64_t E, pk_stream_t stream) {
+  if (const int rc = check(A, H, I, E)) return rc;
+  return dgrad_dh(d_y, d_y_scales, row_map, row_map_div, scores, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales, ds_part, A,
+                  H, I, E, false, stream);
+}
+
+int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div, const float* scores,
+                      const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u, const int32_t* plan, void* d_gT, void* d_uT, void* hT,
+                      int64_t ldt, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H,
+                      int64_t I, int64_t E, pk_stream_t stream) {
+  if (const int rc = check(A, H, I, E)) return rc;
+  const int64_t need = pk_grouped_swiglu_transposed_ld(A, H, I, E, PK_BF16);
+  if (need <= 0) return PK_ERR_SHAPE;
+  if (A > 0 && (ldt < need || ldt % 64 != 0)) return PK_ERR_ARG;
+  return dgrad_dh(d_y, d_y_scales, row_map, row_map_div, scores, w2_t, s2, g, u, plan, d_gT, d_uT, hT, d_g8, d_g_scales, d_u8, d_u_scales, ds_part, A,
+                  H, I, E, true, stream);
+}
+
+int pk_fp8_row_map(const int32_t* plan, int64_t E, int64_t A, int32_t* row_map, pk_stream_t stream) {
+  if (A < 0 || E <= 0) return PK_ERR_ARG;
+  if (E > PK_MAX_EXPERTS || A > 0x7fffffffll) return PK_ERR_SHAPE;
+  if (A == 0) return PK_OK;
+  if (!plan || !row_map) return PK_ERR_ARG;
+  PK_LAUNCH_NOCHECK(pk_timing::K_MISC, (hipStream_t)stream, row_map_kernel, dim3((unsigned)pk_ceil_div(A, THREADS)), dim3(THREADS), 0,
+                    (hipStream_t)stream, plan + E, A, row_map);
+  PK_RETURN_IF_LAUNCH_FAILED();
+  return PK_OK;
 }
 
 int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales, const uint8_t* w1_t,
@@ -1099,7 +1184,10 @@ int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_
 
 int pk_fp8_few_rows_pays(int64_t A, int64_t H, int64_t I, int64_t E) {
   if (check(A, H, I, E) != PK_OK || A == 0) return 0;
-  return A <= 8 * E;
+  // us, this -> tiles (without the zeros behind the last row, 4 us): 128 experts 2048 x 768: 8 rows an expert 164 -> 187, 12 rows 183 ->
+  // 187, 16 rows 236 -> 187; with few workgroups the tiles cannot be filled: 8 experts 2048 x 768: 4 rows 24 -> 50, 16 rows 34 -> 51,
+  // 32 rows 42 -> 53; 24 experts 1000 x 360: 4 rows 26 -> 38, 16 rows 35 -> 38, 32 rows 51 -> 40
+  return A <= 12 * E || (A <= 20 * E && E * blocks_of(I) <= 96);
 }
 
 int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64, const uint8_t* w1, const uint8_t* s1, const uint8_t* w2,

@@ -1057,20 +1057,37 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
                  us = b.add(scales(A, I));
     b.allocate(x);
     const auto p = [&](size_t pos) { return static_cast<uint8_t*>(b.at_(pos)); };
-    Tensor dguh = at::empty({3, A, I}, x.options()), d_x;      // d_g, d_u, h
+    // d_g, d_u, h for the weight gradients: row-major, or with more rows an expert as the transposed copies that their faster kernels
+    // read (the line is that of the region's backward)
+    const bool any_w = n1 || n2 || n3;
+    const int64_t ldt = any_w && A > 40 * E && pk_region_transposed_pays(A, H, I, E, PK_BF16) ? pk_grouped_swiglu_transposed_ld(A, H, I, E, PK_BF16) : 0;
+    const int64_t copy = ldt > 0 ? ldt * I * 2 : step;
+    Tensor dguh = at::empty({3 * copy / 2}, x.options()), map, d_x;
     char* const dg = static_cast<char*>(dguh.data_ptr());
     PK_CALL(pk_fp8_quantize_rows, ptr(d_y), PK_BF16, nullptr, 1, p(y8), p(ys), A, H, st);
-    PK_CALL(pk_fp8_dgrad_dh, p(y8), p(ys), nullptr, 1, nullptr, u8(t2), u8(s2), g, g + step, at, dg, dg + step, dg + 2 * step, p(g8), p(gs), p(u8_),
-            p(us), nullptr, A, H, I, E, st);
+    if (ldt > 0) {
+      map = at::empty({A}, starts.options());
+      PK_CALL(pk_fp8_row_map, at, E, A, map.data_ptr<int32_t>(), st);
+      PK_CALL(pk_fp8_dgrad_dh_t, p(y8), p(ys), nullptr, 1, nullptr, u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, ldt, p(g8), p(gs),
+              p(u8_), p(us), nullptr, A, H, I, E, st);
+    } else {
+      PK_CALL(pk_fp8_dgrad_dh, p(y8), p(ys), nullptr, 1, nullptr, u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, p(g8), p(gs), p(u8_),
+              p(us), nullptr, A, H, I, E, st);
+    }
     if (nx) {
       d_x = at::empty({A, H}, x.options());
       PK_CALL(pk_fp8_dgrad_dx, p(g8), p(gs), p(u8_), p(us), u8(t1), u8(s1), u8(t3), u8(s3), at, ptr(d_x), A, H, I, E, st);
       zero_tail(d_x, starts, E);
     }
-    const auto wgrad = [d_y, dguh, x, starts, A, H, I, E, step](const Tensor& d1, const Tensor& d2, const Tensor& d3, bool accumulate) {
+    const auto wgrad = [d_y, dguh, map, x, starts, A, H, I, E, ldt, copy](const Tensor& d1, const Tensor& d2, const Tensor& d3, bool accumulate) {
       char* const ds = static_cast<char*>(dguh.data_ptr());
-      PK_CALL(pk_grouped_swiglu_wgrad, ptr(d_y), ds + 2 * step, ds, ds + step, ptr(x), nullptr, 1, starts.data_ptr<int32_t>(), nullptr, ptr(d1),
-              ptr(d2), ptr(d3), accumulate, A, H, I, E, PK_BF16, stream_of(x));
+      const int32_t* const at = starts.data_ptr<int32_t>();
+      if (ldt > 0)
+        PK_CALL(pk_grouped_swiglu_wgrad_scaled_t, ptr(d_y), ds + 2 * copy, ds, ds + copy, ldt, ptr(x), map.data_ptr<int32_t>(), 1, at, nullptr, ptr(d1),
+                ptr(d2), ptr(d3), accumulate, A, H, I, E, PK_BF16, stream_of(x));
+      else
+        PK_CALL(pk_grouped_swiglu_wgrad, ptr(d_y), ds + 2 * copy, ds, ds + copy, ptr(x), nullptr, 1, at, nullptr, ptr(d1), ptr(d2), ptr(d3), accumulate,
+                A, H, I, E, PK_BF16, stream_of(x));
     };
     Tensor d1, d2, d3;
     if (n1 && n2 && n3 && g_deferring.load() && leaf(p1) && leaf(p2) && leaf(p3)) {

@@ -56,6 +56,19 @@ def test_products(p):
         assert list(calls(A, H, I, E)) == [want] * 4, (A, H, I, E)
     assert list(calls(1, 128, 128, 1, None)) == [ARG] * 4
     assert list(calls(1, 128, 128, 1, p + 8)) == [ALIGN] * 4
+    def dh_t(ldt, H=256, I=256, A=10, q=p):
+        return lib.pk_fp8_dgrad_dh_t(q, p, None, 1, None, p, p, p, p, p, p, p, p, ldt, p, p, p, p, None, A, H, I, 2, None)
+
+    enough = lib.pk_grouped_swiglu_transposed_ld(10, 256, 256, 2, _lib.PK_BF16)
+    assert dh_t(enough, H=128) == SHAPE and dh_t(enough, I=384) == SHAPE and dh_t(enough - 64) == ARG and dh_t(enough + 1) == ARG
+    assert dh_t(enough, q=None) == ARG and dh_t(enough, q=p + 8) == ALIGN and dh_t(enough, A=0) == 0 and dh_t(enough, A=-1) == ARG
+    assert lib.pk_fp8_row_map(p, 0, 4, p, None) == ARG and lib.pk_fp8_row_map(p, 4, -1, p, None) == ARG and lib.pk_fp8_row_map(None, 4, 4, p, None) == ARG
+    assert lib.pk_fp8_row_map(p, 1025, 4, p, None) == SHAPE and lib.pk_fp8_row_map(None, 4, 0, None, None) == 0
+    # few rows
+    few = lambda A=4, H=128, I=128, E=2, x=p, g=p, u=p, w=p: lib.pk_fp8_experts_few_rows(x, p, 0, w, p, p, p, p, p, g, u, p, p, A, H, I, E, None)  # noqa: E731
+    assert few(A=-1) == ARG and few(H=0) == ARG and few(x=None) == ARG and few(g=None) == ARG and few(w=p + 8) == ALIGN and few(H=8200) == SHAPE
+    assert few(A=0) == 0 and lib.pk_fp8_few_rows_pays(0, 128, 128, 4) == 0 and lib.pk_fp8_few_rows_pays(8, 0, 128, 4) == 0
+    assert lib.pk_fp8_few_rows_pays(8, 2048, 768, 128) == 1 and lib.pk_fp8_few_rows_pays(32768, 2048, 768, 128) == 0
     # one of gate and up alone, a divisor without sense, scores without a map or without their sums
     assert lib.pk_fp8_gate_up(p, p, None, 1, p, p, p, p, p, p, None, p, p, 1, 128, 128, 1, None) == ARG
     assert lib.pk_fp8_gate_up(p, p, None, 0, p, p, p, p, p, p, p, p, p, 1, 128, 128, 1, None) == ARG

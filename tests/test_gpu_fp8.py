@@ -110,6 +110,7 @@ SHAPES = [
     (3, 384, 512, [255, 256, 129], 1, "around a tile's rows"),
     (2, 257, 300, [30, 12], 0, "odd widths of two and three blocks"),
     (70, 128, 128, [i % 4 for i in range(70)], 0, "more experts than lanes"),
+    (4, 256, 512, [200, 33, 0, 64], 7, "weight gradients from transposed copies if that pays"),
 ]
 
 
@@ -253,6 +254,53 @@ def test_empty_input(dev):
     assert got[0].shape == (0, 256) and all((t == 0).all() for t in got[1:4]) and got[4].shape == (0, 256)
     got = _pass(w, x, d_y, n)                              # rows, but nobody's
     assert all((t == 0).all() for t in got)
+
+
+@pytest.mark.parametrize("counts,spare", [([45, 0, 64, 131], 70), ([1, 500, 31, 32], 0), ([0, 0, 0, 200], 3)])
+def test_transposed_copies_give_the_same_weight_gradients(dev, counts, spare):
+    """pk_fp8_dgrad_dh_t with pk_fp8_row_map and pk_grouped_swiglu_wgrad_scaled_t against the row-major pair.  What stands in rows of no
+    expert does not matter."""
+    print(f"[case] fp8 d_h, transposed copies, {counts}", flush=True)
+    lib, E, H, I = _lib.load(), 4, 512, 256
+    A, st = sum(counts) + spare, _lib.current_stream(dev)
+    w1, w2, w3, x, d_y = (t.to(dev) for t in _inputs(E, H, I, counts, spare, 3, False))
+    x[sum(counts):] = math.nan
+    d_y[sum(counts):] = math.inf
+    e = F_.quantize_experts(w1, w2, w3)
+    gu = (torch.randn(2, A, I, generator=torch.Generator().manual_seed(1))).bfloat16().to(dev)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    n = torch.tensor(counts, dtype=torch.int32, device=dev)
+    plan = torch.empty(lib.pk_fp8_plan_bytes(A, E) // 4, dtype=torch.int32, device=dev)
+    assert lib.pk_fp8_plan(p(n), 0, E, A, p(plan), st) == 0
+    q, s = ops.quantize_rows_fp8(d_y)
+    ldt = lib.pk_grouped_swiglu_transposed_ld(A, H, I, E, _lib.PK_BF16)
+    sides = []
+    for transposed in (False, True):
+        codes = [torch.zeros(A, I, dtype=torch.uint8, device=dev) for _ in range(2)] + [torch.zeros(A, I // 128, dtype=torch.uint8, device=dev) for _ in range(2)]
+        g8, u8, gs, us = codes
+        copies = torch.full((3, ldt if transposed else A, I), math.nan, device=dev).bfloat16()
+        args = (p(q), p(s), None, 1, None, p(e.t2), p(e.s2), p(gu[0]), p(gu[1]), p(plan), p(copies[0]), p(copies[1]), p(copies[2]))
+        tail = (p(g8), p(gs), p(u8), p(us), None, A, H, I, E, st)
+        d1, d2, d3 = (torch.empty(s_, device=dev).bfloat16() for s_ in ((E, I, H), (E, H, I), (E, I, H)))
+        if transposed:
+            row_map = torch.empty(A, dtype=torch.int32, device=dev)
+            assert lib.pk_fp8_row_map(p(plan), E, A, p(row_map), st) == 0
+            assert row_map.tolist() == [min(r, sum(counts) - 1) for r in range(A)]
+            assert lib.pk_fp8_dgrad_dh_t(*args, ldt, *tail) == 0
+            assert lib.pk_grouped_swiglu_wgrad_scaled_t(p(d_y), p(copies[2]), p(copies[0]), p(copies[1]), ldt, p(x), p(row_map), 1, p(plan), None, p(d1),
+                                                        p(d2), p(d3), 0, A, H, I, E, _lib.PK_BF16, st) == 0
+        else:
+            assert lib.pk_fp8_dgrad_dh(*args, *tail) == 0
+            assert lib.pk_grouped_swiglu_wgrad(p(d_y), p(copies[2]), p(copies[0]), p(copies[1]), p(x), None, 1, p(plan), None, p(d1), p(d2), p(d3), 0, A, H,
+                                               I, E, _lib.PK_BF16, st) == 0
+        sides.append((codes, (d1, d2, d3)))
+    for a, b in zip(*(side[0] for side in sides)):
+        assert torch.equal(a, b)
+    for a, b in zip(*(side[1] for side in sides)):
+        # the same bf16 operands, summed in another order: both are within the rounding of the result and of n sums
+        assert torch.isfinite(a).all()
+        size = a.double().abs() + 2.0 ** -20 * max(counts) * a.double().abs().max()
+        assert ((a.double() - b.double()).abs() <= 2.0 ** -7 * size).all()
 
 
 def test_accumulated_and_postponed_weight_gradients(dev):
