@@ -430,7 +430,8 @@ PK_API int pk_sched_slot_index(int device, uint64_t stream_handle, uint64_t capt
  * values of a row; weights: 128 x 128), held as its biased exponent: value = code * 2^(byte - 127).  The
  * byte is the smallest, from 1 on, with which the block's largest magnitude is at most 448 in codes; codes
  * round to nearest even; a block with an infinity or a NaN is NaN throughout.  With w' = ceil(w / 128) * 128:
- *   rows     q [R][K'] (zeros behind K), scales [R][K'/128]
+ *   rows     q [R][K'] (zeros behind K), scales [R][S], S = K'/128 rounded up to a multiple of 4 (what stands behind
+ *            K'/128 is neither written nor used), 4-byte aligned
  *   weights  q [E][N][K'], scales [E][N'/128][K'/128]; transposed codes q_t [E][K][N'] share the scales
  * Code buffers must be 16-byte aligned.  The products take bf16 tensors of any width up to
  * H = PK_FP8_MAX_HIDDEN, I = PK_FP8_MAX_INTER; an operand's codes must span less than 4 GiB
@@ -456,12 +457,10 @@ PK_API int64_t pk_fp8_plan_bytes(int64_t A, int64_t E);
 PK_API int pk_fp8_plan(const void* counts, int counts_is_i64, int64_t E, int64_t A, int32_t* plan, pk_stream_t stream);
 
 /* g = x . w1[e]^T, u = x . w3[e]^T (both bf16 [A, I], or both NULL where no backward follows), and
- * h = silu(g) * u of what g and u hold, in blocks.  Operand row r is x[r], or x[row_map[r] / row_map_div];
- * the rows that the map can name are the first ceil(A / row_map_div). */
-PK_API int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const int32_t* row_map, int64_t row_map_div,
-                   const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3, const int32_t* plan,
-                   void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E,
-                   pk_stream_t stream);
+ * h = silu(g) * u of what g and u hold, in blocks. */
+PK_API int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w1, const uint8_t* s1,
+                   const uint8_t* w3, const uint8_t* s3, const int32_t* plan, void* g, void* u, uint8_t* h,
+                   uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
 /* y[A, H] (bf16) = h . w2[e]^T */
 PK_API int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2,
                 const int32_t* plan, void* y, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
@@ -475,22 +474,17 @@ PK_API int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts
                             float* h, void* y, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
 /* d_h = d_y . w2[e] (w2_t: the transposed codes) in fp32, and from it d_g = d_h * u * silu'(g) and
  * d_u = d_h * silu(g), both bf16 [A, I] (for pk_grouped_swiglu_wgrad) and in blocks (for pk_fp8_dgrad_dx), and
- * h = silu(g) * u (bf16).  With scores (f32, of every routed slot) and row_map, as
- * pk_grouped_swiglu_dgrad_dh_scaled: d_y is d_out, operand row r is d_out[row_map[r] / row_map_div], d_h is
- * multiplied by scores[row_map[r]], so is h, and ds_part [ceil(I / 128)][A] receives the parts of
- * <d_out . w2, silu(g) * u> that pk_region_router_bwd adds up. */
-PK_API int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div,
-                    const float* scores, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
-                    const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales,
-                    uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H, int64_t I, int64_t E,
-                    pk_stream_t stream);
+ * h = silu(g) * u (bf16). */
+PK_API int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2,
+                    const void* g, const void* u, const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8,
+                    uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, int64_t A, int64_t H, int64_t I,
+                    int64_t E, pk_stream_t stream);
 /* The same with d_g, d_u and h as the transposed copies [ldt / 32][I][32] of pk_grouped_swiglu_dgrad_dh_scaled_t (which
  * see), for pk_grouped_swiglu_wgrad_scaled_t: the faster pair with more than about 40 rows an expert.  ldt and the shapes that
  * have such a path: pk_grouped_swiglu_transposed_ld. */
-PK_API int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div,
-                      const float* scores, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
-                      const int32_t* plan, void* d_gT, void* d_uT, void* hT, int64_t ldt, uint8_t* d_g8,
-                      uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H,
+PK_API int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2,
+                      const void* g, const void* u, const int32_t* plan, void* d_gT, void* d_uT, void* hT, int64_t ldt,
+                      uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, int64_t A, int64_t H,
                       int64_t I, int64_t E, pk_stream_t stream);
 /* row_map[r] = r for rows of an expert, the last such row for the others: the row map (divisor 1) of
  * pk_grouped_swiglu_wgrad_scaled_t where the rows are sorted already. */

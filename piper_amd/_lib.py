@@ -110,12 +110,12 @@ SIGNATURES = {
     "pk_fp8_plan_bytes": (_c_i64, [_c_i64, _c_i64]),
     "pk_fp8_plan": (_c_int, [_p, _c_int, _c_i64, _c_i64, _p, _p]),
     # ... A H I E stream
-    "pk_fp8_gate_up": (_c_int, [_p, _p, _p, _c_i64, *[_p] * 9, *[_c_i64] * 4, _p]),
+    "pk_fp8_gate_up": (_c_int, [*[_p] * 11, *[_c_i64] * 4, _p]),
     "pk_fp8_down": (_c_int, [*[_p] * 6, *[_c_i64] * 4, _p]),
     "pk_fp8_few_rows_pays": (_c_int, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "pk_fp8_experts_few_rows": (_c_int, [_p, _p, _c_int, *[_p] * 10, *[_c_i64] * 4, _p]),
-    "pk_fp8_dgrad_dh": (_c_int, [_p, _p, _p, _c_i64, *[_p] * 14, *[_c_i64] * 4, _p]),
-    "pk_fp8_dgrad_dh_t": (_c_int, [_p, _p, _p, _c_i64, *[_p] * 9, _c_i64, *[_p] * 5, *[_c_i64] * 4, _p]),
+    "pk_fp8_dgrad_dh": (_c_int, [*[_p] * 14, *[_c_i64] * 4, _p]),
+    "pk_fp8_dgrad_dh_t": (_c_int, [*[_p] * 10, _c_i64, *[_p] * 4, *[_c_i64] * 4, _p]),
     "pk_fp8_row_map": (_c_int, [_p, _c_i64, _c_i64, _p, _p]),
     "pk_fp8_dgrad_dx": (_c_int, [*[_p] * 10, *[_c_i64] * 4, _p]),
     # master m m_scale v v_scale grad shadow shadow_dtype n lr b1 b2 eps wd step seed grad_scale zero_grad stream

@@ -14,6 +14,8 @@ constexpr int THREADS = 256;
 using pk_units::FastDiv;
 
 inline int64_t blocks_of(int64_t n) { return pk_ceil_div(n, BLOCK); }
+// bytes of a row of scales: whole words
+__host__ __device__ inline int scale_row(int blocks) { return (blocks + 3) & ~3; }
 
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int have, bool vec, float (&f)[8]) {
@@ -50,7 +52,7 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T* __restr
   uint32_t codes[2], byte;
   pk_fp8::quantize8(f, codes, byte);
   *reinterpret_cast<u32x2_t*>(q + unit * BLOCK + lane * 8) = u32x2_t{codes[0], codes[1]};
-  if (lane == 0) s[unit] = (uint8_t)byte;
+  if (lane == 0) s[(int64_t)r * scale_row(kb) + b] = (uint8_t)byte;
 }
 
 // ------------------------------------------------------------------------------------------------ weights
@@ -195,18 +197,15 @@ __global__ __launch_bounds__(THREADS) void row_map_kernel(const int32_t* __restr
 }
 
 // ------------------------------------------------------------------------------------------------ products
-// C[rows_e, N] = sum_seg A_seg[rows_e, K] . B_seg[e][N, K]^T, one workgroup to a tile of BM rows and 256 columns (gate and up: 128
-// of each).
-enum Epilogue { PLAIN = 0, GATE_UP = 1, BWD = 2, BWD_SCALED = 3 };
+// C[rows_e, N] = sum_seg A_seg[rows_e, K] . B_seg[e][N, K]^T in tiles (units) of 128 rows and 256 columns (gate and up: 128 of each).
+enum Epilogue { PLAIN = 0, GATE_UP = 1, BWD = 2 };
 
 typedef int intx8_t __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 struct Product {
   const uint8_t* A[2];      // codes of the rows, by segment [., lda]
-  const uint8_t* As[2];     // and their scales [., kt]
-  const int32_t* row_map;   // optional gather: A row = row_map[sorted row] / map_div
-  FastDiv map_div;
+  const uint8_t* As[2];     // and their scales [., scale_row(kt)]
   const uint8_t* B[2];      // weights of a segment (GATE_UP: gate, up), rows of ld codes
   const uint8_t* Bs[2];     // scale of block (n, k) of expert e: Bs[e * bs_e + n * bs_n + k * bs_k]
   int64_t ld, strideB, bs_e;
@@ -217,28 +216,27 @@ struct Product {
   bool vec;                 // rows of the bf16 tensors are whole 16-byte pieces
   bf16_t* O0;               // C;  GATE_UP: g (optional);  BWD: d_g
   bf16_t* O1;               //     GATE_UP: u (optional);  BWD: d_u
-  bf16_t* O2;               //                             BWD: h (BWD_SCALED: score * h);  with TRANSPOSED the transposed copies
+  bf16_t* O2;               //                             BWD: h;  with TRANSPOSED the transposed copies
   uint8_t* Q[2];            //     GATE_UP: h;             BWD: d_g, d_u   in blocks
   uint8_t* Qs[2];
   const bf16_t* G;          // BWD: g and u of the forward
   const bf16_t* U;
-  const float* scores;      // BWD_SCALED: of every routed slot
-  float* ds_part;           //             [N / 128][total_rows]: the score gradient in parts
-  int64_t total_rows;
-  int32_t units, head;      // most units that a plan for as many rows can have; words in front of its table
+  int32_t head;             // words in front of the plan's table
 };
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(lds_ptr_t)p; }
 // 16 bytes per lane straight into LDS, lane l's at lds_base + 16 l, from a wave-uniform base and an offset per lane.  The
 // compiler does not see the transfer: dma_wait and a barrier stand before what reads it.
+__device__ __forceinline__ void dma4(uint32_t voff, const void* sbase, uint32_t lds_base) {      // lane l's 4 bytes at lds_base + 4 l
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_base), "v"(voff), "s"(sbase) : "memory");
+}
 __device__ __forceinline__ void dma16(uint32_t voff, const void* sbase, uint32_t lds_base) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_base), "v"(voff), "s"(sbase) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void block_barrier() {
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // what the wave has read of the LDS or written to it is done
 }
 __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
   const uint64_t v = (uint64_t)(uintptr_t)p;
@@ -246,19 +244,18 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
   return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
 }
 
-// A k-tile is KB bytes of every row: a block of 128, or half of one.  16-byte pieces of a row are XOR-ed with bits of the row, so that 16
-// neighbouring rows' pieces of one number cover the banks.
-template <int KB>
-__device__ __forceinline__ int swz(int r) { return KB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+// A k-tile is a block: 128 bytes of every row, a whole line of the caches (64 bytes at a time come at 39 bytes a cycle and CU out of
+// the L2, 128 at 65).  16-byte pieces of a row are XOR-ed with bits of the row, so that 16 neighbouring rows' pieces of one number
+// cover the banks.
+__device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 
 // 32 of the 64 reduction bytes of step `half` of a k-tile, for row row0 + lane % 32.  Both operands are dealt alike, and a
-// step has one scale, so it does not matter which lane holds which of them.
-template <int KB>
+// k-tile has one scale, so it does not matter which lane holds which of them.
 __device__ __forceinline__ intx8_t fragment(const char* tile, int row0, int half, int lane) {
   const int r = row0 + (lane & 31), c = 4 * half + 2 * (lane >> 5);
-  const char* const p = tile + r * KB;
-  const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(p + ((c ^ swz<KB>(r)) << 4));
-  const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(p + (((c + 1) ^ swz<KB>(r)) << 4));
+  const char* const p = tile + r * BLOCK;
+  const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(p + ((c ^ swz(r)) << 4));
+  const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(p + (((c + 1) ^ swz(r)) << 4));
   return intx8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
@@ -323,26 +320,26 @@ __device__ __forceinline__ void load16(const bf16_t* p, int have, bool vec, bf16
 __device__ __forceinline__ float held(float v) { return (float)(bf16_t)v; }
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
-// A wave's way of 32 rows x 128 columns of bf16 to 128 columns of 32 rows.  16-byte pieces of a row are XOR-ed with a mix of the row's bits
-// that keeps 16 neighbouring rows' writes and the four rows of each of two groups of a transposing read on banks of their own.
-constexpr int TR_BYTES = 32 * 128 * 2;
+// A wave's way of 32 rows x 64 columns of bf16 to 64 columns of 32 rows.  16-byte pieces of a row are XOR-ed with a mix of the row's bits
+// that spreads 8 neighbouring rows' writes, and the four rows of a group of a transposing read, over the banks.
+constexpr int TR_BYTES = 32 * 64 * 2;
 typedef short shortx4_t __attribute__((ext_vector_type(4)));
 typedef short shortx8_t __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ int tr_swz(int r) { return (r & 3) << 1 | (r >> 2 & 1) | (r & 8); }
+__device__ __forceinline__ int tr_swz(int r) { return ((r & 3) << 1 | (r >> 2 & 1)) ^ (r >> 3 & 1); }
 __device__ __forceinline__ void put_row(char* t, int row, int piece, bf16x8_t v) {
-  *reinterpret_cast<bf16x8_t*>(t + row * 256 + ((piece ^ tr_swz(row)) << 4)) = v;
+  *reinterpret_cast<bf16x8_t*>(t + row * 128 + ((piece ^ tr_swz(row)) << 4)) = v;
 }
 __device__ __forceinline__ void store_columns(const char* t, int lane, bf16_t* to) {
   // within 16 lanes, lane i points at 4 neighbouring columns of row i / 4 and receives 4 neighbouring rows of column i
   const int g = lane >> 4, i = lane & 15;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
+  for (int c = 0; c < 4; ++c) {
     shortx4_t half[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row = 8 * g + 4 * h + (i >> 2), col = 16 * c + 4 * (i & 3);
       half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) shortx4_t*)(t + row * 256 + (((col >> 3) ^ tr_swz(row)) << 4) + (col & 7) * 2));
+          (__attribute__((address_space(3))) shortx4_t*)(t + row * 128 + (((col >> 3) ^ tr_swz(row)) << 4) + (col & 7) * 2));
     }
     *reinterpret_cast<shortx8_t*>(to + (16 * c + i) * 32 + 8 * g) = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
   }
@@ -354,301 +351,339 @@ __device__ __forceinline__ int unit_of_block(int b) {      // neighbouring units
   return ((q / unit_chunk) * pk_rules::NXCD + x) * unit_chunk + (q % unit_chunk);
 }
 
-// WM x 2 waves of 64 x 128 outputs; NS k-tiles of KB bytes a row in the ring.
-// TRANSPOSED (BWD, whole blocks of columns): O0 to O2 are the transposed copies that pk_grouped_swiglu_wgrad_scaled_t reads,
+// One persistent workgroup to a CU, eight waves (2 x 4) of 64 x 64 outputs, a ring of three k-tiles.  A workgroup goes through its
+// units one after the other: behind a unit's last k-tile it requests the first two of the next one, and the epilogue, which
+// needs the LDS for the blocks' maxima alone, runs while they are on their way.
+// What bounds it: the memory takes 1.7 us to answer while the chip streams weights, in which a CU multiplies 2.5 k-tiles, and the ring
+// holds three; 128 rows and 256 columns are what fits it.  128 experts of 2048 x 768 with 512 rows each, us, against two workgroups of
+// four waves to a CU with half-block k-tiles: gate and up 363 : 376, down 225 : 261, d_h (row-major copies) 326 : 354; with 111 rows
+// each 105 : 110 and 64 : 68, which is 4.2 TB/s.  Dealing neighbouring units by 8, 16 or 32 to an XCD made no difference.
+// TRANSPOSED (BWD, N a multiple of 256): O0 to O2 are the transposed copies that pk_grouped_swiglu_wgrad_scaled_t reads,
 // [padded rows / 32][N][32], expert e's rows from (begin & ~63) + 64 e on, zeros behind its last row up to the end of its last block.
-template <int WM, int KB, int NS, int EPI, bool VEC, bool TRANSPOSED>
-__global__ __launch_bounds__(128 * WM, 2) void product_kernel(const Product p) {
-  constexpr int NT = 128 * WM, BM = 64 * WM, BN = 256, TM = 2, TN = 4;
-  constexpr int PIECES = KB / 16, LA = BM * PIECES / NT, LB = BN * PIECES / NT, L = LA + LB;
-  constexpr int A_BYTES = BM * KB, STAGE = A_BYTES + BN * KB;
-  constexpr int PER_BLOCK = BLOCK / KB;      // k-tiles of a block
+constexpr int NT = 512, BM = TILE_ROWS, BN = 256, STAGES = 3, A_BYTES = BM * BLOCK, STAGE = A_BYTES + BN * BLOCK;
+inline int product_lds(int nblk4) { return STAGES * STAGE + nblk4 * BM + 2 * nblk4; }
+
+template <int EPI, bool VEC, bool TRANSPOSED>
+__global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
+  constexpr int TM = 2, TN = 2, LA = BM * 8 / NT, LB = BN * 8 / NT, L = LA + LB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
-  static_assert(BM == TILE_ROWS, "the plan's tiles");
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
+  const int kt4 = scale_row(p.kt), nblk = p.kt * p.nseg, n_blocks = (p.N + BLOCK - 1) / BLOCK, out4 = scale_row(n_blocks);
+  const int total = pk_units::as_const(p.plan)[p.E + 1] * p.n_tiles;
+  int step = blockIdx.x;
+  if (unit_of_block(step) >= total) return;
+  char* const sa = smem + STAGES * STAGE;    // scales of the unit's rows, [words of a row][128]
+  char* const sb = sa + kt4 * p.nseg * BM;   // and of its two blocks of columns (GATE_UP: gate, up), [2][nblk]
+
   // units of an expert are laid out [column tile][row tile]: neighbours share the weights
-  const int unit = unit_of_block(blockIdx.x);
-  if (unit >= p.units) return;
-  const pk_units::const_i32_ptr plan = pk_units::as_const(p.plan);
-  const pk_units::const_i32_ptr entry = plan + p.head + pk_units::fastdiv(unit, p.by_n_tiles) * ENTRY;
-  const int total = plan[p.E + 1], e = entry[0], first = entry[1], tiles = entry[2], begin = entry[3], end = entry[4];
-  if (unit >= total * p.n_tiles) return;
-  const int local = unit - first * p.n_tiles, nt = local / tiles, mt = local - nt * tiles;
-  const int row0 = begin + mt * BM, rows = min(BM, end - row0);
-  const int nblk = p.kt * p.nseg, nkt = nblk * PER_BLOCK;
-  const int n0 = nt * (EPI == GATE_UP ? BLOCK : BN);
+  int e = 0, nt = 0, mt = 0, begin = 0, rows = 0, row0 = 0, n0 = 0;
+  const auto take = [&](int unit, u32x4_t entry, int end) {
+    e = __builtin_amdgcn_readfirstlane((int)entry[0]);
+    const int first = __builtin_amdgcn_readfirstlane((int)entry[1]), tiles = __builtin_amdgcn_readfirstlane((int)entry[2]);
+    begin = __builtin_amdgcn_readfirstlane((int)entry[3]);
+    const int local = unit - first * p.n_tiles;
+    nt = __builtin_amdgcn_readfirstlane(local / tiles);
+    mt = local - nt * tiles;
+    row0 = begin + mt * BM;
+    rows = min(BM, __builtin_amdgcn_readfirstlane(end) - row0);
+    n0 = nt * (EPI == GATE_UP ? BLOCK : BN);
+  };
+  const auto entry_of = [&](int unit) { return p.plan + p.head + (int64_t)pk_units::fastdiv(unit, p.by_n_tiles) * ENTRY; };
 
   // Byte offsets of the 16-byte pieces that the thread brings; rows past the expert's end and columns past N read the tile's first
   // ones instead, and what comes of them is stored nowhere.
   uint32_t a_off[LA], b_off[LB];
-#pragma unroll
-  for (int i = 0; i < LA; ++i) {
-    const int s = tid + i * NT, r = s / PIECES, c = (s % PIECES) ^ swz<KB>(r);
-    int64_t src = row0 + (r < rows ? r : 0);
-    if (p.row_map) src = pk_units::fastdiv(p.row_map[src], p.map_div);
-    a_off[i] = (uint32_t)(src * p.ld + c * 16);
-  }
-#pragma unroll
-  for (int i = 0; i < LB; ++i) {
-    const int s = tid + i * NT, r = s / PIECES, c = (s % PIECES) ^ swz<KB>(r);
-    // GATE_UP: a wave has 64 columns of both: rows [64 gate | 64 up] for each of the two
-    const int n = n0 + (EPI == GATE_UP ? (r >> 7) * 64 + (r & 63) : r);
-    b_off[i] = (uint32_t)((int64_t)(n < p.N ? n : n0) * p.ld + c * 16);
-  }
-  const uint32_t ring = lds_addr(smem) + wave * 1024;
+  uint32_t scale_b = 0;                      // of the unit that comes next, on its way into sb
+  const uint32_t ring = lds_addr(smem) + wave * 1024, ring_sa = lds_addr(sa);
+  const auto source = [&](int r) { return (int64_t)row0 + (r < rows ? r : 0); };
   const auto fetch = [&](int kt, int stage) {
-    const int seg = kt >= p.kt * PER_BLOCK, k = (seg ? kt - p.kt * PER_BLOCK : kt) * KB;
+    const int seg = kt >= p.kt, k = (seg ? kt - p.kt : kt) * BLOCK;
     const uint8_t* const a = uniform(p.A[seg] + k);
+    // GATE_UP: a wave's 64 columns are 32 of gate and 32 of up, and so are the tile's rows of B
+    const uint8_t* const b = uniform(p.B[EPI == GATE_UP ? wave >> 2 & 1 : seg] + e * p.strideB + k);
     const uint32_t at = ring + stage * STAGE;
 #pragma unroll
     for (int i = 0; i < LA; ++i) dma16(a_off[i], a, at + i * NT * 16);
 #pragma unroll
-    for (int i = 0; i < LB; ++i) {
-      const int which = EPI == GATE_UP ? (i * NT + wave * 64) / (64 * PIECES) & 1 : seg;
-      dma16(b_off[i], uniform(p.B[which] + e * p.strideB + k), at + A_BYTES + i * NT * 16);
-    }
+    for (int i = 0; i < LB; ++i) dma16(b_off[i], b, at + A_BYTES + i * NT * 16);
   };
+  // everything that the k-loop of the unit taken needs, up to two k-tiles, the first one into `stage`
+  const auto start = [&](int stage) {
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s)
-    if (s < nkt) fetch(s, s);
-
-  // scales of the tile's rows and columns, behind the ring: a row of them is nblk bytes
-  char* const sa = smem + NS * STAGE;
-  const int sld = (nblk + 7) / 8 * 8 + 4;
-  char* const sb = sa + BM * sld;
-  const int n_blocks = (p.N + BLOCK - 1) / BLOCK;
-  {
-    const int r = tid >> 1, part = tid & 1;  // two threads to a row
-    int64_t src = row0 + (r < rows ? r : 0);
-    if (p.row_map) src = pk_units::fastdiv(p.row_map[src], p.map_div);
-    char* const to = sa + r * sld;
-    for (int seg = 0; seg < p.nseg; ++seg) {
-      const uint8_t* const from = p.As[seg] + src * p.kt;
-      if (p.kt % 16 == 0 && ((uintptr_t)p.As[seg] & 7) == 0) {      // rows are whole 16-byte pieces, 8 bytes for each of the two
-        for (int k = part * 8; k < p.kt; k += 16) {
-          const u32x2_t v = *reinterpret_cast<const u32x2_t*>(from + k);
-          *reinterpret_cast<uint32_t*>(to + seg * p.kt + k) = v[0];
-          *reinterpret_cast<uint32_t*>(to + seg * p.kt + k + 4) = v[1];
-        }
-      } else {
-#pragma unroll 4
-        for (int k = part; k < p.kt; k += 2) to[seg * p.kt + k] = (char)from[k];
-      }
+    for (int i = 0; i < LA; ++i) {
+      const int s = tid + i * NT, r = s >> 3;
+      a_off[i] = (uint32_t)(source(r) * p.ld + ((s & 7) ^ swz(r)) * 16);
     }
-    for (int i = tid; i < 2 * nblk; i += NT) {
-      const int b = i >= nblk, k = b ? i - nblk : i, seg = k >= p.kt;
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+      const int s = tid + i * NT, r = s >> 3;
+      const int n = n0 + (EPI == GATE_UP ? (r >> 6) * 32 + (r & 31) : r);
+      b_off[i] = (uint32_t)((int64_t)(n < p.N ? n : n0) * p.ld + ((s & 7) ^ swz(r)) * 16);
+    }
+    const uint32_t s_off = (uint32_t)(source((wave & 1) * 64 + lane) * kt4);
+    for (int w = wave; w < kt4 / 2 * p.nseg; w += 8) {      // words of scales, 64 rows at a time
+      const int seg = w >= kt4 / 2, d = (seg ? w - kt4 / 2 : w) >> 1;
+      dma4(s_off, uniform(p.As[seg] + d * 4), ring_sa + w * 256);
+    }
+    if (tid < 2 * nblk) {
+      const int b = tid >= nblk, k = b ? tid - nblk : tid, seg = k >= p.kt;
       const int nb = EPI == GATE_UP ? nt : min(2 * nt + b, n_blocks - 1);
-      sb[i] = (char)p.Bs[EPI == GATE_UP ? b : seg][e * p.bs_e + (int64_t)nb * p.bs_n + (int64_t)(seg ? k - p.kt : k) * p.bs_k];
+      scale_b = p.Bs[EPI == GATE_UP ? b : seg][e * p.bs_e + (int64_t)nb * p.bs_n + (int64_t)(seg ? k - p.kt : k) * p.bs_k];
     }
-  }
+    fetch(0, stage);
+    if (nblk > 1) fetch(1, stage == STAGES - 1 ? 0 : stage + 1);
+  };
 
-  floatx16_t acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
-  __syncthreads();                           // the scales are there
-  const bool wave_has_rows = wm * 64 < rows;
+  {
+    const int unit = unit_of_block(step);
+    const int32_t* const entry = entry_of(unit);
+    take(unit, *reinterpret_cast<const u32x4_t*>(entry), entry[4]);
+  }
   int stage = 0;
-  for (int kt = 0; kt < nkt; ++kt) {
-    // all but the youngest NS - 2 k-tiles have landed, everywhere; the stage that the next one goes to has been read
-    if (NS > 2 && kt + NS - 2 < nkt) dma_wait<(NS - 2) * L>();
-    else dma_wait<0>();
-    block_barrier();
-    const int next = stage == 0 ? NS - 1 : stage - 1;
-    if (kt + NS - 1 < nkt) fetch(kt + NS - 1, next);
-    if (wave_has_rows) {
-      const char* const at = smem + stage * STAGE;
-      const int scale_b = (unsigned char)sb[(EPI == GATE_UP ? 0 : wn * nblk) + kt / PER_BLOCK];
-      const int scale_u = EPI == GATE_UP ? (unsigned char)sb[nblk + kt / PER_BLOCK] : scale_b;
-      int scale_a[TM];
+  start(stage);
+  for (;;) {
+    if (tid < 2 * nblk) sb[tid] = (char)scale_b;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    floatx16_t acc[TM][TN];
 #pragma unroll
-      for (int i = 0; i < TM; ++i) scale_a[i] = (unsigned char)sa[(wm * 64 + i * 32 + (lane & 31)) * sld + kt / PER_BLOCK];
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int half = 0; half < KB / 64; ++half) {
-        intx8_t a[TM], b[TN];
+      for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int i = 0; i < TM; ++i) a[i] = fragment<KB>(at, wm * 64 + i * 32, half, lane);
+        for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+    const bool wave_has_rows = wm * 64 < rows;
+    step += gridDim.x;
+    const int next_unit = unit_of_block(step);
+    const bool more = next_unit < total;
+    u32x4_t next_entry = {};
+    int next_end = 0;
+    for (int kt = 0; kt < nblk; ++kt) {
+      // all but the youngest k-tile have landed, everywhere; the stage that the next one goes to has been read
+      if (kt + 1 < nblk) dma_wait<L>();
+      else dma_wait<0>();
+      block_barrier();
+      if (kt == 0 && more) {                 // (behind the wait for what it is not to hold up)
+        const int32_t* const entry = entry_of(next_unit);
+        next_entry = *reinterpret_cast<const u32x4_t*>(entry);
+        next_end = entry[4];
+      }
+      if (kt + 2 < nblk) fetch(kt + 2, stage == 0 ? STAGES - 1 : stage - 1);
+      if (wave_has_rows) {
+        const char* const at = smem + stage * STAGE;
+        const int seg = kt >= p.kt, k = seg ? kt - p.kt : kt;
+        const char* const sa_at = sa + (seg * kt4 + (k & ~3)) * BM + (k & 3) + (wm * 64 + (lane & 31)) * 4;
+        const int sc0 = (unsigned char)sb[(EPI == GATE_UP ? 0 : wn >> 1) * nblk + kt];
+        const int sc1 = EPI == GATE_UP ? (unsigned char)sb[nblk + kt] : sc0;
+        int scale_a[TM];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) b[j] = fragment<KB>(at + A_BYTES, wn * 128 + j * 32, half, lane);
+        for (int i = 0; i < TM; ++i) scale_a[i] = (unsigned char)sa_at[i * 128];
+        intx8_t a[2][TM], b[2][TN];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) a[half][i] = fragment(at, wm * 64 + i * 32, half, lane);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) b[half][j] = fragment(at + A_BYTES, wn * 64 + j * 32, half, lane);
+        }
         // operands swapped: a lane then holds 4 neighbouring columns of one row,
         //   acc[v] = C[row = lane % 32][col = 8 * (v / 4) + 4 * (lane / 32) + v % 4]
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int j = 0; j < TN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][j], 0, 0, 0, j < TN / 2 ? scale_b : scale_u, 0,
-                                                                        scale_a[i]);
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[half][j], a[half][i], acc[i][j], 0, 0, 0, j ? sc1 : sc0, 0, scale_a[i]);
       }
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
-    stage = stage == NS - 1 ? 0 : stage + 1;
-  }
+    block_barrier();                         // the scales and the last k-tile have been read
+    char* const spare = smem + (stage == 0 ? STAGES - 1 : stage - 1) * STAGE;      // its place, free until the next unit's third one
 
-  // A lane and the one 32 further have the 32 columns of a row of acc[i][j], in fours; after exchanging halves of them each has 16
-  // neighbouring ones, so that loads and stores are 16 bytes wide without a way through the LDS, and the wave's 128
-  // columns of a row, a block, are in these two lanes.
-  if (TRANSPOSED) __syncthreads();           // the ring has been read
-  if (!wave_has_rows && EPI != GATE_UP) return;
-  const int half16 = (lane >> 5) * 16;
+    // The unit that is stored from here on, while the next one is taken.
+    const int u_e = e, u_rows = rows, u_row0 = row0, u_n0 = n0, u_nt = nt, u_begin = begin, u_mt = mt;
+    const int half16 = (lane >> 5) * 16;
+    // BWD: the wave's part of g and u, requested before the next unit's k-tiles, which would be waited for as well
+    bf16x8_t gs[TM][TN][2], us[TM][TN][2];
+    if constexpr (EPI == BWD) {
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    asm volatile("" ::: "memory");           // the second half's loads and addresses not before the first half has left its registers
-    __builtin_amdgcn_sched_barrier(0);
-    const int r = wm * 64 + 32 * i + (lane & 31);
-    const bool live = r < rows;              // the same in both lanes of a row
-    float f[TN][16];                         // (scalars: a vector keeps its 16 registers until its last element has been used)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) exchange_halves(acc[i][j], f[j]);
-    const int64_t row = row0 + (live ? r : 0);
-    if constexpr (EPI == PLAIN) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int n = n0 + wn * 128 + 32 * j + half16;
-        if (live) store16(p.O0 + row * p.N + n, p.N - n, VEC, f[j]);
-      }
-    } else if constexpr (EPI == GATE_UP) {
-      // 64 columns of h here, 64 in the other wave of these rows
-      float h[2][16];
-      uint32_t m = 0u;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int n = n0 + wn * 64 + 32 * j + half16;
-        int have = p.N - n;
-        asm volatile("" : "+v"(have));       // compared here and not kept: such masks are more than there are scalar registers
-        float g[16], u[16];
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          g[v] = held(f[j][v]);     // g and u are bf16 tensors, written or not
-          u[v] = held(f[j + 2][v]);
-          h[j][v] = (VEC ? have > v / 8 * 8 : have > v) ? g[v] * sigmoid(g[v]) * u[v] : 0.f;
-          m = umax(m, __float_as_uint(h[j][v]) & 0x7fffffffu);
-        }
-        if (live && p.O0) {
-          store16(p.O0 + row * p.N + n, p.N - n, VEC, g);
-          store16(p.O1 + row * p.N + n, p.N - n, VEC, u);
-        }
-      }
-      m = umax(m, other_half(m));
-      uint32_t* const amax = reinterpret_cast<uint32_t*>(smem);      // [TM][2][BM / TM]
-      if (i == 0) __syncthreads();           // the ring has been read
-      amax[(i * 2 + wn) * 32 * WM + wm * 32 + (lane & 31)] = m;
-      __syncthreads();
-      m = umax(m, amax[(i * 2 + (wn ^ 1)) * 32 * WM + wm * 32 + (lane & 31)]);
-      const pk_fp8::BlockScale sc = pk_fp8::block_scale(m);
-      if (live) {
-        const int64_t block = row * n_blocks + nt;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) *reinterpret_cast<u32x4_t*>(p.Q[0] + block * BLOCK + wn * 64 + 32 * j + half16) = pk_fp8::codes16(h[j], sc);
-        if (wn == 0 && lane < 32) p.Qs[0][block] = (uint8_t)sc.byte;
-      }
-    } else {
-      const int nb = 2 * nt + wn;            // the wave's block of columns
-      if (nb >= n_blocks) return;            // (the same for the whole wave)
-      // g and u of 32 columns are requested while the 32 before them are worked on; what becomes of them takes the place of
-      // the accumulators
-      bf16x8_t gs[2][2], us[2][2], dgs[TN][2], dus[TN][2];
-      const bf16_t* const gp = p.G + row * p.N;
-      const bf16_t* const up = p.U + row * p.N;
-      const auto request = [&](int j) {
-        const int n = nb * BLOCK + 32 * j + half16;
-        load16(gp + n, p.N - n, VEC, gs[j & 1]);
-        load16(up + n, p.N - n, VEC, us[j & 1]);
-      };
-      request(0);
-      static_assert(!TRANSPOSED || 4 * TR_BYTES * WM <= NS * STAGE, "two tiles of 32 x 128 for every wave in the ring");
-      char* const tr = smem + wave * 2 * TR_BYTES;
-      if (TRANSPOSED && wm * 64 + 32 * i >= rows) break;              // (the same for the whole wave)
-      const int64_t padded = (begin & ~63) + 64 * (int64_t)e + mt * BM + wm * 64 + 32 * i;
-      const int64_t tr_at = (padded / 32 * p.N + nb * BLOCK) * 32;
-      const float score = EPI == BWD_SCALED ? p.scores[p.row_map[row]] : 1.f;
-      float ds = 0.f;
-      uint32_t mg = 0u, mu = 0u;
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        if (j + 1 < TN) request(j + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {        // eight columns at a time
-          const int n = nb * BLOCK + 32 * j + half16 + 8 * k;
-          int have = p.N - n;
-          asm volatile("" : "+v"(have));     // compared here and not kept: 64 such masks are more than there are scalar registers
-          float g[8], u[8], h[8];
-#pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            const float gv = (float)gs[j & 1][k][v], uv = (float)us[j & 1][k][v], a = f[j][8 * k + v];
-            const float sg = sigmoid(gv), silu = gv * sg, hv = silu * uv, d = score * a;
-            const bool in = TRANSPOSED ? live : VEC ? have > 0 : have > v;
-            if (EPI == BWD_SCALED) ds += in ? a * hv : 0.f;
-            h[v] = !TRANSPOSED || in ? score * hv : 0.f;
-            const float dg = d * uv * (sg * (1.f + gv * (1.f - sg))), du = d * silu;
-            g[v] = in ? held(dg) : 0.f;      // bf16 tensors, whose blocks are of what they hold
-            u[v] = in ? held(du) : 0.f;
-            mg = umax(mg, __float_as_uint(g[v]) & 0x7fffffffu);
-            mu = umax(mu, __float_as_uint(u[v]) & 0x7fffffffu);
-          }
-          asm volatile("" : "+v"(mg), "+v"(mu), "+v"(ds));      // step by step: as one reduction it would keep all values
-          dgs[j][k] = kept(pack8(g));
-          dus[j][k] = kept(pack8(u));
-          if constexpr (TRANSPOSED) {
-            put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, pack8(h));
-            put_row(tr + TR_BYTES, lane & 31, 4 * j + 2 * (lane >> 5) + k, dgs[j][k]);
-          } else if (live) {
-            store8(p.O0 + row * p.N + n, have, VEC, dgs[j][k]);
-            store8(p.O1 + row * p.N + n, have, VEC, dus[j][k]);
-            store8(p.O2 + row * p.N + n, have, VEC, pack8(h));
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-      if constexpr (TRANSPOSED) {
-        store_columns(tr, lane, p.O2 + tr_at);
-        store_columns(tr + TR_BYTES, lane, p.O0 + tr_at);
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, dus[j][k]);
-        store_columns(tr, lane, p.O1 + tr_at);
-      }
-      mg = umax(mg, other_half(mg));
-      mu = umax(mu, other_half(mu));
-      const pk_fp8::BlockScale scg = pk_fp8::block_scale(mg), scu = pk_fp8::block_scale(mu);
-      if (EPI == BWD_SCALED) ds += __uint_as_float(other_half(__float_as_uint(ds)));
-      if (live) {
-        const int64_t block = row * n_blocks + nb;
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          float g[16], u[16];
-#pragma unroll
-          for (int v = 0; v < 16; ++v) { g[v] = (float)dgs[j][v >> 3][v & 7]; u[v] = (float)dus[j][v >> 3][v & 7]; }
-          *reinterpret_cast<u32x4_t*>(p.Q[0] + block * BLOCK + 32 * j + half16) = pk_fp8::codes16(g, scg);
-          *reinterpret_cast<u32x4_t*>(p.Q[1] + block * BLOCK + 32 * j + half16) = pk_fp8::codes16(u, scu);
+          const int r = wm * 64 + 32 * i + (lane & 31), n = u_n0 + wn * 64 + 32 * j + half16;
+          const int64_t row = u_row0 + (r < u_rows ? r : 0);
+          load16(p.G + row * p.N + n, p.N - n, VEC, gs[i][j]);
+          load16(p.U + row * p.N + n, p.N - n, VEC, us[i][j]);
         }
-        if (lane < 32) {
-          p.Qs[0][block] = (uint8_t)scg.byte;
-          p.Qs[1][block] = (uint8_t)scu.byte;
-          if (EPI == BWD_SCALED) p.ds_part[(int64_t)nb * p.total_rows + row0 + r] = ds;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (more) {
+      take(next_unit, next_entry, next_end);
+      start(stage);
+    }
+
+    // A lane and the one 32 further have the 32 columns of a row of acc[i][j], in fours; after exchanging halves of them each has 16
+    // neighbouring ones, so that loads and stores are 16 bytes wide without a way through the LDS.
+    if constexpr (EPI == PLAIN) {
+      if (wave_has_rows) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const int r = wm * 64 + 32 * i + (lane & 31);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            float f[16];
+            exchange_halves(acc[i][j], f);
+            const int n = u_n0 + wn * 64 + 32 * j + half16;
+            if (r < u_rows) store16(p.O0 + (int64_t)(u_row0 + r) * p.N + n, p.N - n, VEC, f);
+          }
+        }
+      }
+    } else if constexpr (EPI == GATE_UP) {
+      // 32 columns of h in a wave, four waves to a block
+      const int n = u_n0 + wn * 32 + half16;
+      uint32_t* const amax = reinterpret_cast<uint32_t*>(spare);      // [4 waves][128 rows]
+      float h[TM][16];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int r = wm * 64 + 32 * i + (lane & 31);
+        const bool live = r < u_rows;        // the same in both lanes of a row
+        float g[16], u[16];
+        exchange_halves(acc[i][0], g);
+        exchange_halves(acc[i][1], u);
+        uint32_t m = 0u;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          g[v] = held(g[v]);                 // g and u are bf16 tensors, written or not
+          u[v] = held(u[v]);
+          h[i][v] = (VEC ? p.N - n > v / 8 * 8 : p.N - n > v) ? g[v] * sigmoid(g[v]) * u[v] : 0.f;
+          m = umax(m, __float_as_uint(h[i][v]) & 0x7fffffffu);
+        }
+        amax[wn * BM + r] = umax(m, other_half(m));
+        if (live && p.O0) {
+          const int64_t o = (int64_t)(u_row0 + r) * p.N + n;
+          store16(p.O0 + o, p.N - n, VEC, g);
+          store16(p.O1 + o, p.N - n, VEC, u);
+        }
+      }
+      block_barrier();
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int r = wm * 64 + 32 * i + (lane & 31);
+        const pk_fp8::BlockScale sc = pk_fp8::block_scale(umax(umax(amax[r], amax[BM + r]), umax(amax[2 * BM + r], amax[3 * BM + r])));
+        if (r < u_rows) {
+          const int64_t row = u_row0 + r;
+          *reinterpret_cast<u32x4_t*>(p.Q[0] + (row * n_blocks + u_nt) * BLOCK + wn * 32 + half16) = pk_fp8::codes16(h[i], sc);
+          if (wn == 0 && lane < 32) p.Qs[0][row * out4 + u_nt] = (uint8_t)sc.byte;
+        }
+      }
+    } else {
+      const int nb = 2 * u_nt + (wn >> 1);   // the wave's block of columns, shared with its neighbour
+      uint32_t* const amax = reinterpret_cast<uint32_t*>(spare);      // [2: d_g, d_u][4 waves][128 rows]
+      char* const tr = spare + 8 * BM * 4 + wave * TR_BYTES;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        asm volatile("" ::: "memory");       // the second half's work not before the first half has left its registers
+        __builtin_amdgcn_sched_barrier(0);
+        const int r = wm * 64 + 32 * i + (lane & 31);
+        const bool live = r < u_rows;        // the same in both lanes of a row
+        const int64_t row = u_row0 + (live ? r : 0);
+        const bool chunk = wm * 64 + 32 * i < u_rows;      // (the same for the whole wave)
+        uint32_t mg = 0u, mu = 0u;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          float f[16];
+          exchange_halves(acc[i][j], f);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {      // eight columns at a time
+            const int n = u_n0 + wn * 64 + 32 * j + half16 + 8 * k;
+            int have = p.N - n;
+            asm volatile("" : "+v"(have));   // compared here and not kept: 32 such masks are more than there are scalar registers
+            float g[8], u[8], h[8];
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              const float gv = (float)gs[i][j][k][v], uv = (float)us[i][j][k][v], d = f[8 * k + v];
+              const float sg = sigmoid(gv), silu = gv * sg;
+              const bool in = TRANSPOSED ? live : VEC ? have > 0 : have > v;
+              h[v] = !TRANSPOSED || in ? silu * uv : 0.f;
+              const float dg = d * uv * (sg * (1.f + gv * (1.f - sg))), du = d * silu;
+              g[v] = in ? held(dg) : 0.f;    // bf16 tensors, whose blocks are of what they hold
+              u[v] = in ? held(du) : 0.f;
+              mg = umax(mg, __float_as_uint(g[v]) & 0x7fffffffu);
+              mu = umax(mu, __float_as_uint(u[v]) & 0x7fffffffu);
+            }
+            asm volatile("" : "+v"(mg), "+v"(mu));      // step by step: as one reduction it would keep all values
+            gs[i][j][k] = kept(pack8(g));    // d_g and d_u take the place of g and u
+            us[i][j][k] = kept(pack8(u));
+            if constexpr (TRANSPOSED) {
+              put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, pack8(h));
+            } else if (live) {
+              store8(p.O0 + row * p.N + n, have, VEC, gs[i][j][k]);
+              store8(p.O1 + row * p.N + n, have, VEC, us[i][j][k]);
+              store8(p.O2 + row * p.N + n, have, VEC, pack8(h));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        if constexpr (TRANSPOSED) {
+          if (chunk) {
+            const int64_t padded = (u_begin & ~63) + 64 * (int64_t)u_e + u_mt * BM + wm * 64 + 32 * i;
+            const int64_t to = (padded / 32 * p.N + u_n0 + wn * 64) * 32;
+            store_columns(tr, lane, p.O2 + to);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, gs[i][j][k]);
+            store_columns(tr, lane, p.O0 + to);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, us[i][j][k]);
+            store_columns(tr, lane, p.O1 + to);
+          }
+        }
+        amax[wn * BM + r] = umax(mg, other_half(mg));
+        amax[(4 + wn) * BM + r] = umax(mu, other_half(mu));
+      }
+      block_barrier();
+      if (nb < n_blocks) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const int r = wm * 64 + 32 * i + (lane & 31);
+          const pk_fp8::BlockScale scg = pk_fp8::block_scale(umax(amax[wn * BM + r], amax[(wn ^ 1) * BM + r]));
+          const pk_fp8::BlockScale scu = pk_fp8::block_scale(umax(amax[(4 + wn) * BM + r], amax[(4 + (wn ^ 1)) * BM + r]));
+          if (r < u_rows) {
+            const int64_t row = u_row0 + r, at = (row * n_blocks + nb) * BLOCK + (wn & 1) * 64 + half16;
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+              float g[16], u[16];
+#pragma unroll
+              for (int v = 0; v < 16; ++v) { g[v] = (float)gs[i][j][v >> 3][v & 7]; u[v] = (float)us[i][j][v >> 3][v & 7]; }
+              *reinterpret_cast<u32x4_t*>(p.Q[0] + at + 32 * j) = pk_fp8::codes16(g, scg);
+              *reinterpret_cast<u32x4_t*>(p.Q[1] + at + 32 * j) = pk_fp8::codes16(u, scu);
+            }
+            if ((wn & 1) == 0 && lane < 32) {
+              p.Qs[0][row * out4 + nb] = (uint8_t)scg.byte;
+              p.Qs[1][row * out4 + nb] = (uint8_t)scu.byte;
+            }
+          }
         }
       }
     }
+    if (!more) return;
   }
 }
 
-template <int WM, int KB, int NS, int EPI>
-int launch_tiles(Product p, int64_t A, bool transposed, int kernel_id, hipStream_t s) {
-  constexpr int BM = 64 * WM, STAGE = (BM + 256) * KB;
-  p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP ? BLOCK : 256);
+template <int EPI>
+int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool transposed = false) {
+  p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP ? BLOCK : BN);
   p.by_n_tiles = pk_units::make_fastdiv(p.n_tiles);
   p.head = (int32_t)plan_head(p.E);
   const int64_t units = plan_tiles(A, p.E) * p.n_tiles;
-  if (units > 0x7fffff00ll) return PK_ERR_SHAPE;
-  p.units = (int32_t)units;
-  const int nblk = p.kt * p.nseg, sld = (nblk + 7) / 8 * 8 + 4;
-  const int lds = NS * STAGE + BM * sld + 2 * nblk;
-  const int64_t per = unit_chunk * pk_rules::NXCD;
-  const dim3 grid((unsigned)(pk_ceil_div(units, per) * per)), block(128 * WM);
+  if (units > 0x7fff0000ll) return PK_ERR_SHAPE;      // (steps past the last unit are formed as well)
+  const int64_t per = unit_chunk * pk_rules::NXCD, all = pk_ceil_div(units, per) * per;
+  const dim3 grid((unsigned)(all < 256 ? all : 256)), block(NT);      // one for every CU
+  const int lds = product_lds(scale_row(p.kt) * p.nseg);
   const auto launch = [&](auto kernel, bool (&ready)[PK_MAX_DEVICES]) -> int {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= PK_MAX_DEVICES) return PK_ERR_UNSUPPORTED;
@@ -662,14 +697,9 @@ int launch_tiles(Product p, int64_t A, bool transposed, int kernel_id, hipStream
     return PK_OK;
   };
   static bool ready[3][PK_MAX_DEVICES] = {};
-  if constexpr (EPI == BWD || EPI == BWD_SCALED)
-    if (transposed) return launch(product_kernel<WM, KB, NS, EPI, true, true>, ready[2]);
-  return p.vec ? launch(product_kernel<WM, KB, NS, EPI, true, false>, ready[1]) : launch(product_kernel<WM, KB, NS, EPI, false, false>, ready[0]);
-}
-
-template <int EPI>
-int launch_product(const Product& p, int64_t A, int kernel_id, hipStream_t s, bool transposed = false) {
-  return launch_tiles<2, 64, 3, EPI>(p, A, transposed, kernel_id, s);
+  if constexpr (EPI == BWD)
+    if (transposed) return launch(product_kernel<EPI, true, true>, ready[2]);
+  return p.vec ? launch(product_kernel<EPI, true, false>, ready[1]) : launch(product_kernel<EPI, false, false>, ready[0]);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -1000,6 +1030,11 @@ bool all_aligned(std::initializer_list<const void*> ps) {
     if (!pk_aligned16(q)) return false;
   return true;
 }
+bool word_aligned(std::initializer_list<const void*> ps) {
+  for (const void* q : ps)
+    if ((uintptr_t)q & 3) return false;
+  return true;
+}
 bool all_set(std::initializer_list<const void*> ps) {
   for (const void* q : ps)
     if (!q) return false;
@@ -1070,17 +1105,15 @@ int pk_fp8_plan(const void* counts, int counts_is_i64, int64_t E, int64_t A, int
   return PK_OK;
 }
 
-int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const int32_t* row_map, int64_t row_map_div, const uint8_t* w1, const uint8_t* s1,
-                   const uint8_t* w3, const uint8_t* s3, const int32_t* plan, void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A,
-                   int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
+int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3,
+                   const int32_t* plan, void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E,
+                   pk_stream_t stream) {
   if (const int rc = check(A, H, I, E)) return rc;
-  if (row_map_div < 1 || row_map_div > 0x7fffffffll) return PK_ERR_ARG;
   if (A == 0) return PK_OK;
   if (!all_set({x, x_scales, w1, s1, w3, s3, plan, h, h_scales}) || !g != !u) return PK_ERR_ARG;
-  if (!all_aligned({x, w1, w3, h, plan})) return PK_ERR_ALIGN;
+  if (!all_aligned({x, w1, w3, h, plan}) || !word_aligned({x_scales})) return PK_ERR_ALIGN;
   Product p = {};
-  p.A[0] = x; p.As[0] = x_scales; p.row_map = row_map; p.map_div = pk_units::make_fastdiv(row_map_div);
-  p.A[1] = x; p.As[1] = x_scales;
+  p.A[0] = p.A[1] = x; p.As[0] = p.As[1] = x_scales;
   p.B[0] = w1; p.B[1] = w3; p.Bs[0] = s1; p.Bs[1] = s3;
   p.kt = (int32_t)blocks_of(H); p.nseg = 1; p.N = (int32_t)I; p.E = (int32_t)E; p.plan = plan;
   p.ld = blocks_of(H) * BLOCK; p.strideB = I * p.ld;
@@ -1095,7 +1128,7 @@ int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, co
   if (const int rc = check(A, H, I, E)) return rc;
   if (A == 0) return PK_OK;
   if (!all_set({h, h_scales, w2, s2, plan, y})) return PK_ERR_ARG;
-  if (!all_aligned({h, w2, plan})) return PK_ERR_ALIGN;
+  if (!all_aligned({h, w2, plan}) || !word_aligned({h_scales})) return PK_ERR_ALIGN;
   Product p = {};
   p.A[0] = p.A[1] = h; p.As[0] = p.As[1] = h_scales;
   p.B[0] = p.B[1] = w2; p.Bs[0] = p.Bs[1] = s2;
@@ -1107,17 +1140,14 @@ int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, co
   return launch_product<PLAIN>(p, A, pk_timing::K_FP8_DOWN, (hipStream_t)stream);
 }
 
-static int dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div, const float* scores,
-                    const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u, const int32_t* plan, void* d_g, void* d_u, void* h,
-                    uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H, int64_t I,
-                    int64_t E, bool transposed, pk_stream_t stream) {
-  if (row_map_div < 1 || row_map_div > 0x7fffffffll) return PK_ERR_ARG;
+static int dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
+                    const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales,
+                    int64_t A, int64_t H, int64_t I, int64_t E, bool transposed, pk_stream_t stream) {
   if (A == 0) return PK_OK;
   if (!all_set({d_y, d_y_scales, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales})) return PK_ERR_ARG;
-  if (!scores != !ds_part || (scores && !row_map)) return PK_ERR_ARG;
-  if (!all_aligned({d_y, w2_t, d_g8, d_u8, plan})) return PK_ERR_ALIGN;
+  if (!all_aligned({d_y, w2_t, d_g8, d_u8, plan}) || !word_aligned({d_y_scales})) return PK_ERR_ALIGN;
   Product p = {};
-  p.A[0] = p.A[1] = d_y; p.As[0] = p.As[1] = d_y_scales; p.row_map = row_map; p.map_div = pk_units::make_fastdiv(row_map_div);
+  p.A[0] = p.A[1] = d_y; p.As[0] = p.As[1] = d_y_scales;
   p.B[0] = p.B[1] = w2_t; p.Bs[0] = p.Bs[1] = s2;
   p.kt = (int32_t)blocks_of(H); p.nseg = 1; p.N = (int32_t)I; p.E = (int32_t)E; p.plan = plan;
   p.ld = blocks_of(H) * BLOCK; p.strideB = I * p.ld;
@@ -1127,30 +1157,24 @@ static int dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t
   p.O0 = (bf16_t*)d_g; p.O1 = (bf16_t*)d_u; p.O2 = (bf16_t*)h;
   p.Q[0] = d_g8; p.Qs[0] = d_g_scales; p.Q[1] = d_u8; p.Qs[1] = d_u_scales;
   p.G = (const bf16_t*)g; p.U = (const bf16_t*)u;
-  p.scores = scores; p.ds_part = ds_part; p.total_rows = A;
-  return scores ? launch_product<BWD_SCALED>(p, A, pk_timing::K_FP8_DGRAD_DH, (hipStream_t)stream, transposed)
-                : launch_product<BWD>(p, A, pk_timing::K_FP8_DGRAD_DH, (hipStream_t)stream, transposed);
+  return launch_product<BWD>(p, A, pk_timing::K_FP8_DGRAD_DH, (hipStream_t)stream, transposed);
 }
 
-int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div, const float* scores,
-                    const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u, const int32_t* plan, void* d_g, void* d_u, void* h,
-                    uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H, int64_t I,
-                    int64_t E, pk_stream_t stream) {
+int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
+                    const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales,
+                    int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
   if (const int rc = check(A, H, I, E)) return rc;
-  return dgrad_dh(d_y, d_y_scales, row_map, row_map_div, scores, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales, ds_part, A,
-                  H, I, E, false, stream);
+  return dgrad_dh(d_y, d_y_scales, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, false, stream);
 }
 
-int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, const int32_t* row_map, int64_t row_map_div, const float* scores,
-                      const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u, const int32_t* plan, void* d_gT, void* d_uT, void* hT,
-                      int64_t ldt, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, float* ds_part, int64_t A, int64_t H,
-                      int64_t I, int64_t E, pk_stream_t stream) {
+int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
+                      const int32_t* plan, void* d_gT, void* d_uT, void* hT, int64_t ldt, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8,
+                      uint8_t* d_u_scales, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
   if (const int rc = check(A, H, I, E)) return rc;
   const int64_t need = pk_grouped_swiglu_transposed_ld(A, H, I, E, PK_BF16);
   if (need <= 0) return PK_ERR_SHAPE;
   if (A > 0 && (ldt < need || ldt % 64 != 0)) return PK_ERR_ARG;
-  return dgrad_dh(d_y, d_y_scales, row_map, row_map_div, scores, w2_t, s2, g, u, plan, d_gT, d_uT, hT, d_g8, d_g_scales, d_u8, d_u_scales, ds_part, A,
-                  H, I, E, true, stream);
+  return dgrad_dh(d_y, d_y_scales, w2_t, s2, g, u, plan, d_gT, d_uT, hT, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, true, stream);
 }
 
 int pk_fp8_row_map(const int32_t* plan, int64_t E, int64_t A, int32_t* row_map, pk_stream_t stream) {
@@ -1170,7 +1194,7 @@ int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_
   if (const int rc = check(A, H, I, E)) return rc;
   if (A == 0) return PK_OK;
   if (!all_set({d_g8, d_g_scales, d_u8, d_u_scales, w1_t, s1, w3_t, s3, plan, d_x})) return PK_ERR_ARG;
-  if (!all_aligned({d_g8, d_u8, w1_t, w3_t, plan})) return PK_ERR_ALIGN;
+  if (!all_aligned({d_g8, d_u8, w1_t, w3_t, plan}) || !word_aligned({d_g_scales, d_u_scales})) return PK_ERR_ALIGN;
   Product p = {};
   p.A[0] = d_g8; p.As[0] = d_g_scales; p.A[1] = d_u8; p.As[1] = d_u_scales;
   p.B[0] = w1_t; p.Bs[0] = s1; p.B[1] = w3_t; p.Bs[1] = s3;

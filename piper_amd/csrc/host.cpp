@@ -951,10 +951,10 @@ std::pair<Tensor, Tensor> quantize_rows(const Tensor& x_, const OptTensor& row_m
   c10::hip::HIPGuard device(x_.device().index());
   const Tensor x = contig(x_);
   const int64_t R = row_map.defined() ? row_map.numel() : x.size(0), K = x.size(1), kb = whole_blocks(K);
-  Tensor q = at::empty({R, kb * PK_FP8_BLOCK}, x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({R, kb}, x.options().dtype(at::kFloat8_e8m0fnu));
+  Tensor q = at::empty({R, kb * PK_FP8_BLOCK}, x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({R, (kb + 3) / 4 * 4}, x.options().dtype(at::kFloat8_e8m0fnu));
   PK_CALL(pk_fp8_quantize_rows, ptr(x), dtype_code(x), row_map.defined() ? row_map.data_ptr<int32_t>() : nullptr, map_div, u8(q), u8(s), R, K,
           stream_of(x));
-  return {q, s};
+  return {q, s.narrow(1, 0, kb)};
 }
 
 // The experts' quantized weights, checked against each other.
@@ -984,7 +984,7 @@ struct Fp8Weights {
 struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
   // buffers of a pass over A rows: x, d_y in blocks ([A, H']), h, d_g, d_u in blocks ([A, I'])
   static int64_t codes(int64_t A, int64_t width) { return A * whole_blocks(width) * PK_FP8_BLOCK; }
-  static int64_t scales(int64_t A, int64_t width) { return A * whole_blocks(width); }
+  static int64_t scales(int64_t A, int64_t width) { return A * ((whole_blocks(width) + 3) / 4 * 4); }
   static void zero_tail(const Tensor& buf, const Tensor& plan, int64_t E) {
     PK_CALL(pk_zero_rows_from, ptr(buf), PK_BF16, plan.data_ptr<int32_t>() + E, buf.size(0), buf.size(1), stream_of(buf));
   }
@@ -1022,7 +1022,7 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     const int32_t* const at = plan.data_ptr<int32_t>();
     const auto p = [&](size_t pos) { return static_cast<uint8_t*>(b.at_(pos)); };
     PK_CALL(pk_fp8_quantize_rows, ptr(x), PK_BF16, nullptr, 1, p(x8), p(xs), A, H, st);
-    PK_CALL(pk_fp8_gate_up, p(x8), p(xs), nullptr, 1, u8(w.q[0]), u8(w.s[0]), u8(w.q[2]), u8(w.s[2]), at, g, u, p(h8), p(hs), A, H, I, E, st);
+    PK_CALL(pk_fp8_gate_up, p(x8), p(xs), u8(w.q[0]), u8(w.s[0]), u8(w.q[2]), u8(w.s[2]), at, g, u, p(h8), p(hs), A, H, I, E, st);
     PK_CALL(pk_fp8_down, p(h8), p(hs), u8(w.q[1]), u8(w.s[1]), at, ptr(y), A, H, I, E, st);
     zero_tail(y, plan, E);
     if (plan_out) *plan_out = plan;
@@ -1068,11 +1068,11 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     if (ldt > 0) {
       map = at::empty({A}, starts.options());
       PK_CALL(pk_fp8_row_map, at, E, A, map.data_ptr<int32_t>(), st);
-      PK_CALL(pk_fp8_dgrad_dh_t, p(y8), p(ys), nullptr, 1, nullptr, u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, ldt, p(g8), p(gs),
-              p(u8_), p(us), nullptr, A, H, I, E, st);
+      PK_CALL(pk_fp8_dgrad_dh_t, p(y8), p(ys), u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, ldt, p(g8), p(gs),
+              p(u8_), p(us), A, H, I, E, st);
     } else {
-      PK_CALL(pk_fp8_dgrad_dh, p(y8), p(ys), nullptr, 1, nullptr, u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, p(g8), p(gs), p(u8_),
-              p(us), nullptr, A, H, I, E, st);
+      PK_CALL(pk_fp8_dgrad_dh, p(y8), p(ys), u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, p(g8), p(gs), p(u8_),
+              p(us), A, H, I, E, st);
     }
     if (nx) {
       d_x = at::empty({A, H}, x.options());

@@ -45,9 +45,9 @@ def test_products(p):
     assert lib.pk_fp8_plan_bytes(1000, 6) == 4 * (8 + 8 * (1000 // 128 + 6)) and lib.pk_fp8_plan_bytes(0, 7) == 4 * 16
 
     def calls(A, H, I, E, q=p):
-        yield lib.pk_fp8_gate_up(q, p, None, 1, p, p, p, p, p, p, p, p, p, A, H, I, E, None)
+        yield lib.pk_fp8_gate_up(q, p, p, p, p, p, p, p, p, p, p, A, H, I, E, None)
         yield lib.pk_fp8_down(q, p, p, p, p, p, A, H, I, E, None)
-        yield lib.pk_fp8_dgrad_dh(q, p, None, 1, None, p, p, p, p, p, p, p, p, p, p, p, p, None, A, H, I, E, None)
+        yield lib.pk_fp8_dgrad_dh(q, p, p, p, p, p, p, p, p, p, p, p, p, p, A, H, I, E, None)
         yield lib.pk_fp8_dgrad_dx(q, p, p, p, p, p, p, p, p, p, A, H, I, E, None)
 
     for A, H, I, E, want in ((-1, 128, 128, 1, ARG), (1, 0, 128, 1, ARG), (1, 128, 0, 1, ARG), (1, 128, 128, 0, ARG), (1, 8193, 128, 1, SHAPE),
@@ -56,8 +56,9 @@ def test_products(p):
         assert list(calls(A, H, I, E)) == [want] * 4, (A, H, I, E)
     assert list(calls(1, 128, 128, 1, None)) == [ARG] * 4
     assert list(calls(1, 128, 128, 1, p + 8)) == [ALIGN] * 4
+
     def dh_t(ldt, H=256, I=256, A=10, q=p):
-        return lib.pk_fp8_dgrad_dh_t(q, p, None, 1, None, p, p, p, p, p, p, p, p, ldt, p, p, p, p, None, A, H, I, 2, None)
+        return lib.pk_fp8_dgrad_dh_t(q, p, p, p, p, p, p, p, p, p, ldt, p, p, p, p, A, H, I, 2, None)
 
     enough = lib.pk_grouped_swiglu_transposed_ld(10, 256, 256, 2, _lib.PK_BF16)
     assert dh_t(enough, H=128) == SHAPE and dh_t(enough, I=384) == SHAPE and dh_t(enough - 64) == ARG and dh_t(enough + 1) == ARG
@@ -69,11 +70,10 @@ def test_products(p):
     assert few(A=-1) == ARG and few(H=0) == ARG and few(x=None) == ARG and few(g=None) == ARG and few(w=p + 8) == ALIGN and few(H=8200) == SHAPE
     assert few(A=0) == 0 and lib.pk_fp8_few_rows_pays(0, 128, 128, 4) == 0 and lib.pk_fp8_few_rows_pays(8, 0, 128, 4) == 0
     assert lib.pk_fp8_few_rows_pays(8, 2048, 768, 128) == 1 and lib.pk_fp8_few_rows_pays(32768, 2048, 768, 128) == 0
-    # one of gate and up alone, a divisor without sense, scores without a map or without their sums
-    assert lib.pk_fp8_gate_up(p, p, None, 1, p, p, p, p, p, p, None, p, p, 1, 128, 128, 1, None) == ARG
-    assert lib.pk_fp8_gate_up(p, p, None, 0, p, p, p, p, p, p, p, p, p, 1, 128, 128, 1, None) == ARG
-    assert lib.pk_fp8_dgrad_dh(p, p, None, 1, p, p, p, p, p, p, p, p, p, p, p, p, p, p, 1, 128, 128, 1, None) == ARG
-    assert lib.pk_fp8_dgrad_dh(p, p, p, 1, p, p, p, p, p, p, p, p, p, p, p, p, p, None, 1, 128, 128, 1, None) == ARG
+    # one of gate and up alone; scales of rows that are not words
+    assert lib.pk_fp8_gate_up(p, p, p, p, p, p, p, p, None, p, p, 1, 128, 128, 1, None) == ARG
+    assert lib.pk_fp8_down(p, p + 2, p, p, p, p, 1, 128, 128, 1, None) == ALIGN
+    assert lib.pk_fp8_dgrad_dx(p, p, p, p + 1, p, p, p, p, p, p, 1, 128, 128, 1, None) == ALIGN
 
 
 def test_adamw8(p):

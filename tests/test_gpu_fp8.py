@@ -164,12 +164,12 @@ def test_both_ways_of_the_forward_take_any_rows(dev, E, H, I, counts, spare):
     assert torch.equal(y, bare)
     q, s = ops.quantize_rows_fp8(xd)
     plan = torch.empty(lib.pk_fp8_plan_bytes(A, E) // 4, dtype=torch.int32, device=dev)
-    h8, hs = torch.empty(A, -(-I // 128) * 128, dtype=torch.uint8, device=dev), torch.empty(A, -(-I // 128), dtype=torch.uint8, device=dev)
+    h8, hs = torch.empty(A, -(-I // 128) * 128, dtype=torch.uint8, device=dev), torch.empty(A, -(-I // 512) * 4, dtype=torch.uint8, device=dev)
     tiles = torch.full((A, H), 7.0, device=dev).bfloat16()
     g2, u2 = (torch.empty(A, I, device=dev).bfloat16() for _ in range(2))
     assert lib.pk_fp8_plan(p(n), 1, E, A, p(plan), st) == 0
     assert plan[:E + 1].tolist() == [0] + torch.tensor(counts).cumsum(0).tolist()
-    assert lib.pk_fp8_gate_up(p(q), p(s), None, 1, p(e.q1), p(e.s1), p(e.q3), p(e.s3), p(plan), p(g2), p(u2), p(h8), p(hs), A, H, I, E, st) == 0
+    assert lib.pk_fp8_gate_up(p(q), p(s), p(e.q1), p(e.s1), p(e.q3), p(e.s3), p(plan), p(g2), p(u2), p(h8), p(hs), A, H, I, E, st) == 0
     assert lib.pk_fp8_down(p(h8), p(hs), p(e.q2), p(e.s2), p(plan), p(tiles), A, H, I, E, st) == 0
     owned = sum(counts)
     assert (tiles[owned:] == 7.0).all() and (y[owned:] == 0).all()
@@ -276,11 +276,11 @@ def test_transposed_copies_give_the_same_weight_gradients(dev, counts, spare):
     ldt = lib.pk_grouped_swiglu_transposed_ld(A, H, I, E, _lib.PK_BF16)
     sides = []
     for transposed in (False, True):
-        codes = [torch.zeros(A, I, dtype=torch.uint8, device=dev) for _ in range(2)] + [torch.zeros(A, I // 128, dtype=torch.uint8, device=dev) for _ in range(2)]
+        codes = [torch.zeros(A, I, dtype=torch.uint8, device=dev) for _ in range(2)] + [torch.zeros(A, -(-I // 512) * 4, dtype=torch.uint8, device=dev) for _ in range(2)]
         g8, u8, gs, us = codes
         copies = torch.full((3, ldt if transposed else A, I), math.nan, device=dev).bfloat16()
-        args = (p(q), p(s), None, 1, None, p(e.t2), p(e.s2), p(gu[0]), p(gu[1]), p(plan), p(copies[0]), p(copies[1]), p(copies[2]))
-        tail = (p(g8), p(gs), p(u8), p(us), None, A, H, I, E, st)
+        args = (p(q), p(s), p(e.t2), p(e.s2), p(gu[0]), p(gu[1]), p(plan), p(copies[0]), p(copies[1]), p(copies[2]))
+        tail = (p(g8), p(gs), p(u8), p(us), A, H, I, E, st)
         d1, d2, d3 = (torch.empty(s_, device=dev).bfloat16() for s_ in ((E, I, H), (E, H, I), (E, I, H)))
         if transposed:
             row_map = torch.empty(A, dtype=torch.int32, device=dev)
