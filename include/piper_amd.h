@@ -435,8 +435,8 @@ PK_API int pk_sched_slot_index(int device, uint64_t stream_handle, uint64_t capt
  *   weights  q [E][N][K'], scales [E][N'/128][K'/128]; transposed codes q_t [E][K][N'] share the scales
  * Code buffers must be 16-byte aligned.  The products take bf16 tensors of any width up to
  * H = PK_FP8_MAX_HIDDEN, I = PK_FP8_MAX_INTER; an operand's codes must span less than 4 GiB
- * (PK_ERR_SHAPE).  Which rows are whose comes from a plan (pk_fp8_plan); rows of no expert are neither
- * read nor written. */
+ * (PK_ERR_SHAPE).  Which rows are whose comes from a plan (pk_fp8_plan); rows of no expert are not
+ * read, and zeros in y and d_x. */
 #define PK_FP8_BLOCK 128
 #define PK_FP8_MAX_HIDDEN 8192
 #define PK_FP8_MAX_INTER 4096
@@ -455,6 +455,13 @@ PK_API int pk_fp8_quantize_weights(const void* w, int dtype, uint8_t* q, uint8_t
  * count as zero, and rows past A are cut off.  A plan serves passes over the A and E that it was made for. */
 PK_API int64_t pk_fp8_plan_bytes(int64_t A, int64_t E);
 PK_API int pk_fp8_plan(const void* counts, int counts_is_i64, int64_t E, int64_t A, int32_t* plan, pk_stream_t stream);
+/* What a pass begins with, in one launch.  Forward: x (bf16 [A, H]) in blocks, as pk_fp8_quantize_rows, and pk_fp8_plan.  Backward: d_y
+ * in blocks and, unless NULL, row_map[r] = r for rows of an expert, the last such row for the others: the row map (divisor 1) of
+ * pk_grouped_swiglu_wgrad_scaled_t where the rows are sorted already. */
+PK_API int pk_fp8_begin(const void* x, const void* counts, int counts_is_i64, uint8_t* q, uint8_t* scales, int32_t* plan,
+                 int64_t A, int64_t H, int64_t E, pk_stream_t stream);
+PK_API int pk_fp8_begin_backward(const void* d_y, const int32_t* plan, uint8_t* q, uint8_t* scales, int32_t* row_map,
+                          int64_t A, int64_t H, int64_t E, pk_stream_t stream);
 
 /* g = x . w1[e]^T, u = x . w3[e]^T (both bf16 [A, I], or both NULL where no backward follows), and
  * h = silu(g) * u of what g and u hold, in blocks. */
@@ -486,9 +493,6 @@ PK_API int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, cons
                       const void* g, const void* u, const int32_t* plan, void* d_gT, void* d_uT, void* hT, int64_t ldt,
                       uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, int64_t A, int64_t H,
                       int64_t I, int64_t E, pk_stream_t stream);
-/* row_map[r] = r for rows of an expert, the last such row for the others: the row map (divisor 1) of
- * pk_grouped_swiglu_wgrad_scaled_t where the rows are sorted already. */
-PK_API int pk_fp8_row_map(const int32_t* plan, int64_t E, int64_t A, int32_t* row_map, pk_stream_t stream);
 /* d_x[A, H] (bf16) = d_g . w1[e] + d_u . w3[e] (w1_t, w3_t: the transposed codes) */
 PK_API int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales,
                     const uint8_t* w1_t, const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3,

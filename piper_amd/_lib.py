@@ -116,7 +116,8 @@ SIGNATURES = {
     "pk_fp8_experts_few_rows": (_c_int, [_p, _p, _c_int, *[_p] * 10, *[_c_i64] * 4, _p]),
     "pk_fp8_dgrad_dh": (_c_int, [*[_p] * 14, *[_c_i64] * 4, _p]),
     "pk_fp8_dgrad_dh_t": (_c_int, [*[_p] * 10, _c_i64, *[_p] * 4, *[_c_i64] * 4, _p]),
-    "pk_fp8_row_map": (_c_int, [_p, _c_i64, _c_i64, _p, _p]),
+    "pk_fp8_begin": (_c_int, [_p, _p, _c_int, *[_p] * 3, *[_c_i64] * 3, _p]),
+    "pk_fp8_begin_backward": (_c_int, [*[_p] * 5, *[_c_i64] * 3, _p]),
     "pk_fp8_dgrad_dx": (_c_int, [*[_p] * 10, *[_c_i64] * 4, _p]),
     # master m m_scale v v_scale grad shadow shadow_dtype n lr b1 b2 eps wd step seed grad_scale zero_grad stream
     "pk_adamw8_fused": (_c_int, [*[_p] * 7, _c_int, _c_i64, *[C.c_double] * 5, _c_i64, C.c_uint32, _c_f32, _c_int, _p]),

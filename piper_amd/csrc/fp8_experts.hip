@@ -37,22 +37,25 @@ __device__ __forceinline__ void load8(const T* p, int have, bool vec, float (&f)
 
 // ------------------------------------------------------------------------------------------------ rows
 // 16 lanes to a block, one pass: 2 (bf16) or 4 bytes read and 1 written per value, bound by the memory.
+// One block of a row, by 16 lanes.
 template <typename T>
-__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ row_map, FastDiv map_div,
-                                                                uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t units, int K, int kb,
-                                                                FastDiv by_kb, bool vec) {
-  const int64_t unit = (int64_t)blockIdx.x * (THREADS / 16) + (threadIdx.x >> 4);
-  if (unit >= units) return;                 // whole groups of 16 lanes
-  const int lane = threadIdx.x & 15;
-  const int r = pk_units::fastdiv((int)unit, by_kb), b = (int)unit - r * kb;
-  const int64_t src = row_map ? pk_units::fastdiv(row_map[r], map_div) : r;
-  const int k = b * BLOCK + lane * 8;
+__device__ __forceinline__ void quantize_block(const T* x, int64_t src, uint8_t* q, uint8_t* s, int64_t unit, int r, int K, int kb, bool vec) {
+  const int lane = threadIdx.x & 15, b = (int)(unit - (int64_t)r * kb), k = b * BLOCK + lane * 8;
   float f[8];
   load8<T>(x + src * K + k, K - k, vec, f);
   uint32_t codes[2], byte;
   pk_fp8::quantize8(f, codes, byte);
   *reinterpret_cast<u32x2_t*>(q + unit * BLOCK + lane * 8) = u32x2_t{codes[0], codes[1]};
   if (lane == 0) s[(int64_t)r * scale_row(kb) + b] = (uint8_t)byte;
+}
+template <typename T>
+__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ row_map, FastDiv map_div,
+                                                                uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t units, int K, int kb,
+                                                                FastDiv by_kb, bool vec) {
+  const int64_t unit = (int64_t)blockIdx.x * (THREADS / 16) + (threadIdx.x >> 4);
+  if (unit >= units) return;                 // whole groups of 16 lanes
+  const int r = pk_units::fastdiv((int)unit, by_kb);
+  quantize_block<T>(x, row_map ? pk_units::fastdiv(row_map[r], map_div) : r, q, s, unit, r, K, kb, vec);
 }
 
 // ------------------------------------------------------------------------------------------------ weights
@@ -155,7 +158,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* waves /* 16 */
   *total = all;
   return before + incl - v;
 }
-__global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const void* counts, int is_i64, int E, int64_t A, int32_t* __restrict__ plan) {
+__device__ __forceinline__ void make_plan(const void* counts, int is_i64, int E, int64_t A, int32_t* plan) {
   __shared__ int64_t waves[16];
   __shared__ int32_t first[PK_MAX_EXPERTS + 1], begin[PK_MAX_EXPERTS + 1];
   const int e = threadIdx.x;
@@ -189,11 +192,37 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const void* counts, 
   }
 }
 
-// Every row its own number, those of no expert the last one that has one: a row map for pk_grouped_swiglu_wgrad_scaled_t, which multiplies
+__global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const void* counts, int is_i64, int E, int64_t A, int32_t* plan) {
+  make_plan(counts, is_i64, E, A, plan);
+}
+
+// What a pass begins with, in one launch: its rows in blocks, and in front of the forward its plan (by the first workgroup), in front of
+// the backward a row map.  (1,777 tokens of 2048 in 8 places each: 18 us, and 5 for either of the others by itself.)
+// The map: every row its own number, those of no expert the last one that has one, for pk_grouped_swiglu_wgrad_scaled_t, which multiplies
 // rows behind an expert's last one by zeros.  What stands in rows of no expert (it may be anything) is thereby not read.
-__global__ __launch_bounds__(THREADS) void row_map_kernel(const int32_t* __restrict__ owned, int64_t A, int32_t* __restrict__ map) {
-  const int64_t r = (int64_t)blockIdx.x * THREADS + threadIdx.x;
-  if (r < A) map[r] = (int32_t)(r < *owned ? r : *owned > 0 ? *owned - 1 : 0);
+struct Begin {
+  const bf16_t* x;
+  uint8_t *q, *s;
+  int64_t units, A;
+  int32_t K, kb, E, is_i64;
+  FastDiv by_kb;
+  bool vec;
+  const void* counts;       // forward
+  int32_t* plan;
+  const int32_t* owned;     // backward: rows that have an expert
+  int32_t* map;
+};
+template <bool FORWARD>
+__global__ __launch_bounds__(PLAN_THREADS) void begin_kernel(const Begin p) {
+  if (FORWARD && blockIdx.x == 0) {
+    make_plan(p.counts, p.is_i64, p.E, p.A, p.plan);
+    return;
+  }
+  const int64_t unit = (int64_t)(blockIdx.x - (FORWARD ? 1 : 0)) * (PLAN_THREADS / 16) + (threadIdx.x >> 4);
+  if (unit >= p.units) return;               // whole groups of 16 lanes
+  const int r = pk_units::fastdiv((int)unit, p.by_kb);
+  quantize_block<bf16_t>(p.x, r, p.q, p.s, unit, r, p.K, p.kb, p.vec);
+  if (!FORWARD && p.map && unit == (int64_t)r * p.kb && (threadIdx.x & 15) == 0) p.map[r] = r < *p.owned ? r : *p.owned > 0 ? *p.owned - 1 : 0;
 }
 
 // ------------------------------------------------------------------------------------------------ products
@@ -221,6 +250,7 @@ struct Product {
   uint8_t* Qs[2];
   const bf16_t* G;          // BWD: g and u of the forward
   const bf16_t* U;
+  int64_t A_rows;
   int32_t head;             // words in front of the plan's table
 };
 
@@ -354,10 +384,12 @@ __device__ __forceinline__ int unit_of_block(int b) {      // neighbouring units
 // One persistent workgroup to a CU, eight waves (2 x 4) of 64 x 64 outputs, a ring of three k-tiles.  A workgroup goes through its
 // units one after the other: behind a unit's last k-tile it requests the first two of the next one, and the epilogue, which
 // needs the LDS for the blocks' maxima alone, runs while they are on their way.
-// What bounds it: the memory takes 1.7 us to answer while the chip streams weights, in which a CU multiplies 2.5 k-tiles, and the ring
-// holds three; 128 rows and 256 columns are what fits it.  128 experts of 2048 x 768 with 512 rows each, us, against two workgroups of
-// four waves to a CU with half-block k-tiles: gate and up 363 : 376, down 225 : 261, d_h (row-major copies) 326 : 354; with 111 rows
-// each 105 : 110 and 64 : 68, which is 4.2 TB/s.  Dealing neighbouring units by 8, 16 or 32 to an XCD made no difference.
+// What bounds it: a CU has no more than some 128 cache lines (16 KB) on their way from the L2, in order; with 128 experts of 2048 x 768
+// and 512 rows each a line of gate and up takes 664 cycles on average (7 of 10 are in the L2), which is the 24 bytes a cycle that
+// the transfers reach by themselves.  Multiplying is not it: two halves of the waves that took turns at reading the LDS and at
+// multiplying changed nothing.  Nor did dealing neighbouring units by 8, 16 or 32 to an XCD, or experts that start at different k-tiles.
+// 128 experts of 2048 x 768 with 512 rows each, us, against two workgroups of four waves to a CU with half-block k-tiles: gate and up
+// 363 : 376, down 225 : 261, d_h (row-major copies) 326 : 354; with 111 rows each 105 : 110 and 64 : 68, which is 4.2 TB/s.
 // TRANSPOSED (BWD, N a multiple of 256): O0 to O2 are the transposed copies that pk_grouped_swiglu_wgrad_scaled_t reads,
 // [padded rows / 32][N][32], expert e's rows from (begin & ~63) + 64 e on, zeros behind its last row up to the end of its last block.
 constexpr int NT = 512, BM = TILE_ROWS, BN = 256, STAGES = 3, A_BYTES = BM * BLOCK, STAGE = A_BYTES + BN * BLOCK;
@@ -371,6 +403,15 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
   const int kt4 = scale_row(p.kt), nblk = p.kt * p.nseg, n_blocks = (p.N + BLOCK - 1) / BLOCK, out4 = scale_row(n_blocks);
   const int total = pk_units::as_const(p.plan)[p.E + 1] * p.n_tiles;
+  if constexpr (EPI == PLAIN) {              // rows of no expert: zeros
+    const int64_t end = p.A_rows * p.N, at = (int64_t)blockIdx.x * NT + tid, threads = (int64_t)gridDim.x * NT;
+    const int64_t first = (int64_t)pk_units::as_const(p.plan)[p.E] * p.N;
+    if constexpr (VEC) {
+      for (int64_t i = first + at * 8; i < end; i += threads * 8) *reinterpret_cast<u32x4_t*>(p.O0 + i) = u32x4_t{};
+    } else {
+      for (int64_t i = first + at; i < end; i += threads) p.O0[i] = (bf16_t)0.f;
+    }
+  }
   int step = blockIdx.x;
   if (unit_of_block(step) >= total) return;
   char* const sa = smem + STAGES * STAGE;    // scales of the unit's rows, [words of a row][128]
@@ -679,6 +720,7 @@ int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool tran
   p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP ? BLOCK : BN);
   p.by_n_tiles = pk_units::make_fastdiv(p.n_tiles);
   p.head = (int32_t)plan_head(p.E);
+  p.A_rows = A;
   const int64_t units = plan_tiles(A, p.E) * p.n_tiles;
   if (units > 0x7fff0000ll) return PK_ERR_SHAPE;      // (steps past the last unit are formed as well)
   const int64_t per = unit_chunk * pk_rules::NXCD, all = pk_ceil_div(units, per) * per;
@@ -1105,6 +1147,42 @@ int pk_fp8_plan(const void* counts, int counts_is_i64, int64_t E, int64_t A, int
   return PK_OK;
 }
 
+static int begin(Begin p, const void* x, uint8_t* q, uint8_t* scales, int64_t A, int64_t K, int64_t E, bool forward, pk_stream_t stream) {
+  if (!all_set({x, q, scales, p.plan})) return PK_ERR_ARG;
+  if (!all_aligned({q, p.plan})) return PK_ERR_ALIGN;
+  p.x = (const bf16_t*)x; p.q = q; p.s = scales; p.A = A; p.K = (int32_t)K; p.E = (int32_t)E; p.kb = (int32_t)blocks_of(K);
+  p.by_kb = pk_units::make_fastdiv(p.kb);
+  p.units = A * p.kb;
+  if (p.units > 0x7fffffffll) return PK_ERR_SHAPE;
+  p.vec = bf16_pieces(K, {x});
+  const dim3 grid((unsigned)(pk_ceil_div(p.units, PLAN_THREADS / 16) + (forward ? 1 : 0))), block(PLAN_THREADS);
+  const hipStream_t s = (hipStream_t)stream;
+  if (forward) PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (begin_kernel<true>), grid, block, 0, s, p);
+  else PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (begin_kernel<false>), grid, block, 0, s, p);
+  PK_RETURN_IF_LAUNCH_FAILED();
+  return PK_OK;
+}
+
+int pk_fp8_begin(const void* x, const void* counts, int counts_is_i64, uint8_t* q, uint8_t* scales, int32_t* plan, int64_t A, int64_t H, int64_t E,
+                 pk_stream_t stream) {
+  if (const int rc = check(A, H, 1, E)) return rc;
+  if (A == 0) return pk_fp8_plan(counts, counts_is_i64, E, A, plan, stream);
+  if (!counts) return PK_ERR_ARG;
+  Begin p = {};
+  p.counts = counts; p.is_i64 = counts_is_i64; p.plan = plan;
+  return begin(p, x, q, scales, A, H, E, true, stream);
+}
+
+int pk_fp8_begin_backward(const void* d_y, const int32_t* plan, uint8_t* q, uint8_t* scales, int32_t* row_map, int64_t A, int64_t H, int64_t E,
+                          pk_stream_t stream) {
+  if (const int rc = check(A, H, 1, E)) return rc;
+  if (A == 0) return PK_OK;
+  if (!plan) return PK_ERR_ARG;
+  Begin p = {};
+  p.plan = const_cast<int32_t*>(plan); p.owned = plan + E; p.map = row_map;
+  return begin(p, d_y, q, scales, A, H, E, false, stream);
+}
+
 int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3,
                    const int32_t* plan, void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E,
                    pk_stream_t stream) {
@@ -1175,17 +1253,6 @@ int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8
   if (need <= 0) return PK_ERR_SHAPE;
   if (A > 0 && (ldt < need || ldt % 64 != 0)) return PK_ERR_ARG;
   return dgrad_dh(d_y, d_y_scales, w2_t, s2, g, u, plan, d_gT, d_uT, hT, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, true, stream);
-}
-
-int pk_fp8_row_map(const int32_t* plan, int64_t E, int64_t A, int32_t* row_map, pk_stream_t stream) {
-  if (A < 0 || E <= 0) return PK_ERR_ARG;
-  if (E > PK_MAX_EXPERTS || A > 0x7fffffffll) return PK_ERR_SHAPE;
-  if (A == 0) return PK_OK;
-  if (!plan || !row_map) return PK_ERR_ARG;
-  PK_LAUNCH_NOCHECK(pk_timing::K_MISC, (hipStream_t)stream, row_map_kernel, dim3((unsigned)pk_ceil_div(A, THREADS)), dim3(THREADS), 0,
-                    (hipStream_t)stream, plan + E, A, row_map);
-  PK_RETURN_IF_LAUNCH_FAILED();
-  return PK_OK;
 }
 
 int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales, const uint8_t* w1_t,

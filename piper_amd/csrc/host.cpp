@@ -985,16 +985,11 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
   // buffers of a pass over A rows: x, d_y in blocks ([A, H']), h, d_g, d_u in blocks ([A, I'])
   static int64_t codes(int64_t A, int64_t width) { return A * whole_blocks(width) * PK_FP8_BLOCK; }
   static int64_t scales(int64_t A, int64_t width) { return A * ((whole_blocks(width) + 3) / 4 * 4); }
-  static void zero_tail(const Tensor& buf, const Tensor& plan, int64_t E) {
-    PK_CALL(pk_zero_rows_from, ptr(buf), PK_BF16, plan.data_ptr<int32_t>() + E, buf.size(0), buf.size(1), stream_of(buf));
-  }
-  // The plan of a pass; it begins with starts[]
-  static Tensor plan_of(const Tensor& counts, int64_t E, int64_t A) {
+  // The plan of a pass, to be filled in; it begins with starts[]
+  static Tensor empty_plan(const Tensor& counts, int64_t E, int64_t A) {
     const int64_t bytes = pk_fp8_plan_bytes(A, E);
     TORCH_CHECK(bytes > 0, "pk_fp8_plan_bytes failed: ", pk_status_string((int)bytes));
-    Tensor plan = at::empty({bytes / 4}, counts.options().dtype(at::kInt));
-    PK_CALL(pk_fp8_plan, ptr(counts), counts.scalar_type() == at::kLong, E, A, plan.data_ptr<int32_t>(), stream_of(counts));
-    return plan;
+    return at::empty({bytes / 4}, counts.options().dtype(at::kInt));
   }
   // y [A,H]; gu [2,A,I]: where the pre-activations are left, plan_out: the pass's plan (both null without a backward)
   static Tensor run(const Fp8Weights& w, const Tensor& x, const Tensor& counts, Tensor* gu, Tensor* plan_out) {
@@ -1013,18 +1008,20 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
       b.allocate(x);
       PK_CALL(pk_fp8_experts_few_rows, ptr(x), ptr(counts), counts.scalar_type() == at::kLong, u8(w.q[0]), u8(w.s[0]), u8(w.q[1]), u8(w.s[1]),
               u8(w.q[2]), u8(w.s[2]), g, u, b.f32(h), ptr(y), A, H, I, E, st);
-      if (plan_out) *plan_out = plan_of(counts, E, A);
+      if (plan_out) {
+        *plan_out = empty_plan(counts, E, A);
+        PK_CALL(pk_fp8_plan, ptr(counts), counts.scalar_type() == at::kLong, E, A, plan_out->data_ptr<int32_t>(), st);
+      }
       return y;
     }
     const size_t x8 = b.add(codes(A, H)), xs = b.add(scales(A, H)), h8 = b.add(codes(A, I)), hs = b.add(scales(A, I));
     b.allocate(x);
-    const Tensor plan = plan_of(counts, E, A);
-    const int32_t* const at = plan.data_ptr<int32_t>();
+    const Tensor plan = empty_plan(counts, E, A);
+    int32_t* const at = plan.data_ptr<int32_t>();
     const auto p = [&](size_t pos) { return static_cast<uint8_t*>(b.at_(pos)); };
-    PK_CALL(pk_fp8_quantize_rows, ptr(x), PK_BF16, nullptr, 1, p(x8), p(xs), A, H, st);
+    PK_CALL(pk_fp8_begin, ptr(x), ptr(counts), counts.scalar_type() == at::kLong, p(x8), p(xs), at, A, H, E, st);
     PK_CALL(pk_fp8_gate_up, p(x8), p(xs), u8(w.q[0]), u8(w.s[0]), u8(w.q[2]), u8(w.s[2]), at, g, u, p(h8), p(hs), A, H, I, E, st);
     PK_CALL(pk_fp8_down, p(h8), p(hs), u8(w.q[1]), u8(w.s[1]), at, ptr(y), A, H, I, E, st);
-    zero_tail(y, plan, E);
     if (plan_out) *plan_out = plan;
     return y;
   }
@@ -1064,10 +1061,9 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     const int64_t copy = ldt > 0 ? ldt * I * 2 : step;
     Tensor dguh = at::empty({3 * copy / 2}, x.options()), map, d_x;
     char* const dg = static_cast<char*>(dguh.data_ptr());
-    PK_CALL(pk_fp8_quantize_rows, ptr(d_y), PK_BF16, nullptr, 1, p(y8), p(ys), A, H, st);
+    if (ldt > 0) map = at::empty({A}, starts.options());
+    PK_CALL(pk_fp8_begin_backward, ptr(d_y), at, p(y8), p(ys), ldt > 0 ? map.data_ptr<int32_t>() : nullptr, A, H, E, st);
     if (ldt > 0) {
-      map = at::empty({A}, starts.options());
-      PK_CALL(pk_fp8_row_map, at, E, A, map.data_ptr<int32_t>(), st);
       PK_CALL(pk_fp8_dgrad_dh_t, p(y8), p(ys), u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, ldt, p(g8), p(gs),
               p(u8_), p(us), A, H, I, E, st);
     } else {
@@ -1077,7 +1073,6 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     if (nx) {
       d_x = at::empty({A, H}, x.options());
       PK_CALL(pk_fp8_dgrad_dx, p(g8), p(gs), p(u8_), p(us), u8(t1), u8(s1), u8(t3), u8(s3), at, ptr(d_x), A, H, I, E, st);
-      zero_tail(d_x, starts, E);
     }
     const auto wgrad = [d_y, dguh, map, x, starts, A, H, I, E, ldt, copy](const Tensor& d1, const Tensor& d2, const Tensor& d3, bool accumulate) {
       char* const ds = static_cast<char*>(dguh.data_ptr());

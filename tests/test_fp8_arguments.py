@@ -63,8 +63,12 @@ def test_products(p):
     enough = lib.pk_grouped_swiglu_transposed_ld(10, 256, 256, 2, _lib.PK_BF16)
     assert dh_t(enough, H=128) == SHAPE and dh_t(enough, I=384) == SHAPE and dh_t(enough - 64) == ARG and dh_t(enough + 1) == ARG
     assert dh_t(enough, q=None) == ARG and dh_t(enough, q=p + 8) == ALIGN and dh_t(enough, A=0) == 0 and dh_t(enough, A=-1) == ARG
-    assert lib.pk_fp8_row_map(p, 0, 4, p, None) == ARG and lib.pk_fp8_row_map(p, 4, -1, p, None) == ARG and lib.pk_fp8_row_map(None, 4, 4, p, None) == ARG
-    assert lib.pk_fp8_row_map(p, 1025, 4, p, None) == SHAPE and lib.pk_fp8_row_map(None, 4, 0, None, None) == 0
+    begin = lambda A=4, H=128, E=2, x=p, n=p, q=p, sc=p, plan=p: lib.pk_fp8_begin(x, n, 0, q, sc, plan, A, H, E, None)  # noqa: E731
+    back = lambda A=4, H=128, E=2, x=p, q=p, sc=p, plan=p: lib.pk_fp8_begin_backward(x, plan, q, sc, p, A, H, E, None)  # noqa: E731
+    for f in (begin, back):
+        assert [f(A=-1), f(H=0), f(E=0), f(x=None), f(q=None), f(sc=None), f(plan=None)] == [ARG] * 7
+        assert [f(H=8193), f(E=1025), f(A=2 ** 31), f(A=2 ** 20, H=8192)] == [SHAPE] * 4 and [f(q=p + 8), f(plan=p + 4)] == [ALIGN] * 2
+    assert begin(n=None) == ARG and begin(A=0, n=None) == ARG and back(A=0) == 0
     # few rows
     few = lambda A=4, H=128, I=128, E=2, x=p, g=p, u=p, w=p: lib.pk_fp8_experts_few_rows(x, p, 0, w, p, p, p, p, p, g, u, p, p, A, H, I, E, None)  # noqa: E731
     assert few(A=-1) == ARG and few(H=0) == ARG and few(x=None) == ARG and few(g=None) == ARG and few(w=p + 8) == ALIGN and few(H=8200) == SHAPE
