@@ -2,6 +2,7 @@
 no counterpart in the reference).  Values, not codes: a quantized tensor is what its codes and scales stand for."""
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -173,19 +174,18 @@ def weights_with_floor(w):
 GROUP, GROUP_BITS = 8, 13
 
 
-def product_between(a, b):
-    """a @ b for a = (value, error, floor), b = (value, floor), as the matrix instructions form it.  They align the products of
-    GROUP neighbouring values to the largest exponent among them and keep GROUP_BITS bits below it, which loses at most
+def product_between(a, b, decoded=False):
+    """a @ b for a = (value, error, floor), b = (value, floor), as the matrix instructions form it.  Those for codes align the products
+    of GROUP neighbouring values to the largest exponent among them and keep GROUP_BITS bits below it, which loses at most
     2^-GROUP_BITS of that power of two for each (a code below the normal ones counts with the least normal exponent), and add
-    such sums up in fp32 in some order."""
+    such sums up in fp32 in some order.  Those for decoded values add exact products up in fp32."""
     (v, err, floor), (w, w_floor) = a, b
     K = v.shape[1]
     size = v.abs() @ w.abs() + err @ w.abs()
-    aligned = torch.zeros_like(size)
+    lost = K * U32 * size
     top, w_top = torch.maximum(v.abs() + err, floor), torch.maximum(w.abs(), w_floor)
-    for k in range(0, K, GROUP):
-        aligned += (top[:, k:k + GROUP, None] * w_top[None, k:k + GROUP]).amax(1)
-    lost = K * U32 * size + GROUP * 2.0 ** -GROUP_BITS * aligned
+    for k in range(0, 0 if decoded else K, GROUP):
+        lost += GROUP * 2.0 ** -GROUP_BITS * (top[:, k:k + GROUP, None] * w_top[None, k:k + GROUP]).amax(1)
     # and the deviation if the errors of the summands have nothing to do with each other
     return v @ w, err @ w.abs() + lost, (err.square() @ w.square() + lost.square()).sqrt()
 
@@ -195,10 +195,11 @@ def exactly(x):
     return rounded_rows_between(x.double(), torch.zeros(x.shape, dtype=torch.float64))
 
 
-def experts_between(w1, w2, w3, x, counts, d_y=None):
+def experts_between(w1, w2, w3, x, counts, d_y=None, decoded=False):
     """experts() with the error of every output: {name: (value, error, deviation)}, names y, d_x, d_w1, d_w2, d_w3.  The error is what a
     value can be off by if every uncertain rounding falls the wrong way with the same sign; the deviation takes the summands'
-    errors as unrelated, and bounds the 2-norm over a whole output."""
+    errors as unrelated, and bounds the 2-norm over a whole output.  decoded: see product_between."""
+    product = functools.partial(product_between, decoded=decoded)
     zero = torch.zeros_like
     (v1, f1), (v2, f2), (v3, f3) = (weights_with_floor(w) for w in (w1, w2, w3))
     names = ("y",) if d_y is None else ("y", "d_x", "d_w1", "d_w2", "d_w3")
@@ -216,17 +217,17 @@ def experts_between(w1, w2, w3, x, counts, d_y=None):
         if n == 0:
             continue
         xr = exactly(x[r])
-        g, ge = held_between(*product_between(xr, (v1[e].t(), f1[e].t()))[:2])
-        u, ue = held_between(*product_between(xr, (v3[e].t(), f3[e].t()))[:2])
+        g, ge = held_between(*product(xr, (v1[e].t(), f1[e].t()))[:2])
+        u, ue = held_between(*product(xr, (v3[e].t(), f3[e].t()))[:2])
         sg = torch.sigmoid(g)
         # silu has a slope of at most 1.1; exponential, sum, reciprocal and two products are within 12 half steps together, and an
         # exponential's argument of size |g| moves it by |g| half steps
         h = g * sg * u
         he = 1.1 * ge * (u.abs() + ue) + (g * sg).abs() * ue + (12 + g.abs()) * U32 * h.abs()
-        put("y", r, *product_between(rounded_rows_between(h, he), (v2[e].t(), f2[e].t())))
+        put("y", r, *product(rounded_rows_between(h, he), (v2[e].t(), f2[e].t())))
         if d_y is None:
             continue
-        d_h, de, _ = product_between(exactly(d_y[r]), (v2[e], f2[e]))
+        d_h, de, _ = product(exactly(d_y[r]), (v2[e], f2[e]))
         slope = sg * (1 + g * (1 - sg))
         # slope is within 1.1 and has a slope of at most 1/2; its parts are at most 1 + |g| and rounded a dozen times
         rough = (16 + g.abs()) * U32 * (1 + g.abs())
@@ -236,8 +237,8 @@ def experts_between(w1, w2, w3, x, counts, d_y=None):
         due = de * ((g * sg).abs() + 1.1 * ge) + d_h.abs() * (1.1 * ge) + (d_h * g).abs() * (16 + g.abs()) * U32
         d_g, dge = held_between(d_g, dge)
         d_u, due = held_between(d_u, due)
-        a, ae, ad = product_between(rounded_rows_between(d_g, dge), (v1[e], f1[e]))
-        b, be, bd = product_between(rounded_rows_between(d_u, due), (v3[e], f3[e]))
+        a, ae, ad = product(rounded_rows_between(d_g, dge), (v1[e], f1[e]))
+        b, be, bd = product(rounded_rows_between(d_u, due), (v3[e], f3[e]))
         sums = I_SUMS * U32 * (a.abs() + b.abs())
         put("d_x", r, a + b, ae + be + sums, (ad.square() + bd.square() + sums.square()).sqrt())
         xd = x[r].double()

@@ -1,8 +1,14 @@
 // The experts' products in 8-bit floating point: e4m3 values with a power of two for each block of 128 (fp8_blocks.h).
-//   rows:     [R][K'] codes, K' = K rounded up to 128 (the rest zeros), and [R][K'/128] scale bytes
+//   rows:     [R][K'] codes, K' = K rounded up to 128 (the rest zeros), and K'/128 scale bytes a row, rows of whole words
 //   weights:  [E][N][K'] codes and [E][N/128][K'/128] bytes, blocks of 128 x 128; the transposed codes [E][K][N'] share the bytes
-// v_mfma_scale_f32_32x32x64_f8f6f4 multiplies the codes at twice the rate of bf16, applies both scale bytes to the products and
-// adds in fp32.
+// Products are exact and added in fp32 where values are decoded into bf16, their power of two included, and multiplied there.
+// v_mfma_scale_f32_32x32x64_f8f6f4 takes codes and scale bytes as they are, at twice the rate (measured 4.5 PFLOP/s against 2.2), but of 8
+// neighbouring products' sum it keeps 13 bits below the largest product's leading one (measured; the other instructions for 8-bit values
+// do the same, those for bf16 keep all).  An error of 2^-13 is small next to the codes' own 2^-4, but g, u and d_h are rounded to
+// bf16 next, and h, d_g and d_u to codes again: a value that falls to the other side there is a step off, 2^-8 or 2^-3.  Against
+// exact sums y of one token was off by 0.007 of its size, four times bf16's own rounding, y of many rows by 0.0013 and d_w by 0.001.
+// So passes with few rows, which the memory bounds and where single values count, decode; with many rows (exact_products) the codes'
+// own errors (0.03) are all that matters, and the matrix units would be the bound.
 #include "fp8_blocks.h"
 #include "launch_rules.h"
 #include "unit_index.h"
@@ -36,7 +42,8 @@ __device__ __forceinline__ void load8(const T* p, int have, bool vec, float (&f)
 }
 
 // ------------------------------------------------------------------------------------------------ rows
-// 16 lanes to a block, one pass: 2 (bf16) or 4 bytes read and 1 written per value, bound by the memory.
+// 16 lanes to a block, one pass: 2 (bf16) or 4 bytes read and 1 written per value, bound by the memory (32,768 x 2048 bf16: 37 us,
+// 5.4 TB/s, where a copy of 2 GiB reaches 4.9).
 // One block of a row, by 16 lanes.
 template <typename T>
 __device__ __forceinline__ void quantize_block(const T* x, int64_t src, uint8_t* q, uint8_t* s, int64_t unit, int r, int K, int kb, bool vec) {
@@ -59,7 +66,8 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T* __restr
 }
 
 // ------------------------------------------------------------------------------------------------ weights
-// A workgroup has one block of 128 x 128: 16 lanes to a row of it, the codes once row-major and once, through the LDS, transposed.
+// A workgroup has one block of 128 x 128: 16 lanes to a row of it, the codes once row-major and once, through the LDS, transposed.  Bound
+// by the memory: 128 experts' three weights of 2048 x 768 in bf16 take 469 us, 5.2 TB/s.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void quantize_weights_kernel(const T* __restrict__ w, uint8_t* __restrict__ q, uint8_t* __restrict__ t,
                                                                    uint8_t* __restrict__ s, int N, int K, bool vec) {
@@ -232,6 +240,13 @@ enum Epilogue { PLAIN = 0, GATE_UP = 1, BWD = 2 };
 typedef int intx8_t __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
+// 8 codes and their power of two
+__device__ __forceinline__ bf16x8_t decode8(uint32_t lo, uint32_t hi, float scale) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const auto c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  return bf16x8_t{(bf16_t)a[0], (bf16_t)a[1], (bf16_t)b[0], (bf16_t)b[1], (bf16_t)c[0], (bf16_t)c[1], (bf16_t)d[0], (bf16_t)d[1]};
+}
+
 struct Product {
   const uint8_t* A[2];      // codes of the rows, by segment [., lda]
   const uint8_t* As[2];     // and their scales [., scale_row(kt)]
@@ -395,7 +410,7 @@ __device__ __forceinline__ int unit_of_block(int b) {      // neighbouring units
 constexpr int NT = 512, BM = TILE_ROWS, BN = 256, STAGES = 3, A_BYTES = BM * BLOCK, STAGE = A_BYTES + BN * BLOCK;
 inline int product_lds(int nblk4) { return STAGES * STAGE + nblk4 * BM + 2 * nblk4; }
 
-template <int EPI, bool VEC, bool TRANSPOSED>
+template <int EPI, bool VEC, bool TRANSPOSED, bool EXACT>
 __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
   constexpr int TM = 2, TN = 2, LA = BM * 8 / NT, LB = BN * 8 / NT, L = LA + LB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -530,12 +545,28 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
         // operands swapped: a lane then holds 4 neighbouring columns of one row,
         //   acc[v] = C[row = lane % 32][col = 8 * (v / 4) + 4 * (lane / 32) + v % 4]
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < 2; ++half) {
+          if constexpr (EXACT) {
 #pragma unroll
-          for (int i = 0; i < TM; ++i)
+            for (int c = 0; c < 8; c += 2) {
+              bf16x8_t av[TM], bv[TN];
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[half][j], a[half][i], acc[i][j], 0, 0, 0, j ? sc1 : sc0, 0, scale_a[i]);
+              for (int i = 0; i < TM; ++i) av[i] = decode8(a[half][i][c], a[half][i][c + 1], pk_fp8::scale_of(scale_a[i]));
+#pragma unroll
+              for (int j = 0; j < TN; ++j) bv[j] = decode8(b[half][j][c], b[half][j][c + 1], pk_fp8::scale_of(j ? sc1 : sc0));
+#pragma unroll
+              for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bv[j], av[i], acc[i][j], 0, 0, 0);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int j = 0; j < TN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[half][j], a[half][i], acc[i][j], 0, 0, 0, j ? sc1 : sc0, 0, scale_a[i]);
+          }
+        }
       }
       stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
@@ -715,6 +746,11 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
   }
 }
 
+// us, codes : decoded, gate and up, down, d_h, d_x with n rows an expert.  128 experts 2048 x 768: 32 rows 133 : 136, 82 : 83, 108 : 108,
+// 130 : 134; 48 rows 137 : 140, 85 : 86, 110 : 112, 131 : 134; 64 rows 139 : 149, 88 : 92, 115 : 120, 136 : 148; 512 rows 370 : 572, 225 : 310,
+// 323 : 420.  24 experts 1000 x 360, 32 rows: 19 : 20, 10 : 12, 25 : 26, 14 : 15.
+bool exact_products(int64_t A, int64_t E) { return A <= 40 * E || A <= TILE_ROWS; }
+
 template <int EPI>
 int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool transposed = false) {
   p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP ? BLOCK : BN);
@@ -738,20 +774,24 @@ int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool tran
     PK_RETURN_IF_LAUNCH_FAILED();
     return PK_OK;
   };
-  static bool ready[3][PK_MAX_DEVICES] = {};
+  static bool ready[5][PK_MAX_DEVICES] = {};
   if constexpr (EPI == BWD)
-    if (transposed) return launch(product_kernel<EPI, true, true>, ready[2]);
-  return p.vec ? launch(product_kernel<EPI, true, false>, ready[1]) : launch(product_kernel<EPI, false, false>, ready[0]);
+    if (transposed) return launch(product_kernel<EPI, true, true, false>, ready[4]);
+  if (exact_products(A, p.E))
+    return p.vec ? launch(product_kernel<EPI, true, false, true>, ready[3]) : launch(product_kernel<EPI, false, false, true>, ready[2]);
+  return p.vec ? launch(product_kernel<EPI, true, false, false>, ready[1]) : launch(product_kernel<EPI, false, false, false>, ready[0]);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
 // A handful of rows an expert: the weights are the traffic (one token, 8 of 128 experts, 2048 x 768: 38 MB), so every wave requests
 // all it needs of them at once, straight into registers, and nothing runs before that needs a launch of its own.  The rows are
-// quantized on their way in, and a workgroup finds its expert in the row counts by itself.  v_mfma_scale_f32_16x16x128_f8f6f4: 16
+// quantized on their way in, and a workgroup finds its expert in the row counts by itself.  Four v_mfma_f32_16x16x32_bf16: 16
 // rows of x, 16 of a weight, one block of both.
 //   gate_up_few: 16 columns of gate and up to a workgroup, its eight waves take every eighth block of the reduction; h stays fp32,
 //                since a block of it belongs to eight workgroups
 //   down_few:    h in blocks into the LDS, then 16 columns to each of four waves
+// One token of 8 experts of 2048 x 768 takes 11.6 + 7.2 us, of which the weights are 7.7 at the rate of a copy: the rest is the chain of
+// counts, weights, sums, twice.  24 tokens (some 100 of 128 experts) 82 + 43 us for 470 MB, 3.8 TB/s.
 constexpr int FEW_ROWS = 16;
 
 struct Few {
@@ -821,8 +861,13 @@ __device__ __forceinline__ uint32_t max_of_row(uint32_t m) {      // over the fo
   m = umax(m, __shfl_xor(m, 16));
   return umax(m, __shfl_xor(m, 32));
 }
-__device__ __forceinline__ floatx4_t mfma16(intx8_t w, int sw, intx8_t x, int sx, floatx4_t acc) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc, 0, 0, 0, sw, 0, sx);
+// a block: 32 codes of each to a lane
+__device__ __forceinline__ floatx4_t multiply_block(intx8_t w, int sw, intx8_t x, int sx, floatx4_t acc) {
+  const float fw = pk_fp8::scale_of((uint32_t)sw), fx = pk_fp8::scale_of((uint32_t)sx);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decode8(w[2 * c], w[2 * c + 1], fw), decode8(x[2 * c], x[2 * c + 1], fx), acc, 0, 0, 0);
+  return acc;
 }
 __device__ __forceinline__ intx8_t as_fragment(u32x4_t a, u32x4_t b) {
   return intx8_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
@@ -881,8 +926,8 @@ __global__ __launch_bounds__(512, 2) void gate_up_few_kernel(const Few p) {
       }
       const pk_fp8::BlockScale sc = pk_fp8::block_scale(max_of_row(m));
       const intx8_t xf = as_fragment(pk_fp8::codes16(f[0], sc), pk_fp8::codes16(f[1], sc));
-      ag = mfma16(as_fragment(wg[t][0], wg[t][1]), sg[t], xf, (int)sc.byte, ag);
-      au = mfma16(as_fragment(wu[t][0], wu[t][1]), su[t], xf, (int)sc.byte, au);
+      ag = multiply_block(as_fragment(wg[t][0], wg[t][1]), sg[t], xf, (int)sc.byte, ag);
+      au = multiply_block(as_fragment(wu[t][0], wu[t][1]), su[t], xf, (int)sc.byte, au);
     }
   }
   // acc[v] = C[row = lane % 16][col = 4 * (lane / 16) + v]
@@ -964,7 +1009,7 @@ __device__ __forceinline__ void stream_columns(const uint8_t* const (&w)[MATS], 
     const intx8_t x = as_fragment(f[0], f[1]);
     const int sx = qs[r * nb + b];
 #pragma unroll
-    for (int m = 0; m < MATS; ++m) acc[m] = mfma16(as_fragment(slot[m][0], slot[m][1]), sw[m][c * next_scale + b], x, sx, acc[m]);
+    for (int m = 0; m < MATS; ++m) acc[m] = multiply_block(as_fragment(slot[m][0], slot[m][1]), sw[m][c * next_scale + b], x, sx, acc[m]);
     if (++b == nb) {
       done(c, acc);
 #pragma unroll
@@ -1275,10 +1320,11 @@ int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_
 
 int pk_fp8_few_rows_pays(int64_t A, int64_t H, int64_t I, int64_t E) {
   if (check(A, H, I, E) != PK_OK || A == 0) return 0;
-  // us, this -> tiles (without the zeros behind the last row, 4 us): 128 experts 2048 x 768: 8 rows an expert 164 -> 187, 12 rows 183 ->
-  // 187, 16 rows 236 -> 187; with few workgroups the tiles cannot be filled: 8 experts 2048 x 768: 4 rows 24 -> 50, 16 rows 34 -> 51,
-  // 32 rows 42 -> 53; 24 experts 1000 x 360: 4 rows 26 -> 38, 16 rows 35 -> 38, 32 rows 51 -> 40
-  return A <= 12 * E || (A <= 20 * E && E * blocks_of(I) <= 96);
+  // us, this : quantization, plan and tiles.  128 experts 2048 x 768: 8 rows an expert 143 : 173, 11 rows 150 : 173, 12 rows 190 : 174, 16
+  // rows 229 : 177 (where an expert has more than 16 its weights are read again); 32 of them: 8 rows 53 : 71, 12 rows 62 : 72, 16 rows
+  // 88 : 73; 24 experts 1000 x 360: 8 rows 28 : 29, 12 rows 30 : 29, 16 rows 37 : 30.  128 rows in all: one expert 2048 x 768 26 : 40, two
+  // 35 : 42, eight 29 : 38, eight of 4096 x 1408 63 : 81.
+  return A <= 11 * E || A <= TILE_ROWS;
 }
 
 int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64, const uint8_t* w1, const uint8_t* s1, const uint8_t* w2,
@@ -1294,7 +1340,9 @@ int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64
   p.g = (bf16_t*)g; p.u = (bf16_t*)u; p.h = h; p.y = (bf16_t*)y;
   p.vec = bf16_pieces(H, {x});
   const int64_t tiles = A / FEW_ROWS + (A < E ? A : E);
-  // whole reductions to a wave where that gives every CU a workgroup
+  // whole reductions to a wave where that gives every CU a workgroup, and four column tiles to a wave of down where that fills the chip
+  // eight times (both : eight waves to a reduction : one column tile, us; 128 experts 2048 x 768, 2 rows each 146 : 176 : 154, 8
+  // rows 161 : 203 : 170; of 8 experts with a row each 40 and 35 with either forced : 21 without)
   const bool stream_up = tiles * blocks_of(I) >= 256;
   const int64_t up = stream_up ? blocks_of(I) : pk_ceil_div(I, 16), per = tiles * pk_ceil_div(H, 64) >= 2048 ? 4 : 1, down = pk_ceil_div(H, 64 * per);
   if (tiles * up > 0x7fffff00ll || tiles * down > 0x7fffff00ll) return PK_ERR_SHAPE;

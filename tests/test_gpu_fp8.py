@@ -101,6 +101,11 @@ def _within(name, got, value, err, deviation):
     assert far.norm() <= deviation.norm(), f"{name}: off by {(far.norm() / value.norm()).item():.3g}, at most {(deviation.norm() / value.norm()).item():.3g}"
 
 
+def _decoded(E, rows):
+    """Whether a pass over so many rows multiplies decoded values."""
+    return rows <= max(40 * E, 128)
+
+
 SHAPES = [
     (2, 256, 128, [5, 0], 0, "one row tile, an empty expert"),
     (3, 128, 256, [1, 257, 0], 3, "a row, a row more than a tile, none; rows of nobody"),
@@ -110,6 +115,7 @@ SHAPES = [
     (3, 384, 512, [255, 256, 129], 1, "around a tile's rows"),
     (2, 257, 300, [30, 12], 0, "odd widths of two and three blocks"),
     (70, 128, 128, [i % 4 for i in range(70)], 0, "more experts than lanes"),
+    (2, 257, 300, [140, 90], 3, "odd widths and many rows"),
     (4, 256, 512, [200, 33, 0, 64], 7, "weight gradients from transposed copies if that pays"),
 ]
 
@@ -119,7 +125,7 @@ SHAPES = [
 def test_forward_and_backward_are_within_their_bounds(dev, E, H, I, counts, spare, what, integers):
     print(f"[case] fp8 experts {what} integers={integers}", flush=True)
     w1, w2, w3, x, d_y = _inputs(E, H, I, counts, spare, E + H, integers)
-    want = B.experts_between(w1, w2, w3, x, counts, d_y)
+    want = B.experts_between(w1, w2, w3, x, counts, d_y, decoded=_decoded(E, sum(counts) + spare))
     leaves = [t.to(dev).requires_grad_(True) for t in (w1, w2, w3, x)]
     n = torch.tensor(counts, dtype=torch.int32, device=dev)
     y = F_.bmm_experts_fp8(F_.quantize_experts(*leaves[:3]), leaves[3], n)
@@ -138,7 +144,7 @@ def test_few_rows(dev, A, E, H, I):
     g = torch.Generator().manual_seed(A)
     counts = torch.bincount(torch.randint(0, E, (A,), generator=g), minlength=E).tolist()
     w1, w2, w3, x, _ = _inputs(E, H, I, counts, 0, A, False)
-    want = B.experts_between(w1, w2, w3, x, counts)
+    want = B.experts_between(w1, w2, w3, x, counts, decoded=_decoded(E, x.shape[0]))
     with torch.no_grad():
         y = F_.bmm_experts_fp8(F_.quantize_experts(*(w.to(dev) for w in (w1, w2, w3)), for_backward=False), x.to(dev),
                                torch.tensor(counts, device=dev))
@@ -151,7 +157,7 @@ def test_both_ways_of_the_forward_take_any_rows(dev, E, H, I, counts, spare):
     print(f"[case] fp8 experts both ways E={E} H={H} I={I}", flush=True)
     lib, A = _lib.load(), sum(counts) + spare
     w1, w2, w3, x, _ = _inputs(E, H, I, counts, spare, 9, False)
-    want = B.experts_between(w1, w2, w3, x, counts)
+    want = B.experts_between(w1, w2, w3, x, counts, decoded=_decoded(E, x.shape[0]))
     e = F_.quantize_experts(*(w.to(dev) for w in (w1, w2, w3)))
     xd, n, st = x.to(dev), torch.tensor(counts, dtype=torch.int64, device=dev), _lib.current_stream(dev)
     p = lambda t: t.data_ptr()  # noqa: E731
@@ -177,6 +183,34 @@ def test_both_ways_of_the_forward_take_any_rows(dev, E, H, I, counts, spare):
     # both are the bf16 rounding of sums that differ in the last places
     for a, b in ((g, g2), (u, u2)):
         assert ((a[:owned].float() - b[:owned].float()).abs() <= 2.0 ** -7 * a[:owned].float().abs() + 1e-3).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_few_rows_lose_no_small_products(dev, rows):
+    """Two large products that cancel, 126 others that are 2^-15 of them: exact in fp32 (and in bf16 at the end) if nothing is cut off."""
+    print(f"[case] fp8 experts, products of very different size, {rows} rows", flush=True)
+    lib, E, H, I, st = _lib.load(), 2, 128, 136, _lib.current_stream(dev)
+    x = torch.full((rows, H), 2.0 ** -6)
+    x[:, 0], x[:, 8] = 256.0, -256.0
+    w = torch.full((E, I, H), 0.5)
+    w[:, :, 0] = w[:, :, 8] = 1.0
+    x, w, w2 = x.bfloat16().to(dev), w.bfloat16().to(dev), torch.zeros(E, H, I).bfloat16().to(dev)
+    with torch.no_grad():
+        e = F_.quantize_experts(w, w2, w)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    n = torch.tensor([rows // 2, rows - rows // 2], device=dev)
+    plan = torch.empty(lib.pk_fp8_plan_bytes(rows, E) // 4, dtype=torch.int32, device=dev)
+    q, s = torch.empty(rows, 128, dtype=torch.uint8, device=dev), torch.empty(rows, 4, dtype=torch.uint8, device=dev)
+    h8, hs = torch.empty(rows, 256, dtype=torch.uint8, device=dev), torch.empty(rows, 4, dtype=torch.uint8, device=dev)
+    h, y = torch.empty(rows, I, device=dev), torch.empty(rows, H, device=dev).bfloat16()
+    for few in (True, False):
+        g, u = (torch.zeros(rows, I, device=dev).bfloat16() for _ in range(2))
+        if few:
+            assert lib.pk_fp8_experts_few_rows(p(x), p(n), 1, p(e.q1), p(e.s1), p(e.q2), p(e.s2), p(e.q3), p(e.s3), p(g), p(u), p(h), p(y), rows, H, I, E, st) == 0
+        else:
+            assert lib.pk_fp8_begin(p(x), p(n), 1, p(q), p(s), p(plan), rows, H, E, st) == 0
+            assert lib.pk_fp8_gate_up(p(q), p(s), p(e.q1), p(e.s1), p(e.q3), p(e.s3), p(plan), p(g), p(u), p(h8), p(hs), rows, H, I, E, st) == 0
+        assert (g == 126 * 2.0 ** -7).all() and torch.equal(g, u)
 
 
 def test_counts_that_do_not_fit_lead_nowhere(dev):
