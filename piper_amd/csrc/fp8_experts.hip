@@ -790,8 +790,8 @@ int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool tran
 //   gate_up_few: 16 columns of gate and up to a workgroup, its eight waves take every eighth block of the reduction; h stays fp32,
 //                since a block of it belongs to eight workgroups
 //   down_few:    h in blocks into the LDS, then 16 columns to each of four waves
-// One token of 8 experts of 2048 x 768 takes 11.6 + 7.2 us, of which the weights are 7.7 at the rate of a copy: the rest is the chain of
-// counts, weights, sums, twice.  24 tokens (some 100 of 128 experts) 82 + 43 us for 470 MB, 3.8 TB/s.
+// One token of 8 experts of 2048 x 768 takes 11.9 + 7.1 us, of which the weights are 7.7 at the rate of a copy: the rest is the chain of
+// counts, weights, sums, twice.  24 tokens (some 100 of 128 experts) 73 + 44 us for 470 MB, 4.0 TB/s.
 constexpr int FEW_ROWS = 16;
 
 struct Few {
@@ -808,48 +808,51 @@ struct Few {
   bool vec;                 // x: rows are whole 16-byte pieces
 };
 
+// Sums over the lanes up to this one, cut off at `cap` (of numbers up to 2^31 that are not negative cutting off can be done at every
+// step): shifts within rows of 16 lanes, then the rows' last lanes to the rows behind them.
+__device__ __forceinline__ uint32_t scan(uint32_t v, uint32_t cap) {
+#define PK_STEP(CTRL, ROWS)                                                                                    \
+  {                                                                                                            \
+    const uint32_t sum = v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); \
+    v = sum < cap ? sum : cap;                                                                                 \
+  }
+  PK_STEP(0x111, 0xf) PK_STEP(0x112, 0xf) PK_STEP(0x114, 0xf) PK_STEP(0x118, 0xf) PK_STEP(0x142, 0xa) PK_STEP(0x143, 0xc)
+#undef PK_STEP
+  return v;
+}
+
 // The row tile of that number: its expert and rows.  Every wave looks for itself.  total_rows: rows that belong to an expert.
 __device__ __forceinline__ bool find_rows(const Few& p, int tile, int& e_out, int& row0, int& rows, int& total_rows) {
   const int lane = threadIdx.x & 63, epl = (p.E + 63) >> 6, lo = lane * epl, hi = min(p.E, lo + epl);
-  const auto count = [&](int e) {
+  const uint32_t A = (uint32_t)p.A;
+  const auto count = [&](int e) -> uint32_t {
     const int64_t n = p.is_i64 ? reinterpret_cast<const int64_t*>(p.counts)[e] : reinterpret_cast<const int32_t*>(p.counts)[e];
-    return n < 0 ? (int64_t)0 : n > p.A ? p.A : n;
+    return n < 0 ? 0u : n > p.A ? A : (uint32_t)n;
   };
-  int64_t mine = 0;
-  for (int e = lo; e < hi; ++e) mine += count(e);
-  int64_t incl = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t o = __shfl_up(incl, off, PK_WAVE);
-    if (lane >= off) incl += o;
-  }
-  const int64_t begin = min(incl - mine, p.A);
-  total_rows = (int)min(__shfl(incl, 63, PK_WAVE), p.A);
-  int tiles = 0;
-  for (int64_t e = lo, at = begin; e < hi; ++e) {
-    const int64_t end = min(at + count((int)e), p.A);
-    tiles += (int)((end - at + FEW_ROWS - 1) / FEW_ROWS);
+  uint32_t mine = 0u;
+  for (int e = lo; e < hi; ++e) mine = min(mine + count(e), A);
+  const uint32_t incl = scan(mine, A);
+  const uint32_t begin = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)incl, 0x138, 0xf, 0xf, false);      // of the lane before
+  total_rows = (int)__builtin_amdgcn_readlane((int)incl, 63);
+  uint32_t tiles = 0u;
+  for (uint32_t e = lo, at = begin; (int)e < hi; ++e) {
+    const uint32_t end = min(at + count((int)e), A);
+    tiles += (end - at + FEW_ROWS - 1) / FEW_ROWS;
     at = end;
   }
-  int sum = tiles;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(sum, off, PK_WAVE);
-    if (lane >= off) sum += o;
-  }
-  const unsigned long long owner = __ballot(tile >= sum - tiles && tile < sum);
+  const uint32_t sum = scan(tiles, 0x7fffffffu);
+  const unsigned long long owner = __ballot(tile >= (int)(sum - tiles) && tile < (int)sum);
   if (owner == 0ull) return false;
   const int src = __ffsll((long long)owner) - 1;
-  int left = tile - __shfl(sum - tiles, src, PK_WAVE);
-  int64_t at = __shfl(begin, src, PK_WAVE);
+  uint32_t left = (uint32_t)(tile - __builtin_amdgcn_readlane((int)(sum - tiles), src));
+  uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)begin, src);
   int e = src * epl;
   for (;; ++e) {                             // ends: the tile is one of this lane's experts'
-    const int64_t end = min(at + count(e), p.A);
-    const int n = (int)((end - at + FEW_ROWS - 1) / FEW_ROWS);
+    const uint32_t end = min(at + count(e), A), n = (end - at + FEW_ROWS - 1) / FEW_ROWS;
     if (left < n) {
       e_out = __builtin_amdgcn_readfirstlane(e);
-      row0 = __builtin_amdgcn_readfirstlane((int)at + left * FEW_ROWS);
-      rows = __builtin_amdgcn_readfirstlane((int)min((int64_t)FEW_ROWS, end - at - left * FEW_ROWS));
+      row0 = __builtin_amdgcn_readfirstlane((int)(at + left * FEW_ROWS));
+      rows = __builtin_amdgcn_readfirstlane((int)min((uint32_t)FEW_ROWS, end - at - left * FEW_ROWS));
       return true;
     }
     left -= n;
@@ -1342,7 +1345,7 @@ int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64
   const int64_t tiles = A / FEW_ROWS + (A < E ? A : E);
   // whole reductions to a wave where that gives every CU a workgroup, and four column tiles to a wave of down where that fills the chip
   // eight times (both : eight waves to a reduction : one column tile, us; 128 experts 2048 x 768, 2 rows each 146 : 176 : 154, 8
-  // rows 161 : 203 : 170; of 8 experts with a row each 40 and 35 with either forced : 21 without)
+  // rows 161 : 203 : 170; 8 experts with a row each 21 without, 40 and 35 with one of them)
   const bool stream_up = tiles * blocks_of(I) >= 256;
   const int64_t up = stream_up ? blocks_of(I) : pk_ceil_div(I, 16), per = tiles * pk_ceil_div(H, 64) >= 2048 ? 4 : 1, down = pk_ceil_div(H, 64 * per);
   if (tiles * up > 0x7fffff00ll || tiles * down > 0x7fffff00ll) return PK_ERR_SHAPE;
