@@ -229,16 +229,16 @@ def test_counts_that_do_not_fit_lead_nowhere(dev):
                 assert torch.equal(F_.bmm_experts_fp8(e, x[:A], b), F_.bmm_experts_fp8(e, x[:A], torch.tensor(g, device=dev)))
 
 
-def test_a_row_that_is_not_finite_stays_a_row(dev):
-    print("[case] fp8 experts, NaN and infinity", flush=True)
-    counts = [4, 5]
+@pytest.mark.parametrize("counts", [[4, 5], [170, 161]])
+def test_a_row_that_is_not_finite_stays_a_row(dev, counts):
+    print(f"[case] fp8 experts, NaN and infinity, {counts}", flush=True)
     w1, w2, w3, x, _ = _inputs(2, 256, 128, counts, 0, 5, False)
     bad = x.clone()
     bad[1, 7], bad[6, 200] = math.inf, math.nan
     experts = F_.quantize_experts(*(w.to(dev) for w in (w1, w2, w3)))
     n = torch.tensor(counts, device=dev)
     y, z = F_.bmm_experts_fp8(experts, x.to(dev), n), F_.bmm_experts_fp8(experts, bad.to(dev), n)
-    whole = torch.ones(9, dtype=torch.bool)
+    whole = torch.ones(sum(counts), dtype=torch.bool)
     whole[[1, 6]] = False
     assert torch.equal(y[whole], z[whole]) and torch.isnan(z[~whole]).all()
 
@@ -384,6 +384,125 @@ def test_captured_and_replayed(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, forward()), f"replay {rep}"
+
+
+MANY = dict(counts=(300, 0, 129, 171), H=512, I=256)      # tiles, products of codes, transposed copies where they pay
+
+
+def test_many_rows_strides_streams_and_accumulation(dev):
+    """What the tests above ask of a few rows, of passes that go through the tiles."""
+    print("[case] fp8 experts, many rows: strides, streams, partial gradients, accumulate, defer", flush=True)
+    w, x, d_y, n = _setup(dev, **MANY)
+    want = _pass(w, x, d_y, n)
+    xt = x.detach().t().contiguous().t().requires_grad_(True)
+    assert _equal(want, _pass(w, xt, d_y.t().contiguous().t(), n))
+    odd = torch.cat([x.new_zeros(1), x.detach().reshape(-1)])[1:].view(x.shape).requires_grad_(True)      # 2-byte aligned rows
+    got = _pass(w, odd, d_y, n)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[4], want[4])
+    # the weights' gradients are summed in another order where 16-byte loads do not fit
+    bounds = B.experts_between(*(t.detach().cpu() for t in (*w, x)), MANY["counts"], d_y.cpu())
+    for name, t in zip(("d_w1", "d_w2", "d_w3"), got[1:4]):
+        _within(name, t, *bounds[name])
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for side in sides:                                     # two passes at once
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got.append(_pass(w, x, d_y, n))
+    for side, g in zip(sides, got):
+        torch.cuda.current_stream().wait_stream(side)
+        assert _equal(want, g)
+    experts = F_.quantize_experts(*w)
+    only_x = torch.autograd.grad(F_.bmm_experts_fp8(experts._replace(w1=None, w2=None, w3=None), x, n), x, d_y)[0]
+    only_w = torch.autograd.grad(F_.bmm_experts_fp8(experts, x.detach(), n), w[1], d_y)[0]
+    assert torch.equal(only_x, want[4]) and torch.equal(only_w, want[2])
+    with F_.defer_weight_grads() as q:
+        F_.bmm_experts_fp8(experts, x, n).backward(d_y)
+    assert torch.equal(x.grad, want[4]) and all(p.grad is None for p in w)
+    q.run()
+    assert _equal([p.grad for p in w], want[1:4])
+    kept = [p.grad for p in w]
+    with F_.accumulate_weight_grads():
+        F_.bmm_experts_fp8(experts, x, n).backward(d_y)
+    for p, k, g in zip(w, kept, want[1:4]):
+        assert p.grad is k
+        # as above: half a step of bf16 of the sum, and of the new gradient
+        assert ((p.grad.double() - 2 * g.double()).abs() <= 2.0 ** -8 * 2 * g.double().abs() + 2.0 ** -8 * g.double().abs()).all()
+
+
+def test_many_rows_and_counts_that_do_not_fit(dev):
+    print("[case] fp8 experts, many rows, counts that do not fit, rows of nobody", flush=True)
+    w, x, d_y, n = _setup(dev, **MANY)
+    for bad, good in (((300, -3, 1000, 5), (300, 0, 300, 0)), ((10 ** 6, 5, 5, 5), (600, 0, 0, 0)), ((-1, -1, 7, -2 ** 31), (0, 0, 7, 0)),
+                      ((2 ** 40,) * 4, (600, 0, 0, 0)), ((0, 0, 0, 0), (0, 0, 0, 0))):
+        got, want = (_pass(w, x, d_y, torch.tensor(c, device=dev)) for c in (bad, good))
+        assert _equal(got, want)
+        assert all((t[sum(good):] == 0).all() for t in (got[0], got[4]))
+        assert all((g[e] == 0).all() for g in got[1:4] for e in range(4) if good[e] == 0)
+
+
+def test_many_rows_captured_and_replayed_with_their_backward(dev):
+    print("[case] fp8 experts, many rows, forward and backward in a graph", flush=True)
+    w, x, d_y, n = _setup(dev, **MANY)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _pass(w, x, d_y, n)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _pass(w, x, d_y, n)
+    for rep in range(4):
+        g = torch.Generator().manual_seed(rep)
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, generator=g))
+            w[1].mul_(0.5)
+        d_y.copy_(torch.randn(d_y.shape, generator=g))
+        n.copy_(torch.tensor([(600, 0, 0, 0), (1, 1, 597, 1), (0, 0, 17, 200), (150, 150, 150, 150)][rep], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert _equal(out, _pass(w, x, d_y, n)), f"replay {rep}"
+
+
+@pytest.mark.parametrize("rows", [20, 300])
+def test_largest_widths(dev, rows):
+    """H 8192 and I 4096, through the C ABI, on integers whose sums are exact in any order (products are at most 16 units, so the matrix
+    instructions cut nothing off either)."""
+    print(f"[case] fp8 experts, largest widths, {rows} rows", flush=True)
+    lib, E, H, I, st = _lib.load(), 1, 8192, 4096, _lib.current_stream(dev)
+    w1, w2, w3, x, d_y = (t.to(dev) for t in _inputs(E, H, I, [rows], 0, 5, True))
+    e = F_.quantize_experts(w1, w2, w3)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    n = torch.tensor([rows], dtype=torch.int32, device=dev)
+    new = lambda *shape, dtype=torch.bfloat16: torch.zeros(shape, dtype=dtype, device=dev)  # noqa: E731
+    plan, byte = torch.empty(lib.pk_fp8_plan_bytes(rows, E) // 4, dtype=torch.int32, device=dev), dict(dtype=torch.uint8)
+    q, s, h8, hs = new(rows, H, **byte), new(rows, H // 128, **byte), new(rows, I, **byte), new(rows, I // 128, **byte)
+    g, u, y, d_x = new(rows, I), new(rows, I), new(rows, H), new(rows, H)
+    dot = lambda a, b: (a.double() @ b.double().t().contiguous())  # noqa: E731
+    assert lib.pk_fp8_begin(p(x), p(n), 0, p(q), p(s), p(plan), rows, H, E, st) == 0
+    assert lib.pk_fp8_gate_up(p(q), p(s), p(e.q1), p(e.s1), p(e.q3), p(e.s3), p(plan), p(g), p(u), p(h8), p(hs), rows, H, I, E, st) == 0
+    assert torch.equal(g, dot(x, w1[0]).bfloat16()) and torch.equal(u, dot(x, w3[0]).bfloat16())
+    if rows <= 128:
+        g2, u2, h = new(rows, I), new(rows, I), new(rows, I, dtype=torch.float32)
+        assert lib.pk_fp8_experts_few_rows(p(x), p(n), 0, p(e.q1), p(e.s1), p(e.q2), p(e.s2), p(e.q3), p(e.s3), p(g2), p(u2), p(h), p(y), rows, H, I, E, st) == 0
+        assert torch.equal(g, g2) and torch.equal(u, u2) and torch.isfinite(y).all()
+    ints = x[:, :I].contiguous()                           # in the place of h, d_g and d_u
+    hq, hqs = ops.quantize_rows_fp8(ints)
+    assert lib.pk_fp8_down(p(hq), p(hqs), p(e.q2), p(e.s2), p(plan), p(y), rows, H, I, E, st) == 0
+    assert torch.equal(y, dot(ints, w2[0]).bfloat16())
+    assert lib.pk_fp8_dgrad_dx(p(hq), p(hqs), p(hq), p(hqs), p(e.t1), p(e.s1), p(e.t3), p(e.s3), p(plan), p(d_x), rows, H, I, E, st) == 0
+    assert torch.equal(d_x, (ints.double() @ (w1[0].double() + w3[0].double())).bfloat16())
+    # silu(64) = 64 in fp32, so d_u = 64 d_h
+    g.fill_(64.0)
+    u.fill_(1.0)
+    out = [new(rows, I) for _ in range(3)]
+    codes = [new(rows, I, **byte), new(rows, I // 128, **byte), new(rows, I, **byte), new(rows, I // 128, **byte)]
+    assert lib.pk_fp8_begin_backward(p(d_y), p(plan), p(q), p(s), None, rows, H, E, st) == 0
+    assert lib.pk_fp8_dgrad_dh(p(q), p(s), p(e.t2), p(e.s2), p(g), p(u), p(plan), *(p(t) for t in out), *(p(t) for t in codes), rows, H, I, E, st) == 0
+    want = 64 * (d_y.double() @ w2[0].double())
+    assert torch.equal(out[1], want.bfloat16()) and (out[2] == 64).all()
+    wq, ws = B.rows(out[1].cpu())
+    assert _same(codes[2].view(E4M3), wq) and torch.equal(_exponents(codes[3]), ws)
 
 
 def test_modules_call_it(dev):
