@@ -13,6 +13,8 @@
 #include "launch_rules.h"
 #include "unit_index.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int BLOCK = PK_FP8_BLOCK;
@@ -407,15 +409,18 @@ __device__ __forceinline__ int unit_of_block(int b) {      // neighbouring units
 // 363 : 376, down 225 : 261, d_h (row-major copies) 326 : 354; with 111 rows each 105 : 110 and 64 : 68, which is 4.2 TB/s.
 // TRANSPOSED (BWD, N a multiple of 256): O0 to O2 are the transposed copies that pk_grouped_swiglu_wgrad_scaled_t reads,
 // [padded rows / 32][N][32], expert e's rows from (begin & ~63) + 64 e on, zeros behind its last row up to the end of its last block.
-constexpr int NT = 512, BM = TILE_ROWS, BN = 256, STAGES = 3, A_BYTES = BM * BLOCK, STAGE = A_BYTES + BN * BLOCK;
+// NARROW (not GATE_UP, whose unit has to have whole blocks of h): units of 128 columns, waves (4 x 2) of 32 x 64, for launches that
+// leave CUs without a unit.
+constexpr int NT = 512, BM = TILE_ROWS, WIDE = 256, STAGES = 3, A_BYTES = BM * BLOCK, STAGE = A_BYTES + WIDE * BLOCK;
 inline int product_lds(int nblk4) { return STAGES * STAGE + nblk4 * BM + 2 * nblk4; }
 
-template <int EPI, bool VEC, bool TRANSPOSED, bool EXACT>
+template <int EPI, bool VEC, bool TRANSPOSED, bool EXACT, bool NARROW>
 __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
-  constexpr int TM = 2, TN = 2, LA = BM * 8 / NT, LB = BN * 8 / NT, L = LA + LB;
+  constexpr int BN = NARROW ? BLOCK : WIDE, TM = NARROW ? 1 : 2, TN = 2, LA = BM * 8 / NT, LB = BN * 8 / NT, L = LA + LB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 2, wn = wave & 3;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = NARROW ? wave >> 1 : wave >> 2, wn = NARROW ? wave & 1 : wave & 3;
+  const int wave_row = wm * 32 * TM;         // the wave's first row in the unit
   const int kt4 = scale_row(p.kt), nblk = p.kt * p.nseg, n_blocks = (p.N + BLOCK - 1) / BLOCK, out4 = scale_row(n_blocks);
   const int total = pk_units::as_const(p.plan)[p.E + 1] * p.n_tiles;
   if constexpr (EPI == PLAIN) {              // rows of no expert: zeros
@@ -484,7 +489,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
     }
     if (tid < 2 * nblk) {
       const int b = tid >= nblk, k = b ? tid - nblk : tid, seg = k >= p.kt;
-      const int nb = EPI == GATE_UP ? nt : min(2 * nt + b, n_blocks - 1);
+      const int nb = EPI == GATE_UP ? nt : min(nt * (BN / BLOCK) + b, n_blocks - 1);
       scale_b = p.Bs[EPI == GATE_UP ? b : seg][e * p.bs_e + (int64_t)nb * p.bs_n + (int64_t)(seg ? k - p.kt : k) * p.bs_k];
     }
     fetch(0, stage);
@@ -508,7 +513,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
-    const bool wave_has_rows = wm * 64 < rows;
+    const bool wave_has_rows = wave_row < rows;
     step += gridDim.x;
     const int next_unit = unit_of_block(step);
     const bool more = next_unit < total;
@@ -528,7 +533,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
       if (wave_has_rows) {
         const char* const at = smem + stage * STAGE;
         const int seg = kt >= p.kt, k = seg ? kt - p.kt : kt;
-        const char* const sa_at = sa + (seg * kt4 + (k & ~3)) * BM + (k & 3) + (wm * 64 + (lane & 31)) * 4;
+        const char* const sa_at = sa + (seg * kt4 + (k & ~3)) * BM + (k & 3) + (wave_row + (lane & 31)) * 4;
         const int sc0 = (unsigned char)sb[(EPI == GATE_UP ? 0 : wn >> 1) * nblk + kt];
         const int sc1 = EPI == GATE_UP ? (unsigned char)sb[nblk + kt] : sc0;
         int scale_a[TM];
@@ -538,7 +543,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
 #pragma unroll
-          for (int i = 0; i < TM; ++i) a[half][i] = fragment(at, wm * 64 + i * 32, half, lane);
+          for (int i = 0; i < TM; ++i) a[half][i] = fragment(at, wave_row + i * 32, half, lane);
 #pragma unroll
           for (int j = 0; j < TN; ++j) b[half][j] = fragment(at + A_BYTES, wn * 64 + j * 32, half, lane);
         }
@@ -583,7 +588,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          const int r = wm * 64 + 32 * i + (lane & 31), n = u_n0 + wn * 64 + 32 * j + half16;
+          const int r = wave_row + 32 * i + (lane & 31), n = u_n0 + wn * 64 + 32 * j + half16;
           const int64_t row = u_row0 + (r < u_rows ? r : 0);
           load16(p.G + row * p.N + n, p.N - n, VEC, gs[i][j]);
           load16(p.U + row * p.N + n, p.N - n, VEC, us[i][j]);
@@ -601,7 +606,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
       if (wave_has_rows) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          const int r = wm * 64 + 32 * i + (lane & 31);
+          const int r = wave_row + 32 * i + (lane & 31);
 #pragma unroll
           for (int j = 0; j < TN; ++j) {
             float f[16];
@@ -618,7 +623,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
       float h[TM][16];
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const int r = wm * 64 + 32 * i + (lane & 31);
+        const int r = wave_row + 32 * i + (lane & 31);
         const bool live = r < u_rows;        // the same in both lanes of a row
         float g[16], u[16];
         exchange_halves(acc[i][0], g);
@@ -641,7 +646,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
       block_barrier();
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const int r = wm * 64 + 32 * i + (lane & 31);
+        const int r = wave_row + 32 * i + (lane & 31);
         const pk_fp8::BlockScale sc = pk_fp8::block_scale(umax(umax(amax[r], amax[BM + r]), umax(amax[2 * BM + r], amax[3 * BM + r])));
         if (r < u_rows) {
           const int64_t row = u_row0 + r;
@@ -650,17 +655,17 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
         }
       }
     } else {
-      const int nb = 2 * u_nt + (wn >> 1);   // the wave's block of columns, shared with its neighbour
+      const int nb = u_nt * (BN / BLOCK) + (wn >> 1);      // the wave's block of columns, shared with its neighbour
       uint32_t* const amax = reinterpret_cast<uint32_t*>(spare);      // [2: d_g, d_u][4 waves][128 rows]
       char* const tr = spare + 8 * BM * 4 + wave * TR_BYTES;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         asm volatile("" ::: "memory");       // the second half's work not before the first half has left its registers
         __builtin_amdgcn_sched_barrier(0);
-        const int r = wm * 64 + 32 * i + (lane & 31);
+        const int r = wave_row + 32 * i + (lane & 31);
         const bool live = r < u_rows;        // the same in both lanes of a row
         const int64_t row = u_row0 + (live ? r : 0);
-        const bool chunk = wm * 64 + 32 * i < u_rows;      // (the same for the whole wave)
+        const bool chunk = wave_row + 32 * i < u_rows;      // (the same for the whole wave)
         uint32_t mg = 0u, mu = 0u;
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
@@ -699,7 +704,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
         }
         if constexpr (TRANSPOSED) {
           if (chunk) {
-            const int64_t padded = (u_begin & ~63) + 64 * (int64_t)u_e + u_mt * BM + wm * 64 + 32 * i;
+            const int64_t padded = (u_begin & ~63) + 64 * (int64_t)u_e + u_mt * BM + wave_row + 32 * i;
             const int64_t to = (padded / 32 * p.N + u_n0 + wn * 64) * 32;
             store_columns(tr, lane, p.O2 + to);
 #pragma unroll
@@ -721,7 +726,7 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
       if (nb < n_blocks) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          const int r = wm * 64 + 32 * i + (lane & 31);
+          const int r = wave_row + 32 * i + (lane & 31);
           const pk_fp8::BlockScale scg = pk_fp8::block_scale(umax(amax[wn * BM + r], amax[(wn ^ 1) * BM + r]));
           const pk_fp8::BlockScale scu = pk_fp8::block_scale(umax(amax[(4 + wn) * BM + r], amax[(4 + (wn ^ 1)) * BM + r]));
           if (r < u_rows) {
@@ -751,9 +756,15 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
 // 323 : 420.  24 experts 1000 x 360, 32 rows: 19 : 20, 10 : 12, 25 : 26, 14 : 15.
 bool exact_products(int64_t A, int64_t E) { return A <= 40 * E || A <= TILE_ROWS; }
 
+// Of as many wide units, at most, a launch is made of narrow ones, us, wide : narrow, down, d_h, d_x.  2048 x 768: 4 experts of 64 rows 14 : 11,
+// 33 : 22, 21 : 15; 8 of 200 16 : 14, 40 : 27, 23 : 19; 16 of 30 17 : 16, 35 : 24, 26 : 24; 16 of 200 (328 units, in d_h 123) 20 : 21, 42 : 30,
+// 31 : 33; 32 of 200 (656, 246) 35 : 37, 53 : 55, 56 : 60.  24 experts of 172 rows 1000 x 360 (224, 112) 15 : 15, 31 : 22, 18 : 19.
+constexpr int NARROW_UNITS = 192;
+
 template <int EPI>
 int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool transposed = false) {
-  p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP ? BLOCK : BN);
+  const bool narrow = EPI != GATE_UP && !transposed && plan_tiles(A, p.E) * pk_ceil_div(p.N, WIDE) <= NARROW_UNITS;
+  p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP || narrow ? BLOCK : WIDE);
   p.by_n_tiles = pk_units::make_fastdiv(p.n_tiles);
   p.head = (int32_t)plan_head(p.E);
   p.A_rows = A;
@@ -774,12 +785,18 @@ int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool tran
     PK_RETURN_IF_LAUNCH_FAILED();
     return PK_OK;
   };
-  static bool ready[5][PK_MAX_DEVICES] = {};
+  static bool ready[9][PK_MAX_DEVICES] = {};
   if constexpr (EPI == BWD)
-    if (transposed) return launch(product_kernel<EPI, true, true, false>, ready[4]);
-  if (exact_products(A, p.E))
-    return p.vec ? launch(product_kernel<EPI, true, false, true>, ready[3]) : launch(product_kernel<EPI, false, false, true>, ready[2]);
-  return p.vec ? launch(product_kernel<EPI, true, false, false>, ready[1]) : launch(product_kernel<EPI, false, false, false>, ready[0]);
+    if (transposed) return launch(product_kernel<EPI, true, true, false, false>, ready[8]);
+  const auto pick = [&](auto wide_or_narrow, bool (*done)[PK_MAX_DEVICES]) {
+    constexpr bool N = decltype(wide_or_narrow)::value;
+    if (exact_products(A, p.E))
+      return p.vec ? launch(product_kernel<EPI, true, false, true, N>, done[3]) : launch(product_kernel<EPI, false, false, true, N>, done[2]);
+    return p.vec ? launch(product_kernel<EPI, true, false, false, N>, done[1]) : launch(product_kernel<EPI, false, false, false, N>, done[0]);
+  };
+  if constexpr (EPI != GATE_UP)
+    if (narrow) return pick(std::true_type(), ready + 4);
+  return pick(std::false_type(), ready);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows

@@ -116,6 +116,10 @@ SHAPES = [
     (2, 257, 300, [30, 12], 0, "odd widths of two and three blocks"),
     (70, 128, 128, [i % 4 for i in range(70)], 0, "more experts than lanes"),
     (2, 257, 300, [140, 90], 3, "odd widths and many rows"),
+    (200, 200, 136, [i % 31 for i in range(200)], 5, "enough experts for wide units, decoded values"),
+    (200, 199, 139, [i % 31 for i in range(200)], 0, "the same with odd widths"),
+    (200, 200, 136, [i % 87 for i in range(200)], 9, "the same with more rows"),
+    (200, 199, 139, [i % 87 for i in range(200)], 0, "the same with odd widths and more rows"),
     (4, 256, 512, [200, 33, 0, 64], 7, "weight gradients from transposed copies if that pays"),
 ]
 
