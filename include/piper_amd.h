@@ -440,14 +440,16 @@ PK_API int pk_sched_slot_index(int device, uint64_t stream_handle, uint64_t capt
 #define PK_FP8_BLOCK 128
 #define PK_FP8_MAX_HIDDEN 8192
 #define PK_FP8_MAX_INTER 4096
+#define PK_FP8_MAX_WEIGHTS 3
 
 /* Rows of x [., K] (dtype) in blocks: row r of the result is x[r], or with row_map (i32 [rows])
  * x[row_map[r] / row_map_div]. */
 PK_API int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map, int64_t row_map_div, uint8_t* q,
                          uint8_t* scales, int64_t rows, int64_t K, pk_stream_t stream);
-/* w [E, N, K] (dtype) in blocks; q_t may be NULL. */
-PK_API int pk_fp8_quantize_weights(const void* w, int dtype, uint8_t* q, uint8_t* q_t, uint8_t* scales, int64_t E,
-                            int64_t N, int64_t K, pk_stream_t stream);
+/* `count` weights (up to PK_FP8_MAX_WEIGHTS) of the same E experts in blocks: w[i] [E, N[i], K[i]] (dtype).  w, q, q_t, scales,
+ * N, K: HOST arrays; q_t and entries of it may be NULL. */
+PK_API int pk_fp8_quantize_weights(int count, const void* const* w, int dtype, uint8_t* const* q, uint8_t* const* q_t,
+                            uint8_t* const* scales, int64_t E, const int64_t* N, const int64_t* K, pk_stream_t stream);
 
 /* The row ranges of a pass over A rows, for the four products below: expert e owns counts[e] rows (int32, or
  * int64 with counts_is_i64) behind those of the experts before it.  plan: pk_fp8_plan_bytes(A, E) bytes, 16-byte

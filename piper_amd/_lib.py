@@ -106,7 +106,7 @@ SIGNATURES = {
                                        _c_f32, _c_f32, _c_i64, _c_f32, _c_int, _p]),
     # rows: x dtype row_map div q scales rows K stream; weights: w dtype q q_t scales E N K stream
     "pk_fp8_quantize_rows": (_c_int, [_p, _c_int, _p, _c_i64, _p, _p, _c_i64, _c_i64, _p]),
-    "pk_fp8_quantize_weights": (_c_int, [_p, _c_int, _p, _p, _p, _c_i64, _c_i64, _c_i64, _p]),
+    "pk_fp8_quantize_weights": (_c_int, [_c_int, _p, _c_int, *[_p] * 3, _c_i64, _p, _p, _p]),
     "pk_fp8_plan_bytes": (_c_i64, [_c_i64, _c_i64]),
     "pk_fp8_plan": (_c_int, [_p, _c_int, _c_i64, _c_i64, _p, _p]),
     # ... A H I E stream

@@ -69,18 +69,32 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T* __restr
 
 // ------------------------------------------------------------------------------------------------ weights
 // A workgroup has one block of 128 x 128: 16 lanes to a row of it, the codes once row-major and once, through the LDS, transposed.  Bound
-// by the memory: 128 experts' three weights of 2048 x 768 in bf16 take 469 us, 5.2 TB/s.
+// by the memory: 128 experts' three weights of 2048 x 768 in bf16 take 457 us, 5.3 TB/s.  All weights of a call share a launch (24 experts'
+// three of 363 x 1000 in fp32, 576 workgroups each: 41 us, in three launches 57; the others 469).
+struct Weights {
+  const void* w[PK_FP8_MAX_WEIGHTS];
+  uint8_t *q[PK_FP8_MAX_WEIGHTS], *t[PK_FP8_MAX_WEIGHTS], *s[PK_FP8_MAX_WEIGHTS];
+  int32_t first[PK_FP8_MAX_WEIGHTS], N[PK_FP8_MAX_WEIGHTS], K[PK_FP8_MAX_WEIGHTS];      // first: its first workgroup
+  FastDiv by_nb[PK_FP8_MAX_WEIGHTS], by_kb[PK_FP8_MAX_WEIGHTS];
+  bool vec[PK_FP8_MAX_WEIGHTS];
+  int32_t count;
+};
 template <typename T>
-__global__ __launch_bounds__(THREADS) void quantize_weights_kernel(const T* __restrict__ w, uint8_t* __restrict__ q, uint8_t* __restrict__ t,
-                                                                   uint8_t* __restrict__ s, int N, int K, bool vec) {
+__global__ __launch_bounds__(THREADS) void quantize_weights_kernel(const Weights p) {
   constexpr int LD = BLOCK + 4;              // of the LDS rows: columns of bytes spread over the banks
   __shared__ uint32_t amax_of[4];
   __shared__ __attribute__((aligned(16))) uint8_t tile[BLOCK * LD];
-  const int kb = gridDim.x, nb = gridDim.y;
-  const int64_t e = blockIdx.z;
-  const int n0 = blockIdx.y * BLOCK, k0 = blockIdx.x * BLOCK, Kp = kb * BLOCK, Np = nb * BLOCK;
+  int which = 0;
+  while (which + 1 < p.count && (int)blockIdx.x >= p.first[which + 1]) ++which;
+  const int N = p.N[which], K = p.K[which], kb = (K + BLOCK - 1) / BLOCK, nb = (N + BLOCK - 1) / BLOCK;
+  const bool vec = p.vec[which];
+  uint8_t *const __restrict__ q = p.q[which], *const __restrict__ t = p.t[which], *const __restrict__ s = p.s[which];
+  const int local = (int)blockIdx.x - p.first[which], row_block = pk_units::fastdiv(local, p.by_kb[which]), kblock = local - row_block * kb;
+  const int64_t e = pk_units::fastdiv(row_block, p.by_nb[which]);
+  const int nblock = row_block - (int)e * nb;
+  const int n0 = nblock * BLOCK, k0 = kblock * BLOCK, Kp = kb * BLOCK, Np = nb * BLOCK;
   const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, k = k0 + lane * 8;
-  const T* const src = w + e * N * K;
+  const T* const __restrict__ src = reinterpret_cast<const T*>(p.w[which]) + e * N * K;
   float f[8][8];
   uint32_t m = 0u;
 #pragma unroll
@@ -105,7 +119,7 @@ __global__ __launch_bounds__(THREADS) void quantize_weights_kernel(const T* __re
   const bool finite = m < pk_fp8::INF_BITS;
   const uint32_t byte = finite ? pk_fp8::scale_byte(m, pk_fp8::TOP_E4M3) : 127u;
   const float inv = pk_fp8::inverse_scale_of(byte);
-  if (threadIdx.x == 0) s[(e * nb + blockIdx.y) * kb + blockIdx.x] = (uint8_t)byte;
+  if (threadIdx.x == 0) s[(e * nb + nblock) * kb + kblock] = (uint8_t)byte;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     u32x2_t c;
@@ -1175,23 +1189,30 @@ int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map, int64
   return PK_OK;
 }
 
-int pk_fp8_quantize_weights(const void* w, int dtype, uint8_t* q, uint8_t* q_t, uint8_t* scales, int64_t E, int64_t N, int64_t K,
-                            pk_stream_t stream) {
-  if (E < 0 || N <= 0 || K <= 0 || !pk_dtype_ok(dtype)) return PK_ERR_ARG;
-  if (E == 0) return PK_OK;
-  if (!all_set({w, q, scales})) return PK_ERR_ARG;
-  if (!all_aligned({q, q_t})) return PK_ERR_ALIGN;
-  const int64_t nb = blocks_of(N), kb = blocks_of(K);
-  if (E > 65535 || nb > 65535 || kb > 0x7fffffll) return PK_ERR_SHAPE;
-  const bool vec = K * (int64_t)pk_dtype_size(dtype) % 16 == 0 && pk_aligned16(w);
+int pk_fp8_quantize_weights(int count, const void* const* w, int dtype, uint8_t* const* q, uint8_t* const* q_t, uint8_t* const* scales, int64_t E,
+                            const int64_t* N, const int64_t* K, pk_stream_t stream) {
+  if (count < 0 || count > PK_FP8_MAX_WEIGHTS || E < 0 || !pk_dtype_ok(dtype)) return PK_ERR_ARG;
+  if (count == 0 || E == 0) return PK_OK;
+  if (!all_set({w, q, scales, N, K})) return PK_ERR_ARG;
+  Weights p = {};
+  p.count = count;
+  int64_t blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    if (N[i] <= 0 || K[i] <= 0 || !all_set({w[i], q[i], scales[i]})) return PK_ERR_ARG;
+    if (!all_aligned({q[i], q_t ? q_t[i] : nullptr})) return PK_ERR_ALIGN;
+    if (N[i] > 0x7fffff00ll || K[i] > 0x7fffff00ll) return PK_ERR_SHAPE;
+    const int64_t nb = blocks_of(N[i]), kb = blocks_of(K[i]);
+    if (E > 0x7fffffffll / nb || E * nb > (0x7fffffffll - blocks) / kb) return PK_ERR_SHAPE;
+    p.w[i] = w[i]; p.q[i] = q[i]; p.t[i] = q_t ? q_t[i] : nullptr; p.s[i] = scales[i];
+    p.first[i] = (int32_t)blocks; p.N[i] = (int32_t)N[i]; p.K[i] = (int32_t)K[i];
+    p.by_nb[i] = pk_units::make_fastdiv(nb); p.by_kb[i] = pk_units::make_fastdiv(kb);
+    p.vec[i] = K[i] * (int64_t)pk_dtype_size(dtype) % 16 == 0 && pk_aligned16(w[i]);
+    blocks += E * nb * kb;
+  }
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)kb, (unsigned)nb, (unsigned)E), block(THREADS);
-  if (dtype == PK_BF16)
-    PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_weights_kernel<bf16_t>), grid, block, 0, s, (const bf16_t*)w, q, q_t, scales, (int)N,
-                      (int)K, vec);
-  else
-    PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_weights_kernel<float>), grid, block, 0, s, (const float*)w, q, q_t, scales, (int)N,
-                      (int)K, vec);
+  const dim3 grid((unsigned)blocks), block(THREADS);
+  if (dtype == PK_BF16) PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_weights_kernel<bf16_t>), grid, block, 0, s, p);
+  else PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_weights_kernel<float>), grid, block, 0, s, p);
   PK_RETURN_IF_LAUNCH_FAILED();
   return PK_OK;
 }

@@ -912,16 +912,6 @@ std::optional<Tensor> bmm_experts(const Tensor& w1, const Tensor& w2, const Tens
 int64_t whole_blocks(int64_t n) { return (n + PK_FP8_BLOCK - 1) / PK_FP8_BLOCK; }
 uint8_t* u8(const Tensor& t) { return static_cast<uint8_t*>(ptr(t)); }
 
-// Of one weight [E, N, K]: codes, scales and, where wanted, the transposed codes
-std::array<Tensor, 3> quantize_weight(const Tensor& w_, bool transposed) {
-  const Tensor w = contig(w_);
-  const int64_t E = w.size(0), N = w.size(1), K = w.size(2), nb = whole_blocks(N), kb = whole_blocks(K);
-  const auto f8 = w.options().dtype(at::kFloat8_e4m3fn);
-  Tensor q = at::empty({E, N, kb * PK_FP8_BLOCK}, f8), s = at::empty({E, nb, kb}, w.options().dtype(at::kFloat8_e8m0fnu)), t;
-  if (transposed) t = at::empty({E, K, nb * PK_FP8_BLOCK}, f8);
-  PK_CALL(pk_fp8_quantize_weights, ptr(w), dtype_code(w), u8(q), u8(t), u8(s), E, N, K, stream_of(w));
-  return {q, s, t};
-}
 // [q1, q2, q3, s1, s2, s3, t1, t2, t3]; the transposed codes undefined where not wanted
 std::vector<Tensor> quantize_experts(const Tensor& w1, const Tensor& w2, const Tensor& w3, bool transposed) {
   require_gpu(w1);
@@ -934,8 +924,21 @@ std::vector<Tensor> quantize_experts(const Tensor& w1, const Tensor& w2, const T
   same_device(w1, {&w2, &w3});
   at::NoGradGuard no_grad;
   c10::hip::HIPGuard device(w1.device().index());
-  const auto a = quantize_weight(w1, transposed), b = quantize_weight(w2, transposed), c = quantize_weight(w3, transposed);
-  return {a[0], b[0], c[0], a[1], b[1], c[1], a[2], b[2], c[2]};
+  const Tensor w[3] = {contig(w1), contig(w2), contig(w3)};
+  const int64_t E = w1.size(0), N[3] = {w1.size(1), w2.size(1), w3.size(1)}, K[3] = {w1.size(2), w2.size(2), w3.size(2)};
+  const auto f8 = w1.options().dtype(at::kFloat8_e4m3fn);
+  std::vector<Tensor> out(9);
+  const void* from[3];
+  uint8_t *q[3], *t[3], *s[3];
+  for (int i = 0; i < 3; ++i) {
+    const int64_t nb = whole_blocks(N[i]), kb = whole_blocks(K[i]);
+    out[i] = at::empty({E, N[i], kb * PK_FP8_BLOCK}, f8);
+    out[3 + i] = at::empty({E, nb, kb}, w1.options().dtype(at::kFloat8_e8m0fnu));
+    if (transposed) out[6 + i] = at::empty({E, K[i], nb * PK_FP8_BLOCK}, f8);
+    from[i] = ptr(w[i]); q[i] = u8(out[i]); s[i] = u8(out[3 + i]); t[i] = u8(out[6 + i]);
+  }
+  PK_CALL(pk_fp8_quantize_weights, 3, from, dtype_code(w1), q, t, s, E, N, K, stream_of(w1));
+  return out;
 }
 // Rows of x [., K] in blocks: (codes [R, K'], scales [R, K' / 128])
 std::pair<Tensor, Tensor> quantize_rows(const Tensor& x_, const OptTensor& row_map_, int64_t map_div) {

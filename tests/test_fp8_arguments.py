@@ -20,7 +20,7 @@ def p():
 
 def test_quantize(p):
     lib = _lib.load()
-    rows, weights = lib.pk_fp8_quantize_rows, lib.pk_fp8_quantize_weights
+    rows = lib.pk_fp8_quantize_rows
     assert rows(p, 7, None, 1, p, p, 1, 128, None) == ARG
     assert rows(p, 1, None, 0, p, p, 1, 128, None) == ARG
     assert rows(p, 1, None, 1, p, p, -1, 128, None) == ARG
@@ -30,11 +30,17 @@ def test_quantize(p):
     assert rows(p, 1, None, 1, p, p, 2 ** 31, 128, None) == SHAPE
     assert rows(p, 1, None, 1, p, p, 2 ** 30, 1024, None) == SHAPE
     assert rows(None, 1, None, 1, None, None, 0, 128, None) == 0
-    assert weights(p, 1, p, p, p, -1, 1, 1, None) == ARG and weights(p, 1, p, p, p, 1, 0, 1, None) == ARG
-    assert weights(p, 2, p, p, p, 1, 1, 1, None) == ARG and weights(p, 1, None, p, p, 1, 1, 1, None) == ARG
-    assert weights(p, 1, p, p + 8, p, 1, 1, 1, None) == ALIGN
-    assert weights(p, 1, p, p, p, 65536, 1, 1, None) == SHAPE
-    assert weights(None, 1, None, None, None, 0, 1, 1, None) == 0
+
+    def weights(count=1, w=p, dtype=1, q=p, t=p, sc=p, E=1, N=1, K=1):
+        at = lambda v: (ctypes.c_void_p * 4)(*[v] * 4)  # noqa: E731
+        size = lambda v: (ctypes.c_int64 * 4)(*[v] * 4)  # noqa: E731
+        return lib.pk_fp8_quantize_weights(count, at(w), dtype, at(q), at(t), at(sc), E, size(N), size(K), None)
+
+    assert [weights(E=-1), weights(N=0), weights(K=0), weights(dtype=2), weights(w=None), weights(q=None), weights(sc=None), weights(count=-1),
+            weights(count=4)] == [ARG] * 9
+    assert [weights(q=p + 8), weights(t=p + 8)] == [ALIGN] * 2
+    assert [weights(E=2 ** 31), weights(E=2 ** 20, N=2 ** 18), weights(E=2 ** 29, N=256, K=256), weights(count=3, E=2 ** 30), weights(N=2 ** 31)] == [SHAPE] * 5
+    assert weights(E=0, w=None) == 0 and weights(count=0) == 0 and lib.pk_fp8_quantize_weights(1, None, 1, None, None, None, 1, None, None, None) == ARG
 
 
 def test_products(p):
