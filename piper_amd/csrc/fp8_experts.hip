@@ -44,27 +44,39 @@ __device__ __forceinline__ void load8(const T* p, int have, bool vec, float (&f)
 }
 
 // ------------------------------------------------------------------------------------------------ rows
-// 16 lanes to a block, one pass: 2 (bf16) or 4 bytes read and 1 written per value, bound by the memory (32,768 x 2048 bf16: 37 us,
-// 5.4 TB/s, where a copy of 2 GiB reaches 4.9).
-// One block of a row, by 16 lanes.
-template <typename T>
-__device__ __forceinline__ void quantize_block(const T* x, int64_t src, uint8_t* q, uint8_t* s, int64_t unit, int r, int K, int kb, bool vec) {
-  const int lane = threadIdx.x & 15, b = (int)(unit - (int64_t)r * kb), k = b * BLOCK + lane * 8;
-  float f[8];
-  load8<T>(x + src * K + k, K - k, vec, f);
-  uint32_t codes[2], byte;
-  pk_fp8::quantize8(f, codes, byte);
-  *reinterpret_cast<u32x2_t*>(q + unit * BLOCK + lane * 8) = u32x2_t{codes[0], codes[1]};
-  if (lane == 0) s[(int64_t)r * scale_row(kb) + b] = (uint8_t)byte;
+// 16 lanes to a block, one pass: 2 (bf16) or 4 bytes read and 1 written per value, bound by the memory (32,768 x 2048 bf16: 35 us,
+// 5.7 TB/s, where a copy of 2 GiB reaches 4.9; with one or four blocks on their way in a lane 38).
+// N blocks of rows, by 16 lanes; block i is number `unit` + i * step of all, and there if below `units`.
+template <typename T, int N, typename Source>
+__device__ __forceinline__ void quantize_blocks(const T* x, Source&& source, uint8_t* q, uint8_t* s, int64_t unit, int step, int64_t units, int K,
+                                                int kb, FastDiv by_kb, bool vec) {
+  const int lane = threadIdx.x & 15;
+  int r[N], b[N];
+  float f[N][8];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t u = min(unit + i * step, units - 1);
+    r[i] = pk_units::fastdiv((int)u, by_kb);
+    b[i] = (int)(u - (int64_t)r[i] * kb);
+    const int k = b[i] * BLOCK + lane * 8;
+    load8<T>(x + source(r[i]) * K + k, K - k, vec, f[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (unit + i * step >= units) return;    // whole groups of 16 lanes
+    uint32_t codes[2], byte;
+    pk_fp8::quantize8(f[i], codes, byte);
+    *reinterpret_cast<u32x2_t*>(q + (unit + i * step) * BLOCK + lane * 8) = u32x2_t{codes[0], codes[1]};
+    if (lane == 0) s[(int64_t)r[i] * scale_row(kb) + b[i]] = (uint8_t)byte;
+  }
 }
+constexpr int ROW_BLOCKS = 2;
 template <typename T>
 __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ row_map, FastDiv map_div,
                                                                 uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t units, int K, int kb,
                                                                 FastDiv by_kb, bool vec) {
-  const int64_t unit = (int64_t)blockIdx.x * (THREADS / 16) + (threadIdx.x >> 4);
-  if (unit >= units) return;                 // whole groups of 16 lanes
-  const int r = pk_units::fastdiv((int)unit, by_kb);
-  quantize_block<T>(x, row_map ? pk_units::fastdiv(row_map[r], map_div) : r, q, s, unit, r, K, kb, vec);
+  const auto source = [&](int r) { return (int64_t)(row_map ? pk_units::fastdiv(row_map[r], map_div) : r); };
+  quantize_blocks<T, ROW_BLOCKS>(x, source, q, s, (int64_t)blockIdx.x * (THREADS / 16 * ROW_BLOCKS) + (threadIdx.x >> 4), THREADS / 16, units, K, kb, by_kb, vec);
 }
 
 // ------------------------------------------------------------------------------------------------ weights
@@ -154,8 +166,8 @@ __global__ __launch_bounds__(THREADS) void quantize_weights_kernel(const Weights
 
 // ------------------------------------------------------------------------------------------------ plan
 // Where every expert's rows are and which expert a tile of TILE_ROWS rows belongs to, once for all products of a pass: a workgroup of a product
-// then finds its tile with one read of the table, where a search through starts[] costs it three dependent ones, 2 us each while the
-// chip is busy (per workgroup, 512 rows an expert, 2048 x 768: 6.5 -> 3 us in front of a loop of 30).
+// then finds its next unit with one read of the table, requested while it multiplies the one before, where a search through starts[] takes
+// three dependent ones, 2 us each while the chip is busy.
 //   [E + 1] starts (cut off at A), tiles, padding to 8; then for every tile 8 words: expert, its first tile, its tiles, its first
 //   row and the row behind its last, padding.  Counts that do not fit into A rows, or are negative, cannot lead a kernel out of bounds.
 constexpr int TILE_ROWS = 128, PLAN_THREADS = 1024, ENTRY = 8;
@@ -221,7 +233,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const void* counts, 
 }
 
 // What a pass begins with, in one launch: its rows in blocks, and in front of the forward its plan (by the first workgroup), in front of
-// the backward a row map.  (1,777 tokens of 2048 in 8 places each: 18 us, and 5 for either of the others by itself.)
+// the backward a row map.  (1,777 tokens of 2048 in 8 places each: 17 us, and 5 for either of the others by itself.)
 // The map: every row its own number, those of no expert the last one that has one, for pk_grouped_swiglu_wgrad_scaled_t, which multiplies
 // rows behind an expert's last one by zeros.  What stands in rows of no expert (it may be anything) is thereby not read.
 struct Begin {
@@ -242,11 +254,13 @@ __global__ __launch_bounds__(PLAN_THREADS) void begin_kernel(const Begin p) {
     make_plan(p.counts, p.is_i64, p.E, p.A, p.plan);
     return;
   }
-  const int64_t unit = (int64_t)(blockIdx.x - (FORWARD ? 1 : 0)) * (PLAN_THREADS / 16) + (threadIdx.x >> 4);
-  if (unit >= p.units) return;               // whole groups of 16 lanes
-  const int r = pk_units::fastdiv((int)unit, p.by_kb);
-  quantize_block<bf16_t>(p.x, r, p.q, p.s, unit, r, p.K, p.kb, p.vec);
-  if (!FORWARD && p.map && unit == (int64_t)r * p.kb && (threadIdx.x & 15) == 0) p.map[r] = r < *p.owned ? r : *p.owned > 0 ? *p.owned - 1 : 0;
+  const int group = threadIdx.x >> 4;
+  const int64_t unit = (int64_t)(blockIdx.x - (FORWARD ? 1 : 0)) * (PLAN_THREADS / 16 * ROW_BLOCKS) + group;
+  quantize_blocks<bf16_t, ROW_BLOCKS>(p.x, [](int r) { return (int64_t)r; }, p.q, p.s, unit, PLAN_THREADS / 16, p.units, p.K, p.kb, p.by_kb, p.vec);
+  if (!FORWARD && p.map) {
+    const int64_t r = (int64_t)blockIdx.x * PLAN_THREADS + threadIdx.x;
+    if (r < p.A) p.map[r] = (int32_t)(r < *p.owned ? r : *p.owned > 0 ? *p.owned - 1 : 0);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ products
@@ -1178,7 +1192,7 @@ int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map, int64
   const bool vec = K * (int64_t)pk_dtype_size(dtype) % 16 == 0 && pk_aligned16(x);
   const FastDiv div = pk_units::make_fastdiv(row_map_div), by_kb = pk_units::make_fastdiv(kb);
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)pk_ceil_div(units, THREADS / 16)), block(THREADS);
+  const dim3 grid((unsigned)pk_ceil_div(units, THREADS / 16 * ROW_BLOCKS)), block(THREADS);
   if (dtype == PK_BF16)
     PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_rows_kernel<bf16_t>), grid, block, 0, s, (const bf16_t*)x, row_map, div, q, scales,
                       units, (int)K, (int)kb, by_kb, vec);
@@ -1241,7 +1255,7 @@ static int begin(Begin p, const void* x, uint8_t* q, uint8_t* scales, int64_t A,
   p.units = A * p.kb;
   if (p.units > 0x7fffffffll) return PK_ERR_SHAPE;
   p.vec = bf16_pieces(K, {x});
-  const dim3 grid((unsigned)(pk_ceil_div(p.units, PLAN_THREADS / 16) + (forward ? 1 : 0))), block(PLAN_THREADS);
+  const dim3 grid((unsigned)(pk_ceil_div(p.units, PLAN_THREADS / 16 * ROW_BLOCKS) + (forward ? 1 : 0))), block(PLAN_THREADS);
   const hipStream_t s = (hipStream_t)stream;
   if (forward) PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (begin_kernel<true>), grid, block, 0, s, p);
   else PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (begin_kernel<false>), grid, block, 0, s, p);
