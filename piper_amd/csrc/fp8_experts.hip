@@ -363,33 +363,22 @@ __device__ __forceinline__ bf16x8_t kept(bf16x8_t v) {
   return __builtin_bit_cast(bf16x8_t, w);
 }
 // Eight neighbouring bf16 of a row, of which the first `have` are there (any number); vec: rows are whole 16-byte pieces
-__device__ __forceinline__ void store8(bf16_t* p, int have, bool vec, bf16x8_t v) {
-  if (vec) {
-    if (have > 0) *reinterpret_cast<bf16x8_t*>(p) = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < have) p[i] = v[i];
-  }
+__device__ __forceinline__ void store8(bf16_t* p, int have, bf16x8_t v) {      // whole pieces
+  if (have > 0) *reinterpret_cast<bf16x8_t*>(p) = v;
 }
-__device__ __forceinline__ void store16(bf16_t* p, int have, bool vec, const float (&f)[16]) {
+// 16 values as two pieces
+__device__ __forceinline__ void pack16(const float (&f)[16], bf16x8_t (&v)[2]) {
   float a[8], b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) { a[i] = f[i]; b[i] = f[8 + i]; }
-  store8(p, have, vec, pack8(a));
-  store8(p + 8, have - 8, vec, pack8(b));
+  v[0] = pack8(a);
+  v[1] = pack8(b);
 }
-__device__ __forceinline__ void load16(const bf16_t* p, int have, bool vec, bf16x8_t (&v)[2]) {
+__device__ __forceinline__ void load16(const bf16_t* p, int have, bf16x8_t (&v)[2]) {      // whole pieces
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     v[h] = bf16x8_t{};
-    if (vec) {
-      if (have > 8 * h) v[h] = *reinterpret_cast<const bf16x8_t*>(p + 8 * h);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (8 * h + i < have) v[h][i] = p[8 * h + i];
-    }
+    if (have > 8 * h) v[h] = *reinterpret_cast<const bf16x8_t*>(p + 8 * h);
   }
 }
 __device__ __forceinline__ float held(float v) { return (float)(bf16_t)v; }
@@ -403,6 +392,34 @@ typedef short shortx8_t __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ int tr_swz(int r) { return ((r & 3) << 1 | (r >> 2 & 1)) ^ (r >> 3 & 1); }
 __device__ __forceinline__ void put_row(char* t, int row, int piece, bf16x8_t v) {
   *reinterpret_cast<bf16x8_t*>(t + row * 128 + ((piece ^ tr_swz(row)) << 4)) = v;
+}
+__device__ __forceinline__ bf16x8_t get_row(const char* t, int row, int piece) {
+  return *reinterpret_cast<const bf16x8_t*>(t + row * 128 + ((piece ^ tr_swz(row)) << 4));
+}
+__device__ __forceinline__ int tr_value(int row, int col) { return row * 128 + (((col >> 3) ^ tr_swz(row)) << 4) + (col & 7) * 2; }
+// Rows whose pieces are not 16-byte aligned: a row's 64 columns at a time, a lane to a column, `to` its place in row 0.  (Values by themselves
+// from where the products leave them touch 64 lines with an instruction: 4 experts of 2,700 rows 1145 x 1536, down 91 -> 45 us,
+// d_x 116 -> 71; 24 of 200 rows 1001 x 361, gate and up 44 -> 25, d_h 62 -> 31.)
+__device__ __forceinline__ void store_rows(const char* t, int lane, bf16_t* to, int64_t ld, int rows, bool in) {
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    bf16_t v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] = *reinterpret_cast<const bf16_t*>(t + tr_value(r0 + r, lane));
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (in && r0 + r < rows) to[(r0 + r) * ld] = v[r];
+  }
+}
+__device__ __forceinline__ void load_rows(char* t, int lane, const bf16_t* from, int64_t ld, int rows, bool in) {
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    bf16_t v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] = in && r0 + r < rows ? from[(r0 + r) * ld] : (bf16_t)0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) *reinterpret_cast<bf16_t*>(t + tr_value(r0 + r, lane)) = v[r];
+  }
 }
 __device__ __forceinline__ void store_columns(const char* t, int lane, bf16_t* to) {
   // within 16 lanes, lane i points at 4 neighbouring columns of row i / 4 and receives 4 neighbouring rows of column i
@@ -611,16 +628,32 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
     const int half16 = (lane >> 5) * 16;
     // BWD: the wave's part of g and u, requested before the next unit's k-tiles, which would be waited for as well
     bf16x8_t gs[TM][TN][2], us[TM][TN][2];
+    [[maybe_unused]] char* const tr = spare + 8 * BM * 4 + wave * TR_BYTES;
+    [[maybe_unused]] const int col = u_n0 + wn * 64 + lane;      // of a lane that has a column
     if constexpr (EPI == BWD) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const int r = wave_row + 32 * i + (lane & 31), n = u_n0 + wn * 64 + 32 * j + half16;
+      for (int i = 0; i < TM; ++i) {
+        if constexpr (VEC) {
+          const int r = wave_row + 32 * i + (lane & 31);
           const int64_t row = u_row0 + (r < u_rows ? r : 0);
-          load16(p.G + row * p.N + n, p.N - n, VEC, gs[i][j]);
-          load16(p.U + row * p.N + n, p.N - n, VEC, us[i][j]);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const int n = u_n0 + wn * 64 + 32 * j + half16;
+            load16(p.G + row * p.N + n, p.N - n, gs[i][j]);
+            load16(p.U + row * p.N + n, p.N - n, us[i][j]);
+          }
+        } else {
+          const int64_t at = (int64_t)(u_row0 + wave_row + 32 * i) * p.N + col;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            load_rows(tr, lane, (w ? p.U : p.G) + at, p.N, u_rows - wave_row - 32 * i, col < p.N);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) (w ? us : gs)[i][j][k] = get_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k);
+          }
         }
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     if (more) {
@@ -638,9 +671,19 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
 #pragma unroll
           for (int j = 0; j < TN; ++j) {
             float f[16];
+            bf16x8_t v[2];
             exchange_halves(acc[i][j], f);
+            pack16(f, v);
             const int n = u_n0 + wn * 64 + 32 * j + half16;
-            if (r < u_rows) store16(p.O0 + (int64_t)(u_row0 + r) * p.N + n, p.N - n, VEC, f);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              if constexpr (!VEC) put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, v[k]);
+              else if (r < u_rows) store8(p.O0 + (int64_t)(u_row0 + r) * p.N + n + 8 * k, p.N - n - 8 * k, v[k]);
+            }
+          }
+          if constexpr (!VEC) {
+            const int first = wave_row + 32 * i;
+            store_rows(tr, lane, p.O0 + (int64_t)(u_row0 + first) * p.N + col, p.N, u_rows - first, col < p.N);
           }
         }
       }
@@ -665,10 +708,25 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
           m = umax(m, __float_as_uint(h[i][v]) & 0x7fffffffu);
         }
         amax[wn * BM + r] = umax(m, other_half(m));
-        if (live && p.O0) {
+        if (p.O0) {
           const int64_t o = (int64_t)(u_row0 + r) * p.N + n;
-          store16(p.O0 + o, p.N - n, VEC, g);
-          store16(p.O1 + o, p.N - n, VEC, u);
+          bf16x8_t gv[2], uv[2];
+          pack16(g, gv);
+          pack16(u, uv);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if constexpr (!VEC) {              // 32 columns of g, then those of u
+              put_row(tr, lane & 31, 2 * (lane >> 5) + k, gv[k]);
+              put_row(tr, lane & 31, 4 + 2 * (lane >> 5) + k, uv[k]);
+            } else if (live) {
+              store8(p.O0 + o + 8 * k, p.N - n - 8 * k, gv[k]);
+              store8(p.O1 + o + 8 * k, p.N - n - 8 * k, uv[k]);
+            }
+          }
+          if constexpr (!VEC) {
+            const int first = wave_row + 32 * i, c = u_n0 + wn * 32 + (lane & 31);
+            store_rows(tr, lane, (lane < 32 ? p.O0 : p.O1) + (int64_t)(u_row0 + first) * p.N + c, p.N, u_rows - first, c < p.N);
+          }
         }
       }
       block_barrier();
@@ -685,7 +743,6 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
     } else {
       const int nb = u_nt * (BN / BLOCK) + (wn >> 1);      // the wave's block of columns, shared with its neighbour
       uint32_t* const amax = reinterpret_cast<uint32_t*>(spare);      // [2: d_g, d_u][4 waves][128 rows]
-      char* const tr = spare + 8 * BM * 4 + wave * TR_BYTES;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         asm volatile("" ::: "memory");       // the second half's work not before the first half has left its registers
@@ -720,31 +777,38 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
             asm volatile("" : "+v"(mg), "+v"(mu));      // step by step: as one reduction it would keep all values
             gs[i][j][k] = kept(pack8(g));    // d_g and d_u take the place of g and u
             us[i][j][k] = kept(pack8(u));
-            if constexpr (TRANSPOSED) {
+            if constexpr (TRANSPOSED || !VEC) {
               put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, pack8(h));
             } else if (live) {
-              store8(p.O0 + row * p.N + n, have, VEC, gs[i][j][k]);
-              store8(p.O1 + row * p.N + n, have, VEC, us[i][j][k]);
-              store8(p.O2 + row * p.N + n, have, VEC, pack8(h));
+              store8(p.O0 + row * p.N + n, have, gs[i][j][k]);
+              store8(p.O1 + row * p.N + n, have, us[i][j][k]);
+              store8(p.O2 + row * p.N + n, have, pack8(h));
             }
             __builtin_amdgcn_sched_barrier(0);
           }
         }
-        if constexpr (TRANSPOSED) {
+        if constexpr (TRANSPOSED || !VEC) {
           if (chunk) {
-            const int64_t padded = (u_begin & ~63) + 64 * (int64_t)u_e + u_mt * BM + wave_row + 32 * i;
-            const int64_t to = (padded / 32 * p.N + u_n0 + wn * 64) * 32;
-            store_columns(tr, lane, p.O2 + to);
+            const int first = wave_row + 32 * i;
+            const auto store = [&](bf16_t* out) {
+              if constexpr (TRANSPOSED) {
+                const int64_t padded = (u_begin & ~63) + 64 * (int64_t)u_e + u_mt * BM + first;
+                store_columns(tr, lane, out + (padded / 32 * p.N + u_n0 + wn * 64) * 32);
+              } else {
+                store_rows(tr, lane, out + (int64_t)(u_row0 + first) * p.N + col, p.N, u_rows - first, col < p.N);
+              }
+            };
+            store(p.O2);
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
               for (int k = 0; k < 2; ++k) put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, gs[i][j][k]);
-            store_columns(tr, lane, p.O0 + to);
+            store(p.O0);
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
               for (int k = 0; k < 2; ++k) put_row(tr, lane & 31, 4 * j + 2 * (lane >> 5) + k, us[i][j][k]);
-            store_columns(tr, lane, p.O1 + to);
+            store(p.O1);
           }
         }
         amax[wn * BM + r] = umax(mg, other_half(mg));
