@@ -25,18 +25,15 @@ inline int64_t blocks_of(int64_t n) { return pk_ceil_div(n, BLOCK); }
 // bytes of a row of scales: whole words
 __host__ __device__ inline int scale_row(int blocks) { return (blocks + 3) & ~3; }
 
+// 8 neighbouring values, zeros behind the first `have`.  Rows of odd widths start anywhere: 16-byte loads need no alignment (24 experts'
+// weights of 363 x 1000 in fp32 41 -> 34 us against value by value, 10,975 rows of 1145 bf16 values 19 -> 10).
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int have, bool vec, float (&f)[8]) {
-  if (vec && have >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      const bf16x8_t v = *reinterpret_cast<const bf16x8_t*>(p);
+__device__ __forceinline__ void load8(const T* p, int have, float (&f)[8]) {
+  if (have >= 8) {
+    T v[8];
+    __builtin_memcpy(v, p, sizeof v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = (float)v[i];
-    } else {
-      const floatx4_t a = *reinterpret_cast<const floatx4_t*>(p), b = *reinterpret_cast<const floatx4_t*>(p + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { f[i] = a[i]; f[4 + i] = b[i]; }
-    }
+    for (int i = 0; i < 8; ++i) f[i] = (float)v[i];
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = i < have ? pk_to_float<T>(p[i]) : 0.f;
@@ -49,7 +46,7 @@ __device__ __forceinline__ void load8(const T* p, int have, bool vec, float (&f)
 // N blocks of rows, by 16 lanes; block i is number `unit` + i * step of all, and there if below `units`.
 template <typename T, int N, typename Source>
 __device__ __forceinline__ void quantize_blocks(const T* x, Source&& source, uint8_t* q, uint8_t* s, int64_t unit, int step, int64_t units, int K,
-                                                int kb, FastDiv by_kb, bool vec) {
+                                                int kb, FastDiv by_kb) {
   const int lane = threadIdx.x & 15;
   int r[N], b[N];
   float f[N][8];
@@ -59,7 +56,7 @@ __device__ __forceinline__ void quantize_blocks(const T* x, Source&& source, uin
     r[i] = pk_units::fastdiv((int)u, by_kb);
     b[i] = (int)(u - (int64_t)r[i] * kb);
     const int k = b[i] * BLOCK + lane * 8;
-    load8<T>(x + source(r[i]) * K + k, K - k, vec, f[i]);
+    load8<T>(x + source(r[i]) * K + k, K - k, f[i]);
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -74,21 +71,20 @@ constexpr int ROW_BLOCKS = 2;
 template <typename T>
 __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ row_map, FastDiv map_div,
                                                                 uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t units, int K, int kb,
-                                                                FastDiv by_kb, bool vec) {
+                                                                FastDiv by_kb) {
   const auto source = [&](int r) { return (int64_t)(row_map ? pk_units::fastdiv(row_map[r], map_div) : r); };
-  quantize_blocks<T, ROW_BLOCKS>(x, source, q, s, (int64_t)blockIdx.x * (THREADS / 16 * ROW_BLOCKS) + (threadIdx.x >> 4), THREADS / 16, units, K, kb, by_kb, vec);
+  quantize_blocks<T, ROW_BLOCKS>(x, source, q, s, (int64_t)blockIdx.x * (THREADS / 16 * ROW_BLOCKS) + (threadIdx.x >> 4), THREADS / 16, units, K, kb, by_kb);
 }
 
 // ------------------------------------------------------------------------------------------------ weights
 // A workgroup has one block of 128 x 128: 16 lanes to a row of it, the codes once row-major and once, through the LDS, transposed.  Bound
 // by the memory: 128 experts' three weights of 2048 x 768 in bf16 take 457 us, 5.3 TB/s.  All weights of a call share a launch (24 experts'
-// three of 363 x 1000 in fp32, 576 workgroups each: 41 us, in three launches 57; the others 469).
+// three of 363 x 1000 in fp32, 576 workgroups each: three launches took 57 us where one took 41; those 469).
 struct Weights {
   const void* w[PK_FP8_MAX_WEIGHTS];
   uint8_t *q[PK_FP8_MAX_WEIGHTS], *t[PK_FP8_MAX_WEIGHTS], *s[PK_FP8_MAX_WEIGHTS];
   int32_t first[PK_FP8_MAX_WEIGHTS], N[PK_FP8_MAX_WEIGHTS], K[PK_FP8_MAX_WEIGHTS];      // first: its first workgroup
   FastDiv by_nb[PK_FP8_MAX_WEIGHTS], by_kb[PK_FP8_MAX_WEIGHTS];
-  bool vec[PK_FP8_MAX_WEIGHTS];
   int32_t count;
 };
 template <typename T>
@@ -99,7 +95,6 @@ __global__ __launch_bounds__(THREADS) void quantize_weights_kernel(const Weights
   int which = 0;
   while (which + 1 < p.count && (int)blockIdx.x >= p.first[which + 1]) ++which;
   const int N = p.N[which], K = p.K[which], kb = (K + BLOCK - 1) / BLOCK, nb = (N + BLOCK - 1) / BLOCK;
-  const bool vec = p.vec[which];
   uint8_t *const __restrict__ q = p.q[which], *const __restrict__ t = p.t[which], *const __restrict__ s = p.s[which];
   const int local = (int)blockIdx.x - p.first[which], row_block = pk_units::fastdiv(local, p.by_kb[which]), kblock = local - row_block * kb;
   const int64_t e = pk_units::fastdiv(row_block, p.by_nb[which]);
@@ -112,7 +107,7 @@ __global__ __launch_bounds__(THREADS) void quantize_weights_kernel(const Weights
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int n = n0 + row + 16 * i;
-    load8<T>(src + (int64_t)(n < N ? n : n0) * K + k, n < N ? K - k : 0, vec, f[i]);
+    load8<T>(src + (int64_t)(n < N ? n : n0) * K + k, n < N ? K - k : 0, f[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t b = __float_as_uint(f[i][j]) & 0x7fffffffu;
@@ -242,7 +237,6 @@ struct Begin {
   int64_t units, A;
   int32_t K, kb, E, is_i64;
   FastDiv by_kb;
-  bool vec;
   const void* counts;       // forward
   int32_t* plan;
   const int32_t* owned;     // backward: rows that have an expert
@@ -256,7 +250,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void begin_kernel(const Begin p) {
   }
   const int group = threadIdx.x >> 4;
   const int64_t unit = (int64_t)(blockIdx.x - (FORWARD ? 1 : 0)) * (PLAN_THREADS / 16 * ROW_BLOCKS) + group;
-  quantize_blocks<bf16_t, ROW_BLOCKS>(p.x, [](int r) { return (int64_t)r; }, p.q, p.s, unit, PLAN_THREADS / 16, p.units, p.K, p.kb, p.by_kb, p.vec);
+  quantize_blocks<bf16_t, ROW_BLOCKS>(p.x, [](int r) { return (int64_t)r; }, p.q, p.s, unit, PLAN_THREADS / 16, p.units, p.K, p.kb, p.by_kb);
   if (!FORWARD && p.map) {
     const int64_t r = (int64_t)blockIdx.x * PLAN_THREADS + threadIdx.x;
     if (r < p.A) p.map[r] = (int32_t)(r < *p.owned ? r : *p.owned > 0 ? *p.owned - 1 : 0);
@@ -362,7 +356,7 @@ __device__ __forceinline__ bf16x8_t kept(bf16x8_t v) {
   asm volatile("" : "+v"(w));
   return __builtin_bit_cast(bf16x8_t, w);
 }
-// Eight neighbouring bf16 of a row, of which the first `have` are there (any number); vec: rows are whole 16-byte pieces
+// Eight neighbouring bf16 of a row in whole 16-byte pieces, of which the first `have` are there (any number)
 __device__ __forceinline__ void store8(bf16_t* p, int have, bf16x8_t v) {      // whole pieces
   if (have > 0) *reinterpret_cast<bf16x8_t*>(p) = v;
 }
@@ -913,8 +907,8 @@ struct Few {
   float* h;                 // [A, I]
   bf16_t* y;
   int32_t n_cols;           // column tiles
+  bool whole;               // H is a multiple of 8
   FastDiv by_cols;
-  bool vec;                 // x: rows are whole 16-byte pieces
 };
 
 // Sums over the lanes up to this one, cut off at `cap` (of numbers up to 2^31 that are not negative cutting off can be done at every
@@ -1017,9 +1011,9 @@ __global__ __launch_bounds__(512, 2) void gate_up_few_kernel(const Few p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int k = b * BLOCK + quarter * 32 + 8 * i, have = r < rows ? p.H - k : 0;
-        if (p.vec) {
+        if (p.whole) {
           xs[t][i] = bf16x8_t{};
-          if (have > 0) xs[t][i] = *reinterpret_cast<const bf16x8_t*>(x + b * BLOCK + 8 * i);
+          if (have > 0) __builtin_memcpy(&xs[t][i], x + b * BLOCK + 8 * i, 16);
         } else {
 #pragma unroll
           for (int v = 0; v < 8; ++v) xs[t][i][v] = v < have ? x[b * BLOCK + 8 * i + v] : (bf16_t)0.f;
@@ -1071,12 +1065,12 @@ __global__ __launch_bounds__(512, 2) void gate_up_few_kernel(const Few p) {
 // A row tile's rows of K values in blocks into the LDS, 16 lanes to a block; rows that are not there stay as they are, since no other
 // row sees them.
 template <typename T>
-__device__ __forceinline__ void rows_into_lds(const T* from, int64_t ld_from, int rows, int K, bool vec, uint8_t* q, int ld, uint8_t* qs) {
+__device__ __forceinline__ void rows_into_lds(const T* from, int64_t ld_from, int rows, int K, uint8_t* q, int ld, uint8_t* qs) {
   const int nb = (K + BLOCK - 1) / BLOCK;
   for (int i = threadIdx.x >> 4; i < rows * nb; i += (int)blockDim.x >> 4) {
     const int r = i / nb, b = i - r * nb, k = b * BLOCK + (threadIdx.x & 15) * 8;
     float f[8];
-    load8<T>(from + r * ld_from + k, K - k, vec, f);
+    load8<T>(from + r * ld_from + k, K - k, f);
     uint32_t codes[2], byte;
     pk_fp8::quantize8(f, codes, byte);
     *reinterpret_cast<u32x2_t*>(q + r * ld + k) = u32x2_t{codes[0], codes[1]};
@@ -1159,7 +1153,7 @@ __global__ __launch_bounds__(512, 4) void gate_up_stream_kernel(const Few p) {
   const int64_t at = ((int64_t)e * p.I + (n0 + r < p.I ? n0 + r : 0)) * Hp + quarter * 32, sat = ((int64_t)e * ib + ct) * hb;
   const uint8_t* const w[2] = {p.q1 + at, p.q3 + at};
   const uint8_t* const sw[2] = {p.s1 + sat, p.s3 + sat};
-  rows_into_lds<bf16_t>(p.x + (int64_t)row0 * p.H, p.H, rows, p.H, p.vec, q, ld, qs);
+  rows_into_lds<bf16_t>(p.x + (int64_t)row0 * p.H, p.H, rows, p.H, q, ld, qs);
   stream_columns<2, 4>(w, 0, sw, 0, hb, 1, q, ld, qs, false, [&](int, const floatx4_t (&acc)[2]) {
     if (r >= rows) return;
 #pragma unroll
@@ -1196,7 +1190,7 @@ __global__ __launch_bounds__(256, 4) void down_few_kernel(const Few p, int units
   uint8_t* const q = reinterpret_cast<uint8_t*>(smem);
   uint8_t* const qs = q + FEW_ROWS * ld;
   const int mine = min(tiles, (p.H - n0 + 15) / 16);
-  rows_into_lds<float>(p.h + (int64_t)row0 * p.I, p.I, rows, p.I, p.I % 4 == 0 && ((uintptr_t)p.h & 15) == 0, q, ld, qs);
+  rows_into_lds<float>(p.h + (int64_t)row0 * p.I, p.I, rows, p.I, q, ld, qs);
   __syncthreads();
   if (mine <= 0) return;
   for (int c0 = 0; c0 < mine;) {             // columns that share a row of scales, and whole tiles or a last one that is not
@@ -1253,16 +1247,15 @@ int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map, int64
   if (!pk_aligned16(q)) return PK_ERR_ALIGN;
   const int64_t kb = blocks_of(K), units = rows * kb;
   if (K > 0x7fffff00ll || rows > 0x7fffffffll || units > 0x7fffffffll || row_map_div > 0x7fffffffll) return PK_ERR_SHAPE;
-  const bool vec = K * (int64_t)pk_dtype_size(dtype) % 16 == 0 && pk_aligned16(x);
   const FastDiv div = pk_units::make_fastdiv(row_map_div), by_kb = pk_units::make_fastdiv(kb);
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)pk_ceil_div(units, THREADS / 16 * ROW_BLOCKS)), block(THREADS);
   if (dtype == PK_BF16)
     PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_rows_kernel<bf16_t>), grid, block, 0, s, (const bf16_t*)x, row_map, div, q, scales,
-                      units, (int)K, (int)kb, by_kb, vec);
+                      units, (int)K, (int)kb, by_kb);
   else
     PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_rows_kernel<float>), grid, block, 0, s, (const float*)x, row_map, div, q, scales,
-                      units, (int)K, (int)kb, by_kb, vec);
+                      units, (int)K, (int)kb, by_kb);
   PK_RETURN_IF_LAUNCH_FAILED();
   return PK_OK;
 }
@@ -1284,7 +1277,6 @@ int pk_fp8_quantize_weights(int count, const void* const* w, int dtype, uint8_t*
     p.w[i] = w[i]; p.q[i] = q[i]; p.t[i] = q_t ? q_t[i] : nullptr; p.s[i] = scales[i];
     p.first[i] = (int32_t)blocks; p.N[i] = (int32_t)N[i]; p.K[i] = (int32_t)K[i];
     p.by_nb[i] = pk_units::make_fastdiv(nb); p.by_kb[i] = pk_units::make_fastdiv(kb);
-    p.vec[i] = K[i] * (int64_t)pk_dtype_size(dtype) % 16 == 0 && pk_aligned16(w[i]);
     blocks += E * nb * kb;
   }
   hipStream_t s = (hipStream_t)stream;
@@ -1318,7 +1310,6 @@ static int begin(Begin p, const void* x, uint8_t* q, uint8_t* scales, int64_t A,
   p.by_kb = pk_units::make_fastdiv(p.kb);
   p.units = A * p.kb;
   if (p.units > 0x7fffffffll) return PK_ERR_SHAPE;
-  p.vec = bf16_pieces(K, {x});
   const dim3 grid((unsigned)(pk_ceil_div(p.units, PLAN_THREADS / 16 * ROW_BLOCKS) + (forward ? 1 : 0))), block(PLAN_THREADS);
   const hipStream_t s = (hipStream_t)stream;
   if (forward) PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (begin_kernel<true>), grid, block, 0, s, p);
@@ -1457,7 +1448,7 @@ int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64
   p.counts = counts; p.is_i64 = counts_is_i64; p.E = (int32_t)E; p.H = (int32_t)H; p.I = (int32_t)I; p.A = A;
   p.x = (const bf16_t*)x; p.q1 = w1; p.s1 = s1; p.q2 = w2; p.s2 = s2; p.q3 = w3; p.s3 = s3;
   p.g = (bf16_t*)g; p.u = (bf16_t*)u; p.h = h; p.y = (bf16_t*)y;
-  p.vec = bf16_pieces(H, {x});
+  p.whole = H % 8 == 0;
   const int64_t tiles = A / FEW_ROWS + (A < E ? A : E);
   // whole reductions to a wave where that gives every CU a workgroup, and four column tiles to a wave of down where that fills the chip
   // eight times (both : eight waves to a reduction : one column tile, us; 128 experts 2048 x 768, 2 rows each 146 : 176 : 154, 8
