@@ -499,6 +499,25 @@ PK_API int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, cons
 PK_API int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales,
                     const uint8_t* w1_t, const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3,
                     const int32_t* plan, void* d_x, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
+/* The same five with short sums: of the sum of 8 neighbouring products 13 bits below the largest one are kept, as the matrix
+ * instructions for 8-bit values do, where the products above are added in fp32.  For callers to whom 0.001 of a result's size counts less than
+ * the time; passes of up to 40 rows an expert, or 128 in all, are no faster for it and add in fp32. */
+PK_API int pk_fp8_gate_up_short(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w1, const uint8_t* s1,
+                         const uint8_t* w3, const uint8_t* s3, const int32_t* plan, void* g, void* u, uint8_t* h,
+                         uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
+PK_API int pk_fp8_down_short(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2,
+                      const int32_t* plan, void* y, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
+PK_API int pk_fp8_dgrad_dh_short(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2,
+                          const void* g, const void* u, const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8,
+                          uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, int64_t A, int64_t H, int64_t I,
+                          int64_t E, pk_stream_t stream);
+PK_API int pk_fp8_dgrad_dh_t_short(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2,
+                            const void* g, const void* u, const int32_t* plan, void* d_gT, void* d_uT, void* hT, int64_t ldt,
+                            uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales, int64_t A, int64_t H,
+                            int64_t I, int64_t E, pk_stream_t stream);
+PK_API int pk_fp8_dgrad_dx_short(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales,
+                          const uint8_t* w1_t, const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3,
+                          const int32_t* plan, void* d_x, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream);
 
 /* ------------------------------------------------------------- ZeRO bucket path */
 

@@ -128,6 +128,8 @@ SIGNATURES = {
     "pk_timing_select": (_c_int, [_c_int]),
     "pk_timing_kernel_name": (C.c_char_p, [_c_int]),
 }
+SIGNATURES.update({f"{name}_short": SIGNATURES[name] for name in
+                   ("pk_fp8_gate_up", "pk_fp8_down", "pk_fp8_dgrad_dh", "pk_fp8_dgrad_dh_t", "pk_fp8_dgrad_dx")})
 
 _lib = None
 

@@ -1,14 +1,13 @@
 // The experts' products in 8-bit floating point: e4m3 values with a power of two for each block of 128 (fp8_blocks.h).
 //   rows:     [R][K'] codes, K' = K rounded up to 128 (the rest zeros), and K'/128 scale bytes a row, rows of whole words
 //   weights:  [E][N][K'] codes and [E][N/128][K'/128] bytes, blocks of 128 x 128; the transposed codes [E][K][N'] share the bytes
-// Products are exact and added in fp32 where values are decoded into bf16, their power of two included, and multiplied there.
+// Values are decoded into bf16, their power of two included, and multiplied there: products are exact, and added in fp32.
 // v_mfma_scale_f32_32x32x64_f8f6f4 takes codes and scale bytes as they are, at twice the rate (measured 4.5 PFLOP/s against 2.2), but of 8
 // neighbouring products' sum it keeps 13 bits below the largest product's leading one (measured; the other instructions for 8-bit values
 // do the same, those for bf16 keep all).  An error of 2^-13 is small next to the codes' own 2^-4, but g, u and d_h are rounded to
 // bf16 next, and h, d_g and d_u to codes again: a value that falls to the other side there is a step off, 2^-8 or 2^-3.  Against
 // exact sums y of one token was off by 0.007 of its size, four times bf16's own rounding, y of many rows by 0.0013 and d_w by 0.001.
-// So passes with few rows, which the memory bounds and where single values count, decode; with many rows (exact_products) the codes'
-// own errors (0.03) are all that matters, and the matrix units would be the bound.
+// So these short sums are for callers who ask for them (the entry points ending in _short), where they are faster.
 #include "fp8_blocks.h"
 #include "launch_rules.h"
 #include "unit_index.h"
@@ -837,10 +836,10 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
   }
 }
 
-// us, codes : decoded, gate and up, down, d_h, d_x with n rows an expert.  128 experts 2048 x 768: 32 rows 133 : 136, 82 : 83, 108 : 108,
+// Short sums where they are asked for and faster.  us, codes : decoded, gate and up, down, d_h, d_x with n rows an expert.  128 experts 2048 x 768: 32 rows 133 : 136, 82 : 83, 108 : 108,
 // 130 : 134; 48 rows 137 : 140, 85 : 86, 110 : 112, 131 : 134; 64 rows 139 : 149, 88 : 92, 115 : 120, 136 : 148; 512 rows 370 : 572, 225 : 310,
 // 323 : 420.  24 experts 1000 x 360, 32 rows: 19 : 20, 10 : 12, 25 : 26, 14 : 15.
-bool exact_products(int64_t A, int64_t E) { return A <= 40 * E || A <= TILE_ROWS; }
+bool exact_products(bool short_sums, int64_t A, int64_t E) { return !short_sums || A <= 40 * E || A <= TILE_ROWS; }
 
 // Of as many wide units, at most, a launch is made of narrow ones, us, wide : narrow, down, d_h, d_x.  2048 x 768: 4 experts of 64 rows 14 : 11,
 // 33 : 22, 21 : 15; 8 of 200 16 : 14, 40 : 27, 23 : 19; 16 of 30 17 : 16, 35 : 24, 26 : 24; 16 of 200 (328 units, in d_h 123) 20 : 21, 42 : 30,
@@ -848,7 +847,7 @@ bool exact_products(int64_t A, int64_t E) { return A <= 40 * E || A <= TILE_ROWS
 constexpr int NARROW_UNITS = 192;
 
 template <int EPI>
-int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool transposed = false) {
+int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool short_sums, bool transposed = false) {
   const bool narrow = EPI != GATE_UP && !transposed && plan_tiles(A, p.E) * pk_ceil_div(p.N, WIDE) <= NARROW_UNITS;
   p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP || narrow ? BLOCK : WIDE);
   p.by_n_tiles = pk_units::make_fastdiv(p.n_tiles);
@@ -871,12 +870,14 @@ int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool tran
     PK_RETURN_IF_LAUNCH_FAILED();
     return PK_OK;
   };
-  static bool ready[9][PK_MAX_DEVICES] = {};
+  static bool ready[10][PK_MAX_DEVICES] = {};
+  const bool exact = exact_products(short_sums, A, p.E);
   if constexpr (EPI == BWD)
-    if (transposed) return launch(product_kernel<EPI, true, true, false, false>, ready[8]);
+    if (transposed)
+      return exact ? launch(product_kernel<EPI, true, true, true, false>, ready[9]) : launch(product_kernel<EPI, true, true, false, false>, ready[8]);
   const auto pick = [&](auto wide_or_narrow, bool (*done)[PK_MAX_DEVICES]) {
     constexpr bool N = decltype(wide_or_narrow)::value;
-    if (exact_products(A, p.E))
+    if (exact)
       return p.vec ? launch(product_kernel<EPI, true, false, true, N>, done[3]) : launch(product_kernel<EPI, false, false, true, N>, done[2]);
     return p.vec ? launch(product_kernel<EPI, true, false, false, N>, done[1]) : launch(product_kernel<EPI, false, false, false, N>, done[0]);
   };
@@ -1338,9 +1339,9 @@ int pk_fp8_begin_backward(const void* d_y, const int32_t* plan, uint8_t* q, uint
   return begin(p, d_y, q, scales, A, H, E, false, stream);
 }
 
-int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3,
+static int gate_up(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3,
                    const int32_t* plan, void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E,
-                   pk_stream_t stream) {
+                   pk_stream_t stream, bool short_sums) {
   if (const int rc = check(A, H, I, E)) return rc;
   if (A == 0) return PK_OK;
   if (!all_set({x, x_scales, w1, s1, w3, s3, plan, h, h_scales}) || !g != !u) return PK_ERR_ARG;
@@ -1353,11 +1354,23 @@ int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w1,
   p.bs_n = p.kt; p.bs_k = 1; p.bs_e = blocks_of(I) * p.kt;
   p.vec = bf16_pieces(I, {g, u});
   p.O0 = (bf16_t*)g; p.O1 = (bf16_t*)u; p.Q[0] = h; p.Qs[0] = h_scales;
-  return launch_product<GATE_UP>(p, A, pk_timing::K_FP8_GATE_UP, (hipStream_t)stream);
+  return launch_product<GATE_UP>(p, A, pk_timing::K_FP8_GATE_UP, (hipStream_t)stream, short_sums);
 }
 
-int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2, const int32_t* plan, void* y, int64_t A,
-                int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
+int pk_fp8_gate_up(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3,
+                   const int32_t* plan, void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E,
+                   pk_stream_t stream) {
+  return gate_up(x, x_scales, w1, s1, w3, s3, plan, g, u, h, h_scales, A, H, I, E, stream, false);
+}
+
+int pk_fp8_gate_up_short(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w1, const uint8_t* s1, const uint8_t* w3, const uint8_t* s3,
+                         const int32_t* plan, void* g, void* u, uint8_t* h, uint8_t* h_scales, int64_t A, int64_t H, int64_t I, int64_t E,
+                         pk_stream_t stream) {
+  return gate_up(x, x_scales, w1, s1, w3, s3, plan, g, u, h, h_scales, A, H, I, E, stream, true);
+}
+
+static int down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2, const int32_t* plan, void* y, int64_t A,
+                int64_t H, int64_t I, int64_t E, pk_stream_t stream, bool short_sums) {
   if (const int rc = check(A, H, I, E)) return rc;
   if (A == 0) return PK_OK;
   if (!all_set({h, h_scales, w2, s2, plan, y})) return PK_ERR_ARG;
@@ -1370,12 +1383,22 @@ int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, co
   p.bs_n = p.kt; p.bs_k = 1; p.bs_e = blocks_of(H) * p.kt;
   p.vec = bf16_pieces(H, {y});
   p.O0 = (bf16_t*)y;
-  return launch_product<PLAIN>(p, A, pk_timing::K_FP8_DOWN, (hipStream_t)stream);
+  return launch_product<PLAIN>(p, A, pk_timing::K_FP8_DOWN, (hipStream_t)stream, short_sums);
+}
+
+int pk_fp8_down(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2, const int32_t* plan, void* y, int64_t A,
+                int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
+  return down(h, h_scales, w2, s2, plan, y, A, H, I, E, stream, false);
+}
+
+int pk_fp8_down_short(const uint8_t* h, const uint8_t* h_scales, const uint8_t* w2, const uint8_t* s2, const int32_t* plan, void* y, int64_t A,
+                      int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
+  return down(h, h_scales, w2, s2, plan, y, A, H, I, E, stream, true);
 }
 
 static int dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
                     const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales,
-                    int64_t A, int64_t H, int64_t I, int64_t E, bool transposed, pk_stream_t stream) {
+                    int64_t A, int64_t H, int64_t I, int64_t E, bool transposed, pk_stream_t stream, bool short_sums) {
   if (A == 0) return PK_OK;
   if (!all_set({d_y, d_y_scales, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales})) return PK_ERR_ARG;
   if (!all_aligned({d_y, w2_t, d_g8, d_u8, plan}) || !word_aligned({d_y_scales})) return PK_ERR_ALIGN;
@@ -1390,29 +1413,48 @@ static int dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t
   p.O0 = (bf16_t*)d_g; p.O1 = (bf16_t*)d_u; p.O2 = (bf16_t*)h;
   p.Q[0] = d_g8; p.Qs[0] = d_g_scales; p.Q[1] = d_u8; p.Qs[1] = d_u_scales;
   p.G = (const bf16_t*)g; p.U = (const bf16_t*)u;
-  return launch_product<BWD>(p, A, pk_timing::K_FP8_DGRAD_DH, (hipStream_t)stream, transposed);
+  return launch_product<BWD>(p, A, pk_timing::K_FP8_DGRAD_DH, (hipStream_t)stream, short_sums, transposed);
 }
 
 int pk_fp8_dgrad_dh(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
                     const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales,
                     int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
   if (const int rc = check(A, H, I, E)) return rc;
-  return dgrad_dh(d_y, d_y_scales, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, false, stream);
+  return dgrad_dh(d_y, d_y_scales, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, false, stream, false);
+}
+
+int pk_fp8_dgrad_dh_short(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
+                          const int32_t* plan, void* d_g, void* d_u, void* h, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8, uint8_t* d_u_scales,
+                          int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
+  if (const int rc = check(A, H, I, E)) return rc;
+  return dgrad_dh(d_y, d_y_scales, w2_t, s2, g, u, plan, d_g, d_u, h, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, false, stream, true);
+}
+
+static int dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
+                      const int32_t* plan, void* d_gT, void* d_uT, void* hT, int64_t ldt, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8,
+                      uint8_t* d_u_scales, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream, bool short_sums) {
+  if (const int rc = check(A, H, I, E)) return rc;
+  const int64_t need = pk_grouped_swiglu_transposed_ld(A, H, I, E, PK_BF16);
+  if (need <= 0) return PK_ERR_SHAPE;
+  if (A > 0 && (ldt < need || ldt % 64 != 0)) return PK_ERR_ARG;
+  return dgrad_dh(d_y, d_y_scales, w2_t, s2, g, u, plan, d_gT, d_uT, hT, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, true, stream, short_sums);
 }
 
 int pk_fp8_dgrad_dh_t(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
                       const int32_t* plan, void* d_gT, void* d_uT, void* hT, int64_t ldt, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8,
                       uint8_t* d_u_scales, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
-  if (const int rc = check(A, H, I, E)) return rc;
-  const int64_t need = pk_grouped_swiglu_transposed_ld(A, H, I, E, PK_BF16);
-  if (need <= 0) return PK_ERR_SHAPE;
-  if (A > 0 && (ldt < need || ldt % 64 != 0)) return PK_ERR_ARG;
-  return dgrad_dh(d_y, d_y_scales, w2_t, s2, g, u, plan, d_gT, d_uT, hT, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, true, stream);
+  return dgrad_dh_t(d_y, d_y_scales, w2_t, s2, g, u, plan, d_gT, d_uT, hT, ldt, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, stream, false);
 }
 
-int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales, const uint8_t* w1_t,
+int pk_fp8_dgrad_dh_t_short(const uint8_t* d_y, const uint8_t* d_y_scales, const uint8_t* w2_t, const uint8_t* s2, const void* g, const void* u,
+                            const int32_t* plan, void* d_gT, void* d_uT, void* hT, int64_t ldt, uint8_t* d_g8, uint8_t* d_g_scales, uint8_t* d_u8,
+                            uint8_t* d_u_scales, int64_t A, int64_t H, int64_t I, int64_t E, pk_stream_t stream) {
+  return dgrad_dh_t(d_y, d_y_scales, w2_t, s2, g, u, plan, d_gT, d_uT, hT, ldt, d_g8, d_g_scales, d_u8, d_u_scales, A, H, I, E, stream, true);
+}
+
+static int dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales, const uint8_t* w1_t,
                     const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3, const int32_t* plan, void* d_x, int64_t A, int64_t H, int64_t I,
-                    int64_t E, pk_stream_t stream) {
+                    int64_t E, pk_stream_t stream, bool short_sums) {
   if (const int rc = check(A, H, I, E)) return rc;
   if (A == 0) return PK_OK;
   if (!all_set({d_g8, d_g_scales, d_u8, d_u_scales, w1_t, s1, w3_t, s3, plan, d_x})) return PK_ERR_ARG;
@@ -1425,7 +1467,19 @@ int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_
   p.bs_n = 1; p.bs_k = (int32_t)blocks_of(H); p.bs_e = blocks_of(H) * blocks_of(I);
   p.vec = bf16_pieces(H, {d_x});
   p.O0 = (bf16_t*)d_x;
-  return launch_product<PLAIN>(p, A, pk_timing::K_FP8_DGRAD_DX, (hipStream_t)stream);
+  return launch_product<PLAIN>(p, A, pk_timing::K_FP8_DGRAD_DX, (hipStream_t)stream, short_sums);
+}
+
+int pk_fp8_dgrad_dx(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales, const uint8_t* w1_t,
+                    const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3, const int32_t* plan, void* d_x, int64_t A, int64_t H, int64_t I,
+                    int64_t E, pk_stream_t stream) {
+  return dgrad_dx(d_g8, d_g_scales, d_u8, d_u_scales, w1_t, s1, w3_t, s3, plan, d_x, A, H, I, E, stream, false);
+}
+
+int pk_fp8_dgrad_dx_short(const uint8_t* d_g8, const uint8_t* d_g_scales, const uint8_t* d_u8, const uint8_t* d_u_scales, const uint8_t* w1_t,
+                          const uint8_t* s1, const uint8_t* w3_t, const uint8_t* s3, const int32_t* plan, void* d_x, int64_t A, int64_t H, int64_t I,
+                          int64_t E, pk_stream_t stream) {
+  return dgrad_dx(d_g8, d_g_scales, d_u8, d_u_scales, w1_t, s1, w3_t, s3, plan, d_x, A, H, I, E, stream, true);
 }
 
 int pk_fp8_few_rows_pays(int64_t A, int64_t H, int64_t I, int64_t E) {

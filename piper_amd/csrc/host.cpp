@@ -994,8 +994,9 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     TORCH_CHECK(bytes > 0, "pk_fp8_plan_bytes failed: ", pk_status_string((int)bytes));
     return at::empty({bytes / 4}, counts.options().dtype(at::kInt));
   }
-  // y [A,H]; gu [2,A,I]: where the pre-activations are left, plan_out: the pass's plan (both null without a backward)
-  static Tensor run(const Fp8Weights& w, const Tensor& x, const Tensor& counts, Tensor* gu, Tensor* plan_out) {
+  // y [A,H]; short_sums: see pk_fp8_gate_up_short; gu [2,A,I]: where the pre-activations are left, plan_out: the pass's plan (both null
+  // without a backward)
+  static Tensor run(const Fp8Weights& w, bool short_sums, const Tensor& x, const Tensor& counts, Tensor* gu, Tensor* plan_out) {
     const int64_t A = x.size(0), H = w.H, I = w.I, E = w.E;
     Tensor y = at::empty({A, H}, x.options());
     char *g = nullptr, *u = nullptr;
@@ -1023,20 +1024,22 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     int32_t* const at = plan.data_ptr<int32_t>();
     const auto p = [&](size_t pos) { return static_cast<uint8_t*>(b.at_(pos)); };
     PK_CALL(pk_fp8_begin, ptr(x), ptr(counts), counts.scalar_type() == at::kLong, p(x8), p(xs), at, A, H, E, st);
-    PK_CALL(pk_fp8_gate_up, p(x8), p(xs), u8(w.q[0]), u8(w.s[0]), u8(w.q[2]), u8(w.s[2]), at, g, u, p(h8), p(hs), A, H, I, E, st);
-    PK_CALL(pk_fp8_down, p(h8), p(hs), u8(w.q[1]), u8(w.s[1]), at, ptr(y), A, H, I, E, st);
+    PK_CALL((short_sums ? pk_fp8_gate_up_short : pk_fp8_gate_up), p(x8), p(xs), u8(w.q[0]), u8(w.s[0]), u8(w.q[2]), u8(w.s[2]), at, g, u, p(h8), p(hs),
+            A, H, I, E, st);
+    PK_CALL((short_sums ? pk_fp8_down_short : pk_fp8_down), p(h8), p(hs), u8(w.q[1]), u8(w.s[1]), at, ptr(y), A, H, I, E, st);
     if (plan_out) *plan_out = plan;
     return y;
   }
   static Tensor forward(AutogradContext* ctx, const OptTensor& w1, const OptTensor& w2, const OptTensor& w3, const Tensor& x, const Fp8Weights* w,
-                        const Tensor& counts) {
+                        bool short_sums, const Tensor& counts) {
     Tensor gu, plan;
     const Tensor xc = contig(x);
-    Tensor y = run(*w, xc, counts, &gu, &plan);
+    Tensor y = run(*w, short_sums, xc, counts, &gu, &plan);
     ctx->save_for_backward({xc, plan, gu, w->t[0], w->t[1], w->t[2], w->s[0], w->s[1], w->s[2]});
     const Tensor p1 = opt(w1), p2 = opt(w2), p3 = opt(w3);
     keep_parameters(ctx, {&p1, &p2, &p3});
     ctx->saved_data["weights"] = p1.defined();
+    ctx->saved_data["short_sums"] = short_sums;
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -1045,7 +1048,7 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     const Tensor &p1 = params[0], &p2 = params[1], &p3 = params[2], starts = sv[1], gu = sv[2];
     const Tensor x = sv[0], d_y = contig(grads[0]), &t1 = sv[3], &t2 = sv[4], &t3 = sv[5], &s1 = sv[6], &s2 = sv[7], &s3 = sv[8];
     const int64_t E = t1.size(0), H = t1.size(1), I = t2.size(1), A = x.size(0);
-    const bool weights = ctx->saved_data["weights"].toBool();
+    const bool weights = ctx->saved_data["weights"].toBool(), short_sums = ctx->saved_data["short_sums"].toBool();
     const bool n1 = weights && ctx->needs_input_grad(0), n2 = weights && ctx->needs_input_grad(1), n3 = weights && ctx->needs_input_grad(2);
     const bool nx = ctx->needs_input_grad(weights ? 3 : 0);
     const pk_stream_t st = stream_of(x);
@@ -1058,7 +1061,7 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     b.allocate(x);
     const auto p = [&](size_t pos) { return static_cast<uint8_t*>(b.at_(pos)); };
     // d_g, d_u, h for the weight gradients: row-major, or with more rows an expert as the transposed copies that their faster kernels
-    // read (the line is that of the region's backward; passes of up to 128 rows multiply decoded values, which have no such path)
+    // read (the line is that of the region's backward)
     const bool any_w = n1 || n2 || n3;
     const int64_t ldt = any_w && A > 40 * E && A > 128 && pk_region_transposed_pays(A, H, I, E, PK_BF16) ? pk_grouped_swiglu_transposed_ld(A, H, I, E, PK_BF16) : 0;
     const int64_t copy = ldt > 0 ? ldt * I * 2 : step;
@@ -1067,15 +1070,15 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     if (ldt > 0) map = at::empty({A}, starts.options());
     PK_CALL(pk_fp8_begin_backward, ptr(d_y), at, p(y8), p(ys), ldt > 0 ? map.data_ptr<int32_t>() : nullptr, A, H, E, st);
     if (ldt > 0) {
-      PK_CALL(pk_fp8_dgrad_dh_t, p(y8), p(ys), u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, ldt, p(g8), p(gs),
-              p(u8_), p(us), A, H, I, E, st);
+      PK_CALL((short_sums ? pk_fp8_dgrad_dh_t_short : pk_fp8_dgrad_dh_t), p(y8), p(ys), u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, ldt,
+              p(g8), p(gs), p(u8_), p(us), A, H, I, E, st);
     } else {
-      PK_CALL(pk_fp8_dgrad_dh, p(y8), p(ys), u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, p(g8), p(gs), p(u8_),
-              p(us), A, H, I, E, st);
+      PK_CALL((short_sums ? pk_fp8_dgrad_dh_short : pk_fp8_dgrad_dh), p(y8), p(ys), u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, p(g8), p(gs),
+              p(u8_), p(us), A, H, I, E, st);
     }
     if (nx) {
       d_x = at::empty({A, H}, x.options());
-      PK_CALL(pk_fp8_dgrad_dx, p(g8), p(gs), p(u8_), p(us), u8(t1), u8(s1), u8(t3), u8(s3), at, ptr(d_x), A, H, I, E, st);
+      PK_CALL((short_sums ? pk_fp8_dgrad_dx_short : pk_fp8_dgrad_dx), p(g8), p(gs), p(u8_), p(us), u8(t1), u8(s1), u8(t3), u8(s3), at, ptr(d_x), A, H, I, E, st);
     }
     const auto wgrad = [d_y, dguh, map, x, starts, A, H, I, E, ldt, copy](const Tensor& d1, const Tensor& d2, const Tensor& d3, bool accumulate) {
       char* const ds = static_cast<char*>(dguh.data_ptr());
@@ -1098,13 +1101,12 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
       d3 = at::empty({E, I, H}, x.options());
       wgrad(d1, d2, d3, false);
     }
-    if (!weights) return {Tensor(), Tensor(), Tensor(), d_x, Tensor(), Tensor()};
-    return {d1, d2, d3, d_x, Tensor(), Tensor()};
+    return {d1, d2, d3, d_x, Tensor(), Tensor(), Tensor()};
   }
 };
 std::optional<Tensor> bmm_experts_fp8(const OptTensor& w1_, const OptTensor& w2_, const OptTensor& w3_, const Tensor& q1, const Tensor& q2,
                                       const Tensor& q3, const Tensor& s1, const Tensor& s2, const Tensor& s3, const OptTensor& t1_,
-                                      const OptTensor& t2_, const OptTensor& t3_, const Tensor& x, const Tensor& counts, bool direct) {
+                                      const OptTensor& t2_, const OptTensor& t3_, bool short_sums, const Tensor& x, const Tensor& counts, bool direct) {
   const Tensor w1 = opt(w1_), w2 = opt(w2_), w3 = opt(w3_), t1 = opt(t1_), t2 = opt(t2_), t3 = opt(t3_);
   if (direct && !plain({&w1, &w2, &w3, &q1, &q2, &q3, &s1, &s2, &s3, &t1, &t2, &t3, &x, &counts})) return std::nullopt;
   refuse_transforms({&w1, &w2, &w3, &q1, &q2, &q3, &s1, &s2, &s3, &t1, &t2, &t3, &x, &counts}, "bmm_experts_fp8");
@@ -1126,9 +1128,9 @@ std::optional<Tensor> bmm_experts_fp8(const OptTensor& w1_, const OptTensor& w2_
     TORCH_CHECK_VALUE(t1.defined(), "bmm_experts_fp8: a backward needs the transposed codes (quantize_experts(..., for_backward=True))");
     TORCH_CHECK_TYPE(!wants_grad({&w1, &w2, &w3}) || (w1.scalar_type() == at::kBFloat16 && w2.scalar_type() == at::kBFloat16 && w3.scalar_type() == at::kBFloat16),
                      "bmm_experts_fp8: weights that want gradients are bfloat16");
-    return Fp8ExpertsFn::apply(w1_, w2_, w3_, x, &w, n);
+    return Fp8ExpertsFn::apply(w1_, w2_, w3_, x, &w, short_sums, n);
   }
-  return Fp8ExpertsFn::run(w, contig(x), n, nullptr, nullptr);
+  return Fp8ExpertsFn::run(w, short_sums, contig(x), n, nullptr, nullptr);
 }
 
 // ------------------------------------------------------------------------------ bucket path

@@ -72,9 +72,9 @@ class BmmExperts(nn.Module):
         self.w2 = nn.Parameter(torch.empty(num_experts, dim, hidden_dim, dtype=dtype))
         self.w3 = nn.Parameter(torch.empty(num_experts, hidden_dim, dim, dtype=dtype))
 
-    def quantize(self, *, for_backward: bool = True) -> F_.Fp8Experts:
+    def quantize(self, *, for_backward: bool = True, short_sums: bool = False) -> F_.Fp8Experts:
         """The weights as they are now in 8-bit blocks, for forward passes until the next optimizer step."""
-        return F_.quantize_experts(self.w1, self.w2, self.w3, for_backward=for_backward)
+        return F_.quantize_experts(self.w1, self.w2, self.w3, for_backward=for_backward, short_sums=short_sums)
 
     def forward(self, x: torch.Tensor, num_tokens_per_expert: torch.Tensor, experts_fp8: F_.Fp8Experts | None = None) -> torch.Tensor:
         """``experts_fp8`` (of ``quantize``): the products run in 8-bit floating point."""

@@ -1,0 +1,102 @@
+"""The experts in 8-bit blocks with many rows an expert: what every sum keeps, and the kernels that passes of real size run."""
+import pytest
+import torch
+
+from oracle import blocks as B
+from piper_amd import _lib, ops
+from piper_amd import functional as F_
+from test_gpu_fp8 import _inputs, _within
+
+pytestmark = pytest.mark.gpu
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _plan(lib, counts, A, dev):
+    n = torch.tensor(counts, dtype=torch.int32, device=dev)
+    plan = torch.empty(lib.pk_fp8_plan_bytes(A, len(counts)) // 4, dtype=torch.int32, device=dev)
+    assert lib.pk_fp8_plan(_p(n), 0, len(counts), A, _p(plan), _lib.current_stream(dev)) == 0
+    return plan
+
+
+# ------------------------------------------------------------------------------ sums
+def _cancelling(rows, K):
+    """Rows whose products with ones are 256, 2^-6, ..., -256 within eight values: 2^-6 (K - 2) in all, exact in fp32 and lost if
+    less than 15 bits are kept below the largest product."""
+    x = torch.full((rows, K), 2.0 ** -6)
+    x[:, 0], x[:, 5] = 256.0, -256.0
+    return x.bfloat16()
+
+
+# (2 experts: units of 128 columns; 130: of 256, and more of them than CUs)
+@pytest.mark.parametrize("E,each,N", [(2, 150, 264), (130, 45, 512), (130, 45, 391)])
+def test_many_rows_lose_no_small_products(dev, E, each, N):
+    print(f"[case] fp8 experts, products of very different size, {E} x {each} rows, {N} columns", flush=True)
+    lib, K, A, st = _lib.load(), 256, E * each, _lib.current_stream(dev)
+    assert A > 40 * E and A > 128
+    plan = _plan(lib, [each] * E, A, dev)
+    q, s = ops.quantize_rows_fp8(_cancelling(A, K).to(dev))
+    ones = lambda *shape: torch.ones(shape, device=dev).bfloat16()  # noqa: E731
+    e = F_.quantize_experts(ones(E, N, K), ones(E, K, N), ones(E, N, K))
+    down = F_.quantize_experts(ones(E, K, N), ones(E, N, K), ones(E, K, N))      # [N, K] as the second weight, and its transposes
+    new = lambda w, dtype=torch.bfloat16: torch.zeros(A, w, dtype=dtype, device=dev)  # noqa: E731
+    whole, words = -(-N // 128) * 128, -(-N // 512) * 4
+    codes = lambda: [new(whole, torch.uint8), new(words, torch.uint8), new(whole, torch.uint8), new(words, torch.uint8)]  # noqa: E731
+    want = 2.0 ** -6 * (K - 2)                             # 127 * 2^-5: seven bits, a bf16 value
+    g, u, c = new(N), new(N), codes()
+    assert lib.pk_fp8_gate_up(_p(q), _p(s), _p(e.q1), _p(e.s1), _p(e.q3), _p(e.s3), _p(plan), _p(g), _p(u), _p(c[0]), _p(c[1]), A, K, N, E, st) == 0
+    assert (g == want).all() and (u == want).all()
+    y = new(N)
+    assert lib.pk_fp8_down(_p(q), _p(s), _p(down.q2), _p(down.s2), _p(plan), _p(y), A, N, K, E, st) == 0
+    assert (y == want).all()
+    d_x = new(N)
+    assert lib.pk_fp8_dgrad_dx(_p(q), _p(s), _p(q), _p(s), _p(down.t1), _p(down.s1), _p(down.t3), _p(down.s3), _p(plan), _p(d_x), A, N, K, E, st) == 0
+    assert (d_x == 2 * want).all()
+    # silu(64) = 64 in fp32: d_u = 64 d_h
+    g.fill_(64.0)
+    u.fill_(1.0)
+    out = [new(N) for _ in range(3)]
+    assert lib.pk_fp8_dgrad_dh(_p(q), _p(s), _p(e.t2), _p(e.s2), _p(g), _p(u), _p(plan), *map(_p, out), *map(_p, codes()), A, K, N, E, st) == 0
+    assert (out[1] == 64 * want).all()
+    if N % 256 == 0:
+        ldt = lib.pk_grouped_swiglu_transposed_ld(A, K, N, E, _lib.PK_BF16)
+        t = torch.zeros(3, ldt // 32, N, 32, dtype=torch.bfloat16, device=dev)
+        assert lib.pk_fp8_dgrad_dh_t(_p(q), _p(s), _p(e.t2), _p(e.s2), _p(g), _p(u), _p(plan), _p(t[0]), _p(t[1]), _p(t[2]), ldt, *map(_p, codes()), A, K, N,
+                                     E, st) == 0
+        assert set(t[1].unique().tolist()) <= {0.0, 64 * want} and int((t[1] != 0).sum()) == A * N
+
+
+@pytest.mark.parametrize("E,H,I,counts,spare", [(4, 256, 512, [200, 33, 0, 64], 7), (3, 257, 300, [150, 140, 90], 3)])
+def test_many_rows_are_within_the_bounds_of_fp32_sums(dev, E, H, I, counts, spare):
+    print(f"[case] fp8 experts, sums in fp32, {counts}", flush=True)
+    w1, w2, w3, x, d_y = _inputs(E, H, I, counts, spare, E, False)
+    want = B.experts_between(w1, w2, w3, x, counts, d_y, decoded=True)
+    leaves = [t.to(dev).requires_grad_(True) for t in (w1, w2, w3, x)]
+    y = F_.bmm_experts_fp8(F_.quantize_experts(*leaves[:3]), leaves[3], torch.tensor(counts, device=dev))
+    y.backward(d_y.to(dev))
+    for name, t in zip(("y", "d_w1", "d_w2", "d_w3", "d_x"), (y, *(leaf.grad for leaf in leaves))):
+        _within(name, t, *want[name])
+
+
+@pytest.mark.parametrize("E,H,I,counts,spare", [(4, 256, 512, [200, 33, 0, 64], 7), (3, 257, 300, [150, 140, 90], 3), (2, 256, 128, [30, 40], 0)])
+def test_short_sums_are_the_callers_choice(dev, E, H, I, counts, spare):
+    """Within the bounds that contain what the matrix instructions cut off; passes that are no faster for it are the default's."""
+    print(f"[case] fp8 experts, short sums, {counts}", flush=True)
+    w1, w2, w3, x, d_y = _inputs(E, H, I, counts, spare, E, False)
+    few = x.shape[0] <= max(40 * E, 128)
+    want = B.experts_between(w1, w2, w3, x, counts, d_y, decoded=few)
+    n, passes = torch.tensor(counts, device=dev), []
+    for short in (True, False):
+        leaves = [t.to(dev).requires_grad_(True) for t in (w1, w2, w3, x)]
+        experts = F_.quantize_experts(*leaves[:3], short_sums=short)
+        assert experts.short_sums is short
+        y = F_.bmm_experts_fp8(experts, leaves[3], n)
+        y.backward(d_y.to(dev))
+        with torch.no_grad():
+            assert torch.equal(y, F_.bmm_experts_fp8(experts, leaves[3], n))
+        passes.append((y.detach(), *(leaf.grad for leaf in leaves)))
+    for name, t in zip(("y", "d_w1", "d_w2", "d_w3", "d_x"), passes[0]):
+        _within(name, t, *want[name])
+    assert not few or all(torch.equal(a, b) for a, b in zip(*passes))
