@@ -1046,7 +1046,8 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     const variable_list sv = ctx->get_saved_variables();
     const variable_list params = parameters_of(ctx);
     const Tensor &p1 = params[0], &p2 = params[1], &p3 = params[2], starts = sv[1], gu = sv[2];
-    const Tensor x = sv[0], d_y = contig(grads[0]), &t1 = sv[3], &t2 = sv[4], &t3 = sv[5], &s1 = sv[6], &s2 = sv[7], &s3 = sv[8];
+    Tensor x = sv[0], d_y = contig(grads[0]);
+    const Tensor &t1 = sv[3], &t2 = sv[4], &t3 = sv[5], &s1 = sv[6], &s2 = sv[7], &s3 = sv[8];
     const int64_t E = t1.size(0), H = t1.size(1), I = t2.size(1), A = x.size(0);
     const bool weights = ctx->saved_data["weights"].toBool(), short_sums = ctx->saved_data["short_sums"].toBool();
     const bool n1 = weights && ctx->needs_input_grad(0), n2 = weights && ctx->needs_input_grad(1), n3 = weights && ctx->needs_input_grad(2);
@@ -1067,7 +1068,12 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     const int64_t copy = ldt > 0 ? ldt * I * 2 : step;
     Tensor dguh = at::empty({3 * copy / 2}, x.options()), map, d_x;
     char* const dg = static_cast<char*>(dguh.data_ptr());
-    if (ldt > 0) map = at::empty({A}, starts.options());
+    if (ldt > 0) {
+      map = at::empty({A}, starts.options());
+      // those kernels take 16-byte aligned tensors only, and a view may start anywhere
+      if (!aligned16(x)) x = x.clone();
+      if (!aligned16(d_y)) d_y = d_y.clone();
+    }
     PK_CALL(pk_fp8_begin_backward, ptr(d_y), at, p(y8), p(ys), ldt > 0 ? map.data_ptr<int32_t>() : nullptr, A, H, E, st);
     if (ldt > 0) {
       PK_CALL((short_sums ? pk_fp8_dgrad_dh_t_short : pk_fp8_dgrad_dh_t), p(y8), p(ys), u8(t2), u8(s2), g, g + step, at, dg, dg + copy, dg + 2 * copy, ldt,
@@ -1083,12 +1089,19 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     const auto wgrad = [d_y, dguh, map, x, starts, A, H, I, E, ldt, copy](const Tensor& d1, const Tensor& d2, const Tensor& d3, bool accumulate) {
       char* const ds = static_cast<char*>(dguh.data_ptr());
       const int32_t* const at = starts.data_ptr<int32_t>();
-      if (ldt > 0)
-        PK_CALL(pk_grouped_swiglu_wgrad_scaled_t, ptr(d_y), ds + 2 * copy, ds, ds + copy, ldt, ptr(x), map.data_ptr<int32_t>(), 1, at, nullptr, ptr(d1),
-                ptr(d2), ptr(d3), accumulate, A, H, I, E, PK_BF16, stream_of(x));
-      else
+      if (ldt > 0) {
+        at::NoGradGuard no_grad;
+        const Tensor* const to[3] = {&d1, &d2, &d3};      // (a gradient that is added to may be such a view as well)
+        Tensor in[3];
+        for (int i = 0; i < 3; ++i) in[i] = aligned16(*to[i]) ? *to[i] : accumulate ? to[i]->clone() : at::empty_like(*to[i]);
+        PK_CALL(pk_grouped_swiglu_wgrad_scaled_t, ptr(d_y), ds + 2 * copy, ds, ds + copy, ldt, ptr(x), map.data_ptr<int32_t>(), 1, at, nullptr, ptr(in[0]),
+                ptr(in[1]), ptr(in[2]), accumulate, A, H, I, E, PK_BF16, stream_of(x));
+        for (int i = 0; i < 3; ++i)
+          if (!in[i].is_same(*to[i])) to[i]->copy_(in[i]);
+      } else {
         PK_CALL(pk_grouped_swiglu_wgrad, ptr(d_y), ds + 2 * copy, ds, ds + copy, ptr(x), nullptr, 1, at, nullptr, ptr(d1), ptr(d2), ptr(d3), accumulate,
                 A, H, I, E, PK_BF16, stream_of(x));
+      }
     };
     Tensor d1, d2, d3;
     if (n1 && n2 && n3 && g_deferring.load() && leaf(p1) && leaf(p2) && leaf(p3)) {

@@ -100,3 +100,57 @@ def test_short_sums_are_the_callers_choice(dev, E, H, I, counts, spare):
     for name, t in zip(("y", "d_w1", "d_w2", "d_w3", "d_x"), passes[0]):
         _within(name, t, *want[name])
     assert not few or all(torch.equal(a, b) for a, b in zip(*passes))
+
+
+# ------------------------------------------------------------------------------ weight gradients from transposed copies
+PAYS = dict(E=4, H=2048, I=1024, counts=(50, 0, 97, 60))      # 128 units of 256 x 256 for fewer experts than XCDs
+
+
+def _case(dev, E, H, I, counts, spare=0, seed=0):
+    assert _lib.load().pk_region_transposed_pays(sum(counts) + spare, H, I, E, _lib.PK_BF16) == 1 and sum(counts) + spare > max(40 * E, 128)
+    w1, w2, w3, x, d_y = (t.to(dev) for t in _inputs(E, H, I, counts, spare, seed, False))
+    return [w.requires_grad_(True) for w in (w1, w2, w3)], x.requires_grad_(True), d_y, torch.tensor(counts, dtype=torch.int32, device=dev)
+
+
+def _pass(w, x, d_y, n):
+    y = F_.bmm_experts_fp8(F_.quantize_experts(*w), x, n)
+    return (y.detach(), *torch.autograd.grad(y, (*w, x), d_y))
+
+
+def _equal(a, b):
+    return len(a) == len(b) and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def _odd(t):
+    """The same values two bytes behind a 16-byte boundary."""
+    t = t.detach()
+    v = torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+    assert v.data_ptr() % 16 == 2
+    return v
+
+
+def test_views_that_start_anywhere(dev):
+    print("[case] fp8 experts, transposed copies: unaligned rows, gradients and places of gradients", flush=True)
+    w, x, d_y, n = _case(dev, **PAYS)
+    want = _pass(w, x, d_y, n)
+    assert _equal(want, _pass(w, _odd(x).requires_grad_(True), d_y, n))
+    assert _equal(want, _pass(w, x, _odd(d_y), n))
+    experts = F_.quantize_experts(*w)
+
+    def added(places):
+        for p, at in zip(w, places):
+            p.grad = at
+        F_.bmm_experts_fp8(experts, x, n).backward(d_y)
+        assert all(p.grad is at for p, at in zip(w, places))
+        return places
+
+    with F_.accumulate_weight_grads():
+        sums = added([g.clone() for g in want[1:4]])
+        assert _equal(sums, added([_odd(g) for g in want[1:4]]))
+        assert _equal(sums, added([want[1].clone(), _odd(want[2]), want[3].clone()]))
+    places = [_odd(g) for g in want[1:4]]
+    with F_.defer_weight_grads() as q:
+        added(places)
+        assert _equal(places, want[1:4])
+    q.run()
+    assert _equal(sums, places)
