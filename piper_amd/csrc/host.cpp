@@ -1062,9 +1062,9 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
     b.allocate(x);
     const auto p = [&](size_t pos) { return static_cast<uint8_t*>(b.at_(pos)); };
     // d_g, d_u, h for the weight gradients: row-major, or with more rows an expert as the transposed copies that their faster kernels
-    // read (the line is that of the region's backward)
+    // read (the line is that of the region's backward), with offsets of 32 bits into the rows
     const bool any_w = n1 || n2 || n3;
-    const int64_t ldt = any_w && A > 40 * E && A > 128 && pk_region_transposed_pays(A, H, I, E, PK_BF16) ? pk_grouped_swiglu_transposed_ld(A, H, I, E, PK_BF16) : 0;
+    const int64_t ldt = any_w && A > 40 * E && A > 128 && A * H * 2 <= 0xffffffffll && pk_region_transposed_pays(A, H, I, E, PK_BF16) ? pk_grouped_swiglu_transposed_ld(A, H, I, E, PK_BF16) : 0;
     const int64_t copy = ldt > 0 ? ldt * I * 2 : step;
     Tensor dguh = at::empty({3 * copy / 2}, x.options()), map, d_x;
     char* const dg = static_cast<char*>(dguh.data_ptr());

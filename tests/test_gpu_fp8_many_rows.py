@@ -154,3 +154,19 @@ def test_views_that_start_anywhere(dev):
         assert _equal(places, want[1:4])
     q.run()
     assert _equal(sums, places)
+
+
+def test_rows_behind_4_gib(dev):
+    """One expert has 1.05 million rows, those of the others begin behind 4 GiB of x and d_y, where the transposed pair's offsets end."""
+    E, H, I, tail = 4, 2048, 1024, [0, 0, 50, 60]
+    many = 1_049_900
+    print(f"[case] fp8 experts, {many} rows and {tail}", flush=True)
+    w1, w2, w3, x, d_y = _inputs(E, H, I, tail, 0, 4, False)
+    want = B.experts_between(w1, w2, w3, x, tail, d_y, decoded=True)
+    x_all, d_all = (torch.cat([torch.zeros(many, H, dtype=t.dtype, device=dev), t.to(dev)]).requires_grad_(t is x) for t in (x, d_y))
+    assert many * H * 2 > 2 ** 32
+    got = _pass([w.to(dev).requires_grad_(True) for w in (w1, w2, w3)], x_all, d_all, torch.tensor([many, *tail[1:]], device=dev))
+    for name, t in zip(("y", "d_w1", "d_w2", "d_w3", "d_x"), got):
+        rows = name in ("y", "d_x")
+        assert (t[:many] == 0).all() if rows else (t[:2] == 0).all()
+        _within(name, t[many:] if rows else t, *want[name])
