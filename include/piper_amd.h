@@ -363,12 +363,9 @@ PK_API int pk_grouped_swiglu_wgrad_scaled(const void* d_out, const void* hs, con
  * pk_grouped_swiglu_wgrad_scaled_t computes the same d_w1, d_w2, d_w3 as
  * pk_grouped_swiglu_wgrad_scaled from d_out, x (through row_map / row_map_div) and the transposed
  * copies.  Both replace the autograd of qwen3_bmm_experts_patch.py:39-41 like the pair above.
- * Restriction of pk_grouped_swiglu_wgrad_scaled_t: the last 32-row block of an expert multiplies
- * the zeros of the transposed copy with the rows of x / d_out that the row map names behind the
- * expert's last row (rows of the next expert's tokens).  Zero times a finite value is zero; zero
- * times Inf or NaN is NaN.  A non-finite row of x or d_out can therefore reach the weight gradients
- * of the expert in front of the one it was routed to, which pk_grouped_swiglu_wgrad_scaled (rows
- * past an expert's end read as zeros) confines to its own experts. 
+ * The last 32-row block of an expert multiplies the zeros of the transposed copy with the expert's last
+ * row of x / d_out.  Zero times Inf or NaN is NaN: where that row is not finite, so are its expert's weight
+ * gradients, and as with pk_grouped_swiglu_wgrad_scaled no other's.
  * d_scores may be NULL: the score gradients then stay in the workspace as ceil(I / 64) partial sums per
  * sorted row, [ceil(I / 64)][A] fp32, for pk_region_router_bwd. */
 PK_API int64_t pk_grouped_swiglu_transposed_ld(int64_t A, int64_t H, int64_t I, int64_t E, int dtype);

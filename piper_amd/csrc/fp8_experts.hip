@@ -228,8 +228,8 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_kernel(const void* counts, 
 
 // What a pass begins with, in one launch: its rows in blocks, and in front of the forward its plan (by the first workgroup), in front of
 // the backward a row map.  (1,777 tokens of 2048 in 8 places each: 17 us, and 5 for either of the others by itself.)
-// The map: every row its own number, those of no expert the last one that has one, for pk_grouped_swiglu_wgrad_scaled_t, which multiplies
-// rows behind an expert's last one by zeros.  What stands in rows of no expert (it may be anything) is thereby not read.
+// The map: every row its own number, those of no expert the last one that has one, for pk_grouped_swiglu_wgrad_scaled_t, whose loader
+// may stand behind the last expert's rows.  What is in rows of no expert (it may be anything) is thereby not read.
 struct Begin {
   const bf16_t* x;
   uint8_t *q, *s;

@@ -1717,8 +1717,8 @@ struct WgradKcParams {
 //    and an index into the row map; a load is the scalar-base + 32-bit-lane-offset form.  The row
 //    map entries of the slot after the one being requested are fetched with one 16-byte scalar
 //    load per wave and picked up, per lane, one k-tile later.
-//  * Rows of the gathered operand past the expert's end read whatever row the map holds next (a
-//    valid, finite row): they meet the zeros of the transposed copy.
+//  * Rows of the gathered operand past the expert's end read its last row, and meet the zeros of the transposed
+//    copy: of what is not finite (zero times Inf is NaN) a gradient sees its own expert's rows only.
 //  * One lane resolves the unit after the next one -- ticket, expert, row range -- behind its
 //    epilogue's stores and hands it over through LDS at the top of the next unit, so no wave waits
 //    for a chain of scalar loads between two k-loops.
@@ -1869,19 +1869,19 @@ __global__ __launch_bounds__(64 * WMW * WNW) void wgrad_pp_kernel(const WgradKcP
   const char* ld_kc = nullptr;
   const char* ld_kc0 = nullptr;
   const char* ld_r = nullptr;
-  int ld_map = 0, ld_map0 = 0, ld_rem = 0;
+  int ld_map = 0, ld_map0 = 0, ld_rem = 0, ld_end = 0;      // ld_end: behind the expert's last entry of the row map
   bool ld_on_next = false, ld_idle = false, next_known = false;
   int rows_n[NR];
   static_assert(NR == 4, "a wave's rows of a k-tile are one 16-byte scalar load");
   typedef int i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
   auto fetch_rows = [&]() {
     const int idx = ld_map + wave * NR;
-    if (idx + NR <= p.total_rows) {
+    if (idx + NR <= ld_end) {
       const i32x4_a4 v = *reinterpret_cast<const __attribute__((address_space(4))) i32x4_a4*>(row_map + idx);
       rows_n[0] = v[0]; rows_n[1] = v[1]; rows_n[2] = v[2]; rows_n[3] = v[3];
-    } else {      // the last entries of the row map
+    } else {      // the expert's last entries
 #pragma unroll
-      for (int i = 0; i < NR; ++i) rows_n[i] = row_map[min(idx + i, p.total_rows - 1)];
+      for (int i = 0; i < NR; ++i) rows_n[i] = row_map[min(idx + i, ld_end - 1)];
     }
   };
   auto ld_enter = [&](const Unit& t) {
@@ -1891,6 +1891,7 @@ __global__ __launch_bounds__(64 * WMW * WNW) void wgrad_pp_kernel(const WgradKcP
     ld_kc = ld_kc0;
     ld_map = ld_map0;
     ld_rem = t.nkt;
+    ld_end = t.rows > 0 ? t.s0 + t.rows : p.total_rows;
     ld_idle = false;
     if (ld_rem == 0) { ld_idle = true; ld_rem = 1; }    // an expert without rows: nothing to request
   };

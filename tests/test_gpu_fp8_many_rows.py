@@ -170,3 +170,24 @@ def test_rows_behind_4_gib(dev):
         rows = name in ("y", "d_x")
         assert (t[:many] == 0).all() if rows else (t[:2] == 0).all()
         _within(name, t[many:] if rows else t, *want[name])
+
+
+@pytest.mark.parametrize("shape", [PAYS, dict(E=4, H=256, I=512, counts=(50, 0, 97, 60))])      # transposed copies, row-major operands
+def test_weight_gradients_of_rows_that_are_not_finite(dev, shape):
+    """The first and the last row of an expert, in x and in d_y: nobody else's gradients change."""
+    counts, E = shape["counts"], shape["E"]
+    print(f"[case] fp8 experts, backward with NaN and infinity, {shape}", flush=True)
+    assert _lib.load().pk_region_transposed_pays(sum(counts), shape["H"], shape["I"], E, _lib.PK_BF16) == (shape is PAYS)
+    w1, w2, w3, x, d_y = (t.to(dev) for t in _inputs(E, shape["H"], shape["I"], counts, 0, 8, False))
+    w = [t.requires_grad_(True) for t in (w1, w2, w3)]
+    n = torch.tensor(counts, device=dev)
+    want = _pass(w, x.requires_grad_(True), d_y, n)
+    for row, value in ((50, float("inf")), (146, float("nan"))):
+        for which in (0, 1):
+            rows = [x.detach().clone(), d_y.clone()]
+            rows[which][row, ::9] = value
+            got = _pass(w, rows[0].requires_grad_(True), rows[1], n)
+            for g, t in zip(got[1:4], want[1:4]):
+                assert not torch.isfinite(g[2]).all() and all(torch.equal(g[e], t[e]) for e in (0, 1, 3))
+            others = torch.arange(sum(counts), device=dev) != row
+            assert torch.equal(got[4][others], want[4][others]) and torch.isnan(got[4][row]).any()
