@@ -119,18 +119,17 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
-        """torch's, which gives every floating-point state the parameter's type: the 8-bit moments and their master keep theirs."""
-        super().load_state_dict(state_dict)
+        """torch's, which gives every floating-point state the parameter's type: the 8-bit moments and their master keep theirs.  A state
+        of the other ``state_bits`` or of other sizes is a ValueError that leaves the optimizer as it was."""
+        saved = []      # what the pre-hooks of the program make of state_dict: ours is the last to run
+        last = self.register_load_state_dict_pre_hook(lambda _, given: saved.extend(self._checked(given)))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            last.remove()
         if self.state_bits != 8:
             return
-        params = [p for group in self.param_groups for p in group["params"]]
-        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
-        for p, i in zip(params, saved):
-            st = state_dict["state"].get(i)
-            if st is None:
-                continue
-            if any(k not in st for k in _MOMENTS8):
-                raise ValueError("FusedAdamW(state_bits=8): the saved state has no 8-bit moments")
+        for p, st in saved:
             for name in _MOMENTS8:
                 self.state[p][name] = st[name].to(p.device).clone()
             if p.dtype == torch.float32:      # its own master
@@ -138,5 +137,25 @@ class FusedAdamW(torch.optim.Optimizer):
             else:
                 self.state[p]["master"] = st["master"].to(p.device).clone()
 
+    def _checked(self, state_dict) -> list:
+        """[(parameter, its saved state)] of a state dict that this optimizer can take."""
+        params = [p for group in self.param_groups for p in group["params"]]
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        found = [(p, state_dict["state"][i]) for p, i in zip(params, ids) if state_dict["state"].get(i)]
+        for p, st in found:
+            n, blocks = p.numel(), -(-p.numel() // ops.ADAMW8_BLOCK)
+            if self.state_bits == 8:
+                sizes = dict(zip(_MOMENTS8, (n, blocks, n, blocks)), master=n)
+                if any(k not in st or st[k].dtype != dt for k, dt in zip(_MOMENTS8, _TYPES8)) or "seed" not in st:
+                    raise ValueError("FusedAdamW(state_bits=8): the saved state has no 8-bit moments")
+            else:
+                sizes = dict(exp_avg=n, exp_avg_sq=n, master=n)
+                if any(k in st for k in _MOMENTS8[1::2]) or any(st[k].dtype in _TYPES8 for k in _MOMENTS8[::2] if k in st):
+                    raise ValueError("FusedAdamW(state_bits=32): the saved state has 8-bit moments, codes that are nothing without their scales")
+            if "step" not in st or any(k not in st or st[k].numel() != size for k, size in sizes.items()):
+                raise ValueError(f"FusedAdamW: the saved state is not one of a parameter of {n} elements")
+        return found
+
 
 _MOMENTS8 = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
+_TYPES8 = (torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.float8_e5m2, torch.float8_e8m0fnu)
