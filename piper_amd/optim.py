@@ -119,23 +119,28 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
-        """torch's, which gives every floating-point state the parameter's type: the 8-bit moments and their master keep theirs.  A state
-        of the other ``state_bits`` or of other sizes is a ValueError that leaves the optimizer as it was."""
-        saved = []      # what the pre-hooks of the program make of state_dict: ours is the last to run
-        last = self.register_load_state_dict_pre_hook(lambda _, given: saved.extend(self._checked(given)))
+        """torch's, which gives every floating-point state the parameter's type, a copy of its own: moments and master keep theirs here, and
+        an fp32 parameter stays its own master.  A state of the other ``state_bits`` or of other sizes is a ValueError that leaves the
+        optimizer as it was."""
+        saved = []      # what the program's own pre-hooks make of state_dict: this one is the last to run
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, given: saved.extend(self._checked(given))),
+                 self.register_load_state_dict_post_hook(lambda _: self._restore(saved), prepend=True))
         try:
             super().load_state_dict(state_dict)
         finally:
-            last.remove()
-        if self.state_bits != 8:
-            return
+            for hook in hooks:
+                hook.remove()
+
+    def _restore(self, saved) -> None:
+        types = dict(zip(_MOMENTS8, _TYPES8)) if self.state_bits == 8 else dict(exp_avg=torch.float32, exp_avg_sq=torch.float32)
         for p, st in saved:
-            for name in _MOMENTS8:
-                self.state[p][name] = st[name].to(p.device).clone()
-            if p.dtype == torch.float32:      # its own master
-                self.state[p]["master"] = p.detach().reshape(-1)
+            own = self.state[p]
+            for name, dtype in types.items():
+                own[name] = st[name].to(device=p.device, dtype=dtype, copy=True)
+            if p.dtype == torch.float32:
+                own["master"] = p.detach().reshape(-1)
             else:
-                self.state[p]["master"] = st["master"].to(p.device).clone()
+                own["master"] = st["master"].to(device=p.device, dtype=torch.float32, copy=True)
 
     def _checked(self, state_dict) -> list:
         """[(parameter, its saved state)] of a state dict that this optimizer can take."""

@@ -75,3 +75,24 @@ def test_a_hook_of_the_program_comes_first():
     opt.register_load_state_dict_pre_hook(lambda _, sd: dict(sd, state={}))
     opt.load_state_dict(eight.state_dict())
     assert not any(opt.state.get(p) for p in params)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_what_is_loaded_is_what_was_saved(bits, dtype):
+    theirs, source = _optimizer(bits, dtype, seed=1)
+    params, opt = _optimizer(bits, dtype)
+    with torch.no_grad():
+        for p, q in zip(params, theirs):
+            p.copy_(q)
+    saved = copy.deepcopy(source.state_dict())
+    seen = []
+    opt.register_load_state_dict_post_hook(lambda o: seen.append(o.state[params[0]]["master"].dtype))
+    opt.load_state_dict(saved)
+    assert seen == [torch.float32] and len(opt._optimizer_load_state_dict_post_hooks) == 1
+    for i, (p, q) in enumerate(zip(params, theirs)):
+        st = opt.state[p]
+        assert _same(st, source.state[q]) and st["master"].dtype == torch.float32
+        assert (st["master"].data_ptr() == p.data_ptr()) == (dtype == torch.float32)      # a step of the master is one of the parameter
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert st[name].data_ptr() != saved["state"][i][name].data_ptr()
