@@ -440,7 +440,10 @@ PK_API int pk_sched_slot_index(int device, uint64_t stream_handle, uint64_t capt
 #define PK_FP8_MAX_WEIGHTS 3
 
 /* Rows of x [., K] (dtype) in blocks: row r of the result is x[r], or with row_map (i32 [rows])
- * x[row_map[r] / row_map_div]. */
+ * x[row_map[r] / row_map_div].  pk_fp8_quantize_rows_of knows how many rows x has: entries that name none of them
+ * make rows of NaN, where pk_fp8_quantize_rows follows them. */
+PK_API int pk_fp8_quantize_rows_of(const void* x, int dtype, int64_t x_rows, const int32_t* row_map, int64_t row_map_div,
+                            uint8_t* q, uint8_t* scales, int64_t rows, int64_t K, pk_stream_t stream);
 PK_API int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map, int64_t row_map_div, uint8_t* q,
                          uint8_t* scales, int64_t rows, int64_t K, pk_stream_t stream);
 /* `count` weights (up to PK_FP8_MAX_WEIGHTS) of the same E experts in blocks: w[i] [E, N[i], K[i]] (dtype).  w, q, q_t, scales,

@@ -104,7 +104,8 @@ SIGNATURES = {
                                 _c_f32, _c_i64, _c_f32, _c_int, _p]),
     "pk_adamw_fused_packed": (_c_int, [_p, _p, _p, _p, _p, _p, _p, _c_i64, _c_int, _p, _c_int, _c_f32, _c_f32, _c_f32,
                                        _c_f32, _c_f32, _c_i64, _c_f32, _c_int, _p]),
-    # rows: x dtype row_map div q scales rows K stream; weights: w dtype q q_t scales E N K stream
+    # rows: x dtype (x_rows) row_map div q scales rows K stream; weights: count w dtype q q_t scales E N K stream
+    "pk_fp8_quantize_rows_of": (_c_int, [_p, _c_int, _c_i64, _p, _c_i64, _p, _p, _c_i64, _c_i64, _p]),
     "pk_fp8_quantize_rows": (_c_int, [_p, _c_int, _p, _c_i64, _p, _p, _c_i64, _c_i64, _p]),
     "pk_fp8_quantize_weights": (_c_int, [_c_int, _p, _c_int, *[_p] * 3, _c_i64, _p, _p, _p]),
     "pk_fp8_plan_bytes": (_c_i64, [_c_i64, _c_i64]),

@@ -42,7 +42,8 @@ __device__ __forceinline__ void load8(const T* p, int have, float (&f)[8]) {
 // ------------------------------------------------------------------------------------------------ rows
 // 16 lanes to a block, one pass: 2 (bf16) or 4 bytes read and 1 written per value, bound by the memory (32,768 x 2048 bf16: 35 us,
 // 5.7 TB/s, where a copy of 2 GiB reaches 4.9; with one or four blocks on their way in a lane 38).
-// N blocks of rows, by 16 lanes; block i is number `unit` + i * step of all, and there if below `units`.
+// N blocks of rows, by 16 lanes; block i is number `unit` + i * step of all, and there if below `units`.  source(r): the row of x that
+// is row r, negative where there is none: such rows are NaN.
 template <typename T, int N, typename Source>
 __device__ __forceinline__ void quantize_blocks(const T* x, Source&& source, uint8_t* q, uint8_t* s, int64_t unit, int step, int64_t units, int K,
                                                 int kb, FastDiv by_kb) {
@@ -55,7 +56,9 @@ __device__ __forceinline__ void quantize_blocks(const T* x, Source&& source, uin
     r[i] = pk_units::fastdiv((int)u, by_kb);
     b[i] = (int)(u - (int64_t)r[i] * kb);
     const int k = b[i] * BLOCK + lane * 8;
-    load8<T>(x + source(r[i]) * K + k, K - k, f[i]);
+    const int64_t from = source(r[i]);
+    load8<T>(x + (from < 0 ? 0 : from) * K + k, from < 0 ? 0 : K - k, f[i]);
+    if (from < 0) f[i][0] = __builtin_nanf("");
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -68,10 +71,14 @@ __device__ __forceinline__ void quantize_blocks(const T* x, Source&& source, uin
 }
 constexpr int ROW_BLOCKS = 2;
 template <typename T>
-__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ row_map, FastDiv map_div,
-                                                                uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t units, int K, int kb,
-                                                                FastDiv by_kb) {
-  const auto source = [&](int r) { return (int64_t)(row_map ? pk_units::fastdiv(row_map[r], map_div) : r); };
+__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ row_map, int64_t entries,
+                                                                FastDiv map_div, uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t units,
+                                                                int K, int kb, FastDiv by_kb) {
+  const auto source = [&](int r) -> int64_t {
+    if (!row_map) return (int64_t)(uint32_t)r;
+    const int entry = row_map[r];
+    return entry < 0 || entry >= entries ? -1 : (int64_t)(uint32_t)pk_units::fastdiv(entry, map_div);
+  };
   quantize_blocks<T, ROW_BLOCKS>(x, source, q, s, (int64_t)blockIdx.x * (THREADS / 16 * ROW_BLOCKS) + (threadIdx.x >> 4), THREADS / 16, units, K, kb, by_kb);
 }
 
@@ -249,7 +256,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void begin_kernel(const Begin p) {
   }
   const int group = threadIdx.x >> 4;
   const int64_t unit = (int64_t)(blockIdx.x - (FORWARD ? 1 : 0)) * (PLAN_THREADS / 16 * ROW_BLOCKS) + group;
-  quantize_blocks<bf16_t, ROW_BLOCKS>(p.x, [](int r) { return (int64_t)r; }, p.q, p.s, unit, PLAN_THREADS / 16, p.units, p.K, p.kb, p.by_kb);
+  quantize_blocks<bf16_t, ROW_BLOCKS>(p.x, [](int r) { return (int64_t)(uint32_t)r; }, p.q, p.s, unit, PLAN_THREADS / 16, p.units, p.K, p.kb, p.by_kb);
   if (!FORWARD && p.map) {
     const int64_t r = (int64_t)blockIdx.x * PLAN_THREADS + threadIdx.x;
     if (r < p.A) p.map[r] = (int32_t)(r < *p.owned ? r : *p.owned > 0 ? *p.owned - 1 : 0);
@@ -1240,25 +1247,32 @@ bool bf16_pieces(int64_t width, std::initializer_list<const void*> ps) { return 
 
 extern "C" {
 
-int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map, int64_t row_map_div, uint8_t* q, uint8_t* scales, int64_t rows,
-                         int64_t K, pk_stream_t stream) {
-  if (rows < 0 || K <= 0 || row_map_div < 1 || !pk_dtype_ok(dtype)) return PK_ERR_ARG;
+int pk_fp8_quantize_rows_of(const void* x, int dtype, int64_t x_rows, const int32_t* row_map, int64_t row_map_div, uint8_t* q, uint8_t* scales,
+                            int64_t rows, int64_t K, pk_stream_t stream) {
+  if (rows < 0 || x_rows < 0 || K <= 0 || row_map_div < 1 || !pk_dtype_ok(dtype) || (!row_map && rows > x_rows)) return PK_ERR_ARG;
   if (rows == 0) return PK_OK;
   if (!all_set({x, q, scales})) return PK_ERR_ARG;
   if (!pk_aligned16(q)) return PK_ERR_ALIGN;
   const int64_t kb = blocks_of(K), units = rows * kb;
   if (K > 0x7fffff00ll || rows > 0x7fffffffll || units > 0x7fffffffll || row_map_div > 0x7fffffffll) return PK_ERR_SHAPE;
   const FastDiv div = pk_units::make_fastdiv(row_map_div), by_kb = pk_units::make_fastdiv(kb);
+  // of the row map, those that name a row of x
+  const int64_t entries = x_rows > 0x7fffffffll / row_map_div ? 0x80000000ll : x_rows * row_map_div;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)pk_ceil_div(units, THREADS / 16 * ROW_BLOCKS)), block(THREADS);
   if (dtype == PK_BF16)
-    PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_rows_kernel<bf16_t>), grid, block, 0, s, (const bf16_t*)x, row_map, div, q, scales,
-                      units, (int)K, (int)kb, by_kb);
+    PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_rows_kernel<bf16_t>), grid, block, 0, s, (const bf16_t*)x, row_map, entries, div, q,
+                      scales, units, (int)K, (int)kb, by_kb);
   else
-    PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_rows_kernel<float>), grid, block, 0, s, (const float*)x, row_map, div, q, scales,
-                      units, (int)K, (int)kb, by_kb);
+    PK_LAUNCH_NOCHECK(pk_timing::K_FP8_QUANTIZE, s, (quantize_rows_kernel<float>), grid, block, 0, s, (const float*)x, row_map, entries, div, q,
+                      scales, units, (int)K, (int)kb, by_kb);
   PK_RETURN_IF_LAUNCH_FAILED();
   return PK_OK;
+}
+
+int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map, int64_t row_map_div, uint8_t* q, uint8_t* scales, int64_t rows,
+                         int64_t K, pk_stream_t stream) {
+  return pk_fp8_quantize_rows_of(x, dtype, 0x7fffffffffffffffll, row_map, row_map_div, q, scales, rows, K, stream);
 }
 
 int pk_fp8_quantize_weights(int count, const void* const* w, int dtype, uint8_t* const* q, uint8_t* const* q_t, uint8_t* const* scales, int64_t E,

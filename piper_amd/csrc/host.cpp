@@ -955,7 +955,7 @@ std::pair<Tensor, Tensor> quantize_rows(const Tensor& x_, const OptTensor& row_m
   const Tensor x = contig(x_);
   const int64_t R = row_map.defined() ? row_map.numel() : x.size(0), K = x.size(1), kb = whole_blocks(K);
   Tensor q = at::empty({R, kb * PK_FP8_BLOCK}, x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({R, (kb + 3) / 4 * 4}, x.options().dtype(at::kFloat8_e8m0fnu));
-  PK_CALL(pk_fp8_quantize_rows, ptr(x), dtype_code(x), row_map.defined() ? row_map.data_ptr<int32_t>() : nullptr, map_div, u8(q), u8(s), R, K,
+  PK_CALL(pk_fp8_quantize_rows_of, ptr(x), dtype_code(x), x.size(0), row_map.defined() ? row_map.data_ptr<int32_t>() : nullptr, map_div, u8(q), u8(s), R, K,
           stream_of(x));
   return {q, s.narrow(1, 0, kb)};
 }

@@ -394,8 +394,8 @@ def grouped_swiglu_wgrad(d_y, h, d_g, d_u, x_rows, starts, E, *, row_map=None, r
 
 def quantize_rows_fp8(x: torch.Tensor, row_map: torch.Tensor | None = None, row_map_div: int = 1):
     """Rows of x [R,K] (or x[row_map // row_map_div]) in 8-bit floating point: (e4m3 codes [R,K'], e8m0 scales [R,K'/128]) with
-    K' = ceil(K / 128) * 128; a value is code * scale of its block of 128, the rest of the last block is zero.  In memory a row of scales
-    is a whole number of 32-bit words."""
+    K' = ceil(K / 128) * 128; a value is code * scale of its block of 128, the rest of the last block is zero.  Entries of the row map that name
+    no row of x make rows of NaN.  In memory a row of scales is a whole number of 32-bit words."""
     return host().quantize_rows(x, row_map, int(row_map_div))
 
 
