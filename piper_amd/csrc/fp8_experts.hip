@@ -171,9 +171,9 @@ __global__ __launch_bounds__(THREADS) void quantize_weights_kernel(const Weights
 // three dependent ones, 2 us each while the chip is busy.
 //   [E + 1] starts (cut off at A), tiles, padding to 8; then for every tile 8 words: expert, its first tile, its tiles, its first
 //   row and the row behind its last, padding.  Counts that do not fit into A rows, or are negative, cannot lead a kernel out of bounds.
-constexpr int TILE_ROWS = 128, PLAN_THREADS = 1024, ENTRY = 8;
+constexpr int TILE_ROWS = pk_rules::FP8_TILE_ROWS, PLAN_THREADS = 1024, ENTRY = 8;
 __host__ __device__ inline int64_t plan_head(int64_t E) { return (E + 2 + ENTRY - 1) / ENTRY * ENTRY; }
-__host__ __device__ inline int64_t plan_tiles(int64_t A, int64_t E) { return A / TILE_ROWS + (A < E ? A : E); }
+inline int64_t plan_tiles(int64_t A, int64_t E) { return pk_rules::fp8_tiles(A, E, TILE_ROWS); }
 
 // sum over the threads before this one (exclusive), all of PLAN_THREADS; *total: over all of them
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* waves /* 16 */, int64_t* total) {
@@ -456,7 +456,7 @@ __device__ __forceinline__ int unit_of_block(int b) {      // neighbouring units
 // [padded rows / 32][N][32], expert e's rows from (begin & ~63) + 64 e on, zeros behind its last row up to the end of its last block.
 // NARROW (not GATE_UP, whose unit has to have whole blocks of h): units of 128 columns, waves (4 x 2) of 32 x 64, for launches that
 // leave CUs without a unit.
-constexpr int NT = 512, BM = TILE_ROWS, WIDE = 256, STAGES = 3, A_BYTES = BM * BLOCK, STAGE = A_BYTES + WIDE * BLOCK;
+constexpr int NT = 512, BM = TILE_ROWS, WIDE = pk_rules::FP8_WIDE, STAGES = 3, A_BYTES = BM * BLOCK, STAGE = A_BYTES + WIDE * BLOCK;
 inline int product_lds(int nblk4) { return STAGES * STAGE + nblk4 * BM + 2 * nblk4; }
 
 template <int EPI, bool VEC, bool TRANSPOSED, bool EXACT, bool NARROW>
@@ -843,19 +843,9 @@ __global__ __launch_bounds__(NT, 2) void product_kernel(const Product p) {
   }
 }
 
-// Short sums where they are asked for and faster.  us, codes : decoded, gate and up, down, d_h, d_x with n rows an expert.  128 experts 2048 x 768: 32 rows 133 : 136, 82 : 83, 108 : 108,
-// 130 : 134; 48 rows 137 : 140, 85 : 86, 110 : 112, 131 : 134; 64 rows 139 : 149, 88 : 92, 115 : 120, 136 : 148; 512 rows 370 : 572, 225 : 310,
-// 323 : 420.  24 experts 1000 x 360, 32 rows: 19 : 20, 10 : 12, 25 : 26, 14 : 15.
-bool exact_products(bool short_sums, int64_t A, int64_t E) { return !short_sums || A <= 40 * E || A <= TILE_ROWS; }
-
-// Of as many wide units, at most, a launch is made of narrow ones, us, wide : narrow, down, d_h, d_x.  2048 x 768: 4 experts of 64 rows 14 : 11,
-// 33 : 22, 21 : 15; 8 of 200 16 : 14, 40 : 27, 23 : 19; 16 of 30 17 : 16, 35 : 24, 26 : 24; 16 of 200 (328 units, in d_h 123) 20 : 21, 42 : 30,
-// 31 : 33; 32 of 200 (656, 246) 35 : 37, 53 : 55, 56 : 60.  24 experts of 172 rows 1000 x 360 (224, 112) 15 : 15, 31 : 22, 18 : 19.
-constexpr int NARROW_UNITS = 192;
-
 template <int EPI>
 int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool short_sums, bool transposed = false) {
-  const bool narrow = EPI != GATE_UP && !transposed && plan_tiles(A, p.E) * pk_ceil_div(p.N, WIDE) <= NARROW_UNITS;
+  const bool narrow = EPI != GATE_UP && !transposed && pk_rules::fp8_narrow(A, p.E, p.N);
   p.n_tiles = (int32_t)pk_ceil_div(p.N, EPI == GATE_UP || narrow ? BLOCK : WIDE);
   p.by_n_tiles = pk_units::make_fastdiv(p.n_tiles);
   p.head = (int32_t)plan_head(p.E);
@@ -878,7 +868,7 @@ int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool shor
     return PK_OK;
   };
   static bool ready[10][PK_MAX_DEVICES] = {};
-  const bool exact = exact_products(short_sums, A, p.E);
+  const bool exact = pk_rules::fp8_exact(short_sums, A, p.E);
   if constexpr (EPI == BWD)
     if (transposed)
       return exact ? launch(product_kernel<EPI, true, true, true, false>, ready[9]) : launch(product_kernel<EPI, true, true, false, false>, ready[8]);
@@ -903,7 +893,7 @@ int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool shor
 //   down_few:    h in blocks into the LDS, then 16 columns to each of four waves
 // One token of 8 experts of 2048 x 768 takes 11.9 + 7.1 us, of which the weights are 7.7 at the rate of a copy: the rest is the chain of
 // counts, weights, sums, twice.  24 tokens (some 100 of 128 experts) 73 + 44 us for 470 MB, 4.0 TB/s.
-constexpr int FEW_ROWS = 16;
+constexpr int FEW_ROWS = pk_rules::FP8_FEW_ROWS;
 
 struct Few {
   const void* counts;
@@ -1498,11 +1488,7 @@ int pk_fp8_dgrad_dx_short(const uint8_t* d_g8, const uint8_t* d_g_scales, const 
 
 int pk_fp8_few_rows_pays(int64_t A, int64_t H, int64_t I, int64_t E) {
   if (check(A, H, I, E) != PK_OK || A == 0) return 0;
-  // us, this : quantization, plan and tiles.  128 experts 2048 x 768: 8 rows an expert 143 : 173, 11 rows 150 : 173, 12 rows 190 : 174, 16
-  // rows 229 : 177 (where an expert has more than 16 its weights are read again); 32 of them: 8 rows 53 : 71, 12 rows 62 : 72, 16 rows
-  // 88 : 73; 24 experts 1000 x 360: 8 rows 28 : 29, 12 rows 30 : 29, 16 rows 37 : 30.  128 rows in all: one expert 2048 x 768 26 : 40, two
-  // 35 : 42, eight 29 : 38, eight of 4096 x 1408 63 : 81.
-  return A <= 11 * E || A <= TILE_ROWS;
+  return pk_rules::fp8_few_rows(A, E);
 }
 
 int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64, const uint8_t* w1, const uint8_t* s1, const uint8_t* w2,
@@ -1517,12 +1503,9 @@ int pk_fp8_experts_few_rows(const void* x, const void* counts, int counts_is_i64
   p.x = (const bf16_t*)x; p.q1 = w1; p.s1 = s1; p.q2 = w2; p.s2 = s2; p.q3 = w3; p.s3 = s3;
   p.g = (bf16_t*)g; p.u = (bf16_t*)u; p.h = h; p.y = (bf16_t*)y;
   p.whole = H % 8 == 0;
-  const int64_t tiles = A / FEW_ROWS + (A < E ? A : E);
-  // whole reductions to a wave where that gives every CU a workgroup, and four column tiles to a wave of down where that fills the chip
-  // eight times (both : eight waves to a reduction : one column tile, us; 128 experts 2048 x 768, 2 rows each 146 : 176 : 154, 8
-  // rows 161 : 203 : 170; 8 experts with a row each 21 without, 40 and 35 with one of them)
-  const bool stream_up = tiles * blocks_of(I) >= 256;
-  const int64_t up = stream_up ? blocks_of(I) : pk_ceil_div(I, 16), per = tiles * pk_ceil_div(H, 64) >= 2048 ? 4 : 1, down = pk_ceil_div(H, 64 * per);
+  const int64_t tiles = pk_rules::fp8_tiles(A, E, FEW_ROWS);
+  const bool stream_up = pk_rules::fp8_stream_up(A, E, I);
+  const int64_t up = stream_up ? blocks_of(I) : pk_ceil_div(I, 16), per = pk_rules::fp8_down_tiles(A, E, H), down = pk_ceil_div(H, 64 * per);
   if (tiles * up > 0x7fffff00ll || tiles * down > 0x7fffff00ll) return PK_ERR_SHAPE;
   static bool ready[PK_MAX_DEVICES] = {};
   int dev = 0;

@@ -132,4 +132,27 @@ constexpr bool absent_rows_left_out(bool gate_up, int64_t A, int64_t E, int64_t 
   return 2 * A <= tile_rows * experts && k_tiles >= 12 && experts * col_tiles <= (gate_up ? 3 : 4) * cus;
 }
 
+// ---- experts in 8-bit blocks
+constexpr int FP8_TILE_ROWS = 128, FP8_FEW_ROWS = 16, FP8_WIDE = 256;
+// row tiles, at most
+constexpr int64_t fp8_tiles(int64_t A, int64_t E, int64_t rows) { return A / rows + (A < E ? A : E); }
+// fp32 sums unless short ones are asked for and faster.  us, codes : decoded, gate and up, down, d_h, d_x with n rows an expert.  128 experts
+// 2048 x 768: 32 rows 133 : 136, 82 : 83, 108 : 108, 130 : 134; 48 rows 137 : 140, 85 : 86, 110 : 112, 131 : 134; 64 rows 139 : 149, 88 : 92, 115 : 120, 136 : 148; 512 rows 370 : 572, 225 : 310,
+// 323 : 420.  24 experts 1000 x 360, 32 rows: 19 : 20, 10 : 12, 25 : 26, 14 : 15.
+constexpr bool fp8_exact(bool short_sums, int64_t A, int64_t E) { return !short_sums || A <= 40 * E || A <= FP8_TILE_ROWS; }
+// Of as many wide units, at most, a launch is made of narrow ones, us, wide : narrow, down, d_h, d_x.  2048 x 768: 4 experts of 64 rows 14 : 11,
+// 33 : 22, 21 : 15; 8 of 200 16 : 14, 40 : 27, 23 : 19; 16 of 30 17 : 16, 35 : 24, 26 : 24; 16 of 200 (328 units, in d_h 123) 20 : 21, 42 : 30,
+// 31 : 33; 32 of 200 (656, 246) 35 : 37, 53 : 55, 56 : 60.  24 experts of 172 rows 1000 x 360 (224, 112) 15 : 15, 31 : 22, 18 : 19.
+constexpr bool fp8_narrow(int64_t A, int64_t E, int64_t N) { return fp8_tiles(A, E, FP8_TILE_ROWS) * ceil_div(N, FP8_WIDE) <= 192; }
+// The way of few rows.  us, this : quantization, plan and tiles.  128 experts 2048 x 768: 8 rows an expert 143 : 173, 11 rows 150 : 173, 12 rows 190 : 174, 16
+// rows 229 : 177 (where an expert has more than 16 its weights are read again); 32 of them: 8 rows 53 : 71, 12 rows 62 : 72, 16 rows
+// 88 : 73; 24 experts 1000 x 360: 8 rows 28 : 29, 12 rows 30 : 29, 16 rows 37 : 30.  128 rows in all: one expert 2048 x 768 26 : 40, two
+// 35 : 42, eight 29 : 38, eight of 4096 x 1408 63 : 81.
+constexpr bool fp8_few_rows(int64_t A, int64_t E) { return A <= 11 * E || A <= FP8_TILE_ROWS; }
+// Its variants: whole reductions to a wave where that gives every CU a workgroup, and four column tiles to a wave of down where that fills
+// the chip eight times (both : eight waves to a reduction : one column tile, us; 128 experts 2048 x 768, 2 rows each 146 : 176 : 154, 8
+// rows 161 : 203 : 170; 8 experts with a row each 21 without, 40 and 35 with one of them)
+constexpr bool fp8_stream_up(int64_t A, int64_t E, int64_t I) { return fp8_tiles(A, E, FP8_FEW_ROWS) * ceil_div(I, 128) >= 256; }
+constexpr int fp8_down_tiles(int64_t A, int64_t E, int64_t H) { return fp8_tiles(A, E, FP8_FEW_ROWS) * ceil_div(H, 64) >= 2048 ? 4 : 1; }
+
 }  // namespace pk_rules
