@@ -1119,7 +1119,7 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
 };
 std::optional<Tensor> bmm_experts_fp8(const OptTensor& w1_, const OptTensor& w2_, const OptTensor& w3_, const Tensor& q1, const Tensor& q2,
                                       const Tensor& q3, const Tensor& s1, const Tensor& s2, const Tensor& s3, const OptTensor& t1_,
-                                      const OptTensor& t2_, const OptTensor& t3_, bool short_sums, const Tensor& x, const Tensor& counts, bool direct) {
+                                      const OptTensor& t2_, const OptTensor& t3_, const Tensor& x, const Tensor& counts, bool short_sums, bool direct) {
   const Tensor w1 = opt(w1_), w2 = opt(w2_), w3 = opt(w3_), t1 = opt(t1_), t2 = opt(t2_), t3 = opt(t3_);
   if (direct && !plain({&w1, &w2, &w3, &q1, &q2, &q3, &s1, &s2, &s3, &t1, &t2, &t3, &x, &counts})) return std::nullopt;
   refuse_transforms({&w1, &w2, &w3, &q1, &q2, &q3, &s1, &s2, &s3, &t1, &t2, &t3, &x, &counts}, "bmm_experts_fp8");

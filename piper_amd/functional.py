@@ -205,13 +205,14 @@ def quantize_experts(w1, w2, w3, *, for_backward: bool = True, short_sums: bool 
 
 
 def _bmm_experts_fp8(*args):
-    x = args[13]
+    tensors, short_sums = args[:14], len(args) > 14 and args[14]      # (the dispatcher leaves out what is the default)
+    x = tensors[12]
     if _traced_without_data(x):
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (*args[:3], x) if t is not None):
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (*tensors[:3], x) if t is not None):
             out.requires_grad_(True)
         return out
-    return host().bmm_experts_fp8(*args, False)
+    return host().bmm_experts_fp8(*tensors, short_sums, False)
 
 
 def _bmm_experts_fp8_forward_only(*args):
@@ -228,12 +229,12 @@ def bmm_experts_fp8(experts: Fp8Experts, x, num_tokens_per_expert):
     Backward: d_y and the gradients of gate and up are held in the same blocks for the products that lead to x, rounding counts
     as the identity; the weights' gradients (of ``experts.w1``, ``w2``, ``w3``) are bfloat16 products of the rows as they came.
     ``defer_weight_grads`` and ``accumulate_weight_grads`` apply as they do to ``bmm_experts``."""
-    args = (*experts, x, num_tokens_per_expert)
-    if _direct(*args):
-        out = host().bmm_experts_fp8(*args, True)
+    tensors = (*experts[:12], x, num_tokens_per_expert)
+    if _direct(*tensors):
+        out = host().bmm_experts_fp8(*tensors, experts.short_sums, True)
         if out is not None:
             return out
-    return torch.ops.piper_amd.bmm_experts_fp8(*args)
+    return torch.ops.piper_amd.bmm_experts_fp8(*tensors, experts.short_sums)
 
 
 def _combine(y, perm, top_scores):
@@ -362,7 +363,7 @@ def register_region_ops() -> bool:
                "int top_k, bool route_norm, float route_scale, Tensor? residual) -> Tensor")
     lib.define("rmsnorm(Tensor x, Tensor weight, float eps) -> Tensor")
     lib.define("bmm_experts_fp8(Tensor? w1, Tensor? w2, Tensor? w3, Tensor q1, Tensor q2, Tensor q3, Tensor s1, Tensor s2, Tensor s3, "
-               "Tensor? t1, Tensor? t2, Tensor? t3, bool short_sums, Tensor x, Tensor num_tokens_per_expert) -> Tensor")
+               "Tensor? t1, Tensor? t2, Tensor? t3, Tensor x, Tensor num_tokens_per_expert, bool short_sums=False) -> Tensor")
     for name, fwd, auto in (("expert_region", _expert_region_forward_only, _expert_region_autograd),
                             ("rmsnorm", _rmsnorm_forward_only, _rmsnorm_autograd),
                             ("bmm_experts_fp8", _bmm_experts_fp8_forward_only, _bmm_experts_fp8)):

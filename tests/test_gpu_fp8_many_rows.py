@@ -394,3 +394,29 @@ def test_few_rows_of_many_experts(dev, E, H, I, A):
         assert torch.equal(got[0], F_.bmm_experts_fp8(F_.quantize_experts(*w, for_backward=False), x.to(dev), n))
     for name, t in zip(("y", "d_w1", "d_w2", "d_w3", "d_x"), got):
         _within(name, t, *want[name])
+
+
+def test_the_operator_takes_the_choice_last(dev):
+    """Called by its name, as a captured graph does: without the choice it is the default."""
+    print("[case] fp8 experts through the dispatcher, short sums", flush=True)
+    w1, w2, w3, x, d_y = (t.to(dev) for t in _inputs(2, 256, 128, [150, 140], 0, 9, False))
+    n = torch.tensor([150, 140], device=dev)
+    F_.register_region_ops()
+    for short in (False, True):
+        e = F_.quantize_experts(w1, w2, w3, short_sums=short)
+        want = F_.bmm_experts_fp8(e, x, n)
+        tensors = (*e[:12], x, n)
+        assert torch.equal(want, torch.ops.piper_amd.bmm_experts_fp8(*tensors, short))
+        if not short:
+            assert torch.equal(want, torch.ops.piper_amd.bmm_experts_fp8(*tensors))
+        rows = x.clone().requires_grad_(True)
+        got = torch.ops.piper_amd.bmm_experts_fp8(*e[:12], rows, n, short_sums=short)
+        assert torch.equal(want, got)
+        again = x.clone().requires_grad_(True)
+        assert torch.equal(torch.autograd.grad(got, rows, d_y)[0], torch.autograd.grad(F_.bmm_experts_fp8(e, again, n), again, d_y)[0])
+
+    @torch.compile(backend="eager", fullgraph=True)
+    def compiled(x):
+        return F_.bmm_experts_fp8(e, x, n)
+
+    assert torch.equal(compiled(x), want)
