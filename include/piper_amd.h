@@ -432,7 +432,7 @@ PK_API int pk_sched_slot_index(int device, uint64_t stream_handle, uint64_t capt
  *   weights  q [E][N][K'], scales [E][N'/128][K'/128]; transposed codes q_t [E][K][N'] share the scales
  * Code buffers must be 16-byte aligned.  The products take bf16 tensors of any width up to
  * H = PK_FP8_MAX_HIDDEN, I = PK_FP8_MAX_INTER; an operand's codes must span less than 4 GiB
- * (PK_ERR_SHAPE).  Which rows are whose comes from a plan (pk_fp8_plan); rows of no expert are not
+ * (PK_ERR_SHAPE).  Products are exact and added in fp32 but for the entry points ending in _short.  Which rows are whose comes from a plan (pk_fp8_plan); rows of no expert are not
  * read, and zeros in y and d_x. */
 #define PK_FP8_BLOCK 128
 #define PK_FP8_MAX_HIDDEN 8192
@@ -451,7 +451,7 @@ PK_API int pk_fp8_quantize_rows(const void* x, int dtype, const int32_t* row_map
 PK_API int pk_fp8_quantize_weights(int count, const void* const* w, int dtype, uint8_t* const* q, uint8_t* const* q_t,
                             uint8_t* const* scales, int64_t E, const int64_t* N, const int64_t* K, pk_stream_t stream);
 
-/* The row ranges of a pass over A rows, for the four products below: expert e owns counts[e] rows (int32, or
+/* The row ranges of a pass over A rows, for the products below: expert e owns counts[e] rows (int32, or
  * int64 with counts_is_i64) behind those of the experts before it.  plan: pk_fp8_plan_bytes(A, E) bytes, 16-byte
  * aligned; its first E + 1 words are starts[] as the other entry points take them.  Counts that are negative
  * count as zero, and rows past A are cut off.  A plan serves passes over the A and E that it was made for. */

@@ -367,7 +367,7 @@ __global__ __launch_bounds__(kStreamThreads) void adamw_packed_kernel(
 // of 64 is 16 lanes, whose largest magnitude takes four vector instructions and no LDS.  Scales are powers of two, so decoding and
 // scaling are exact, and everything in between is the fp32 update with every operation rounded by itself
 // (no contraction): the same codes come out wherever it is computed.  Bound by the memory, 16.06 bytes an element with bf16 gradients and
-// parameters: 160 M elements in 0.45 ms, 5.7 TB/s (with fp32 moments 28 bytes and 0.78 ms).
+// parameters: 160 M elements in 0.45 to 0.47 ms, 5.4 to 5.7 TB/s (with fp32 moments 28 bytes and 0.78 ms).
 struct Adam8Args {
   float decay, one_m_b1, beta2, one_m_b2, step_size, inv_bc2_sqrt, eps, grad_scale;
   uint32_t seed;

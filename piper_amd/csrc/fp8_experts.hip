@@ -446,12 +446,16 @@ __device__ __forceinline__ int unit_of_block(int b) {      // neighbouring units
 // One persistent workgroup to a CU, eight waves (2 x 4) of 64 x 64 outputs, a ring of three k-tiles.  A workgroup goes through its
 // units one after the other: behind a unit's last k-tile it requests the first two of the next one, and the epilogue, which
 // needs the LDS for the blocks' maxima alone, runs while they are on their way.
-// What bounds it: a CU has no more than some 128 cache lines (16 KB) on their way from the L2, in order; with 128 experts of 2048 x 768
-// and 512 rows each a line of gate and up takes 664 cycles on average (7 of 10 are in the L2), which is the 24 bytes a cycle that
-// the transfers reach by themselves.  Multiplying is not it: two halves of the waves that took turns at reading the LDS and at
-// multiplying changed nothing.  Nor did dealing neighbouring units by 8, 16 or 32 to an XCD, or experts that start at different k-tiles.
-// 128 experts of 2048 x 768 with 512 rows each, us, against two workgroups of four waves to a CU with half-block k-tiles: gate and up
-// 363 : 376, down 225 : 261, d_h (row-major copies) 326 : 354; with 111 rows each 105 : 110 and 64 : 68, which is 4.2 TB/s.
+// What bounds it: multiplying and decoding.  With 128 experts of 2048 x 768 and 256 rows each gate and up take 295 us, in which the matrix
+// units are busy for 40 % of the cycles and the vector units, which mostly decode (a wave 128 pairs a lane and k-tile for its 32
+// products of 32 x 32 x 16), for another 40 %; with 111 rows 156.
+// With short sums: a CU has no more than some 128 cache lines (16 KB) on their way from the L2, in order; with 512 rows each a line of
+// gate and up takes 664 cycles on average (7 of 10 are in the L2), which is the 24 bytes a cycle that the transfers reach by themselves
+// (a unit's first wait, for a scale byte and the first k-tile, takes the stores of the one before along; what that costs is not known).
+// Two halves of the waves that took turns at reading the LDS and at multiplying changed nothing, nor did dealing neighbouring units
+// by 8, 16 or 32 to an XCD, or experts that start at different k-tiles.  512 rows each, us, against two workgroups of four waves to a CU with
+// half-block k-tiles: gate and up 363 : 376, down 225 : 261, d_h (row-major copies) 326 : 354; with 111 rows each 105 : 110 and 64 : 68,
+// which is 4.2 TB/s.
 // TRANSPOSED (BWD, N a multiple of 256): O0 to O2 are the transposed copies that pk_grouped_swiglu_wgrad_scaled_t reads,
 // [padded rows / 32][N][32], expert e's rows from (begin & ~63) + 64 e on, zeros behind its last row up to the end of its last block.
 // NARROW (not GATE_UP, whose unit has to have whole blocks of h): units of 128 columns, waves (4 x 2) of 32 x 64, for launches that
@@ -892,7 +896,8 @@ int launch_product(Product p, int64_t A, int kernel_id, hipStream_t s, bool shor
 //                since a block of it belongs to eight workgroups
 //   down_few:    h in blocks into the LDS, then 16 columns to each of four waves
 // One token of 8 experts of 2048 x 768 takes 11.9 + 7.1 us, of which the weights are 7.7 at the rate of a copy: the rest is the chain of
-// counts, weights, sums, twice.  24 tokens (some 100 of 128 experts) 73 + 44 us for 470 MB, 4.0 TB/s.
+// counts, weights, sums, twice.  24 tokens (some 100 of 128 experts) 73 + 44 us for 470 MB, 4.0 TB/s.  Where H is no multiple of 8
+// gate_up_few loads its rows value by value (8 rows of 8 experts, 2048 x 768 16 us, 2047 x 767 21; 128 of 64, 1000 x 360 37, 1001 x 361 55).
 constexpr int FEW_ROWS = pk_rules::FP8_FEW_ROWS;
 
 struct Few {
@@ -1080,8 +1085,9 @@ __host__ __device__ inline int few_lds(int64_t K) {
   return FEW_ROWS * (nb * BLOCK + 16) + FEW_ROWS * nb;
 }
 
-// The products of a row tile in the LDS with `tiles` times 16 columns of MATS weights, a block after the other with D blocks of them
-// in flight; done(c, acc) for every 16 columns.  w: the lane's part of column tile 0, `next` bytes further for the next one.
+// The products of a row tile in the LDS with `tiles` times 16 columns of MATS weights, block after block, each requested D steps ahead (but
+// a step waits for its scale byte, requested last, and memory answers in order: what was requested before is waited for as well);
+// done(c, acc) for every 16 columns.  w: the lane's part of column tile 0, `next` bytes further for the next one.
 template <int MATS, int D, typename Done>
 __device__ __forceinline__ void stream_columns(const uint8_t* const (&w)[MATS], int64_t next, const uint8_t* const (&sw)[MATS], int64_t next_scale,
                                                int nb, int tiles, const uint8_t* q, int ld, const uint8_t* qs, bool ready, Done&& done) {

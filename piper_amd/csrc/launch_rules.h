@@ -140,9 +140,10 @@ constexpr int64_t fp8_tiles(int64_t A, int64_t E, int64_t rows) { return A / row
 // 2048 x 768: 32 rows 133 : 136, 82 : 83, 108 : 108, 130 : 134; 48 rows 137 : 140, 85 : 86, 110 : 112, 131 : 134; 64 rows 139 : 149, 88 : 92, 115 : 120, 136 : 148; 512 rows 370 : 572, 225 : 310,
 // 323 : 420.  24 experts 1000 x 360, 32 rows: 19 : 20, 10 : 12, 25 : 26, 14 : 15.
 constexpr bool fp8_exact(bool short_sums, int64_t A, int64_t E) { return !short_sums || A <= 40 * E || A <= FP8_TILE_ROWS; }
-// Of as many wide units, at most, a launch is made of narrow ones, us, wide : narrow, down, d_h, d_x.  2048 x 768: 4 experts of 64 rows 14 : 11,
-// 33 : 22, 21 : 15; 8 of 200 16 : 14, 40 : 27, 23 : 19; 16 of 30 17 : 16, 35 : 24, 26 : 24; 16 of 200 (328 units, in d_h 123) 20 : 21, 42 : 30,
-// 31 : 33; 32 of 200 (656, 246) 35 : 37, 53 : 55, 56 : 60.  24 experts of 172 rows 1000 x 360 (224, 112) 15 : 15, 31 : 22, 18 : 19.
+// A launch of so few wide units, at most, is made of narrow ones, us, wide : narrow, down, d_h, d_x, weights in the caches.  2048 x 768: 4 experts
+// of 64 rows 10 : 7, 29 : 18, 16 : 10; 16 of 30 9 : 7, 27 : 18, 16 : 11; 8 of 200 (160 units, in d_h 60) 14 : 10, 40 : 24, 23 : 16; 16 of 200
+// (328, 123) 16.6 : 17.8, 41 : 26, 27 : 29; 32 of 200 (656, 246) 30 : 32, 42 : 46, 50 : 54.  24 experts of 172 rows 1000 x 360 (224, 112) 10.6 : 11.2,
+// 27 : 18, 15.6 : 16.5.
 constexpr bool fp8_narrow(int64_t A, int64_t E, int64_t N) { return fp8_tiles(A, E, FP8_TILE_ROWS) * ceil_div(N, FP8_WIDE) <= 192; }
 // The way of few rows.  us, this : quantization, plan and tiles.  128 experts 2048 x 768: 8 rows an expert 143 : 173, 11 rows 150 : 173, 12 rows 190 : 174, 16
 // rows 229 : 177 (where an expert has more than 16 its weights are read again); 32 of them: 8 rows 53 : 71, 12 rows 62 : 72, 16 rows

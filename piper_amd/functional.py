@@ -228,7 +228,8 @@ def bmm_experts_fp8(experts: Fp8Experts, x, num_tokens_per_expert):
 
     Backward: d_y and the gradients of gate and up are held in the same blocks for the products that lead to x, rounding counts
     as the identity; the weights' gradients (of ``experts.w1``, ``w2``, ``w3``) are bfloat16 products of the rows as they came.
-    ``defer_weight_grads`` and ``accumulate_weight_grads`` apply as they do to ``bmm_experts``."""
+    ``defer_weight_grads`` and ``accumulate_weight_grads`` apply as they do to ``bmm_experts``.  A row of x or d_y that is not finite
+    makes its own results so and its expert's weight gradients, nobody else's."""
     tensors = (*experts[:12], x, num_tokens_per_expert)
     if _direct(*tensors):
         out = host().bmm_experts_fp8(*tensors, experts.short_sums, True)
