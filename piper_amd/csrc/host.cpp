@@ -338,6 +338,19 @@ Tensor region_forward(const Shape& s, PyObject* route, Saved& sv, bool keep_gu, 
 }
 
 // Weight-gradient kernels of the fused region with everything they read.
+// kernel(three gradients) for kernels that take 16-byte aligned ones only: a gradient that is added to may be a view that starts anywhere,
+// and goes through a copy then
+template <typename F>
+void through_aligned(const Tensor& d1, const Tensor& d2, const Tensor& d3, bool accumulate, const F& kernel) {
+  at::NoGradGuard no_grad;
+  const Tensor* const to[3] = {&d1, &d2, &d3};
+  Tensor in[3];
+  for (int i = 0; i < 3; ++i) in[i] = aligned16_all({to[i]}) ? *to[i] : accumulate ? to[i]->clone() : at::empty_like(*to[i]);
+  kernel(in[0], in[1], in[2]);
+  for (int i = 0; i < 3; ++i)
+    if (!in[i].is_same(*to[i])) to[i]->copy_(in[i]);
+}
+
 struct RegionWgrad {
   Shape s;
   Tensor d_out, x, rows, grads;           // owners of the memory below (x: undefined where the rows are a norm's output)
@@ -348,8 +361,10 @@ struct RegionWgrad {
   void operator()(const Tensor& dw1, const Tensor& dw2, const Tensor& dw3, bool accumulate) const {
     const pk_stream_t st = stream_of(d_out);
     if (ldt > 0)
-      PK_CALL(pk_grouped_swiglu_wgrad_scaled_t, ptr(d_out), hsT, d_gT, d_uT, ldt, x_rows, perm, s.K, starts, order, ptr(dw1), ptr(dw2),
-              ptr(dw3), accumulate, s.A, s.H, s.I, s.E, s.dtype, st);
+      through_aligned(dw1, dw2, dw3, accumulate, [&](const Tensor& d1, const Tensor& d2, const Tensor& d3) {
+        PK_CALL(pk_grouped_swiglu_wgrad_scaled_t, ptr(d_out), hsT, d_gT, d_uT, ldt, x_rows, perm, s.K, starts, order, ptr(d1), ptr(d2),
+                ptr(d3), accumulate, s.A, s.H, s.I, s.E, s.dtype, st);
+      });
     else
       PK_CALL(pk_grouped_swiglu_wgrad_scaled, ptr(d_out), hs, d_g, d_u, x_rows, perm, s.K, starts, order, ptr(dw1), ptr(dw2), ptr(dw3),
               accumulate, s.A, s.H, s.I, s.E, s.dtype, st);
@@ -464,11 +479,10 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
     const bool present[N_TENSORS] = {true, true, bias.defined(), true, true, true, ctx->saved_data["residual"].toBool(), norm};
     for (int i = 0, edge = 0; i < N_TENSORS; ++i) need[i] = present[i] && ctx->needs_input_grad(edge++);
     const bool need_xn = need[X] || (norm && need[NORM_W]);      // the gradient of what the router and the experts read
-    const Tensor d_out = contig(grads[0]);
-    const Tensor xc = contig(x), w1 = contig(saved[3]), w2 = contig(saved[4]), w3 = contig(saved[5]);
+    Tensor d_out = contig(grads[0]), xc = contig(x);
+    const Tensor w1 = contig(saved[3]), w2 = contig(saved[4]), w3 = contig(saved[5]);
     Tensor w_gate = contig(saved[1]);
     if (!aligned16(w_gate)) w_gate = w_gate.clone();
-    const void* x_rows = norm ? r.at_(sv.xn) : xc.data_ptr();
     const int32_t *perm = r.i32(sv.perm), *starts = r.i32(sv.starts);
     // what the gradients are put into where this node does it itself (undefined: not a leaf)
     const variable_list params = parameters_of(ctx);
@@ -491,7 +505,13 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
     // token: the order of the sums behind the score's gradient stays, see pk_tile::launch_ragged_m.)
     const int64_t dh_units = (s.A / 128 + std::min(s.A, s.E) / 2) * ((s.I + 255) / 256);
     const bool few_rows = s.K > 1 && s.A <= (dh_units > 256 ? 32 : 40) * s.E;
-    const int64_t ldt = !few_rows && pk_region_transposed_pays(s.A, s.H, s.I, s.E, s.dtype) ? pk_grouped_swiglu_transposed_ld(s.A, s.H, s.I, s.E, s.dtype) : 0;
+    const int64_t ldt = !few_rows && aligned16_all({&w1, &w2, &w3}) && pk_region_transposed_pays(s.A, s.H, s.I, s.E, s.dtype)
+                            ? pk_grouped_swiglu_transposed_ld(s.A, s.H, s.I, s.E, s.dtype) : 0;
+    if (ldt > 0) {                         // its kernels take 16-byte aligned tensors only, and a view may start anywhere
+      if (!aligned16(xc)) xc = xc.clone();
+      if (!aligned16(d_out)) d_out = d_out.clone();
+    }
+    const void* x_rows = norm ? r.at_(sv.xn) : xc.data_ptr();
     const bool blocks_only = ldt > 0 && pk_grouped_swiglu_dx_from_transposed_pays(s.A, s.H, s.I, s.E, s.dtype);
     // w: what the weight gradients read, t: the rest
     Block w, t;
@@ -601,7 +621,7 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
     if (overlap) {
       const auto side = side_stream(x.get_device());
       wait_stream(cur, side);
-      for (const Tensor* b : {&d_out, &xc, &r.memory(), &w.memory()}) b->record_stream(as_cuda(side));
+      for (const Tensor* b : std::initializer_list<const Tensor*>{&d_out, &xc, &r.memory(), &w.memory()}) b->record_stream(as_cuda(side));
       for (const Tensor* b : {&d_w1, &d_w2, &d_w3}) b->record_stream(as_cuda(cur));
     }
     return {d_x, d_wg, d_b, d_w1, d_w2, d_w3, d_res, d_norm_w, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
@@ -1090,14 +1110,10 @@ struct Fp8ExpertsFn : public torch::autograd::Function<Fp8ExpertsFn> {
       char* const ds = static_cast<char*>(dguh.data_ptr());
       const int32_t* const at = starts.data_ptr<int32_t>();
       if (ldt > 0) {
-        at::NoGradGuard no_grad;
-        const Tensor* const to[3] = {&d1, &d2, &d3};      // (a gradient that is added to may be such a view as well)
-        Tensor in[3];
-        for (int i = 0; i < 3; ++i) in[i] = aligned16(*to[i]) ? *to[i] : accumulate ? to[i]->clone() : at::empty_like(*to[i]);
-        PK_CALL(pk_grouped_swiglu_wgrad_scaled_t, ptr(d_y), ds + 2 * copy, ds, ds + copy, ldt, ptr(x), map.data_ptr<int32_t>(), 1, at, nullptr, ptr(in[0]),
-                ptr(in[1]), ptr(in[2]), accumulate, A, H, I, E, PK_BF16, stream_of(x));
-        for (int i = 0; i < 3; ++i)
-          if (!in[i].is_same(*to[i])) to[i]->copy_(in[i]);
+        through_aligned(d1, d2, d3, accumulate, [&](const Tensor& to1, const Tensor& to2, const Tensor& to3) {
+          PK_CALL(pk_grouped_swiglu_wgrad_scaled_t, ptr(d_y), ds + 2 * copy, ds, ds + copy, ldt, ptr(x), map.data_ptr<int32_t>(), 1, at, nullptr, ptr(to1),
+                  ptr(to2), ptr(to3), accumulate, A, H, I, E, PK_BF16, stream_of(x));
+        });
       } else {
         PK_CALL(pk_grouped_swiglu_wgrad, ptr(d_y), ds + 2 * copy, ds, ds + copy, ptr(x), nullptr, 1, at, nullptr, ptr(d1), ptr(d2), ptr(d3), accumulate,
                 A, H, I, E, PK_BF16, stream_of(x));
