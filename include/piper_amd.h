@@ -611,6 +611,39 @@ PK_API int pk_adamw8_fused_packed(float* master, uint8_t* exp_avg, uint8_t* exp_
                            int shadow_dtype, double lr, double beta1, double beta2, double eps, double weight_decay,
                            int64_t step, uint32_t seed, float grad_scale, int zero_grad, pk_stream_t stream);
 
+/* --------------------------------------------- orthogonalization, the step built on it
+ * Newton-Schulz products: X = U / max(|U|, eps) (Frobenius norm), `steps` times (0 to 100)
+ *   A = X X^T,  X <- a X + (b A + c A A) X
+ * on the transposed matrix where it has more rows than columns.  Sides of at most PK_MAX_MATRIX_SIDE.
+ * `precise`: results as exact as products in fp32 (three products of fp16 halves); otherwise single fp16
+ * products, 2e-3 or less off, for results in bf16.  Sums are fp32 either way.  A matrix with a value that is
+ * not finite becomes NaN, and no other one does; a matrix of zeros stays.  No counterpart in the reference.
+ *
+ * Bytes of workspace (HOST arrays; n stacks of counts[i] matrices) that a call runs best with: it goes through
+ * its matrices in groups of what the workspace holds, which has to be the largest matrix at least
+ * (PK_ERR_WORKSPACE), and this is as much as stays in the memory-side cache. */
+#define PK_MAX_MATRIX_SIDE 32768
+PK_API int64_t pk_orthogonalize_workspace_bytes(const int64_t* counts, const int64_t* rows, const int64_t* cols,
+                                         int64_t n, int precise);
+/* out [count, rows, cols] = the result for each matrix of x, in x's dtype (f32: precise). */
+PK_API int pk_orthogonalize(const void* x, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps,
+                     float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes,
+                     pk_stream_t stream);
+/* One optimizer step of n stacks of matrices (HOST arrays of device pointers and sizes):
+ *   g = flat_grads[i] + grads[i] (each may be NULL, the arrays too)    m <- m + (1 - momentum)(g - m)
+ *   U = g + momentum (m - g) with nesterov, m without
+ *   w <- w (1 - lr weight_decay) - lr s X(U)
+ * s: PK_MUON_ASPECT sqrt(max(1, rows / cols)), PK_MUON_RMS 0.2 sqrt(max(rows, cols)).  masters (w) and
+ * momenta (m) are f32, grads grad_dtype, flat_grads f32 (cleared with zero_flat), shadows[i] (may be NULL) the
+ * bf16 copy of w.  Buffers must not overlap. */
+#define PK_MUON_ASPECT 0
+#define PK_MUON_RMS 1
+PK_API int pk_muon_fused(float* const* masters, float* const* momenta, const void* const* grads,
+                  float* const* flat_grads, void* const* shadows, const int64_t* counts, const int64_t* rows,
+                  const int64_t* cols, int64_t n, int grad_dtype, double lr, double momentum, double weight_decay,
+                  int nesterov, int adjust, int zero_flat, int precise, int steps, float a, float b, float c,
+                  float eps, void* workspace, int64_t workspace_bytes, pk_stream_t stream);
+
 /* ------------------------------------------------------------- kernel timing
  * Measurement aid with no counterpart in the reference: when enabled, every kernel launch of
  * the library is bracketed by two hipEventRecord calls on its stream.  pk_timing_collect

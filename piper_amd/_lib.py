@@ -124,6 +124,11 @@ SIGNATURES = {
     "pk_adamw8_fused": (_c_int, [*[_p] * 7, _c_int, _c_i64, *[C.c_double] * 5, _c_i64, C.c_uint32, _c_f32, _c_int, _p]),
     # master m m_scale v v_scale flat_grad grads offsets numels n grad_dtype shadow shadow_dtype lr ... stream
     "pk_adamw8_fused_packed": (_c_int, [*[_p] * 9, _c_i64, _c_int, _p, _c_int, *[C.c_double] * 5, _c_i64, C.c_uint32, _c_f32, _c_int, _p]),
+    "pk_orthogonalize_workspace_bytes": (_c_i64, [_p, _p, _p, _c_i64, _c_int]),
+    # x dtype out count rows cols steps a b c eps ws ws_bytes stream
+    "pk_orthogonalize": (_c_int, [_p, _c_int, _p, *[_c_i64] * 3, _c_int, *[_c_f32] * 4, _p, _c_i64, _p]),
+    # masters momenta grads flat_grads shadows counts rows cols n dtype lr mu decay nesterov adjust zero precise steps a b c eps ws ws_bytes stream
+    "pk_muon_fused": (_c_int, [*[_p] * 8, _c_i64, _c_int, *[C.c_double] * 3, *[_c_int] * 5, *[_c_f32] * 4, _p, _c_i64, _p]),
     "pk_timing_enable": (_c_int, [_c_int]),
     "pk_timing_collect": (_c_i64, [_p, _p, _c_i64]),
     "pk_timing_select": (_c_int, [_c_int]),

@@ -1329,6 +1329,84 @@ void adamw8_packed(const Tensor& master, const std::array<Tensor, 4>& moments, c
           eps, weight_decay, step, seed, (float)grad_scale, zero_grad, stream_of(master));
 }
 
+// ------------------------------------------------------------------------------ orthogonalization and the step built on it
+// The matrices of a tensor [.., rows, cols]: (count, rows, cols)
+std::array<int64_t, 3> matrices_of(const Tensor& t, const char* what) {
+  TORCH_CHECK_VALUE(t.dim() >= 2, what, ": matrices, or stacks of them [.., rows, cols], got a tensor of ", t.dim(), " dimensions");
+  const int64_t r = t.size(-2), c = t.size(-1);
+  return {r * c > 0 ? t.numel() / (r * c) : 0, r, c};
+}
+Tensor orthogonalize(const Tensor& x_, int64_t steps, std::array<double, 3> k, double eps) {
+  require_gpu(x_);
+  refuse_transforms({&x_}, "orthogonalize");
+  const auto m = matrices_of(x_, "orthogonalize");
+  const int code = dtype_code(x_);
+  TORCH_CHECK_VALUE(steps >= 0 && steps <= 100 && eps > 0, "orthogonalize: 0 to 100 steps and a positive eps");
+  at::NoGradGuard no_grad;
+  c10::hip::HIPGuard device(x_.device().index());
+  const Tensor x = contig(x_);
+  Tensor out = at::empty(x.sizes(), x.options());
+  const int64_t bytes = pk_orthogonalize_workspace_bytes(&m[0], &m[1], &m[2], 1, code == PK_F32);
+  TORCH_CHECK_VALUE(bytes >= 0, "orthogonalize: matrices of at most ", PK_MAX_MATRIX_SIDE, " rows and columns");
+  const Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  PK_CALL(pk_orthogonalize, ptr(x), code, ptr(out), m[0], m[1], m[2], (int)steps, (float)k[0], (float)k[1], (float)k[2], (float)eps, ptr(ws), bytes,
+          stream_of(x));
+  return out;
+}
+
+void muon(const std::vector<Tensor>& masters, const std::vector<Tensor>& momenta, const std::vector<OptTensor>& grads,
+          const std::vector<OptTensor>& flats, const std::vector<OptTensor>& shadows, double lr, double momentum, double weight_decay, bool nesterov,
+          const std::string& adjust, bool zero_flat, bool precise, int64_t steps, std::array<double, 3> k, double eps) {
+  const size_t n = masters.size();
+  TORCH_CHECK_VALUE(momenta.size() == n && grads.size() == n && flats.size() == n && shadows.size() == n, "muon_fused: one momentum, gradient and copy per tensor");
+  TORCH_CHECK_VALUE(adjust == "original" || adjust == "match_rms_adamw", "muon_fused: adjust_lr is 'original' or 'match_rms_adamw', not '", adjust, "'");
+  TORCH_CHECK_VALUE(steps >= 0 && steps <= 100 && eps > 0, "muon_fused: 0 to 100 steps and a positive eps");
+  TORCH_CHECK_VALUE(lr >= 0 && momentum >= 0 && momentum < 1 && weight_decay >= 0, "muon_fused: invalid hyper-parameters");
+  if (n == 0) return;
+  require_gpu(masters[0]);
+  c10::hip::HIPGuard device(masters[0].device().index());
+  std::vector<float*> w(n), m(n), flat(n);
+  std::vector<const void*> g(n);
+  std::vector<void*> copy(n);
+  std::vector<int64_t> size[3];
+  std::vector<Tensor> keep;
+  std::optional<at::ScalarType> dtype;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor flat_i = opt(flats[i]), copy_i = opt(shadows[i]), grad_i = opt(grads[i]);
+    const auto of = matrices_of(masters[i], "muon_fused");
+    for (int d = 0; d < 3; ++d) size[d].push_back(of[d]);
+    const int64_t total = masters[i].numel();
+    const auto buffer = [&](const Tensor& t, at::ScalarType type, const char* what) {
+      TORCH_CHECK_VALUE(t.scalar_type() == type && t.numel() == total && t.is_contiguous(), "muon_fused: ", what, ": a contiguous ", type, " tensor of ",
+                        total, " elements");
+    };
+    buffer(masters[i], at::kFloat, "weights");
+    buffer(momenta[i], at::kFloat, "momentum");
+    if (flat_i.defined()) buffer(flat_i, at::kFloat, "flat gradient");
+    if (copy_i.defined()) buffer(copy_i, at::kBFloat16, "shadow");
+    refuse_transforms({&masters[i], &momenta[i], &flat_i, &copy_i, &grad_i}, "muon_fused");
+    same_device(masters[0], {&masters[i], &momenta[i], &flat_i, &copy_i, &grad_i});
+    if (grad_i.defined()) {
+      TORCH_CHECK_VALUE(grad_i.numel() == total, "muon_fused: gradient size differs from the tensor's");
+      TORCH_CHECK_VALUE(!dtype || *dtype == grad_i.scalar_type(), "muon_fused: gradients of one call must share a dtype");
+      dtype = grad_i.scalar_type();
+      dtype_code(grad_i);
+      keep.push_back(contig(grad_i));
+      g[i] = keep.back().data_ptr();
+    }
+    w[i] = masters[i].data_ptr<float>();
+    m[i] = momenta[i].data_ptr<float>();
+    flat[i] = static_cast<float*>(ptr(flat_i));
+    copy[i] = ptr(copy_i);
+  }
+  const int64_t bytes = pk_orthogonalize_workspace_bytes(size[0].data(), size[1].data(), size[2].data(), (int64_t)n, precise);
+  TORCH_CHECK_VALUE(bytes >= 0, "muon_fused: matrices of at most ", PK_MAX_MATRIX_SIDE, " rows and columns");
+  const Tensor ws = at::empty({bytes}, masters[0].options().dtype(at::kByte));
+  PK_CALL(pk_muon_fused, w.data(), m.data(), g.data(), flat.data(), copy.data(), size[0].data(), size[1].data(), size[2].data(), (int64_t)n,
+          dtype == at::kFloat ? PK_F32 : PK_BF16, lr, momentum, weight_decay, nesterov, adjust == "original" ? PK_MUON_ASPECT : PK_MUON_RMS, zero_flat,
+          precise, (int)steps, (float)k[0], (float)k[1], (float)k[2], (float)eps, ptr(ws), bytes, stream_of(masters[0]));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1350,6 +1428,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     adamw_packed(master, exp_avg, exp_avg_sq, opt(flat_grad), grads, offsets, numels, step, lr, beta1, beta2, eps, weight_decay, opt(shadow),
                  grad_scale, zero_grad);
   });
+  m.def("orthogonalize", &orthogonalize, nogil);
+  m.def("muon", &muon, nogil);
   m.def("quantize_experts", &quantize_experts, nogil);
   m.def("quantize_rows", &quantize_rows, nogil);
   m.def("bmm_experts_fp8", &bmm_experts_fp8, nogil);

@@ -1,0 +1,563 @@
+// Newton-Schulz orthogonalization of matrices, and the optimizer step built on it.
+//
+//   X = U / max(|U|_F, eps);   `steps` times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
+//
+// An odd polynomial of X's singular values, applied again and again, which drives them towards 1 without computing them.  U [r, c]
+// is worked on with the shorter side as rows: X [m, n], m = min(r, c).  The step: m <- m + (1 - mu)(g - m), U = g + mu (m - g)
+// (nesterov; otherwise m), w <- w (1 - lr decay) - lr s X.
+//
+// Numbers.  X lives between the products as two planes of fp16 (hi + lo: 22 bits), scaled by a power of two so that its typical
+// value is near 1; A and B, whose values are at most a few units and whose absolute error is what counts beside a X, as they
+// are.  All sums are fp32.  Results in bf16 come from single products, of the upper planes alone, with a X from both: an error of a
+// product is bounded by the strong directions and turns them a little, while an error of X itself, a full matrix of noise, grows with
+// the weak ones, up to 3.4 times a step.  (256 x 683, relative to 64 bits: gradients with 8 strong directions 4e-4 as
+// here, 0.04 with X in one plane, 0.3 with everything in bf16; random ones 1.7e-3, the rounding to bf16 by itself 1.7e-3.)  Results
+// in fp32 (and the fp32 weights of the step) take three products, hi hi + lo hi + hi lo, of all operands: 2e-6 to 3e-5,
+// what products in fp32 give, at three times the matrix operations of the other and a third of the time of fp32 instructions.
+// So do bf16 ones of matrices with a side of at most 128: errors of a few directions do not average out (7e-3 of 3 x 1100), and
+// these matrices cost next to nothing.
+//
+// Work is laid out for many matrices: a launch runs one product of all matrices of a group, as many as the workspace holds.  Padded
+// to multiples of 128 with zeros there (zeros stay zeros under the products), so that only the first and the last kernel see
+// where a matrix ends.
+#include "pk_common.h"
+#include "lds_tiles.h"
+#include <algorithm>
+#include <cmath>
+
+namespace {
+
+using namespace pk_lds;
+
+typedef _Float16 f16_t;
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kPad = 128;
+constexpr int kMaxEntries = 40;              // shapes of a group: keeps the kernels' arguments below 4 KiB
+constexpr int kChunk = 8192;                 // elements a workgroup of begin_kernel takes
+constexpr int kThreads = 256;
+constexpr int64_t kGroupBytes = 192 << 20;   // workspace that is asked for: what the 256 MiB memory-side cache can hold
+
+// Matrices of one shape that lie one behind the other, as the kernels at both ends see them.
+struct Entry {
+  const void* src;       // what is orthogonalized, or the gradients (may be null: zeros)
+  float* flat;           // step: fp32 gradients to add to them (may be null)
+  float* momentum;       // step only
+  float* master;         // step only
+  void* out;             // the result, or the step's bf16 weights (may be null)
+  int64_t ws;            // bytes from the workspace to the first matrix's buffers
+  int32_t rows, cols, count;
+  int32_t mp, np;        // padded sides, mp the shorter
+  int32_t first_chunk, first_tile;
+  float rate;            // step: lr * s
+};
+struct Ends {
+  Entry e[kMaxEntries];
+  char* ws;
+  int32_t n;
+  float mu, keep, eps;   // keep: 1 - lr decay
+  int32_t nesterov, zero_flat, precise;
+};
+static_assert(sizeof(Ends) <= 4096, "kernel arguments");
+struct Gemm {
+  struct { int64_t ws, stride; int32_t mp, np, first_unit; } e[kMaxEntries];
+  char* ws;
+  int32_t n;
+  int32_t from;          // which of the two X the products read
+  float a, b, c;
+};
+
+// X is held times 2^12 and A times 2^8: elements of large normalised matrices are small, as A's off the diagonal are, and
+// the lower plane of a small one would be below fp16's range.  (Singular values up to 16 stay in it; those of the usual coefficients
+// stay below 1.3.)
+constexpr int kXLog2 = 12, kALog2 = 8;
+constexpr float kX = 1 << kXLog2, kA = 1 << kALog2;
+
+// Buffers of one matrix: X twice, each as hi and lo; A, B (with precise sums hi and lo); partial sums of squares.
+__host__ __device__ inline int64_t plane_x(int mp, int np) { return (int64_t)mp * np * 2; }
+__host__ __device__ inline int64_t plane_a(int mp) { return (int64_t)mp * mp * 2; }
+__host__ __device__ inline int64_t at_a(int mp, int np) { return 4 * plane_x(mp, np); }
+__host__ __device__ inline int64_t at_b(int mp, int np, bool precise) { return at_a(mp, np) + (precise ? 2 : 1) * plane_a(mp); }
+__host__ __device__ inline int64_t at_sums(int mp, int np, bool precise) { return at_a(mp, np) + (precise ? 4 : 2) * plane_a(mp); }
+__host__ __device__ inline int64_t matrix_bytes(int rows, int cols, int mp, int np, bool precise) {
+  const int64_t chunks = ((int64_t)rows * cols + kChunk - 1) / kChunk;
+  return (at_sums(mp, np, precise) + chunks * 8 + 255) / 256 * 256;
+}
+template <typename F>
+__device__ __forceinline__ int entry_of(int n, int block, F&& first) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first(mid) <= block) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// ---------------------------------------------------------------- the ends
+// The gradient of element i of an entry; the momentum after this step and U, from the momentum before.
+template <typename TG>
+__device__ __forceinline__ float gradient(const Entry& e, int64_t i) {
+  float g = e.flat ? e.flat[i] : 0.f;
+  if (e.src) g += pk_to_float<TG>(reinterpret_cast<const TG*>(e.src)[i]);
+  return g;
+}
+__device__ __forceinline__ float next_momentum(float m, float g, float mu) { return m + (1.f - mu) * (g - m); }
+__device__ __forceinline__ float update_of(float m, float g, float mu, bool nesterov) { return nesterov ? g + mu * (m - g) : m; }
+
+// Momentum, and the sum of squares of every chunk of a matrix of U, in 64 bits (squares of fp32 values reach past fp32's range).
+template <typename TG, bool STEP>
+__global__ __launch_bounds__(kThreads) void begin_kernel(const Ends p) {
+  __shared__ double part[kThreads / 64];
+  const int en = entry_of(p.n, blockIdx.x, [&](int i) { return p.e[i].first_chunk; });
+  const Entry& e = p.e[en];
+  const int64_t size = (int64_t)e.rows * e.cols;
+  const int chunks = (int)((size + kChunk - 1) / kChunk);
+  const int local = blockIdx.x - e.first_chunk, mat = local / chunks, chunk = local % chunks;
+  const int64_t base = (int64_t)mat * size + (int64_t)chunk * kChunk;
+  const int n = (int)min((int64_t)kChunk, size - (int64_t)chunk * kChunk);
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const float g = gradient<TG>(e, base + i);
+    float u = g;
+    if (STEP) {
+      const float m = next_momentum(e.momentum[base + i], g, p.mu);
+      e.momentum[base + i] = m;
+      u = update_of(m, g, p.mu, p.nesterov);
+    }
+    sum += (double)u * u;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int w = 0; w < kThreads / 64; ++w) s += part[w];
+    char* const mem = p.ws + e.ws + mat * matrix_bytes(e.rows, e.cols, e.mp, e.np, p.precise);
+    reinterpret_cast<double*>(mem + at_sums(e.mp, e.np, p.precise))[chunk] = s;
+  }
+}
+
+struct Tile {            // 64 x 64 of a matrix's padded X
+  const Entry& e;
+  int mat, i0, j0;
+  bool tall;
+  char* mem;
+};
+__device__ __forceinline__ Tile tile_of(const Ends& p, int block) {
+  const Entry& e = p.e[entry_of(p.n, block, [&](int i) { return p.e[i].first_tile; })];
+  const int tm = e.mp / 64, tn = e.np / 64, local = block - e.first_tile;
+  const int mat = local / (tm * tn), t = local % (tm * tn);
+  return Tile{e, mat, t / tn * 64, t % tn * 64, e.rows > e.cols, p.ws + e.ws + mat * matrix_bytes(e.rows, e.cols, e.mp, e.np, p.precise)};
+}
+
+// X = U / max(|U|, eps) in two planes, its longer side along the rows in memory, zeros around it.
+template <typename TG, bool STEP>
+__global__ __launch_bounds__(kThreads) void convert_kernel(const Ends p) {
+  __shared__ double part[kThreads / 64];
+  __shared__ float turned[64][65];
+  const Tile t = tile_of(p, blockIdx.x);
+  const Entry& e = t.e;
+  const int tid = threadIdx.x;
+  const int64_t size = (int64_t)e.rows * e.cols;
+  const int chunks = (int)((size + kChunk - 1) / kChunk);
+  const double* sums = reinterpret_cast<const double*>(t.mem + at_sums(e.mp, e.np, p.precise));
+  double sum = 0.0;
+  for (int i = tid; i < chunks; i += kThreads) sum += sums[i];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if ((tid & 63) == 0) part[tid >> 6] = sum;
+  __syncthreads();
+  const double norm = sqrt(part[0] + part[1] + part[2] + part[3]);
+  const double factor = (double)kX / (norm < (double)p.eps ? (double)p.eps : norm);   // (NaN stays)
+  const int64_t base = (int64_t)t.mat * size;
+  f16_t* const hi = reinterpret_cast<f16_t*>(t.mem);
+  f16_t* const lo = reinterpret_cast<f16_t*>(t.mem + plane_x(e.mp, e.np));
+  const int r0 = t.tall ? t.j0 : t.i0, c0 = t.tall ? t.i0 : t.j0;
+  for (int q = tid; q < 64 * 64; q += kThreads) {
+    const int r = r0 + (q >> 6), c = c0 + (q & 63);
+    float x = 0.f;
+    if (r < e.rows && c < e.cols) {
+      const int64_t i = base + (int64_t)r * e.cols + c;
+      const float g = gradient<TG>(e, i);
+      const float u = STEP ? update_of(e.momentum[i], g, p.mu, p.nesterov) : g;
+      if (STEP && p.zero_flat && e.flat) e.flat[i] = 0.f;
+      x = (float)((double)u * factor);
+    }
+    turned[q >> 6][q & 63] = x;
+  }
+  __syncthreads();
+  for (int q = tid; q < 64 * 16; q += kThreads) {
+    const int i = q >> 4, j = (q & 15) * 4;
+    f16x4_t h, l;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float x = t.tall ? turned[j + v][i] : turned[i][j + v];
+      h[v] = (f16_t)x;
+      l[v] = (f16_t)(x - (float)h[v]);
+    }
+    const int64_t at = (int64_t)(t.i0 + i) * e.np + t.j0 + j;
+    *reinterpret_cast<f16x4_t*>(hi + at) = h;
+    *reinterpret_cast<f16x4_t*>(lo + at) = l;
+  }
+}
+
+// The result (TG), or with STEP the weights and their bf16 copy.
+template <typename TG, bool STEP>
+__global__ __launch_bounds__(kThreads) void finish_kernel(const Ends p, int from) {
+  __shared__ float turned[64][65];
+  const Tile t = tile_of(p, blockIdx.x);
+  const Entry& e = t.e;
+  const int tid = threadIdx.x;
+  const int64_t size = (int64_t)e.rows * e.cols;
+  const f16_t* const hi = reinterpret_cast<const f16_t*>(t.mem + 2 * from * plane_x(e.mp, e.np));
+  const f16_t* const lo = hi + (int64_t)e.mp * e.np;
+  for (int q = tid; q < 64 * 16; q += kThreads) {
+    const int i = q >> 4, j = (q & 15) * 4;
+    const int64_t at = (int64_t)(t.i0 + i) * e.np + t.j0 + j;
+    const f16x4_t h = *reinterpret_cast<const f16x4_t*>(hi + at), l = *reinterpret_cast<const f16x4_t*>(lo + at);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) (t.tall ? turned[j + v][i] : turned[i][j + v]) = ((float)h[v] + (float)l[v]) * (1.f / kX);
+  }
+  __syncthreads();
+  const int r0 = t.tall ? t.j0 : t.i0, c0 = t.tall ? t.i0 : t.j0;
+  const int64_t base = (int64_t)t.mat * size;
+  for (int q = tid; q < 64 * 64; q += kThreads) {
+    const int r = r0 + (q >> 6), c = c0 + (q & 63);
+    if (r >= e.rows || c >= e.cols) continue;
+    const int64_t i = base + (int64_t)r * e.cols + c;
+    const float o = turned[q >> 6][q & 63];
+    if (STEP) {
+      const float w = e.master[i] * p.keep - e.rate * o;
+      e.master[i] = w;
+      if (e.out) reinterpret_cast<bf16_t*>(e.out)[i] = (bf16_t)w;
+    } else {
+      reinterpret_cast<TG*>(e.out)[i] = pk_from_float<TG>(o);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the products
+enum Product { GRAM, POLY, UPDATE };
+
+// 128 x 128 outputs of one product of one matrix, 64-deep k-tiles, two in LDS; four waves of 64 x 64.
+//   GRAM    A = X X^T              rows of X against rows of X
+//   POLY    B = b A + c A A        A is symmetric: its rows against its rows
+//   UPDATE  X' = a X + B X         X comes as [k][columns] and through the transposing LDS read
+// GRAM and POLY are symmetric: the tiles on and below the diagonal are computed and stored twice.
+// PRECISE: three products, hi hi + lo hi + hi lo, one behind the other along k.  The matrix instructions cut what they add to a sum
+// off at its last bit instead of rounding it, which makes long sums of one sign too small (diagonals of 1,100 products by 8e-7, and
+// the result by ten times that): every 128 products the accumulators go into a second set by ordinary additions.
+template <int KIND, bool PRECISE>
+__global__ __launch_bounds__(256) void product_kernel(const Gemm p) {
+  constexpr int BM = 128, BK = 64, TILE = BM * BK * 2, STAGE = 2 * TILE, L = 4;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const int en = entry_of(p.n, blockIdx.x, [&](int i) { return p.e[i].first_unit; });
+  const int mp = p.e[en].mp, np = p.e[en].np, tm = mp / BM, tn = np / BM;
+  const int per = KIND == UPDATE ? tm * tn : tm * (tm + 1) / 2;
+  const int local = blockIdx.x - p.e[en].first_unit, mat = local / per;
+  int mt, nt;
+  if (KIND == UPDATE) {
+    mt = (local % per) / tn;
+    nt = (local % per) % tn;
+  } else {
+    const int t = local % per;
+    mt = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while ((mt + 1) * (mt + 2) / 2 <= t) ++mt;
+    while (mt * (mt + 1) / 2 > t) --mt;
+    nt = t - mt * (mt + 1) / 2;
+  }
+  char* const mem = p.ws + p.e[en].ws + (int64_t)mat * p.e[en].stride;
+  const int64_t px = plane_x(mp, np), pa = plane_a(mp);
+  char* const X = mem + 2 * p.from * px;
+  char* const Xn = mem + 2 * (1 - p.from) * px;
+  char* const A = mem + at_a(mp, np);
+  char* const B = mem + at_b(mp, np, PRECISE);
+
+  const char* const left = KIND == GRAM ? X : KIND == POLY ? A : B;
+  const char* const right = KIND == POLY ? A : X;
+  const int64_t left_plane = KIND == GRAM ? px : pa, right_plane = KIND == POLY ? pa : px;
+  const int lda = KIND == GRAM ? np : mp, ldb = KIND == POLY ? mp : np;
+  const int nkt = (KIND == GRAM ? np : mp) / BK, total = PRECISE ? 3 * nkt : nkt;
+
+  uint32_t va[L], vb[L];
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    int r, k;
+    kc_slot<BK>(wave * L + i, lane, r, k);
+    va[i] = (uint32_t)(r * lda + k) * 2u;
+    if (KIND == UPDATE) mn_slot<BM>(wave * L + i, lane, r, k);
+    vb[i] = (uint32_t)(r * ldb + k) * 2u;
+  }
+  auto request = [&](int kt) {
+    const int seg = PRECISE ? kt / nkt : 0, k = PRECISE ? kt % nkt : kt;
+    const char* a = uniform_ptr(left + (seg == 1 ? left_plane : 0) + ((int64_t)mt * BM * lda + (int64_t)k * BK) * 2);
+    const char* b = uniform_ptr(right + (seg == 2 ? right_plane : 0) +
+                                (KIND == UPDATE ? (int64_t)k * BK * ldb + (int64_t)nt * BM : (int64_t)nt * BM * ldb + (int64_t)k * BK) * 2);
+    const uint32_t to = lds_addr(smem) + (kt & 1) * STAGE + wave * (L * 1024);
+    static_for<L>([&](auto i) { dma16_s<decltype(i)::value * 1024>(va[i], a, to); });
+    static_for<L>([&](auto i) { dma16_s<TILE + decltype(i)::value * 1024>(vb[i], b, to); });
+  };
+  floatx16_t acc[2][2] = {}, sum[2][2] = {};
+  request(0);
+  for (int kt = 0; kt < total; ++kt) {
+    if (kt + 1 < total) {
+      request(kt + 1);
+      wait_dma<2 * L>();
+    } else {
+      wait_dma<0>();
+    }
+    block_barrier();
+    const char* const st = smem + (kt & 1) * STAGE;
+#pragma unroll
+    for (int ks = 0; ks < BK / 16; ++ks) {
+      f16x8_t fa[2], fb[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fa[i] = frag_kc<BK, f16x8_t>(st, wm * 64 + 32 * i, ks, lane);
+        fb[i] = KIND == UPDATE ? frag_mn<BM, f16x8_t>(st + TILE, wn * 64 + 32 * i, ks, lane) : frag_kc<BK, f16x8_t>(st + TILE, wn * 64 + 32 * i, ks, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    block_barrier();
+    if (PRECISE && (kt & 1)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          sum[i][j] += acc[i][j];
+          acc[i][j] = floatx16_t{};
+        }
+    }
+  }
+  if (PRECISE) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] += sum[i][j];
+  }
+  // acc[i][j][v] is row 32 i + lane % 32, column 32 j + 8 (v / 4) + 4 (lane / 32) + v % 4 of the wave's 64 x 64
+  const int ldc = KIND == UPDATE ? np : mp;
+  const int64_t plane_c = KIND == UPDATE ? px : pa;
+  char* const out = KIND == GRAM ? A : KIND == POLY ? B : Xn;
+  const char* const old = KIND == POLY ? A : X;        // what a or b multiplies
+  constexpr float unscale = KIND == GRAM ? kA / (kX * kX) : KIND == POLY ? 1.f / (kA * kA) : 1.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int row = mt * BM + wm * 64 + 32 * i + (lane & 31), col = nt * BM + wn * 64 + 32 * j + 8 * q + 4 * (lane >> 5);
+        const int64_t at = (int64_t)row * ldc + col;
+        float x[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) x[v] = acc[i][j][4 * q + v] * unscale;
+        if (KIND != GRAM) {
+          const f16x4_t h = *reinterpret_cast<const f16x4_t*>(old + at * 2);
+          f16x4_t l = {};
+          if (KIND == UPDATE || PRECISE) l = *reinterpret_cast<const f16x4_t*>(old + plane_c + at * 2);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float o = (float)h[v] + (float)l[v];
+            x[v] = KIND == POLY ? p.b * (o * (1.f / kA)) + p.c * x[v] : p.a * o + x[v];
+          }
+        }
+        f16x4_t h, l;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          h[v] = (f16_t)x[v];
+          l[v] = (f16_t)(x[v] - (float)h[v]);
+        }
+        *reinterpret_cast<f16x4_t*>(out + at * 2) = h;
+        if (KIND == UPDATE || PRECISE) *reinterpret_cast<f16x4_t*>(out + plane_c + at * 2) = l;
+        if (KIND != UPDATE && mt != nt) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int64_t mirror = (int64_t)(col + v) * ldc + row;
+            reinterpret_cast<f16_t*>(out)[mirror] = h[v];
+            if (PRECISE) reinterpret_cast<f16_t*>(out + plane_c)[mirror] = l[v];
+          }
+        }
+      }
+}
+
+// ---------------------------------------------------------------- host
+struct Item {
+  const void* src;
+  float *flat, *momentum, *master;
+  void* out;
+  int64_t count, rows, cols;
+  float rate;
+  bool precise;
+};
+struct Settings {
+  bool step, bf16_src;
+  float mu, keep, eps;
+  bool nesterov, zero_flat;
+  int steps;
+  float a, b, c;
+};
+int padded(int64_t n) { return (int)(pk_ceil_div(n, kPad) * kPad); }
+int64_t bytes_of(int64_t rows, int64_t cols, bool precise) {
+  return matrix_bytes((int)rows, (int)cols, padded(std::min(rows, cols)), padded(std::max(rows, cols)), precise);
+}
+bool sides_ok(int64_t rows, int64_t cols) { return rows <= PK_MAX_MATRIX_SIDE && cols <= PK_MAX_MATRIX_SIDE; }
+
+template <int KIND>
+void launch_product(const Gemm& g, int units, bool precise, int id, hipStream_t s) {
+  if (precise) PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, true>), dim3(units), dim3(256), 0, s, g);
+  else PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, false>), dim3(units), dim3(256), 0, s, g);
+}
+template <typename TG, bool STEP>
+int run_group(Ends& e, Gemm& sym, Gemm& upd, int chunks, int tiles, int sym_units, int upd_units, const Settings& o, hipStream_t s) {
+  const bool precise = e.precise != 0;
+  PK_LAUNCH_NOCHECK(pk_timing::K_MUON_BEGIN, s, (begin_kernel<TG, STEP>), dim3(chunks), dim3(kThreads), 0, s, e);
+  PK_LAUNCH_NOCHECK(pk_timing::K_MUON_CONVERT, s, (convert_kernel<TG, STEP>), dim3(tiles), dim3(kThreads), 0, s, e);
+  int from = 0;
+  for (int i = 0; i < o.steps; ++i) {
+    sym.from = upd.from = from;
+    launch_product<GRAM>(sym, sym_units, precise, pk_timing::K_NS_GRAM, s);
+    launch_product<POLY>(sym, sym_units, precise, pk_timing::K_NS_POLY, s);
+    launch_product<UPDATE>(upd, upd_units, precise, pk_timing::K_NS_UPDATE, s);
+    from = 1 - from;
+  }
+  PK_LAUNCH_NOCHECK(pk_timing::K_MUON_FINISH, s, (finish_kernel<TG, STEP>), dim3(tiles), dim3(kThreads), 0, s, e, from);
+  PK_RETURN_IF_LAUNCH_FAILED();
+  return PK_OK;
+}
+
+// Whether all operands take part with both planes.
+bool precise_result(bool asked, int64_t rows, int64_t cols) { return asked || std::min(rows, cols) <= kPad; }
+
+// All matrices of the items 0 .. n - 1 (item(i); one without matrices has count 0), in groups of what the workspace holds.
+template <typename F>
+int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspace_bytes, hipStream_t s) {
+  bool some = false;
+  for (int64_t i = 0; i < n; ++i) {
+    const Item it = item(i);
+    if (it.count == 0) continue;
+    some = true;
+    if (!workspace || !pk_aligned16(workspace) || bytes_of(it.rows, it.cols, it.precise) > workspace_bytes) return PK_ERR_WORKSPACE;
+  }
+  if (!some) return PK_OK;
+  const int64_t es = o.bf16_src ? 2 : 4;
+  int64_t i = 0, done = 0;        // done: matrices of item i
+  while (i < n) {
+    Ends e = {};
+    Gemm sym = {}, upd = {};
+    e.ws = sym.ws = upd.ws = static_cast<char*>(workspace);
+    e.mu = o.mu; e.keep = o.keep; e.eps = o.eps; e.nesterov = o.nesterov; e.zero_flat = o.zero_flat;
+    sym.a = upd.a = o.a; sym.b = upd.b = o.b; sym.c = upd.c = o.c;
+    int64_t used = 0, chunks = 0, tiles = 0, sym_units = 0, upd_units = 0;
+    while (i < n && e.n < kMaxEntries) {
+      const Item it = item(i);
+      if (it.count == 0) { ++i; continue; }
+      if (e.n > 0 && it.precise != (e.precise != 0)) break;        // the kernels of a group are of one kind
+      e.precise = it.precise;
+      const int64_t each = bytes_of(it.rows, it.cols, it.precise), fit = std::min((workspace_bytes - used) / each, it.count - done);
+      if (fit == 0) break;
+      const int mp = padded(std::min(it.rows, it.cols)), np = padded(std::max(it.rows, it.cols));
+      const int64_t at = done * it.rows * it.cols;
+      Entry& x = e.e[e.n];
+      x.src = it.src ? static_cast<const char*>(it.src) + at * es : nullptr;
+      x.flat = it.flat ? it.flat + at : nullptr;
+      x.momentum = it.momentum ? it.momentum + at : nullptr;
+      x.master = it.master ? it.master + at : nullptr;
+      x.out = it.out ? static_cast<char*>(it.out) + at * (o.step ? 2 : es) : nullptr;
+      x.ws = used;
+      x.rows = (int)it.rows; x.cols = (int)it.cols; x.count = (int)fit; x.mp = mp; x.np = np;
+      x.first_chunk = (int)chunks; x.first_tile = (int)tiles;
+      x.rate = it.rate;
+      const int64_t tm = mp / kPad, tn = np / kPad;
+      sym.e[e.n] = {used, each, mp, np, (int32_t)sym_units};
+      upd.e[e.n] = {used, each, mp, np, (int32_t)upd_units};
+      chunks += fit * pk_ceil_div(it.rows * it.cols, kChunk);
+      tiles += fit * (mp / 64) * (np / 64);
+      sym_units += fit * tm * (tm + 1) / 2;
+      upd_units += fit * tm * tn;
+      used += fit * each;
+      ++e.n;
+      done += fit;
+      if (done == it.count) { ++i; done = 0; }
+    }
+    if (e.n == 0) break;
+    sym.n = upd.n = e.n;
+    if (std::max({chunks, tiles, sym_units, upd_units}) > 0x7fffffffll) return PK_ERR_SHAPE;
+    const int rc = o.step ? (o.bf16_src ? run_group<bf16_t, true>(e, sym, upd, (int)chunks, (int)tiles, (int)sym_units, (int)upd_units, o, s)
+                                        : run_group<float, true>(e, sym, upd, (int)chunks, (int)tiles, (int)sym_units, (int)upd_units, o, s))
+                          : (o.bf16_src ? run_group<bf16_t, false>(e, sym, upd, (int)chunks, (int)tiles, (int)sym_units, (int)upd_units, o, s)
+                                        : run_group<float, false>(e, sym, upd, (int)chunks, (int)tiles, (int)sym_units, (int)upd_units, o, s));
+    if (rc != PK_OK) return rc;
+  }
+  return PK_OK;
+}
+
+bool settings_ok(int steps, float eps) { return steps >= 0 && steps <= 100 && eps > 0.f; }
+
+}  // namespace
+
+extern "C" {
+
+int64_t pk_orthogonalize_workspace_bytes(const int64_t* counts, const int64_t* rows, const int64_t* cols, int64_t n, int precise) {
+  if (n < 0 || (n > 0 && (!counts || !rows || !cols))) return PK_ERR_ARG;
+  int64_t all = 0, most = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    if (counts[i] < 0 || rows[i] < 0 || cols[i] < 0) return PK_ERR_ARG;
+    if (!sides_ok(rows[i], cols[i])) return PK_ERR_SHAPE;
+    if (counts[i] == 0 || rows[i] == 0 || cols[i] == 0) continue;
+    const int64_t each = bytes_of(rows[i], cols[i], precise_result(precise != 0, rows[i], cols[i]));
+    most = std::max(most, each);
+    all = std::min(all, kGroupBytes) + std::min(counts[i], kGroupBytes / each + 1) * each;
+  }
+  return std::max(most, std::min(all, kGroupBytes));
+}
+
+int pk_orthogonalize(const void* x, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps, float a, float b, float c,
+                     float eps, void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
+  if (count < 0 || rows < 0 || cols < 0 || !pk_dtype_ok(dtype) || !settings_ok(steps, eps)) return PK_ERR_ARG;
+  if (!sides_ok(rows, cols)) return PK_ERR_SHAPE;
+  if (count == 0 || rows == 0 || cols == 0) return PK_OK;
+  if (!x || !out) return PK_ERR_ARG;
+  Settings o = {};
+  o.bf16_src = dtype == PK_BF16;
+  o.eps = eps; o.steps = steps; o.a = a; o.b = b; o.c = c;
+  const Item only{x, nullptr, nullptr, nullptr, out, count, rows, cols, 0.f, precise_result(dtype == PK_F32, rows, cols)};
+  return run(1, [&](int64_t) { return only; }, o, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int pk_muon_fused(float* const* masters, float* const* momenta, const void* const* grads, float* const* flat_grads, void* const* shadows,
+                  const int64_t* counts, const int64_t* rows, const int64_t* cols, int64_t n, int grad_dtype, double lr, double momentum,
+                  double weight_decay, int nesterov, int adjust, int zero_flat, int precise, int steps, float a, float b, float c, float eps,
+                  void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
+  if (n < 0 || !pk_dtype_ok(grad_dtype) || !settings_ok(steps, eps) || (adjust != PK_MUON_ASPECT && adjust != PK_MUON_RMS)) return PK_ERR_ARG;
+  if (n == 0) return PK_OK;
+  if (!masters || !momenta || !counts || !rows || !cols) return PK_ERR_ARG;
+  for (int64_t i = 0; i < n; ++i) {
+    if (counts[i] < 0 || rows[i] < 0 || cols[i] < 0) return PK_ERR_ARG;
+    if (!sides_ok(rows[i], cols[i])) return PK_ERR_SHAPE;
+    if (counts[i] > 0 && rows[i] > 0 && cols[i] > 0 && (!masters[i] || !momenta[i])) return PK_ERR_ARG;
+  }
+  const auto item = [&](int64_t i) {
+    const double r = (double)rows[i], k = (double)cols[i];
+    const double scale = adjust == PK_MUON_RMS ? 0.2 * std::sqrt(std::max(r, k)) : std::sqrt(std::max(1.0, r / k));
+    return Item{grads ? grads[i] : nullptr, flat_grads ? flat_grads[i] : nullptr, momenta[i], masters[i], shadows ? shadows[i] : nullptr,
+                rows[i] > 0 && cols[i] > 0 ? counts[i] : 0, rows[i], cols[i], (float)(lr * scale), precise_result(precise != 0, rows[i], cols[i])};
+  };
+  Settings o = {};
+  o.step = true; o.bf16_src = grad_dtype == PK_BF16;
+  o.mu = (float)momentum; o.keep = (float)(1.0 - lr * weight_decay); o.eps = eps;
+  o.nesterov = nesterov != 0; o.zero_flat = zero_flat != 0;
+  o.steps = steps; o.a = a; o.b = b; o.c = c;
+  return run(n, item, o, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+}  // extern "C"

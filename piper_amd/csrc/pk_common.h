@@ -37,7 +37,8 @@ enum KernelId {
   K_SWIGLU_GATE_UP, K_SWIGLU_DOWN, K_SWIGLU_DGRAD_DH, K_SWIGLU_DGRAD_DX, K_SWIGLU_WGRAD,
   K_SIMT_GEMM, K_SWIGLU_ELEMENTWISE, K_BUCKET_PACK, K_BUCKET_UNPACK, K_BUCKET_ZERO, K_ADAMW,
   K_RMSNORM_FWD, K_RMSNORM_BWD, K_MISC, K_SWIGLU_WGRAD_W2, K_SWIGLU_WGRAD_W13,
-  K_FP8_QUANTIZE, K_FP8_GATE_UP, K_FP8_DOWN, K_FP8_DGRAD_DH, K_FP8_DGRAD_DX, K_ADAMW8, K_COUNT
+  K_FP8_QUANTIZE, K_FP8_GATE_UP, K_FP8_DOWN, K_FP8_DGRAD_DH, K_FP8_DGRAD_DX, K_ADAMW8,
+  K_MUON_BEGIN, K_MUON_CONVERT, K_NS_GRAM, K_NS_POLY, K_NS_UPDATE, K_MUON_FINISH, K_BALANCE, K_BALANCE_BWD, K_COUNT
 };
 // Brackets one kernel launch with two event records on `s` when timing is enabled
 // (pk_timing_enable); otherwise does nothing.

@@ -29,7 +29,8 @@ const char* const kNames[K_COUNT] = {
     "swiglu_gate_up", "swiglu_down", "swiglu_dgrad_dh", "swiglu_dgrad_dx", "swiglu_wgrad",
     "simt_gemm", "swiglu_elementwise", "bucket_pack", "bucket_unpack", "bucket_zero", "adamw",
     "rmsnorm_fwd", "rmsnorm_bwd", "misc", "swiglu_wgrad_w2", "swiglu_wgrad_w13",
-    "fp8_quantize", "fp8_gate_up", "fp8_down", "fp8_dgrad_dh", "fp8_dgrad_dx", "adamw8"};
+    "fp8_quantize", "fp8_gate_up", "fp8_down", "fp8_dgrad_dh", "fp8_dgrad_dx", "adamw8",
+    "muon_begin", "muon_convert", "ns_gram", "ns_poly", "ns_update", "muon_finish", "balance", "balance_bwd"};
 
 Scope::Scope(int id, hipStream_t s) : stream_(s), slot_(-1) {
   std::lock_guard<std::mutex> lk(g_mu);

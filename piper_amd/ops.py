@@ -530,3 +530,38 @@ def adamw8_fused_packed(master, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_s
     host().adamw8_packed(master, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, flat_grad, list(grads), list(offsets), list(numels),
                          int(step), float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), int(seed) & 0xFFFFFFFF, shadow,
                          float(grad_scale), bool(zero_grad))
+
+
+# ------------------------------------------------------------------------- orthogonalization, the step built on it
+NEWTON_SCHULZ = (3.4445, -4.775, 2.0315)      # a x + b x^3 + c x^5 takes singular values from about 0.01 to 1 to between 0.7 and 1.2 in five steps
+
+
+def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[float] = NEWTON_SCHULZ, eps: float = 1e-7) -> torch.Tensor:
+    """Every matrix of x [.., rows, cols] (bfloat16 or float32) brought near the closest semi-orthogonal one by Newton-Schulz products:
+    X = x / max(|x|, eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (on the transposed matrix where it is taller
+    than wide).  float32 results are as exact as products in float32; bfloat16 ones take products of 11-bit values, which
+    leaves them 0.002 or less off beside their rounding.  A matrix with a value that is not finite becomes NaN, no other one does.
+    No backward."""
+    return host().orthogonalize(x, int(steps), _three(coefficients), float(eps))
+
+
+def muon_fused(masters: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | None], *,
+               flat_grads: Sequence[torch.Tensor | None] | None = None, shadows: Sequence[torch.Tensor | None] | None = None, lr: float,
+               momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True, steps: int = 5,
+               coefficients: Sequence[float] = NEWTON_SCHULZ, eps: float = 1e-7, adjust_lr: str = "original", zero_grad: bool = False,
+               half_products: bool = False) -> None:
+    """One optimizer step of matrices, or stacks of them, masters[i] [.., rows, cols] (float32), each by its orthogonalized momentum:
+    g = flat_grads[i] + grads[i] (either may be None), m <- m + (1 - momentum)(g - m), u = g + momentum (m - g) (m without
+    `nesterov`), w <- w (1 - lr weight_decay) - lr s orthogonalize(u), with s = sqrt(max(1, rows / cols)) or, for
+    adjust_lr="match_rms_adamw", 0.2 sqrt(max(rows, cols)).  shadows[i]: the bfloat16 copy of w to write.  zero_grad clears flat_grads.
+    half_products: the products of bfloat16 results (``orthogonalize``), a third of the matrix operations, for updates 0.002 off."""
+    none = [None] * len(masters)
+    host().muon(list(masters), list(momenta), list(grads), none if flat_grads is None else list(flat_grads), none if shadows is None else list(shadows),
+                float(lr), float(momentum), float(weight_decay), bool(nesterov), str(adjust_lr), bool(zero_grad), not half_products, int(steps),
+                _three(coefficients), float(eps))
+
+
+def _three(coefficients: Sequence[float]) -> list[float]:
+    got = [float(c) for c in coefficients]
+    _check(len(got) == 3, "Newton-Schulz products take three coefficients")
+    return got
