@@ -180,6 +180,38 @@ PK_API int pk_sort_by_expert_static(const int32_t* top_idx, int64_t A, int64_t E
                              int32_t* starts, int32_t* perm, int32_t* inv_perm, int32_t* order,
                              pk_stream_t stream);
 
+/* --------------------------------------------- the router's balance loss
+ * top_idx [T,K] (i32) are the experts that logits [T,E] (f32) chose.  sequences [S+1] (i32, ascending, within 0 .. T; NULL: S = 1,
+ * all tokens): sequence s has the tokens sequences[s] .. sequences[s+1], L of them; tokens outside all of them are padding.
+ *   counts[S,E] (i32): how often each expert was chosen in each sequence (ids outside [0,E) are not counted)
+ *   f_e = counts_e E / (K L), P_e = mean over the sequence's tokens of softmax(logits)_e
+ *   loss[1] (f32) = balance_coeff * mean over the sequences with tokens of sum_e f_e P_e
+ *                 + z_coeff * mean over the sequences' tokens of logsumexp(logits)^2
+ *   table[S*E+2] (f32): what the backward needs beside the logits
+ * Sums are fp32 over up to 64 (more than 32,768 tokens: T / 512) tokens, 64-bit above, in a fixed order. */
+PK_API int64_t pk_balance_workspace_bytes(int64_t T, int64_t E, int64_t S);
+PK_API int pk_balance_loss(const float* logits, const int32_t* top_idx, const int32_t* sequences, int64_t T, int64_t E,
+                    int64_t K, int64_t S, float balance_coeff, float z_coeff, float* loss, int32_t* counts, float* table,
+                    void* workspace, int64_t workspace_bytes, pk_stream_t stream);
+/* d_logits[T,E] (f32, fully written, zeros for padding) = *d_loss (DEVICE f32) times the gradient of loss; the counts
+ * have none. */
+PK_API int pk_balance_loss_bwd(const float* logits, const int32_t* sequences, const float* table, const float* d_loss,
+                        float* d_logits, int64_t T, int64_t E, int64_t S, pk_stream_t stream);
+/* pk_route_topk_bwd with that gradient added. */
+PK_API int pk_route_topk_balanced_bwd(const float* table, const int32_t* sequences, int64_t S, const float* d_loss,
+                               const float* logits, const int32_t* top_idx, const float* d_top_scores, int64_t T,
+                               int64_t E, int64_t K, int route_norm, float route_scale, float* d_logits, pk_stream_t stream);
+/* pk_region_router_norm_bwd (norm_weight NULL: pk_region_router_bwd of xn and d_xn; x, rstd, d_x_addend, d_x, d_norm_weight are not
+ * looked at) with the gradient of the balance loss of these logits added to d_logits on the way.  Workspace as theirs. */
+PK_API int pk_region_router_balanced_bwd(const float* table, const int32_t* sequences, int64_t S, const float* d_loss,
+                                  const float* logits, const int32_t* top_idx, const float* d_top_scores,
+                                  const float* ds_partial, int64_t n_partial, const int32_t* inv_perm, int route_norm,
+                                  float route_scale, const void* xn, int x_dtype, const float* w_gate, const void* d_rows,
+                                  void* d_xn, float* d_w_gate, float* d_gate_bias, int accumulate, float* d_logits,
+                                  const void* x, const void* norm_weight, const float* rstd, const void* d_x_addend, void* d_x,
+                                  void* d_norm_weight, int64_t T, int64_t H, int64_t E, int64_t K, void* workspace,
+                                  int64_t workspace_bytes, pk_stream_t stream);
+
 /* starts[E+1] (i32) from counts[E] given as int32 (counts_is_i64 == 0) or int64.
  * For callers that hand pk_grouped_swiglu_* a `num_tokens_per_expert` tensor
  * (qwen3_bmm_experts_patch.py:24-27). */

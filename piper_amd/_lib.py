@@ -124,6 +124,10 @@ SIGNATURES = {
     "pk_adamw8_fused": (_c_int, [*[_p] * 7, _c_int, _c_i64, *[C.c_double] * 5, _c_i64, C.c_uint32, _c_f32, _c_int, _p]),
     # master m m_scale v v_scale flat_grad grads offsets numels n grad_dtype shadow shadow_dtype lr ... stream
     "pk_adamw8_fused_packed": (_c_int, [*[_p] * 9, _c_i64, _c_int, _p, _c_int, *[C.c_double] * 5, _c_i64, C.c_uint32, _c_f32, _c_int, _p]),
+    "pk_balance_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    # logits idx sequences T E K S balance z loss counts table ws ws_bytes stream
+    "pk_balance_loss": (_c_int, [_p, _p, _p, *[_c_i64] * 4, _c_f32, _c_f32, _p, _p, _p, _p, _c_i64, _p]),
+    "pk_balance_loss_bwd": (_c_int, [*[_p] * 5, *[_c_i64] * 3, _p]),
     "pk_orthogonalize_workspace_bytes": (_c_i64, [_p, _p, _p, _c_i64, _c_int]),
     # x dtype out count rows cols steps a b c eps ws ws_bytes stream
     "pk_orthogonalize": (_c_int, [_p, _c_int, _p, *[_c_i64] * 3, _c_int, *[_c_f32] * 4, _p, _c_i64, _p]),
@@ -134,6 +138,9 @@ SIGNATURES = {
     "pk_timing_select": (_c_int, [_c_int]),
     "pk_timing_kernel_name": (C.c_char_p, [_c_int]),
 }
+# table sequences S d_loss, then as pk_region_router_norm_bwd
+SIGNATURES["pk_route_topk_balanced_bwd"] = (_c_int, [_p, _p, _c_i64, _p, *SIGNATURES["pk_route_topk_bwd"][1]])
+SIGNATURES["pk_region_router_balanced_bwd"] = (_c_int, [_p, _p, _c_i64, _p, *SIGNATURES["pk_region_router_norm_bwd"][1]])
 SIGNATURES.update({f"{name}_short": SIGNATURES[name] for name in
                    ("pk_fp8_gate_up", "pk_fp8_down", "pk_fp8_dgrad_dh", "pk_fp8_dgrad_dh_t", "pk_fp8_dgrad_dx")})
 

@@ -1,0 +1,36 @@
+// The router's balance loss: what its own kernels and the region's router backward share.
+//
+//   for a sequence of L tokens:  f_e = counts_e E / (K L),  P_e = mean of softmax(logits)_e over its tokens
+//   loss = balance_coeff mean over the sequences that have tokens of sum_e f_e P_e + z_coeff mean over the tokens of lse^2
+//
+// The counts have no gradient.  A token's softmax p sees dloss/dp_e = h_e with h_e = balance_coeff E counts_e / (K L^2 S'), and
+//   d_logit_e = d_loss p_e (h_e - sum_j h_j p_j + 2 z_coeff lse / N).
+// Since the p_j add up to 1, the same constant may be taken from all h: the table holds h - mean(h), from the whole numbers
+// counts_e - K L / E, so that nothing cancels where the experts are nearly balanced.
+#pragma once
+#include "pk_common.h"
+
+namespace pk_balance {
+
+// What a backward needs beside the logits.  table: [S][E] of h - mean(h) without the 1 / S', then 1 / S' and 2 z_coeff / N.
+struct Grad {
+  const float* table;
+  const int32_t* sequences;   // [S + 1], or nullptr: one sequence of all T tokens
+  const float* d_loss;
+  int32_t S;
+};
+
+// Bounds of sequence s.  Offsets ascend within 0 .. T; whatever else they hold, the range stays inside.
+__device__ __forceinline__ int begin_of(const int32_t* sequences, int s, int T) { return sequences ? min(max(sequences[s], 0), T) : 0; }
+__device__ __forceinline__ int end_of(const int32_t* sequences, int s, int T) {
+  return sequences ? min(max(sequences[s + 1], begin_of(sequences, s, T)), T) : T;
+}
+
+// The sequence that token t is in, searched from s on; S: behind the last one, -1: in front of the first one.
+__device__ __forceinline__ int sequence_of(const Grad& g, int s, int t) {
+  if (!g.sequences) return 0;
+  while (s < g.S && g.sequences[s + 1] <= t) ++s;
+  return s == 0 && t < g.sequences[0] ? -1 : s;
+}
+
+}  // namespace pk_balance

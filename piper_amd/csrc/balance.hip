@@ -1,0 +1,345 @@
+// The router's balance loss over packed sequences, with every sequence's tokens per expert, and the gradient of its logits
+// (formulas in balance.h).
+//
+// Memory is what bounds long inputs, 4 bytes a logit forward and 8 backward, launches and their dependent loads short ones.  Forward: a
+// workgroup sums the softmax of up to `chunk` tokens of one sequence, a second launch adds the chunks of every sequence up in a fixed
+// order and 64 bits, and its last workgroup the sequences.  No chunk belongs to two sequences: that of a sequence which starts at
+// token b has the units b / chunk + s and on, which cannot meet (as padded_start in the weight gradients), so that the host needs
+// no look at the lengths.  Backward: one pass, the softmax formed again.
+#include "balance.h"
+#include <algorithm>
+
+namespace {
+
+using namespace pk_balance;
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kChunk = 64, kMostChunks = 512;       // tokens of a chunk: a multiple of kChunk that leaves about kMostChunks of them
+
+// A token's logits lie on LPT lanes, EPL to a lane, 64 / LPT tokens to a wave: expert j * LPT + lane % LPT.
+template <int LPT>
+__device__ __forceinline__ float group_sum(float v) {
+#define PK_STEP(CTRL) v += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true))
+  PK_STEP(0xb1);                       // quad_perm 1 0 3 2
+  PK_STEP(0x4e);                       // quad_perm 2 3 0 1
+  PK_STEP(0x141);                      // row_half_mirror: the other quad of 8 lanes
+  if (LPT > 8) PK_STEP(0x140);         // row_mirror: the other 8 of a row of 16
+#undef PK_STEP
+  const auto add = [](auto r) { return __uint_as_float(r[0]) + __uint_as_float(r[1]); };
+  if (LPT > 16) v = add(__builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  if (LPT > 32) v = add(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return v;
+}
+template <int LPT>
+__device__ __forceinline__ float group_max(float v) {
+#define PK_STEP(CTRL) v = fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true)))
+  PK_STEP(0xb1);
+  PK_STEP(0x4e);
+  PK_STEP(0x141);
+  if (LPT > 8) PK_STEP(0x140);
+#undef PK_STEP
+  const auto most = [](auto r) { return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])); };
+  if (LPT > 16) v = most(__builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  if (LPT > 32) v = most(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return v;
+}
+
+template <int LPT, int EPL>
+__device__ __forceinline__ void load_logits(const float* __restrict__ logits, int64_t t, bool live, int E, int g, float (&x)[EPL]) {
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) x[j] = live && j * LPT + g < E ? logits[t * E + j * LPT + g] : -INFINITY;
+}
+// x becomes the softmax; returns log(sum exp)
+template <int LPT, int EPL>
+__device__ __forceinline__ float softmax(float (&x)[EPL], int E, int g) {
+  float mx = x[0];
+#pragma unroll
+  for (int j = 1; j < EPL; ++j) mx = fmaxf(mx, x[j]);
+  mx = group_max<LPT>(mx);
+  float total = 0.f;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    x[j] = j * LPT + g < E ? expf(x[j] - mx) : 0.f;
+    total += x[j];
+  }
+  total = group_sum<LPT>(total);
+  const float inv = 1.f / total;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) x[j] *= inv;
+  return mx + logf(total);
+}
+
+struct Forward {
+  const float* logits;
+  const int32_t* top_idx;
+  const int32_t* sequences;
+  int32_t T, E, K, S, chunk, units;
+  float balance_coeff, z_coeff;
+  float* part_p;          // [units][E] sums of the softmax
+  int32_t* part_c;        // [units][E] counts
+  float* part_z;          // [units]
+  double* seq;            // [S][2] sum_e f_e P_e and sum of lse^2
+  uint32_t* done;         // workgroups of the second launch that have finished
+  float* loss;
+  int32_t* counts;
+  float* table;
+};
+
+// How many of n things hold, over the workgroup
+template <typename F>
+__device__ __forceinline__ int count_of(int n, int* box, F&& holds) {
+  int c = 0;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) c += holds(i) ? 1 : 0;
+  for (int off = 32; off > 0; off >>= 1) c += __shfl_xor(c, off, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = c;
+  __syncthreads();
+  c = 0;
+  for (int w = 0; w < (int)blockDim.x / 64; ++w) c += box[w];
+  return c;
+}
+
+template <int LPT, int EPL>
+__global__ __launch_bounds__(kThreads) void balance_partial_kernel(const Forward p) {
+  constexpr int EM = LPT * EPL, TPW = 64 / LPT;
+  __shared__ float sum_p[kWaves][EM];
+  __shared__ float sum_z[kWaves];
+  __shared__ int hist[EM];
+  __shared__ int box[kWaves];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
+  const int unit = blockIdx.x;
+  const int s = p.sequences ? count_of(p.S, box, [&](int i) { return begin_of(p.sequences, i, p.T) / p.chunk + i <= unit; }) - 1 : 0;
+  if (s < 0) return;
+  const int b = begin_of(p.sequences, s, p.T), e = end_of(p.sequences, s, p.T);
+  const int first = b + (unit - (b / p.chunk + s)) * p.chunk, n = min(p.chunk, e - first);
+  if (n <= 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane % LPT;
+  for (int i = tid; i < EM; i += kThreads) hist[i] = 0;
+  __syncthreads();
+  for (int i = tid; i < n * p.K; i += kThreads) {
+    const uint32_t id = (uint32_t)p.top_idx[(int64_t)first * p.K + i];
+    if (id < (uint32_t)p.E) atomicAdd(&hist[id], 1);
+  }
+  float sum[EPL] = {}, z = 0.f;
+  for (int i = wave * TPW; i < n; i += kWaves * TPW) {
+    const int t = i + lane / LPT;
+    const bool live = t < n;
+    float x[EPL];
+    load_logits<LPT, EPL>(p.logits, first + t, live, p.E, g, x);
+    const float lse = softmax<LPT, EPL>(x, p.E, g);
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) sum[j] += x[j];
+      z += lse * lse;
+    }
+  }
+#pragma unroll
+  for (int off = LPT; off < 64; off <<= 1) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) sum[j] += __shfl_xor(sum[j], off, 64);
+    z += __shfl_xor(z, off, 64);
+  }
+  if (lane < LPT) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) sum_p[wave][j * LPT + g] = sum[j];
+  }
+  if (lane == 0) sum_z[wave] = z;
+  __syncthreads();
+  for (int i = tid; i < p.E; i += kThreads) {
+    float v = 0.f;
+    for (int w = 0; w < kWaves; ++w) v += sum_p[w][i];
+    p.part_p[(int64_t)unit * p.E + i] = v;
+    p.part_c[(int64_t)unit * p.E + i] = hist[i];
+  }
+  if (tid == 0) p.part_z[unit] = sum_z[0] + sum_z[1] + sum_z[2] + sum_z[3];
+}
+
+__device__ __forceinline__ double block_sum(double v, double* box) {
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int w = 0; w < (int)blockDim.x / 64; ++w) v += box[w];
+  return v;
+}
+
+// A sequence to a workgroup: its chunks added up, its row of the table and of the counts; the last workgroup adds up the sequences.
+constexpr int kMostSum = 1024;
+__global__ __launch_bounds__(kMostSum) void balance_sum_kernel(const Forward p) {
+  __shared__ double sum_p[kMostSum];
+  __shared__ int sum_c[kMostSum];
+  __shared__ double box[kMostSum / 64];
+  __shared__ int ibox[kMostSum / 64];
+  __shared__ int last;
+  const int s = blockIdx.x, tid = threadIdx.x, NT = blockDim.x;
+  const int b = begin_of(p.sequences, s, p.T), e = end_of(p.sequences, s, p.T), L = e - b;
+  const int unit0 = b / p.chunk + s, chunks = min((L + p.chunk - 1) / p.chunk, p.units - unit0);
+  const int width = min((p.E + 63) / 64 * 64, NT), slices = NT / width, slice = tid / width;
+  const double inv = L > 0 ? (double)p.E / ((double)p.K * L * L) : 0.0;
+  double f = 0.0;
+  for (int e0 = 0; e0 < p.E; e0 += width) {
+    const int ex = e0 + tid % width;
+    double v = 0.0;
+    int c = 0;
+    if (ex < p.E && slice < slices) {
+#pragma unroll 8
+      for (int q = slice; q < chunks; q += slices) {
+        v += (double)p.part_p[(int64_t)(unit0 + q) * p.E + ex];
+        c += p.part_c[(int64_t)(unit0 + q) * p.E + ex];
+      }
+    }
+    __syncthreads();
+    sum_p[tid] = v;
+    sum_c[tid] = c;
+    __syncthreads();
+    if (tid < width && ex < p.E) {
+      for (int q = 1; q < slices; ++q) {
+        v += sum_p[q * width + tid];
+        c += sum_c[q * width + tid];
+      }
+      p.counts[(int64_t)s * p.E + ex] = c;
+      p.table[(int64_t)s * p.E + ex] = (float)((double)p.balance_coeff * inv * (c - (double)p.K * L / p.E));
+      f += inv * c * v;
+    }
+  }
+  double z = 0.0;
+  for (int q = tid; q < chunks; q += NT) z += (double)p.part_z[unit0 + q];
+  f = block_sum(f, box);
+  z = block_sum(z, box);
+  if (tid == 0) {
+    __hip_atomic_store(&p.seq[2 * s], f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&p.seq[2 * s + 1], z, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = __hip_atomic_fetch_add(p.done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)p.S - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  double N = 0.0;
+  f = z = 0.0;
+  int some = 0;
+  for (int q = tid; q < p.S; q += NT) {
+    const int l = end_of(p.sequences, q, p.T) - begin_of(p.sequences, q, p.T);
+    N += l;
+    some += l > 0;
+    f += __hip_atomic_load(&p.seq[2 * q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    z += __hip_atomic_load(&p.seq[2 * q + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  f = block_sum(f, box);
+  z = block_sum(z, box);
+  N = block_sum(N, box);
+  const double sequences = block_sum((double)some, box);
+  if (tid == 0) {
+    const double per = sequences > 0 ? 1.0 / sequences : 0.0, each = N > 0 ? (double)p.z_coeff / N : 0.0;
+    *p.loss = (float)((double)p.balance_coeff * f * per + each * z);
+    p.table[(int64_t)p.S * p.E] = (float)per;
+    p.table[(int64_t)p.S * p.E + 1] = (float)(2.0 * each);
+  }
+}
+
+template <int LPT, int EPL>
+__global__ __launch_bounds__(kThreads) void balance_bwd_kernel(const float* __restrict__ logits, const Grad gr, int T, int E, int tokens,
+                                                               float* __restrict__ d_logits) {
+  constexpr int TPW = 64 / LPT;
+  __shared__ int box[kWaves];
+  const int first = blockIdx.x * tokens, n = min(tokens, T - first);
+  const int s0 = gr.sequences ? max(count_of(gr.S + 1, box, [&](int i) { return gr.sequences[i] <= first; }) - 1, 0) : 0;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane % LPT;
+  const float per = gr.table[(int64_t)gr.S * E], slope_z = gr.table[(int64_t)gr.S * E + 1], d_loss = *gr.d_loss;
+  int s = s0;
+  for (int i = wave * TPW; i < n; i += kWaves * TPW) {
+    const int t = i + lane / LPT;
+    if (t >= n) continue;
+    float x[EPL];
+    load_logits<LPT, EPL>(logits, first + t, true, E, g, x);
+    s = sequence_of(gr, max(s, 0), first + t);
+    const bool owned = s >= 0 && s < gr.S;
+    float h[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) h[j] = owned && j * LPT + g < E ? gr.table[(int64_t)s * E + j * LPT + g] : 0.f;
+    const float lse = softmax<LPT, EPL>(x, E, g);
+    float mean = 0.f;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) mean += h[j] * x[j];
+    mean = group_sum<LPT>(mean);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (j * LPT + g < E)
+        d_logits[(int64_t)(first + t) * E + j * LPT + g] = owned ? d_loss * x[j] * (per * (h[j] - mean) + slope_z * lse) : 0.f;
+  }
+}
+
+#define PK_BALANCE_DISPATCH(E, LAUNCH)         \
+  do {                                         \
+    if ((E) <= 8) { LAUNCH(8, 1); }            \
+    else if ((E) <= 16) { LAUNCH(16, 1); }     \
+    else if ((E) <= 32) { LAUNCH(32, 1); }     \
+    else if ((E) <= 64) { LAUNCH(64, 1); }     \
+    else if ((E) <= 128) { LAUNCH(64, 2); }    \
+    else if ((E) <= 256) { LAUNCH(64, 4); }    \
+    else if ((E) <= 512) { LAUNCH(64, 8); }    \
+    else { LAUNCH(64, 16); }                   \
+  } while (0)
+
+int64_t chunk_of(int64_t T) { return kChunk * std::max<int64_t>(1, pk_ceil_div(T, (int64_t)kChunk * kMostChunks)); }
+int64_t units_of(int64_t T, int64_t S) { return T / chunk_of(T) + S + 1; }
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" {
+
+int64_t pk_balance_workspace_bytes(int64_t T, int64_t E, int64_t S) {
+  if (T < 0 || E <= 0 || S <= 0) return PK_ERR_ARG;
+  const int64_t units = units_of(T, S);
+  return 2 * align256(units * E * 4) + align256(units * 4) + align256(S * 16) + 256;
+}
+
+int pk_balance_loss(const float* logits, const int32_t* top_idx, const int32_t* sequences, int64_t T, int64_t E, int64_t K, int64_t S,
+                    float balance_coeff, float z_coeff, float* loss, int32_t* counts, float* table, void* workspace,
+                    int64_t workspace_bytes, pk_stream_t stream) {
+  if (T < 0 || E <= 0 || K <= 0 || S <= 0 || (!sequences && S != 1)) return PK_ERR_ARG;
+  if (E > PK_MAX_EXPERTS || K > PK_MAX_TOPK || T > 0x7fffffffll / K || S > 0x3fffffffll) return PK_ERR_SHAPE;
+  if ((T > 0 && (!logits || !top_idx)) || !loss || !counts || !table) return PK_ERR_ARG;
+  if (!workspace || workspace_bytes < pk_balance_workspace_bytes(T, E, S) || !pk_aligned16(workspace)) return PK_ERR_WORKSPACE;
+  const int64_t units = units_of(T, S);
+  char* at = static_cast<char*>(workspace);
+  const auto take = [&](int64_t bytes) { char* const r = at; at += align256(bytes); return r; };
+  Forward p = {};
+  p.logits = logits; p.top_idx = top_idx; p.sequences = sequences;
+  p.T = (int32_t)T; p.E = (int32_t)E; p.K = (int32_t)K; p.S = (int32_t)S; p.chunk = (int32_t)chunk_of(T); p.units = (int32_t)units;
+  p.balance_coeff = balance_coeff; p.z_coeff = z_coeff;
+  p.part_p = reinterpret_cast<float*>(take(units * E * 4));
+  p.part_c = reinterpret_cast<int32_t*>(take(units * E * 4));
+  p.part_z = reinterpret_cast<float*>(take(units * 4));
+  p.seq = reinterpret_cast<double*>(take(S * 16));
+  p.done = reinterpret_cast<uint32_t*>(at);
+  p.loss = loss; p.counts = counts; p.table = table;
+  hipStream_t s = (hipStream_t)stream;
+#define PK_LAUNCH(LPT, EPL) \
+  PK_LAUNCH_NOCHECK(pk_timing::K_BALANCE, s, (balance_partial_kernel<LPT, EPL>), dim3((unsigned)units), dim3(kThreads), 0, s, p)
+  PK_BALANCE_DISPATCH(E, PK_LAUNCH);
+#undef PK_LAUNCH
+  PK_LAUNCH_NOCHECK(pk_timing::K_BALANCE, s, balance_sum_kernel, dim3((unsigned)S), dim3(units / S >= 8 ? kMostSum : 256), 0, s, p);
+  PK_RETURN_IF_LAUNCH_FAILED();
+  return PK_OK;
+}
+
+int pk_balance_loss_bwd(const float* logits, const int32_t* sequences, const float* table, const float* d_loss, float* d_logits,
+                        int64_t T, int64_t E, int64_t S, pk_stream_t stream) {
+  if (T < 0 || E <= 0 || S <= 0 || (!sequences && S != 1)) return PK_ERR_ARG;
+  if (E > PK_MAX_EXPERTS || T > 0x7fffffffll || S > 0x3fffffffll) return PK_ERR_SHAPE;
+  if (T == 0) return PK_OK;
+  if (!logits || !table || !d_loss || !d_logits) return PK_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  const Grad g{table, sequences, d_loss, (int32_t)S};
+  const int tokens = T >= 16384 ? 64 : 16;
+#define PK_LAUNCH(LPT, EPL)                                                                                                         \
+  PK_LAUNCH_NOCHECK(pk_timing::K_BALANCE_BWD, s, (balance_bwd_kernel<LPT, EPL>), dim3((unsigned)pk_ceil_div(T, tokens)), dim3(kThreads), 0, s, \
+                    logits, g, (int)T, (int)E, tokens, d_logits)
+  PK_BALANCE_DISPATCH(E, PK_LAUNCH);
+#undef PK_LAUNCH
+  PK_RETURN_IF_LAUNCH_FAILED();
+  return PK_OK;
+}
+
+}  // extern "C"

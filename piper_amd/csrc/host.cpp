@@ -223,6 +223,81 @@ void router_weight_grads(const Tensor& p_gate, const Tensor& p_bias, const float
   if (gb.defined()) add_or_set_grad(p_bias, gb);
 }
 
+// ------------------------------------------------------------------------------ the router's balance loss
+struct Balance {
+  bool on = false;
+  double balance = 0, z = 0;
+  Tensor sequences;                                   // offsets, or undefined: one sequence
+  int64_t S() const { return sequences.defined() ? sequences.size(0) - 1 : 1; }
+  const int32_t* offsets() const { return sequences.defined() ? sequences.data_ptr<int32_t>() : nullptr; }
+};
+Balance balance_of(const Tensor& like, const OptTensor& sequences_, double balance, double z) {
+  Balance b;
+  b.on = true;
+  b.balance = balance;
+  b.z = z;
+  b.sequences = opt(sequences_);
+  if (!b.sequences.defined()) return b;
+  TORCH_CHECK_VALUE(b.sequences.dim() == 1 && b.sequences.size(0) >= 2 && b.sequences.scalar_type() == at::kInt,
+                    "balance_loss: sequences are int32 offsets [S + 1], where each begins and the last one ends");
+  same_device(like, {&b.sequences});
+  b.sequences = contig(b.sequences);
+  return b;
+}
+// (loss, counts); table: what the backward needs
+std::pair<Tensor, Tensor> balance_forward(const Balance& b, const float* logits, const int32_t* idx, int64_t T, int64_t E, int64_t K, const Tensor& like,
+                                          Tensor* table) {
+  const auto f32 = like.options().dtype(at::kFloat);
+  const int64_t S = b.S(), bytes = pk_balance_workspace_bytes(T, E, S);
+  TORCH_CHECK(bytes > 0, "pk_balance_workspace_bytes failed: ", pk_status_string((int)bytes));
+  Tensor loss = at::empty({}, f32);
+  Tensor counts = b.sequences.defined() ? at::empty({S, E}, f32.dtype(at::kInt)) : at::empty({E}, f32.dtype(at::kInt));
+  *table = at::empty({S * E + 2}, f32);
+  const Tensor ws = at::empty({bytes}, f32.dtype(at::kByte));
+  PK_CALL(pk_balance_loss, logits, idx, b.offsets(), T, E, K, S, (float)b.balance, (float)b.z, loss.data_ptr<float>(), counts.data_ptr<int32_t>(),
+          table->data_ptr<float>(), ptr(ws), bytes, stream_of(like));
+  return {loss, counts};
+}
+struct BalanceFn : public torch::autograd::Function<BalanceFn> {
+  static variable_list run(const Tensor& logits, const Tensor& idx, const Balance& b, Tensor* table) {
+    TORCH_CHECK_VALUE(logits.dim() == 2 && logits.scalar_type() == at::kFloat, "balance_loss: logits must be float32 [T,E]");
+    TORCH_CHECK_VALUE(idx.dim() == 2 && idx.scalar_type() == at::kInt && idx.size(0) == logits.size(0) && idx.size(1) > 0,
+                      "balance_loss: the chosen experts must be int32 [T,K]");
+    const Tensor lc = contig(logits), ic = contig(idx);
+    auto r = balance_forward(b, fptr(lc), ic.data_ptr<int32_t>(), logits.size(0), logits.size(1), idx.size(1), lc, table);
+    return {r.first, r.second};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& idx, const OptTensor& sequences, double balance, double z) {
+    Tensor table;
+    const Balance b = balance_of(logits, sequences, balance, z);
+    variable_list r = run(logits, idx, b, &table);
+    ctx->save_for_backward({logits, b.sequences, table});
+    ctx->mark_non_differentiable({r[1]});
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list sv = ctx->get_saved_variables();
+    const Tensor logits = contig(sv[0]), d_loss = contig(grads[0]);
+    Tensor d = at::empty_like(logits);
+    PK_CALL(pk_balance_loss_bwd, fptr(logits), sv[1].defined() ? sv[1].data_ptr<int32_t>() : nullptr, fptr(sv[2]), fptr(d_loss), d.data_ptr<float>(),
+            logits.size(0), logits.size(1), sv[1].defined() ? sv[1].size(0) - 1 : 1, stream_of(logits));
+    return {d, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+// None (with `direct`): not ordinary GPU tensors, or a tracing mode is on
+std::optional<variable_list> balance_loss(const Tensor& logits, const Tensor& idx, const OptTensor& sequences_, double balance, double z, bool direct) {
+  const Tensor sequences = opt(sequences_);
+  if (direct && !plain({&logits, &idx, &sequences})) return std::nullopt;
+  refuse_transforms({&logits, &idx, &sequences}, "balance_loss");
+  const RecordDirect record(direct, "piper_amd::balance_loss");
+  require_gpu(logits);
+  same_device(logits, {&idx, &sequences});
+  c10::hip::HIPGuard device(logits.device().index());
+  if (wants_grad({&logits})) return BalanceFn::apply(logits, idx, sequences_, balance, z);
+  Tensor table;
+  return BalanceFn::run(logits, idx, balance_of(logits, sequences_, balance, z), &table);
+}
+
 // ------------------------------------------------------------------------------ the fused region
 struct Shape {
   int64_t T, H, E, I, K, A;
@@ -445,9 +520,10 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
   enum { X, W_GATE, BIAS, W1, W2, W3, RESIDUAL, NORM_W, N_TENSORS };
 
   // (tensors that are absent are passed as empty optionals: autograd gives them no edge)
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const OptTensor& bias_, const Tensor& w1, const Tensor& w2,
-                        const Tensor& w3, const OptTensor& residual_, const OptTensor& norm_w_, int64_t top_k, bool route_norm,
-                        double route_scale, double eps, PyObject* route) {
+  // out; with `balanced` also the balance loss and its counts
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const OptTensor& bias_, const Tensor& w1, const Tensor& w2,
+                               const Tensor& w3, const OptTensor& residual_, const OptTensor& norm_w_, int64_t top_k, bool route_norm,
+                               double route_scale, double eps, PyObject* route, const OptTensor& sequences_, bool balanced, double balance, double z) {
     const Tensor bias = opt(bias_), residual = opt(residual_), norm_w = opt(norm_w_);
     const Shape s = region_shape(x, w_gate, bias, w1, w2, w3, top_k, route_norm, route_scale, eps, residual, norm_w);
     const bool norm = norm_w.defined();
@@ -455,14 +531,25 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
     const Tensor xc = contig(x);
     Tensor out = region_forward(s, route, sv, true, true, xc, contig(w_gate), contig(bias), contig(w1), contig(w2), contig(w3),
                                 norm ? xc : contig(residual), contig(norm_w));
-    ctx->save_for_backward({x, w_gate, bias, w1, w2, w3, norm_w, sv.rows.memory(), sv.mem.memory()});
+    variable_list results = {out};
+    Tensor table;
+    Balance b;
+    if (balanced) {
+      b = balance_of(x, sequences_, balance, z);
+      const auto r = balance_forward(b, sv.mem.f32(sv.logits), sv.mem.i32(sv.idx), s.T, s.E, s.K, x, &table);
+      results.push_back(r.first);
+      results.push_back(r.second);
+      ctx->mark_non_differentiable({r.second});
+      ctx->set_materialize_grads(false);      // a loss that nobody uses costs nothing
+    }
+    ctx->save_for_backward({x, w_gate, bias, w1, w2, w3, norm_w, sv.rows.memory(), sv.mem.memory(), b.sequences, table});
     keep_parameters(ctx, {&w_gate, &bias, &w1, &w2, &w3});
     ctx->saved_data["k"] = top_k;
     ctx->saved_data["norm"] = route_norm;
     ctx->saved_data["scale"] = route_scale;
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["residual"] = residual.defined();
-    return out;
+    return results;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -479,7 +566,9 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
     const bool present[N_TENSORS] = {true, true, bias.defined(), true, true, true, ctx->saved_data["residual"].toBool(), norm};
     for (int i = 0, edge = 0; i < N_TENSORS; ++i) need[i] = present[i] && ctx->needs_input_grad(edge++);
     const bool need_xn = need[X] || (norm && need[NORM_W]);      // the gradient of what the router and the experts read
-    Tensor d_out = contig(grads[0]), xc = contig(x);
+    Tensor d_out = grads[0].defined() ? contig(grads[0]) : at::zeros({s.T, s.H}, x.options()), xc = contig(x);
+    const Tensor &sequences = saved[9], &table = saved[10];
+    const Tensor d_loss = table.defined() && grads[1].defined() ? contig(grads[1]) : Tensor();
     const Tensor w1 = contig(saved[3]), w2 = contig(saved[4]), w3 = contig(saved[5]);
     Tensor w_gate = contig(saved[1]);
     if (!aligned16(w_gate)) w_gate = w_gate.clone();
@@ -562,13 +651,24 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
       if (need_xn) d_x = at::empty({s.T, s.H}, x.options());
       const float *const d_s = n_part > 0 ? nullptr : t.f32(d_scores), *const parts = t.f32(part);
       float *const dwg = static_cast<float*>(ptr(d_wg)), *const db = static_cast<float*>(ptr(d_b));
-      if (!norm || !need_xn) {
+      const bool with_norm = norm && need_xn;
+      if (with_norm && need[NORM_W]) d_norm_w = at::empty({s.H}, norm_w.options());
+      if (d_loss.defined()) {
+        PK_CALL(pk_region_router_balanced_bwd, fptr(table), sequences.defined() ? sequences.data_ptr<int32_t>() : nullptr,
+                sequences.defined() ? sequences.size(0) - 1 : 1, fptr(d_loss), m.f32(sv.logits), m.i32(sv.idx), d_s, parts, n_part, m.i32(sv.inv),
+                s.route_norm, (float)s.route_scale, x_rows, s.dtype, fptr(w_gate), t.at_(d_xs),
+                with_norm ? t.at_(d_xn) : need_xn ? ptr(d_x) : nullptr, dwg, db, 0, w.f32(d_logits), with_norm ? ptr(xc) : nullptr,
+                with_norm ? ptr(contig(norm_w)) : nullptr, with_norm ? m.f32(sv.rstd) : nullptr, with_norm ? ptr(d_out) : nullptr,
+                with_norm ? ptr(d_x) : nullptr, ptr(d_norm_w), s.T, s.H, s.E, s.K, t.at_(router_ws), router_ws_bytes, st);
+        if (with_norm && !need[X]) d_x = Tensor();
+        return;
+      }
+      if (!with_norm) {
         PK_CALL(pk_region_router_bwd, m.f32(sv.logits), m.i32(sv.idx), d_s, parts, n_part, m.i32(sv.inv), s.route_norm, (float)s.route_scale,
                 x_rows, s.dtype, fptr(w_gate), t.at_(d_xs), need_xn ? ptr(d_x) : nullptr, dwg, db, 0, w.f32(d_logits), s.T, s.H, s.E, s.K,
                 t.at_(router_ws), router_ws_bytes, st);
         return;
       }
-      if (need[NORM_W]) d_norm_w = at::empty({s.H}, norm_w.options());
       PK_CALL(pk_region_router_norm_bwd, m.f32(sv.logits), m.i32(sv.idx), d_s, parts, n_part, m.i32(sv.inv), s.route_norm, (float)s.route_scale,
               x_rows, s.dtype, fptr(w_gate), t.at_(d_xs), t.at_(d_xn), dwg, db, 0, w.f32(d_logits), ptr(xc), ptr(contig(norm_w)), m.f32(sv.rstd),
               ptr(d_out), ptr(d_x), ptr(d_norm_w), s.T, s.H, s.E, s.K, t.at_(router_ws), router_ws_bytes, st);
@@ -584,7 +684,8 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
       push_deferred([s, p_gate, p_bias, w_gate, x_rows, dl = w.f32(d_logits), keep = std::array<Tensor, 3>{wgrad.x, wgrad.rows, wgrad.grads}] {
         router_weight_grads(p_gate, p_bias, dl, x_rows, s.dtype, w_gate, s.T, s.H, s.E);
       });
-      return {d_x, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), d_res, d_norm_w, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+      return {d_x, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), d_res, d_norm_w, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(),
+              Tensor(), Tensor()};
     }
     // backward into .grad with gradients already there (a later microbatch of an iteration): the
     // weight-gradient kernels add to them in their epilogues and autograd gets nothing to add
@@ -624,7 +725,7 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
       for (const Tensor* b : std::initializer_list<const Tensor*>{&d_out, &xc, &r.memory(), &w.memory()}) b->record_stream(as_cuda(side));
       for (const Tensor* b : {&d_w1, &d_w2, &d_w3}) b->record_stream(as_cuda(cur));
     }
-    return {d_x, d_wg, d_b, d_w1, d_w2, d_w3, d_res, d_norm_w, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {d_x, d_wg, d_b, d_w1, d_w2, d_w3, d_res, d_norm_w, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -640,7 +741,7 @@ std::optional<Tensor> expert_region(const Tensor& x, const Tensor& w_gate, const
   require_gpu(x);
   c10::hip::HIPGuard device(x.device().index());
   if (wants_grad({&x, &w_gate, &bias, &w1, &w2, &w3, &residual, &norm_w}))
-    return RegionFn::apply(x, w_gate, bias_, w1, w2, w3, residual_, norm_w_, top_k, route_norm, route_scale, eps, route);
+    return RegionFn::apply(x, w_gate, bias_, w1, w2, w3, residual_, norm_w_, top_k, route_norm, route_scale, eps, route, OptTensor(), false, 0.0, 0.0)[0];
   const Shape s = region_shape(x, w_gate, bias, w1, w2, w3, top_k, route_norm, route_scale, eps, residual, norm_w);
   const Tensor xc = contig(x), w1c = contig(w1), w2c = contig(w2), w3c = contig(w3);
   const Tensor gc = contig(w_gate), bc = contig(bias), rc = norm_w.defined() ? xc : contig(residual), nc = contig(norm_w);
@@ -658,6 +759,29 @@ std::optional<Tensor> expert_region(const Tensor& x, const Tensor& w_gate, const
   const bool keep_gu = s.H % piece != 0 || s.I % piece != 0 || !aligned16(xc) || !aligned16(w1c) || !aligned16(w2c) || !aligned16(w3c);
   Saved sv(s, keep_gu, norm_w.defined());
   return region_forward(s, route, sv, keep_gu, false, xc, gc, bc, w1c, w2c, w3c, rc, nc);
+}
+
+// (out, loss, counts): the region with the balance loss of its router
+std::optional<variable_list> expert_region_balanced(const Tensor& x, const Tensor& w_gate, const OptTensor& bias_, const Tensor& w1, const Tensor& w2,
+                                                    const Tensor& w3, int64_t top_k, bool route_norm, double route_scale, const OptTensor& residual_,
+                                                    const OptTensor& sequences_, double balance, double z, const py::object& route_, bool direct) {
+  PyObject* const route = route_.ptr() == Py_None ? nullptr : route_.ptr();
+  const Tensor bias = opt(bias_), residual = opt(residual_), sequences = opt(sequences_);
+  if (direct && !plain({&x, &w_gate, &bias, &w1, &w2, &w3, &residual, &sequences})) return std::nullopt;
+  refuse_transforms({&x, &w_gate, &bias, &w1, &w2, &w3, &residual, &sequences}, "expert_region_balanced");
+  const RecordDirect record(direct, "piper_amd::expert_region_balanced");
+  require_gpu(x);
+  c10::hip::HIPGuard device(x.device().index());
+  if (wants_grad({&x, &w_gate, &bias, &w1, &w2, &w3, &residual}))
+    return RegionFn::apply(x, w_gate, bias_, w1, w2, w3, residual_, OptTensor(), top_k, route_norm, route_scale, 0.0, route, sequences_, true, balance, z);
+  const Shape s = region_shape(x, w_gate, bias, w1, w2, w3, top_k, route_norm, route_scale, 0.0, residual, Tensor());
+  const Balance b = balance_of(x, sequences_, balance, z);
+  Saved sv(s, true, false);
+  const Tensor out = region_forward(s, route, sv, true, false, contig(x), contig(w_gate), contig(bias), contig(w1), contig(w2), contig(w3),
+                                    contig(residual), Tensor());
+  Tensor table;
+  const auto r = balance_forward(b, sv.mem.f32(sv.logits), sv.mem.i32(sv.idx), s.T, s.E, s.K, x, &table);
+  return variable_list{out, r.first, r.second};
 }
 
 // ------------------------------------------------------------------------------ RMSNorm
@@ -721,8 +845,9 @@ std::vector<Tensor> sort_by_expert(const Tensor& top_idx, int64_t E) {
 }
 
 struct RouterFn : public torch::autograd::Function<RouterFn> {
+  // (scores, experts); with `balanced` also the balance loss and its counts
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const OptTensor& bias_, int64_t top_k, bool route_norm,
-                               double route_scale, PyObject* route) {
+                               double route_scale, PyObject* route, const OptTensor& sequences_, bool balanced, double balance, double z) {
     require_gpu(x);
     const Tensor bias = opt(bias_);
     TORCH_CHECK_VALUE(x.dim() == 2 && w_gate.dim() == 2 && x.size(1) == w_gate.size(1), "gate_logits: x [T,H], w_gate [E,H]");
@@ -747,11 +872,23 @@ struct RouterFn : public torch::autograd::Function<RouterFn> {
       PK_CALL(pk_gate_route, ptr(xc), dtype_code(x), fptr(wc), fptr(bc), T, H, E, top_k, route_norm, (float)route_scale, logits.data_ptr<float>(),
               scores.data_ptr<float>(), idx.data_ptr<int32_t>(), ptr(ws), bytes, st);
     }
-    ctx->save_for_backward({x, w_gate, bias, logits, idx});
+    variable_list results = {scores, idx};
+    Tensor table;
+    Balance b;
+    if (balanced) {
+      b = balance_of(x, sequences_, balance, z);
+      const auto r = balance_forward(b, fptr(logits), idx.data_ptr<int32_t>(), T, E, top_k, x, &table);
+      results.push_back(r.first);
+      results.push_back(r.second);
+      ctx->set_materialize_grads(false);
+      ctx->mark_non_differentiable({idx, r.second});
+    } else {
+      ctx->mark_non_differentiable({idx});
+    }
+    ctx->save_for_backward({x, w_gate, bias, logits, idx, b.sequences, table});
     ctx->saved_data["norm"] = route_norm;
     ctx->saved_data["scale"] = route_scale;
-    ctx->mark_non_differentiable({idx});
-    return {scores, idx};
+    return results;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list sv = ctx->get_saved_variables();
@@ -759,14 +896,23 @@ struct RouterFn : public torch::autograd::Function<RouterFn> {
     const int64_t T = x.size(0), H = x.size(1), E = w_gate.size(0), K = idx.size(1);
     Tensor d_s = grads[0].defined() ? contig(grads[0]).to(at::kFloat) : at::zeros({T, K}, logits.options());
     Tensor d_logits = at::empty_like(logits);
-    PK_CALL(pk_route_topk_bwd, fptr(logits), idx.data_ptr<int32_t>(), fptr(d_s), T, E, K, ctx->saved_data["norm"].toBool(),
-            (float)ctx->saved_data["scale"].toDouble(), d_logits.data_ptr<float>(), stream_of(x));
+    const Tensor &sequences = sv[5], &table = sv[6];
+    const bool route_norm = ctx->saved_data["norm"].toBool();
+    const float scale = (float)ctx->saved_data["scale"].toDouble();
+    if (table.defined() && grads[2].defined()) {
+      const Tensor d_loss = contig(grads[2]);
+      PK_CALL(pk_route_topk_balanced_bwd, fptr(table), sequences.defined() ? sequences.data_ptr<int32_t>() : nullptr,
+              sequences.defined() ? sequences.size(0) - 1 : 1, fptr(d_loss), fptr(logits), idx.data_ptr<int32_t>(), fptr(d_s), T, E, K, route_norm, scale,
+              d_logits.data_ptr<float>(), stream_of(x));
+    } else {
+      PK_CALL(pk_route_topk_bwd, fptr(logits), idx.data_ptr<int32_t>(), fptr(d_s), T, E, K, route_norm, scale, d_logits.data_ptr<float>(), stream_of(x));
+    }
     Tensor d_x32, d_w, d_b;
     if (ctx->needs_input_grad(0)) d_x32 = at::empty({T, H}, logits.options());
     if (ctx->needs_input_grad(1)) d_w = at::empty({E, H}, logits.options());
     if (sv[2].defined() && ctx->needs_input_grad(2)) d_b = at::empty({E}, logits.options());
     gate_bwd(fptr(d_logits), ptr(x), dtype_code(x), w_gate, static_cast<float*>(ptr(d_x32)), d_w, d_b, false, T, H, E);
-    return {d_x32.defined() ? d_x32.to(x.scalar_type()) : Tensor(), d_w, d_b, Tensor(), Tensor(), Tensor(), Tensor()};
+    return {d_x32.defined() ? d_x32.to(x.scalar_type()) : Tensor(), d_w, d_b, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 std::pair<Tensor, Tensor> router(const Tensor& x, const Tensor& w_gate, const OptTensor& bias, int64_t top_k, bool route_norm, double route_scale,
@@ -776,8 +922,18 @@ std::pair<Tensor, Tensor> router(const Tensor& x, const Tensor& w_gate, const Op
   require_gpu(x);
   same_device(x, {&w_gate, &b});
   c10::hip::HIPGuard device(x.device().index());
-  auto r = RouterFn::apply(x, w_gate, bias, top_k, route_norm, route_scale, route.ptr() == Py_None ? nullptr : route.ptr());
+  auto r = RouterFn::apply(x, w_gate, bias, top_k, route_norm, route_scale, route.ptr() == Py_None ? nullptr : route.ptr(), OptTensor(), false, 0.0, 0.0);
   return {r[0], r[1]};
+}
+// (scores, experts, loss, counts)
+variable_list router_balanced(const Tensor& x, const Tensor& w_gate, const OptTensor& bias, int64_t top_k, bool route_norm, double route_scale,
+                              const OptTensor& sequences, double balance, double z, const py::object& route) {
+  const Tensor b = opt(bias), seq = opt(sequences);
+  refuse_transforms({&x, &w_gate, &b, &seq}, "router_balanced");
+  require_gpu(x);
+  same_device(x, {&w_gate, &b, &seq});
+  c10::hip::HIPGuard device(x.device().index());
+  return RouterFn::apply(x, w_gate, bias, top_k, route_norm, route_scale, route.ptr() == Py_None ? nullptr : route.ptr(), sequences, true, balance, z);
 }
 
 struct PermuteFn : public torch::autograd::Function<PermuteFn> {
@@ -1412,6 +1568,9 @@ void muon(const std::vector<Tensor>& masters, const std::vector<Tensor>& momenta
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   const auto nogil = py::call_guard<py::gil_scoped_release>();
   m.def("expert_region", &expert_region, nogil);
+  m.def("expert_region_balanced", &expert_region_balanced, nogil);
+  m.def("balance_loss", &balance_loss, nogil);
+  m.def("router_balanced", &router_balanced, nogil);
   m.def("rmsnorm", &rmsnorm, nogil);
   m.def("sort_by_expert", &sort_by_expert, nogil);
   m.def("router", &router, nogil);

@@ -1,6 +1,7 @@
 // Routing: gate logits, wavefront softmax/top-k (+ backward), stable counting sort by expert.
 #include "pk_common.h"
 #include "gate_tail.h"
+#include "balance.h"
 #include "topk.h"
 #include "mfma_x3_gemm.h"
 #include <mutex>
@@ -107,10 +108,11 @@ struct RouteBwdIo {
   int32_t n_part;
   bf16_t* planes;               // optional: d_logits as three bf16 planes [3][T * E] for the gate weight gradient
 };
-template <int EPL>
+// BALANCED: the gradient of the balance loss (balance.h) is added on the way.
+template <int EPL, bool BALANCED>
 __global__ __launch_bounds__(kRouteThreads) void route_topk_bwd_kernel(
     const float* __restrict__ logits, const int32_t* __restrict__ top_idx,
-    const RouteBwdIo io, int T, int E, int K, int route_norm,
+    const RouteBwdIo io, const pk_balance::Grad bal, int T, int E, int K, int route_norm,
     float route_scale, float* __restrict__ d_logits) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int t = blockIdx.x * (kRouteThreads / 64) + wave;
@@ -178,11 +180,32 @@ __global__ __launch_bounds__(kRouteThreads) void route_topk_bwd_kernel(
     for (int j = 0; j < EPL; ++j)
       if (lane + 64 * j == ek) dp[j] = dsk;
   }
+  float h[EPL], h_mean = 0.f, of_lse = 0.f, of_h = 0.f;
+  if (BALANCED) {
+    int seq = 0;          // the token's sequence: the offsets up to t, less one
+    if (bal.sequences) {
+      for (int i = lane; i <= bal.S; i += 64) seq += bal.sequences[i] <= t;
+      seq = (int)wave_sum_f32((float)seq) - 1;
+    }
+    const bool owned = seq >= 0 && seq < bal.S;
+    const float d_loss = owned ? *bal.d_loss : 0.f;
+    const float* const tail = bal.table + (int64_t)bal.S * E;
+    of_h = d_loss * tail[0];
+    of_lse = d_loss * tail[1] * (mx + logf(denom));
+    float part_h = 0.f;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      h[j] = owned && lane + 64 * j < E ? bal.table[(int64_t)seq * E + lane + 64 * j] : 0.f;
+      part_h += h[j] * p[j];
+    }
+    h_mean = wave_sum_f32(part_h);
+  }
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const int e = lane + 64 * j;
     if (e < E) {
-      const float d = p[j] * (dp[j] - D);
+      float d = p[j] * (dp[j] - D);
+      if (BALANCED) d += p[j] * (of_h * (h[j] - h_mean) + of_lse);
       const int64_t at = (int64_t)t * E + e;
       d_logits[at] = d;
       if (io.planes) {
@@ -1445,12 +1468,18 @@ int pk_gate_route(const void* x, int x_dtype, const float* w_gate, const float* 
   return PK_OK;
 }
 
-static int route_topk_bwd(const float* logits, const int32_t* top_idx, const RouteBwdIo& io, int64_t T, int64_t E, int64_t K, int route_norm,
-                          float route_scale, float* d_logits, hipStream_t s) {
+static int route_topk_bwd(const float* logits, const int32_t* top_idx, const RouteBwdIo& io, const pk_balance::Grad* bal, int64_t T, int64_t E,
+                          int64_t K, int route_norm, float route_scale, float* d_logits, hipStream_t s) {
   const dim3 grid((unsigned)pk_ceil_div(T, kRouteThreads / 64)), block(kRouteThreads);
-#define PK_LAUNCH_TOPK_BWD(EPL)                                                                                          \
-  PK_LAUNCH_NOCHECK(pk_timing::K_ROUTE_TOPK_BWD, s, (route_topk_bwd_kernel<EPL>), grid, block, 0, s, logits, top_idx, io, \
-                    (int)T, (int)E, (int)K, route_norm, route_scale, d_logits)
+#define PK_LAUNCH_TOPK_BWD(EPL)                                                                                                    \
+  do {                                                                                                                             \
+    if (bal)                                                                                                                       \
+      PK_LAUNCH_NOCHECK(pk_timing::K_ROUTE_TOPK_BWD, s, (route_topk_bwd_kernel<EPL, true>), grid, block, 0, s, logits, top_idx, io, \
+                        *bal, (int)T, (int)E, (int)K, route_norm, route_scale, d_logits);                                          \
+    else                                                                                                                           \
+      PK_LAUNCH_NOCHECK(pk_timing::K_ROUTE_TOPK_BWD, s, (route_topk_bwd_kernel<EPL, false>), grid, block, 0, s, logits, top_idx, io, \
+                        pk_balance::Grad{}, (int)T, (int)E, (int)K, route_norm, route_scale, d_logits);                            \
+  } while (0)
   PK_DISPATCH_EPL(E, PK_LAUNCH_TOPK_BWD);
 #undef PK_LAUNCH_TOPK_BWD
   PK_RETURN_IF_LAUNCH_FAILED();
@@ -1466,7 +1495,20 @@ int pk_route_topk_bwd(const float* logits, const int32_t* top_idx, const float* 
   if (!logits || !top_idx || !d_top_scores || !d_logits) return PK_ERR_ARG;
   RouteBwdIo io = {};
   io.d_top_scores = d_top_scores;
-  return route_topk_bwd(logits, top_idx, io, T, E, K, route_norm, route_scale, d_logits, (hipStream_t)stream);
+  return route_topk_bwd(logits, top_idx, io, nullptr, T, E, K, route_norm, route_scale, d_logits, (hipStream_t)stream);
+}
+
+int pk_route_topk_balanced_bwd(const float* table, const int32_t* sequences, int64_t S, const float* d_loss, const float* logits,
+                               const int32_t* top_idx, const float* d_top_scores, int64_t T, int64_t E, int64_t K, int route_norm,
+                               float route_scale, float* d_logits, pk_stream_t stream) {
+  if (T < 0 || E <= 0 || K <= 0 || S <= 0 || (!sequences && S != 1)) return PK_ERR_ARG;
+  if (E > PK_MAX_EXPERTS || K > PK_MAX_TOPK || K > E || S > 0x3fffffffll) return PK_ERR_SHAPE;
+  if (T == 0) return PK_OK;
+  if (!logits || !top_idx || !d_top_scores || !d_logits || !table || !d_loss) return PK_ERR_ARG;
+  RouteBwdIo io = {};
+  io.d_top_scores = d_top_scores;
+  const pk_balance::Grad bal{table, sequences, d_loss, (int32_t)S};
+  return route_topk_bwd(logits, top_idx, io, &bal, T, E, K, route_norm, route_scale, d_logits, (hipStream_t)stream);
 }
 
 // workspace of pk_region_router_bwd: [what pk_gate_logits_bwd takes][fp32 d_x for operands that the fused
@@ -1480,8 +1522,8 @@ int64_t pk_region_router_bwd_workspace_bytes(int64_t T, int64_t H, int64_t E, in
 }  // extern "C"
 
 // *tail: what is left for a later launch (launch_gate_tail, or extra blocks of the norm's backward)
-static int region_router_bwd(const float* logits, const int32_t* top_idx, const float* d_top_scores, const float* ds_partial,
-                             int64_t n_partial, const int32_t* inv_perm, int route_norm, float route_scale, const void* x, int x_dtype,
+static int region_router_bwd(const pk_balance::Grad* bal, const float* logits, const int32_t* top_idx, const float* d_top_scores,
+                             const float* ds_partial, int64_t n_partial, const int32_t* inv_perm, int route_norm, float route_scale, const void* x, int x_dtype,
                              const float* w_gate, const void* d_rows, void* d_x, float* d_w_gate, float* d_gate_bias, int accumulate,
                              float* d_logits, int64_t T, int64_t H, int64_t E, int64_t K, void* workspace, int64_t workspace_bytes,
                              GateTail* tail, pk_stream_t stream) {
@@ -1502,7 +1544,7 @@ static int region_router_bwd(const float* logits, const int32_t* top_idx, const 
       io.planes = reinterpret_cast<bf16_t*>(reinterpret_cast<char*>(workspace) + gate_bwd_partial_bytes(T, H, E));
       planes_ready = true;
     }
-    rc = route_topk_bwd(logits, top_idx, io, T, E, K, route_norm, route_scale, d_logits, s);
+    rc = route_topk_bwd(logits, top_idx, io, bal, T, E, K, route_norm, route_scale, d_logits, s);
     if (rc != PK_OK) return rc;
   }
   pk_f32mm::Params p = {};
@@ -1541,7 +1583,7 @@ int pk_region_router_bwd(const float* logits, const int32_t* top_idx, const floa
                          float* d_logits, int64_t T, int64_t H, int64_t E, int64_t K, void* workspace, int64_t workspace_bytes,
                          pk_stream_t stream) {
   GateTail tail = {};
-  const int rc = region_router_bwd(logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, x, x_dtype, w_gate,
+  const int rc = region_router_bwd(nullptr, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, x, x_dtype, w_gate,
                                    d_rows, d_x, d_w_gate, d_gate_bias, accumulate, d_logits, T, H, E, K, workspace, workspace_bytes, &tail,
                                    stream);
   return rc != PK_OK ? rc : launch_gate_tail(tail, (hipStream_t)stream);
@@ -1552,22 +1594,58 @@ int64_t pk_region_router_norm_bwd_workspace_bytes(int64_t T, int64_t H, int64_t 
   return router < 0 ? router : align256(router) + pk_rmsnorm_bwd_workspace_bytes(T, H);
 }
 
+}  // extern "C"
+
+static int region_router_norm_bwd(const pk_balance::Grad* bal, const float* logits, const int32_t* top_idx, const float* d_top_scores,
+                                  const float* ds_partial, int64_t n_partial, const int32_t* inv_perm, int route_norm, float route_scale,
+                                  const void* xn, int x_dtype, const float* w_gate, const void* d_rows, void* d_xn, float* d_w_gate,
+                                  float* d_gate_bias, int accumulate, float* d_logits, const void* x, const void* norm_weight, const float* rstd,
+                                  const void* d_x_addend, void* d_x, void* d_norm_weight, int64_t T, int64_t H, int64_t E, int64_t K,
+                                  void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
+  if (T < 0 || H <= 0 || E <= 0 || !pk_dtype_ok(x_dtype)) return PK_ERR_ARG;
+  if (T > 0 && (!d_xn || !x || !norm_weight || !rstd || !d_x)) return PK_ERR_ARG;
+  const int64_t router = align256(pk_region_router_bwd_workspace_bytes(T, H, E, x_dtype));
+  if (!workspace || workspace_bytes < pk_region_router_norm_bwd_workspace_bytes(T, H, E, x_dtype)) return PK_ERR_WORKSPACE;
+  GateTail tail = {};
+  const int rc = region_router_bwd(bal, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype, w_gate,
+                                   d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, T, H, E, K, workspace, router, &tail, stream);
+  if (rc != PK_OK) return rc;
+  return pk_rmsnorm_bwd_with_tail(d_xn, x, x_dtype, norm_weight, rstd, d_x_addend, d_x, d_norm_weight, accumulate, T, H,
+                                  reinterpret_cast<char*>(workspace) + router, workspace_bytes - router, tail, (hipStream_t)stream);
+}
+
+extern "C" {
+
 int pk_region_router_norm_bwd(const float* logits, const int32_t* top_idx, const float* d_top_scores, const float* ds_partial,
                               int64_t n_partial, const int32_t* inv_perm, int route_norm, float route_scale, const void* xn, int x_dtype,
                               const float* w_gate, const void* d_rows, void* d_xn, float* d_w_gate, float* d_gate_bias, int accumulate,
                               float* d_logits, const void* x, const void* norm_weight, const float* rstd, const void* d_x_addend,
                               void* d_x, void* d_norm_weight, int64_t T, int64_t H, int64_t E, int64_t K, void* workspace,
                               int64_t workspace_bytes, pk_stream_t stream) {
-  if (T < 0 || H <= 0 || E <= 0 || !pk_dtype_ok(x_dtype)) return PK_ERR_ARG;
-  if (T > 0 && (!d_xn || !x || !norm_weight || !rstd || !d_x)) return PK_ERR_ARG;
-  const int64_t router = align256(pk_region_router_bwd_workspace_bytes(T, H, E, x_dtype));
-  if (!workspace || workspace_bytes < pk_region_router_norm_bwd_workspace_bytes(T, H, E, x_dtype)) return PK_ERR_WORKSPACE;
+  return region_router_norm_bwd(nullptr, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype,
+                                w_gate, d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, x, norm_weight, rstd, d_x_addend, d_x,
+                                d_norm_weight, T, H, E, K, workspace, workspace_bytes, stream);
+}
+
+int pk_region_router_balanced_bwd(const float* table, const int32_t* sequences, int64_t S, const float* d_loss, const float* logits,
+                                  const int32_t* top_idx, const float* d_top_scores, const float* ds_partial, int64_t n_partial,
+                                  const int32_t* inv_perm, int route_norm, float route_scale, const void* xn, int x_dtype,
+                                  const float* w_gate, const void* d_rows, void* d_xn, float* d_w_gate, float* d_gate_bias, int accumulate,
+                                  float* d_logits, const void* x, const void* norm_weight, const float* rstd, const void* d_x_addend,
+                                  void* d_x, void* d_norm_weight, int64_t T, int64_t H, int64_t E, int64_t K, void* workspace,
+                                  int64_t workspace_bytes, pk_stream_t stream) {
+  if (S <= 0 || (!sequences && S != 1) || (T > 0 && (!table || !d_loss))) return PK_ERR_ARG;
+  if (S > 0x3fffffffll) return PK_ERR_SHAPE;
+  const pk_balance::Grad bal{table, sequences, d_loss, (int32_t)S};
+  if (norm_weight)
+    return region_router_norm_bwd(&bal, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype,
+                                  w_gate, d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, x, norm_weight, rstd, d_x_addend, d_x,
+                                  d_norm_weight, T, H, E, K, workspace, workspace_bytes, stream);
   GateTail tail = {};
-  const int rc = region_router_bwd(logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype, w_gate,
-                                   d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, T, H, E, K, workspace, router, &tail, stream);
-  if (rc != PK_OK) return rc;
-  return pk_rmsnorm_bwd_with_tail(d_xn, x, x_dtype, norm_weight, rstd, d_x_addend, d_x, d_norm_weight, accumulate, T, H,
-                                  reinterpret_cast<char*>(workspace) + router, workspace_bytes - router, tail, (hipStream_t)stream);
+  const int rc = region_router_bwd(&bal, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype,
+                                   w_gate, d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, T, H, E, K, workspace, workspace_bytes,
+                                   &tail, stream);
+  return rc != PK_OK ? rc : launch_gate_tail(tail, (hipStream_t)stream);
 }
 
 int64_t pk_sort_workspace_bytes(int64_t A, int64_t E) {

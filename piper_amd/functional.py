@@ -1,10 +1,11 @@
 """Autograd wiring of the expert region and registration of the reference's operator.
 
-Two ways in:
+Ways in:
 
 * ``expert_region(...)``: the whole region (gate -> top-k -> sort -> grouped SwiGLU with the permute
   fused into the operand load -> unpermute+combine) as ONE autograd node with a hand-written
   backward.  This is what ``piper_amd.moe.AnnotatedMoE`` runs.
+* ``expert_region_balanced``: the same with the router's balance loss (``balance_loss``);
 * the piecewise operators the reference model code calls one by one
   (examples/models/qwen3.py:237-283): ``router``, ``reorder``, ``permute``, ``bmm_experts``,
   ``combine``.  ``bmm_experts`` is also registered as ``torch.ops.piper_artifact.bmm_experts`` with
@@ -74,6 +75,20 @@ def router(x, w_gate, gate_bias=None, *, top_k: int, route_norm: bool, route_sca
     top_scores, top_idx = call(x, w_gate, gate_bias, int(top_k), bool(route_norm), float(route_scale))
     counts = _sorted_tables(top_idx, w_gate.shape[0])[0]
     return top_scores, top_idx, counts
+
+
+def _router_balanced(x, w_gate, gate_bias, top_k, route_norm, route_scale, sequences, balance_coeff, z_coeff):
+    return tuple(host().router_balanced(x, w_gate, gate_bias, top_k, route_norm, route_scale, sequences, balance_coeff, z_coeff, _replaced_route()))
+
+
+def router_balanced(x, w_gate, gate_bias=None, *, top_k: int, route_norm: bool, route_scale: float = 1.0, balance_coeff: float = 1.0,
+                    z_coeff: float = 0.0, sequences=None):
+    """``router`` with the balance loss of its choice (``balance_loss``): (top_scores, selected_experts_indices, num_tokens_per_expert [E],
+    loss, counts)."""
+    call = torch.ops.piper_amd.router_balanced if _is_tracing() else _router_balanced
+    top_scores, top_idx, loss, counts = call(x, w_gate, gate_bias, int(top_k), bool(route_norm), float(route_scale), sequences,
+                                             float(balance_coeff), float(z_coeff))
+    return top_scores, top_idx, _sorted_tables(top_idx, w_gate.shape[0])[0], loss, counts
 
 
 def reorder(top_scores: torch.Tensor, top_idx: torch.Tensor, num_experts: int):
@@ -169,6 +184,63 @@ def bmm_experts(w1, w2, w3, x, num_tokens_per_expert):
         if out is not None:
             return out
     return torch.ops.piper_artifact.bmm_experts(w1, w2, w3, x, num_tokens_per_expert)
+
+
+# --------------------------------------------------------------------------- balance loss
+def _loss_shapes(like, num_experts, sequences):
+    """(loss, counts) without data"""
+    loss = like.new_empty((), dtype=torch.float32)
+    return loss, like.new_empty((num_experts,) if sequences is None else (sequences.shape[0] - 1, num_experts), dtype=torch.int32)
+
+
+def _balance_loss(logits, top_idx, sequences, balance_coeff, z_coeff):
+    if _traced_without_data(logits):
+        loss, counts = _loss_shapes(logits, logits.shape[1], sequences)
+        if torch.is_grad_enabled() and logits.requires_grad:
+            loss.requires_grad_(True)
+        return loss, counts
+    return tuple(host().balance_loss(logits, top_idx, sequences, balance_coeff, z_coeff, False))
+
+
+def _balance_loss_forward_only(*args):
+    with torch.no_grad():
+        return _balance_loss(*args)
+
+
+def balance_loss(logits, top_idx, *, balance_coeff: float = 1.0, z_coeff: float = 0.0, sequences=None):
+    """(loss, counts) of a router that chose the experts top_idx [T,K] (int32) by logits [T,E] (float32).  With f_e = counts_e E / (K L) and
+    P_e the mean of softmax(logits)_e, both over a sequence of L tokens,
+
+        loss = balance_coeff * mean over the sequences of sum_e f_e P_e + z_coeff * mean over the tokens of logsumexp(logits)^2,
+
+    which is balance_coeff where all experts are chosen and scored alike.  ``sequences`` (int32 [S+1], ascending)
+    says where each sequence begins and the last one ends; sequences without tokens do not count, tokens outside all of them are
+    padding: they are not counted and have a gradient of zero.  None: all tokens are one sequence.  counts: int32 [E], with ``sequences``
+    [S,E]; they have no gradient."""
+    args = (logits, top_idx, sequences, float(balance_coeff), float(z_coeff))
+    if _direct(logits, top_idx, sequences):
+        out = host().balance_loss(*args, True)
+        if out is not None:
+            return tuple(out)
+    return torch.ops.piper_amd.balance_loss(*args)
+
+
+class _WithLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, out, loss):
+        ctx.like = (loss.shape, loss.dtype, loss.device)
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, d_out):
+        shape, dtype, device = ctx.like
+        return d_out, torch.ones(shape, dtype=dtype, device=device)
+
+
+def with_loss(out, loss):
+    """`out`, with `loss` trained beside it: whoever differentiates `out` (a later stage that never sees the loss) adds
+    the gradient of `loss`, times one, on the way."""
+    return _WithLoss.apply(out, loss)
 
 
 # --------------------------------------------------------------------------- experts in 8-bit blocks
@@ -339,6 +411,24 @@ def _expert_region_forward_only(x, w_gate, gate_bias, w1, w2, w3, top_k, route_n
         return _expert_region_autograd(x, w_gate, gate_bias, w1, w2, w3, top_k, route_norm, route_scale, residual)
 
 
+def _expert_region_balanced(x, w_gate, gate_bias, w1, w2, w3, top_k, route_norm, route_scale, residual, sequences, balance_coeff, z_coeff):
+    ts = [t for t in (x, w_gate, gate_bias, w1, w2, w3, residual) if t is not None]
+    if _traced_without_data(*ts):
+        out = torch.empty_like(x)
+        loss, counts = _loss_shapes(x, w_gate.shape[0], sequences)
+        if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+            out.requires_grad_(True)
+            loss.requires_grad_(True)
+        return out, loss, counts
+    return tuple(host().expert_region_balanced(x, w_gate, gate_bias, w1, w2, w3, top_k, route_norm, route_scale, residual, sequences,
+                                               balance_coeff, z_coeff, _replaced_route(), False))
+
+
+def _expert_region_balanced_forward_only(*args):
+    with torch.no_grad():
+        return _expert_region_balanced(*args)
+
+
 def _rmsnorm_autograd(x, weight, eps):
     if _traced_without_data(x, weight):
         out = torch.empty_like(x)
@@ -365,7 +455,12 @@ def register_region_ops() -> bool:
     lib.define("rmsnorm(Tensor x, Tensor weight, float eps) -> Tensor")
     lib.define("bmm_experts_fp8(Tensor? w1, Tensor? w2, Tensor? w3, Tensor q1, Tensor q2, Tensor q3, Tensor s1, Tensor s2, Tensor s3, "
                "Tensor? t1, Tensor? t2, Tensor? t3, Tensor x, Tensor num_tokens_per_expert, bool short_sums=False) -> Tensor")
-    for name, fwd, auto in (("expert_region", _expert_region_forward_only, _expert_region_autograd),
+    lib.define("balance_loss(Tensor logits, Tensor top_idx, Tensor? sequences, float balance_coeff, float z_coeff) -> (Tensor, Tensor)")
+    lib.define("expert_region_balanced(Tensor x, Tensor w_gate, Tensor? gate_bias, Tensor w1, Tensor w2, Tensor w3, int top_k, bool route_norm, "
+               "float route_scale, Tensor? residual, Tensor? sequences, float balance_coeff, float z_coeff) -> (Tensor, Tensor, Tensor)")
+    for name, fwd, auto in (("balance_loss", _balance_loss_forward_only, _balance_loss),
+                            ("expert_region_balanced", _expert_region_balanced_forward_only, _expert_region_balanced),
+                            ("expert_region", _expert_region_forward_only, _expert_region_autograd),
                             ("rmsnorm", _rmsnorm_forward_only, _rmsnorm_autograd),
                             ("bmm_experts_fp8", _bmm_experts_fp8_forward_only, _bmm_experts_fp8)):
         lib.impl(name, fwd, "CUDA")
@@ -378,7 +473,9 @@ def register_region_ops() -> bool:
     lib.define("router(Tensor x, Tensor w_gate, Tensor? gate_bias, int top_k, bool route_norm, float route_scale) -> (Tensor, Tensor)")
     lib.define("permute(Tensor x, Tensor perm, int top_k) -> Tensor")
     lib.define("combine(Tensor y, Tensor perm, Tensor top_scores) -> Tensor")
-    for name, fn in (("router", _router), ("permute", _permute), ("combine", _combine)):
+    lib.define("router_balanced(Tensor x, Tensor w_gate, Tensor? gate_bias, int top_k, bool route_norm, float route_scale, Tensor? sequences, "
+               "float balance_coeff, float z_coeff) -> (Tensor, Tensor, Tensor, Tensor)")
+    for name, fn in (("router", _router), ("permute", _permute), ("combine", _combine), ("router_balanced", _router_balanced)):
         for key in ("CUDA", "AutogradCUDA", "CPU", "AutogradCPU"):
             lib.impl(name, fn, key)
     _REGION_LIBS.append(lib)
@@ -396,6 +493,19 @@ def expert_region(x, w_gate, gate_bias, w1, w2, w3, *, top_k: int, route_norm: b
             return out
     return torch.ops.piper_amd.expert_region(x, w_gate, gate_bias, w1, w2, w3, int(top_k), bool(route_norm),
                                              float(route_scale), residual)
+
+
+def expert_region_balanced(x, w_gate, gate_bias, w1, w2, w3, *, top_k: int, route_norm: bool, route_scale: float = 1.0, residual=None,
+                           balance_coeff: float = 1.0, z_coeff: float = 0.0, sequences=None):
+    """``expert_region`` with the balance loss of its router (``balance_loss``): (out, loss, counts).  The loss's gradient is added where
+    the router's backward forms that of its logits."""
+    args = (x, w_gate, gate_bias, w1, w2, w3, int(top_k), bool(route_norm), float(route_scale), residual, sequences, float(balance_coeff),
+            float(z_coeff))
+    if _direct(x, w_gate, gate_bias, w1, w2, w3, residual, sequences):
+        out = host().expert_region_balanced(*args, _replaced_route(), True)
+        if out is not None:
+            return tuple(out)
+    return torch.ops.piper_amd.expert_region_balanced(*args)
 
 
 def rmsnorm(x, weight, eps: float = 1e-6):

@@ -29,6 +29,9 @@ class MoEArgs:
     score_before_experts: bool = False
     num_shared_experts: int = 0
     load_balance_coeff: float | None = None
+    # what the router is trained on beside its scores (functional.balance_loss); zero: not formed
+    balance_loss_coeff: float = 0.0
+    router_z_loss_coeff: float = 0.0
 
 
 class TokenChoiceTopKRouter(nn.Module):
@@ -40,12 +43,16 @@ class TokenChoiceTopKRouter(nn.Module):
         self.num_experts, self.top_k = num_experts, top_k
         self.route_norm, self.route_scale = route_norm, route_scale
 
-    def forward(self, x: torch.Tensor, expert_bias: torch.Tensor | None = None):
+    def forward(self, x: torch.Tensor, expert_bias: torch.Tensor | None = None, balance: dict | None = None):
+        """``balance`` (arguments of functional.router_balanced): the balance loss and its counts follow."""
         if expert_bias is not None:
             raise NotImplementedError(
                 "selection-only expert_bias (load_balance_coeff) is not part of the reference configurations "
                 "(qwen3.py:48,175 set load_balance_coeff=None); use gate_bias for a logit bias"
             )
+        if balance is not None:
+            return F_.router_balanced(x, self.gate.weight, self.gate.bias, top_k=self.top_k, route_norm=self.route_norm,
+                                      route_scale=self.route_scale, **balance)
         return F_.router(x, self.gate.weight, self.gate.bias, top_k=self.top_k,
                          route_norm=self.route_norm, route_scale=self.route_scale)
 
@@ -88,6 +95,11 @@ class AnnotatedMoE(nn.Module):
     autograd node; ``fused=False`` follows the reference's op-by-op data flow (router, reorderer,
     gather, EP-annotated experts, scatter+combine) through the piecewise HIP operators."""
 
+    balance_loss_coeff = router_z_loss_coeff = 0.0
+    # of the last forward with a balance loss: its value, and the tokens of each expert (with ``sequences`` of each of them)
+    balance_loss: torch.Tensor | None = None
+    tokens_per_expert: torch.Tensor | None = None
+
     def __init__(self, moe_args: MoEArgs, dim: int, hidden_dim: int, dtype: torch.dtype | None = None, fused: bool = True):
         super().__init__()
         if moe_args.score_func != "softmax":
@@ -104,6 +116,17 @@ class AnnotatedMoE(nn.Module):
         self.shared_experts = None
         self.score_before_experts = False
         self.fused = fused
+        self.balance_loss_coeff = getattr(moe_args, "balance_loss_coeff", 0.0)
+        self.router_z_loss_coeff = getattr(moe_args, "router_z_loss_coeff", 0.0)
+
+    @property
+    def balanced(self) -> bool:
+        return self.balance_loss_coeff != 0 or self.router_z_loss_coeff != 0
+
+    def _trained_beside(self, out: torch.Tensor, loss: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
+        """`out`, whose backward also trains the router on `loss`: a stage hands on its output, nobody sees the loss."""
+        self.balance_loss, self.tokens_per_expert = loss.detach(), counts
+        return F_.with_loss(out, loss) if loss.requires_grad else out
 
     def init_weights(self, std: float = 0.02, generator: torch.Generator | None = None) -> None:
         for p in (self.router.gate.weight, self.experts.w1, self.experts.w3, self.experts.w2):
@@ -111,12 +134,22 @@ class AnnotatedMoE(nn.Module):
         if self.router.gate.bias is not None:
             nn.init.zeros_(self.router.gate.bias)
 
-    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, experts_fp8: F_.Fp8Experts | None = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, experts_fp8: F_.Fp8Experts | None = None,
+                sequences: torch.Tensor | None = None) -> torch.Tensor:
         """``residual`` (same shape as x; fused path only) is added in the combine kernel.  ``experts_fp8`` (of
-        ``experts.quantize()``): the experts' products run in 8-bit floating point, through the piecewise operators."""
+        ``experts.quantize()``): the experts' products run in 8-bit floating point, through the piecewise operators.
+        ``sequences`` (int32 offsets into the bs * slen tokens): those of the balance loss, where MoEArgs asks for one."""
         bs, slen, dim = x.shape
         x2 = x.reshape(-1, dim)
         top_k = self.router.top_k
+        loss = dict(balance_coeff=self.balance_loss_coeff, z_coeff=self.router_z_loss_coeff, sequences=sequences) if self.balanced else None
+        if self.fused and experts_fp8 is None and loss is not None:
+            with annotate(EP_TAG):
+                out = self._trained_beside(*F_.expert_region_balanced(
+                    x2, self.router.gate.weight, self.router.gate.bias, self.experts.w1, self.experts.w2, self.experts.w3, top_k=top_k,
+                    route_norm=self.router.route_norm, route_scale=self.router.route_scale,
+                    residual=None if residual is None else residual.reshape(-1, dim), **loss))
+            return out.reshape(bs, slen, dim)
         if self.fused and experts_fp8 is None:
             with annotate(EP_TAG):
                 out = F_.expert_region(x2, self.router.gate.weight, self.router.gate.bias, self.experts.w1,
@@ -125,9 +158,12 @@ class AnnotatedMoE(nn.Module):
                                        residual=None if residual is None else residual.reshape(-1, dim))
             return out.reshape(bs, slen, dim)
         if residual is not None:
-            return residual + self.forward(x, experts_fp8=experts_fp8)
+            return residual + self.forward(x, experts_fp8=experts_fp8, sequences=sequences)
 
-        top_scores, selected_experts_indices, num_tokens_per_expert = self.router(x2, self.expert_bias)
+        if loss is None:
+            top_scores, selected_experts_indices, num_tokens_per_expert = self.router(x2, self.expert_bias)
+        else:
+            top_scores, selected_experts_indices, num_tokens_per_expert, *balance = self.router(x2, self.expert_bias, loss)
         _scores_sorted, token_indices_experts_sorted, num_tokens_per_expert = self.reorderer(
             top_scores, selected_experts_indices)
         routed_input = F_.permute(x2, token_indices_experts_sorted, top_k)
@@ -135,6 +171,8 @@ class AnnotatedMoE(nn.Module):
             gathered_output = (self.experts(routed_input, num_tokens_per_expert) if experts_fp8 is None else
                                self.experts(routed_input, num_tokens_per_expert, experts_fp8))
         out_experts = F_.combine(gathered_output.reshape(-1, dim), token_indices_experts_sorted, top_scores)
+        if loss is not None:
+            out_experts = self._trained_beside(out_experts, *balance)
         return out_experts.reshape(bs, slen, dim)
 
 
@@ -167,13 +205,13 @@ class MoEFeedForwardBlock(nn.Module):
         if torch.compiler.is_compiling():
             return False
         norm, moe = self._modules["ffn_norm"], self._modules["moe"]
-        return (moe.fused and _called_as_defined(norm, RMSNorm) and _called_as_defined(moe, AnnotatedMoE)
+        return (moe.fused and not moe.balanced and _called_as_defined(norm, RMSNorm) and _called_as_defined(moe, AnnotatedMoE)
                 and not (_FORWARD_HOOKS or _FORWARD_PRE_HOOKS or _BACKWARD_HOOKS or _BACKWARD_PRE_HOOKS)
                 and F_.rmsnorm is _OPERATORS[0] and F_.expert_region is _OPERATORS[1])
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, sequences: torch.Tensor | None = None) -> torch.Tensor:
         if not self._one_node():
-            return self.moe(self.ffn_norm(x), residual=x)
+            return self.moe(self.ffn_norm(x), residual=x) if sequences is None else self.moe(self.ffn_norm(x), residual=x, sequences=sequences)
         bs, slen, dim = x.shape
         norm, moe = self.ffn_norm, self.moe
         router, experts = moe.router, moe.experts
