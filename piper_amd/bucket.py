@@ -110,6 +110,8 @@ def flatten_params(bucket: BucketState, params: Sequence[torch.nn.Parameter], *,
     bucket.reduce_scatter_grads = bucket.flat_grads  # dp_degree == 1: reduce-scatter is the identity
     bucket.shard_param = shard_param
     bucket.shard_optimizer = (optim_class or FusedAdamW)([shard_param])
+    if hasattr(bucket.shard_optimizer, "bind_views"):       # an optimizer that asks for the shapes in the bucket (FusedMuon)
+        bucket.shard_optimizer.bind_views(shard_param, view_specs)
     bucket.param_shard_info = (0, padded, orig_numel)
     bucket.param_view_specs = view_specs
     bucket.full_params_fresh = True

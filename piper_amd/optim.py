@@ -18,7 +18,43 @@ import torch
 from . import ops
 
 
-class FusedAdamW(torch.optim.Optimizer):
+class _FlatStateOptimizer(torch.optim.Optimizer):
+    """An optimizer whose states hold flat fp32 (or narrower) buffers and a master of their parameter's weights.  Subclasses say which saved
+    states they take (_checked) and how they become theirs (_restore)."""
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict) -> None:
+        """torch's, which gives every floating-point state the parameter's type, a copy of its own: moments and master keep theirs here, and
+        an fp32 parameter stays its own master.  A state of another kind (``state_bits``) or of other sizes is a ValueError that leaves the
+        optimizer as it was."""
+        saved = []      # what the program's own pre-hooks make of state_dict: this one is the last to run
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, given: saved.extend(self._checked(given))),
+                 self.register_load_state_dict_post_hook(lambda _: self._restore(saved), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _restore_tensors(self, saved, types: dict) -> None:
+        """The tensors `types` names in those types, copies of their own; the master of an fp32 parameter is the parameter."""
+        for p, st in saved:
+            own = self.state[p]
+            for name, dtype in types.items():
+                own[name] = st[name].to(device=p.device, dtype=dtype, copy=True)
+            if p.dtype == torch.float32:
+                own["master"] = p.detach().reshape(-1)
+            else:
+                own["master"] = st["master"].to(device=p.device, dtype=torch.float32, copy=True)
+
+    def _found(self, state_dict) -> list:
+        """[(parameter, its saved state)]"""
+        params = [p for group in self.param_groups for p in group["params"]]
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        return [(p, state_dict["state"][i]) for p, i in zip(params, ids) if state_dict["state"].get(i)]
+
+
+class FusedAdamW(_FlatStateOptimizer):
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, fused: bool = True, zero_grad_in_step: bool = False, state_bits: int = 32,
                  seed: int = 0):
@@ -117,36 +153,12 @@ class FusedAdamW(torch.optim.Optimizer):
     def _step8(self, st: dict, grad: torch.Tensor, group: dict, shadow, zero_grad: bool) -> None:
         ops.adamw8_fused(st["master"], *(st[k] for k in _MOMENTS8), grad, shadow=shadow, zero_grad=zero_grad, **self._how8(st, group))
 
-    @torch.no_grad()
-    def load_state_dict(self, state_dict) -> None:
-        """torch's, which gives every floating-point state the parameter's type, a copy of its own: moments and master keep theirs here, and
-        an fp32 parameter stays its own master.  A state of the other ``state_bits`` or of other sizes is a ValueError that leaves the
-        optimizer as it was."""
-        saved = []      # what the program's own pre-hooks make of state_dict: this one is the last to run
-        hooks = (self.register_load_state_dict_pre_hook(lambda _, given: saved.extend(self._checked(given))),
-                 self.register_load_state_dict_post_hook(lambda _: self._restore(saved), prepend=True))
-        try:
-            super().load_state_dict(state_dict)
-        finally:
-            for hook in hooks:
-                hook.remove()
-
     def _restore(self, saved) -> None:
-        types = dict(zip(_MOMENTS8, _TYPES8)) if self.state_bits == 8 else dict(exp_avg=torch.float32, exp_avg_sq=torch.float32)
-        for p, st in saved:
-            own = self.state[p]
-            for name, dtype in types.items():
-                own[name] = st[name].to(device=p.device, dtype=dtype, copy=True)
-            if p.dtype == torch.float32:
-                own["master"] = p.detach().reshape(-1)
-            else:
-                own["master"] = st["master"].to(device=p.device, dtype=torch.float32, copy=True)
+        self._restore_tensors(saved, dict(zip(_MOMENTS8, _TYPES8)) if self.state_bits == 8 else dict(exp_avg=torch.float32, exp_avg_sq=torch.float32))
 
     def _checked(self, state_dict) -> list:
         """[(parameter, its saved state)] of a state dict that this optimizer can take."""
-        params = [p for group in self.param_groups for p in group["params"]]
-        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        found = [(p, state_dict["state"][i]) for p, i in zip(params, ids) if state_dict["state"].get(i)]
+        found = self._found(state_dict)
         for p, st in found:
             n, blocks = p.numel(), -(-p.numel() // ops.ADAMW8_BLOCK)
             if self.state_bits == 8:
@@ -164,3 +176,147 @@ class FusedAdamW(torch.optim.Optimizer):
 
 _MOMENTS8 = ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")
 _TYPES8 = (torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.float8_e5m2, torch.float8_e8m0fnu)
+
+
+class FusedMuon(_FlatStateOptimizer):
+    """Every matrix by its orthogonalized momentum (ops.muon_fused), what is no matrix by AdamW, in fp32 masters, with the
+    bf16 value the model reads written in the same pass.
+
+    A parameter of two dimensions or more is a matrix, or a stack of them [.., rows, cols].  In a flat bucket the parameters are views:
+    ``bucket.flatten_params(..., optim_class=FusedMuon)`` tells the optimizer where they are (``bind_views``).  ``matrices(param)`` says
+    which parameters are updated as matrices (a router's gate or an embedding is often left to AdamW); default: those of two
+    dimensions or more.  ``adamw``: lr (a schedule of this optimizer's lr moves it in proportion), betas, eps and weight_decay of the others where they
+    differ from this optimizer's lr and weight decay and AdamW's defaults.  ``half_products``: see ops.muon_fused.  4 bytes of state an element (4 more for AdamW's) beside the master."""
+
+    def __init__(self, params, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.1, ns_steps: int = 5,
+                 ns_coefficients=ops.NEWTON_SCHULZ, eps: float = 1e-7, adjust_lr: str = "original", half_products: bool = False,
+                 adamw: dict | None = None, matrices=None, fused: bool = True, zero_grad_in_step: bool = False):
+        other = dict(lr=lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=weight_decay)
+        if adamw:
+            unknown = set(adamw) - set(other)
+            if unknown:
+                raise ValueError(f"FusedMuon: adamw takes lr, betas, eps and weight_decay, not {sorted(unknown)}")
+            other.update(adamw)
+        b1, b2 = other["betas"]
+        if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0 or eps <= 0 or not 0 <= ns_steps <= 100 or len(tuple(ns_coefficients)) != 3 or \
+                adjust_lr not in ("original", "match_rms_adamw"):
+            raise ValueError("invalid Muon hyper-parameters")
+        if adamw and adamw.get("lr", lr) != lr and lr == 0:
+            raise ValueError("FusedMuon: adamw's lr follows lr in proportion, which has to be positive for that")
+        if other["lr"] < 0 or other["eps"] < 0 or not 0 <= b1 < 1 or not 0 <= b2 < 1 or other["weight_decay"] < 0:
+            raise ValueError("invalid AdamW hyper-parameters")
+        defaults = dict(lr=lr, momentum=momentum, nesterov=bool(nesterov), weight_decay=weight_decay, ns_steps=int(ns_steps),
+                        ns_coefficients=tuple(float(c) for c in ns_coefficients), eps=eps, adjust_lr=adjust_lr, adamw_lr_ratio=other["lr"] / lr if lr else 1.0,
+                        adamw_betas=(b1, b2), adamw_eps=other["eps"], adamw_weight_decay=other["weight_decay"])
+        super().__init__(params, defaults)
+        self.half_products, self.zero_grad_in_step = bool(half_products), zero_grad_in_step
+        self._is_matrix = matrices or (lambda p: p.dim() >= 2)
+        self._views: dict = {}
+
+    def bind_views(self, p: torch.Tensor, specs) -> None:
+        """`p` is a flat buffer of the parameters ``specs``: (parameter, offset, number of elements, shape) each."""
+        if self.state.get(p):
+            raise RuntimeError("FusedMuon.bind_views: the parameter has been stepped already")
+        if p.dim() != 1:
+            raise ValueError("FusedMuon.bind_views: views of a flat parameter")
+        places = []
+        for param, offset, numel, shape in specs:
+            if offset < 0 or offset + numel > p.numel() or torch.Size(shape).numel() != numel:
+                raise ValueError(f"FusedMuon.bind_views: {numel} elements at {offset} as {tuple(shape)} are no view of {p.numel()} elements")
+            places.append((offset, numel, tuple(shape), len(shape) >= 2 and bool(self._is_matrix(param))))
+        self._views[p] = places
+
+    def _places(self, p: torch.Tensor) -> list:
+        """(offset, number of elements, shape, whether it is a matrix) of the parameters in p."""
+        if p in self._views:
+            return self._views[p]
+        return [(0, p.numel(), tuple(p.shape), p.dim() >= 2 and bool(self._is_matrix(p)))]
+
+    def _adamw_elements(self, p: torch.Tensor) -> int:
+        return sum(-(-n // 4) * 4 for _, n, _, matrix in self._places(p) if not matrix)
+
+    def _init_state(self, p: torch.Tensor) -> dict:
+        st = self.state[p]
+        if not st:
+            flat = p.detach().reshape(-1)
+            st["step"] = 0
+            st["master"] = flat if p.dtype == torch.float32 else flat.float()
+            st["momentum"] = torch.zeros_like(st["master"])              # of what is no matrix: AdamW's first moment
+            st["exp_avg_sq"] = torch.zeros(self._adamw_elements(p), dtype=torch.float32, device=p.device)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                grad = p.grad.detach()
+                if p in self._views:
+                    flat = grad.reshape(-1)
+                    owned = flat.dtype == torch.float32 and flat.is_contiguous()
+                    self._update(p, group, flat if owned else flat.float().contiguous(), {}, self.zero_grad_in_step and owned)
+                else:
+                    self._update(p, group, None, {0: grad}, False)
+                    if self.zero_grad_in_step:
+                        grad.zero_()
+        return loss
+
+    @torch.no_grad()
+    def step_packed(self, p: torch.Tensor, grads, offsets, numels, flat_grad: torch.Tensor | None = None) -> None:
+        """One step of the bucket `p` whose last gradients have not been packed: see FusedAdamW.step_packed."""
+        group = next(g for g in self.param_groups if any(q is p for q in g["params"]))
+        places = [(o, n) for o, n, *_ in self._places(p)]
+        if p not in self._views or [tuple(x) for x in zip(offsets, numels)] != places:
+            raise RuntimeError("FusedMuon.step_packed: gradients of the views that bind_views has been told of, in their order")
+        self._update(p, group, flat_grad, dict(zip(offsets, grads)), self.zero_grad_in_step and flat_grad is not None)
+
+    def _update(self, p: torch.Tensor, group: dict, flat, own: dict, clear: bool) -> None:
+        if not p.is_contiguous():
+            raise RuntimeError("FusedMuon needs contiguous parameters (flatten them into a bucket)")
+        st = self._init_state(p)
+        st["step"] += 1
+        shadow = None if p.dtype == torch.float32 else p.detach().reshape(-1)
+        cut = lambda t, o, n: None if t is None else t[o:o + n]  # noqa: E731
+        todo, second = [], 0
+        for o, n, shape, matrix in self._places(p):
+            buffers = [cut(t, o, n) for t in (st["master"], st["momentum"], flat, shadow)]
+            if matrix:
+                todo.append([None if t is None else t.view(shape) for t in buffers] + [own.get(o)])
+            elif n:
+                self._adamw(*buffers, own.get(o), st["exp_avg_sq"][second:second + n], st["step"], group, clear)
+                second += -(-n // 4) * 4
+        if todo:
+            masters, momenta, flats, shadows, grads = (list(t) for t in zip(*todo))
+            ops.muon_fused(masters, momenta, grads, flat_grads=flats, shadows=shadows, lr=group["lr"], momentum=group["momentum"],
+                           weight_decay=group["weight_decay"], nesterov=group["nesterov"], steps=group["ns_steps"],
+                           coefficients=group["ns_coefficients"], eps=group["eps"], adjust_lr=group["adjust_lr"], zero_grad=clear,
+                           half_products=self.half_products)
+
+    def _adamw(self, master, exp_avg, flat, shadow, grad, exp_avg_sq, step: int, group: dict, clear: bool) -> None:
+        b1, b2 = group["adamw_betas"]
+        given = (master, exp_avg, flat, shadow)
+        # (16-byte boundaries: a bucket that was flattened without alignment goes through copies)
+        used = [t if t is None or t.data_ptr() % 16 == 0 else t.clone() for t in given]
+        ops.adamw_fused_packed(used[0], used[1], exp_avg_sq, used[2], [None if grad is None else grad.reshape(-1)], [0], [master.numel()], step=step,
+                               lr=group["lr"] * group["adamw_lr_ratio"], beta1=b1, beta2=b2, eps=group["adamw_eps"], weight_decay=group["adamw_weight_decay"],
+                               shadow=used[3], zero_grad=clear and flat is not None)
+        for to, t in zip(given, used):
+            if to is not t:
+                to.copy_(t)
+
+    def _restore(self, saved) -> None:
+        self._restore_tensors(saved, dict(momentum=torch.float32, exp_avg_sq=torch.float32))
+
+    def _checked(self, state_dict) -> list:
+        found = self._found(state_dict)
+        for p, st in found:
+            n = p.numel()
+            sizes = dict(master=n, momentum=n, exp_avg_sq=self._adamw_elements(p))
+            if "step" not in st or any(k not in st or st[k].numel() != size for k, size in sizes.items()):
+                raise ValueError(f"FusedMuon: the saved state is not one of a parameter of {n} elements with {sizes['exp_avg_sq']} in no matrix")
+        return found
