@@ -182,22 +182,6 @@ struct Stage {
     }
   }
 };
-// LDS traffic of one wave is ordered by the hardware; this only stops the compiler from
-// moving the staged reads above the writes.
-__device__ __forceinline__ void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-// Wait until at most `t` (0..MAXT) whole tiles of L loads each are still in flight.
-template <int L, int MAXT>
-__device__ __forceinline__ void wait_tiles(int t) {
-  if (MAXT <= 0 || t <= 0) { wait_dma<0>(); return; }
-  if (t >= MAXT) { wait_dma<(MAXT > 0 ? MAXT : 0) * L>(); return; }
-  wait_tiles<L, (MAXT > 0 ? MAXT - 1 : 0)>(t);
-}
-
 // Wait until at most n (wave-uniform, rounded down to a multiple of 4, capped at 60) vector-memory
 // operations are outstanding.  Loads, stores and atomics retire from the counter in issue
 // order, so with n = a lower bound of the operations issued AFTER the ones of interest this

@@ -121,4 +121,20 @@ __device__ __forceinline__ V frag_mn(const char* tile, int col0, int ks, int lan
   return __builtin_bit_cast(V, v);
 }
 
+// LDS traffic of one wave is ordered by the hardware; this only stops the compiler from
+// moving the staged reads above the writes.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Wait until at most `t` (0..MAXT) whole tiles of L loads each are still in flight.
+template <int L, int MAXT>
+__device__ __forceinline__ void wait_tiles(int t) {
+  if (MAXT <= 0 || t <= 0) { wait_dma<0>(); return; }
+  if (t >= MAXT) { wait_dma<(MAXT > 0 ? MAXT : 0) * L>(); return; }
+  wait_tiles<L, (MAXT > 0 ? MAXT - 1 : 0)>(t);
+}
+
 }  // namespace pk_lds

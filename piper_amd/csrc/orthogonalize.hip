@@ -37,7 +37,9 @@ constexpr int kPad = 128;
 constexpr int kMaxEntries = 40;              // shapes of a group: keeps the kernels' arguments below 4 KiB
 constexpr int kChunk = 8192;                 // elements a workgroup of begin_kernel takes
 constexpr int kThreads = 256;
-constexpr int64_t kGroupBytes = 192 << 20;   // workspace that is asked for: what the 256 MiB memory-side cache can hold
+// Workspace that is asked for.  Groups that stay in the 256 MiB memory-side cache leave too few workgroups a launch: 128 matrices of
+// 768 x 2048, bf16 / fp32 results, ms with 192 MiB 8.6 / 17.4, 384 6.4 / 17.3, 768 6.2 / 15.4, 1,536 5.8 / 14.9, all at once 5.5 / 14.6.
+constexpr int64_t kGroupBytes = 1ll << 30;
 
 // Matrices of one shape that lie one behind the other, as the kernels at both ends see them.
 struct Entry {
@@ -84,6 +86,14 @@ __host__ __device__ inline int64_t matrix_bytes(int rows, int cols, int mp, int 
   const int64_t chunks = ((int64_t)rows * cols + kChunk - 1) / kChunk;
   return (at_sums(mp, np, precise) + chunks * 8 + 255) / 256 * 256;
 }
+// Where element (row, col) of a matrix of ld columns is, in fp16 values from its first one, and its lower part from there.  Single products
+// read the upper plane alone: one plane behind the other.  Three products read both: 32 columns of one, then of the other, so that a k-tile
+// of both is 128 consecutive bytes of a row.
+__host__ __device__ inline int64_t place(bool precise, int row, int col, int ld) {
+  return precise ? (int64_t)row * 2 * ld + (col >> 5) * 64 + (col & 31) : (int64_t)row * ld + col;
+}
+__host__ __device__ inline int64_t to_lower(bool precise, int rows, int ld) { return precise ? 32 : (int64_t)rows * ld; }
+
 template <typename F>
 __device__ __forceinline__ int entry_of(int n, int block, F&& first) {
   int lo = 0, hi = n;
@@ -173,7 +183,7 @@ __global__ __launch_bounds__(kThreads) void convert_kernel(const Ends p) {
   const double factor = (double)kX / (norm < (double)p.eps ? (double)p.eps : norm);   // (NaN stays)
   const int64_t base = (int64_t)t.mat * size;
   f16_t* const hi = reinterpret_cast<f16_t*>(t.mem);
-  f16_t* const lo = reinterpret_cast<f16_t*>(t.mem + plane_x(e.mp, e.np));
+  f16_t* const lo = hi + to_lower(p.precise, e.mp, e.np);
   const int r0 = t.tall ? t.j0 : t.i0, c0 = t.tall ? t.i0 : t.j0;
   for (int q = tid; q < 64 * 64; q += kThreads) {
     const int r = r0 + (q >> 6), c = c0 + (q & 63);
@@ -197,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void convert_kernel(const Ends p) {
       h[v] = (f16_t)x;
       l[v] = (f16_t)(x - (float)h[v]);
     }
-    const int64_t at = (int64_t)(t.i0 + i) * e.np + t.j0 + j;
+    const int64_t at = place(p.precise, t.i0 + i, t.j0 + j, e.np);
     *reinterpret_cast<f16x4_t*>(hi + at) = h;
     *reinterpret_cast<f16x4_t*>(lo + at) = l;
   }
@@ -212,10 +222,10 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const Ends p, int from
   const int tid = threadIdx.x;
   const int64_t size = (int64_t)e.rows * e.cols;
   const f16_t* const hi = reinterpret_cast<const f16_t*>(t.mem + 2 * from * plane_x(e.mp, e.np));
-  const f16_t* const lo = hi + (int64_t)e.mp * e.np;
+  const f16_t* const lo = hi + to_lower(p.precise, e.mp, e.np);
   for (int q = tid; q < 64 * 16; q += kThreads) {
     const int i = q >> 4, j = (q & 15) * 4;
-    const int64_t at = (int64_t)(t.i0 + i) * e.np + t.j0 + j;
+    const int64_t at = place(p.precise, t.i0 + i, t.j0 + j, e.np);
     const f16x4_t h = *reinterpret_cast<const f16x4_t*>(hi + at), l = *reinterpret_cast<const f16x4_t*>(lo + at);
 #pragma unroll
     for (int v = 0; v < 4; ++v) (t.tall ? turned[j + v][i] : turned[i][j + v]) = ((float)h[v] + (float)l[v]) * (1.f / kX);
@@ -241,153 +251,265 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const Ends p, int from
 // ---------------------------------------------------------------- the products
 enum Product { GRAM, POLY, UPDATE };
 
-// 128 x 128 outputs of one product of one matrix, 64-deep k-tiles, two in LDS; four waves of 64 x 64.
+// Row tiles (of BM) of the 256 x 256 blocks on and below the diagonal of a symmetric mp x mp result, block row by block row: a full
+// block row r has r + 1 blocks of 256 / BM tiles, the last one may be half a block high.
+template <int BM>
+__host__ __device__ inline int units_of_symmetric(int mp) {
+  constexpr int R = 256 / BM;
+  const int tm = (mp + BM - 1) / BM, whole = tm / R;
+  return whole * (whole + 1) / 2 * R + (tm % R) * (whole + 1);
+}
+
+// BM x 256 outputs of one product of one matrix (more rows and columns than there are: read from the last ones, not stored).
 //   GRAM    A = X X^T              rows of X against rows of X
 //   POLY    B = b A + c A A        A is symmetric: its rows against its rows
 //   UPDATE  X' = a X + B X         X comes as [k][columns] and through the transposing LDS read
-// GRAM and POLY are symmetric: the tiles on and below the diagonal are computed and stored twice.
-// PRECISE: three products, hi hi + lo hi + hi lo, one behind the other along k.  The matrix instructions cut what they add to a sum
+// GRAM and POLY are symmetric: the 256 x 256 blocks on and below the diagonal are computed, those below it stored twice.
+// PRECISE: three products, lo hi + hi lo + hi hi, of both planes of a k-tile.  The matrix instructions cut what they add to a sum
 // off at its last bit instead of rounding it, which makes long sums of one sign too small (diagonals of 1,100 products by 8e-7, and
-// the result by ten times that): every 128 products the accumulators go into a second set by ordinary additions.
-template <int KIND, bool PRECISE>
-__global__ __launch_bounds__(256) void product_kernel(const Gemm p) {
-  constexpr int BM = 128, BK = 64, TILE = BM * BK * 2, STAGE = 2 * TILE, L = 4;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
+// the result by ten times that): every 64 values of k the accumulators go into a second set by ordinary additions.
+//
+// Eight waves, (BM / 2) x 64 outputs each, in two groups half a k-tile apart, one wave of each on a SIMD: while one multiplies a k-tile
+// out of registers, the other reads its next k-tile's fragments from LDS and requests a later k-tile from memory; a barrier,
+// and they swap (the k-loop of the grouped products).  k-tiles go straight to LDS, NS - 1 of them ahead.  A k-tile has KT values of k; W
+// fp16 values of a row (both planes with PRECISE).
+template <int KIND, bool PRECISE, int BM, int KT, int NS>
+__global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
+  constexpr int BN = 256, NW = 8, WM = BM / 2, TM = WM / 32, TN = 2, KS = KT / 16;
+  constexpr int P = PRECISE ? 2 : 1, W = KT * P;
+  constexpr int A_BYTES = BM * W * 2, STAGE = (BM + BN) * W * 2, LA = A_BYTES / (NW * 1024), LB = BN * W * 2 / (NW * 1024), L = LA + LB;
+  constexpr int STAGING = 32 * 64 * 4;                  // of a wave: 32 rows of its outputs
+  static_assert(NS * STAGE <= 160 * 1024 && NW * STAGING <= NS * STAGE, "LDS budget");
+  static_assert(W == 32 || W == 64, "rows of the LDS tiles");
+  static_assert(!PRECISE || KT == 32, "blocks of 32 of either plane");
+  __shared__ __attribute__((aligned(1024))) char smem[NS * STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave >> 2, wn = wave & 3;
   const int en = entry_of(p.n, blockIdx.x, [&](int i) { return p.e[i].first_unit; });
-  const int mp = p.e[en].mp, np = p.e[en].np, tm = mp / BM, tn = np / BM;
-  const int per = KIND == UPDATE ? tm * tn : tm * (tm + 1) / 2;
-  const int local = blockIdx.x - p.e[en].first_unit, mat = local / per;
-  int mt, nt;
+  const int mp = p.e[en].mp, np = p.e[en].np;
+  const int N = KIND == UPDATE ? np : mp;               // columns of the result
+  const int tm = (mp + BM - 1) / BM, tn = (N + BN - 1) / BN;
+  const int local = blockIdx.x - p.e[en].first_unit;
+  int mat, mt, nt;
   if (KIND == UPDATE) {
-    mt = (local % per) / tn;
-    nt = (local % per) % tn;
+    mat = local / (tm * tn);
+    mt = local % (tm * tn) / tn;
+    nt = local % (tm * tn) % tn;
   } else {
+    constexpr int R = BN / BM;                          // row tiles of a 256 x 256 block
+    const int per = units_of_symmetric<BM>(mp);
+    mat = local / per;
     const int t = local % per;
-    mt = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-    while ((mt + 1) * (mt + 2) / 2 <= t) ++mt;
-    while (mt * (mt + 1) / 2 > t) --mt;
-    nt = t - mt * (mt + 1) / 2;
+    nt = (int)((sqrtf(8.f * (t / R) + 1.f) - 1.f) * 0.5f);       // row of blocks, corrected, and the column in it
+    while ((nt + 1) * (nt + 2) / 2 * R <= t) ++nt;
+    while (nt * (nt + 1) / 2 * R > t) --nt;
+    const int in_row = t - nt * (nt + 1) / 2 * R, rows = min(R, tm - nt * R);
+    mt = nt * R + in_row % rows;
+    nt = in_row / rows;
   }
   char* const mem = p.ws + p.e[en].ws + (int64_t)mat * p.e[en].stride;
-  const int64_t px = plane_x(mp, np), pa = plane_a(mp);
+  const int64_t px = plane_x(mp, np);
   char* const X = mem + 2 * p.from * px;
   char* const Xn = mem + 2 * (1 - p.from) * px;
   char* const A = mem + at_a(mp, np);
   char* const B = mem + at_b(mp, np, PRECISE);
-
   const char* const left = KIND == GRAM ? X : KIND == POLY ? A : B;
   const char* const right = KIND == POLY ? A : X;
-  const int64_t left_plane = KIND == GRAM ? px : pa, right_plane = KIND == POLY ? pa : px;
-  const int lda = KIND == GRAM ? np : mp, ldb = KIND == POLY ? mp : np;
-  const int nkt = (KIND == GRAM ? np : mp) / BK, total = PRECISE ? 3 * nkt : nkt;
+  const int lda = (KIND == GRAM ? np : mp) * P, ldb = (KIND == POLY ? mp : np) * P;      // of a row in memory
+  const int nkt = (KIND == GRAM ? np : mp) / KT;
+  const int row0 = mt * BM, col0 = nt * BN;
 
-  uint32_t va[L], vb[L];
+  // ---- the loader: a lane's byte offsets from two wave-uniform pointers that advance by a constant per k-tile
+  uint32_t va[LA], vb[LB];
 #pragma unroll
-  for (int i = 0; i < L; ++i) {
+  for (int i = 0; i < LA; ++i) {
     int r, k;
-    kc_slot<BK>(wave * L + i, lane, r, k);
-    va[i] = (uint32_t)(r * lda + k) * 2u;
-    if (KIND == UPDATE) mn_slot<BM>(wave * L + i, lane, r, k);
-    vb[i] = (uint32_t)(r * ldb + k) * 2u;
+    kc_slot<W>(wave * LA + i, lane, r, k);
+    va[i] = (uint32_t)(min(r, mp - 1 - row0) * lda + k) * 2u;
   }
-  auto request = [&](int kt) {
-    const int seg = PRECISE ? kt / nkt : 0, k = PRECISE ? kt % nkt : kt;
-    const char* a = uniform_ptr(left + (seg == 1 ? left_plane : 0) + ((int64_t)mt * BM * lda + (int64_t)k * BK) * 2);
-    const char* b = uniform_ptr(right + (seg == 2 ? right_plane : 0) +
-                                (KIND == UPDATE ? (int64_t)k * BK * ldb + (int64_t)nt * BM : (int64_t)nt * BM * ldb + (int64_t)k * BK) * 2);
-    const uint32_t to = lds_addr(smem) + (kt & 1) * STAGE + wave * (L * 1024);
-    static_for<L>([&](auto i) { dma16_s<decltype(i)::value * 1024>(va[i], a, to); });
-    static_for<L>([&](auto i) { dma16_s<TILE + decltype(i)::value * 1024>(vb[i], b, to); });
-  };
-  floatx16_t acc[2][2] = {}, sum[2][2] = {};
-  request(0);
-  for (int kt = 0; kt < total; ++kt) {
-    if (kt + 1 < total) {
-      request(kt + 1);
-      wait_dma<2 * L>();
+#pragma unroll
+  for (int i = 0; i < LB; ++i) {
+    int r, k;
+    if (KIND == UPDATE) {
+      mn_slot<BN * P>(wave * LB + i, lane, r, k);
+      vb[i] = (uint32_t)(r * ldb + min(k, (N - col0) * P - 8)) * 2u;
     } else {
-      wait_dma<0>();
+      kc_slot<W>(wave * LB + i, lane, r, k);
+      vb[i] = (uint32_t)(min(r, N - 1 - col0) * ldb + k) * 2u;
     }
-    block_barrier();
-    const char* const st = smem + (kt & 1) * STAGE;
+  }
+  const char* ld_a = uniform_ptr(left + (int64_t)row0 * lda * 2);
+  const char* ld_b = uniform_ptr(right + (KIND == UPDATE ? (int64_t)col0 * P * 2 : (int64_t)col0 * ldb * 2));
+  const int64_t step_b = KIND == UPDATE ? (int64_t)KT * ldb * 2 : W * 2;
+  auto request = [&](int stage) {
+    const uint32_t to = lds_addr(smem) + stage * STAGE;
+    static_for<LA>([&](auto i) { dma16_s<decltype(i)::value * 1024>(va[i], ld_a, to + wave * (LA * 1024)); });
+    static_for<LB>([&](auto i) { dma16_s<A_BYTES + decltype(i)::value * 1024>(vb[i], ld_b, to + wave * (LB * 1024)); });
+    ld_a += W * 2;
+    ld_b += step_b;
+  };
+
+  floatx16_t acc[TM][TN] = {}, sum[PRECISE ? TM : 1][TN] = {};
 #pragma unroll
-    for (int ks = 0; ks < BK / 16; ++ks) {
-      f16x8_t fa[2], fb[2];
+  for (int s = 0; s < NS - 1; ++s)
+    if (s < nkt) request(s);
+  wait_tiles<L, NS - 2>(min(nkt, NS - 1) - 1);
+  block_barrier();
+  const int grp = wave >> 2;
+  const bool live = row0 + wm * WM < mp && col0 + wn * 64 < N;
+  if (grp == 1) block_barrier();
+  int cur = 0;
+  f16x8_t fa[P][KS][TM], fb[P][KS][TN];       // upper and lower plane
+  // FIRST: the accumulators go into the second set and start again
+  auto k_tile = [&](int kt, auto first) __attribute__((always_inline)) {
+    constexpr bool FIRST = decltype(first)::value;
+    // ---- memory phase
+    const char* const st = smem + cur * STAGE;
+    if (live) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = frag_kc<BK, f16x8_t>(st, wm * 64 + 32 * i, ks, lane);
-        fb[i] = KIND == UPDATE ? frag_mn<BM, f16x8_t>(st + TILE, wn * 64 + 32 * i, ks, lane) : frag_kc<BK, f16x8_t>(st + TILE, wn * 64 + 32 * i, ks, lane);
-      }
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int pl = 0; pl < P; ++pl) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[j], fa[i], acc[i][j], 0, 0, 0);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    block_barrier();
-    if (PRECISE && (kt & 1)) {
+          for (int i = 0; i < TM; ++i) fa[pl][ks][i] = frag_kc<W, f16x8_t>(st, wm * WM + 32 * i, ks + pl * KS, lane);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          sum[i][j] += acc[i][j];
-          acc[i][j] = floatx16_t{};
+          for (int j = 0; j < TN; ++j)
+            fb[pl][ks][j] = KIND == UPDATE ? frag_mn<BN * P, f16x8_t>(st + A_BYTES, (wn * 64 + 32 * j) * P + 32 * pl, ks, lane)
+                                           : frag_kc<W, f16x8_t>(st + A_BYTES, wn * 64 + 32 * j, ks + pl * KS, lane);
         }
     }
-  }
-  if (PRECISE) {
+    __builtin_amdgcn_sched_barrier(0);
+    if (kt + NS - 1 < nkt) request(cur == 0 ? NS - 1 : cur - 1);      // the stage of k-tile kt - 1
+    cur = cur + 1 == NS ? 0 : cur + 1;
+    if (FIRST && live) {      // (while the other group multiplies)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] += sum[i][j];
+        for (int j = 0; j < TN; ++j) sum[PRECISE ? i : 0][j] += acc[i][j];
+    }
+    // a wave's own part of k-tile kt + 1 has landed when the phase before its first read ends
+    const int younger = min(NS - 2, nkt - 2 - kt);
+    if (grp == 1) wait_tiles<L, NS - 2>(younger);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    block_barrier();
+    // ---- compute phase
+    if (live) {
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int pr = PRECISE ? 0 : 2; pr < 3; ++pr)        // lo hi, hi lo, hi hi
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[pr == 1 ? P - 1 : 0][ks][j], fa[pr == 0 ? P - 1 : 0][ks][i],
+                                                                 FIRST && pr == 0 && ks == 0 ? floatx16_t{} : acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_s_setprio(0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (grp == 0) wait_tiles<L, NS - 2>(younger);
+    block_barrier();
+  };
+  if constexpr (PRECISE) {
+    for (int kt = 0; kt < nkt; kt += 2) {                // (k is a multiple of 128)
+      k_tile(kt, std::true_type{});
+      k_tile(kt + 1, std::false_type{});
+    }
+  } else {
+    for (int kt = 0; kt < nkt; ++kt) k_tile(kt, std::false_type{});
   }
-  // acc[i][j][v] is row 32 i + lane % 32, column 32 j + 8 (v / 4) + 4 (lane / 32) + v % 4 of the wave's 64 x 64
-  const int ldc = KIND == UPDATE ? np : mp;
-  const int64_t plane_c = KIND == UPDATE ? px : pa;
+  if (grp == 0) block_barrier();        // the whole ring is free
+  if (!live) return;
+
+  // ---- epilogue: 32 rows of a wave at a time through LDS, so that a lane has 8 neighbouring columns and memory is read and
+  // written 16 bytes a lane.  acc[i][j][v] is row 32 i + lane % 32, column 32 j + 8 (v / 4) + 4 (lane / 32) + v % 4.
+  const int ldc = N;
+  const int64_t lower = to_lower(PRECISE, mp, ldc) * 2;       // bytes
   char* const out = KIND == GRAM ? A : KIND == POLY ? B : Xn;
-  const char* const old = KIND == POLY ? A : X;        // what a or b multiplies
+  const char* const old = KIND == POLY ? A : X;         // what a or b multiplies
   constexpr float unscale = KIND == GRAM ? kA / (kX * kX) : KIND == POLY ? 1.f / (kA * kA) : 1.f;
+  constexpr bool OLD_LO = KIND == UPDATE || (KIND == POLY && PRECISE), OUT_LO = KIND == UPDATE || PRECISE;
+  const bool mirrored = KIND != UPDATE && mt / (BN / BM) != nt;
+  char* const buf = smem + wave * STAGING;
+  const int lr = lane >> 3, lc = lane & 7;              // a lane's row (of 8 in a pass) and columns 8 lc ..
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
+  for (int i = 0; i < TM; ++i) {
+    const int r0 = row0 + wm * WM + 32 * i, c0 = col0 + wn * 64;
+    f16x8_t oh[4], ol[4];
+    if (KIND != GRAM) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int row = mt * BM + wm * 64 + 32 * i + (lane & 31), col = nt * BM + wn * 64 + 32 * j + 8 * q + 4 * (lane >> 5);
-        const int64_t at = (int64_t)row * ldc + col;
-        float x[4];
+        const char* const at = old + place(PRECISE, r0 + 8 * q + lr, c0 + 8 * lc, ldc) * 2;
+        oh[q] = *reinterpret_cast<const f16x8_t*>(at);
+        if (OLD_LO) ol[q] = *reinterpret_cast<const f16x8_t*>(at + lower);
+      }
+    }
+    wave_lds_fence();                                   // the chunk before has been read
 #pragma unroll
-        for (int v = 0; v < 4; ++v) x[v] = acc[i][j][4 * q + v] * unscale;
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        floatx4_t v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (acc[i][j][4 * q + k] + (PRECISE ? sum[PRECISE ? i : 0][j][4 * q + k] : 0.f)) * unscale;
+        const int row = lane & 31, chunk = 8 * j + 2 * q + (lane >> 5);
+        *reinterpret_cast<floatx4_t*>(buf + row * 256 + ((chunk ^ (row & 15)) << 4)) = v;
+      }
+    wave_lds_fence();
+    f16x8_t h[4], l[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int row = 8 * q + lr;
+      float x[8];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const floatx4_t v = *reinterpret_cast<const floatx4_t*>(buf + row * 256 + (((2 * lc + half) ^ (row & 15)) << 4));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[4 * half + k] = v[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
         if (KIND != GRAM) {
-          const f16x4_t h = *reinterpret_cast<const f16x4_t*>(old + at * 2);
-          f16x4_t l = {};
-          if (KIND == UPDATE || PRECISE) l = *reinterpret_cast<const f16x4_t*>(old + plane_c + at * 2);
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const float o = (float)h[v] + (float)l[v];
-            x[v] = KIND == POLY ? p.b * (o * (1.f / kA)) + p.c * x[v] : p.a * o + x[v];
-          }
+          const float o = OLD_LO ? (float)oh[q][k] + (float)ol[q][k] : (float)oh[q][k];
+          x[k] = KIND == POLY ? p.b * (o * (1.f / kA)) + p.c * x[k] : p.a * o + x[k];
         }
-        f16x4_t h, l;
+        h[q][k] = (f16_t)x[k];
+        l[q][k] = (f16_t)(x[k] - (float)h[q][k]);
+      }
+      char* const at = out + place(PRECISE, r0 + row, c0 + 8 * lc, ldc) * 2;
+      *reinterpret_cast<f16x8_t*>(at) = h[q];
+      if (OUT_LO) *reinterpret_cast<f16x8_t*>(at + lower) = l[q];
+    }
+    if (mirrored) {
+      // the same 32 x 64 values turned: fp16 rows of 128 bytes, 16-byte pieces swizzled by the row; within 16 lanes of the
+      // transposing read, lane t points at row t / 4, columns 4 (t % 4) .. and receives rows 0 .. 3 of column t
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          h[v] = (f16_t)x[v];
-          l[v] = (f16_t)(x[v] - (float)h[v]);
+      for (int plane = 0; plane < (OUT_LO ? 2 : 1); ++plane) {
+        wave_lds_fence();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int row = 8 * q + lr;
+          *reinterpret_cast<f16x8_t*>(buf + row * 128 + ((lc ^ (row & 7)) << 4)) = plane ? l[q] : h[q];
         }
-        *reinterpret_cast<f16x4_t*>(out + at * 2) = h;
-        if (KIND == UPDATE || PRECISE) *reinterpret_cast<f16x4_t*>(out + plane_c + at * 2) = l;
-        if (KIND != UPDATE && mt != nt) {
+        wave_lds_fence();
+        const int t = lane & 15, ra = 8 * (lane >> 4) + (t >> 2), rb = ra + 4;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const int64_t mirror = (int64_t)(col + v) * ldc + row;
-            reinterpret_cast<f16_t*>(out)[mirror] = h[v];
-            if (PRECISE) reinterpret_cast<f16_t*>(out + plane_c)[mirror] = l[v];
-          }
+        for (int q = 0; q < 4; ++q) {                   // columns 16 q ..
+          const int c = 16 * q + 4 * (t & 3);
+          const shortx4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) shortx4_t*)(buf + ra * 128 + (((c >> 3) ^ (ra & 7)) << 4) + (c & 7) * 2));
+          const shortx4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) shortx4_t*)(buf + rb * 128 + (((c >> 3) ^ (rb & 7)) << 4) + (c & 7) * 2));
+          typedef short shortx8_t __attribute__((ext_vector_type(8)));
+          *reinterpret_cast<shortx8_t*>(out + plane * lower + place(PRECISE, c0 + 16 * q + t, r0 + 8 * (lane >> 4), ldc) * 2) =
+              __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
       }
+    }
+  }
 }
 
 // ---------------------------------------------------------------- host
@@ -412,10 +534,11 @@ int64_t bytes_of(int64_t rows, int64_t cols, bool precise) {
 }
 bool sides_ok(int64_t rows, int64_t cols) { return rows <= PK_MAX_MATRIX_SIDE && cols <= PK_MAX_MATRIX_SIDE; }
 
+constexpr int kRowsHalf = 256, kRowsPrecise = 128;      // of a workgroup's outputs
 template <int KIND>
 void launch_product(const Gemm& g, int units, bool precise, int id, hipStream_t s) {
-  if (precise) PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, true>), dim3(units), dim3(256), 0, s, g);
-  else PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, false>), dim3(units), dim3(256), 0, s, g);
+  if (precise) PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, true, kRowsPrecise, 32, 3>), dim3(units), dim3(512), 0, s, g);
+  else PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, false, kRowsHalf, 32, 4>), dim3(units), dim3(512), 0, s, g);
 }
 template <typename TG, bool STEP>
 int run_group(Ends& e, Gemm& sym, Gemm& upd, int chunks, int tiles, int sym_units, int upd_units, const Settings& o, hipStream_t s) {
@@ -477,13 +600,13 @@ int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspa
       x.rows = (int)it.rows; x.cols = (int)it.cols; x.count = (int)fit; x.mp = mp; x.np = np;
       x.first_chunk = (int)chunks; x.first_tile = (int)tiles;
       x.rate = it.rate;
-      const int64_t tm = mp / kPad, tn = np / kPad;
+      const int bm = it.precise ? kRowsPrecise : kRowsHalf;
       sym.e[e.n] = {used, each, mp, np, (int32_t)sym_units};
       upd.e[e.n] = {used, each, mp, np, (int32_t)upd_units};
       chunks += fit * pk_ceil_div(it.rows * it.cols, kChunk);
       tiles += fit * (mp / 64) * (np / 64);
-      sym_units += fit * tm * (tm + 1) / 2;
-      upd_units += fit * tm * tn;
+      sym_units += fit * (it.precise ? units_of_symmetric<kRowsPrecise>(mp) : units_of_symmetric<kRowsHalf>(mp));
+      upd_units += fit * pk_ceil_div(mp, bm) * pk_ceil_div(np, 256);
       used += fit * each;
       ++e.n;
       done += fit;
