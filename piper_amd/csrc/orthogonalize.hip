@@ -1,6 +1,6 @@
 // Newton-Schulz orthogonalization of matrices, and the optimizer step built on it.
 //
-//   X = U / max(|U|_F, eps);   `steps` times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
+//   X = U / max(|U|_F, eps);   `steps` times:  A = X X^T,  B = a + b A + c A A,  X <- B X
 //
 // An odd polynomial of X's singular values, applied again and again, which drives them towards 1 without computing them.  U [r, c]
 // is worked on with the shorter side as rows: X [m, n], m = min(r, c).  The step: m <- m + (1 - mu)(g - m), U = g + mu (m - g)
@@ -22,6 +22,7 @@
 // where a matrix ends.
 #include "pk_common.h"
 #include "lds_tiles.h"
+#include "launch_rules.h"
 #include <algorithm>
 #include <cmath>
 
@@ -63,9 +64,9 @@ struct Ends {
 };
 static_assert(sizeof(Ends) <= 4096, "kernel arguments");
 struct Gemm {
-  struct { int64_t ws, stride; int32_t mp, np, first_unit; } e[kMaxEntries];
+  struct Shape { int64_t ws, stride; int32_t mp, np, first_unit; } e[kMaxEntries];      // (first_unit: the number of matrices, until they are numbered)
   char* ws;
-  int32_t n;
+  int32_t n, units, chunk;
   int32_t from;          // which of the two X the products read
   float a, b, c;
 };
@@ -262,8 +263,9 @@ __host__ __device__ inline int units_of_symmetric(int mp) {
 
 // BM x 256 outputs of one product of one matrix (more rows and columns than there are: read from the last ones, not stored).
 //   GRAM    A = X X^T              rows of X against rows of X
-//   POLY    B = b A + c A A        A is symmetric: its rows against its rows
-//   UPDATE  X' = a X + B X         X comes as [k][columns] and through the transposing LDS read
+//   POLY    B = a + b A + c A A    A is symmetric: its rows against its rows
+//   UPDATE  X' = B X               X comes as [k][columns] and through the transposing LDS read
+// Single products of B and X's upper plane leave out B times its lower one; a times it is added, all of it that matters where A is small.
 // GRAM and POLY are symmetric: the 256 x 256 blocks on and below the diagonal are computed, those below it stored twice.
 // PRECISE: three products, lo hi + hi lo + hi hi, of both planes of a k-tile.  The matrix instructions cut what they add to a sum
 // off at its last bit instead of rounding it, which makes long sums of one sign too small (diagonals of 1,100 products by 8e-7, and
@@ -286,11 +288,13 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
-  const int en = entry_of(p.n, blockIdx.x, [&](int i) { return p.e[i].first_unit; });
+  const int unit = pk_rules::dealt_unit(blockIdx.x, p.chunk);      // neighbours share operands in an XCD's L2
+  if (unit >= p.units) return;
+  const int en = entry_of(p.n, unit, [&](int i) { return p.e[i].first_unit; });
   const int mp = p.e[en].mp, np = p.e[en].np;
   const int N = KIND == UPDATE ? np : mp;               // columns of the result
   const int tm = (mp + BM - 1) / BM, tn = (N + BN - 1) / BN;
-  const int local = blockIdx.x - p.e[en].first_unit;
+  const int local = unit - p.e[en].first_unit;
   int mat, mt, nt;
   if (KIND == UPDATE) {
     mat = local / (tm * tn);
@@ -429,9 +433,9 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
   const int ldc = N;
   const int64_t lower = to_lower(PRECISE, mp, ldc) * 2;       // bytes
   char* const out = KIND == GRAM ? A : KIND == POLY ? B : Xn;
-  const char* const old = KIND == POLY ? A : X;         // what a or b multiplies
+  const char* const old = KIND == POLY ? A : X;         // what b or a multiplies
   constexpr float unscale = KIND == GRAM ? kA / (kX * kX) : KIND == POLY ? 1.f / (kA * kA) : 1.f;
-  constexpr bool OLD_LO = KIND == UPDATE || (KIND == POLY && PRECISE), OUT_LO = KIND == UPDATE || PRECISE;
+  constexpr bool OLD_HI = KIND == POLY, OLD_LO = PRECISE ? KIND == POLY : KIND == UPDATE, OUT_LO = KIND == UPDATE || PRECISE;
   const bool mirrored = KIND != UPDATE && mt / (BN / BM) != nt;
   char* const buf = smem + wave * STAGING;
   const int lr = lane >> 3, lc = lane & 7;              // a lane's row (of 8 in a pass) and columns 8 lc ..
@@ -439,11 +443,11 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
   for (int i = 0; i < TM; ++i) {
     const int r0 = row0 + wm * WM + 32 * i, c0 = col0 + wn * 64;
     f16x8_t oh[4], ol[4];
-    if (KIND != GRAM) {
+    if (OLD_HI || OLD_LO) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const char* const at = old + place(PRECISE, r0 + 8 * q + lr, c0 + 8 * lc, ldc) * 2;
-        oh[q] = *reinterpret_cast<const f16x8_t*>(at);
+        if (OLD_HI) oh[q] = *reinterpret_cast<const f16x8_t*>(at);
         if (OLD_LO) ol[q] = *reinterpret_cast<const f16x8_t*>(at + lower);
       }
     }
@@ -472,9 +476,12 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (KIND != GRAM) {
+        if (KIND == POLY) {
           const float o = OLD_LO ? (float)oh[q][k] + (float)ol[q][k] : (float)oh[q][k];
-          x[k] = KIND == POLY ? p.b * (o * (1.f / kA)) + p.c * x[k] : p.a * o + x[k];
+          x[k] = p.b * (o * (1.f / kA)) + p.c * x[k];
+          if (r0 + row == c0 + 8 * lc + k) x[k] += p.a;
+        } else if (OLD_LO) {
+          x[k] += p.a * (float)ol[q][k];
         }
         h[q][k] = (f16_t)x[k];
         l[q][k] = (f16_t)(x[k] - (float)h[q][k]);
@@ -536,21 +543,34 @@ bool sides_ok(int64_t rows, int64_t cols) { return rows <= PK_MAX_MATRIX_SIDE &&
 
 constexpr int kRowsHalf = 256, kRowsPrecise = 128;      // of a workgroup's outputs
 template <int KIND>
-void launch_product(const Gemm& g, int units, bool precise, int id, hipStream_t s) {
-  if (precise) PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, true, kRowsPrecise, 32, 3>), dim3(units), dim3(512), 0, s, g);
-  else PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, false, kRowsHalf, 32, 4>), dim3(units), dim3(512), 0, s, g);
+void launch_product(const Gemm& g, bool precise, int id, hipStream_t s) {
+  if (precise) PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, true, kRowsPrecise, 32, 3>), dim3((unsigned)pk_rules::dealt_blocks(g.units, g.chunk)), dim3(512), 0, s, g);
+  else PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, false, kRowsHalf, 32, 4>), dim3((unsigned)pk_rules::dealt_blocks(g.units, g.chunk)), dim3(512), 0, s, g);
+}
+// Units of a launch: per(mp, np) of them for each matrix.
+template <typename F>
+int64_t number_units(Gemm& g, F&& per) {
+  int64_t at = 0;
+  for (int i = 0; i < g.n; ++i) {
+    const int64_t units = g.e[i].first_unit * (int64_t)per(g.e[i].mp, g.e[i].np);
+    g.e[i].first_unit = (int32_t)at;
+    at += units;
+  }
+  g.units = (int32_t)at;
+  g.chunk = (int32_t)pk_rules::deal_chunk(at, 32);
+  return at;
 }
 template <typename TG, bool STEP>
-int run_group(Ends& e, Gemm& sym, Gemm& upd, int chunks, int tiles, int sym_units, int upd_units, const Settings& o, hipStream_t s) {
+int run_group(Ends& e, Gemm& sym, Gemm& upd, int chunks, int tiles, const Settings& o, hipStream_t s) {
   const bool precise = e.precise != 0;
   PK_LAUNCH_NOCHECK(pk_timing::K_MUON_BEGIN, s, (begin_kernel<TG, STEP>), dim3(chunks), dim3(kThreads), 0, s, e);
   PK_LAUNCH_NOCHECK(pk_timing::K_MUON_CONVERT, s, (convert_kernel<TG, STEP>), dim3(tiles), dim3(kThreads), 0, s, e);
   int from = 0;
   for (int i = 0; i < o.steps; ++i) {
     sym.from = upd.from = from;
-    launch_product<GRAM>(sym, sym_units, precise, pk_timing::K_NS_GRAM, s);
-    launch_product<POLY>(sym, sym_units, precise, pk_timing::K_NS_POLY, s);
-    launch_product<UPDATE>(upd, upd_units, precise, pk_timing::K_NS_UPDATE, s);
+    launch_product<GRAM>(sym, precise, pk_timing::K_NS_GRAM, s);
+    launch_product<POLY>(sym, precise, pk_timing::K_NS_POLY, s);
+    launch_product<UPDATE>(upd, precise, pk_timing::K_NS_UPDATE, s);
     from = 1 - from;
   }
   PK_LAUNCH_NOCHECK(pk_timing::K_MUON_FINISH, s, (finish_kernel<TG, STEP>), dim3(tiles), dim3(kThreads), 0, s, e, from);
@@ -580,7 +600,7 @@ int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspa
     e.ws = sym.ws = upd.ws = static_cast<char*>(workspace);
     e.mu = o.mu; e.keep = o.keep; e.eps = o.eps; e.nesterov = o.nesterov; e.zero_flat = o.zero_flat;
     sym.a = upd.a = o.a; sym.b = upd.b = o.b; sym.c = upd.c = o.c;
-    int64_t used = 0, chunks = 0, tiles = 0, sym_units = 0, upd_units = 0;
+    int64_t used = 0, chunks = 0, tiles = 0;
     while (i < n && e.n < kMaxEntries) {
       const Item it = item(i);
       if (it.count == 0) { ++i; continue; }
@@ -600,25 +620,26 @@ int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspa
       x.rows = (int)it.rows; x.cols = (int)it.cols; x.count = (int)fit; x.mp = mp; x.np = np;
       x.first_chunk = (int)chunks; x.first_tile = (int)tiles;
       x.rate = it.rate;
-      const int bm = it.precise ? kRowsPrecise : kRowsHalf;
-      sym.e[e.n] = {used, each, mp, np, (int32_t)sym_units};
-      upd.e[e.n] = {used, each, mp, np, (int32_t)upd_units};
+      sym.e[e.n] = {used, each, mp, np, (int32_t)fit};
       chunks += fit * pk_ceil_div(it.rows * it.cols, kChunk);
       tiles += fit * (mp / 64) * (np / 64);
-      sym_units += fit * (it.precise ? units_of_symmetric<kRowsPrecise>(mp) : units_of_symmetric<kRowsHalf>(mp));
-      upd_units += fit * pk_ceil_div(mp, bm) * pk_ceil_div(np, 256);
       used += fit * each;
       ++e.n;
       done += fit;
       if (done == it.count) { ++i; done = 0; }
     }
     if (e.n == 0) break;
-    sym.n = upd.n = e.n;
-    if (std::max({chunks, tiles, sym_units, upd_units}) > 0x7fffffffll) return PK_ERR_SHAPE;
-    const int rc = o.step ? (o.bf16_src ? run_group<bf16_t, true>(e, sym, upd, (int)chunks, (int)tiles, (int)sym_units, (int)upd_units, o, s)
-                                        : run_group<float, true>(e, sym, upd, (int)chunks, (int)tiles, (int)sym_units, (int)upd_units, o, s))
-                          : (o.bf16_src ? run_group<bf16_t, false>(e, sym, upd, (int)chunks, (int)tiles, (int)sym_units, (int)upd_units, o, s)
-                                        : run_group<float, false>(e, sym, upd, (int)chunks, (int)tiles, (int)sym_units, (int)upd_units, o, s));
+    sym.n = e.n;
+    // long products first: what is left for the end is short
+    std::sort(sym.e, sym.e + e.n, [](const auto& x, const auto& y) { return (int64_t)x.mp * x.np > (int64_t)y.mp * y.np; });
+    upd = sym;
+    const int64_t sym_units = number_units(sym, [&](int mp, int) { return e.precise ? units_of_symmetric<kRowsPrecise>(mp) : units_of_symmetric<kRowsHalf>(mp); });
+    const int64_t upd_units = number_units(upd, [&](int mp, int np) { return pk_ceil_div(mp, e.precise ? kRowsPrecise : kRowsHalf) * pk_ceil_div(np, 256); });
+    if (std::max({chunks, tiles, sym_units, upd_units}) > 0x3fffffffll) return PK_ERR_SHAPE;
+    const int rc = o.step ? (o.bf16_src ? run_group<bf16_t, true>(e, sym, upd, (int)chunks, (int)tiles, o, s)
+                                        : run_group<float, true>(e, sym, upd, (int)chunks, (int)tiles, o, s))
+                          : (o.bf16_src ? run_group<bf16_t, false>(e, sym, upd, (int)chunks, (int)tiles, o, s)
+                                        : run_group<float, false>(e, sym, upd, (int)chunks, (int)tiles, o, s));
     if (rc != PK_OK) return rc;
   }
   return PK_OK;
