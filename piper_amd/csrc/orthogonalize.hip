@@ -66,7 +66,7 @@ static_assert(sizeof(Ends) <= 4096, "kernel arguments");
 struct Gemm {
   struct Shape { int64_t ws, stride; int32_t mp, np, first_unit; } e[kMaxEntries];      // (first_unit: the number of matrices, until they are numbered)
   char* ws;
-  int32_t n, units, chunk;
+  int32_t n, units, chunk, wide, splits;
   int32_t from;          // which of the two X the products read
   float a, b, c;
 };
@@ -251,33 +251,37 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const Ends p, int from
 
 // ---------------------------------------------------------------- the products
 enum Product { GRAM, POLY, UPDATE };
+enum Phase { WHOLE, PARTIAL, SUMS };
 
-// Row tiles (of BM) of the 256 x 256 blocks on and below the diagonal of a symmetric mp x mp result, block row by block row: a full
-// block row r has r + 1 blocks of 256 / BM tiles, the last one may be half a block high.
-template <int BM>
+// Row tiles (of BM) of the BN x BN blocks on and below the diagonal of a symmetric mp x mp result, block row by block row: a full
+// block row r has r + 1 blocks of BN / BM tiles, the last one may be half a block high.
+template <int BM, int BN>
 __host__ __device__ inline int units_of_symmetric(int mp) {
-  constexpr int R = 256 / BM;
+  constexpr int R = BN / BM;
   const int tm = (mp + BM - 1) / BM, whole = tm / R;
   return whole * (whole + 1) / 2 * R + (tm % R) * (whole + 1);
 }
 
-// BM x 256 outputs of one product of one matrix (more rows and columns than there are: read from the last ones, not stored).
+// BM x BN outputs of one product of one matrix (more rows and columns than there are: read from the last ones, not stored).
 //   GRAM    A = X X^T              rows of X against rows of X
 //   POLY    B = a + b A + c A A    A is symmetric: its rows against its rows
 //   UPDATE  X' = B X               X comes as [k][columns] and through the transposing LDS read
 // Single products of B and X's upper plane leave out B times its lower one; a times it is added, all of it that matters where A is small.
-// GRAM and POLY are symmetric: the 256 x 256 blocks on and below the diagonal are computed, those below it stored twice.
+// GRAM and POLY are symmetric: the BN x BN blocks on and below the diagonal are computed, those below it stored twice.
 // PRECISE: three products, lo hi + hi lo + hi hi, of both planes of a k-tile.  The matrix instructions cut what they add to a sum
 // off at its last bit instead of rounding it, which makes long sums of one sign too small (diagonals of 1,100 products by 8e-7, and
 // the result by ten times that): every 64 values of k the accumulators go into a second set by ordinary additions.
 //
-// Eight waves, (BM / 2) x 64 outputs each, in two groups half a k-tile apart, one wave of each on a SIMD: while one multiplies a k-tile
+// Eight waves, 64 columns of outputs each, in two groups half a k-tile apart, one wave of each on a SIMD: while one multiplies a k-tile
 // out of registers, the other reads its next k-tile's fragments from LDS and requests a later k-tile from memory; a barrier,
 // and they swap (the k-loop of the grouped products).  k-tiles go straight to LDS, NS - 1 of them ahead.  A k-tile has KT values of k; W
 // fp16 values of a row (both planes with PRECISE).
-template <int KIND, bool PRECISE, int BM, int KT, int NS>
+//
+// PHASE (GRAM with few units): PARTIAL leaves the sums of one of p.splits shares of k as they are in Xn, which nobody needs then, SUMS adds
+// them up in their order.
+template <int KIND, bool PRECISE, int BM, int BN, int KT, int NS, int PHASE = WHOLE>
 __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
-  constexpr int BN = 256, NW = 8, WM = BM / 2, TM = WM / 32, TN = 2, KS = KT / 16;
+  constexpr int NW = 8, WNW = BN / 64, WM = BM / (NW / WNW), TM = WM / 32, TN = 2, KS = KT / 16;
   constexpr int P = PRECISE ? 2 : 1, W = KT * P;
   constexpr int A_BYTES = BM * W * 2, STAGE = (BM + BN) * W * 2, LA = A_BYTES / (NW * 1024), LB = BN * W * 2 / (NW * 1024), L = LA + LB;
   constexpr int STAGING = 32 * 64 * 4;                  // of a wave: 32 rows of its outputs
@@ -287,24 +291,25 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
   __shared__ __attribute__((aligned(1024))) char smem[NS * STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 2, wn = wave & 3;
-  const int unit = pk_rules::dealt_unit(blockIdx.x, p.chunk);      // neighbours share operands in an XCD's L2
+  const int wm = wave / WNW, wn = wave % WNW;
+  const int dealt = pk_rules::dealt_unit(blockIdx.x, p.chunk);     // neighbours share operands in an XCD's L2
+  const int unit = PHASE == PARTIAL ? dealt / p.splits : dealt, split = PHASE == PARTIAL ? dealt % p.splits : 0;
   if (unit >= p.units) return;
   const int en = entry_of(p.n, unit, [&](int i) { return p.e[i].first_unit; });
   const int mp = p.e[en].mp, np = p.e[en].np;
   const int N = KIND == UPDATE ? np : mp;               // columns of the result
   const int tm = (mp + BM - 1) / BM, tn = (N + BN - 1) / BN;
   const int local = unit - p.e[en].first_unit;
-  int mat, mt, nt;
+  int mat, mt, nt, in_matrix = 0;
   if (KIND == UPDATE) {
     mat = local / (tm * tn);
     mt = local % (tm * tn) / tn;
     nt = local % (tm * tn) % tn;
   } else {
     constexpr int R = BN / BM;                          // row tiles of a 256 x 256 block
-    const int per = units_of_symmetric<BM>(mp);
+    const int per = units_of_symmetric<BM, BN>(mp);
     mat = local / per;
-    const int t = local % per;
+    const int t = in_matrix = local % per;
     nt = (int)((sqrtf(8.f * (t / R) + 1.f) - 1.f) * 0.5f);       // row of blocks, corrected, and the column in it
     while ((nt + 1) * (nt + 2) / 2 * R <= t) ++nt;
     while (nt * (nt + 1) / 2 * R > t) --nt;
@@ -321,7 +326,9 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
   const char* const left = KIND == GRAM ? X : KIND == POLY ? A : B;
   const char* const right = KIND == POLY ? A : X;
   const int lda = (KIND == GRAM ? np : mp) * P, ldb = (KIND == POLY ? mp : np) * P;      // of a row in memory
-  const int nkt = (KIND == GRAM ? np : mp) / KT;
+  const int pairs = (KIND == GRAM ? np : mp) / (2 * KT);         // of k-tiles: k is a multiple of 128
+  const int kt0 = PHASE == PARTIAL ? 2 * (pairs * split / p.splits) : 0;
+  const int nkt = PHASE == PARTIAL ? 2 * (pairs * (split + 1) / p.splits) - kt0 : 2 * pairs;
   const int row0 = mt * BM, col0 = nt * BN;
 
   // ---- the loader: a lane's byte offsets from two wave-uniform pointers that advance by a constant per k-tile
@@ -343,8 +350,8 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
       vb[i] = (uint32_t)(min(r, N - 1 - col0) * ldb + k) * 2u;
     }
   }
-  const char* ld_a = uniform_ptr(left + (int64_t)row0 * lda * 2);
-  const char* ld_b = uniform_ptr(right + (KIND == UPDATE ? (int64_t)col0 * P * 2 : (int64_t)col0 * ldb * 2));
+  const char* ld_a = uniform_ptr(left + (int64_t)row0 * lda * 2 + (int64_t)kt0 * W * 2);
+  const char* ld_b = uniform_ptr(right + (KIND == UPDATE ? (int64_t)col0 * P * 2 : (int64_t)col0 * ldb * 2 + (int64_t)kt0 * W * 2));
   const int64_t step_b = KIND == UPDATE ? (int64_t)KT * ldb * 2 : W * 2;
   auto request = [&](int stage) {
     const uint32_t to = lds_addr(smem) + stage * STAGE;
@@ -355,13 +362,17 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
   };
 
   floatx16_t acc[TM][TN] = {}, sum[PRECISE ? TM : 1][TN] = {};
+  const int grp = wave >> 2;
+  const bool live = row0 + wm * WM < mp && col0 + wn * 64 < N;
+  // where a split's sums are: [unit of the matrix][split][16 bytes of every lane in turn]
+  constexpr int VECS = TM * TN * 4;
+  floatx4_t* part = reinterpret_cast<floatx4_t*>(Xn) + ((int64_t)in_matrix * (PHASE == WHOLE ? 0 : p.splits) + split) * (VECS * 512) + wave * (VECS * 64) + lane;
+  if constexpr (PHASE != SUMS) {
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s)
     if (s < nkt) request(s);
   wait_tiles<L, NS - 2>(min(nkt, NS - 1) - 1);
   block_barrier();
-  const int grp = wave >> 2;
-  const bool live = row0 + wm * WM < mp && col0 + wn * 64 < N;
   if (grp == 1) block_barrier();
   int cur = 0;
   f16x8_t fa[P][KS][TM], fb[P][KS][TN];       // upper and lower plane
@@ -426,7 +437,35 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
     for (int kt = 0; kt < nkt; ++kt) k_tile(kt, std::false_type{});
   }
   if (grp == 0) block_barrier();        // the whole ring is free
+  }
   if (!live) return;
+  if constexpr (PHASE == PARTIAL) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          floatx4_t v;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * q + k] + (PRECISE ? sum[PRECISE ? i : 0][j][4 * q + k] : 0.f);
+          part[((i * TN + j) * 4 + q) * 64] = v;
+        }
+    return;
+  }
+  if constexpr (PHASE == SUMS) {
+    for (int z = 0; z < p.splits; ++z, part += VECS * 512)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const floatx4_t v = part[((i * TN + j) * 4 + q) * 64];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] += v[k];
+          }
+  }
 
   // ---- epilogue: 32 rows of a wave at a time through LDS, so that a lane has 8 neighbouring columns and memory is read and
   // written 16 bytes a lane.  acc[i][j][v] is row 32 i + lane % 32, column 32 j + 8 (v / 4) + 4 (lane / 32) + v % 4.
@@ -541,11 +580,56 @@ int64_t bytes_of(int64_t rows, int64_t cols, bool precise) {
 }
 bool sides_ok(int64_t rows, int64_t cols) { return rows <= PK_MAX_MATRIX_SIDE && cols <= PK_MAX_MATRIX_SIDE; }
 
-constexpr int kRowsHalf = 256, kRowsPrecise = 128;      // of a workgroup's outputs
+// The tiles: wide ones, 256 x 256 (single products) or 128 x 256, where a launch has this many of them, 128 x 128 otherwise.  us of the five
+// steps, wide -> narrow, X X^T and A A together / the update, with wide tiles of the former / the latter in brackets: 24 x 256 x 512, fp32,
+// 208 -> 173 / 92 -> 78 (48 / 96); 24 x 363 x 1000, bf16, 248 -> 145 / 122 -> 147 (72 / 192), fp32 347 -> 264 / 208 -> 229 (144 / 288); 2048 x 4096,
+// fp32, 1,027 -> 750 / 471 -> 590 (72 / 256), bf16 718 -> 349 / 285 -> 287 (36 / 128); 16 x 768 x 2048, fp32, 766 -> 784 / 690 -> 761 (192 / 768);
+// 64 x 512 x 512, fp32, 695 -> 602 / 346 -> 393 (384 / 512); 128 x 768 x 2048, bf16, 2,013 -> 2,052 / 2,542 -> 3,468 (384 / 1,536 in each of two
+// groups), fp32 4,785 -> 5,062 / 4,941 -> 5,903 (624 / 2,496).  (Half of a wide tile on the diagonal is of no use.)
+constexpr int64_t kWideSymmetric = 512, kWideUpdate = 160;
+constexpr int kWideRows[2] = {256, 128};               // [precise]
 template <int KIND>
 void launch_product(const Gemm& g, bool precise, int id, hipStream_t s) {
-  if (precise) PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, true, kRowsPrecise, 32, 3>), dim3((unsigned)pk_rules::dealt_blocks(g.units, g.chunk)), dim3(512), 0, s, g);
-  else PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, false, kRowsHalf, 32, 4>), dim3((unsigned)pk_rules::dealt_blocks(g.units, g.chunk)), dim3(512), 0, s, g);
+  const dim3 grid((unsigned)pk_rules::dealt_blocks(g.units, g.chunk)), block(512);
+#define PK_LAUNCH(...) PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, __VA_ARGS__>), grid, block, 0, s, g)
+  if (g.wide) { if (precise) PK_LAUNCH(true, 128, 256, 32, 3); else PK_LAUNCH(false, 256, 256, 32, 4); }
+  else if (precise) PK_LAUNCH(true, 128, 128, 32, 4);
+  else PK_LAUNCH(false, 128, 128, 64, 4);
+#undef PK_LAUNCH
+}
+void launch_gram(const Gemm& g, bool precise, hipStream_t s) {
+  if (g.splits == 1) return launch_product<GRAM>(g, precise, pk_timing::K_NS_GRAM, s);
+  Gemm shares = g;
+  shares.chunk = (int32_t)pk_rules::deal_chunk((int64_t)g.units * g.splits, 32);
+  const dim3 grid((unsigned)pk_rules::dealt_blocks((int64_t)g.units * g.splits, shares.chunk)), sums((unsigned)pk_rules::dealt_blocks(g.units, g.chunk)), block(512);
+  const int id = pk_timing::K_NS_GRAM;
+  if (precise) {
+    PK_LAUNCH_NOCHECK(id, s, (product_kernel<GRAM, true, 128, 128, 32, 4, PARTIAL>), grid, block, 0, s, shares);
+    PK_LAUNCH_NOCHECK(id, s, (product_kernel<GRAM, true, 128, 128, 32, 4, SUMS>), sums, block, 0, s, g);
+  } else {
+    PK_LAUNCH_NOCHECK(id, s, (product_kernel<GRAM, false, 128, 128, 64, 4, PARTIAL>), grid, block, 0, s, shares);
+    PK_LAUNCH_NOCHECK(id, s, (product_kernel<GRAM, false, 128, 128, 64, 4, SUMS>), sums, block, 0, s, g);
+  }
+}
+int64_t wide_symmetric(bool precise, int mp) { return precise ? units_of_symmetric<128, 256>(mp) : units_of_symmetric<256, 256>(mp); }
+int64_t wide_update(bool precise, int mp, int np) { return pk_ceil_div(mp, kWideRows[precise]) * pk_ceil_div(np, 256); }
+template <typename F>
+int64_t count_units(const Gemm& g, F&& per) {
+  int64_t units = 0;
+  for (int i = 0; i < g.n; ++i) units += g.e[i].first_unit * (int64_t)per(g.e[i].mp, g.e[i].np);
+  return units;
+}
+// Shares of k that X X^T is cut into: as many as fit Xn and give every CU a unit, of eight k-tiles of 32 at least, where they save
+// sixteen or more.
+int gram_splits(const Gemm& g, int64_t units) {
+  int64_t splits = 256 / std::max<int64_t>(units, 1), longest = 0;
+  for (int i = 0; i < g.n; ++i) {
+    const Gemm::Shape& e = g.e[i];
+    splits = std::min(splits, 2 * plane_x(e.mp, e.np) / (units_of_symmetric<128, 128>(e.mp) * (int64_t)(128 * 128 * 4)));
+    splits = std::min<int64_t>(splits, e.np / 256);
+    longest = std::max<int64_t>(longest, e.np / 32);
+  }
+  return splits < 2 || longest - longest / splits < 16 ? 1 : (int)splits;
 }
 // Units of a launch: per(mp, np) of them for each matrix.
 template <typename F>
@@ -568,7 +652,7 @@ int run_group(Ends& e, Gemm& sym, Gemm& upd, int chunks, int tiles, const Settin
   int from = 0;
   for (int i = 0; i < o.steps; ++i) {
     sym.from = upd.from = from;
-    launch_product<GRAM>(sym, precise, pk_timing::K_NS_GRAM, s);
+    launch_gram(sym, precise, s);
     launch_product<POLY>(sym, precise, pk_timing::K_NS_POLY, s);
     launch_product<UPDATE>(upd, precise, pk_timing::K_NS_UPDATE, s);
     from = 1 - from;
@@ -633,8 +717,12 @@ int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspa
     // long products first: what is left for the end is short
     std::sort(sym.e, sym.e + e.n, [](const auto& x, const auto& y) { return (int64_t)x.mp * x.np > (int64_t)y.mp * y.np; });
     upd = sym;
-    const int64_t sym_units = number_units(sym, [&](int mp, int) { return e.precise ? units_of_symmetric<kRowsPrecise>(mp) : units_of_symmetric<kRowsHalf>(mp); });
-    const int64_t upd_units = number_units(upd, [&](int mp, int np) { return pk_ceil_div(mp, e.precise ? kRowsPrecise : kRowsHalf) * pk_ceil_div(np, 256); });
+    const bool precise = e.precise != 0;
+    sym.wide = count_units(sym, [&](int mp, int) { return wide_symmetric(precise, mp); }) >= kWideSymmetric;
+    upd.wide = count_units(upd, [&](int mp, int np) { return wide_update(precise, mp, np); }) >= kWideUpdate;
+    sym.splits = sym.wide ? 1 : gram_splits(sym, count_units(sym, [](int mp, int) { return units_of_symmetric<128, 128>(mp); }));
+    const int64_t sym_units = number_units(sym, [&](int mp, int) { return sym.wide ? wide_symmetric(precise, mp) : units_of_symmetric<128, 128>(mp); });
+    const int64_t upd_units = number_units(upd, [&](int mp, int np) { return upd.wide ? wide_update(precise, mp, np) : (int64_t)(mp / 128) * (np / 128); });
     if (std::max({chunks, tiles, sym_units, upd_units}) > 0x3fffffffll) return PK_ERR_SHAPE;
     const int rc = o.step ? (o.bf16_src ? run_group<bf16_t, true>(e, sym, upd, (int)chunks, (int)tiles, o, s)
                                         : run_group<float, true>(e, sym, upd, (int)chunks, (int)tiles, o, s))
