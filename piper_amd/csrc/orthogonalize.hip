@@ -106,15 +106,68 @@ __device__ __forceinline__ int entry_of(int n, int block, F&& first) {
 }
 
 // ---------------------------------------------------------------- the ends
-// The gradient of element i of an entry; the momentum after this step and U, from the momentum before.
-template <typename TG>
-__device__ __forceinline__ float gradient(const Entry& e, int64_t i) {
-  float g = e.flat ? e.flat[i] : 0.f;
-  if (e.src) g += pk_to_float<TG>(reinterpret_cast<const TG*>(e.src)[i]);
-  return g;
+// N neighbouring values at p as fp32; VEC: p is on a boundary of their size.
+template <int N, bool VEC, typename T>
+__device__ __forceinline__ void load_n(const T* p, float (&x)[N]) {
+  typedef T vec_t __attribute__((ext_vector_type(VEC ? (sizeof(T) == 2 ? N : 4) : 1)));
+  constexpr int PER = VEC ? (sizeof(T) == 2 ? N : 4) : 1;
+#pragma unroll
+  for (int v = 0; v < N / PER; ++v) {
+    const vec_t t = reinterpret_cast<const vec_t*>(p)[v];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) x[v * PER + k] = (float)t[k];
+  }
+}
+template <int N, bool VEC, typename T>
+__device__ __forceinline__ void store_n(T* p, const float (&x)[N]) {
+  typedef T vec_t __attribute__((ext_vector_type(VEC ? (sizeof(T) == 2 ? N : 4) : 1)));
+  constexpr int PER = VEC ? (sizeof(T) == 2 ? N : 4) : 1;
+#pragma unroll
+  for (int v = 0; v < N / PER; ++v) {
+    vec_t t;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) t[k] = (T)x[v * PER + k];
+    reinterpret_cast<vec_t*>(p)[v] = t;
+  }
+}
+// Whether every buffer of an entry has 16-byte boundaries where a multiple of `piece` elements begins in a matrix.
+__device__ __forceinline__ bool aligned(const Entry& e, int piece) {
+  return ((reinterpret_cast<uintptr_t>(e.src) | reinterpret_cast<uintptr_t>(e.flat) | reinterpret_cast<uintptr_t>(e.momentum) |
+           reinterpret_cast<uintptr_t>(e.master) | reinterpret_cast<uintptr_t>(e.out)) & 15u) == 0 && piece;
+}
+// The gradients of elements i .. i + N - 1 of an entry; the momentum after this step and U, from the momentum before.
+template <int N, bool VEC, typename TG>
+__device__ __forceinline__ void gradient(const Entry& e, int64_t i, float (&g)[N]) {
+  float f[N] = {};
+#pragma unroll
+  for (int k = 0; k < N; ++k) g[k] = 0.f;
+  if (e.flat) load_n<N, VEC>(e.flat + i, f);
+  if (e.src) load_n<N, VEC>(reinterpret_cast<const TG*>(e.src) + i, g);
+  if (e.flat) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) g[k] = f[k] + g[k];
+  }
 }
 __device__ __forceinline__ float next_momentum(float m, float g, float mu) { return m + (1.f - mu) * (g - m); }
 __device__ __forceinline__ float update_of(float m, float g, float mu, bool nesterov) { return nesterov ? g + mu * (m - g) : m; }
+
+template <int N, bool VEC, typename TG, bool STEP>
+__device__ __forceinline__ void begin_piece(const Ends& p, const Entry& e, int64_t i, double& sum) {
+  float u[N];
+  gradient<N, VEC, TG>(e, i, u);
+  if (STEP) {
+    float m[N];
+    load_n<N, VEC>(e.momentum + i, m);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      m[k] = next_momentum(m[k], u[k], p.mu);
+      u[k] = update_of(m[k], u[k], p.mu, p.nesterov);
+    }
+    store_n<N, VEC>(e.momentum + i, m);
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) sum += (double)u[k] * u[k];
+}
 
 // Momentum, and the sum of squares of every chunk of a matrix of U, in 64 bits (squares of fp32 values reach past fp32's range).
 template <typename TG, bool STEP>
@@ -128,15 +181,11 @@ __global__ __launch_bounds__(kThreads) void begin_kernel(const Ends p) {
   const int64_t base = (int64_t)mat * size + (int64_t)chunk * kChunk;
   const int n = (int)min((int64_t)kChunk, size - (int64_t)chunk * kChunk);
   double sum = 0.0;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const float g = gradient<TG>(e, base + i);
-    float u = g;
-    if (STEP) {
-      const float m = next_momentum(e.momentum[base + i], g, p.mu);
-      e.momentum[base + i] = m;
-      u = update_of(m, g, p.mu, p.nesterov);
-    }
-    sum += (double)u * u;
+  if (n == kChunk && aligned(e, size % 8 == 0)) {
+#pragma unroll
+    for (int i = 0; i < kChunk / (kThreads * 8); ++i) begin_piece<8, true, TG, STEP>(p, e, base + (i * kThreads + threadIdx.x) * 8, sum);
+  } else {
+    for (int i = threadIdx.x; i < n; i += kThreads) begin_piece<1, false, TG, STEP>(p, e, base + i, sum);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
@@ -155,12 +204,28 @@ struct Tile {            // 64 x 64 of a matrix's padded X
   int mat, i0, j0;
   bool tall;
   char* mem;
+  int row0, col0;        // the same in the matrix itself, turned where that is taller than wide
+  int64_t base;          // elements to the matrix
+  bool whole;            // four neighbours at a time: no end of a row inside, 16-byte boundaries
 };
 __device__ __forceinline__ Tile tile_of(const Ends& p, int block) {
   const Entry& e = p.e[entry_of(p.n, block, [&](int i) { return p.e[i].first_tile; })];
   const int tm = e.mp / 64, tn = e.np / 64, local = block - e.first_tile;
   const int mat = local / (tm * tn), t = local % (tm * tn);
-  return Tile{e, mat, t / tn * 64, t % tn * 64, e.rows > e.cols, p.ws + e.ws + mat * matrix_bytes(e.rows, e.cols, e.mp, e.np, p.precise)};
+  const bool tall = e.rows > e.cols;
+  const int i0 = t / tn * 64, j0 = t % tn * 64;
+  return Tile{e, mat, i0, j0, tall, p.ws + e.ws + mat * matrix_bytes(e.rows, e.cols, e.mp, e.np, p.precise), tall ? j0 : i0, tall ? i0 : j0,
+              (int64_t)mat * e.rows * e.cols, aligned(e, e.cols % 4 == 0)};
+}
+// f(row in the tile, first of four columns in it, its element, whether all four are there as a vector) for this thread's share of a tile in the
+// matrix's own order
+template <typename F>
+__device__ __forceinline__ void for_pieces(const Tile& t, F&& f) {
+#pragma unroll
+  for (int it = 0; it < 64 * 16 / kThreads; ++it) {
+    const int q = it * kThreads + threadIdx.x, r = q >> 4, c = (q & 15) * 4;
+    f(r, c, t.base + (int64_t)(t.row0 + r) * t.e.cols + t.col0 + c, t.row0 + r < t.e.rows ? min(4, t.e.cols - t.col0 - c) : 0);
+  }
 }
 
 // X = U / max(|U|, eps) in two planes, its longer side along the rows in memory, zeros around it.
@@ -176,41 +241,71 @@ __global__ __launch_bounds__(kThreads) void convert_kernel(const Ends p) {
   const double* sums = reinterpret_cast<const double*>(t.mem + at_sums(e.mp, e.np, p.precise));
   double sum = 0.0;
   for (int i = tid; i < chunks; i += kThreads) sum += sums[i];
+  float u[4][4];
+  int it = 0;
+  const auto piece = [&](int64_t i, int n, float (&x)[4]) {
+    if (t.whole && n == 4) {
+      gradient<4, true, TG>(e, i, x);
+      if (STEP) {
+        float m[4];
+        load_n<4, true>(e.momentum + i, m);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = update_of(m[k], x[k], p.mu, p.nesterov);
+        const float zero[4] = {};
+        if (p.zero_flat && e.flat) store_n<4, true>(e.flat + i, zero);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k] = 0.f;
+        if (k < n) {
+          float g[1];
+          gradient<1, false, TG>(e, i + k, g);
+          x[k] = STEP ? update_of(e.momentum[i + k], g[0], p.mu, p.nesterov) : g[0];
+          if (STEP && p.zero_flat && e.flat) e.flat[i + k] = 0.f;
+        }
+      }
+    }
+  };
+  for_pieces(t, [&](int, int, int64_t i, int n) { piece(i, n, u[it++]); });
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
   if ((tid & 63) == 0) part[tid >> 6] = sum;
   __syncthreads();
   const double norm = sqrt(part[0] + part[1] + part[2] + part[3]);
   const double factor = (double)kX / (norm < (double)p.eps ? (double)p.eps : norm);   // (NaN stays)
-  const int64_t base = (int64_t)t.mat * size;
+  // in two steps of fp32, the first one a power of two: the quotient may be far outside its range, and so may U
+  const int half = factor > 0.0 ? ilogb(factor) / 2 : 0;
+  const float f1 = ldexpf(1.f, half), f2 = (float)ldexp(factor, -half);
   f16_t* const hi = reinterpret_cast<f16_t*>(t.mem);
   f16_t* const lo = hi + to_lower(p.precise, e.mp, e.np);
-  const int r0 = t.tall ? t.j0 : t.i0, c0 = t.tall ? t.i0 : t.j0;
-  for (int q = tid; q < 64 * 64; q += kThreads) {
-    const int r = r0 + (q >> 6), c = c0 + (q & 63);
-    float x = 0.f;
-    if (r < e.rows && c < e.cols) {
-      const int64_t i = base + (int64_t)r * e.cols + c;
-      const float g = gradient<TG>(e, i);
-      const float u = STEP ? update_of(e.momentum[i], g, p.mu, p.nesterov) : g;
-      if (STEP && p.zero_flat && e.flat) e.flat[i] = 0.f;
-      x = (float)((double)u * factor);
-    }
-    turned[q >> 6][q & 63] = x;
-  }
-  __syncthreads();
-  for (int q = tid; q < 64 * 16; q += kThreads) {
-    const int i = q >> 4, j = (q & 15) * 4;
+  const auto put = [&](int i, int j, const float (&x)[4]) {
     f16x4_t h, l;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-      const float x = t.tall ? turned[j + v][i] : turned[i][j + v];
-      h[v] = (f16_t)x;
-      l[v] = (f16_t)(x - (float)h[v]);
+      h[v] = (f16_t)x[v];
+      l[v] = (f16_t)(x[v] - (float)h[v]);
     }
     const int64_t at = place(p.precise, t.i0 + i, t.j0 + j, e.np);
     *reinterpret_cast<f16x4_t*>(hi + at) = h;
     *reinterpret_cast<f16x4_t*>(lo + at) = l;
+  };
+  it = 0;
+  for_pieces(t, [&](int r, int c, int64_t, int) {
+    float x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = u[it][k] * f1 * f2;
+    ++it;
+    if (!t.tall) return put(r, c, x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) turned[r][c + k] = x[k];
+  });
+  if (!t.tall) return;
+  __syncthreads();
+  for (int q = tid; q < 64 * 16; q += kThreads) {
+    const int i = q >> 4, j = (q & 15) * 4;
+    const float x[4] = {turned[j][i], turned[j + 1][i], turned[j + 2][i], turned[j + 3][i]};
+    put(i, j, x);
   }
 }
 
@@ -221,32 +316,58 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const Ends p, int from
   const Tile t = tile_of(p, blockIdx.x);
   const Entry& e = t.e;
   const int tid = threadIdx.x;
-  const int64_t size = (int64_t)e.rows * e.cols;
   const f16_t* const hi = reinterpret_cast<const f16_t*>(t.mem + 2 * from * plane_x(e.mp, e.np));
   const f16_t* const lo = hi + to_lower(p.precise, e.mp, e.np);
-  for (int q = tid; q < 64 * 16; q += kThreads) {
-    const int i = q >> 4, j = (q & 15) * 4;
+  const auto get = [&](int i, int j, float (&x)[4]) {
     const int64_t at = place(p.precise, t.i0 + i, t.j0 + j, e.np);
     const f16x4_t h = *reinterpret_cast<const f16x4_t*>(hi + at), l = *reinterpret_cast<const f16x4_t*>(lo + at);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) (t.tall ? turned[j + v][i] : turned[i][j + v]) = ((float)h[v] + (float)l[v]) * (1.f / kX);
-  }
-  __syncthreads();
-  const int r0 = t.tall ? t.j0 : t.i0, c0 = t.tall ? t.i0 : t.j0;
-  const int64_t base = (int64_t)t.mat * size;
-  for (int q = tid; q < 64 * 64; q += kThreads) {
-    const int r = r0 + (q >> 6), c = c0 + (q & 63);
-    if (r >= e.rows || c >= e.cols) continue;
-    const int64_t i = base + (int64_t)r * e.cols + c;
-    const float o = turned[q >> 6][q & 63];
-    if (STEP) {
-      const float w = e.master[i] * p.keep - e.rate * o;
-      e.master[i] = w;
-      if (e.out) reinterpret_cast<bf16_t*>(e.out)[i] = (bf16_t)w;
-    } else {
-      reinterpret_cast<TG*>(e.out)[i] = pk_from_float<TG>(o);
+    for (int v = 0; v < 4; ++v) x[v] = ((float)h[v] + (float)l[v]) * (1.f / kX);
+  };
+  if (t.tall) {
+    for (int q = tid; q < 64 * 16; q += kThreads) {
+      const int i = q >> 4, j = (q & 15) * 4;
+      float x[4];
+      get(i, j, x);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) turned[j + v][i] = x[v];
     }
+    __syncthreads();
   }
+  for_pieces(t, [&](int r, int c, int64_t i, int n) {
+    if (n <= 0) return;
+    float o[4];
+    if (t.tall) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = turned[r][c + k];
+    } else {
+      get(r, c, o);
+    }
+    if (t.whole && n == 4) {
+      if (STEP) {
+        float w[4];
+        load_n<4, true>(e.master + i, w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = w[k] * p.keep - e.rate * o[k];
+        store_n<4, true>(e.master + i, w);
+        if (e.out) store_n<4, true>(reinterpret_cast<bf16_t*>(e.out) + i, w);
+      } else {
+        store_n<4, true>(reinterpret_cast<TG*>(e.out) + i, o);
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k >= n) continue;
+      if (STEP) {
+        const float w = e.master[i + k] * p.keep - e.rate * o[k];
+        e.master[i + k] = w;
+        if (e.out) reinterpret_cast<bf16_t*>(e.out)[i + k] = (bf16_t)w;
+      } else {
+        reinterpret_cast<TG*>(e.out)[i + k] = pk_from_float<TG>(o[k]);
+      }
+    }
+  });
 }
 
 // ---------------------------------------------------------------- the products
