@@ -16,13 +16,14 @@ using namespace pk_balance;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kChunk = 64, kMostChunks = 512;       // tokens of a chunk: a multiple of kChunk that leaves about kMostChunks of them
 
-// A token's logits lie on LPT lanes, EPL to a lane, 64 / LPT tokens to a wave: expert j * LPT + lane % LPT.
+// A token's logits lie on LPT lanes, EPL to a lane, 64 / LPT tokens to a wave: lane g of a token has the pieces of four neighbouring
+// experts g, g + LPT, ..
 template <int LPT>
 __device__ __forceinline__ float group_sum(float v) {
 #define PK_STEP(CTRL) v += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true))
-  PK_STEP(0xb1);                       // quad_perm 1 0 3 2
-  PK_STEP(0x4e);                       // quad_perm 2 3 0 1
-  PK_STEP(0x141);                      // row_half_mirror: the other quad of 8 lanes
+  if (LPT > 1) PK_STEP(0xb1);          // quad_perm 1 0 3 2
+  if (LPT > 2) PK_STEP(0x4e);          // quad_perm 2 3 0 1
+  if (LPT > 4) PK_STEP(0x141);         // row_half_mirror: the other quad of 8 lanes
   if (LPT > 8) PK_STEP(0x140);         // row_mirror: the other 8 of a row of 16
 #undef PK_STEP
   const auto add = [](auto r) { return __uint_as_float(r[0]) + __uint_as_float(r[1]); };
@@ -33,9 +34,9 @@ __device__ __forceinline__ float group_sum(float v) {
 template <int LPT>
 __device__ __forceinline__ float group_max(float v) {
 #define PK_STEP(CTRL) v = fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true)))
-  PK_STEP(0xb1);
-  PK_STEP(0x4e);
-  PK_STEP(0x141);
+  if (LPT > 1) PK_STEP(0xb1);
+  if (LPT > 2) PK_STEP(0x4e);
+  if (LPT > 4) PK_STEP(0x141);
   if (LPT > 8) PK_STEP(0x140);
 #undef PK_STEP
   const auto most = [](auto r) { return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])); };
@@ -43,11 +44,24 @@ __device__ __forceinline__ float group_max(float v) {
   if (LPT > 32) v = most(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
   return v;
 }
+template <int LPT>
+__device__ __forceinline__ int expert_of(int j, int g) { return ((j >> 2) * LPT + g) * 4 + (j & 3); }
 
-template <int LPT, int EPL>
-__device__ __forceinline__ void load_logits(const float* __restrict__ logits, int64_t t, bool live, int E, int g, float (&x)[EPL]) {
+// VEC: rows are whole 16-byte pieces on their boundaries
+template <int LPT, int EPL, bool VEC>
+__device__ __forceinline__ void load_row(const float* __restrict__ row, bool live, int E, int g, float absent, float (&x)[EPL]) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) x[j] = live && j * LPT + g < E ? logits[t * E + j * LPT + g] : -INFINITY;
+  for (int j = 0; j < EPL; j += 4) {
+    const int e = expert_of<LPT>(j, g);
+    if (VEC) {
+      const floatx4_t v = live && e < E ? *reinterpret_cast<const floatx4_t*>(row + e) : floatx4_t{absent, absent, absent, absent};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[j + k] = v[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[j + k] = live && e + k < E ? row[e + k] : absent;
+    }
+  }
 }
 // x becomes the softmax; returns log(sum exp)
 template <int LPT, int EPL>
@@ -59,7 +73,7 @@ __device__ __forceinline__ float softmax(float (&x)[EPL], int E, int g) {
   float total = 0.f;
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
-    x[j] = j * LPT + g < E ? expf(x[j] - mx) : 0.f;
+    x[j] = expert_of<LPT>(j, g) < E ? expf(x[j] - mx) : 0.f;
     total += x[j];
   }
   total = group_sum<LPT>(total);
@@ -99,7 +113,7 @@ __device__ __forceinline__ int count_of(int n, int* box, F&& holds) {
   return c;
 }
 
-template <int LPT, int EPL>
+template <int LPT, int EPL, bool VEC>
 __global__ __launch_bounds__(kThreads) void balance_partial_kernel(const Forward p) {
   constexpr int EM = LPT * EPL, TPW = 64 / LPT;
   __shared__ float sum_p[kWaves][EM];
@@ -113,7 +127,15 @@ __global__ __launch_bounds__(kThreads) void balance_partial_kernel(const Forward
   const int b = begin_of(p.sequences, s, p.T), e = end_of(p.sequences, s, p.T);
   const int first = b + (unit - (b / p.chunk + s)) * p.chunk, n = min(p.chunk, e - first);
   if (n <= 0) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane % LPT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane % LPT, slot = lane / LPT;
+  // a step's logits are on their way while those of the step before are worked on
+  const float* const logits = p.logits + (int64_t)first * p.E;
+  float next[EPL];
+  const auto request = [&](int i) {
+    const int t = i + slot;
+    load_row<LPT, EPL, VEC>(logits + (int64_t)min(t, n - 1) * p.E, t < n, p.E, g, -INFINITY, next);
+  };
+  request(wave * TPW);
   for (int i = tid; i < EM; i += kThreads) hist[i] = 0;
   __syncthreads();
   for (int i = tid; i < n * p.K; i += kThreads) {
@@ -122,12 +144,12 @@ __global__ __launch_bounds__(kThreads) void balance_partial_kernel(const Forward
   }
   float sum[EPL] = {}, z = 0.f;
   for (int i = wave * TPW; i < n; i += kWaves * TPW) {
-    const int t = i + lane / LPT;
-    const bool live = t < n;
     float x[EPL];
-    load_logits<LPT, EPL>(p.logits, first + t, live, p.E, g, x);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) x[j] = next[j];
+    request(i + kWaves * TPW);
     const float lse = softmax<LPT, EPL>(x, p.E, g);
-    if (live) {
+    if (i + slot < n) {
 #pragma unroll
       for (int j = 0; j < EPL; ++j) sum[j] += x[j];
       z += lse * lse;
@@ -141,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void balance_partial_kernel(const Forward
   }
   if (lane < LPT) {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) sum_p[wave][j * LPT + g] = sum[j];
+    for (int j = 0; j < EPL; ++j) sum_p[wave][expert_of<LPT>(j, g)] = sum[j];
   }
   if (lane == 0) sum_z[wave] = z;
   __syncthreads();
@@ -236,49 +258,73 @@ __global__ __launch_bounds__(kMostSum) void balance_sum_kernel(const Forward p) 
   }
 }
 
-template <int LPT, int EPL>
-__global__ __launch_bounds__(kThreads) void balance_bwd_kernel(const float* __restrict__ logits, const Grad gr, int T, int E, int tokens,
+// A wave takes `steps` times 64 / LPT neighbouring tokens.
+template <int LPT, int EPL, bool VEC>
+__global__ __launch_bounds__(kThreads) void balance_bwd_kernel(const float* __restrict__ logits, const Grad gr, int T, int E, int steps,
                                                                float* __restrict__ d_logits) {
   constexpr int TPW = 64 / LPT;
   __shared__ int box[kWaves];
-  const int first = blockIdx.x * tokens, n = min(tokens, T - first);
-  const int s0 = gr.sequences ? max(count_of(gr.S + 1, box, [&](int i) { return gr.sequences[i] <= first; }) - 1, 0) : 0;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane % LPT;
+  const int block0 = blockIdx.x * kWaves * steps * TPW;
+  const int t0 = block0 + wave * steps * TPW + lane / LPT;
+  float next[EPL];
+  const auto request = [&](int t) { load_row<LPT, EPL, VEC>(logits + (int64_t)min(t, T - 1) * E, true, E, g, -INFINITY, next); };
+  request(t0);
   const float per = gr.table[(int64_t)gr.S * E], slope_z = gr.table[(int64_t)gr.S * E + 1], d_loss = *gr.d_loss;
-  int s = s0;
-  for (int i = wave * TPW; i < n; i += kWaves * TPW) {
-    const int t = i + lane / LPT;
-    if (t >= n) continue;
+  // (the workgroup's first token's sequence: the offsets up to it, less one)
+  int s = gr.sequences ? max(count_of(gr.S + 1, box, [&](int i) { return gr.sequences[i] <= block0; }) - 1, 0) : 0;
+  int of_h = -2;                      // whose table row h is
+  float h[EPL];
+  for (int i = 0; i < steps; ++i) {
+    const int t = t0 + i * TPW;
+    if (t >= T) break;                // (a token's lanes together)
     float x[EPL];
-    load_logits<LPT, EPL>(logits, first + t, true, E, g, x);
-    s = sequence_of(gr, max(s, 0), first + t);
-    const bool owned = s >= 0 && s < gr.S;
-    float h[EPL];
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) h[j] = owned && j * LPT + g < E ? gr.table[(int64_t)s * E + j * LPT + g] : 0.f;
+    for (int j = 0; j < EPL; ++j) x[j] = next[j];
+    if (i + 1 < steps) request(t + TPW);
+    s = sequence_of(gr, max(s, 0), t);
+    const bool owned = s >= 0 && s < gr.S;
+    if (s != of_h) {
+      load_row<LPT, EPL, VEC>(gr.table + (int64_t)(owned ? s : 0) * E, owned, E, g, 0.f, h);
+      of_h = s;
+    }
     const float lse = softmax<LPT, EPL>(x, E, g);
     float mean = 0.f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) mean += h[j] * x[j];
     mean = group_sum<LPT>(mean);
+    const float at_h = owned ? d_loss * per : 0.f, at_lse = owned ? d_loss * slope_z * lse : 0.f;
+    float* const to = d_logits + (int64_t)t * E;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j)
-      if (j * LPT + g < E)
-        d_logits[(int64_t)(first + t) * E + j * LPT + g] = owned ? d_loss * x[j] * (per * (h[j] - mean) + slope_z * lse) : 0.f;
+    for (int j = 0; j < EPL; j += 4) {
+      floatx4_t d;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[k] = owned ? x[j + k] * (at_h * (h[j + k] - mean) + at_lse) : 0.f;
+      const int e = expert_of<LPT>(j, g);
+      if (VEC) {
+        if (e < E) *reinterpret_cast<floatx4_t*>(to + e) = d;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (e + k < E) to[e + k] = d[k];
+      }
+    }
   }
 }
 
-#define PK_BALANCE_DISPATCH(E, LAUNCH)         \
-  do {                                         \
-    if ((E) <= 8) { LAUNCH(8, 1); }            \
-    else if ((E) <= 16) { LAUNCH(16, 1); }     \
-    else if ((E) <= 32) { LAUNCH(32, 1); }     \
-    else if ((E) <= 64) { LAUNCH(64, 1); }     \
-    else if ((E) <= 128) { LAUNCH(64, 2); }    \
-    else if ((E) <= 256) { LAUNCH(64, 4); }    \
-    else if ((E) <= 512) { LAUNCH(64, 8); }    \
-    else { LAUNCH(64, 16); }                   \
+#define PK_BALANCE_DISPATCH(E, vec, LAUNCH)                                                  \
+  do {                                                                                       \
+    if ((E) <= 8) { if (vec) LAUNCH(2, 4, true); else LAUNCH(2, 4, false); }                 \
+    else if ((E) <= 16) { if (vec) LAUNCH(4, 4, true); else LAUNCH(4, 4, false); }           \
+    else if ((E) <= 32) { if (vec) LAUNCH(8, 4, true); else LAUNCH(8, 4, false); }           \
+    else if ((E) <= 64) { if (vec) LAUNCH(16, 4, true); else LAUNCH(16, 4, false); }         \
+    else if ((E) <= 128) { if (vec) LAUNCH(16, 8, true); else LAUNCH(16, 8, false); }        \
+    else if ((E) <= 256) { if (vec) LAUNCH(32, 8, true); else LAUNCH(32, 8, false); }        \
+    else if ((E) <= 512) { if (vec) LAUNCH(64, 8, true); else LAUNCH(64, 8, false); }        \
+    else { if (vec) LAUNCH(64, 16, true); else LAUNCH(64, 16, false); }                      \
   } while (0)
+// tokens that a wave of the above takes at a time
+int tokens_at_once(int64_t E) { return E <= 8 ? 32 : E <= 16 ? 16 : E <= 32 ? 8 : E <= 128 ? 4 : E <= 256 ? 2 : 1; }
 
 int64_t chunk_of(int64_t T) { return kChunk * std::max<int64_t>(1, pk_ceil_div(T, (int64_t)kChunk * kMostChunks)); }
 int64_t units_of(int64_t T, int64_t S) { return T / chunk_of(T) + S + 1; }
@@ -315,9 +361,10 @@ int pk_balance_loss(const float* logits, const int32_t* top_idx, const int32_t* 
   p.done = reinterpret_cast<uint32_t*>(at);
   p.loss = loss; p.counts = counts; p.table = table;
   hipStream_t s = (hipStream_t)stream;
-#define PK_LAUNCH(LPT, EPL) \
-  PK_LAUNCH_NOCHECK(pk_timing::K_BALANCE, s, (balance_partial_kernel<LPT, EPL>), dim3((unsigned)units), dim3(kThreads), 0, s, p)
-  PK_BALANCE_DISPATCH(E, PK_LAUNCH);
+  const bool vec = E % 4 == 0 && pk_aligned16(logits);
+#define PK_LAUNCH(...) \
+  PK_LAUNCH_NOCHECK(pk_timing::K_BALANCE, s, (balance_partial_kernel<__VA_ARGS__>), dim3((unsigned)units), dim3(kThreads), 0, s, p)
+  PK_BALANCE_DISPATCH(E, vec, PK_LAUNCH);
 #undef PK_LAUNCH
   PK_LAUNCH_NOCHECK(pk_timing::K_BALANCE, s, balance_sum_kernel, dim3((unsigned)S), dim3(units / S >= 8 ? kMostSum : 256), 0, s, p);
   PK_RETURN_IF_LAUNCH_FAILED();
@@ -332,11 +379,13 @@ int pk_balance_loss_bwd(const float* logits, const int32_t* sequences, const flo
   if (!logits || !table || !d_loss || !d_logits) return PK_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   const Grad g{table, sequences, d_loss, (int32_t)S};
-  const int tokens = T >= 16384 ? 64 : 16;
-#define PK_LAUNCH(LPT, EPL)                                                                                                         \
-  PK_LAUNCH_NOCHECK(pk_timing::K_BALANCE_BWD, s, (balance_bwd_kernel<LPT, EPL>), dim3((unsigned)pk_ceil_div(T, tokens)), dim3(kThreads), 0, s, \
-                    logits, g, (int)T, (int)E, tokens, d_logits)
-  PK_BALANCE_DISPATCH(E, PK_LAUNCH);
+  // four steps a wave where that leaves every CU eight waves
+  const int64_t at_once = (int64_t)kWaves * tokens_at_once(E), steps = T >= at_once * 4 * 512 ? 4 : 1;
+  const bool vec = E % 4 == 0 && pk_aligned16(logits) && pk_aligned16(table) && pk_aligned16(d_logits);
+#define PK_LAUNCH(...)                                                                                                                        \
+  PK_LAUNCH_NOCHECK(pk_timing::K_BALANCE_BWD, s, (balance_bwd_kernel<__VA_ARGS__>), dim3((unsigned)pk_ceil_div(T, at_once * steps)), dim3(kThreads), 0, s, \
+                    logits, g, (int)T, (int)E, (int)steps, d_logits)
+  PK_BALANCE_DISPATCH(E, vec, PK_LAUNCH);
 #undef PK_LAUNCH
   PK_RETURN_IF_LAUNCH_FAILED();
   return PK_OK;

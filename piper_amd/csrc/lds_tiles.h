@@ -137,4 +137,19 @@ __device__ __forceinline__ void wait_tiles(int t) {
   wait_tiles<L, (MAXT > 0 ? MAXT - 1 : 0)>(t);
 }
 
+// Wait until at most n (wave-uniform, rounded down to a multiple of 4, capped at 60) vector-memory
+// operations are outstanding.  Loads, stores and atomics retire from the counter in issue
+// order, so with n = a lower bound of the operations issued AFTER the ones of interest this
+// waits for those without waiting for the younger ones (for example an epilogue's stores).
+__device__ __forceinline__ void wait_vm_le(int n) {
+  switch ((n < 60 ? n : 60) >> 2) {
+    case 0: wait_dma<0>(); break;    case 1: wait_dma<4>(); break;    case 2: wait_dma<8>(); break;
+    case 3: wait_dma<12>(); break;   case 4: wait_dma<16>(); break;   case 5: wait_dma<20>(); break;
+    case 6: wait_dma<24>(); break;   case 7: wait_dma<28>(); break;   case 8: wait_dma<32>(); break;
+    case 9: wait_dma<36>(); break;   case 10: wait_dma<40>(); break;  case 11: wait_dma<44>(); break;
+    case 12: wait_dma<48>(); break;  case 13: wait_dma<52>(); break;  case 14: wait_dma<56>(); break;
+    default: wait_dma<60>(); break;
+  }
+}
+
 }  // namespace pk_lds

@@ -35,12 +35,15 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kPad = 128;
-constexpr int kMaxEntries = 40;              // shapes of a group: keeps the kernels' arguments below 4 KiB
+// Stacks of matrices in a launch of the kernels at both ends, these launches in a group, and sizes in one of a product: keeps the kernels'
+// arguments below 4 KiB.
+constexpr int kMaxEntries = 40, kMaxEnds = 8, kMaxShapes = 100;
 constexpr int kChunk = 8192;                 // elements a workgroup of begin_kernel takes
 constexpr int kThreads = 256;
-// Workspace that is asked for.  Groups that stay in the 256 MiB memory-side cache leave too few workgroups a launch: 128 matrices of
-// 768 x 2048, bf16 / fp32 results, ms with 192 MiB 8.6 / 17.4, 384 6.4 / 17.3, 768 6.2 / 15.4, 1,536 5.8 / 14.9, all at once 5.5 / 14.6.
-constexpr int64_t kGroupBytes = 1ll << 30;
+// Workspace that is asked for.  Groups that stay in the 256 MiB memory-side cache leave too few workgroups a launch, whose last round is
+// rarely full: 128 matrices of 768 x 2048, bf16 / fp32 results, ms with 192 MiB 8.6 / 14.5, 384 6.4 / 12.8, 768 6.1 / 11.2, 1,536 5.6 / 10.6, all at
+// once 5.2 / 10.1.
+constexpr int64_t kGroupBytes = 2560ll << 20;
 
 // Matrices of one shape that lie one behind the other, as the kernels at both ends see them.
 struct Entry {
@@ -64,12 +67,13 @@ struct Ends {
 };
 static_assert(sizeof(Ends) <= 4096, "kernel arguments");
 struct Gemm {
-  struct Shape { int64_t ws, stride; int32_t mp, np, first_unit; } e[kMaxEntries];      // (first_unit: the number of matrices, until they are numbered)
+  struct Shape { int64_t ws, stride; int32_t mp, np, first_unit; } e[kMaxShapes];      // (first_unit: the number of matrices, until they are numbered)
   char* ws;
-  int32_t n, units, chunk, wide, splits;
+  int32_t n, units, blocks, chunk, wide, splits;      // blocks: of units in the order they are dealt
   int32_t from;          // which of the two X the products read
   float a, b, c;
 };
+static_assert(sizeof(Gemm) <= 4096, "kernel arguments");
 
 // X is held times 2^12 and A times 2^8: elements of large normalised matrices are small, as A's off the diagonal are, and
 // the lower plane of a small one would be below fp16's range.  (Singular values up to 16 stay in it; those of the usual coefficients
@@ -405,75 +409,88 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
   constexpr int NW = 8, WNW = BN / 64, WM = BM / (NW / WNW), TM = WM / 32, TN = 2, KS = KT / 16;
   constexpr int P = PRECISE ? 2 : 1, W = KT * P;
   constexpr int A_BYTES = BM * W * 2, STAGE = (BM + BN) * W * 2, LA = A_BYTES / (NW * 1024), LB = BN * W * 2 / (NW * 1024), L = LA + LB;
-  constexpr int STAGING = 32 * 64 * 4;                  // of a wave: 32 rows of its outputs
-  static_assert(NS * STAGE <= 160 * 1024 && NW * STAGING <= NS * STAGE, "LDS budget");
+  constexpr int STAGING = 32 * 128;                     // of a wave: 32 rows of one plane of its outputs
+  static_assert(NS * STAGE <= 160 * 1024 && NW * STAGING <= STAGE, "LDS budget");
   static_assert(W == 32 || W == 64, "rows of the LDS tiles");
   static_assert(!PRECISE || KT == 32, "blocks of 32 of either plane");
   __shared__ __attribute__((aligned(1024))) char smem[NS * STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WNW, wn = wave % WNW;
-  const int dealt = pk_rules::dealt_unit(blockIdx.x, p.chunk);     // neighbours share operands in an XCD's L2
-  const int unit = PHASE == PARTIAL ? dealt / p.splits : dealt, split = PHASE == PARTIAL ? dealt % p.splits : 0;
-  if (unit >= p.units) return;
-  const int en = entry_of(p.n, unit, [&](int i) { return p.e[i].first_unit; });
-  const int mp = p.e[en].mp, np = p.e[en].np;
-  const int N = KIND == UPDATE ? np : mp;               // columns of the result
-  const int tm = (mp + BM - 1) / BM, tn = (N + BN - 1) / BN;
-  const int local = unit - p.e[en].first_unit;
-  int mat, mt, nt, in_matrix = 0;
-  if (KIND == UPDATE) {
-    mat = local / (tm * tn);
-    mt = local % (tm * tn) / tn;
-    nt = local % (tm * tn) % tn;
-  } else {
-    constexpr int R = BN / BM;                          // row tiles of a 256 x 256 block
-    const int per = units_of_symmetric<BM, BN>(mp);
-    mat = local / per;
-    const int t = in_matrix = local % per;
-    nt = (int)((sqrtf(8.f * (t / R) + 1.f) - 1.f) * 0.5f);       // row of blocks, corrected, and the column in it
-    while ((nt + 1) * (nt + 2) / 2 * R <= t) ++nt;
-    while (nt * (nt + 1) / 2 * R > t) --nt;
-    const int in_row = t - nt * (nt + 1) / 2 * R, rows = min(R, tm - nt * R);
-    mt = nt * R + in_row % rows;
-    nt = in_row / rows;
-  }
-  char* const mem = p.ws + p.e[en].ws + (int64_t)mat * p.e[en].stride;
-  const int64_t px = plane_x(mp, np);
-  char* const X = mem + 2 * p.from * px;
-  char* const Xn = mem + 2 * (1 - p.from) * px;
-  char* const A = mem + at_a(mp, np);
-  char* const B = mem + at_b(mp, np, PRECISE);
-  const char* const left = KIND == GRAM ? X : KIND == POLY ? A : B;
-  const char* const right = KIND == POLY ? A : X;
-  const int lda = (KIND == GRAM ? np : mp) * P, ldb = (KIND == POLY ? mp : np) * P;      // of a row in memory
-  const int pairs = (KIND == GRAM ? np : mp) / (2 * KT);         // of k-tiles: k is a multiple of 128
-  const int kt0 = PHASE == PARTIAL ? 2 * (pairs * split / p.splits) : 0;
-  const int nkt = PHASE == PARTIAL ? 2 * (pairs * (split + 1) / p.splits) - kt0 : 2 * pairs;
-  const int row0 = mt * BM, col0 = nt * BN;
+  const int grp = wave >> 2;
 
+  struct Unit {
+    int mp, np, N;                                      // N: columns of the result
+    int row0, col0, in_matrix, split, nkt;
+    bool mirrored;                                      // off the diagonal of a symmetric result
+    char *X, *Xn, *A, *B;
+  };
+  Unit u;
   // ---- the loader: a lane's byte offsets from two wave-uniform pointers that advance by a constant per k-tile
   uint32_t va[LA], vb[LB];
-#pragma unroll
-  for (int i = 0; i < LA; ++i) {
-    int r, k;
-    kc_slot<W>(wave * LA + i, lane, r, k);
-    va[i] = (uint32_t)(min(r, mp - 1 - row0) * lda + k) * 2u;
-  }
-#pragma unroll
-  for (int i = 0; i < LB; ++i) {
-    int r, k;
+  const char *ld_a, *ld_b;
+  int64_t step_b;
+  auto enter = [&](int dealt) {
+    const int unit = PHASE == PARTIAL ? dealt / p.splits : dealt;
+    u.split = PHASE == PARTIAL ? dealt % p.splits : 0;
+    const int en = entry_of(p.n, unit, [&](int i) { return p.e[i].first_unit; });
+    const int mp = u.mp = p.e[en].mp, np = u.np = p.e[en].np;
+    const int N = u.N = KIND == UPDATE ? np : mp;
+    const int tm = (mp + BM - 1) / BM, tn = (N + BN - 1) / BN;
+    const int local = unit - p.e[en].first_unit;
+    int mat, mt, nt;
     if (KIND == UPDATE) {
-      mn_slot<BN * P>(wave * LB + i, lane, r, k);
-      vb[i] = (uint32_t)(r * ldb + min(k, (N - col0) * P - 8)) * 2u;
+      mat = local / (tm * tn);
+      u.in_matrix = local % (tm * tn);
+      mt = u.in_matrix / tn;
+      nt = u.in_matrix % tn;
     } else {
-      kc_slot<W>(wave * LB + i, lane, r, k);
-      vb[i] = (uint32_t)(min(r, N - 1 - col0) * ldb + k) * 2u;
+      constexpr int R = BN / BM;                        // row tiles of a block
+      const int per = units_of_symmetric<BM, BN>(mp);
+      mat = local / per;
+      const int t = u.in_matrix = local % per;
+      nt = (int)((sqrtf(8.f * (t / R) + 1.f) - 1.f) * 0.5f);     // row of blocks, corrected, and the column in it
+      while ((nt + 1) * (nt + 2) / 2 * R <= t) ++nt;
+      while (nt * (nt + 1) / 2 * R > t) --nt;
+      const int in_row = t - nt * (nt + 1) / 2 * R, rows = min(R, tm - nt * R);
+      mt = nt * R + in_row % rows;
+      nt = in_row / rows;
     }
-  }
-  const char* ld_a = uniform_ptr(left + (int64_t)row0 * lda * 2 + (int64_t)kt0 * W * 2);
-  const char* ld_b = uniform_ptr(right + (KIND == UPDATE ? (int64_t)col0 * P * 2 : (int64_t)col0 * ldb * 2 + (int64_t)kt0 * W * 2));
-  const int64_t step_b = KIND == UPDATE ? (int64_t)KT * ldb * 2 : W * 2;
+    u.mirrored = KIND != UPDATE && mt / (BN / BM) != nt;
+    const int row0 = u.row0 = __builtin_amdgcn_readfirstlane(mt * BM), col0 = u.col0 = __builtin_amdgcn_readfirstlane(nt * BN);
+    char* const mem = const_cast<char*>(uniform_ptr(p.ws + p.e[en].ws + (int64_t)mat * p.e[en].stride));
+    const int64_t px = plane_x(mp, np);
+    u.X = mem + 2 * p.from * px;
+    u.Xn = mem + 2 * (1 - p.from) * px;
+    u.A = mem + at_a(mp, np);
+    u.B = mem + at_b(mp, np, PRECISE);
+    const char* const left = KIND == GRAM ? u.X : KIND == POLY ? u.A : u.B;
+    const char* const right = KIND == POLY ? u.A : u.X;
+    const int lda = (KIND == GRAM ? np : mp) * P, ldb = (KIND == POLY ? mp : np) * P;    // of a row in memory
+    const int pairs = (KIND == GRAM ? np : mp) / (2 * KT);       // of k-tiles: k is a multiple of 128
+    const int kt0 = PHASE == PARTIAL ? 2 * (pairs * u.split / p.splits) : 0;
+    u.nkt = __builtin_amdgcn_readfirstlane(PHASE == PARTIAL ? 2 * (pairs * (u.split + 1) / p.splits) - kt0 : 2 * pairs);
+#pragma unroll
+    for (int i = 0; i < LA; ++i) {
+      int r, k;
+      kc_slot<W>(wave * LA + i, lane, r, k);
+      va[i] = (uint32_t)(min(r, mp - 1 - row0) * lda + k) * 2u;
+    }
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+      int r, k;
+      if (KIND == UPDATE) {
+        mn_slot<BN * P>(wave * LB + i, lane, r, k);
+        vb[i] = (uint32_t)(r * ldb + min(k, (N - col0) * P - 8)) * 2u;
+      } else {
+        kc_slot<W>(wave * LB + i, lane, r, k);
+        vb[i] = (uint32_t)(min(r, N - 1 - col0) * ldb + k) * 2u;
+      }
+    }
+    ld_a = uniform_ptr(left + (int64_t)row0 * lda * 2 + (int64_t)kt0 * W * 2);
+    ld_b = uniform_ptr(right + (KIND == UPDATE ? (int64_t)col0 * P * 2 : (int64_t)col0 * ldb * 2 + (int64_t)kt0 * W * 2));
+    step_b = KIND == UPDATE ? (int64_t)KT * ldb * 2 : W * 2;
+  };
   auto request = [&](int stage) {
     const uint32_t to = lds_addr(smem) + stage * STAGE;
     static_for<LA>([&](auto i) { dma16_s<decltype(i)::value * 1024>(va[i], ld_a, to + wave * (LA * 1024)); });
@@ -481,201 +498,244 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
     ld_a += W * 2;
     ld_b += step_b;
   };
+  int cur = 0;                                          // stage of the unit's first k-tile
+  auto request_first = [&]() {
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s)
+      if (s < u.nkt) request(cur + s >= NS ? cur + s - NS : cur + s);
+  };
 
-  floatx16_t acc[TM][TN] = {}, sum[PRECISE ? TM : 1][TN] = {};
-  const int grp = wave >> 2;
-  const bool live = row0 + wm * WM < mp && col0 + wn * 64 < N;
-  // where a split's sums are: [unit of the matrix][split][16 bytes of every lane in turn]
-  constexpr int VECS = TM * TN * 4;
-  floatx4_t* part = reinterpret_cast<floatx4_t*>(Xn) + ((int64_t)in_matrix * (PHASE == WHOLE ? 0 : p.splits) + split) * (VECS * 512) + wave * (VECS * 64) + lane;
-  if constexpr (PHASE != SUMS) {
+  // this workgroup's units: neighbours share operands in an XCD's L2
+  const int total = PHASE == PARTIAL ? p.units * p.splits : p.units;
+  int at = blockIdx.x;
+  auto next = [&]() {                                   // -1: none
+    for (; at < p.blocks; at += gridDim.x) {
+      const int d = pk_rules::dealt_unit(at, p.chunk);
+      if (d < total) {
+        at += gridDim.x;
+        return d;
+      }
+    }
+    return -1;
+  };
+  int dealt = next();
+  if (dealt < 0) return;
+  enter(dealt);
+  if (PHASE != SUMS) request_first();
+  int stored = 0;                                       // store instructions since those requests
+
+  for (;;) {
+    const Unit w = u;
+    const bool live = w.row0 + wm * WM < w.mp && w.col0 + wn * 64 < w.N;
+    floatx16_t acc[TM][TN] = {}, sum[PRECISE ? TM : 1][TN] = {};
+    if constexpr (PHASE != SUMS) {
+      // k-tile 0 has landed once only the younger ones and the stores behind them are on their way
+      wait_vm_le((min(w.nkt, NS - 1) - 1) * L + stored);
+      block_barrier();
+      if (grp == 1) block_barrier();
+      f16x8_t fa[P][KS][TM], fb[P][KS][TN];             // upper and lower plane
+      // FIRST: the accumulators go into the second set and start again
+      auto k_tile = [&](int kt, auto first) __attribute__((always_inline)) {
+        constexpr bool FIRST = decltype(first)::value;
+        // ---- memory phase
+        const char* const st = smem + cur * STAGE;
+        if (live) {
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s)
-    if (s < nkt) request(s);
-  wait_tiles<L, NS - 2>(min(nkt, NS - 1) - 1);
-  block_barrier();
-  if (grp == 1) block_barrier();
-  int cur = 0;
-  f16x8_t fa[P][KS][TM], fb[P][KS][TN];       // upper and lower plane
-  // FIRST: the accumulators go into the second set and start again
-  auto k_tile = [&](int kt, auto first) __attribute__((always_inline)) {
-    constexpr bool FIRST = decltype(first)::value;
-    // ---- memory phase
-    const char* const st = smem + cur * STAGE;
-    if (live) {
+          for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+            for (int pl = 0; pl < P; ++pl) {
 #pragma unroll
-        for (int pl = 0; pl < P; ++pl) {
+              for (int i = 0; i < TM; ++i) fa[pl][ks][i] = frag_kc<W, f16x8_t>(st, wm * WM + 32 * i, ks + pl * KS, lane);
 #pragma unroll
-          for (int i = 0; i < TM; ++i) fa[pl][ks][i] = frag_kc<W, f16x8_t>(st, wm * WM + 32 * i, ks + pl * KS, lane);
-#pragma unroll
-          for (int j = 0; j < TN; ++j)
-            fb[pl][ks][j] = KIND == UPDATE ? frag_mn<BN * P, f16x8_t>(st + A_BYTES, (wn * 64 + 32 * j) * P + 32 * pl, ks, lane)
-                                           : frag_kc<W, f16x8_t>(st + A_BYTES, wn * 64 + 32 * j, ks + pl * KS, lane);
+              for (int j = 0; j < TN; ++j)
+                fb[pl][ks][j] = KIND == UPDATE ? frag_mn<BN * P, f16x8_t>(st + A_BYTES, (wn * 64 + 32 * j) * P + 32 * pl, ks, lane)
+                                               : frag_kc<W, f16x8_t>(st + A_BYTES, wn * 64 + 32 * j, ks + pl * KS, lane);
+            }
         }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if (kt + NS - 1 < nkt) request(cur == 0 ? NS - 1 : cur - 1);      // the stage of k-tile kt - 1
-    cur = cur + 1 == NS ? 0 : cur + 1;
-    if (FIRST && live) {      // (while the other group multiplies)
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) sum[PRECISE ? i : 0][j] += acc[i][j];
-    }
-    // a wave's own part of k-tile kt + 1 has landed when the phase before its first read ends
-    const int younger = min(NS - 2, nkt - 2 - kt);
-    if (grp == 1) wait_tiles<L, NS - 2>(younger);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    block_barrier();
-    // ---- compute phase
-    if (live) {
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int pr = PRECISE ? 0 : 2; pr < 3; ++pr)        // lo hi, hi lo, hi hi
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+        __builtin_amdgcn_sched_barrier(0);
+        if (kt + NS - 1 < w.nkt) request(cur == 0 ? NS - 1 : cur - 1);      // the stage of k-tile kt - 1
+        cur = cur + 1 == NS ? 0 : cur + 1;
+        if (FIRST && live) {      // (while the other group multiplies)
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[pr == 1 ? P - 1 : 0][ks][j], fa[pr == 0 ? P - 1 : 0][ks][i],
-                                                                 FIRST && pr == 0 && ks == 0 ? floatx16_t{} : acc[i][j], 0, 0, 0);
-      __builtin_amdgcn_s_setprio(0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if (grp == 0) wait_tiles<L, NS - 2>(younger);
-    block_barrier();
-  };
-  if constexpr (PRECISE) {
-    for (int kt = 0; kt < nkt; kt += 2) {                // (k is a multiple of 128)
-      k_tile(kt, std::true_type{});
-      k_tile(kt + 1, std::false_type{});
-    }
-  } else {
-    for (int kt = 0; kt < nkt; ++kt) k_tile(kt, std::false_type{});
-  }
-  if (grp == 0) block_barrier();        // the whole ring is free
-  }
-  if (!live) return;
-  if constexpr (PHASE == PARTIAL) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          floatx4_t v;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * q + k] + (PRECISE ? sum[PRECISE ? i : 0][j][4 * q + k] : 0.f);
-          part[((i * TN + j) * 4 + q) * 64] = v;
+            for (int j = 0; j < TN; ++j) sum[PRECISE ? i : 0][j] += acc[i][j];
         }
-    return;
-  }
-  if constexpr (PHASE == SUMS) {
-    for (int z = 0; z < p.splits; ++z, part += VECS * 512)
+        // a wave's own part of k-tile kt + 1 has landed when the phase before its first read ends; younger than it are the k-tiles after
+        // it and, while it is one of those requested before the epilogue, that one's stores
+        const int tiles = min(NS - 2, w.nkt - 2 - kt);
+        auto wait_next = [&]() {
+          if (kt <= NS - 3) wait_vm_le(max(tiles, 0) * L + stored);
+          else wait_tiles<L, NS - 2>(tiles);
+        };
+        if (grp == 1) wait_next();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        block_barrier();
+        // ---- compute phase
+        if (live) {
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int pr = PRECISE ? 0 : 2; pr < 3; ++pr)        // lo hi, hi lo, hi hi
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+              for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                  acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[pr == 1 ? P - 1 : 0][ks][j], fa[pr == 0 ? P - 1 : 0][ks][i],
+                                                                     FIRST && pr == 0 && ks == 0 ? floatx16_t{} : acc[i][j], 0, 0, 0);
+          __builtin_amdgcn_s_setprio(0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (grp == 0) wait_next();
+        block_barrier();
+      };
+      if constexpr (PRECISE) {
+        for (int kt = 0; kt < w.nkt; kt += 2) {
+          k_tile(kt, std::true_type{});
+          k_tile(kt + 1, std::false_type{});
+        }
+      } else {
+        for (int kt = 0; kt < w.nkt; ++kt) k_tile(kt, std::false_type{});
+      }
+      if constexpr (PRECISE) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] += sum[i][j];
+      }
+      if (grp == 0) block_barrier();        // the whole ring is free
+    }
+    // the next unit's first k-tiles come while this one's results go
+    dealt = next();
+    if (dealt >= 0) {
+      enter(dealt);
+      if (PHASE != SUMS) request_first();
+    }
+    stored = 0;
+
+    // where a split's sums are: [unit of the matrix][split][16 bytes of every lane in turn]
+    constexpr int VECS = TM * TN * 4;
+    floatx4_t* part = reinterpret_cast<floatx4_t*>(w.Xn) + ((int64_t)w.in_matrix * (PHASE == WHOLE ? 0 : p.splits) + w.split) * (VECS * 512) +
+                      wave * (VECS * 64) + lane;
+    if (PHASE == PARTIAL && live) {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const floatx4_t v = part[((i * TN + j) * 4 + q) * 64];
+            floatx4_t v;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] += v[k];
+            for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * q + k];
+            part[((i * TN + j) * 4 + q) * 64] = v;
           }
-  }
-
-  // ---- epilogue: 32 rows of a wave at a time through LDS, so that a lane has 8 neighbouring columns and memory is read and
-  // written 16 bytes a lane.  acc[i][j][v] is row 32 i + lane % 32, column 32 j + 8 (v / 4) + 4 (lane / 32) + v % 4.
-  const int ldc = N;
-  const int64_t lower = to_lower(PRECISE, mp, ldc) * 2;       // bytes
-  char* const out = KIND == GRAM ? A : KIND == POLY ? B : Xn;
-  const char* const old = KIND == POLY ? A : X;         // what b or a multiplies
-  constexpr float unscale = KIND == GRAM ? kA / (kX * kX) : KIND == POLY ? 1.f / (kA * kA) : 1.f;
-  constexpr bool OLD_HI = KIND == POLY, OLD_LO = PRECISE ? KIND == POLY : KIND == UPDATE, OUT_LO = KIND == UPDATE || PRECISE;
-  const bool mirrored = KIND != UPDATE && mt / (BN / BM) != nt;
-  char* const buf = smem + wave * STAGING;
-  const int lr = lane >> 3, lc = lane & 7;              // a lane's row (of 8 in a pass) and columns 8 lc ..
+      stored = VECS;
+    }
+    if (PHASE == SUMS && live) {
+      for (int z = 0; z < p.splits; ++z, part += VECS * 512)
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int r0 = row0 + wm * WM + 32 * i, c0 = col0 + wn * 64;
-    f16x8_t oh[4], ol[4];
-    if (OLD_HI || OLD_LO) {
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const char* const at = old + place(PRECISE, r0 + 8 * q + lr, c0 + 8 * lc, ldc) * 2;
-        if (OLD_HI) oh[q] = *reinterpret_cast<const f16x8_t*>(at);
-        if (OLD_LO) ol[q] = *reinterpret_cast<const f16x8_t*>(at + lower);
+          for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const floatx4_t v = part[((i * TN + j) * 4 + q) * 64];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] += v[k];
+            }
+    }
+    // ---- epilogue, 32 rows of a wave at a time.  acc[i][j][v] is row 32 i + lane % 32, column 32 j + 8 (v / 4) + 4 (lane / 32) + v % 4.  Memory
+    // is read and written 16 bytes a lane, 64 columns a row; LDS turns one into the other: fp16 rows of 128 bytes, their 16-byte
+    // pieces swizzled by the row, in the stage that the coming k-tiles leave free.
+    if (PHASE != PARTIAL && live) {
+      const int ldc = w.N;
+      const int64_t lower = to_lower(PRECISE, w.mp, ldc) * 2;     // bytes
+      char* const out = KIND == GRAM ? w.A : KIND == POLY ? w.B : w.Xn;
+      const char* const old = KIND == POLY ? w.A : w.X;           // what b or a multiplies
+      constexpr float unscale = KIND == GRAM ? kA / (kX * kX) : KIND == POLY ? 1.f / (kA * kA) : 1.f;
+      constexpr bool OLD_HI = KIND == POLY, OLD_LO = PRECISE ? KIND == POLY : KIND == UPDATE, OUT_LO = KIND == UPDATE || PRECISE;
+      char* const buf = smem + (cur == 0 ? NS - 1 : cur - 1) * STAGE + wave * STAGING;
+      int lane_e = lane;                                // (so that its addresses are formed here, not kept in registers through the k-loop)
+      asm volatile("" : "+v"(lane_e));
+      const int lr = lane_e >> 3, lc = lane_e & 7;      // a lane's row (of 8 in a pass) and piece of it in memory
+      const int row = lane_e & 31, col = 4 * (lane_e >> 5);       // and in acc: column 32 j + 8 q + col
+      const auto piece_at = [&](int r, int c) { return buf + r * 128 + ((c ^ (r & 7)) << 4); };
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int r0 = w.row0 + wm * WM + 32 * i, c0 = w.col0 + wn * 64;
+        f16x8_t from_memory[2][4];
+#pragma unroll
+        for (int pl = 0; pl < 2; ++pl)
+          if (pl ? OLD_LO : OLD_HI) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              from_memory[pl][q] = *reinterpret_cast<const f16x8_t*>(old + place(PRECISE, r0 + 8 * q + lr, c0 + 8 * lc, ldc) * 2 + pl * lower);
+          }
+        f16x4_t o[2][TN][4];
+#pragma unroll
+        for (int pl = 0; pl < 2; ++pl)
+          if (pl ? OLD_LO : OLD_HI) {
+            wave_lds_fence();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<f16x8_t*>(piece_at(8 * q + lr, lc)) = from_memory[pl][q];
+            wave_lds_fence();
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) o[pl][j][q] = *reinterpret_cast<const f16x4_t*>(piece_at(row, 4 * j + q) + col * 2);
+          }
+        f16x4_t res[2][TN][4];
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float x = acc[i][j][4 * q + k] * unscale;
+              if (KIND == POLY) {
+                const float before = OLD_LO ? (float)o[0][j][q][k] + (float)o[1][j][q][k] : (float)o[0][j][q][k];
+                x = p.b * (before * (1.f / kA)) + p.c * x;
+                if (r0 + row == c0 + 32 * j + 8 * q + col + k) x += p.a;
+              } else if (OLD_LO) {
+                x += p.a * (float)o[1][j][q][k];
+              }
+              res[0][j][q][k] = (f16_t)x;
+              res[1][j][q][k] = (f16_t)(x - (float)res[0][j][q][k]);
+            }
+#pragma unroll
+        for (int pl = 0; pl < (OUT_LO ? 2 : 1); ++pl) {
+          wave_lds_fence();
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<f16x4_t*>(piece_at(row, 4 * j + q) + col * 2) = res[pl][j][q];
+          wave_lds_fence();
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f16x8_t*>(out + place(PRECISE, r0 + 8 * q + lr, c0 + 8 * lc, ldc) * 2 + pl * lower) =
+                *reinterpret_cast<const f16x8_t*>(piece_at(8 * q + lr, lc));
+          stored += 4;
+          if (KIND != UPDATE && w.mirrored) {
+            // turned: within 16 lanes of the transposing read, lane t points at row t / 4, columns 4 (t % 4) .. and receives rows 0 .. 3 of
+            // column t
+            const int t = lane_e & 15, ra = 8 * (lane_e >> 4) + (t >> 2), rb = ra + 4;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {               // columns 16 q ..
+              const int c = 16 * q + 4 * (t & 3);
+              const shortx4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4_t*)(piece_at(ra, c >> 3) + (c & 7) * 2));
+              const shortx4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4_t*)(piece_at(rb, c >> 3) + (c & 7) * 2));
+              typedef short shortx8_t __attribute__((ext_vector_type(8)));
+              *reinterpret_cast<shortx8_t*>(out + pl * lower + place(PRECISE, c0 + 16 * q + t, r0 + 8 * (lane_e >> 4), ldc) * 2) =
+                  __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            stored += 4;
+          }
+        }
       }
     }
-    wave_lds_fence();                                   // the chunk before has been read
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        floatx4_t v;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = (acc[i][j][4 * q + k] + (PRECISE ? sum[PRECISE ? i : 0][j][4 * q + k] : 0.f)) * unscale;
-        const int row = lane & 31, chunk = 8 * j + 2 * q + (lane >> 5);
-        *reinterpret_cast<floatx4_t*>(buf + row * 256 + ((chunk ^ (row & 15)) << 4)) = v;
-      }
-    wave_lds_fence();
-    f16x8_t h[4], l[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int row = 8 * q + lr;
-      float x[8];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const floatx4_t v = *reinterpret_cast<const floatx4_t*>(buf + row * 256 + (((2 * lc + half) ^ (row & 15)) << 4));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[4 * half + k] = v[k];
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (KIND == POLY) {
-          const float o = OLD_LO ? (float)oh[q][k] + (float)ol[q][k] : (float)oh[q][k];
-          x[k] = p.b * (o * (1.f / kA)) + p.c * x[k];
-          if (r0 + row == c0 + 8 * lc + k) x[k] += p.a;
-        } else if (OLD_LO) {
-          x[k] += p.a * (float)ol[q][k];
-        }
-        h[q][k] = (f16_t)x[k];
-        l[q][k] = (f16_t)(x[k] - (float)h[q][k]);
-      }
-      char* const at = out + place(PRECISE, r0 + row, c0 + 8 * lc, ldc) * 2;
-      *reinterpret_cast<f16x8_t*>(at) = h[q];
-      if (OUT_LO) *reinterpret_cast<f16x8_t*>(at + lower) = l[q];
-    }
-    if (mirrored) {
-      // the same 32 x 64 values turned: fp16 rows of 128 bytes, 16-byte pieces swizzled by the row; within 16 lanes of the
-      // transposing read, lane t points at row t / 4, columns 4 (t % 4) .. and receives rows 0 .. 3 of column t
-#pragma unroll
-      for (int plane = 0; plane < (OUT_LO ? 2 : 1); ++plane) {
-        wave_lds_fence();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int row = 8 * q + lr;
-          *reinterpret_cast<f16x8_t*>(buf + row * 128 + ((lc ^ (row & 7)) << 4)) = plane ? l[q] : h[q];
-        }
-        wave_lds_fence();
-        const int t = lane & 15, ra = 8 * (lane >> 4) + (t >> 2), rb = ra + 4;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {                   // columns 16 q ..
-          const int c = 16 * q + 4 * (t & 3);
-          const shortx4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) shortx4_t*)(buf + ra * 128 + (((c >> 3) ^ (ra & 7)) << 4) + (c & 7) * 2));
-          const shortx4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) shortx4_t*)(buf + rb * 128 + (((c >> 3) ^ (rb & 7)) << 4) + (c & 7) * 2));
-          typedef short shortx8_t __attribute__((ext_vector_type(8)));
-          *reinterpret_cast<shortx8_t*>(out + plane * lower + place(PRECISE, c0 + 16 * q + t, r0 + 8 * (lane >> 4), ldc) * 2) =
-              __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-      }
-    }
+    if (dealt < 0) return;
   }
 }
 
@@ -709,20 +769,25 @@ bool sides_ok(int64_t rows, int64_t cols) { return rows <= PK_MAX_MATRIX_SIDE &&
 // groups), fp32 4,785 -> 5,062 / 4,941 -> 5,903 (624 / 2,496).  (Half of a wide tile on the diagonal is of no use.)
 constexpr int64_t kWideSymmetric = 512, kWideUpdate = 160;
 constexpr int kWideRows[2] = {256, 128};               // [precise]
+constexpr unsigned kGrid = 256;                         // workgroups at most, one to a CU; each takes every kGrid-th unit
 template <int KIND>
 void launch_product(const Gemm& g, bool precise, int id, hipStream_t s) {
-  const dim3 grid((unsigned)pk_rules::dealt_blocks(g.units, g.chunk)), block(512);
+  const dim3 grid(std::min<unsigned>(g.blocks, kGrid)), block(512);
 #define PK_LAUNCH(...) PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, __VA_ARGS__>), grid, block, 0, s, g)
   if (g.wide) { if (precise) PK_LAUNCH(true, 128, 256, 32, 3); else PK_LAUNCH(false, 256, 256, 32, 4); }
   else if (precise) PK_LAUNCH(true, 128, 128, 32, 4);
   else PK_LAUNCH(false, 128, 128, 64, 4);
 #undef PK_LAUNCH
 }
+void deal(Gemm& g, int64_t units) {
+  g.chunk = (int32_t)pk_rules::deal_chunk(units, 32);
+  g.blocks = (int32_t)pk_rules::dealt_blocks(units, g.chunk);
+}
 void launch_gram(const Gemm& g, bool precise, hipStream_t s) {
   if (g.splits == 1) return launch_product<GRAM>(g, precise, pk_timing::K_NS_GRAM, s);
   Gemm shares = g;
-  shares.chunk = (int32_t)pk_rules::deal_chunk((int64_t)g.units * g.splits, 32);
-  const dim3 grid((unsigned)pk_rules::dealt_blocks((int64_t)g.units * g.splits, shares.chunk)), sums((unsigned)pk_rules::dealt_blocks(g.units, g.chunk)), block(512);
+  deal(shares, (int64_t)g.units * g.splits);
+  const dim3 grid(std::min<unsigned>(shares.blocks, kGrid)), sums(std::min<unsigned>(g.blocks, kGrid)), block(512);
   const int id = pk_timing::K_NS_GRAM;
   if (precise) {
     PK_LAUNCH_NOCHECK(id, s, (product_kernel<GRAM, true, 128, 128, 32, 4, PARTIAL>), grid, block, 0, s, shares);
@@ -762,23 +827,33 @@ int64_t number_units(Gemm& g, F&& per) {
     at += units;
   }
   g.units = (int32_t)at;
-  g.chunk = (int32_t)pk_rules::deal_chunk(at, 32);
+  deal(g, at);
   return at;
 }
+// A group of matrices.
+struct Group {
+  Ends ends[kMaxEnds];
+  int64_t chunks[kMaxEnds], tiles[kMaxEnds];            // workgroups of the launches
+  int n;
+  Gemm sym, upd;
+};
 template <typename TG, bool STEP>
-int run_group(Ends& e, Gemm& sym, Gemm& upd, int chunks, int tiles, const Settings& o, hipStream_t s) {
-  const bool precise = e.precise != 0;
-  PK_LAUNCH_NOCHECK(pk_timing::K_MUON_BEGIN, s, (begin_kernel<TG, STEP>), dim3(chunks), dim3(kThreads), 0, s, e);
-  PK_LAUNCH_NOCHECK(pk_timing::K_MUON_CONVERT, s, (convert_kernel<TG, STEP>), dim3(tiles), dim3(kThreads), 0, s, e);
+int run_group(Group& g, const Settings& o, hipStream_t s) {
+  const bool precise = g.ends[0].precise != 0;
+  for (int i = 0; i < g.n; ++i)
+    PK_LAUNCH_NOCHECK(pk_timing::K_MUON_BEGIN, s, (begin_kernel<TG, STEP>), dim3((unsigned)g.chunks[i]), dim3(kThreads), 0, s, g.ends[i]);
+  for (int i = 0; i < g.n; ++i)
+    PK_LAUNCH_NOCHECK(pk_timing::K_MUON_CONVERT, s, (convert_kernel<TG, STEP>), dim3((unsigned)g.tiles[i]), dim3(kThreads), 0, s, g.ends[i]);
   int from = 0;
   for (int i = 0; i < o.steps; ++i) {
-    sym.from = upd.from = from;
-    launch_gram(sym, precise, s);
-    launch_product<POLY>(sym, precise, pk_timing::K_NS_POLY, s);
-    launch_product<UPDATE>(upd, precise, pk_timing::K_NS_UPDATE, s);
+    g.sym.from = g.upd.from = from;
+    launch_gram(g.sym, precise, s);
+    launch_product<POLY>(g.sym, precise, pk_timing::K_NS_POLY, s);
+    launch_product<UPDATE>(g.upd, precise, pk_timing::K_NS_UPDATE, s);
     from = 1 - from;
   }
-  PK_LAUNCH_NOCHECK(pk_timing::K_MUON_FINISH, s, (finish_kernel<TG, STEP>), dim3(tiles), dim3(kThreads), 0, s, e, from);
+  for (int i = 0; i < g.n; ++i)
+    PK_LAUNCH_NOCHECK(pk_timing::K_MUON_FINISH, s, (finish_kernel<TG, STEP>), dim3((unsigned)g.tiles[i]), dim3(kThreads), 0, s, g.ends[i], from);
   PK_RETURN_IF_LAUNCH_FAILED();
   return PK_OK;
 }
@@ -790,32 +865,49 @@ bool precise_result(bool asked, int64_t rows, int64_t cols) { return asked || st
 template <typename F>
 int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspace_bytes, hipStream_t s) {
   bool some = false;
+  int64_t all = 0;
   for (int64_t i = 0; i < n; ++i) {
     const Item it = item(i);
     if (it.count == 0) continue;
     some = true;
+    all += it.count * bytes_of(it.rows, it.cols, it.precise);
     if (!workspace || !pk_aligned16(workspace) || bytes_of(it.rows, it.cols, it.precise) > workspace_bytes) return PK_ERR_WORKSPACE;
   }
   if (!some) return PK_OK;
+  const int64_t share = pk_ceil_div(all, pk_ceil_div(all, workspace_bytes));      // groups of about the same size
   const int64_t es = o.bf16_src ? 2 : 4;
   int64_t i = 0, done = 0;        // done: matrices of item i
   while (i < n) {
-    Ends e = {};
-    Gemm sym = {}, upd = {};
-    e.ws = sym.ws = upd.ws = static_cast<char*>(workspace);
-    e.mu = o.mu; e.keep = o.keep; e.eps = o.eps; e.nesterov = o.nesterov; e.zero_flat = o.zero_flat;
-    sym.a = upd.a = o.a; sym.b = upd.b = o.b; sym.c = upd.c = o.c;
-    int64_t used = 0, chunks = 0, tiles = 0;
-    while (i < n && e.n < kMaxEntries) {
+    Group g;
+    g.n = 0;
+    Gemm sym = {};
+    sym.ws = static_cast<char*>(workspace);
+    sym.a = o.a; sym.b = o.b; sym.c = o.c;
+    int64_t used = 0;
+    bool precise = false;
+    while (i < n) {
       const Item it = item(i);
       if (it.count == 0) { ++i; continue; }
-      if (e.n > 0 && it.precise != (e.precise != 0)) break;        // the kernels of a group are of one kind
-      e.precise = it.precise;
-      const int64_t each = bytes_of(it.rows, it.cols, it.precise), fit = std::min((workspace_bytes - used) / each, it.count - done);
-      if (fit == 0) break;
+      if (used > 0 && it.precise != precise) break;                // the kernels of a group are of one kind
+      precise = it.precise;
+      const int64_t each = bytes_of(it.rows, it.cols, precise), left = std::min(workspace_bytes - used, std::max<int64_t>(share - used, 0) + each - 1);
+      const int64_t fit = std::min(left / each, it.count - done);
       const int mp = padded(std::min(it.rows, it.cols)), np = padded(std::max(it.rows, it.cols));
+      const bool like_last = sym.n > 0 && sym.e[sym.n - 1].mp == mp && sym.e[sym.n - 1].np == np && sym.e[sym.n - 1].stride == each;
+      if (fit <= 0 || (!like_last && sym.n == kMaxShapes)) break;
+      if (g.n == 0 || g.ends[g.n - 1].n == kMaxEntries) {
+        if (g.n == kMaxEnds) break;
+        Ends& e = g.ends[g.n];
+        e.ws = static_cast<char*>(workspace);
+        e.n = 0;
+        e.mu = o.mu; e.keep = o.keep; e.eps = o.eps; e.nesterov = o.nesterov; e.zero_flat = o.zero_flat; e.precise = precise;
+        g.chunks[g.n] = g.tiles[g.n] = 0;
+        ++g.n;
+      }
+      Ends& e = g.ends[g.n - 1];
+      int64_t &chunks = g.chunks[g.n - 1], &tiles = g.tiles[g.n - 1];
       const int64_t at = done * it.rows * it.cols;
-      Entry& x = e.e[e.n];
+      Entry& x = e.e[e.n++];
       x.src = it.src ? static_cast<const char*>(it.src) + at * es : nullptr;
       x.flat = it.flat ? it.flat + at : nullptr;
       x.momentum = it.momentum ? it.momentum + at : nullptr;
@@ -825,30 +917,28 @@ int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspa
       x.rows = (int)it.rows; x.cols = (int)it.cols; x.count = (int)fit; x.mp = mp; x.np = np;
       x.first_chunk = (int)chunks; x.first_tile = (int)tiles;
       x.rate = it.rate;
-      sym.e[e.n] = {used, each, mp, np, (int32_t)fit};
+      if (like_last) sym.e[sym.n - 1].first_unit += (int32_t)fit;
+      else sym.e[sym.n++] = {used, each, mp, np, (int32_t)fit};
       chunks += fit * pk_ceil_div(it.rows * it.cols, kChunk);
       tiles += fit * (mp / 64) * (np / 64);
+      if (std::max(chunks, tiles) > 0x3fffffffll) return PK_ERR_SHAPE;
       used += fit * each;
-      ++e.n;
       done += fit;
       if (done == it.count) { ++i; done = 0; }
     }
-    if (e.n == 0) break;
-    sym.n = e.n;
+    if (g.n == 0) break;
     // long products first: what is left for the end is short
-    std::sort(sym.e, sym.e + e.n, [](const auto& x, const auto& y) { return (int64_t)x.mp * x.np > (int64_t)y.mp * y.np; });
-    upd = sym;
-    const bool precise = e.precise != 0;
-    sym.wide = count_units(sym, [&](int mp, int) { return wide_symmetric(precise, mp); }) >= kWideSymmetric;
-    upd.wide = count_units(upd, [&](int mp, int np) { return wide_update(precise, mp, np); }) >= kWideUpdate;
-    sym.splits = sym.wide ? 1 : gram_splits(sym, count_units(sym, [](int mp, int) { return units_of_symmetric<128, 128>(mp); }));
-    const int64_t sym_units = number_units(sym, [&](int mp, int) { return sym.wide ? wide_symmetric(precise, mp) : units_of_symmetric<128, 128>(mp); });
-    const int64_t upd_units = number_units(upd, [&](int mp, int np) { return upd.wide ? wide_update(precise, mp, np) : (int64_t)(mp / 128) * (np / 128); });
-    if (std::max({chunks, tiles, sym_units, upd_units}) > 0x3fffffffll) return PK_ERR_SHAPE;
-    const int rc = o.step ? (o.bf16_src ? run_group<bf16_t, true>(e, sym, upd, (int)chunks, (int)tiles, o, s)
-                                        : run_group<float, true>(e, sym, upd, (int)chunks, (int)tiles, o, s))
-                          : (o.bf16_src ? run_group<bf16_t, false>(e, sym, upd, (int)chunks, (int)tiles, o, s)
-                                        : run_group<float, false>(e, sym, upd, (int)chunks, (int)tiles, o, s));
+    std::sort(sym.e, sym.e + sym.n, [](const auto& x, const auto& y) { return (int64_t)x.mp * x.np > (int64_t)y.mp * y.np; });
+    g.sym = g.upd = sym;
+    g.sym.wide = count_units(sym, [&](int mp, int) { return wide_symmetric(precise, mp); }) >= kWideSymmetric;
+    g.upd.wide = count_units(sym, [&](int mp, int np) { return wide_update(precise, mp, np); }) >= kWideUpdate;
+    g.sym.splits = g.sym.wide ? 1 : gram_splits(sym, count_units(sym, [](int mp, int) { return units_of_symmetric<128, 128>(mp); }));
+    const int64_t sym_units = number_units(g.sym, [&](int mp, int) { return g.sym.wide ? wide_symmetric(precise, mp) : units_of_symmetric<128, 128>(mp); });
+    const int64_t upd_units =
+        number_units(g.upd, [&](int mp, int np) { return g.upd.wide ? wide_update(precise, mp, np) : (int64_t)(mp / 128) * (np / 128); });
+    if (std::max(sym_units, upd_units) > 0x3fffffffll) return PK_ERR_SHAPE;
+    const int rc = o.step ? (o.bf16_src ? run_group<bf16_t, true>(g, o, s) : run_group<float, true>(g, o, s))
+                          : (o.bf16_src ? run_group<bf16_t, false>(g, o, s) : run_group<float, false>(g, o, s));
     if (rc != PK_OK) return rc;
   }
   return PK_OK;

@@ -30,9 +30,9 @@ def test_workspace_query():
     assert ws(i64(3), i64(300), i64(100), 1, 1) == 3 * one
     assert ws(i64(1), i64(100), i64(300), 1, 0) == one                      # a short side: the products of float32 in any case
     assert ws(i64(1), i64(200), i64(300), 1, 0) < ws(i64(1), i64(200), i64(300), 1, 1)
-    largest = ws(i64(1), i64(8192), i64(8192), 1, 1)
-    assert ws(i64(1, 5), i64(8192, 10), i64(8192, 10), 2, 1) == largest     # what the largest matrix takes
-    assert ws(i64(100000), i64(128), i64(128), 1, 1) <= 1 << 30             # groups
+    largest = ws(i64(1), i64(16384), i64(16384), 1, 1)
+    assert ws(i64(1, 5), i64(16384, 10), i64(16384, 10), 2, 1) == largest   # what the largest matrix takes
+    assert ws(i64(100000), i64(128), i64(128), 1, 1) <= 2560 << 20          # groups
     assert ws(i64(0, 4), i64(8, 0), i64(8, 8), 2, 1) == 0 == ws(None, None, None, 0, 1)
     refused(ws(i64(1), i64(32769), i64(1), 1, 1), "shape")
     refused(ws(i64(-1), i64(1), i64(1), 1, 1), "argument")
