@@ -182,7 +182,7 @@ PK_API int pk_sort_by_expert_static(const int32_t* top_idx, int64_t A, int64_t E
 
 /* --------------------------------------------- the router's balance loss
  * top_idx [T,K] (i32) are the experts that logits [T,E] (f32) chose.  sequences [S+1] (i32, ascending, within 0 .. T; NULL: S = 1,
- * all tokens): sequence s has the tokens sequences[s] .. sequences[s+1], L of them; tokens outside all of them are padding.
+ * all tokens; S < 2^20): sequence s has the tokens sequences[s] .. sequences[s+1], L of them; tokens outside all of them are padding.
  *   counts[S,E] (i32): how often each expert was chosen in each sequence (ids outside [0,E) are not counted)
  *   f_e = counts_e E / (K L), P_e = mean over the sequence's tokens of softmax(logits)_e
  *   loss[1] (f32) = balance_coeff * mean over the sequences with tokens of sum_e f_e P_e

@@ -12,6 +12,9 @@
 
 namespace pk_balance {
 
+// of a call: every workgroup of the first launch counts the sequences that begin before it, 2^40 reads at this many
+constexpr int64_t kMostSequences = 0xfffff;
+
 // What a backward needs beside the logits.  table: [S][E] of h - mean(h) without the 1 / S', then 1 / S' and 2 z_coeff / N.
 struct Grad {
   const float* table;

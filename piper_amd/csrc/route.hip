@@ -1502,7 +1502,7 @@ int pk_route_topk_balanced_bwd(const float* table, const int32_t* sequences, int
                                const int32_t* top_idx, const float* d_top_scores, int64_t T, int64_t E, int64_t K, int route_norm,
                                float route_scale, float* d_logits, pk_stream_t stream) {
   if (T < 0 || E <= 0 || K <= 0 || S <= 0 || (!sequences && S != 1)) return PK_ERR_ARG;
-  if (E > PK_MAX_EXPERTS || K > PK_MAX_TOPK || K > E || S > 0x3fffffffll) return PK_ERR_SHAPE;
+  if (E > PK_MAX_EXPERTS || K > PK_MAX_TOPK || K > E || S > pk_balance::kMostSequences) return PK_ERR_SHAPE;
   if (T == 0) return PK_OK;
   if (!logits || !top_idx || !d_top_scores || !d_logits || !table || !d_loss) return PK_ERR_ARG;
   RouteBwdIo io = {};
@@ -1635,7 +1635,7 @@ int pk_region_router_balanced_bwd(const float* table, const int32_t* sequences, 
                                   void* d_x, void* d_norm_weight, int64_t T, int64_t H, int64_t E, int64_t K, void* workspace,
                                   int64_t workspace_bytes, pk_stream_t stream) {
   if (S <= 0 || (!sequences && S != 1) || (T > 0 && (!table || !d_loss))) return PK_ERR_ARG;
-  if (S > 0x3fffffffll) return PK_ERR_SHAPE;
+  if (S > pk_balance::kMostSequences) return PK_ERR_SHAPE;
   const pk_balance::Grad bal{table, sequences, d_loss, (int32_t)S};
   if (norm_weight)
     return region_router_norm_bwd(&bal, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype,
