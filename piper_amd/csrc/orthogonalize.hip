@@ -71,6 +71,7 @@ struct Gemm {
   char* ws;
   int32_t n, units, blocks, chunk, wide, splits;      // blocks: of units in the order they are dealt
   int32_t from;          // which of the two X the products read
+  int32_t lower;         // whether UPDATE's result needs its lower plane
   float a, b, c;
 };
 static_assert(sizeof(Gemm) <= 4096, "kernel arguments");
@@ -313,9 +314,9 @@ __global__ __launch_bounds__(kThreads) void convert_kernel(const Ends p) {
   }
 }
 
-// The result (TG), or with STEP the weights and their bf16 copy.
+// The result (TG), or with STEP the weights and their bf16 copy.  lower: whether X has its lower plane.
 template <typename TG, bool STEP>
-__global__ __launch_bounds__(kThreads) void finish_kernel(const Ends p, int from) {
+__global__ __launch_bounds__(kThreads) void finish_kernel(const Ends p, int from, int lower) {
   __shared__ float turned[64][65];
   const Tile t = tile_of(p, blockIdx.x);
   const Entry& e = t.e;
@@ -324,7 +325,7 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const Ends p, int from
   const f16_t* const lo = hi + to_lower(p.precise, e.mp, e.np);
   const auto get = [&](int i, int j, float (&x)[4]) {
     const int64_t at = place(p.precise, t.i0 + i, t.j0 + j, e.np);
-    const f16x4_t h = *reinterpret_cast<const f16x4_t*>(hi + at), l = *reinterpret_cast<const f16x4_t*>(lo + at);
+    const f16x4_t h = *reinterpret_cast<const f16x4_t*>(hi + at), l = lower ? *reinterpret_cast<const f16x4_t*>(lo + at) : f16x4_t{};
 #pragma unroll
     for (int v = 0; v < 4; ++v) x[v] = ((float)h[v] + (float)l[v]) * (1.f / kX);
   };
@@ -706,6 +707,7 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
             }
 #pragma unroll
         for (int pl = 0; pl < (OUT_LO ? 2 : 1); ++pl) {
+          if (KIND == UPDATE && !PRECISE && pl == 1 && !p.lower) break;
           wave_lds_fence();
 #pragma unroll
           for (int j = 0; j < TN; ++j)
@@ -844,16 +846,19 @@ int run_group(Group& g, const Settings& o, hipStream_t s) {
     PK_LAUNCH_NOCHECK(pk_timing::K_MUON_BEGIN, s, (begin_kernel<TG, STEP>), dim3((unsigned)g.chunks[i]), dim3(kThreads), 0, s, g.ends[i]);
   for (int i = 0; i < g.n; ++i)
     PK_LAUNCH_NOCHECK(pk_timing::K_MUON_CONVERT, s, (convert_kernel<TG, STEP>), dim3((unsigned)g.tiles[i]), dim3(kThreads), 0, s, g.ends[i]);
+  // Single products end with the upper plane alone, off by 2^-12 where they are by 2e-3: 16 bits a value less to write and to read
+  const auto lower = [&](int step) { return precise || step == 0 || step < o.steps; };
   int from = 0;
   for (int i = 0; i < o.steps; ++i) {
     g.sym.from = g.upd.from = from;
+    g.upd.lower = lower(i + 1);
     launch_gram(g.sym, precise, s);
     launch_product<POLY>(g.sym, precise, pk_timing::K_NS_POLY, s);
     launch_product<UPDATE>(g.upd, precise, pk_timing::K_NS_UPDATE, s);
     from = 1 - from;
   }
   for (int i = 0; i < g.n; ++i)
-    PK_LAUNCH_NOCHECK(pk_timing::K_MUON_FINISH, s, (finish_kernel<TG, STEP>), dim3((unsigned)g.tiles[i]), dim3(kThreads), 0, s, g.ends[i], from);
+    PK_LAUNCH_NOCHECK(pk_timing::K_MUON_FINISH, s, (finish_kernel<TG, STEP>), dim3((unsigned)g.tiles[i]), dim3(kThreads), 0, s, g.ends[i], from, (int)lower(o.steps));
   PK_RETURN_IF_LAUNCH_FAILED();
   return PK_OK;
 }
