@@ -293,3 +293,45 @@ def test_through_the_dispatcher():
     def step(x, w):
         return F_.expert_region_balanced(x, w, None, t["w1"], t["w2"], t["w3"], top_k=2, route_norm=True)
     assert all(torch.equal(a, b) for a, b in zip(step(t["x"], t["w_gate"]), direct))
+
+
+@pytest.mark.parametrize("E,K", [(200, 8), (300, 8), (600, 8)])
+@pytest.mark.parametrize("S,T", [(3, 400), (150, 1500), (1025, 3000)])
+def test_many_and_few_sequences_of_many_experts(E, K, S, T):
+    """Five, three and one of a workgroup's sequences at once; ragged lengths, a third of them nothing, padding at both ends."""
+    gen = torch.Generator().manual_seed(S + E)
+    cuts = torch.randint(7, T - 7, (S + 1,), generator=gen)
+    cuts[::3] = cuts[1::3][0]
+    check(T, E, K, 1.0, 1e-3, sorted(cuts.tolist()), seed=S, skew=0.5)
+
+
+def test_two_losses_at_once_and_a_captured_one():
+    """On two streams at the same time, and in a graph that is replayed with other inputs between other work: the same bits each time."""
+    cases = [(*inputs(2000, 60, 4, s, 0.5), torch.tensor([0, 100 + s, 700, 700, 1900], dtype=torch.int32)) for s in range(4)]
+
+    def run(x, idx, off):
+        loss, counts = F_.balance_loss(x, idx, z_coeff=1e-3, sequences=off)
+        return loss.detach(), counts, torch.autograd.grad(loss, x)[0]
+    on = [(x.to(DEV).requires_grad_(True), i.to(DEV), o.to(DEV)) for x, i, o in cases]
+    want = [run(*c) for c in on]
+    streams = [torch.cuda.Stream() for _ in on]
+    got = [None] * len(on)
+    for k, s in enumerate(streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got[k] = run(*on[k])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    fixed = (torch.zeros_like(on[0][0]).requires_grad_(True), torch.zeros_like(on[0][1]), torch.zeros_like(on[0][2]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*fixed)
+    for c, w in zip(on, want):
+        with torch.no_grad():
+            for a, b in zip(fixed, c):
+                a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, w))
+        run(*c)

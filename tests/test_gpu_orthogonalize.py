@@ -170,3 +170,80 @@ def test_step_with_half_products():
     for i, s in enumerate(STEP_SHAPES):
         want_w, _ = O.muon_step(ws[i].double(), ms[i].double(), gs[i].double(), lr=0.01, momentum=0.95, weight_decay=0.0)
         assert off(w[i].cpu().double() - ws[i].double(), want_w - ws[i].double()) <= BF16_TOL
+
+
+# ------------------------------------------------------------------------------------------------ many units, long sums, mixed sizes
+# (definitions in 64 bits on the GPU: the library's products of doubles)
+def off_each(a, b):
+    d = (a.double() - b).flatten(1).norm(dim=1) / b.flatten(1).norm(dim=1).clamp_min(1e-300)
+    return d
+
+
+@pytest.mark.parametrize("shape", [(176, 300, 600), (176, 700, 290), (40, 1100, 520), (260, 257, 385)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_enough_matrices_for_wide_tiles(shape, dtype):
+    """Sides whose last wide tile is half a tile or a few rows."""
+    x = torch.cat([matrices((shape[0] // 4, *shape[1:]), 11 + i, kind, dtype).to(DEV) for i, kind in enumerate(["spiked", "rows", "lowrank", "spiked"])])
+    exact = O.orthogonalize(x.double())
+    got = ops.orthogonalize(x)
+    if dtype == torch.float32:
+        assert (off_each(got, exact) <= 2 * off_each(O.orthogonalize(x), exact) + 5 * 2.0 ** -22).all()
+    else:
+        assert (off_each(got, exact) <= BF16_TOL).all()
+    assert torch.equal(ops.orthogonalize(x), got)
+
+
+@pytest.mark.parametrize("shape", [(1, 100, 1900), (1, 200, 1500), (1, 2100, 260), (2, 128, 4000), (1, 1, 5000), (1, 513, 2048)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_few_matrices_of_long_rows(shape, dtype):
+    """X X^T in shares of k, whose numbers do not divide k."""
+    x = matrices(shape, 12, "spiked", dtype).to(DEV)
+    exact = O.orthogonalize(x.double())
+    got = ops.orthogonalize(x)
+    if dtype == torch.float32:
+        assert (off_each(got, exact) <= 2 * off_each(O.orthogonalize(x), exact) + 5 * 2.0 ** -22).all()
+    else:
+        assert (off_each(got, exact) <= BF16_TOL).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_step_of_many_sizes(half):
+    """Small and large matrices, tall and wide ones, single and stacked, in one call: their tiles share launches."""
+    shapes = [(24, 500, 640)] + [(300 + 8 * i, 900 - 8 * i) for i in range(24)] + [(1100, 512)] * 6 + [(5, 100, 70), (64, 1000), (1, 1), (700, 2), (1024, 1024)]
+    w, m, g = ([matrices(s, k + i).to(DEV) * f for i, s in enumerate(shapes)] for k, f in ((20, 20), (60, 1), (100, 1)))
+    start = [(a.double(), b.double(), c.double()) for a, b, c in zip(w, m, g)]
+    hyper = dict(lr=0.05, momentum=0.9, weight_decay=0.0)
+    plain = [O.muon_step(a.clone(), b.clone(), c, **hyper)[0] for a, b, c in zip(w, m, g)]
+    ops.muon_fused(w, m, g, half_products=half, **hyper)
+    for (a, b, c), p, x in zip(start, plain, w):
+        want = O.muon_step(a, b, c, **hyper)[0]
+        size = lambda t: t.double().norm().item()  # noqa: E731
+        update = size(want - a)
+        if half and min(x.shape[-2:]) > 128:      # and a rounding of the weights
+            assert size(x.double() - want) <= BF16_TOL * update + 2.0 ** -23 * size(want)
+        else:
+            assert size(x.double() - want) <= 2 * size(p.double() - want) + 5 * 2.0 ** -22 * update + 2.0 ** -23 * size(want)
+
+
+@pytest.mark.parametrize("shape,dtype", [((3, 200, 1500), torch.bfloat16), ((1, 100, 1900), torch.float32), ((20, 300, 600), torch.bfloat16)])
+def test_two_at_once_and_a_captured_one(shape, dtype):
+    xs = [matrices(shape, 30 + i, dtype=dtype).to(DEV) for i in range(3)]
+    want = [ops.orthogonalize(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = []
+    for x, s in zip(xs, streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(ops.orthogonalize(x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    fixed = torch.zeros_like(xs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.orthogonalize(fixed)
+    for x, w in zip(xs, want):
+        fixed.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, w)
+        ops.orthogonalize(x.float())
