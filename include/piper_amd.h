@@ -653,7 +653,7 @@ PK_API int pk_adamw8_fused_packed(float* master, uint8_t* exp_avg, uint8_t* exp_
  *
  * Bytes of workspace (HOST arrays; n stacks of counts[i] matrices) that a call runs best with: it goes through
  * its matrices in groups of what the workspace holds, which has to be the largest matrix at least
- * (PK_ERR_WORKSPACE), and this is as much as stays in the memory-side cache. */
+ * (PK_ERR_WORKSPACE), and this holds all of them up to 2.5 GiB. */
 #define PK_MAX_MATRIX_SIDE 32768
 PK_API int64_t pk_orthogonalize_workspace_bytes(const int64_t* counts, const int64_t* rows, const int64_t* cols,
                                          int64_t n, int precise);

@@ -1555,6 +1555,13 @@ void muon(const std::vector<Tensor>& masters, const std::vector<Tensor>& momenta
     flat[i] = static_cast<float*>(ptr(flat_i));
     copy[i] = ptr(copy_i);
   }
+  std::vector<std::pair<const char*, const char*>> written;
+  for (size_t i = 0; i < n; ++i)
+    for (const auto& [at, width] : {std::pair<void*, int64_t>{w[i], 4}, {m[i], 4}, {zero_flat ? flat[i] : nullptr, 4}, {copy[i], 2}})
+      if (at && masters[i].numel() > 0) written.emplace_back(static_cast<const char*>(at), static_cast<const char*>(at) + masters[i].numel() * width);
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    TORCH_CHECK_VALUE(written[i - 1].second <= written[i].first, "muon_fused: two of the buffers that are written overlap (a tensor given twice?)");
   const int64_t bytes = pk_orthogonalize_workspace_bytes(size[0].data(), size[1].data(), size[2].data(), (int64_t)n, precise);
   TORCH_CHECK_VALUE(bytes >= 0, "muon_fused: matrices of at most ", PK_MAX_MATRIX_SIDE, " rows and columns");
   const Tensor ws = at::empty({bytes}, masters[0].options().dtype(at::kByte));

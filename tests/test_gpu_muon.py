@@ -244,3 +244,14 @@ def test_a_layer_trained_with_both(dev, dtype):
     assert all(0 < v < 10 for v in losses)
     assert experts.shard_optimizer.state[experts.shard_param]["exp_avg_sq"].numel() == 0
     assert router.shard_optimizer.state[router.shard_param]["exp_avg_sq"].numel() == gate.numel()
+
+
+def test_a_tensor_given_twice_is_refused(dev):
+    w, m, g = (torch.zeros(3, 4, 6, device=dev) for _ in range(3))
+    sh = torch.zeros(4, 6, dtype=torch.bfloat16, device=dev)
+    for args in (dict(masters=[w[0], w[0]]), dict(momenta=[m[1], m[1]]), dict(momenta=[m[0], w[1]]), dict(shadows=[sh, sh]), dict(flat_grads=[g[0], g[0]], zero_grad=True),
+                 dict(masters=[w.view(-1)[:24].view(4, 6), w.view(-1)[20:44].view(4, 6)])):
+        args = dict(masters=[w[0], w[1]], momenta=[m[0], m[1]], grads=[g[0], g[0]]) | args
+        with pytest.raises(ValueError, match="overlap"):
+            ops.muon_fused(args.pop("masters"), args.pop("momenta"), args.pop("grads"), lr=0.1, **args)
+    ops.muon_fused([w[0], w[1], w[2, :0]], [m[0], m[1], m[2, :0]], [g[0], g[0], None], flat_grads=[g[2], g[2], None], lr=0.1)      # read, not written

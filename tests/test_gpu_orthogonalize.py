@@ -247,3 +247,14 @@ def test_two_at_once_and_a_captured_one(shape, dtype):
         torch.cuda.synchronize()
         assert torch.equal(out, w)
         ops.orthogonalize(x.float())
+
+
+def test_more_elements_than_32_bits_count():
+    """2.2e9 of them, in several groups: matrices at either end as by themselves."""
+    x = torch.zeros(2800, 1024, 768, dtype=torch.bfloat16, device=DEV)
+    ends = matrices((4, 1024, 768), 40, dtype=torch.bfloat16).to(DEV)
+    x[:2], x[-2:] = ends[:2], ends[2:]
+    got = ops.orthogonalize(x)
+    exact = O.orthogonalize(ends.double())
+    assert (off_each(torch.cat([got[:2], got[-2:]]), exact) <= BF16_TOL).all()
+    assert not got[2:-2].any()
