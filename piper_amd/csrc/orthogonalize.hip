@@ -67,9 +67,11 @@ struct Ends {
 };
 static_assert(sizeof(Ends) <= 4096, "kernel arguments");
 struct Gemm {
-  struct Shape { int64_t ws, stride; int32_t mp, np, first_unit; } e[kMaxShapes];      // (first_unit: the number of matrices, until they are numbered)
+  // (first_unit: the number of matrices, until they are numbered; first_k: with shares, the pairs of k-tiles before the shape's first unit)
+  struct Shape { int64_t ws, stride; int32_t mp, np, first_unit, first_k; } e[kMaxShapes];
   char* ws;
-  int32_t n, units, blocks, chunk, wide, splits;      // blocks: of units in the order they are dealt
+  int32_t n, units, blocks, chunk, wide;      // blocks: of units in the order they are dealt
+  int32_t shares, pairs, slots;               // X X^T in shares of all units' pairs of k-tiles; a unit's sums lie in `slots` places
   int32_t from;          // which of the two X the products read
   int32_t lower;         // whether UPDATE's result needs its lower plane
   float a, b, c;
@@ -82,12 +84,15 @@ static_assert(sizeof(Gemm) <= 4096, "kernel arguments");
 constexpr int kXLog2 = 12, kALog2 = 8;
 constexpr float kX = 1 << kXLog2, kA = 1 << kALog2;
 
-// Buffers of one matrix: X twice, each as hi and lo; A, B (with precise sums hi and lo); partial sums of squares.
+// Buffers of one matrix: X twice, each as hi and lo; A, B (with precise sums hi and lo); for each wave of the 128 x 128 tiles on and below A's
+// diagonal, how many sums of shares of k there are; partial sums of squares.
 __host__ __device__ inline int64_t plane_x(int mp, int np) { return (int64_t)mp * np * 2; }
 __host__ __device__ inline int64_t plane_a(int mp) { return (int64_t)mp * mp * 2; }
 __host__ __device__ inline int64_t at_a(int mp, int np) { return 4 * plane_x(mp, np); }
 __host__ __device__ inline int64_t at_b(int mp, int np, bool precise) { return at_a(mp, np) + (precise ? 2 : 1) * plane_a(mp); }
-__host__ __device__ inline int64_t at_sums(int mp, int np, bool precise) { return at_a(mp, np) + (precise ? 4 : 2) * plane_a(mp); }
+__host__ __device__ inline int64_t at_counts(int mp, int np, bool precise) { return at_a(mp, np) + (precise ? 4 : 2) * plane_a(mp); }
+__host__ __device__ inline int64_t counts_of(int mp) { return (int64_t)(mp / 128) * (mp / 128 + 1) / 2 * 8; }
+__host__ __device__ inline int64_t at_sums(int mp, int np, bool precise) { return at_counts(mp, np, precise) + counts_of(mp) * 4; }
 __host__ __device__ inline int64_t matrix_bytes(int rows, int cols, int mp, int np, bool precise) {
   const int64_t chunks = ((int64_t)rows * cols + kChunk - 1) / kChunk;
   return (at_sums(mp, np, precise) + chunks * 8 + 255) / 256 * 256;
@@ -174,7 +179,8 @@ __device__ __forceinline__ void begin_piece(const Ends& p, const Entry& e, int64
   for (int k = 0; k < N; ++k) sum += (double)u[k] * u[k];
 }
 
-// Momentum, and the sum of squares of every chunk of a matrix of U, in 64 bits (squares of fp32 values reach past fp32's range).
+// Momentum, and the sum of squares of every chunk of a matrix of U, in 64 bits (squares of fp32 values reach past fp32's range); counts of
+// zero.
 template <typename TG, bool STEP>
 __global__ __launch_bounds__(kThreads) void begin_kernel(const Ends p) {
   __shared__ double part[kThreads / 64];
@@ -185,6 +191,7 @@ __global__ __launch_bounds__(kThreads) void begin_kernel(const Ends p) {
   const int local = blockIdx.x - e.first_chunk, mat = local / chunks, chunk = local % chunks;
   const int64_t base = (int64_t)mat * size + (int64_t)chunk * kChunk;
   const int n = (int)min((int64_t)kChunk, size - (int64_t)chunk * kChunk);
+  char* const mem = p.ws + e.ws + mat * matrix_bytes(e.rows, e.cols, e.mp, e.np, p.precise);
   double sum = 0.0;
   if (n == kChunk && aligned(e, size % 8 == 0)) {
 #pragma unroll
@@ -199,8 +206,11 @@ __global__ __launch_bounds__(kThreads) void begin_kernel(const Ends p) {
   if (threadIdx.x == 0) {
     double s = 0.0;
     for (int w = 0; w < kThreads / 64; ++w) s += part[w];
-    char* const mem = p.ws + e.ws + mat * matrix_bytes(e.rows, e.cols, e.mp, e.np, p.precise);
     reinterpret_cast<double*>(mem + at_sums(e.mp, e.np, p.precise))[chunk] = s;
+  }
+  if (chunk == 0) {
+    uint32_t* const counts = reinterpret_cast<uint32_t*>(mem + at_counts(e.mp, e.np, p.precise));
+    for (int i = threadIdx.x; i < (int)counts_of(e.mp); i += kThreads) counts[i] = 0;
   }
 }
 
@@ -377,7 +387,6 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(const Ends p, int from
 
 // ---------------------------------------------------------------- the products
 enum Product { GRAM, POLY, UPDATE };
-enum Phase { WHOLE, PARTIAL, SUMS };
 
 // Row tiles (of BM) of the BN x BN blocks on and below the diagonal of a symmetric mp x mp result, block row by block row: a full
 // block row r has r + 1 blocks of BN / BM tiles, the last one may be half a block high.
@@ -403,9 +412,10 @@ __host__ __device__ inline int units_of_symmetric(int mp) {
 // and they swap (the k-loop of the grouped products).  k-tiles go straight to LDS, NS - 1 of them ahead.  A k-tile has KT values of k; W
 // fp16 values of a row (both planes with PRECISE).
 //
-// PHASE (GRAM with few units): PARTIAL leaves the sums of one of p.splits shares of k as they are in Xn, which nobody needs then, SUMS adds
-// them up in their order.
-template <int KIND, bool PRECISE, int BM, int BN, int KT, int NS, int PHASE = WHOLE>
+// SHARED (GRAM and POLY with few units, 128 x 128): the pairs of k-tiles of all units, one unit's behind the other's, are cut into
+// p.shares equal shares, one to a workgroup.  A wave leaves its sums of a part of a unit as they are in Xn, which nobody needs then, and
+// counts them; the one that finds the others' there adds them up in their order and goes on to the epilogue.
+template <int KIND, bool PRECISE, int BM, int BN, int KT, int NS, bool SHARED = false>
 __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
   constexpr int NW = 8, WNW = BN / 64, WM = BM / (NW / WNW), TM = WM / 32, TN = 2, KS = KT / 16;
   constexpr int P = PRECISE ? 2 : 1, W = KT * P;
@@ -422,23 +432,32 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
 
   struct Unit {
     int mp, np, N;                                      // N: columns of the result
-    int row0, col0, in_matrix, split, nkt;
+    int row0, col0, in_matrix, part, parts, nkt;        // parts: shares that the unit is in, part: which of them this is
     bool mirrored;                                      // off the diagonal of a symmetric result
     char *X, *Xn, *A, *B;
+    uint32_t* counts;
   };
   Unit u;
   // ---- the loader: a lane's byte offsets from two wave-uniform pointers that advance by a constant per k-tile
   uint32_t va[LA], vb[LB];
   const char *ld_a, *ld_b;
   int64_t step_b;
+  // this workgroup's units: neighbours share operands in an XCD's L2; with SHARED, its pairs of k-tiles
+  int at = SHARED ? (int)(blockIdx.x * p.pairs / p.shares) : (int)blockIdx.x;
+  const int end = SHARED ? (int)((blockIdx.x + 1) * p.pairs / p.shares) : p.blocks;
+  auto share_of = [&](int pair) { return ((pair + 1) * p.shares - 1) / p.pairs; };      // the last that starts at or before it
   auto enter = [&](int dealt) {
-    const int unit = PHASE == PARTIAL ? dealt / p.splits : dealt;
-    u.split = PHASE == PARTIAL ? dealt % p.splits : 0;
-    const int en = entry_of(p.n, unit, [&](int i) { return p.e[i].first_unit; });
+    const int en = entry_of(p.n, dealt, [&](int i) { return SHARED ? p.e[i].first_k : p.e[i].first_unit; });
     const int mp = u.mp = p.e[en].mp, np = u.np = p.e[en].np;
     const int N = u.N = KIND == UPDATE ? np : mp;
     const int tm = (mp + BM - 1) / BM, tn = (N + BN - 1) / BN;
-    const int local = unit - p.e[en].first_unit;
+    const int pairs = (KIND == GRAM ? np : mp) / (2 * KT);       // of k-tiles: k is a multiple of 128
+    const int local = SHARED ? (dealt - p.e[en].first_k) / pairs : dealt - p.e[en].first_unit;
+    const int first_pair = p.e[en].first_k + local * pairs, pair0 = SHARED ? dealt - first_pair : 0;
+    if (SHARED) {
+      u.part = blockIdx.x - share_of(first_pair);
+      u.parts = share_of(first_pair + pairs - 1) - share_of(first_pair) + 1;
+    }
     int mat, mt, nt;
     if (KIND == UPDATE) {
       mat = local / (tm * tn);
@@ -465,12 +484,13 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
     u.Xn = mem + 2 * (1 - p.from) * px;
     u.A = mem + at_a(mp, np);
     u.B = mem + at_b(mp, np, PRECISE);
+    u.counts = reinterpret_cast<uint32_t*>(mem + at_counts(mp, np, PRECISE)) + u.in_matrix * 8;
     const char* const left = KIND == GRAM ? u.X : KIND == POLY ? u.A : u.B;
     const char* const right = KIND == POLY ? u.A : u.X;
     const int lda = (KIND == GRAM ? np : mp) * P, ldb = (KIND == POLY ? mp : np) * P;    // of a row in memory
-    const int pairs = (KIND == GRAM ? np : mp) / (2 * KT);       // of k-tiles: k is a multiple of 128
-    const int kt0 = PHASE == PARTIAL ? 2 * (pairs * u.split / p.splits) : 0;
-    u.nkt = __builtin_amdgcn_readfirstlane(PHASE == PARTIAL ? 2 * (pairs * (u.split + 1) / p.splits) - kt0 : 2 * pairs);
+    const int kt0 = 2 * pair0;
+    u.nkt = __builtin_amdgcn_readfirstlane(2 * (SHARED ? min(pairs - pair0, end - dealt) : pairs));
+    if (SHARED) at = dealt + u.nkt / 2;
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
       int r, k;
@@ -506,13 +526,11 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
       if (s < u.nkt) request(cur + s >= NS ? cur + s - NS : cur + s);
   };
 
-  // this workgroup's units: neighbours share operands in an XCD's L2
-  const int total = PHASE == PARTIAL ? p.units * p.splits : p.units;
-  int at = blockIdx.x;
   auto next = [&]() {                                   // -1: none
-    for (; at < p.blocks; at += gridDim.x) {
+    if (SHARED) return at < end ? at : -1;
+    for (; at < end; at += gridDim.x) {
       const int d = pk_rules::dealt_unit(at, p.chunk);
-      if (d < total) {
+      if (d < p.units) {
         at += gridDim.x;
         return d;
       }
@@ -522,14 +540,14 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
   int dealt = next();
   if (dealt < 0) return;
   enter(dealt);
-  if (PHASE != SUMS) request_first();
+  request_first();
   int stored = 0;                                       // store instructions since those requests
 
   for (;;) {
     const Unit w = u;
     const bool live = w.row0 + wm * WM < w.mp && w.col0 + wn * 64 < w.N;
     floatx16_t acc[TM][TN] = {}, sum[PRECISE ? TM : 1][TN] = {};
-    if constexpr (PHASE != SUMS) {
+    {
       // k-tile 0 has landed once only the younger ones and the stores behind them are on their way
       wait_vm_le((min(w.nkt, NS - 1) - 1) * L + stored);
       block_barrier();
@@ -612,45 +630,52 @@ __global__ __launch_bounds__(512) void product_kernel(const Gemm p) {
     dealt = next();
     if (dealt >= 0) {
       enter(dealt);
-      if (PHASE != SUMS) request_first();
+      request_first();
     }
     stored = 0;
 
-    // where a split's sums are: [unit of the matrix][split][16 bytes of every lane in turn]
-    constexpr int VECS = TM * TN * 4;
-    floatx4_t* part = reinterpret_cast<floatx4_t*>(w.Xn) + ((int64_t)w.in_matrix * (PHASE == WHOLE ? 0 : p.splits) + w.split) * (VECS * 512) +
-                      wave * (VECS * 64) + lane;
-    if (PHASE == PARTIAL && live) {
+    bool last = true;
+    if (SHARED && live && w.parts > 1) {
+      // [unit of the matrix][slot][8 bytes of every lane in turn].  Other XCDs read them: these stores go through the L2 to memory and the loads
+      // past it, which costs less than fences, each of which walks a whole L2 (2048 x 4096 in fp32: X X^T 162 us with fences).
+      typedef uint32_t uintx2_t __attribute__((ext_vector_type(2)));
+      constexpr int VECS = TM * TN * 8;
+      uint64_t* const sums = reinterpret_cast<uint64_t*>(w.Xn) + (int64_t)w.in_matrix * p.slots * (VECS * 512) + wave * (VECS * 64) + lane;
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            floatx4_t v;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * q + k];
-            part[((i * TN + j) * 4 + q) * 64] = v;
+          for (int q = 0; q < 8; ++q) {
+            const uintx2_t v = {__float_as_uint(acc[i][j][2 * q]), __float_as_uint(acc[i][j][2 * q + 1])};
+            __hip_atomic_store(sums + (int64_t)w.part * (VECS * 512) + ((i * TN + j) * 8 + q) * 64, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
           }
-      stored = VECS;
-    }
-    if (PHASE == SUMS && live) {
-      for (int z = 0; z < p.splits; ++z, part += VECS * 512)
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // they are there
+      uint32_t before = 0;
+      if (lane == 0) before = __hip_atomic_fetch_add(w.counts + wave, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = __builtin_amdgcn_readfirstlane(before) == (uint32_t)w.parts - 1;
+      asm volatile("" ::: "memory");
+      if (last) {
+        if (lane == 0) __hip_atomic_store(w.counts + wave, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);      // (for the next launch)
+        for (int z = 0; z < w.parts; ++z)
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+          for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int j = 0; j < TN; ++j)
+            for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const floatx4_t v = part[((i * TN + j) * 4 + q) * 64];
+              for (int q = 0; q < 8; ++q) {
+                const uintx2_t v = __builtin_bit_cast(uintx2_t, __hip_atomic_load(sums + (int64_t)z * (VECS * 512) + ((i * TN + j) * 8 + q) * 64,
+                                                                                  __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 #pragma unroll
-              for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] += v[k];
-            }
+                for (int k = 0; k < 2; ++k) acc[i][j][2 * q + k] = z == 0 ? __uint_as_float(v[k]) : acc[i][j][2 * q + k] + __uint_as_float(v[k]);
+              }
+      }
     }
     // ---- epilogue, 32 rows of a wave at a time.  acc[i][j][v] is row 32 i + lane % 32, column 32 j + 8 (v / 4) + 4 (lane / 32) + v % 4.  Memory
     // is read and written 16 bytes a lane, 64 columns a row; LDS turns one into the other: fp16 rows of 128 bytes, their 16-byte
     // pieces swizzled by the row, in the stage that the coming k-tiles leave free.
-    if (PHASE != PARTIAL && live) {
+    if (last && live) {
       const int ldc = w.N;
       const int64_t lower = to_lower(PRECISE, w.mp, ldc) * 2;     // bytes
       char* const out = KIND == GRAM ? w.A : KIND == POLY ? w.B : w.Xn;
@@ -776,6 +801,12 @@ template <int KIND>
 void launch_product(const Gemm& g, bool precise, int id, hipStream_t s) {
   const dim3 grid(std::min<unsigned>(g.blocks, kGrid)), block(512);
 #define PK_LAUNCH(...) PK_LAUNCH_NOCHECK(id, s, (product_kernel<KIND, __VA_ARGS__>), grid, block, 0, s, g)
+  if constexpr (KIND != UPDATE)
+    if (g.shares > 0) {
+      const dim3 grid(g.shares);
+      if (precise) PK_LAUNCH(true, 128, 128, 32, 4, true); else PK_LAUNCH(false, 128, 128, 64, 4, true);
+      return;
+    }
   if (g.wide) { if (precise) PK_LAUNCH(true, 128, 256, 32, 3); else PK_LAUNCH(false, 256, 256, 32, 4); }
   else if (precise) PK_LAUNCH(true, 128, 128, 32, 4);
   else PK_LAUNCH(false, 128, 128, 64, 4);
@@ -785,20 +816,6 @@ void deal(Gemm& g, int64_t units) {
   g.chunk = (int32_t)pk_rules::deal_chunk(units, 32);
   g.blocks = (int32_t)pk_rules::dealt_blocks(units, g.chunk);
 }
-void launch_gram(const Gemm& g, bool precise, hipStream_t s) {
-  if (g.splits == 1) return launch_product<GRAM>(g, precise, pk_timing::K_NS_GRAM, s);
-  Gemm shares = g;
-  deal(shares, (int64_t)g.units * g.splits);
-  const dim3 grid(std::min<unsigned>(shares.blocks, kGrid)), sums(std::min<unsigned>(g.blocks, kGrid)), block(512);
-  const int id = pk_timing::K_NS_GRAM;
-  if (precise) {
-    PK_LAUNCH_NOCHECK(id, s, (product_kernel<GRAM, true, 128, 128, 32, 4, PARTIAL>), grid, block, 0, s, shares);
-    PK_LAUNCH_NOCHECK(id, s, (product_kernel<GRAM, true, 128, 128, 32, 4, SUMS>), sums, block, 0, s, g);
-  } else {
-    PK_LAUNCH_NOCHECK(id, s, (product_kernel<GRAM, false, 128, 128, 64, 4, PARTIAL>), grid, block, 0, s, shares);
-    PK_LAUNCH_NOCHECK(id, s, (product_kernel<GRAM, false, 128, 128, 64, 4, SUMS>), sums, block, 0, s, g);
-  }
-}
 int64_t wide_symmetric(bool precise, int mp) { return precise ? units_of_symmetric<128, 256>(mp) : units_of_symmetric<256, 256>(mp); }
 int64_t wide_update(bool precise, int mp, int np) { return pk_ceil_div(mp, kWideRows[precise]) * pk_ceil_div(np, 256); }
 template <typename F>
@@ -807,17 +824,32 @@ int64_t count_units(const Gemm& g, F&& per) {
   for (int i = 0; i < g.n; ++i) units += g.e[i].first_unit * (int64_t)per(g.e[i].mp, g.e[i].np);
   return units;
 }
-// Shares of k that X X^T is cut into: as many as fit Xn and give every CU a unit, of eight k-tiles of 32 at least, where they save
-// sixteen or more.
-int gram_splits(const Gemm& g, int64_t units) {
-  int64_t splits = 256 / std::max<int64_t>(units, 1), longest = 0;
-  for (int i = 0; i < g.n; ++i) {
-    const Gemm::Shape& e = g.e[i];
-    splits = std::min(splits, 2 * plane_x(e.mp, e.np) / (units_of_symmetric<128, 128>(e.mp) * (int64_t)(128 * 128 * 4)));
-    splits = std::min<int64_t>(splits, e.np / 256);
-    longest = std::max<int64_t>(longest, e.np / 32);
+// Whether X X^T (A A with poly) of `units` (at most one to a CU) is cut into shares, of at least 256 values of k: where a unit's sums fit Xn
+// and the longest unit is kLeastSaved k-tiles of 32 longer than a share, about what leaving and adding the sums takes.  2048 x 4096 in fp32,
+// 136 units: X X^T (60 k-tiles saved of 128) 101 -> 81 us, A A (30 of 64) 57 -> 53; 128 x 2048, one unit: the orthogonalization 188 -> 180
+// against shares whose sums a second launch adds up, which 2048 x 4096 runs in 1,147 us and this in 1,058.
+constexpr int kLeastSaved = 16;
+void cut(Gemm& g, bool precise, bool poly, int64_t units) {
+  if (units == 0 || units > kGrid) return;
+  const int64_t per_pair = precise ? 64 : 128;          // values of k
+  int64_t pairs = 0, longest = 0;
+  for (int i = 0, at = 0; i < g.n; ++i) {
+    const int64_t matrices = g.e[i].first_unit, of_unit = (poly ? g.e[i].mp : g.e[i].np) / per_pair;
+    g.e[i].first_k = at;
+    pairs += matrices * units_of_symmetric<128, 128>(g.e[i].mp) * of_unit;
+    at = (int)pairs;
+    longest = std::max(longest, of_unit);
   }
-  return splits < 2 || longest - longest / splits < 16 ? 1 : (int)splits;
+  const auto slots = [&](int64_t shares) {              // a unit's ends may lie inside shares, unless shares and units end together
+    const bool whole = g.n == 1 && shares % units == 0;
+    return pk_ceil_div(longest * shares, pairs) + (whole ? 0 : 1);
+  };
+  int64_t room = kGrid + 1, shares = std::min<int64_t>(kGrid, pairs * per_pair / 256);
+  for (int i = 0; i < g.n; ++i)
+    room = std::min(room, 2 * plane_x(g.e[i].mp, g.e[i].np) / (units_of_symmetric<128, 128>(g.e[i].mp) * (int64_t)(128 * 128 * 4)));
+  while (shares > units && slots(shares) > room) --shares;
+  if (shares <= units || (longest - pk_ceil_div(pairs, shares)) * per_pair < kLeastSaved * 32) return;
+  g.shares = (int)shares; g.pairs = (int)pairs; g.slots = (int)slots(shares);
 }
 // Units of a launch: per(mp, np) of them for each matrix.
 template <typename F>
@@ -837,7 +869,7 @@ struct Group {
   Ends ends[kMaxEnds];
   int64_t chunks[kMaxEnds], tiles[kMaxEnds];            // workgroups of the launches
   int n;
-  Gemm sym, upd;
+  Gemm sym, poly, upd;
 };
 template <typename TG, bool STEP>
 int run_group(Group& g, const Settings& o, hipStream_t s) {
@@ -850,10 +882,10 @@ int run_group(Group& g, const Settings& o, hipStream_t s) {
   const auto lower = [&](int step) { return precise || step == 0 || step < o.steps; };
   int from = 0;
   for (int i = 0; i < o.steps; ++i) {
-    g.sym.from = g.upd.from = from;
+    g.sym.from = g.poly.from = g.upd.from = from;
     g.upd.lower = lower(i + 1);
-    launch_gram(g.sym, precise, s);
-    launch_product<POLY>(g.sym, precise, pk_timing::K_NS_POLY, s);
+    launch_product<GRAM>(g.sym, precise, pk_timing::K_NS_GRAM, s);
+    launch_product<POLY>(g.poly, precise, pk_timing::K_NS_POLY, s);
     launch_product<UPDATE>(g.upd, precise, pk_timing::K_NS_UPDATE, s);
     from = 1 - from;
   }
@@ -937,8 +969,15 @@ int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspa
     g.sym = g.upd = sym;
     g.sym.wide = count_units(sym, [&](int mp, int) { return wide_symmetric(precise, mp); }) >= kWideSymmetric;
     g.upd.wide = count_units(sym, [&](int mp, int np) { return wide_update(precise, mp, np); }) >= kWideUpdate;
-    g.sym.splits = g.sym.wide ? 1 : gram_splits(sym, count_units(sym, [](int mp, int) { return units_of_symmetric<128, 128>(mp); }));
-    const int64_t sym_units = number_units(g.sym, [&](int mp, int) { return g.sym.wide ? wide_symmetric(precise, mp) : units_of_symmetric<128, 128>(mp); });
+    g.poly = g.sym;
+    if (!g.sym.wide) {
+      const int64_t units = count_units(sym, [](int mp, int) { return units_of_symmetric<128, 128>(mp); });
+      cut(g.sym, precise, false, units);
+      cut(g.poly, precise, true, units);
+    }
+    const auto of_symmetric = [&](int mp, int) { return g.sym.wide ? wide_symmetric(precise, mp) : units_of_symmetric<128, 128>(mp); };
+    const int64_t sym_units = number_units(g.sym, of_symmetric);
+    number_units(g.poly, of_symmetric);
     const int64_t upd_units =
         number_units(g.upd, [&](int mp, int np) { return g.upd.wide ? wide_update(precise, mp, np) : (int64_t)(mp / 128) * (np / 128); });
     if (std::max(sym_units, upd_units) > 0x3fffffffll) return PK_ERR_SHAPE;
