@@ -7,13 +7,13 @@
 // (nesterov; otherwise m), w <- w (1 - lr decay) - lr s X.
 //
 // Numbers.  X lives between the products as two planes of fp16 (hi + lo: 22 bits), scaled by a power of two so that its typical
-// value is near 1; A and B, whose values are at most a few units and whose absolute error is what counts beside a X, as they
-// are.  All sums are fp32.  Results in bf16 come from single products, of the upper planes alone, with a X from both: an error of a
+// value is near 1, A times 2^8, B as it is: their values are at most a few units and their absolute error is what counts beside
+// a X.  All sums are fp32.  Results in bf16 come from single products, of the upper planes alone, with a X from both: an error of a
 // product is bounded by the strong directions and turns them a little, while an error of X itself, a full matrix of noise, grows with
 // the weak ones, up to 3.4 times a step.  (256 x 683, relative to 64 bits: gradients with 8 strong directions 4e-4 as
 // here, 0.04 with X in one plane, 0.3 with everything in bf16; random ones 1.7e-3, the rounding to bf16 by itself 1.7e-3.)  Results
-// in fp32 (and the fp32 weights of the step) take three products, hi hi + lo hi + hi lo, of all operands: 2e-6 to 3e-5,
-// what products in fp32 give, at three times the matrix operations of the other and a third of the time of fp32 instructions.
+// in fp32 (and the fp32 weights of the step) take three products, hi hi + lo hi + hi lo, of all operands: 1e-6 to 2e-6,
+// what products in fp32 give or less, at three times the matrix operations of the other and a third of the time of fp32 instructions.
 // So do bf16 ones of matrices with a side of at most 128: errors of a few directions do not average out (7e-3 of 3 x 1100), and
 // these matrices cost next to nothing.
 //
@@ -41,8 +41,7 @@ constexpr int kMaxEntries = 40, kMaxEnds = 8, kMaxShapes = 100;
 constexpr int kChunk = 8192;                 // elements a workgroup of begin_kernel takes
 constexpr int kThreads = 256;
 // Workspace that is asked for.  Groups that stay in the 256 MiB memory-side cache leave too few workgroups a launch, whose last round is
-// rarely full: 128 matrices of 768 x 2048, bf16 / fp32 results, ms with 192 MiB 8.6 / 14.5, 384 6.4 / 12.8, 768 6.1 / 11.2, 1,536 5.6 / 10.6, all at
-// once 5.2 / 10.1.
+// rarely full: 128 matrices of 768 x 2048, bf16 / fp32 results, ms with 192 MiB 8.1 / 12.8, 384 6.2 / 11.4, 768 5.4 / 11.0, 1,536 5.0 / 9.9, 2,560 4.5 / 9.6.
 constexpr int64_t kGroupBytes = 2560ll << 20;
 
 // Matrices of one shape that lie one behind the other, as the kernels at both ends see them.
@@ -788,13 +787,15 @@ int64_t bytes_of(int64_t rows, int64_t cols, bool precise) {
 }
 bool sides_ok(int64_t rows, int64_t cols) { return rows <= PK_MAX_MATRIX_SIDE && cols <= PK_MAX_MATRIX_SIDE; }
 
-// The tiles: wide ones, 256 x 256 (single products) or 128 x 256, where a launch has this many of them, 128 x 128 otherwise.  us of the five
-// steps, wide -> narrow, X X^T and A A together / the update, with wide tiles of the former / the latter in brackets: 24 x 256 x 512, fp32,
-// 208 -> 173 / 92 -> 78 (48 / 96); 24 x 363 x 1000, bf16, 248 -> 145 / 122 -> 147 (72 / 192), fp32 347 -> 264 / 208 -> 229 (144 / 288); 2048 x 4096,
-// fp32, 1,027 -> 750 / 471 -> 590 (72 / 256), bf16 718 -> 349 / 285 -> 287 (36 / 128); 16 x 768 x 2048, fp32, 766 -> 784 / 690 -> 761 (192 / 768);
-// 64 x 512 x 512, fp32, 695 -> 602 / 346 -> 393 (384 / 512); 128 x 768 x 2048, bf16, 2,013 -> 2,052 / 2,542 -> 3,468 (384 / 1,536 in each of two
-// groups), fp32 4,785 -> 5,062 / 4,941 -> 5,903 (624 / 2,496).  (Half of a wide tile on the diagonal is of no use.)
-constexpr int64_t kWideSymmetric = 512, kWideUpdate = 160;
+// The tiles: wide ones, 256 x 256 (single products) or 128 x 256, or 128 x 128, by the rounds that their units take on the CUs; a round of wide
+// ones takes 2.5 to 3 (1.5 to 1.75 with three products) of the others.  us of the five steps, wide / narrow, X X^T and A A together, the
+// update, and in brackets their wide units: 24 x 256 x 512, fp32, 225 / 174, 97 / 80 (48, 96); 24 x 363 x 1000, bf16, 244 / 147, 127 / 154 (72, 192),
+// fp32 351 / 260, 223 / 220 (96, 288); 2048 x 4096, fp32, 1,020 / 644, 483 / 636 (72, 256), bf16 695 / 389, 285 / 270 (36, 128); 16 x 768 x 2048, fp32,
+// 726 / 797, 657 / 753 (192, 768); 64 x 512 x 512, fp32, 612 / 599, 318 / 368 (384, 512); 128 x 768 x 2048, bf16, 1,713 / 1,923, 2,342 / 3,256
+// (768, 3,072), fp32 4,261 / 4,456, 4,541 / 5,661 (1,536, 6,144).  (Half of a wide tile on the diagonal is of no use.)
+bool pays_wide(bool precise, int64_t wide, int64_t narrow) {
+  return pk_ceil_div(wide, 256) * (precise ? 5 / 3.0 : 11 / 4.0) < (double)pk_ceil_div(narrow, 256);
+}
 constexpr int kWideRows[2] = {256, 128};               // [precise]
 constexpr unsigned kGrid = 256;                         // workgroups at most, one to a CU; each takes every kGrid-th unit
 template <int KIND>
@@ -967,13 +968,14 @@ int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspa
     // long products first: what is left for the end is short
     std::sort(sym.e, sym.e + sym.n, [](const auto& x, const auto& y) { return (int64_t)x.mp * x.np > (int64_t)y.mp * y.np; });
     g.sym = g.upd = sym;
-    g.sym.wide = count_units(sym, [&](int mp, int) { return wide_symmetric(precise, mp); }) >= kWideSymmetric;
-    g.upd.wide = count_units(sym, [&](int mp, int np) { return wide_update(precise, mp, np); }) >= kWideUpdate;
+    const int64_t narrow_sym = count_units(sym, [](int mp, int) { return units_of_symmetric<128, 128>(mp); });
+    g.sym.wide = pays_wide(precise, count_units(sym, [&](int mp, int) { return wide_symmetric(precise, mp); }), narrow_sym);
+    g.upd.wide = pays_wide(precise, count_units(sym, [&](int mp, int np) { return wide_update(precise, mp, np); }),
+                           count_units(sym, [](int mp, int np) { return (int64_t)(mp / 128) * (np / 128); }));
     g.poly = g.sym;
     if (!g.sym.wide) {
-      const int64_t units = count_units(sym, [](int mp, int) { return units_of_symmetric<128, 128>(mp); });
-      cut(g.sym, precise, false, units);
-      cut(g.poly, precise, true, units);
+      cut(g.sym, precise, false, narrow_sym);
+      cut(g.poly, precise, true, narrow_sym);
     }
     const auto of_symmetric = [&](int mp, int) { return g.sym.wide ? wide_symmetric(precise, mp) : units_of_symmetric<128, 128>(mp); };
     const int64_t sym_units = number_units(g.sym, of_symmetric);

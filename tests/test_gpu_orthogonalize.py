@@ -179,7 +179,7 @@ def off_each(a, b):
     return d
 
 
-@pytest.mark.parametrize("shape", [(176, 300, 600), (176, 700, 290), (40, 1100, 520), (260, 257, 385)])
+@pytest.mark.parametrize("shape", [(176, 300, 600), (176, 700, 290), (40, 1100, 520), (260, 257, 385), (102, 800, 900), (16, 700, 1500), (128, 700, 800)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_enough_matrices_for_wide_tiles(shape, dtype):
     """Sides whose last wide tile is half a tile or a few rows."""
