@@ -792,7 +792,7 @@ bool sides_ok(int64_t rows, int64_t cols) { return rows <= PK_MAX_MATRIX_SIDE &&
 // update, and in brackets their wide units: 24 x 256 x 512, fp32, 225 / 174, 97 / 80 (48, 96); 24 x 363 x 1000, bf16, 244 / 147, 127 / 154 (72, 192),
 // fp32 351 / 260, 223 / 220 (96, 288); 2048 x 4096, fp32, 1,020 / 644, 483 / 636 (72, 256), bf16 695 / 389, 285 / 270 (36, 128); 16 x 768 x 2048, fp32,
 // 726 / 797, 657 / 753 (192, 768); 64 x 512 x 512, fp32, 612 / 599, 318 / 368 (384, 512); 128 x 768 x 2048, bf16, 1,713 / 1,923, 2,342 / 3,256
-// (768, 3,072), fp32 4,261 / 4,456, 4,541 / 5,661 (1,536, 6,144).  (Half of a wide tile on the diagonal is of no use.)
+// (3 and 12 rounds), fp32 4,261 / 4,456, 4,541 / 5,661 (6 and 24).  (Half of a wide tile on the diagonal is of no use.)
 bool pays_wide(bool precise, int64_t wide, int64_t narrow) {
   return pk_ceil_div(wide, 256) * (precise ? 5 / 3.0 : 11 / 4.0) < (double)pk_ceil_div(narrow, 256);
 }
