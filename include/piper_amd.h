@@ -201,16 +201,14 @@ PK_API int pk_balance_loss_bwd(const float* logits, const int32_t* sequences, co
 PK_API int pk_route_topk_balanced_bwd(const float* table, const int32_t* sequences, int64_t S, const float* d_loss,
                                const float* logits, const int32_t* top_idx, const float* d_top_scores, int64_t T,
                                int64_t E, int64_t K, int route_norm, float route_scale, float* d_logits, pk_stream_t stream);
-/* pk_region_router_norm_bwd (norm_weight NULL: pk_region_router_bwd of xn and d_xn; x, rstd, d_x_addend, d_x, d_norm_weight are not
- * looked at) with the gradient of the balance loss of these logits added to d_logits on the way.  Workspace as theirs. */
+/* pk_region_router_bwd with that gradient added to d_logits on the way.  Workspace as its. */
 PK_API int pk_region_router_balanced_bwd(const float* table, const int32_t* sequences, int64_t S, const float* d_loss,
                                   const float* logits, const int32_t* top_idx, const float* d_top_scores,
                                   const float* ds_partial, int64_t n_partial, const int32_t* inv_perm, int route_norm,
-                                  float route_scale, const void* xn, int x_dtype, const float* w_gate, const void* d_rows,
-                                  void* d_xn, float* d_w_gate, float* d_gate_bias, int accumulate, float* d_logits,
-                                  const void* x, const void* norm_weight, const float* rstd, const void* d_x_addend, void* d_x,
-                                  void* d_norm_weight, int64_t T, int64_t H, int64_t E, int64_t K, void* workspace,
-                                  int64_t workspace_bytes, pk_stream_t stream);
+                                  float route_scale, const void* x, int x_dtype, const float* w_gate, const void* d_rows,
+                                  void* d_x, float* d_w_gate, float* d_gate_bias, int accumulate, float* d_logits, int64_t T,
+                                  int64_t H, int64_t E, int64_t K, void* workspace, int64_t workspace_bytes,
+                                  pk_stream_t stream);
 
 /* starts[E+1] (i32) from counts[E] given as int32 (counts_is_i64 == 0) or int64.
  * For callers that hand pk_grouped_swiglu_* a `num_tokens_per_expert` tensor

@@ -140,7 +140,7 @@ SIGNATURES = {
 }
 # table sequences S d_loss, then as pk_region_router_norm_bwd
 SIGNATURES["pk_route_topk_balanced_bwd"] = (_c_int, [_p, _p, _c_i64, _p, *SIGNATURES["pk_route_topk_bwd"][1]])
-SIGNATURES["pk_region_router_balanced_bwd"] = (_c_int, [_p, _p, _c_i64, _p, *SIGNATURES["pk_region_router_norm_bwd"][1]])
+SIGNATURES["pk_region_router_balanced_bwd"] = (_c_int, [_p, _p, _c_i64, _p, *SIGNATURES["pk_region_router_bwd"][1]])
 SIGNATURES.update({f"{name}_short": SIGNATURES[name] for name in
                    ("pk_fp8_gate_up", "pk_fp8_down", "pk_fp8_dgrad_dh", "pk_fp8_dgrad_dh_t", "pk_fp8_dgrad_dx")})
 

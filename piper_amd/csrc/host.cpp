@@ -651,24 +651,20 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
       if (need_xn) d_x = at::empty({s.T, s.H}, x.options());
       const float *const d_s = n_part > 0 ? nullptr : t.f32(d_scores), *const parts = t.f32(part);
       float *const dwg = static_cast<float*>(ptr(d_wg)), *const db = static_cast<float*>(ptr(d_b));
-      const bool with_norm = norm && need_xn;
-      if (with_norm && need[NORM_W]) d_norm_w = at::empty({s.H}, norm_w.options());
-      if (d_loss.defined()) {
+      if (d_loss.defined()) {               // (there is no norm in front of a region with a balance loss)
         PK_CALL(pk_region_router_balanced_bwd, fptr(table), sequences.defined() ? sequences.data_ptr<int32_t>() : nullptr,
                 sequences.defined() ? sequences.size(0) - 1 : 1, fptr(d_loss), m.f32(sv.logits), m.i32(sv.idx), d_s, parts, n_part, m.i32(sv.inv),
-                s.route_norm, (float)s.route_scale, x_rows, s.dtype, fptr(w_gate), t.at_(d_xs),
-                with_norm ? t.at_(d_xn) : need_xn ? ptr(d_x) : nullptr, dwg, db, 0, w.f32(d_logits), with_norm ? ptr(xc) : nullptr,
-                with_norm ? ptr(contig(norm_w)) : nullptr, with_norm ? m.f32(sv.rstd) : nullptr, with_norm ? ptr(d_out) : nullptr,
-                with_norm ? ptr(d_x) : nullptr, ptr(d_norm_w), s.T, s.H, s.E, s.K, t.at_(router_ws), router_ws_bytes, st);
-        if (with_norm && !need[X]) d_x = Tensor();
+                s.route_norm, (float)s.route_scale, x_rows, s.dtype, fptr(w_gate), t.at_(d_xs), need_xn ? ptr(d_x) : nullptr, dwg, db, 0,
+                w.f32(d_logits), s.T, s.H, s.E, s.K, t.at_(router_ws), router_ws_bytes, st);
         return;
       }
-      if (!with_norm) {
+      if (!norm || !need_xn) {
         PK_CALL(pk_region_router_bwd, m.f32(sv.logits), m.i32(sv.idx), d_s, parts, n_part, m.i32(sv.inv), s.route_norm, (float)s.route_scale,
                 x_rows, s.dtype, fptr(w_gate), t.at_(d_xs), need_xn ? ptr(d_x) : nullptr, dwg, db, 0, w.f32(d_logits), s.T, s.H, s.E, s.K,
                 t.at_(router_ws), router_ws_bytes, st);
         return;
       }
+      if (need[NORM_W]) d_norm_w = at::empty({s.H}, norm_w.options());
       PK_CALL(pk_region_router_norm_bwd, m.f32(sv.logits), m.i32(sv.idx), d_s, parts, n_part, m.i32(sv.inv), s.route_norm, (float)s.route_scale,
               x_rows, s.dtype, fptr(w_gate), t.at_(d_xs), t.at_(d_xn), dwg, db, 0, w.f32(d_logits), ptr(xc), ptr(contig(norm_w)), m.f32(sv.rstd),
               ptr(d_out), ptr(d_x), ptr(d_norm_w), s.T, s.H, s.E, s.K, t.at_(router_ws), router_ws_bytes, st);

@@ -1594,57 +1594,36 @@ int64_t pk_region_router_norm_bwd_workspace_bytes(int64_t T, int64_t H, int64_t 
   return router < 0 ? router : align256(router) + pk_rmsnorm_bwd_workspace_bytes(T, H);
 }
 
-}  // extern "C"
-
-static int region_router_norm_bwd(const pk_balance::Grad* bal, const float* logits, const int32_t* top_idx, const float* d_top_scores,
-                                  const float* ds_partial, int64_t n_partial, const int32_t* inv_perm, int route_norm, float route_scale,
-                                  const void* xn, int x_dtype, const float* w_gate, const void* d_rows, void* d_xn, float* d_w_gate,
-                                  float* d_gate_bias, int accumulate, float* d_logits, const void* x, const void* norm_weight, const float* rstd,
-                                  const void* d_x_addend, void* d_x, void* d_norm_weight, int64_t T, int64_t H, int64_t E, int64_t K,
-                                  void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
-  if (T < 0 || H <= 0 || E <= 0 || !pk_dtype_ok(x_dtype)) return PK_ERR_ARG;
-  if (T > 0 && (!d_xn || !x || !norm_weight || !rstd || !d_x)) return PK_ERR_ARG;
-  const int64_t router = align256(pk_region_router_bwd_workspace_bytes(T, H, E, x_dtype));
-  if (!workspace || workspace_bytes < pk_region_router_norm_bwd_workspace_bytes(T, H, E, x_dtype)) return PK_ERR_WORKSPACE;
-  GateTail tail = {};
-  const int rc = region_router_bwd(bal, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype, w_gate,
-                                   d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, T, H, E, K, workspace, router, &tail, stream);
-  if (rc != PK_OK) return rc;
-  return pk_rmsnorm_bwd_with_tail(d_xn, x, x_dtype, norm_weight, rstd, d_x_addend, d_x, d_norm_weight, accumulate, T, H,
-                                  reinterpret_cast<char*>(workspace) + router, workspace_bytes - router, tail, (hipStream_t)stream);
-}
-
-extern "C" {
-
 int pk_region_router_norm_bwd(const float* logits, const int32_t* top_idx, const float* d_top_scores, const float* ds_partial,
                               int64_t n_partial, const int32_t* inv_perm, int route_norm, float route_scale, const void* xn, int x_dtype,
                               const float* w_gate, const void* d_rows, void* d_xn, float* d_w_gate, float* d_gate_bias, int accumulate,
                               float* d_logits, const void* x, const void* norm_weight, const float* rstd, const void* d_x_addend,
                               void* d_x, void* d_norm_weight, int64_t T, int64_t H, int64_t E, int64_t K, void* workspace,
                               int64_t workspace_bytes, pk_stream_t stream) {
-  return region_router_norm_bwd(nullptr, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype,
-                                w_gate, d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, x, norm_weight, rstd, d_x_addend, d_x,
-                                d_norm_weight, T, H, E, K, workspace, workspace_bytes, stream);
+  if (T < 0 || H <= 0 || E <= 0 || !pk_dtype_ok(x_dtype)) return PK_ERR_ARG;
+  if (T > 0 && (!d_xn || !x || !norm_weight || !rstd || !d_x)) return PK_ERR_ARG;
+  const int64_t router = align256(pk_region_router_bwd_workspace_bytes(T, H, E, x_dtype));
+  if (!workspace || workspace_bytes < pk_region_router_norm_bwd_workspace_bytes(T, H, E, x_dtype)) return PK_ERR_WORKSPACE;
+  GateTail tail = {};
+  const int rc = region_router_bwd(nullptr, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype, w_gate,
+                                   d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, T, H, E, K, workspace, router, &tail, stream);
+  if (rc != PK_OK) return rc;
+  return pk_rmsnorm_bwd_with_tail(d_xn, x, x_dtype, norm_weight, rstd, d_x_addend, d_x, d_norm_weight, accumulate, T, H,
+                                  reinterpret_cast<char*>(workspace) + router, workspace_bytes - router, tail, (hipStream_t)stream);
 }
 
 int pk_region_router_balanced_bwd(const float* table, const int32_t* sequences, int64_t S, const float* d_loss, const float* logits,
                                   const int32_t* top_idx, const float* d_top_scores, const float* ds_partial, int64_t n_partial,
-                                  const int32_t* inv_perm, int route_norm, float route_scale, const void* xn, int x_dtype,
-                                  const float* w_gate, const void* d_rows, void* d_xn, float* d_w_gate, float* d_gate_bias, int accumulate,
-                                  float* d_logits, const void* x, const void* norm_weight, const float* rstd, const void* d_x_addend,
-                                  void* d_x, void* d_norm_weight, int64_t T, int64_t H, int64_t E, int64_t K, void* workspace,
-                                  int64_t workspace_bytes, pk_stream_t stream) {
+                                  const int32_t* inv_perm, int route_norm, float route_scale, const void* x, int x_dtype, const float* w_gate,
+                                  const void* d_rows, void* d_x, float* d_w_gate, float* d_gate_bias, int accumulate, float* d_logits,
+                                  int64_t T, int64_t H, int64_t E, int64_t K, void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
   if (S <= 0 || (!sequences && S != 1) || (T > 0 && (!table || !d_loss))) return PK_ERR_ARG;
   if (S > pk_balance::kMostSequences) return PK_ERR_SHAPE;
   const pk_balance::Grad bal{table, sequences, d_loss, (int32_t)S};
-  if (norm_weight)
-    return region_router_norm_bwd(&bal, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype,
-                                  w_gate, d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, x, norm_weight, rstd, d_x_addend, d_x,
-                                  d_norm_weight, T, H, E, K, workspace, workspace_bytes, stream);
   GateTail tail = {};
-  const int rc = region_router_bwd(&bal, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, xn, x_dtype,
-                                   w_gate, d_rows, d_xn, d_w_gate, d_gate_bias, accumulate, d_logits, T, H, E, K, workspace, workspace_bytes,
-                                   &tail, stream);
+  const int rc = region_router_bwd(&bal, logits, top_idx, d_top_scores, ds_partial, n_partial, inv_perm, route_norm, route_scale, x, x_dtype, w_gate,
+                                   d_rows, d_x, d_w_gate, d_gate_bias, accumulate, d_logits, T, H, E, K, workspace, workspace_bytes, &tail,
+                                   stream);
   return rc != PK_OK ? rc : launch_gate_tail(tail, (hipStream_t)stream);
 }
 

@@ -52,7 +52,7 @@ def test_backward_refuses(p):
     assert lib.pk_route_topk_balanced_bwd(p, None, 1, p, *args[:3], 0, *args[4:]) == 0
     for first in ((None, None, 1, p), (p, None, 1, None), (p, None, 2, p), (p, None, 0, p)):
         refused(lib.pk_route_topk_balanced_bwd(*first, *args), "argument")
-    region = [p, p, p, None, 0, p, 1, 1.0, p, 1, p, p, p, None, None, 0, p, None, None, None, None, None, None, 4, 64, 8, 2, None, 0, None]
+    region = [p, p, p, None, 0, p, 1, 1.0, p, 1, p, p, p, None, None, 0, p, 4, 64, 8, 2, None, 0, None]
     refused(lib.pk_region_router_balanced_bwd(p, None, 2, p, *region), "argument")
     refused(lib.pk_region_router_balanced_bwd(p, None, 1, None, *region), "argument")
     refused(lib.pk_region_router_balanced_bwd(p, None, 1, p, *region), "workspace")
