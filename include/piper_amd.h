@@ -645,9 +645,11 @@ PK_API int pk_adamw8_fused_packed(float* master, uint8_t* exp_avg, uint8_t* exp_
  * Newton-Schulz products: X = U / max(|U|, eps) (Frobenius norm), `steps` times (0 to 100)
  *   A = X X^T,  X <- a X + (b A + c A A) X
  * on the transposed matrix where it has more rows than columns.  Sides of at most PK_MAX_MATRIX_SIDE.
- * `precise`: results as exact as products in fp32 (three products of fp16 halves); otherwise single fp16
- * products, 2e-3 or less off, for results in bf16.  Sums are fp32 either way.  A matrix with a value that is
- * not finite becomes NaN, and no other one does; a matrix of zeros stays.  No counterpart in the reference.
+ * `precise`: results as exact as products in fp32 (three products of fp16 halves); otherwise, where both sides
+ * are longer than 128, single fp16 products, about 2e-3 off for matrices with many directions of like strength,
+ * 1e-2 for those of few values (few rows that are not zero, a scaled identity), below 4e-2 for any one direction.
+ * Sums are fp32 either way.  A matrix with a value that is not finite becomes NaN, and no other one does; a matrix
+ * of zeros stays.  No counterpart in the reference.
  *
  * Bytes of workspace (HOST arrays; n stacks of counts[i] matrices) that a call runs best with: it goes through
  * its matrices in groups of what the workspace holds, which has to be the largest matrix at least
@@ -655,10 +657,14 @@ PK_API int pk_adamw8_fused_packed(float* master, uint8_t* exp_avg, uint8_t* exp_
 #define PK_MAX_MATRIX_SIDE 32768
 PK_API int64_t pk_orthogonalize_workspace_bytes(const int64_t* counts, const int64_t* rows, const int64_t* cols,
                                          int64_t n, int precise);
-/* out [count, rows, cols] = the result for each matrix of x, in x's dtype (f32: precise). */
+/* out [count, rows, cols] = the result for each matrix of x, in x's dtype: precise, rounded once. */
 PK_API int pk_orthogonalize(const void* x, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps,
                      float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes,
                      pk_stream_t stream);
+/* The same with single products. */
+PK_API int pk_orthogonalize_half(const void* x, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps,
+                          float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes,
+                          pk_stream_t stream);
 /* One optimizer step of n stacks of matrices (HOST arrays of device pointers and sizes):
  *   g = flat_grads[i] + grads[i] (each may be NULL, the arrays too)    m <- m + (1 - momentum)(g - m)
  *   U = g + momentum (m - g) with nesterov, m without

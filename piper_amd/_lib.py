@@ -131,6 +131,7 @@ SIGNATURES = {
     "pk_orthogonalize_workspace_bytes": (_c_i64, [_p, _p, _p, _c_i64, _c_int]),
     # x dtype out count rows cols steps a b c eps ws ws_bytes stream
     "pk_orthogonalize": (_c_int, [_p, _c_int, _p, *[_c_i64] * 3, _c_int, *[_c_f32] * 4, _p, _c_i64, _p]),
+    "pk_orthogonalize_half": (_c_int, [_p, _c_int, _p, *[_c_i64] * 3, _c_int, *[_c_f32] * 4, _p, _c_i64, _p]),
     # masters momenta grads flat_grads shadows counts rows cols n dtype lr mu decay nesterov adjust zero precise steps a b c eps ws ws_bytes stream
     "pk_muon_fused": (_c_int, [*[_p] * 8, _c_i64, _c_int, *[C.c_double] * 3, *[_c_int] * 5, *[_c_f32] * 4, _p, _c_i64, _p]),
     "pk_timing_enable": (_c_int, [_c_int]),

@@ -1488,7 +1488,7 @@ std::array<int64_t, 3> matrices_of(const Tensor& t, const char* what) {
   const int64_t r = t.size(-2), c = t.size(-1);
   return {r * c > 0 ? t.numel() / (r * c) : 0, r, c};
 }
-Tensor orthogonalize(const Tensor& x_, int64_t steps, std::array<double, 3> k, double eps) {
+Tensor orthogonalize(const Tensor& x_, int64_t steps, std::array<double, 3> k, double eps, bool half) {
   require_gpu(x_);
   refuse_transforms({&x_}, "orthogonalize");
   const auto m = matrices_of(x_, "orthogonalize");
@@ -1498,11 +1498,14 @@ Tensor orthogonalize(const Tensor& x_, int64_t steps, std::array<double, 3> k, d
   c10::hip::HIPGuard device(x_.device().index());
   const Tensor x = contig(x_);
   Tensor out = at::empty(x.sizes(), x.options());
-  const int64_t bytes = pk_orthogonalize_workspace_bytes(&m[0], &m[1], &m[2], 1, code == PK_F32);
+  const int64_t bytes = pk_orthogonalize_workspace_bytes(&m[0], &m[1], &m[2], 1, !half);
   TORCH_CHECK_VALUE(bytes >= 0, "orthogonalize: matrices of at most ", PK_MAX_MATRIX_SIDE, " rows and columns");
   const Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
-  PK_CALL(pk_orthogonalize, ptr(x), code, ptr(out), m[0], m[1], m[2], (int)steps, (float)k[0], (float)k[1], (float)k[2], (float)eps, ptr(ws), bytes,
-          stream_of(x));
+  const auto call = [&](auto* entry, const char* name) {
+    ok(entry(ptr(x), code, ptr(out), m[0], m[1], m[2], (int)steps, (float)k[0], (float)k[1], (float)k[2], (float)eps, ptr(ws), bytes, stream_of(x)), name);
+  };
+  if (half) call(pk_orthogonalize_half, "pk_orthogonalize_half");
+  else call(pk_orthogonalize, "pk_orthogonalize");
   return out;
 }
 

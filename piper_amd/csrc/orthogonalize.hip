@@ -8,14 +8,15 @@
 //
 // Numbers.  X lives between the products as two planes of fp16 (hi + lo: 22 bits), scaled by a power of two so that its typical
 // value is near 1, A times 2^8, B as it is: their values are at most a few units and their absolute error is what counts beside
-// a X.  All sums are fp32.  Results in bf16 come from single products, of the upper planes alone, with a X from both: an error of a
-// product is bounded by the strong directions and turns them a little, while an error of X itself, a full matrix of noise, grows with
-// the weak ones, up to 3.4 times a step.  (256 x 683, relative to 64 bits: gradients with 8 strong directions 4e-4 as
-// here, 0.04 with X in one plane, 0.3 with everything in bf16; random ones 1.7e-3, the rounding to bf16 by itself 1.7e-3.)  Results
-// in fp32 (and the fp32 weights of the step) take three products, hi hi + lo hi + hi lo, of all operands: 1e-6 to 2e-6,
-// what products in fp32 give or less, at three times the matrix operations of the other and a third of the time of fp32 instructions.
-// So do bf16 ones of matrices with a side of at most 128: errors of a few directions do not average out (7e-3 of 3 x 1100), and
-// these matrices cost next to nothing.
+// a X.  All sums are fp32.  Results take three products, hi hi + lo hi + hi lo, of all operands: 1e-6 to 2e-6 off, what products in fp32
+// give or less, in a third of the time of fp32 instructions; a bf16 result is then the rounding of one in fp32 (1.7e-3 off 64 bits).
+//
+// Where the caller asks for it, single products, of the upper planes alone, with a X from both: a third of the matrix operations.  An
+// error of a product is bounded by the strong directions and turns them a little, while an error of X itself, a full matrix of noise, grows
+// with the weak ones, up to 3.4 times a step.  (256 x 683, relative to 64 bits: gradients with 8 strong directions 4e-4 as here, 0.04
+// with X in one plane, 0.3 with everything in bf16; random ones 1.7e-3.)  Errors of a few directions do not average out: matrices with
+// few rows that are not zero 2e-3 to 7e-3, scaled identities up to 0.012, any one direction below 0.04.  Those with a side of
+// at most 128 take three products in any case, as they cost next to nothing.
 //
 // Work is laid out for many matrices: a launch runs one product of all matrices of a group, as many as the workspace holds.  Padded
 // to multiples of 128 with zeros there (zeros stay zeros under the products), so that only the first and the last kernel see
@@ -1015,8 +1016,8 @@ int64_t pk_orthogonalize_workspace_bytes(const int64_t* counts, const int64_t* r
   return std::max(most, std::min(all, kGroupBytes));
 }
 
-int pk_orthogonalize(const void* x, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps, float a, float b, float c,
-                     float eps, void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
+static int orthogonalize(bool precise, const void* x, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps, float a,
+                         float b, float c, float eps, void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
   if (count < 0 || rows < 0 || cols < 0 || !pk_dtype_ok(dtype) || !settings_ok(steps, eps)) return PK_ERR_ARG;
   if (!sides_ok(rows, cols)) return PK_ERR_SHAPE;
   if (count == 0 || rows == 0 || cols == 0) return PK_OK;
@@ -1024,8 +1025,16 @@ int pk_orthogonalize(const void* x, int dtype, void* out, int64_t count, int64_t
   Settings o = {};
   o.bf16_src = dtype == PK_BF16;
   o.eps = eps; o.steps = steps; o.a = a; o.b = b; o.c = c;
-  const Item only{x, nullptr, nullptr, nullptr, out, count, rows, cols, 0.f, precise_result(dtype == PK_F32, rows, cols)};
+  const Item only{x, nullptr, nullptr, nullptr, out, count, rows, cols, 0.f, precise_result(precise, rows, cols)};
   return run(1, [&](int64_t) { return only; }, o, workspace, workspace_bytes, (hipStream_t)stream);
+}
+int pk_orthogonalize(const void* x, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps, float a, float b, float c,
+                     float eps, void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
+  return orthogonalize(true, x, dtype, out, count, rows, cols, steps, a, b, c, eps, workspace, workspace_bytes, stream);
+}
+int pk_orthogonalize_half(const void* x, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps, float a, float b, float c,
+                          float eps, void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
+  return orthogonalize(false, x, dtype, out, count, rows, cols, steps, a, b, c, eps, workspace, workspace_bytes, stream);
 }
 
 int pk_muon_fused(float* const* masters, float* const* momenta, const void* const* grads, float* const* flat_grads, void* const* shadows,

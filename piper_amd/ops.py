@@ -536,13 +536,15 @@ def adamw8_fused_packed(master, exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_s
 NEWTON_SCHULZ = (3.4445, -4.775, 2.0315)      # a x + b x^3 + c x^5 takes singular values from about 0.01 to 1 to between 0.7 and 1.2 in five steps
 
 
-def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[float] = NEWTON_SCHULZ, eps: float = 1e-7) -> torch.Tensor:
+def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[float] = NEWTON_SCHULZ, eps: float = 1e-7,
+                  half_products: bool = False) -> torch.Tensor:
     """Every matrix of x [.., rows, cols] (bfloat16 or float32) brought near the closest semi-orthogonal one by Newton-Schulz products:
     X = x / max(|x|, eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (on the transposed matrix where it is taller
-    than wide).  float32 results are as exact as products in float32; bfloat16 ones take products of 11-bit values, which
-    leaves them 0.002 or less off beside their rounding.  A matrix with a value that is not finite becomes NaN, no other one does.
-    No backward."""
-    return host().orthogonalize(x, int(steps), _three(coefficients), float(eps))
+    than wide).  Results are as exact as products in float32, bfloat16 ones rounded once.  half_products: products of 11-bit values (of
+    matrices whose sides are both longer than 128), a third of the matrix operations, for results about 0.002 off; 0.01 for
+    matrices of few values (few rows that are not zero, a scaled identity), below 0.04 for any one direction.  A matrix with a value that
+    is not finite becomes NaN, no other one does.  No backward."""
+    return host().orthogonalize(x, int(steps), _three(coefficients), float(eps), bool(half_products))
 
 
 def muon_fused(masters: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | None], *,
@@ -554,7 +556,7 @@ def muon_fused(masters: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor],
     g = flat_grads[i] + grads[i] (either may be None), m <- m + (1 - momentum)(g - m), u = g + momentum (m - g) (m without
     `nesterov`), w <- w (1 - lr weight_decay) - lr s orthogonalize(u), with s = sqrt(max(1, rows / cols)) or, for
     adjust_lr="match_rms_adamw", 0.2 sqrt(max(rows, cols)).  shadows[i]: the bfloat16 copy of w to write.  zero_grad clears flat_grads.
-    half_products: the products of bfloat16 results (``orthogonalize``), a third of the matrix operations, for updates 0.002 off."""
+    half_products: as of ``orthogonalize``."""
     none = [None] * len(masters)
     host().muon(list(masters), list(momenta), list(grads), none if flat_grads is None else list(flat_grads), none if shadows is None else list(shadows),
                 float(lr), float(momentum), float(weight_decay), bool(nesterov), str(adjust_lr), bool(zero_grad), not half_products, int(steps),
