@@ -655,6 +655,11 @@ PK_API int pk_adamw8_fused_packed(float* master, uint8_t* exp_avg, uint8_t* exp_
  * its matrices in groups of what the workspace holds, which has to be the largest matrix at least
  * (PK_ERR_WORKSPACE), and this holds all of them up to 2.5 GiB. */
 #define PK_MAX_MATRIX_SIDE 32768
+/* X is held in a range of singular values up to PK_NEWTON_SCHULZ_RANGE: where `steps` of the polynomial a x + b x^3 + c x^5
+ * may take one in [0, 1] past it (this returns the largest they may reach, with room for roundings; infinity for coefficients that
+ * are not finite), the calls below return PK_ERR_ARG.  Coefficients that bring singular values near 1 stay below 2. */
+#define PK_NEWTON_SCHULZ_RANGE 15.0
+PK_API double pk_newton_schulz_range(int steps, float a, float b, float c);
 PK_API int64_t pk_orthogonalize_workspace_bytes(const int64_t* counts, const int64_t* rows, const int64_t* cols,
                                          int64_t n, int precise);
 /* out [count, rows, cols] = the result for each matrix of x, in x's dtype: precise, rounded once. */

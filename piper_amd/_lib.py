@@ -128,6 +128,7 @@ SIGNATURES = {
     # logits idx sequences T E K S balance z loss counts table ws ws_bytes stream
     "pk_balance_loss": (_c_int, [_p, _p, _p, *[_c_i64] * 4, _c_f32, _c_f32, _p, _p, _p, _p, _c_i64, _p]),
     "pk_balance_loss_bwd": (_c_int, [*[_p] * 5, *[_c_i64] * 3, _p]),
+    "pk_newton_schulz_range": (C.c_double, [_c_int, *[_c_f32] * 3]),
     "pk_orthogonalize_workspace_bytes": (_c_i64, [_p, _p, _p, _c_i64, _c_int]),
     # x dtype out count rows cols steps a b c eps ws ws_bytes stream
     "pk_orthogonalize": (_c_int, [_p, _c_int, _p, *[_c_i64] * 3, _c_int, *[_c_f32] * 4, _p, _c_i64, _p]),

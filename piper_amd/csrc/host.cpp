@@ -1488,12 +1488,18 @@ std::array<int64_t, 3> matrices_of(const Tensor& t, const char* what) {
   const int64_t r = t.size(-2), c = t.size(-1);
   return {r * c > 0 ? t.numel() / (r * c) : 0, r, c};
 }
+void newton_schulz_in_range(int64_t steps, const std::array<double, 3>& k) {
+  const double most = pk_newton_schulz_range((int)steps, (float)k[0], (float)k[1], (float)k[2]);
+  TORCH_CHECK_VALUE(most <= PK_NEWTON_SCHULZ_RANGE, "Newton-Schulz products: ", steps, " steps with coefficients ", k[0], ", ", k[1], ", ", k[2],
+                    " may take singular values to ", most, ", past ", PK_NEWTON_SCHULZ_RANGE, ", what the matrices are held in");
+}
 Tensor orthogonalize(const Tensor& x_, int64_t steps, std::array<double, 3> k, double eps, bool half) {
   require_gpu(x_);
   refuse_transforms({&x_}, "orthogonalize");
   const auto m = matrices_of(x_, "orthogonalize");
   const int code = dtype_code(x_);
   TORCH_CHECK_VALUE(steps >= 0 && steps <= 100 && eps > 0, "orthogonalize: 0 to 100 steps and a positive eps");
+  newton_schulz_in_range(steps, k);
   at::NoGradGuard no_grad;
   c10::hip::HIPGuard device(x_.device().index());
   const Tensor x = contig(x_);
@@ -1516,6 +1522,7 @@ void muon(const std::vector<Tensor>& masters, const std::vector<Tensor>& momenta
   TORCH_CHECK_VALUE(momenta.size() == n && grads.size() == n && flats.size() == n && shadows.size() == n, "muon_fused: one momentum, gradient and copy per tensor");
   TORCH_CHECK_VALUE(adjust == "original" || adjust == "match_rms_adamw", "muon_fused: adjust_lr is 'original' or 'match_rms_adamw', not '", adjust, "'");
   TORCH_CHECK_VALUE(steps >= 0 && steps <= 100 && eps > 0, "muon_fused: 0 to 100 steps and a positive eps");
+  newton_schulz_in_range(steps, k);
   TORCH_CHECK_VALUE(lr >= 0 && momentum >= 0 && momentum < 1 && weight_decay >= 0, "muon_fused: invalid hyper-parameters");
   if (n == 0) return;
   require_gpu(masters[0]);

@@ -26,6 +26,7 @@
 #include "launch_rules.h"
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 namespace {
 
@@ -79,8 +80,8 @@ struct Gemm {
 static_assert(sizeof(Gemm) <= 4096, "kernel arguments");
 
 // X is held times 2^12 and A times 2^8: elements of large normalised matrices are small, as A's off the diagonal are, and
-// the lower plane of a small one would be below fp16's range.  (Singular values up to 16 stay in it; those of the usual coefficients
-// stay below 1.3.)
+// the lower plane of a small one would be below fp16's range.  Singular values up to 15 stay in it (2^12 * 15 and 2^8 * 15^2 are below
+// 65504), and calls whose coefficients may lead past that are refused (settings_ok); those of the usual ones stay below 1.3.
 constexpr int kXLog2 = 12, kALog2 = 8;
 constexpr float kX = 1 << kXLog2, kA = 1 << kALog2;
 
@@ -996,11 +997,44 @@ int run(int64_t n, F&& item, const Settings& o, void* workspace, int64_t workspa
   return PK_OK;
 }
 
-bool settings_ok(int steps, float eps) { return steps >= 0 && steps <= 100 && eps > 0.f; }
+bool settings_ok(int steps, float a, float b, float c, float eps) {
+  return steps >= 0 && steps <= 100 && eps > 0.f && pk_newton_schulz_range(steps, a, b, c) <= PK_NEWTON_SCHULZ_RANGE;
+}
 
 }  // namespace
 
 extern "C" {
+
+// A step takes singular values x in [0, m] onto p(x) = a x + b x^3 + c x^5, an interval around 0, whose ends are p at m or where p' = a + 3 b
+// x^2 + 5 c x^4 is 0.  2^-6 at the start and at every step is room for the roundings (single products: below 2^-8 of a value, the
+// head of this file), which coefficients that hold 1 in place without holding its neighbours would carry on.  B = p(x) / x is fp16 too: it
+// counts with a factor of 15 / 60000.
+double pk_newton_schulz_range(int steps, float a, float b, float c) {
+  const double room = 1.0 + 1.0 / 64, none = std::numeric_limits<double>::infinity();
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return none;
+  double m = room, most = m;
+  for (int i = 0; i < steps; ++i) {
+    const auto poly = [&](double t) { return a + t * (b + t * (double)c); };      // of t = x^2
+    const double end = m * m;
+    double at[5] = {0.0, end, end, end, end};
+    const double disc = 9.0 * b * b - 20.0 * a * (double)c;
+    if (c != 0 && disc >= 0)
+      for (int k = 0; k < 2; ++k) at[2 + k] = (-3.0 * b + (k ? 1 : -1) * std::sqrt(disc)) / (10.0 * c);
+    else if (c == 0 && b != 0)
+      at[2] = -(double)a / (3.0 * b);
+    if (c != 0) at[4] = -(double)b / (2.0 * c);                                   // where B turns
+    double next = 0.0;
+    for (const double t : at) {
+      if (!(t >= 0.0 && t <= end)) continue;
+      next = std::max(next, std::abs(std::sqrt(t) * poly(t)));
+      most = std::max(most, std::abs(poly(t)) * (PK_NEWTON_SCHULZ_RANGE / 60000.0));
+    }
+    m = next * room;
+    most = std::max(most, m);
+    if (!(most <= PK_NEWTON_SCHULZ_RANGE)) return std::isfinite(most) ? most : none;
+  }
+  return most;
+}
 
 int64_t pk_orthogonalize_workspace_bytes(const int64_t* counts, const int64_t* rows, const int64_t* cols, int64_t n, int precise) {
   if (n < 0 || (n > 0 && (!counts || !rows || !cols))) return PK_ERR_ARG;
@@ -1018,7 +1052,7 @@ int64_t pk_orthogonalize_workspace_bytes(const int64_t* counts, const int64_t* r
 
 static int orthogonalize(bool precise, const void* x, int dtype, void* out, int64_t count, int64_t rows, int64_t cols, int steps, float a,
                          float b, float c, float eps, void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
-  if (count < 0 || rows < 0 || cols < 0 || !pk_dtype_ok(dtype) || !settings_ok(steps, eps)) return PK_ERR_ARG;
+  if (count < 0 || rows < 0 || cols < 0 || !pk_dtype_ok(dtype) || !settings_ok(steps, a, b, c, eps)) return PK_ERR_ARG;
   if (!sides_ok(rows, cols)) return PK_ERR_SHAPE;
   if (count == 0 || rows == 0 || cols == 0) return PK_OK;
   if (!x || !out) return PK_ERR_ARG;
@@ -1041,7 +1075,7 @@ int pk_muon_fused(float* const* masters, float* const* momenta, const void* cons
                   const int64_t* counts, const int64_t* rows, const int64_t* cols, int64_t n, int grad_dtype, double lr, double momentum,
                   double weight_decay, int nesterov, int adjust, int zero_flat, int precise, int steps, float a, float b, float c, float eps,
                   void* workspace, int64_t workspace_bytes, pk_stream_t stream) {
-  if (n < 0 || !pk_dtype_ok(grad_dtype) || !settings_ok(steps, eps) || (adjust != PK_MUON_ASPECT && adjust != PK_MUON_RMS)) return PK_ERR_ARG;
+  if (n < 0 || !pk_dtype_ok(grad_dtype) || !settings_ok(steps, a, b, c, eps) || (adjust != PK_MUON_ASPECT && adjust != PK_MUON_RMS)) return PK_ERR_ARG;
   if (n == 0) return PK_OK;
   if (!masters || !momenta || !counts || !rows || !cols) return PK_ERR_ARG;
   for (int64_t i = 0; i < n; ++i) {

@@ -543,7 +543,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     than wide).  Results are as exact as products in float32, bfloat16 ones rounded once.  half_products: products of 11-bit values (of
     matrices whose sides are both longer than 128), a third of the matrix operations, for results about 0.002 off; 0.01 for
     matrices of few values (few rows that are not zero, a scaled identity), below 0.04 for any one direction.  A matrix with a value that
-    is not finite becomes NaN, no other one does.  No backward."""
+    is not finite becomes NaN, no other one does.  Coefficients and steps that may take a singular value past 15 are refused; those that
+    bring them near 1 stay below 2.  No backward."""
     return host().orthogonalize(x, int(steps), _three(coefficients), float(eps), bool(half_products))
 
 
@@ -561,6 +562,11 @@ def muon_fused(masters: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor],
     host().muon(list(masters), list(momenta), list(grads), none if flat_grads is None else list(flat_grads), none if shadows is None else list(shadows),
                 float(lr), float(momentum), float(weight_decay), bool(nesterov), str(adjust_lr), bool(zero_grad), not half_products, int(steps),
                 _three(coefficients), float(eps))
+
+
+def newton_schulz_in_range(steps: int, coefficients: Sequence[float]) -> bool:
+    """Whether ``orthogonalize`` and ``muon_fused`` take these."""
+    return _lib.load().pk_newton_schulz_range(int(steps), *_three(coefficients)) <= 15.0
 
 
 def _three(coefficients: Sequence[float]) -> list[float]:

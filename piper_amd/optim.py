@@ -201,6 +201,8 @@ class FusedMuon(_FlatStateOptimizer):
         if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0 or eps <= 0 or not 0 <= ns_steps <= 100 or len(tuple(ns_coefficients)) != 3 or \
                 adjust_lr not in ("original", "match_rms_adamw"):
             raise ValueError("invalid Muon hyper-parameters")
+        if not ops.newton_schulz_in_range(ns_steps, ns_coefficients):
+            raise ValueError("FusedMuon: coefficients that may take singular values past 15 (ops.orthogonalize)")
         if adamw and adamw.get("lr", lr) != lr and lr == 0:
             raise ValueError("FusedMuon: adamw's lr follows lr in proportion, which has to be positive for that")
         if other["lr"] < 0 or other["eps"] < 0 or not 0 <= b1 < 1 or not 0 <= b2 < 1 or other["weight_decay"] < 0:

@@ -114,3 +114,15 @@ def test_half_products_captured():
         torch.cuda.synchronize()
         assert torch.equal(out, w)
         ops.orthogonalize(x.float())
+
+
+def test_singular_values_up_to_the_range_are_right_and_past_it_refused():
+    one = torch.ones(1, 1, device=DEV)
+    assert ops.orthogonalize(one, steps=1, coefficients=(14.0, 0.0, 0.0)).item() == 14.0
+    for coefficients in ((14.0, 0.0, 0.0), (-9.0, -3.0, -2.0)):
+        x = torch.cat([few_rows(200, 330, 1, s, torch.float32)[None] for s in range(2)] + [matrices((2, 200, 330), 7)]).to(DEV)
+        exact = O.orthogonalize(x.double(), 1, coefficients)
+        for half, tol in ((False, 2 * off_each(O.orthogonalize(x, 1, coefficients), exact) + 2.0 ** -22), (True, BF16_TOL)):
+            assert (off_each(ops.orthogonalize(x, steps=1, coefficients=coefficients, half_products=half), exact) <= tol).all()
+    with pytest.raises(ValueError, match="singular values to 20"):
+        ops.orthogonalize(one, steps=1, coefficients=(20.0, 0.0, 0.0))
