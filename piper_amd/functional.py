@@ -229,7 +229,7 @@ class _WithLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, out, loss):
         ctx.like = (loss.shape, loss.dtype, loss.device)
-        return out.view_as(out)
+        return out.detach()      # no view of a custom function's: callers may add to it in place
 
     @staticmethod
     def backward(ctx, d_out):

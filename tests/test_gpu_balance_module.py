@@ -1,0 +1,54 @@
+"""The modules with a balance loss on the GPU: what a program does with their outputs, in training and without gradients.
+
+Gradients of the gate: two sums of the same fp32 terms in different orders, 1e-5 of the largest (as tests/test_gpu_balance.py)."""
+import pytest
+import torch
+
+from piper_amd import functional as F_, ops
+from piper_amd.moe import AnnotatedMoE, MoEArgs, MoEFeedForwardBlock
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+ARGS = dict(num_experts=8, top_k=2, route_norm=True)
+LOSS = dict(balance_loss_coeff=0.5, router_z_loss_coeff=0.1)
+
+
+def rel(a, b):
+    a, b = a.detach().double(), b.detach().double()
+    return ((a - b).abs().max() / b.abs().max().clamp_min(1e-30)).item()
+
+
+def pair(cls, dtype=None, seed=0, dims=(64, 32), **args):
+    """The module without and with a balance loss, of the same weights."""
+    args = ARGS | args
+    plain, with_it = (cls(MoEArgs(**args, **more), *dims, dtype=dtype).to(DEV) for more in ({}, LOSS))
+    moe = plain.moe if cls is MoEFeedForwardBlock else plain
+    moe.init_weights(std=0.1, generator=torch.Generator(device=DEV).manual_seed(seed))
+    with_it.load_state_dict(plain.state_dict())
+    return plain, with_it
+
+
+def tokens(*shape, seed=1, dtype=torch.float32):
+    return torch.randn(*shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed)).to(dtype)
+
+
+def loss_gradient(moe, x2, sequences=None):
+    """The loss's gradient of the gate, formed apart."""
+    logits = ops.gate_logits(x2.detach(), moe.router.gate.weight.detach()).requires_grad_(True)
+    idx = ops.route_topk(logits.detach(), moe.router.top_k, True)[1]
+    loss, _ = F_.balance_loss(logits, idx, balance_coeff=LOSS["balance_loss_coeff"], z_coeff=LOSS["router_z_loss_coeff"], sequences=sequences)
+    d, = torch.autograd.grad(loss, logits)
+    return d.double().t() @ x2.detach().double()
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_output_changed_in_place(fused):
+    plain, with_it = pair(AnnotatedMoE)
+    plain.fused = with_it.fused = fused
+    x = tokens(2, 30, 64)
+    for moe in (plain, with_it):
+        out = moe(x)
+        out += x
+        out.mul_(2).sum().backward()
+    want = plain.router.gate.weight.grad.double() + loss_gradient(with_it, x.reshape(-1, 64))
+    assert rel(with_it.router.gate.weight.grad, want) <= 1e-5
