@@ -227,20 +227,21 @@ def balance_loss(logits, top_idx, *, balance_coeff: float = 1.0, z_coeff: float 
 
 class _WithLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, out, loss):
-        ctx.like = (loss.shape, loss.dtype, loss.device)
+    def forward(ctx, out, loss, scale):
+        ctx.like, ctx.scale = (loss.shape, loss.dtype, loss.device), scale
         return out.detach()      # no view of a custom function's: callers may add to it in place
 
     @staticmethod
     def backward(ctx, d_out):
         shape, dtype, device = ctx.like
-        return d_out, torch.ones(shape, dtype=dtype, device=device)
+        return d_out, torch.ones(shape, dtype=dtype, device=device) * ctx.scale, None
 
 
-def with_loss(out, loss):
+def with_loss(out, loss, scale=1.0):
     """`out`, with `loss` trained beside it: whoever differentiates `out` (a later stage that never sees the loss) adds
-    the gradient of `loss`, times one, on the way."""
-    return _WithLoss.apply(out, loss)
+    the gradient of `loss`, times `scale`, on the way.  A program that scales its own loss (for narrow gradients, or by the number of
+    microbatches) gives the same factor here: a number, or a tensor of one element, which is read when the backward runs."""
+    return _WithLoss.apply(out, loss, scale.detach() if isinstance(scale, torch.Tensor) else float(scale))
 
 
 # --------------------------------------------------------------------------- experts in 8-bit blocks

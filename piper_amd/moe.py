@@ -96,6 +96,8 @@ class AnnotatedMoE(nn.Module):
     gather, EP-annotated experts, scatter+combine) through the piecewise HIP operators."""
 
     balance_loss_coeff = router_z_loss_coeff = 0.0
+    # factor of the balance loss's gradient (functional.with_loss): a program that scales its loss sets the same one here
+    balance_loss_scale: float | torch.Tensor = 1.0
     # of the last forward with a balance loss: its value, and the tokens of each expert (with ``sequences`` of each of them)
     balance_loss: torch.Tensor | None = None
     tokens_per_expert: torch.Tensor | None = None
@@ -126,7 +128,7 @@ class AnnotatedMoE(nn.Module):
     def _trained_beside(self, out: torch.Tensor, loss: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
         """`out`, whose backward also trains the router on `loss`: a stage hands on its output, nobody sees the loss."""
         self.balance_loss, self.tokens_per_expert = loss.detach(), counts
-        return F_.with_loss(out, loss) if loss.requires_grad else out
+        return F_.with_loss(out, loss, self.balance_loss_scale) if loss.requires_grad else out
 
     def init_weights(self, std: float = 0.02, generator: torch.Generator | None = None) -> None:
         for p in (self.router.gate.weight, self.experts.w1, self.experts.w3, self.experts.w2):

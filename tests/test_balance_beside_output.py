@@ -1,4 +1,4 @@
-"""A loss that is trained beside an output (functional.with_loss), on the CPU: what callers may do with the output."""
+"""A loss that is trained beside an output (functional.with_loss), on the CPU: what callers may do with the output, and its scale."""
 import pytest
 import torch
 
@@ -28,10 +28,20 @@ def test_a_change_in_place_that_the_backward_needs_is_refused():
         out.sum().backward()
 
 
+@pytest.mark.parametrize("scale", [3, 0.5, torch.tensor(4.0), torch.tensor([4.0])])
+def test_scale(scale):
+    x = leaf()
+    out = F_.with_loss(x * 5, (x * x).sum(), scale)
+    if isinstance(scale, torch.Tensor):
+        scale.fill_(7)                     # between the forward and the backward
+    (1024 * out).sum().backward()
+    assert torch.equal(x.grad, 1024 * 5 + 2 * float(scale) * x.detach())
+
+
 def test_compiled():
     @torch.compile(fullgraph=True, backend="eager")
     def step(x):
-        return F_.with_loss(x * 5, (x * x).sum()).add_(1)
+        return F_.with_loss(x * 5, (x * x).sum(), 2.0).add_(1)
     x = leaf()
     step(x).sum().backward()
-    assert torch.equal(x.grad, 5 + 2 * x.detach())
+    assert torch.equal(x.grad, 5 + 4 * x.detach())

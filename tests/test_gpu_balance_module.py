@@ -52,3 +52,18 @@ def test_output_changed_in_place(fused):
         out.mul_(2).sum().backward()
     want = plain.router.gate.weight.grad.double() + loss_gradient(with_it, x.reshape(-1, 64))
     assert rel(with_it.router.gate.weight.grad, want) <= 1e-5
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("scale", [1024.0, torch.tensor(1024.0)])
+def test_a_scaled_loss(fused, scale):
+    """The factor of the program's loss, taken off the gradients afterwards: the gradients without it."""
+    _, moe = pair(AnnotatedMoE)
+    moe.fused = fused
+    x, d = tokens(2, 30, 64), tokens(2, 30, 64, seed=2)
+    moe(x).backward(d)
+    want = moe.router.gate.weight.grad.clone()
+    moe.zero_grad()
+    moe.balance_loss_scale = scale.to(DEV) if isinstance(scale, torch.Tensor) else scale
+    moe(x).backward(d * 1024)
+    assert torch.equal(moe.router.gate.weight.grad / 1024, want)      # (a power of two)
