@@ -207,7 +207,7 @@ class MoEFeedForwardBlock(nn.Module):
         if torch.compiler.is_compiling():
             return False
         norm, moe = self._modules["ffn_norm"], self._modules["moe"]
-        return (moe.fused and not moe.balanced and _called_as_defined(norm, RMSNorm) and _called_as_defined(moe, AnnotatedMoE)
+        return (_called_as_defined(norm, RMSNorm) and _called_as_defined(moe, AnnotatedMoE) and moe.fused and not moe.balanced
                 and not (_FORWARD_HOOKS or _FORWARD_PRE_HOOKS or _BACKWARD_HOOKS or _BACKWARD_PRE_HOOKS)
                 and F_.rmsnorm is _OPERATORS[0] and F_.expert_region is _OPERATORS[1])
 
