@@ -98,7 +98,10 @@ class AnnotatedMoE(nn.Module):
     balance_loss_coeff = router_z_loss_coeff = 0.0
     # factor of the balance loss's gradient (functional.with_loss): a program that scales its loss sets the same one here
     balance_loss_scale: float | torch.Tensor = 1.0
-    # of the last forward with a balance loss: its value, and the tokens of each expert (with ``sequences`` of each of them)
+    # whether a forward without gradients forms the loss too (for its value), at the price of the kernels that serve without one
+    balance_loss_without_grad = False
+    # of the last forward with a balance loss: its value, and the tokens of each expert (with ``sequences`` of each of them); None after
+    # one that formed none
     balance_loss: torch.Tensor | None = None
     tokens_per_expert: torch.Tensor | None = None
 
@@ -125,6 +128,10 @@ class AnnotatedMoE(nn.Module):
     def balanced(self) -> bool:
         return self.balance_loss_coeff != 0 or self.router_z_loss_coeff != 0
 
+    def _forms_loss(self) -> bool:
+        """Whether a forward now forms the loss: where nothing can be trained on it the module is the one without it."""
+        return self.balanced and (torch.is_grad_enabled() or self.balance_loss_without_grad)
+
     def _trained_beside(self, out: torch.Tensor, loss: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
         """`out`, whose backward also trains the router on `loss`: a stage hands on its output, nobody sees the loss."""
         self.balance_loss, self.tokens_per_expert = loss.detach(), counts
@@ -144,7 +151,11 @@ class AnnotatedMoE(nn.Module):
         bs, slen, dim = x.shape
         x2 = x.reshape(-1, dim)
         top_k = self.router.top_k
-        loss = dict(balance_coeff=self.balance_loss_coeff, z_coeff=self.router_z_loss_coeff, sequences=sequences) if self.balanced else None
+        loss = None
+        if self._forms_loss():
+            loss = dict(balance_coeff=self.balance_loss_coeff, z_coeff=self.router_z_loss_coeff, sequences=sequences)
+        elif self.balanced:
+            self.balance_loss = self.tokens_per_expert = None
         if self.fused and experts_fp8 is None and loss is not None:
             with annotate(EP_TAG):
                 out = self._trained_beside(*F_.expert_region_balanced(
@@ -207,7 +218,7 @@ class MoEFeedForwardBlock(nn.Module):
         if torch.compiler.is_compiling():
             return False
         norm, moe = self._modules["ffn_norm"], self._modules["moe"]
-        return (_called_as_defined(norm, RMSNorm) and _called_as_defined(moe, AnnotatedMoE) and moe.fused and not moe.balanced
+        return (_called_as_defined(norm, RMSNorm) and _called_as_defined(moe, AnnotatedMoE) and moe.fused and not moe._forms_loss()
                 and not (_FORWARD_HOOKS or _FORWARD_PRE_HOOKS or _BACKWARD_HOOKS or _BACKWARD_PRE_HOOKS)
                 and F_.rmsnorm is _OPERATORS[0] and F_.expert_region is _OPERATORS[1])
 
@@ -216,6 +227,8 @@ class MoEFeedForwardBlock(nn.Module):
             return self.moe(self.ffn_norm(x), residual=x) if sequences is None else self.moe(self.ffn_norm(x), residual=x, sequences=sequences)
         bs, slen, dim = x.shape
         norm, moe = self.ffn_norm, self.moe
+        if moe.balanced:
+            moe.balance_loss = moe.tokens_per_expert = None
         router, experts = moe.router, moe.experts
         with annotate(EP_TAG):
             out = F_.moe_block(x.reshape(-1, dim), norm.weight, router.gate.weight, router.gate.bias, experts.w1, experts.w2,

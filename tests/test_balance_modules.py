@@ -21,3 +21,13 @@ def test_a_block_with_somebody_elses_experts():
     assert torch.equal(block(x), 3 * x)
     del Doubling.fused
     assert torch.equal(block(x), 3 * x)
+
+
+def test_without_gradients_a_block_is_the_one_without_a_loss():
+    plain, with_it = (MoEFeedForwardBlock(MoEArgs(num_experts=4, top_k=2, **more), 16, 8) for more in ({}, dict(balance_loss_coeff=0.1)))
+    assert plain._one_node() and not with_it._one_node()
+    with torch.no_grad():
+        assert plain._one_node() and with_it._one_node()
+        with_it.moe.balance_loss_without_grad = True
+        assert not with_it._one_node()
+    assert isinstance(with_it.moe, AnnotatedMoE) and not AnnotatedMoE.balance_loss_without_grad

@@ -4,7 +4,7 @@ Gradients of the gate: two sums of the same fp32 terms in different orders, 1e-5
 import pytest
 import torch
 
-from piper_amd import functional as F_, ops
+from piper_amd import _lib, functional as F_, ops
 from piper_amd.moe import AnnotatedMoE, MoEArgs, MoEFeedForwardBlock
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +67,39 @@ def test_a_scaled_loss(fused, scale):
     moe.balance_loss_scale = scale.to(DEV) if isinstance(scale, torch.Tensor) else scale
     moe(x).backward(d * 1024)
     assert torch.equal(moe.router.gate.weight.grad / 1024, want)      # (a power of two)
+
+
+@pytest.mark.parametrize("cls", [AnnotatedMoE, MoEFeedForwardBlock])
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("dtype,dims,experts", [(torch.bfloat16, (512, 256), 16), (torch.float32, (64, 32), 8)])
+@pytest.mark.parametrize("T", [1, 3, 200])
+def test_without_gradients_it_is_the_module_without_the_loss(cls, fused, dtype, dims, experts, T):
+    """The same launches and bits, single tokens among them, and no value of a loss that was not formed."""
+    plain, with_it = pair(cls, dtype, dims=dims, num_experts=experts)
+    of = lambda m: m.moe if cls is MoEFeedForwardBlock else m  # noqa: E731
+    of(plain).fused = of(with_it).fused = fused
+    x = tokens(1, T, dims[0], dtype=dtype)
+    off = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    with_it(x, sequences=off)
+    assert of(with_it).balance_loss is not None and of(with_it).tokens_per_expert.shape == (1, experts)
+    launches = []
+    with torch.no_grad():
+        for m, more in ((plain, {}), (with_it, dict(sequences=off))):
+            m(x, **more)
+            torch.cuda.synchronize()
+            _lib.timing_enable(True)
+            try:
+                out = m(x, **more)
+                torch.cuda.synchronize()
+                launches.append([name for name, _ in _lib.timing_collect()])
+            finally:
+                _lib.timing_enable(False)
+            if m is plain:
+                want = out
+    assert torch.equal(out, want) and launches[0] == launches[1] and len(launches[0]) > 0
+    assert of(with_it).balance_loss is None and of(with_it).tokens_per_expert is None
+    of(with_it).balance_loss_without_grad = True
+    with torch.no_grad():
+        again = with_it(x, sequences=off)
+    assert rel(again, want) <= (2e-2 if dtype == torch.bfloat16 else 1e-5)
+    assert of(with_it).balance_loss.shape == () and int(of(with_it).tokens_per_expert.sum()) == T * 2
