@@ -725,6 +725,12 @@ struct RegionFn : public torch::autograd::Function<RegionFn> {
   }
 };
 
+// Whether a forward without a backward writes the pre-activations: only the any-width kernels need them
+bool needs_pre_activations(const Shape& s, const Tensor& x, const Tensor& w1, const Tensor& w2, const Tensor& w3) {
+  const int64_t piece = 16 / s.es;
+  return s.H % piece != 0 || s.I % piece != 0 || !aligned16(x) || !aligned16(w1) || !aligned16(w2) || !aligned16(w3);
+}
+
 // None (with `direct`): not ordinary GPU tensors, or a tracing mode is on
 std::optional<Tensor> expert_region(const Tensor& x, const Tensor& w_gate, const OptTensor& bias_, const Tensor& w1, const Tensor& w2,
                                     const Tensor& w3, int64_t top_k, bool route_norm, double route_scale, const OptTensor& residual_,
@@ -750,9 +756,7 @@ std::optional<Tensor> expert_region(const Tensor& x, const Tensor& w_gate, const
             (float)s.route_scale, ptr(rc), ptr(out), s.T, s.H, s.E, s.I, s.K, ptr(ws), decode_ws, stream_of(x));
     return out;
   }
-  // without a backward the pre-activations need not be written, except by the any-width kernels
-  const int64_t piece = 16 / s.es;
-  const bool keep_gu = s.H % piece != 0 || s.I % piece != 0 || !aligned16(xc) || !aligned16(w1c) || !aligned16(w2c) || !aligned16(w3c);
+  const bool keep_gu = needs_pre_activations(s, xc, w1c, w2c, w3c);
   Saved sv(s, keep_gu, norm_w.defined());
   return region_forward(s, route, sv, keep_gu, false, xc, gc, bc, w1c, w2c, w3c, rc, nc);
 }
@@ -772,9 +776,10 @@ std::optional<variable_list> expert_region_balanced(const Tensor& x, const Tenso
     return RegionFn::apply(x, w_gate, bias_, w1, w2, w3, residual_, OptTensor(), top_k, route_norm, route_scale, 0.0, route, sequences_, true, balance, z);
   const Shape s = region_shape(x, w_gate, bias, w1, w2, w3, top_k, route_norm, route_scale, 0.0, residual, Tensor());
   const Balance b = balance_of(x, sequences_, balance, z);
-  Saved sv(s, true, false);
-  const Tensor out = region_forward(s, route, sv, true, false, contig(x), contig(w_gate), contig(bias), contig(w1), contig(w2), contig(w3),
-                                    contig(residual), Tensor());
+  const Tensor xc = contig(x), w1c = contig(w1), w2c = contig(w2), w3c = contig(w3);
+  const bool keep_gu = needs_pre_activations(s, xc, w1c, w2c, w3c);
+  Saved sv(s, keep_gu, false);
+  const Tensor out = region_forward(s, route, sv, keep_gu, false, xc, contig(w_gate), contig(bias), w1c, w2c, w3c, contig(residual), Tensor());
   Tensor table;
   const auto r = balance_forward(b, sv.mem.f32(sv.logits), sv.mem.i32(sv.idx), s.T, s.E, s.K, x, &table);
   return variable_list{out, r.first, r.second};

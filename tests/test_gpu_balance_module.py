@@ -103,3 +103,26 @@ def test_without_gradients_it_is_the_module_without_the_loss(cls, fused, dtype, 
         again = with_it(x, sequences=off)
     assert rel(again, want) <= (2e-2 if dtype == torch.bfloat16 else 1e-5)
     assert of(with_it).balance_loss.shape == () and int(of(with_it).tokens_per_expert.sum()) == T * 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,I", [(128, 512), (130, 515)])
+def test_region_without_gradients_writes_no_pre_activations(dtype, H, I):
+    """The region with the loss under no_grad: the bits of the one without it, in as little memory (and the loss's own)."""
+    T, E = 2048, 8
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=gen)  # noqa: E731
+    args = (r(T, H).to(dtype), r(E, H) * 0.1, None, *((r(*s) * 0.05).to(dtype) for s in ((E, I, H), (E, H, I), (E, I, H))))
+    peaks, outs = [], []
+    with torch.no_grad():
+        for run in (F_.expert_region, lambda *a, **k: F_.expert_region_balanced(*a, **k)[0]):
+            run(*args, top_k=2, route_norm=True)
+            torch.cuda.synchronize()
+            torch.cuda.empty_cache()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            outs.append(run(*args, top_k=2, route_norm=True))
+            peaks.append(torch.cuda.max_memory_allocated() - before)
+    assert torch.equal(*outs)
+    # one of the two pre-activations alone would be more than the loss's workspace (33 chunks of 8 experts) and roundings of allocations
+    assert peaks[1] <= peaks[0] + 2 * T * I * args[0].element_size() // 2
