@@ -261,9 +261,9 @@ class FusedMuon(_FlatStateOptimizer):
                 if p in self._views:
                     flat = grad.reshape(-1)
                     owned = flat.dtype == torch.float32 and flat.is_contiguous()
-                    self._update(p, group, flat if owned else flat.float().contiguous(), {}, self.zero_grad_in_step and owned)
+                    self._update(p, group, flat if owned else flat.float().contiguous(), [None] * len(self._views[p]), self.zero_grad_in_step and owned)
                 else:
-                    self._update(p, group, None, {0: grad}, False)
+                    self._update(p, group, None, [grad], False)
                     if self.zero_grad_in_step:
                         grad.zero_()
         return loss
@@ -275,22 +275,26 @@ class FusedMuon(_FlatStateOptimizer):
         places = [(o, n) for o, n, *_ in self._places(p)]
         if p not in self._views or [tuple(x) for x in zip(offsets, numels)] != places:
             raise RuntimeError("FusedMuon.step_packed: gradients of the views that bind_views has been told of, in their order")
-        self._update(p, group, flat_grad, dict(zip(offsets, grads)), self.zero_grad_in_step and flat_grad is not None)
+        self._update(p, group, flat_grad, grads, self.zero_grad_in_step and flat_grad is not None)
 
-    def _update(self, p: torch.Tensor, group: dict, flat, own: dict, clear: bool) -> None:
+    def _update(self, p: torch.Tensor, group: dict, flat, grads, clear: bool) -> None:
+        """grads: of each of _places, None: nothing beside `flat`"""
         if not p.is_contiguous():
             raise RuntimeError("FusedMuon needs contiguous parameters (flatten them into a bucket)")
+        self._check_grads(p, flat, grads)
         st = self._init_state(p)
         st["step"] += 1
         shadow = None if p.dtype == torch.float32 else p.detach().reshape(-1)
         cut = lambda t, o, n: None if t is None else t[o:o + n]  # noqa: E731
         todo, second = [], 0
-        for o, n, shape, matrix in self._places(p):
+        for (o, n, shape, matrix), grad in zip(self._places(p), grads):
+            if n == 0:
+                continue
             buffers = [cut(t, o, n) for t in (st["master"], st["momentum"], flat, shadow)]
             if matrix:
-                todo.append([None if t is None else t.view(shape) for t in buffers] + [own.get(o)])
-            elif n:
-                self._adamw(*buffers, own.get(o), st["exp_avg_sq"][second:second + n], st["step"], group, clear)
+                todo.append([None if t is None else t.view(shape) for t in buffers] + [grad])
+            else:
+                self._adamw(*buffers, grad, st["exp_avg_sq"][second:second + n], st["step"], group, clear)
                 second += -(-n // 4) * 4
         if todo:
             masters, momenta, flats, shadows, grads = (list(t) for t in zip(*todo))
@@ -298,6 +302,24 @@ class FusedMuon(_FlatStateOptimizer):
                            weight_decay=group["weight_decay"], nesterov=group["nesterov"], steps=group["ns_steps"],
                            coefficients=group["ns_coefficients"], eps=group["eps"], adjust_lr=group["adjust_lr"], zero_grad=clear,
                            half_products=self.half_products)
+
+    def _check_grads(self, p: torch.Tensor, flat, grads) -> None:
+        """Before anything is changed: a step refused for its gradients leaves weights and state as they were."""
+        places = self._places(p)
+        if len(grads) != len(places):
+            raise ValueError(f"FusedMuon: {len(grads)} gradients of {len(places)} parameters")
+        types = set()
+        for (_, n, _, matrix), grad in zip(places, grads):
+            if grad is None:
+                continue
+            if grad.numel() != n or grad.device != p.device or grad.dtype not in (torch.float32, torch.bfloat16):
+                raise ValueError(f"FusedMuon: a gradient of {grad.numel()} {grad.dtype} elements on {grad.device} for a parameter of {n} on {p.device}")
+            if matrix and n:
+                types.add(grad.dtype)
+        if len(types) > 1:
+            raise ValueError("FusedMuon: the matrices' gradients of one step share a dtype")
+        if flat is not None and (flat.dtype != torch.float32 or flat.numel() != p.numel() or flat.device != p.device or not flat.is_contiguous()):
+            raise ValueError(f"FusedMuon: the flat gradient is a contiguous float32 tensor of {p.numel()} elements on {p.device}")
 
     def _adamw(self, master, exp_avg, flat, shadow, grad, exp_avg_sq, step: int, group: dict, clear: bool) -> None:
         b1, b2 = group["adamw_betas"]
