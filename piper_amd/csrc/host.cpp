@@ -1566,13 +1566,26 @@ void muon(const std::vector<Tensor>& masters, const std::vector<Tensor>& momenta
     flat[i] = static_cast<float*>(ptr(flat_i));
     copy[i] = ptr(copy_i);
   }
-  std::vector<std::pair<const char*, const char*>> written;
-  for (size_t i = 0; i < n; ++i)
-    for (const auto& [at, width] : {std::pair<void*, int64_t>{w[i], 4}, {m[i], 4}, {zero_flat ? flat[i] : nullptr, 4}, {copy[i], 2}})
-      if (at && masters[i].numel() > 0) written.emplace_back(static_cast<const char*>(at), static_cast<const char*>(at) + masters[i].numel() * width);
-  std::sort(written.begin(), written.end());
-  for (size_t i = 1; i < written.size(); ++i)
-    TORCH_CHECK_VALUE(written[i - 1].second <= written[i].first, "muon_fused: two of the buffers that are written overlap (a tensor given twice?)");
+  struct Range { const char *begin, *end; bool written; };
+  std::vector<Range> ranges;
+  for (size_t i = 0; i < n; ++i) {
+    const auto add = [&](const void* at, int64_t width, bool written) {
+      const char* const begin = static_cast<const char*>(at);
+      if (at && masters[i].numel() > 0) ranges.push_back({begin, begin + masters[i].numel() * width, written});
+    };
+    add(w[i], 4, true);
+    add(m[i], 4, true);
+    add(copy[i], 2, true);
+    add(flat[i], 4, zero_flat);
+    add(g[i], dtype == at::kFloat ? 4 : 2, false);
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  const char *any = nullptr, *written = nullptr;        // where what begins earlier ends
+  for (const Range& r : ranges) {
+    TORCH_CHECK_VALUE(r.begin >= (r.written ? any : written), "muon_fused: a buffer that is written overlaps another one (a tensor given twice?)");
+    any = std::max(any, r.end);
+    if (r.written) written = std::max(written, r.end);
+  }
   const int64_t bytes = pk_orthogonalize_workspace_bytes(size[0].data(), size[1].data(), size[2].data(), (int64_t)n, precise);
   TORCH_CHECK_VALUE(bytes >= 0, "muon_fused: matrices of at most ", PK_MAX_MATRIX_SIDE, " rows and columns");
   const Tensor ws = at::empty({bytes}, masters[0].options().dtype(at::kByte));

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from oracle import bucket as OB
+from piper_amd import ops
 from piper_amd.bucket import BucketState, ParamStorage, StageStore, flatten_params
 from piper_amd.optim import FusedMuon
 from test_gpu_muon import HYPER, check_matrix, make, put_grads
@@ -72,3 +73,17 @@ def test_held_and_packed_steps_are_the_same_bits(dev, align):
             storage.step_zero_shard_optimizers()
         got.append((bucket.flat_params, *(bucket.shard_optimizer.state[bucket.shard_param][k] for k in ("master", "momentum", "exp_avg_sq"))))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_a_gradient_in_a_buffer_that_is_written_is_refused(dev):
+    room = torch.zeros(8, 4, 6, device=dev)
+    w, m, g, f = room[:2], room[2:4], room[4:6], room[6:8]
+    half = w[0].view(-1).view(torch.bfloat16)[:24].view(4, 6)
+    for bad in (dict(grads=[m[0], g[1]]), dict(grads=[g[0], w[0]]), dict(grads=[room.view(-1)[36:60].view(4, 6), g[1]]), dict(flat_grads=[w[1], f[1]]),
+                dict(flat_grads=[f[0], f[1]], grads=[g[0], f[0]], zero_grad=True), dict(grads=[half, None])):
+        args = dict(grads=[g[0], g[1]], flat_grads=[f[0], f[1]]) | bad
+        with pytest.raises(ValueError, match="overlap"):
+            ops.muon_fused([w[0], w[1]], [m[0], m[1]], args.pop("grads"), lr=0.1, **args)
+    # read twice, neighbours
+    ops.muon_fused([w[0], w[1]], [m[0], m[1]], [g[0], g[0]], flat_grads=[g[0], f[1]], lr=0.1)
+    ops.muon_fused([w[0], w[1]], [m[0], m[1]], [g[0], g[1]], flat_grads=[f[0], f[1]], lr=0.1, zero_grad=True)
