@@ -12,7 +12,7 @@
 
 namespace pk_balance {
 
-// of a call: every workgroup of the first launch counts the sequences that begin before it, 2^40 reads at this many
+// of a call: the first launch has a workgroup for each and more
 constexpr int64_t kMostSequences = 0xfffff;
 
 // What a backward needs beside the logits.  table: [S][E] of h - mean(h) without the 1 / S', then 1 / S' and 2 z_coeff / N.
@@ -29,10 +29,43 @@ __device__ __forceinline__ int end_of(const int32_t* sequences, int s, int T) {
   return sequences ? min(max(sequences[s + 1], begin_of(sequences, s, T)), T) : T;
 }
 
+// How many of the first n things hold, where whatever follows one that does not hold does not either: WIDTH things are looked at together,
+// evenly spaced in what is left while that is more than `scan`.  count(m, f): how many of f(0) .. f(m - 1) hold, the same for all of those
+// who ask.  (Things in another order: some number from 0 to n.)
+template <int WIDTH, typename C, typename F>
+__device__ __forceinline__ int leading(int n, int scan, C&& count, F&& holds) {
+  int lo = 0, left = n;
+  while (left > scan) {
+    const int stride = (left + WIDTH - 1) / WIDTH;
+    const int c = count(WIDTH, [&](int k) { return (k + 1) * stride <= left && holds(lo + (k + 1) * stride - 1); });
+    lo += c * stride;
+    left = min(stride - 1, left - c * stride);
+  }
+  return lo + count(left, [&](int i) { return holds(lo + i); });
+}
+// For a wave: up to 128 things take two loads of a lane at once, 2^20 three rounds of one and the same.
+template <typename F>
+__device__ __forceinline__ int wave_leading(int n, F&& holds) {
+  const int lane = threadIdx.x & 63;
+  return leading<64>(n, 128, [&](int m, auto&& f) {
+    int c = 0;
+    for (int i = 0; i < m; i += 64) c += __popcll(__ballot(i + lane < m && f(i + lane)));
+    return c;
+  }, holds);
+}
+
 // The sequence that token t is in, searched from s on; S: behind the last one, -1: in front of the first one.
 __device__ __forceinline__ int sequence_of(const Grad& g, int s, int t) {
   if (!g.sequences) return 0;
-  while (s < g.S && g.sequences[s + 1] <= t) ++s;
+  for (int n = 0; s < g.S && g.sequences[s + 1] <= t; ++s)
+    if (++n == 4) {                  // (many without tokens)
+      int end = g.S;                 // the first of s .. S that ends behind t, or S
+      while (s < end) {
+        const int mid = s + (end - s) / 2;
+        if (g.sequences[mid + 1] <= t) s = mid + 1; else end = mid;
+      }
+      break;
+    }
   return s == 0 && t < g.sequences[0] ? -1 : s;
 }
 

@@ -125,6 +125,12 @@ __device__ __forceinline__ int count_of(int n, int* box, F&& holds) {
   return c;
 }
 
+// As wave_leading, for a workgroup of kThreads: up to 1,024 things take four loads of a thread at once.
+template <typename F>
+__device__ __forceinline__ int block_leading(int n, int* box, F&& holds) {
+  return leading<kThreads>(n, 4 * kThreads, [&](int m, auto&& f) { return __builtin_amdgcn_readfirstlane(count_of(m, box, f)); }, holds);
+}
+
 template <int LPT, int EPL, bool VEC>
 __global__ __launch_bounds__(kThreads) void balance_partial_kernel(const Forward p) {
   constexpr int EM = LPT * EPL, TPW = 64 / LPT;
@@ -134,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void balance_partial_kernel(const Forward
   __shared__ int box[kWaves];
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
   const int unit = blockIdx.x;
-  const int s = p.sequences ? count_of(p.S, box, [&](int i) { return begin_of(p.sequences, i, p.T) / p.chunk + i <= unit; }) - 1 : 0;
+  const int s = p.sequences ? block_leading(p.S, box, [&](int i) { return begin_of(p.sequences, i, p.T) / p.chunk + i <= unit; }) - 1 : 0;
   if (s < 0) return;
   const int b = begin_of(p.sequences, s, p.T), e = end_of(p.sequences, s, p.T);
   const int64_t from = b + (int64_t)(unit - (b / p.chunk + s)) * p.chunk;
@@ -330,7 +336,7 @@ __global__ __launch_bounds__(kThreads) void balance_bwd_kernel(const float* __re
   request(t0);
   const float per = gr.table[(int64_t)gr.S * E], slope_z = gr.table[(int64_t)gr.S * E + 1], d_loss = *gr.d_loss;
   // (the workgroup's first token's sequence: the offsets up to it, less one)
-  int s = gr.sequences ? max(count_of(gr.S + 1, box, [&](int i) { return gr.sequences[i] <= block0; }) - 1, 0) : 0;
+  int s = gr.sequences ? max(block_leading(gr.S + 1, box, [&](int i) { return gr.sequences[i] <= block0; }) - 1, 0) : 0;
   int of_h = -2;                      // whose table row h is
   float h[EPL];
   for (int i = 0; i < steps; ++i) {

@@ -182,11 +182,8 @@ __global__ __launch_bounds__(kRouteThreads) void route_topk_bwd_kernel(
   }
   float h[EPL], h_mean = 0.f, of_lse = 0.f, of_h = 0.f;
   if (BALANCED) {
-    int seq = 0;          // the token's sequence: the offsets up to t, less one
-    if (bal.sequences) {
-      for (int i = lane; i <= bal.S; i += 64) seq += bal.sequences[i] <= t;
-      seq = (int)wave_sum_f32((float)seq) - 1;
-    }
+    // the token's sequence: the offsets up to t, less one
+    const int seq = bal.sequences ? pk_balance::wave_leading(bal.S + 1, [&](int i) { return bal.sequences[i] <= t; }) - 1 : 0;
     const bool owned = seq >= 0 && seq < bal.S;
     const float d_loss = owned ? *bal.d_loss : 0.f;
     const float* const tail = bal.table + (int64_t)bal.S * E;
