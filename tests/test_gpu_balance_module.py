@@ -5,7 +5,9 @@ import pytest
 import torch
 
 from piper_amd import _lib, functional as F_, ops
+from piper_amd.bucket import BucketState, ParamStorage, StageStore, flatten_params
 from piper_amd.moe import AnnotatedMoE, MoEArgs, MoEFeedForwardBlock
+from piper_amd.optim import FusedMuon
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -126,3 +128,55 @@ def test_region_without_gradients_writes_no_pre_activations(dtype, H, I):
     assert torch.equal(*outs)
     # one of the two pre-activations alone would be more than the loss's workspace (33 chunks of 8 experts) and roundings of allocations
     assert peaks[1] <= peaks[0] + 2 * T * I * args[0].element_size() // 2
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("sequences", [False, True])
+def test_block_trains_its_gate_on_the_loss(fused, sequences):
+    """The block as it is, with the residual in its experts' last kernel or added by the unfused path."""
+    plain, with_it = pair(MoEFeedForwardBlock)
+    plain.moe.fused = with_it.moe.fused = fused
+    x, d = tokens(2, 50, 64), tokens(2, 50, 64, seed=2)
+    off = torch.tensor([0, 30, 30, 90], dtype=torch.int32, device=DEV) if sequences else None
+    more = dict(sequences=off) if sequences else {}
+    a, b = plain(x), with_it(x, **more)
+    assert rel(b, a) <= 1e-6
+    a.backward(d)
+    b.backward(d)
+    xn = F_.rmsnorm(x.reshape(-1, 64), with_it.ffn_norm.weight).detach()
+    extra = loss_gradient(with_it.moe, xn, off)
+    g0, g1 = (m.moe.router.gate.weight.grad for m in (plain, with_it))
+    assert rel(g1, g0.double() + extra) <= 1e-5 and extra.abs().max() > 1e-3 * g0.abs().max()      # (and it is not nothing)
+    for n in ("w1", "w2", "w3"):
+        assert rel(getattr(with_it.moe.experts, n).grad, getattr(plain.moe.experts, n).grad) <= 1e-5
+    assert int(with_it.moe.tokens_per_expert.sum()) == (180 if sequences else 200)
+
+
+def test_experts_in_8_bits_train_the_gate_on_the_loss():
+    plain, with_it = pair(AnnotatedMoE, torch.bfloat16, dims=(128, 64))
+    x, d = tokens(2, 40, 128, dtype=torch.bfloat16), tokens(2, 40, 128, seed=2, dtype=torch.bfloat16)
+    for m in (plain, with_it):
+        m(x, experts_fp8=m.experts.quantize()).backward(d)
+    g0, g1 = (m.router.gate.weight.grad for m in (plain, with_it))
+    extra = loss_gradient(with_it, x.reshape(-1, 128))
+    assert rel(g1 - g0, extra) <= 1e-5 * (1 + (g0.abs().max() / extra.abs().max()).item()) and rel(with_it.experts.w1.grad, plain.experts.w1.grad) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hold", [False, True])
+def test_a_step_of_the_gate_takes_the_loss(dtype, hold):
+    """Two microbatches into a bucket and FusedMuon's step over it: the gate's momentum holds what the loss adds to its gradient."""
+    momenta, extra = [], 0
+    for moe in pair(AnnotatedMoE, dtype):
+        gate = moe.router.gate.weight
+        router = flatten_params(BucketState(), [gate], optim_class=lambda q: FusedMuon(q, matrices=lambda p: p is not gate, adamw=dict(betas=(0.5, 0.9))))  # noqa: B023
+        storage = ParamStorage(StageStore(buckets={0: router}, zero_managed_ubids={0}))
+        for mb in range(2):
+            x, d = (tokens(2, 32, 64, seed=10 * mb + k, dtype=dtype) for k in (1, 2))
+            if moe.balanced:
+                extra = extra + loss_gradient(moe, x.reshape(-1, 64))
+            moe(x).backward(d * 1e-2)
+            (storage.hold_param_grads if hold and mb else storage.accumulate_zero_param_grads_to_flat)(0)
+        storage.step_zero_shard_optimizers()
+        momenta.append(router.shard_optimizer.state[router.shard_param]["momentum"][:gate.numel()].view(gate.shape).clone())
+    assert rel(momenta[1], momenta[0].double() + 0.5 * extra) <= 1e-5 and extra.abs().max() > 1e-2 * momenta[0].abs().max()
