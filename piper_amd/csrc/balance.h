@@ -15,13 +15,24 @@ namespace pk_balance {
 // of a call: the first launch has a workgroup for each and more
 constexpr int64_t kMostSequences = 0xfffff;
 
-// What a backward needs beside the logits.  table: [S][E] of h - mean(h) without the 1 / S', then 1 / S' and 2 z_coeff / N.
+// What a backward needs beside the logits.  table: [S][E] of h - mean(h) without the 1 / S', then S' and 2 z_coeff / N.
 struct Grad {
   const float* table;
   const int32_t* sequences;   // [S + 1], or nullptr: one sequence of all T tokens
   const float* d_loss;
   int32_t S;
 };
+
+// d_loss / S', a factor of every element: its rounding would make all of them too large or too small together, so it comes in two parts.
+struct Factor {
+  float hi, lo;
+  __device__ __forceinline__ float times(float v) const { return fmaf(hi, v, lo * v); }
+};
+__device__ __forceinline__ Factor factor_of(float d_loss, float some) {
+  const double f = (double)d_loss / some;
+  const float hi = (float)f;
+  return {hi, __builtin_isfinite(hi) ? (float)(f - hi) : 0.f};
+}
 
 // Bounds of sequence s.  Offsets ascend within 0 .. T; whatever else they hold, the range stays inside.
 __device__ __forceinline__ int begin_of(const int32_t* sequences, int s, int T) { return sequences ? min(max(sequences[s], 0), T) : 0; }

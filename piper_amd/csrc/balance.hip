@@ -297,7 +297,7 @@ __global__ __launch_bounds__(kSumThreads) void balance_sum_kernel(const Forward 
   const auto finish = [&]() {
     const double per = all[3] > 0 ? 1.0 / all[3] : 0.0, each = all[2] > 0 ? (double)p.z_coeff / all[2] : 0.0;
     *p.loss = (float)((double)p.balance_coeff * all[0] * per + each * all[1]);
-    p.table[(int64_t)p.S * p.E] = (float)per;
+    p.table[(int64_t)p.S * p.E] = (float)all[3];        // (below 2^20: as it is)
     p.table[(int64_t)p.S * p.E + 1] = (float)(2.0 * each);
   };
   if (gridDim.x == 1) {
@@ -334,10 +334,11 @@ __global__ __launch_bounds__(kThreads) void balance_bwd_kernel(const float* __re
   float next[EPL];
   const auto request = [&](int t) { load_row<LPT, EPL, VEC>(logits + (int64_t)min(t, T - 1) * E, E, g, -INFINITY, next); };
   request(t0);
-  const float per = gr.table[(int64_t)gr.S * E], slope_z = gr.table[(int64_t)gr.S * E + 1], d_loss = *gr.d_loss;
+  const float slope_z = gr.table[(int64_t)gr.S * E + 1], d_loss = *gr.d_loss;
+  const Factor of_h = factor_of(d_loss, gr.table[(int64_t)gr.S * E]);
   // (the workgroup's first token's sequence: the offsets up to it, less one)
   int s = gr.sequences ? max(block_leading(gr.S + 1, box, [&](int i) { return gr.sequences[i] <= block0; }) - 1, 0) : 0;
-  int of_h = -2;                      // whose table row h is
+  int row_of = -2;                    // whose table row h is
   float h[EPL];
   for (int i = 0; i < steps; ++i) {
     const int t = t0 + i * TPW;
@@ -348,22 +349,22 @@ __global__ __launch_bounds__(kThreads) void balance_bwd_kernel(const float* __re
     if (i + 1 < steps) request(t + TPW);
     s = sequence_of(gr, max(s, 0), t);
     const bool owned = s >= 0 && s < gr.S;
-    if (s != of_h) {
+    if (s != row_of) {
       load_row<LPT, EPL, VEC>(gr.table + (int64_t)(owned ? s : 0) * E, E, g, 0.f, h);
-      of_h = s;
+      row_of = s;
     }
     const float lse = softmax<LPT, EPL>(x);
     float mean = 0.f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) mean += h[j] * x[j];
     mean = group_sum<LPT>(mean);
-    const float at_h = owned ? d_loss * per : 0.f, at_lse = owned ? d_loss * slope_z * lse : 0.f;
+    const float of_lse = d_loss * slope_z * lse;
     float* const to = d_logits + (int64_t)t * E;
 #pragma unroll
     for (int j = 0; j < EPL; j += 4) {
       floatx4_t d;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) d[k] = owned ? x[j + k] * (at_h * (h[j + k] - mean) + at_lse) : 0.f;
+      for (int k = 0; k < 4; ++k) d[k] = owned ? x[j + k] * (of_h.times(h[j + k] - mean) + of_lse) : 0.f;
       const int e = expert_of<LPT>(j, g);
       if (VEC) {
         if (e < E) *reinterpret_cast<floatx4_t*>(to + e) = d;

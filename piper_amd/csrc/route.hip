@@ -180,14 +180,15 @@ __global__ __launch_bounds__(kRouteThreads) void route_topk_bwd_kernel(
     for (int j = 0; j < EPL; ++j)
       if (lane + 64 * j == ek) dp[j] = dsk;
   }
-  float h[EPL], h_mean = 0.f, of_lse = 0.f, of_h = 0.f;
+  float h[EPL], h_mean = 0.f, of_lse = 0.f;
+  pk_balance::Factor of_h = {0.f, 0.f};
   if (BALANCED) {
     // the token's sequence: the offsets up to t, less one
     const int seq = bal.sequences ? pk_balance::wave_leading(bal.S + 1, [&](int i) { return bal.sequences[i] <= t; }) - 1 : 0;
     const bool owned = seq >= 0 && seq < bal.S;
     const float d_loss = owned ? *bal.d_loss : 0.f;
     const float* const tail = bal.table + (int64_t)bal.S * E;
-    of_h = d_loss * tail[0];
+    if (owned) of_h = pk_balance::factor_of(d_loss, tail[0]);
     of_lse = d_loss * tail[1] * (mx + logf(denom));
     float part_h = 0.f;
 #pragma unroll
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_topk_bwd_kernel(
     const int e = lane + 64 * j;
     if (e < E) {
       float d = p[j] * (dp[j] - D);
-      if (BALANCED) d += p[j] * (of_h * (h[j] - h_mean) + of_lse);
+      if (BALANCED) d += p[j] * (of_h.times(h[j] - h_mean) + of_lse);
       const int64_t at = (int64_t)t * E + e;
       d_logits[at] = d;
       if (io.planes) {
