@@ -188,7 +188,7 @@ PK_API int pk_sort_by_expert_static(const int32_t* top_idx, int64_t A, int64_t E
  *   loss[1] (f32) = balance_coeff * mean over the sequences with tokens of sum_e f_e P_e
  *                 + z_coeff * mean over the sequences' tokens of logsumexp(logits)^2
  *   table[S*E+2] (f32): what the backward needs beside the logits
- * Sums are fp32 over up to 64 (more than 32,768 tokens: T / 512) tokens, 64-bit above, in a fixed order. */
+ * Sums are fp32 over up to 64 ceil(T / 32768) tokens, 64-bit above, in a fixed order. */
 PK_API int64_t pk_balance_workspace_bytes(int64_t T, int64_t E, int64_t S);
 PK_API int pk_balance_loss(const float* logits, const int32_t* top_idx, const int32_t* sequences, int64_t T, int64_t E,
                     int64_t K, int64_t S, float balance_coeff, float z_coeff, float* loss, int32_t* counts, float* table,

@@ -140,7 +140,7 @@ SIGNATURES = {
     "pk_timing_select": (_c_int, [_c_int]),
     "pk_timing_kernel_name": (C.c_char_p, [_c_int]),
 }
-# table sequences S d_loss, then as pk_region_router_norm_bwd
+# table sequences S d_loss, then as the ones without a balance loss
 SIGNATURES["pk_route_topk_balanced_bwd"] = (_c_int, [_p, _p, _c_i64, _p, *SIGNATURES["pk_route_topk_bwd"][1]])
 SIGNATURES["pk_region_router_balanced_bwd"] = (_c_int, [_p, _p, _c_i64, _p, *SIGNATURES["pk_region_router_bwd"][1]])
 SIGNATURES.update({f"{name}_short": SIGNATURES[name] for name in

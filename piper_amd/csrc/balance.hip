@@ -5,7 +5,7 @@
 // workgroup sums the softmax of up to `chunk` tokens of one sequence, a second launch adds the chunks of every sequence up in a fixed
 // order and 64 bits, and its last workgroup the sequences.  No chunk belongs to two sequences: that of a sequence which starts at
 // token b has the units b / chunk + s and on, which cannot meet (as padded_start in the weight gradients), so that the host needs
-// no look at the lengths.  Backward: one pass, the softmax formed again.  131,072 tokens of 128 experts in 512 sequences: 21 + 9 + 24 us (the
+// no look at the lengths.  Backward: one pass, the softmax formed again.  131,072 tokens of 128 experts in 512 sequences: 21 + 9 + 23 us (the
 // logits once in 67 MB, twice in the backward), 256 of 8 experts 4.6 + 4.8 + 3.0.
 #include "balance.h"
 #include <algorithm>

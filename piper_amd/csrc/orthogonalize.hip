@@ -43,7 +43,7 @@ constexpr int kMaxEntries = 40, kMaxEnds = 8, kMaxShapes = 100;
 constexpr int kChunk = 8192;                 // elements a workgroup of begin_kernel takes
 constexpr int kThreads = 256;
 // Workspace that is asked for.  Groups that stay in the 256 MiB memory-side cache leave too few workgroups a launch, whose last round is
-// rarely full: 128 matrices of 768 x 2048, bf16 / fp32 results, ms with 192 MiB 8.1 / 12.8, 384 6.2 / 11.4, 768 5.4 / 11.0, 1,536 5.0 / 9.9, 2,560 4.5 / 9.6.
+// rarely full: 128 matrices of 768 x 2048, single / three products, ms with 192 MiB 8.1 / 12.8, 384 6.2 / 11.4, 768 5.4 / 11.0, 1,536 5.0 / 9.9, 2,560 4.5 / 9.6.
 constexpr int64_t kGroupBytes = 2560ll << 20;
 
 // Matrices of one shape that lie one behind the other, as the kernels at both ends see them.
@@ -117,7 +117,7 @@ __device__ __forceinline__ int entry_of(int n, int block, F&& first) {
 }
 
 // ---------------------------------------------------------------- the ends
-// Memory bounds them: 128 matrices of 768 x 2048 in bf16 94 + 226 + 141 us (4.3, 5.3, 5.7 TB/s), a step of 170 million bf16 values 335 + 361 + 487.
+// Memory bounds them: 128 matrices of 768 x 2048 in bf16 90 + 256 + 232 us (4.5, 4.7, 5.2 TB/s), a step of 170 million bf16 values 336 + 359 + 487.
 // N neighbouring values at p as fp32; VEC: p is on a boundary of their size.
 template <int N, bool VEC, typename T>
 __device__ __forceinline__ void load_n(const T* p, float (&x)[N]) {
@@ -414,9 +414,9 @@ __host__ __device__ inline int units_of_symmetric(int mp) {
 // and they swap (the k-loop of the grouped products).  k-tiles go straight to LDS, NS - 1 of them ahead.  A k-tile has KT values of k; W
 // fp16 values of a row (both planes with PRECISE).
 //
-// us a launch, 128 matrices of 768 x 2048, single products: X X^T 219, A A 127, B X 475 (of which its products are 295 and its 1.6 GB 310: the
-// stores of a unit's end are not under the next one's products); one of 2048 x 4096, three products: 82, 54, 103 (1.0 PFLOP/s, what the
-// card's power allows).
+// us a launch, 128 matrices of 768 x 2048, three products: X X^T 564, A A 282, B X 918 (1.05 PFLOP/s of the products that it needs), single ones:
+// 216, 126, 473 (of which its products are 295 and its 1.6 GB 310: the stores of a unit's end are not under the next one's products);
+// one of 2048 x 4096, three products: 81, 54, 102 (1.0 PFLOP/s).
 //
 // SHARED (GRAM and POLY with few units, 128 x 128): the pairs of k-tiles of all units, one unit's behind the other's, are cut into
 // p.shares equal shares, one to a workgroup.  A wave leaves its sums of a part of a unit as they are in Xn, which nobody needs then, and
@@ -796,7 +796,7 @@ bool sides_ok(int64_t rows, int64_t cols) { return rows <= PK_MAX_MATRIX_SIDE &&
 
 // The tiles: wide ones, 256 x 256 (single products) or 128 x 256, or 128 x 128, by the rounds that their units take on the CUs; a round of wide
 // ones takes 2.5 to 3 (1.5 to 1.75 with three products) of the others.  us of the five steps, wide / narrow, X X^T and A A together, the
-// update, and in brackets their wide units: 24 x 256 x 512, fp32, 225 / 174, 97 / 80 (48, 96); 24 x 363 x 1000, bf16, 244 / 147, 127 / 154 (72, 192),
+// update, and in brackets their wide units; fp32: three products, bf16: single ones: 24 x 256 x 512, fp32, 225 / 174, 97 / 80 (48, 96); 24 x 363 x 1000, bf16, 244 / 147, 127 / 154 (72, 192),
 // fp32 351 / 260, 223 / 220 (96, 288); 2048 x 4096, fp32, 1,020 / 644, 483 / 636 (72, 256), bf16 695 / 389, 285 / 270 (36, 128); 16 x 768 x 2048, fp32,
 // 726 / 797, 657 / 753 (192, 768); 64 x 512 x 512, fp32, 612 / 599, 318 / 368 (384, 512); 128 x 768 x 2048, bf16, 1,713 / 1,923, 2,342 / 3,256
 // (3 and 12 rounds), fp32 4,261 / 4,456, 4,541 / 5,661 (6 and 24).  (Half of a wide tile on the diagonal is of no use.)

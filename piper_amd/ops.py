@@ -544,7 +544,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     matrices whose sides are both longer than 128), a third of the matrix operations, for results about 0.002 off; 0.01 for
     matrices of few values (few rows that are not zero, a scaled identity), below 0.04 for any one direction.  A matrix with a value that
     is not finite becomes NaN, no other one does.  Coefficients and steps that may take a singular value past 15 are refused; those that
-    bring them near 1 stay below 2.  No backward."""
+    bring them near 1 stay below 2.  A call takes up to 2.5 GiB of workspace.  No backward."""
     return host().orthogonalize(x, int(steps), _three(coefficients), float(eps), bool(half_products))
 
 
