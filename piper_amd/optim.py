@@ -278,7 +278,7 @@ class FusedMuon(_FlatStateOptimizer):
         places = [(o, n) for o, n, *_ in self._places(p)]
         if p not in self._views or [tuple(x) for x in zip(offsets, numels)] != places:
             raise RuntimeError("FusedMuon.step_packed: gradients of the views that bind_views has been told of, in their order")
-        self._update(p, group, flat_grad, grads, self.zero_grad_in_step and flat_grad is not None)
+        self._update(p, group, flat_grad, list(grads), self.zero_grad_in_step and flat_grad is not None)
 
     def _update(self, p: torch.Tensor, group: dict, flat, grads, clear: bool) -> None:
         """grads: of each of _places, None: nothing beside `flat`"""
@@ -307,8 +307,10 @@ class FusedMuon(_FlatStateOptimizer):
                            half_products=self.half_products)
 
     def _check_grads(self, p: torch.Tensor, flat, grads) -> None:
-        """Before anything is changed: a step refused for its gradients leaves weights and state as they were."""
+        """Before anything is changed: a step refused for its tensors leaves weights and state as they were."""
         places = self._places(p)
+        if p.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"FusedMuon: parameters are float32 or bfloat16, not {p.dtype}")
         if len(grads) != len(places):
             raise ValueError(f"FusedMuon: {len(grads)} gradients of {len(places)} parameters")
         types = set()

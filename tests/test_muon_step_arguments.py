@@ -66,6 +66,22 @@ def test_gradients_reach_their_own_parameters(calls, order):
         SHAPES = shapes
 
 
+def test_parameters_of_other_types_are_refused_before_anything_changes(calls):
+    for shape in ((4, 6), (5,)):
+        p = torch.nn.Parameter(torch.randn(shape).half())
+        p.grad = torch.randn(shape).half()
+        opt = FusedMuon([p])
+        with pytest.raises(ValueError, match="float32 or bfloat16"):
+            opt.step()
+        assert not calls and not opt.state.get(p)
+
+
+def test_gradients_of_any_iterable(calls):
+    p, opt, offsets, numels = bucket()
+    opt.step_packed(p, (torch.zeros(s) for s in SHAPES), iter(offsets), iter(numels))
+    assert len(calls) == sum(n > 0 for n in numels)
+
+
 def broken(grads, flat):
     yield [None] * 7, flat
     for i, g in ((1, torch.zeros(199)), (1, torch.zeros(10, 20, dtype=torch.float64)), (1, grads[1].to("meta")), (5, torch.zeros(6)), (1, grads[1].bfloat16())):
